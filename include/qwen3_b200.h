@@ -337,6 +337,125 @@ int q3_engine_fill_kv_normal(q3_engine *e, int n_positions, unsigned long long s
 
 int q3_engine_info(const q3_engine *e, q3_engine_buffers *out);
 
+/* ---------------------------------------------------------------------------------------
+ * Paged serving: ragged batches of new tokens over a paged KV cache. No counterpart in the
+ * reference, whose cache is one slab for one sequence.
+ *
+ * One step of a server holds `n_seqs` sequences. Sequence s brings q_len = q_start[s+1] -
+ * q_start[s] new tokens (a decode step's one, a few drafts, or a chunk of a prompt), rows
+ * q_start[s] .. of the step's q/k/v, and has kv_len[s] positions once they are in; its token i
+ * is at position kv_len[s] - q_len + i. Position t of sequence s lives in slot t % page_size of
+ * page page_table[s * max_pages + t / page_size]. Pages may be shared between sequences.
+ *
+ * q3_paged_plan turns this description into a work list on the device once per step; the step's
+ * layers then all use the same plan. A plan is plain device memory: launchers read nothing on
+ * the host, so plan and layers can be captured in one CUDA graph whose q_start, kv_len and
+ * page_table change from replay to replay.
+ *
+ * Padding and bad descriptions:
+ *   - tokens at negative positions (q_len > kv_len) are padding: nothing is stored for them and
+ *     their q_out and attention rows are zero;
+ *   - rows of the batch outside [q_start[0], q_start[n_seqs]) are neither read nor written;
+ *   - q_start not rising within [0, n_tokens], q_len above max_q_len, kv_len outside
+ *     [0, max_pages * page_size] or a used page outside [0, n_pages) sets device error bit 2;
+ *     the sequence (every sequence, if q_start does not rise) is then treated as having no
+ *     positions, so all its rows are padding.
+ * ------------------------------------------------------------------------------------- */
+
+typedef struct q3_paged_shape {
+    int n_seqs;      /* at most 4096 */
+    int n_tokens;    /* rows of q, k, v and the outputs */
+    int max_q_len;   /* most new tokens any sequence brings */
+    int n_heads, n_kv_heads, head_dim;
+    int page_size;   /* positions per page, a multiple of 8 */
+    int n_pages;     /* pages in the cache */
+    int max_pages;   /* row length of page_table */
+} q3_paged_shape;
+
+/* One layer's pages: slot t of kv head h of page p starts at
+ * base + p * page_stride + h * head_stride + t * pos_stride (elements, multiples of 8). */
+typedef struct q3_paged_cache {
+    q3_bf16 *key_pages, *value_pages;
+    long long page_stride, head_stride, pos_stride;
+} q3_paged_cache;
+
+/* Bytes of a plan, and of the scratch q3_paged_attention needs, for a shape (0 if the shape is
+ * not supported: head_dim not a multiple of 8 up to 128, n_heads not a multiple of n_kv_heads or
+ * more than 128 query heads per kv head). Neither needs initialization. Calls that share a plan's
+ * scratch must not overlap on the GPU. */
+size_t q3_paged_plan_bytes(const q3_paged_shape *shape);
+size_t q3_paged_attention_scratch_bytes(const q3_paged_shape *shape);
+
+/* Writes the plan for one step. */
+int q3_paged_plan(void *plan, const q3_paged_shape *shape, const int *q_start, const int *kv_len,
+                  const int *page_table, void *stream);
+
+/* Per new token: q and k heads are RMS-normed (y = x * rsqrt(mean(x^2) + eps) * w; skipped where
+ * q_norm_w / k_norm_w is null), the first rope_dim elements of each head are rotated by
+ * position * inv_freq[j] with cos and sin multiplied by `amplitude`, q goes to q_out, and k and v
+ * to their slots in the cache. Pairs are (j, j + rope_dim/2), or (2j, 2j+1) with `interleaved`.
+ * All in fp32, the angle's reduction in fp64, rounded to bf16 once. Strides are elements between
+ * tokens; q_out may be q (same stride). inv_freq is device memory, rope_dim/2 floats
+ * (q3_rope_inv_freq); rope_dim 0 rotates nothing. */
+int q3_paged_rope_append(q3_bf16 *q_out, long long q_out_stride, const q3_bf16 *q, long long q_stride,
+                         const q3_bf16 *k, long long k_stride, const q3_bf16 *v, long long v_stride,
+                         const q3_bf16 *q_norm_w, const q3_bf16 *k_norm_w, float eps, const float *inv_freq,
+                         int rope_dim, int interleaved, float amplitude, const q3_paged_cache *cache,
+                         const q3_paged_shape *shape, const void *plan, void *stream);
+
+/* out = softmax(scale * q . k) . v per new token and query head over positions 0 .. its own;
+ * query head h reads kv head h / (n_heads / n_kv_heads). Strides are elements between tokens.
+ * Scores, softmax statistics and sums in fp32; the unnormalized probabilities enter the second
+ * product as bf16. NaN or infinite values in the cache reach only the rows that attend to their
+ * position. */
+int q3_paged_attention(q3_bf16 *out, long long out_stride, const q3_bf16 *q, long long q_stride,
+                       const q3_paged_cache *cache, float scale, const q3_paged_shape *shape, const void *plan,
+                       void *scratch, void *stream);
+
+/* How the rotation frequencies theta^(-2j/rope_dim) are changed for contexts longer than the
+ * trained one. */
+enum q3_rope_kind {
+    Q3_ROPE_PLAIN = 0,
+    Q3_ROPE_LINEAR = 1,   /* all divided by factor (position interpolation) */
+    Q3_ROPE_BY_PARTS = 2, /* wavelengths above original_max / low_freq_factor divided by factor, below
+                             original_max / high_freq_factor kept, linear in original_max / wavelength
+                             between */
+    Q3_ROPE_YARN = 3      /* YaRN: a linear ramp over j between the pairs that turn beta_fast and beta_slow
+                             times within original_max; cos and sin scaled by `attention_factor`, or by
+                             0.1 ln(factor) + 1 where that is 0 */
+};
+typedef struct q3_rope_scaling {
+    int kind;
+    float factor;                           /* >= 1 */
+    float low_freq_factor, high_freq_factor; /* by parts: low < high */
+    float beta_fast, beta_slow;             /* YaRN: fast > slow */
+    float attention_factor;
+    int original_max;                       /* trained positions (by parts, YaRN) */
+} q3_rope_scaling;
+
+/* Fills the HOST array inv_freq[rope_dim / 2] and *amplitude for q3_paged_rope_append; scaling null
+ * is plain. Runs on the CPU, once per model. */
+int q3_rope_inv_freq(float *inv_freq, float *amplitude, int rope_dim, float theta, const q3_rope_scaling *scaling);
+
+/* Logits of `rows` sequences before sampling, in this order, in fp32, rounded once to the
+ * logits' type (0: bf16, 1: fp32). Row r's history is hist_ids[hist_start[r] .. hist_start[r+1]):
+ * prompt tokens up to hist_split[r], generated ones from it.
+ *   1. tokens in the history: x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   2. generated tokens, n times: x -= frequency[r] * n + presence[r]
+ *   3. x += bias[i] for token bias_ids[i], i in bias_start[r] .. bias_start[r+1]; the last entry
+ *      of a repeated id counts
+ *   4. mask bit (mask[r * mask_stride + t / 32] >> t % 32) clear: x = -inf, whatever x was
+ * Null hist_start (or any of the three factors), bias_start or mask leaves that part out. Ids outside
+ * [0, vocab) are ignored (negative ids can pad). hist_start and bias_start must not fall; a row for
+ * which one does, or whose split is outside its history, sets device error bit 2 and is treated
+ * as having none. Strides are elements between rows (mask_stride: words); out may be logits (same
+ * stride). */
+int q3_logits_process(void *out, const void *logits, int dtype, int rows, int vocab, long long out_stride,
+                      long long stride, const int *hist_start, const int *hist_split, const int *hist_ids,
+                      const float *repetition, const float *frequency, const float *presence, const int *bias_start,
+                      const int *bias_ids, const float *bias, const unsigned *mask, long long mask_stride,
+                      void *stream);
+
 #ifdef __cplusplus
 }
 #endif

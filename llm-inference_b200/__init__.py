@@ -12,11 +12,14 @@ token buffers torch.int32, and ``stream`` defaults to torch's current stream. Er
 from __future__ import annotations
 
 from ._lib import Q3Error, call, load  # noqa: F401
+from .paged import (PagedPlan, logits_process, paged_attention, paged_rope_append,  # noqa: F401
+                    rope_inv_freq)
 
 __all__ = [
     "Q3Error", "load", "embedding_forward", "rmsnorm_forward", "gemv_forward",
     "gemv_residual_forward", "qkv_forward", "gate_up_forward", "qk_norm_rope_forward",
     "attention_forward", "argmax_forward", "sample_forward", "device_error",
+    "PagedPlan", "paged_rope_append", "paged_attention", "rope_inv_freq", "logits_process",
 ]
 
 

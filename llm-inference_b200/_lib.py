@@ -66,8 +66,16 @@ SIGNATURES: dict[str, list] = {
     "q3_engine_prefill": [_P, _I, _P, _I, _I],
     "q3_engine_fill_kv_normal": [_P, _I, ctypes.c_ulonglong],
     "q3_engine_info": [_P, _P],
+    "q3_paged_plan_bytes": [_P],
+    "q3_paged_attention_scratch_bytes": [_P],
+    "q3_paged_plan": [_P, _P, _P, _P, _P, _P],
+    "q3_paged_rope_append": [_P, _LL, _P, _LL, _P, _LL, _P, _LL, _P, _P, _F, _P, _I, _I, _F, _P, _P, _P, _P],
+    "q3_paged_attention": [_P, _LL, _P, _LL, _P, _F, _P, _P, _P, _P],
+    "q3_rope_inv_freq": [_P, _P, _I, _F, _P],
+    "q3_logits_process": [_P, _P, _I, _I, _I, _LL, _LL, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _LL, _P],
 }
 RESTYPES = {"q3_status_string": ctypes.c_char_p, "q3_attention_scratch_bytes": ctypes.c_size_t,
+            "q3_paged_plan_bytes": ctypes.c_size_t, "q3_paged_attention_scratch_bytes": ctypes.c_size_t,
             "q3_weight_bytes_per_step": ctypes.c_size_t, "q3_kv_bytes_per_position": ctypes.c_size_t}
 
 _lib = None

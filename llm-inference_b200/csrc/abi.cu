@@ -35,6 +35,8 @@ unsigned take_error_tc();
 unsigned take_error_stream();
 unsigned take_error_attn_fused();
 unsigned take_error_selftest();
+unsigned take_error_paged();
+unsigned take_error_logits();
 
 namespace {
 constexpr int MAX_DEVICES = 64;
@@ -139,7 +141,8 @@ int q3_device_error(void *stream, unsigned *flags) {
     cudaError_t e = cudaStreamSynchronize(S(stream));
     if (e != cudaSuccess) return q3::record_cuda_error(e);
     *flags = q3::take_error_gemv() | q3::take_error_decode() | q3::take_error_attention() | q3::take_error_tc() |
-             q3::take_error_stream() | q3::take_error_attn_fused() | q3::take_error_selftest();
+             q3::take_error_stream() | q3::take_error_attn_fused() | q3::take_error_selftest() | q3::take_error_paged() |
+             q3::take_error_logits();
     return Q3_OK;
 }
 

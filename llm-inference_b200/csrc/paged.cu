@@ -1,0 +1,526 @@
+// Paged serving: the step plan, the append of new tokens with rotary positions, and attention over
+// the pages (include/qwen3_b200.h, "Paged serving").
+#include <math.h>
+
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace q3 {
+int check_device();
+
+namespace {
+
+__device__ unsigned g_dev_error;
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// ------------------------------------------------------------------ plan
+// One CTA. The description is checked here once, so that the kernels of every layer can use the
+// plan's copy of the page table and the token map without checks of their own.
+constexpr int PLAN_THREADS = 1024;
+
+struct PlanArgs {
+    char *plan;
+    PagedPlanLayout l;
+    q3_paged_shape s;
+    const int *q_start, *kv_len, *page_table;
+};
+
+__global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_constant__ PlanArgs a) {
+    __shared__ int start_s[PAGED_MAX_SEQS + 1];
+    pdl_trigger();
+    pdl_wait();
+    const int n = a.s.n_seqs, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    PagedSeq *seqs = reinterpret_cast<PagedSeq *>(a.plan + a.l.seqs);
+    int *table = reinterpret_cast<int *>(a.plan + a.l.table);
+    int4 *toks = reinterpret_cast<int4 *>(a.plan + a.l.toks);
+
+    for (int i = tid; i <= n; i += PLAN_THREADS) start_s[i] = a.q_start[i];
+    __syncthreads();
+    bool falls = false;
+    for (int i = tid; i <= n; i += PLAN_THREADS)
+        falls |= start_s[i] < 0 || start_s[i] > a.s.n_tokens || (i > 0 && start_s[i] < start_s[i - 1]);
+    const bool bad_starts = __syncthreads_or(falls);
+
+    for (int b = warp; b < n; b += PLAN_THREADS / 32) {  // a warp checks a sequence's pages
+        const int q0 = start_s[b], q_len = start_s[b + 1] - q0, kv = a.kv_len[b];
+        const int used = (int)min(((long long)kv + a.s.page_size - 1) / a.s.page_size, (long long)a.s.max_pages);
+        bool bad = bad_starts || q_len > a.s.max_q_len || kv < 0 || kv > (long long)a.s.max_pages * a.s.page_size;
+        for (int i = lane; i < a.s.max_pages; i += 32) {
+            int page = -1;
+            if (i < used && !bad) {
+                page = a.page_table[(size_t)b * a.s.max_pages + i];
+                if (page < 0 || page >= a.s.n_pages) {
+                    bad = true;
+                    page = -1;
+                }
+            }
+            table[(size_t)b * a.s.max_pages + i] = page;
+        }
+        bad = __any_sync(0xffffffffu, bad);
+        if (lane == 0) {
+            if (bad) atomicOr(&g_dev_error, DEV_ERR_POS_RANGE);
+            seqs[b] = {bad_starts ? 0 : q0, bad_starts ? 0 : q_len, bad ? 0 : kv, 0};
+        }
+    }
+    __syncthreads();
+    for (int t = tid; t < a.s.n_tokens; t += PLAN_THREADS) {
+        int4 tok = make_int4(-1, bad_starts ? -1 : PAGED_OUTSIDE, -1, -1);
+        if (!bad_starts && n > 0 && t >= start_s[0] && t < start_s[n]) {
+            int lo = 0, hi = n - 1;  // the last sequence that starts at or before t and is not empty there
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (start_s[mid] <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            const PagedSeq q = seqs[lo];
+            const int pos = q.kv_len - q.q_len + (t - q.q0);
+            tok.x = lo;
+            tok.y = pos < 0 ? -1 : pos;
+            if (pos >= 0) {
+                tok.z = table[(size_t)lo * a.s.max_pages + pos / a.s.page_size];
+                tok.w = pos % a.s.page_size;
+            }
+        }
+        toks[t] = tok;
+    }
+}
+
+// ------------------------------------------------------------------ append
+// One CTA per token. A unit is two 8-element chunks of a head that one lane holds in registers: for
+// half-split pairs chunk u and its partner u + rope_dim/16, so a pair's two elements sit in one lane;
+// otherwise neighbours. A head is a group of `lph` lanes (a power of two), so the sum of squares
+// is a few shuffles. The angles depend on the token alone: the CTA computes them once, then every
+// head reads them from shared memory.
+//
+// The angle is reduced in fp64: pos * inv_freq reaches 10^5 rad and more, where an fp32 product is
+// off by up to 2^-25 of itself, more than a bf16 result may be. turns = pos * inv_freq / 2 pi, its
+// nearest integer dropped, goes to sincospif.
+constexpr int APPEND_THREADS = 128;
+
+struct AppendArgs {
+    bf16 *q_out;
+    const bf16 *q, *k, *v;
+    const bf16 *q_norm_w, *k_norm_w;
+    const float *inv_freq;
+    bf16 *key_pages, *value_pages;
+    long long q_out_stride, q_stride, k_stride, v_stride, page_stride, head_stride, pos_stride;
+    const int4 *toks;
+    int n_heads, n_kv_heads, head_dim, rope_dim, lph;
+    float eps, amplitude;
+};
+
+__device__ __forceinline__ void unpack8(const uint4 &u, float *f) {
+    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 p = __bfloat1622float2(h[i]);
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+    }
+}
+
+__device__ __forceinline__ uint4 pack8(const float *f) {
+    uint4 u;
+    __nv_bfloat162 *h = reinterpret_cast<__nv_bfloat162 *>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    return u;
+}
+
+__device__ __forceinline__ void rope_angle(int pos, float inv_freq, float amplitude, float *c, float *s) {
+    const double turns = (double)pos * (double)inv_freq * 0.15915494309189533577;  // 1 / 2 pi
+    float cs, sn;
+    sincospif((float)(2.0 * (turns - rint(turns))), &sn, &cs);
+    *c = cs * amplitude;
+    *s = sn * amplitude;
+}
+
+template <bool INTERLEAVED>
+__global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+    __shared__ float cos_s[PAGED_MAX_HEAD_DIM / 2], sin_s[PAGED_MAX_HEAD_DIM / 2];
+    pdl_trigger();
+    pdl_wait();
+    const int t = blockIdx.x;
+    const int4 tok = a.toks[t];
+    const int pos = tok.y;
+    if (pos == PAGED_OUTSIDE) return;
+    const int half = a.rope_dim / 2;
+    for (int j = threadIdx.x; j < half; j += APPEND_THREADS)
+        if (pos >= 0) rope_angle(pos, a.inv_freq[j], a.amplitude, &cos_s[j], &sin_s[j]);
+    __syncthreads();
+    const int u = threadIdx.x % a.lph, nc = a.head_dim / 8, hc = INTERLEAVED ? 0 : half / 8;
+    const int c0 = INTERLEAVED ? 2 * u : u < hc ? u : 2 * u;  // units past the rotated pairs: chunks 2u, 2u + 1
+    const int c1 = !INTERLEAVED && u < hc ? u + hc : c0 + 1;
+    const bool in0 = c0 < nc, in1 = c1 < nc;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int h = threadIdx.x / a.lph; h < a.n_heads + 2 * a.n_kv_heads; h += APPEND_THREADS / a.lph) {
+        const int kh = h - a.n_heads, vh = kh - a.n_kv_heads;
+        const bf16 *src;
+        bf16 *dst;
+        const bf16 *w = nullptr;
+        if (kh < 0) {
+            src = a.q + t * a.q_stride + (long long)h * a.head_dim;
+            dst = a.q_out + t * a.q_out_stride + (long long)h * a.head_dim;
+            w = a.q_norm_w;
+        } else {
+            const long long slot = tok.z * a.page_stride + tok.w * a.pos_stride;
+            src = vh < 0 ? a.k + t * a.k_stride + (long long)kh * a.head_dim
+                         : a.v + t * a.v_stride + (long long)vh * a.head_dim;
+            dst = vh < 0 ? a.key_pages + slot + kh * a.head_stride : a.value_pages + slot + vh * a.head_stride;
+            w = a.k_norm_w;
+        }
+        if (pos < 0) {  // padding: zero query rows, nothing stored
+            if (kh < 0 && in0) reinterpret_cast<uint4 *>(dst)[c0] = zero;
+            if (kh < 0 && in1) reinterpret_cast<uint4 *>(dst)[c1] = zero;
+            continue;
+        }
+        const uint4 r0 = in0 ? reinterpret_cast<const uint4 *>(src)[c0] : zero;
+        const uint4 r1 = in1 ? reinterpret_cast<const uint4 *>(src)[c1] : zero;
+        uint4 o0 = r0, o1 = r1;
+        if (vh < 0) {
+            float x[16];
+            unpack8(r0, x);
+            unpack8(r1, x + 8);
+            if (w != nullptr) {  // uniform over q heads and over k heads, whose groups of lanes may share a warp
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; i++) sum = __fmaf_rn(x[i], x[i], sum);
+                const unsigned group = (a.lph == 32 ? 0xffffffffu : (1u << a.lph) - 1) << (threadIdx.x % 32 / a.lph * a.lph);
+                for (int off = a.lph / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(group, sum, off);
+                const float inv = rsqrtf(sum / a.head_dim + a.eps);
+                float g[16];
+                unpack8(in0 ? reinterpret_cast<const uint4 *>(w)[c0] : zero, g);
+                unpack8(in1 ? reinterpret_cast<const uint4 *>(w)[c1] : zero, g + 8);
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[i] = x[i] * inv * g[i];
+            }
+            if constexpr (INTERLEAVED) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int j = 8 * u + i;  // pair (2j, 2j + 1)
+                    if (j < half) {
+                        const float e = x[2 * i], o = x[2 * i + 1], c = cos_s[j], s = sin_s[j];
+                        x[2 * i] = e * c - o * s;
+                        x[2 * i + 1] = o * c + e * s;
+                    }
+                }
+            } else if (u < hc) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float e = x[i], o = x[8 + i], c = cos_s[8 * u + i], s = sin_s[8 * u + i];
+                    x[i] = e * c - o * s;
+                    x[8 + i] = o * c + e * s;
+                }
+            }
+            o0 = pack8(x);
+            o1 = pack8(x + 8);
+        }
+        if (in0) reinterpret_cast<uint4 *>(dst)[c0] = o0;
+        if (in1) reinterpret_cast<uint4 *>(dst)[c1] = o1;
+    }
+}
+
+// Half-split pairs whose distance is not a multiple of 8 elements: one warp per head, the head's
+// fp32 values in the warp's shared memory.
+__global__ void __launch_bounds__(APPEND_THREADS) paged_append_odd_kernel(const __grid_constant__ AppendArgs a) {
+    __shared__ float cos_s[PAGED_MAX_HEAD_DIM / 2], sin_s[PAGED_MAX_HEAD_DIM / 2];
+    __shared__ float head_s[APPEND_THREADS / 32][PAGED_MAX_HEAD_DIM];
+    pdl_trigger();
+    pdl_wait();
+    const int t = blockIdx.x, lane = threadIdx.x % 32;
+    const int4 tok = a.toks[t];
+    const int pos = tok.y, D = a.head_dim, half = a.rope_dim / 2;
+    if (pos == PAGED_OUTSIDE) return;
+    for (int j = threadIdx.x; j < half; j += APPEND_THREADS)
+        if (pos >= 0) rope_angle(pos, a.inv_freq[j], a.amplitude, &cos_s[j], &sin_s[j]);
+    __syncthreads();
+    float *x = head_s[threadIdx.x / 32];
+    for (int h = threadIdx.x / 32; h < a.n_heads + 2 * a.n_kv_heads; h += APPEND_THREADS / 32) {
+        const int kh = h - a.n_heads, vh = kh - a.n_kv_heads;
+        if (pos < 0) {
+            if (kh < 0)
+                for (int d = lane; d < D; d += 32)
+                    a.q_out[t * a.q_out_stride + (long long)h * D + d] = __float2bfloat16(0.0f);
+            continue;
+        }
+        const long long slot = tok.z * a.page_stride + tok.w * a.pos_stride;
+        if (vh >= 0) {
+            for (int d = lane; d < D; d += 32)
+                a.value_pages[slot + vh * a.head_stride + d] = a.v[t * a.v_stride + (long long)vh * D + d];
+            continue;
+        }
+        const bf16 *src = kh < 0 ? a.q + t * a.q_stride + (long long)h * D : a.k + t * a.k_stride + (long long)kh * D;
+        bf16 *dst = kh < 0 ? a.q_out + t * a.q_out_stride + (long long)h * D : a.key_pages + slot + kh * a.head_stride;
+        const bf16 *w = kh < 0 ? a.q_norm_w : a.k_norm_w;
+        float sum = 0.0f;
+        for (int d = lane; d < D; d += 32) {
+            const float v = __bfloat162float(src[d]);
+            x[d] = v;
+            sum = __fmaf_rn(v, v, sum);
+        }
+        if (w != nullptr) {
+            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            const float inv = rsqrtf(sum / D + a.eps);
+            for (int d = lane; d < D; d += 32) x[d] = x[d] * inv * __bfloat162float(w[d]);
+        }
+        __syncwarp();
+        for (int d = lane; d < D; d += 32) {
+            float y = x[d];
+            if (d < half) y = x[d] * cos_s[d] - x[d + half] * sin_s[d];
+            else if (d < 2 * half) y = x[d] * cos_s[d - half] + x[d - half] * sin_s[d - half];
+            dst[d] = __float2bfloat16(y);
+        }
+        __syncwarp();
+    }
+}
+
+// ------------------------------------------------------------------ attention
+struct PagedAttnArgs {
+    bf16 *out;
+    const bf16 *q, *key_pages, *value_pages;
+    long long out_stride, q_stride, page_stride, head_stride, pos_stride;
+    const int *table;
+    const int4 *toks;
+    int n_heads, rep, head_dim, page_size, max_pages;
+    float scale_log2;  // scale * log2(e)
+};
+
+// One warp per (token, query head), positions one after the other with the running maximum and sum.
+__global__ void __launch_bounds__(128) paged_attention_simple_kernel(const __grid_constant__ PagedAttnArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int t = blockIdx.x, h = blockIdx.y * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int4 tok = a.toks[t];
+    if (h >= a.n_heads || tok.y == PAGED_OUTSIDE) return;
+    float q[4], o[4] = {}, m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int d = lane + 32 * j;
+        q[j] = d < a.head_dim ? __bfloat162float(a.q[t * a.q_stride + (long long)h * a.head_dim + d]) * a.scale_log2 : 0.0f;
+    }
+    const int *pages = a.table + (size_t)max(tok.x, 0) * a.max_pages;
+    for (int p = 0; p <= tok.y; p++) {
+        const long long at = pages[p / a.page_size] * a.page_stride + h / a.rep * a.head_stride + p % a.page_size * a.pos_stride;
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int d = lane + 32 * j;
+            if (d < a.head_dim) s = __fmaf_rn(q[j], __bfloat162float(a.key_pages[at + d]), s);
+        }
+        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        const float m2 = fmaxf(m, s), base = m2 == -INFINITY ? 0.0f : m2;
+        const float c = exp2f(m - base), w = exp2f(s - base);
+        m = m2;
+        l = l * c + w;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int d = lane + 32 * j;
+            if (d < a.head_dim) o[j] = o[j] * c + w * __bfloat162float(a.value_pages[at + d]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int d = lane + 32 * j;
+        if (d < a.head_dim)
+            a.out[t * a.out_stride + (long long)h * a.head_dim + d] = __float2bfloat16(tok.y < 0 ? 0.0f : o[j] / l);
+    }
+}
+
+}  // namespace
+
+unsigned take_error_paged() {
+    unsigned v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_dev_error, sizeof(v)) != cudaSuccess) return 0;
+    if (v) cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(zero));
+    return v;
+}
+
+int paged_shape_check(const q3_paged_shape *s) {
+    if (!s) return Q3_ERR_ARG;
+    if (s->n_seqs < 0 || s->n_seqs > PAGED_MAX_SEQS || s->n_tokens < 0 || s->max_q_len < 0) return Q3_ERR_SHAPE;
+    if (s->n_heads <= 0 || s->n_kv_heads <= 0 || s->n_heads % s->n_kv_heads != 0 || s->n_heads / s->n_kv_heads > 128)
+        return Q3_ERR_SHAPE;
+    if (s->head_dim <= 0 || s->head_dim % 8 != 0 || s->head_dim > PAGED_MAX_HEAD_DIM) return Q3_ERR_SHAPE;
+    if (s->page_size <= 0 || s->page_size % 8 != 0 || s->n_pages <= 0 || s->max_pages <= 0) return Q3_ERR_SHAPE;
+    // a position, and the index of a page-table entry, fit an int
+    if ((long long)s->max_pages * s->page_size > (1ll << 30) || (long long)s->n_seqs * s->max_pages > (1ll << 30))
+        return Q3_ERR_SHAPE;
+    return Q3_OK;
+}
+
+namespace {
+int cache_check(const q3_paged_cache *c) {
+    if (!c || !c->key_pages || !c->value_pages) return Q3_ERR_ARG;
+    if (c->page_stride <= 0 || c->head_stride <= 0 || c->pos_stride <= 0) return Q3_ERR_SHAPE;
+    if (!aligned16(c->key_pages) || !aligned16(c->value_pages) || c->page_stride % 8 || c->head_stride % 8 || c->pos_stride % 8)
+        return Q3_ERR_ALIGN;
+    return Q3_OK;
+}
+
+// a row tensor: 16-byte aligned rows, at least `width` elements apart
+int rows_check(const void *p, long long stride, long long width) {
+    if (!p) return Q3_ERR_ARG;
+    if (stride < width) return Q3_ERR_SHAPE;
+    return !aligned16(p) || stride % 8 ? Q3_ERR_ALIGN : Q3_OK;
+}
+}  // namespace
+
+}  // namespace q3
+
+using namespace q3;
+
+#define TRY(expr)                     \
+    do {                              \
+        int st_ = (expr);             \
+        if (st_ != Q3_OK) return st_; \
+    } while (0)
+
+extern "C" {
+
+size_t q3_paged_plan_bytes(const q3_paged_shape *shape) {
+    return paged_shape_check(shape) == Q3_OK ? std::max<size_t>(paged_plan_layout(*shape).bytes, 256) : 0;
+}
+
+size_t q3_paged_attention_scratch_bytes(const q3_paged_shape *shape) {
+    return paged_shape_check(shape) == Q3_OK ? 256 : 0;
+}
+
+int q3_paged_plan(void *plan, const q3_paged_shape *shape, const int *q_start, const int *kv_len,
+                  const int *page_table, void *stream) {
+    TRY(paged_shape_check(shape));
+    if (!plan || !q_start || !kv_len || !page_table) return Q3_ERR_ARG;
+    if (!aligned16(plan)) return Q3_ERR_ALIGN;
+    TRY(check_device());
+    PlanArgs a = {static_cast<char *>(plan), paged_plan_layout(*shape), *shape, q_start, kv_len, page_table};
+    Q3_TRY_LAUNCH(launch(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, (cudaStream_t)stream, 1, a));
+    return Q3_OK;
+}
+
+int q3_paged_rope_append(q3_bf16 *q_out, long long q_out_stride, const q3_bf16 *q, long long q_stride,
+                         const q3_bf16 *k, long long k_stride, const q3_bf16 *v, long long v_stride,
+                         const q3_bf16 *q_norm_w, const q3_bf16 *k_norm_w, float eps, const float *inv_freq,
+                         int rope_dim, int interleaved, float amplitude, const q3_paged_cache *cache,
+                         const q3_paged_shape *shape, const void *plan, void *stream) {
+    TRY(paged_shape_check(shape));
+    const q3_paged_shape &s = *shape;
+    const long long qd = (long long)s.n_heads * s.head_dim, kd = (long long)s.n_kv_heads * s.head_dim;
+    if (!plan) return Q3_ERR_ARG;
+    TRY(rows_check(q_out, q_out_stride, qd));
+    TRY(rows_check(q, q_stride, qd));
+    TRY(rows_check(k, k_stride, kd));
+    TRY(rows_check(v, v_stride, kd));
+    TRY(cache_check(cache));
+    if (rope_dim < 0 || rope_dim > s.head_dim || rope_dim % 2 != 0) return Q3_ERR_SHAPE;
+    if (rope_dim > 0 && !inv_freq) return Q3_ERR_ARG;
+    if (q_out == q && q_out_stride != q_stride) return Q3_ERR_SHAPE;
+    if (!aligned16(q_norm_w) || !aligned16(k_norm_w) || !aligned16(plan)) return Q3_ERR_ALIGN;
+    TRY(check_device());
+    if (s.n_tokens == 0) return Q3_OK;
+    AppendArgs a;
+    a.q_out = (bf16 *)q_out;
+    a.q = (const bf16 *)q;
+    a.k = (const bf16 *)k;
+    a.v = (const bf16 *)v;
+    a.q_norm_w = (const bf16 *)q_norm_w;
+    a.k_norm_w = (const bf16 *)k_norm_w;
+    a.inv_freq = inv_freq;
+    a.key_pages = (bf16 *)cache->key_pages;
+    a.value_pages = (bf16 *)cache->value_pages;
+    a.q_out_stride = q_out_stride;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.page_stride = cache->page_stride;
+    a.head_stride = cache->head_stride;
+    a.pos_stride = cache->pos_stride;
+    a.toks = reinterpret_cast<const int4 *>(static_cast<const char *>(plan) + paged_plan_layout(s).toks);
+    a.n_heads = s.n_heads;
+    a.n_kv_heads = s.n_kv_heads;
+    a.head_dim = s.head_dim;
+    a.rope_dim = rope_dim;
+    a.eps = eps;
+    a.amplitude = amplitude;
+    const int chunks = s.head_dim / 8, hc = interleaved ? 0 : rope_dim / 16;
+    const int units = hc + (chunks - 2 * hc + 1) / 2;
+    for (a.lph = 1; a.lph < units;) a.lph *= 2;
+    cudaStream_t st = (cudaStream_t)stream;
+    const dim3 grid(s.n_tokens), block(APPEND_THREADS);
+    if (interleaved) Q3_TRY_LAUNCH(launch(paged_append_kernel<true>, grid, block, 0, st, 1, a));
+    else if (rope_dim % 16 == 0) Q3_TRY_LAUNCH(launch(paged_append_kernel<false>, grid, block, 0, st, 1, a));
+    else Q3_TRY_LAUNCH(launch(paged_append_odd_kernel, grid, block, 0, st, 1, a));
+    return Q3_OK;
+}
+
+int q3_paged_attention(q3_bf16 *out, long long out_stride, const q3_bf16 *q, long long q_stride,
+                       const q3_paged_cache *cache, float scale, const q3_paged_shape *shape, const void *plan,
+                       void *scratch, void *stream) {
+    TRY(paged_shape_check(shape));
+    const q3_paged_shape &s = *shape;
+    const long long qd = (long long)s.n_heads * s.head_dim;
+    if (!plan || !scratch) return Q3_ERR_ARG;
+    TRY(rows_check(out, out_stride, qd));
+    TRY(rows_check(q, q_stride, qd));
+    TRY(cache_check(cache));
+    if (!aligned16(plan) || !aligned16(scratch)) return Q3_ERR_ALIGN;
+    TRY(check_device());
+    if (s.n_tokens == 0) return Q3_OK;
+    const PagedPlanLayout l = paged_plan_layout(s);
+    PagedAttnArgs a;
+    a.out = (bf16 *)out;
+    a.q = (const bf16 *)q;
+    a.key_pages = (const bf16 *)cache->key_pages;
+    a.value_pages = (const bf16 *)cache->value_pages;
+    a.out_stride = out_stride;
+    a.q_stride = q_stride;
+    a.page_stride = cache->page_stride;
+    a.head_stride = cache->head_stride;
+    a.pos_stride = cache->pos_stride;
+    a.table = reinterpret_cast<const int *>(static_cast<const char *>(plan) + l.table);
+    a.toks = reinterpret_cast<const int4 *>(static_cast<const char *>(plan) + l.toks);
+    a.n_heads = s.n_heads;
+    a.rep = s.n_heads / s.n_kv_heads;
+    a.head_dim = s.head_dim;
+    a.page_size = s.page_size;
+    a.max_pages = s.max_pages;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    Q3_TRY_LAUNCH(launch(paged_attention_simple_kernel, dim3(s.n_tokens, (s.n_heads + 3) / 4), dim3(128), 0,
+                         (cudaStream_t)stream, 1, a));
+    return Q3_OK;
+}
+
+int q3_rope_inv_freq(float *inv_freq, float *amplitude, int rope_dim, float theta, const q3_rope_scaling *scaling) {
+    if (!inv_freq || !amplitude) return Q3_ERR_ARG;
+    if (rope_dim <= 0 || rope_dim % 2 != 0 || !(theta > 1.0f)) return Q3_ERR_SHAPE;
+    q3_rope_scaling sc = {};
+    if (scaling) sc = *scaling;
+    const double pi = 3.14159265358979323846;
+    const bool parts = sc.kind == Q3_ROPE_BY_PARTS, yarn = sc.kind == Q3_ROPE_YARN;
+    if (sc.kind < Q3_ROPE_PLAIN || sc.kind > Q3_ROPE_YARN) return Q3_ERR_ARG;
+    if (sc.kind != Q3_ROPE_PLAIN && !(sc.factor >= 1.0f && std::isfinite(sc.factor))) return Q3_ERR_SHAPE;
+    if ((parts || yarn) && sc.original_max <= 0) return Q3_ERR_SHAPE;
+    if (parts && !(sc.low_freq_factor > 0 && sc.high_freq_factor > sc.low_freq_factor)) return Q3_ERR_SHAPE;
+    if (yarn && !(sc.beta_slow > 0 && sc.beta_fast > sc.beta_slow && sc.attention_factor >= 0)) return Q3_ERR_SHAPE;
+    // YaRN: pair j turns original_max * theta^(-2j/d) / 2 pi times; the j that turns beta times
+    auto pair_of = [&](double beta) {
+        return rope_dim * log(sc.original_max / (beta * 2 * pi)) / (2 * log((double)theta));
+    };
+    const double low = yarn ? std::max(floor(pair_of(sc.beta_fast)), 0.0) : 0.0;
+    const double high = yarn ? std::min(ceil(pair_of(sc.beta_slow)), (double)(rope_dim - 1)) : 1.0;
+    for (int j = 0; j < rope_dim / 2; j++) {
+        double f = pow((double)theta, -2.0 * j / rope_dim);
+        double keep = 1.0;  // share of the unscaled frequency
+        if (sc.kind == Q3_ROPE_LINEAR) keep = 0.0;
+        if (parts)
+            keep = std::min(1.0, std::max(0.0, (sc.original_max * f / (2 * pi) - sc.low_freq_factor) /
+                                                   ((double)sc.high_freq_factor - sc.low_freq_factor)));
+        if (yarn) keep = 1.0 - std::min(1.0, std::max(0.0, (j - low) / std::max(high - low, 0.001)));
+        if (sc.kind != Q3_ROPE_PLAIN) f = keep * f + (1.0 - keep) * f / sc.factor;
+        inv_freq[j] = (float)f;
+    }
+    *amplitude = !yarn ? 1.0f : sc.attention_factor > 0 ? sc.attention_factor : (float)(0.1 * log((double)sc.factor) + 1.0);
+    return Q3_OK;
+}
+
+}  // extern "C"

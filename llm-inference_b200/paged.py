@@ -1,0 +1,193 @@
+"""Paged serving: the step plan, rotary append, attention over pages and logits processing.
+
+Page tensors are [n_pages, n_kv_heads, page_size, head_dim] torch views with a contiguous last
+dimension; a pool laid out [n_pages, page_size, n_kv_heads, head_dim] is passed as
+``pool.transpose(1, 2)``. Launches go to torch's current stream unless one is given.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+
+from ._lib import Q3Error, call, load
+
+_SHAPE, _ARG = 1, 5
+
+
+class Q3PagedShape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("n_seqs", "n_tokens", "max_q_len", "n_heads", "n_kv_heads", "head_dim",
+                                            "page_size", "n_pages", "max_pages")]
+
+
+class Q3PagedCache(ctypes.Structure):
+    _fields_ = [("key_pages", ctypes.c_void_p), ("value_pages", ctypes.c_void_p), ("page_stride", ctypes.c_longlong),
+                ("head_stride", ctypes.c_longlong), ("pos_stride", ctypes.c_longlong)]
+
+
+class Q3RopeScaling(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int), ("factor", ctypes.c_float), ("low_freq_factor", ctypes.c_float),
+                ("high_freq_factor", ctypes.c_float), ("beta_fast", ctypes.c_float), ("beta_slow", ctypes.c_float),
+                ("attention_factor", ctypes.c_float), ("original_max", ctypes.c_int)]
+
+
+ROPE_KINDS = {"plain": 0, "linear": 1, "by_parts": 2, "yarn": 3}
+
+
+def _stream(stream):
+    if stream is not None:
+        return stream
+    import torch
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _refuse(name, what, status=_ARG):
+    raise Q3Error(name, status, what)
+
+
+def _rows(name, t, what, width, dtype):
+    """Row stride of a [rows, ...] tensor whose rows are `width` contiguous elements."""
+    if t.dtype != dtype or not t.is_cuda:
+        _refuse(name, f"{what} must be a CUDA tensor of {dtype}")
+    n = 1
+    for size, step in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if size != 1 and step != n:
+            _refuse(name, f"{what}: a row's elements must be contiguous")
+        n *= size
+    if n != width:
+        _refuse(name, f"{what}: {n} elements a row, expected {width}", _SHAPE)
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+def _vector(name, t, what, size, dtype):
+    if t is None:
+        return None
+    if t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
+        _refuse(name, f"{what} must be a contiguous CUDA tensor of {dtype}")
+    if size is not None and t.numel() != size:
+        _refuse(name, f"{what}: {t.numel()} elements, expected {size}", _SHAPE)
+    return t.data_ptr()
+
+
+class PagedPlan:
+    """Device work list of a step (q3_paged_plan): make one for the step's shape, `update` it once
+    per step, use it in every layer. Owns the attention's scratch too, so calls that share a plan
+    must follow each other on one stream (or be ordered by the caller)."""
+
+    def __init__(self, n_seqs: int, n_tokens: int, max_q_len: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                 page_size: int, n_pages: int, max_pages: int, device="cuda"):
+        import torch
+        self.shape = Q3PagedShape(n_seqs, n_tokens, max_q_len, n_heads, n_kv_heads, head_dim, page_size, n_pages,
+                                  max_pages)
+        self._shape = ctypes.byref(self.shape)
+        n = load().q3_paged_plan_bytes(self._shape)
+        if n == 0:
+            _refuse("q3_paged_plan", "the shape is not supported", _SHAPE)
+        self.plan = torch.empty(n, dtype=torch.uint8, device=device)
+        self.scratch = torch.empty(load().q3_paged_attention_scratch_bytes(self._shape), dtype=torch.uint8,
+                                   device=device)
+        self._caches = {}
+
+    def update(self, q_start, kv_len, page_table, stream=None):
+        import torch
+        s, name = self.shape, "q3_paged_plan"
+        call(name, self.plan.data_ptr(), self._shape, _vector(name, q_start, "q_start", s.n_seqs + 1, torch.int32),
+             _vector(name, kv_len, "kv_len", s.n_seqs, torch.int32),
+             _vector(name, page_table, "page_table", s.n_seqs * s.max_pages, torch.int32), _stream(stream))
+
+    def cache(self, name, key_pages, value_pages) -> Q3PagedCache:
+        import torch
+        s = self.shape
+        want = (s.n_pages, s.n_kv_heads, s.page_size, s.head_dim)
+        for t in (key_pages, value_pages):
+            if t.dtype != torch.bfloat16 or not t.is_cuda:
+                _refuse(name, "pages must be CUDA tensors of torch.bfloat16")
+            if tuple(t.shape) != want:
+                _refuse(name, f"pages {tuple(t.shape)}, expected {want}", _SHAPE)
+            if t.stride(3) != 1:
+                _refuse(name, "pages: the last dimension must be contiguous")
+        if key_pages.stride() != value_pages.stride():
+            _refuse(name, "key and value pages must have the same strides", _SHAPE)
+        return Q3PagedCache(key_pages.data_ptr(), value_pages.data_ptr(), key_pages.stride(0), key_pages.stride(1),
+                            key_pages.stride(2))
+
+
+def _tokens(name, plan, **tensors):
+    for what, t in tensors.items():
+        if t.shape[0] != plan.shape.n_tokens:
+            _refuse(name, f"{what}: {t.shape[0]} rows, the plan has {plan.shape.n_tokens}", _SHAPE)
+
+
+def paged_rope_append(q_out, q, k, v, key_pages, value_pages, plan: PagedPlan, inv_freq=None, q_norm_w=None,
+                      k_norm_w=None, eps: float = 1e-6, interleaved: bool = False, amplitude: float = 1.0, stream=None):
+    """Norms, rotary positions and the write into the pages (q3_paged_rope_append). inv_freq holds
+    rope_dim / 2 fp32 frequencies on the device (`rope_inv_freq`); None rotates nothing."""
+    import torch
+    name, s, bf = "q3_paged_rope_append", plan.shape, torch.bfloat16
+    qd, kd = s.n_heads * s.head_dim, s.n_kv_heads * s.head_dim
+    _tokens(name, plan, q_out=q_out, q=q, k=k, v=v)
+    call(name, q_out.data_ptr(), _rows(name, q_out, "q_out", qd, bf), q.data_ptr(), _rows(name, q, "q", qd, bf),
+         k.data_ptr(), _rows(name, k, "k", kd, bf), v.data_ptr(), _rows(name, v, "v", kd, bf),
+         _vector(name, q_norm_w, "q_norm_w", s.head_dim, bf), _vector(name, k_norm_w, "k_norm_w", s.head_dim, bf), eps,
+         _vector(name, inv_freq, "inv_freq", None, torch.float32), 0 if inv_freq is None else 2 * inv_freq.numel(),
+         int(interleaved), amplitude, ctypes.byref(plan.cache(name, key_pages, value_pages)), plan._shape,
+         plan.plan.data_ptr(), _stream(stream))
+
+
+def paged_attention(out, q, key_pages, value_pages, plan: PagedPlan, scale: float | None = None, stream=None):
+    """Attention of the step's new tokens over the pages (q3_paged_attention); scale defaults to
+    1 / sqrt(head_dim)."""
+    import torch
+    name, s, bf = "q3_paged_attention", plan.shape, torch.bfloat16
+    qd = s.n_heads * s.head_dim
+    _tokens(name, plan, out=out, q=q)
+    call(name, out.data_ptr(), _rows(name, out, "out", qd, bf), q.data_ptr(), _rows(name, q, "q", qd, bf),
+         ctypes.byref(plan.cache(name, key_pages, value_pages)), s.head_dim ** -0.5 if scale is None else scale,
+         plan._shape, plan.plan.data_ptr(), plan.scratch.data_ptr(), _stream(stream))
+
+
+def rope_inv_freq(rope_dim: int, theta: float, kind: str = "plain", **scaling) -> tuple[np.ndarray, float]:
+    """(fp32 frequencies, amplitude of cos and sin) on the host (q3_rope_inv_freq). kind is 'plain',
+    'linear', 'by_parts' or 'yarn'; the other arguments are q3_rope_scaling's fields."""
+    if kind not in ROPE_KINDS:
+        _refuse("q3_rope_inv_freq", f"unknown kind {kind!r}")
+    sc = Q3RopeScaling(kind=ROPE_KINDS[kind], **scaling)
+    out = np.zeros(max(rope_dim // 2, 1), np.float32)
+    amplitude = ctypes.c_float(0.0)
+    call("q3_rope_inv_freq", out.ctypes.data, ctypes.byref(amplitude), rope_dim, theta, ctypes.byref(sc))
+    return out, amplitude.value
+
+
+def logits_process(out, logits, hist_start=None, hist_split=None, hist_ids=None, repetition=None, frequency=None,
+                   presence=None, bias_start=None, bias_ids=None, bias=None, mask=None, stream=None):
+    """Penalties, biases and grammar masks on [rows, vocab] logits, bf16 or fp32 (q3_logits_process);
+    out may be logits. mask is int32 [rows, >= ceil(vocab / 32)], one bit per allowed token."""
+    import torch
+    name = "q3_logits_process"
+    if logits.dim() != 2 or out.shape != logits.shape:
+        _refuse(name, "logits and out must both be [rows, vocab]", _SHAPE)
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        _refuse(name, "logits must be bfloat16 or float32")
+    rows, vocab = logits.shape
+    i32, f32 = torch.int32, torch.float32
+    mask_stride = 0
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[0] != rows:
+            _refuse(name, "mask must be [rows, words]", _SHAPE)
+        mask_stride = _rows(name, mask, "mask", mask.shape[1], i32)
+        if mask.shape[1] * 32 < vocab:
+            _refuse(name, "mask: too few words a row", _SHAPE)
+    if bias is not None and bias_ids is not None and bias.numel() != bias_ids.numel():
+        _refuse(name, "bias and bias_ids differ in length", _SHAPE)
+    if hist_ids is not None and hist_ids.numel() == 0:  # an empty tensor has no address to pass
+        hist_start = hist_split = hist_ids = None
+    if bias_ids is not None and bias_ids.numel() == 0:
+        bias_start = bias_ids = bias = None
+    call(name, out.data_ptr(), logits.data_ptr(), int(logits.dtype == f32), rows, vocab,
+         _rows(name, out, "out", vocab, logits.dtype), _rows(name, logits, "logits", vocab, logits.dtype),
+         _vector(name, hist_start, "hist_start", rows + 1, i32), _vector(name, hist_split, "hist_split", rows, i32),
+         _vector(name, hist_ids, "hist_ids", None, i32), _vector(name, repetition, "repetition", rows, f32),
+         _vector(name, frequency, "frequency", rows, f32), _vector(name, presence, "presence", rows, f32),
+         _vector(name, bias_start, "bias_start", rows + 1, i32), _vector(name, bias_ids, "bias_ids", None, i32),
+         _vector(name, bias, "bias", None, f32), None if mask is None else mask.data_ptr(), mask_stride,
+         _stream(stream))

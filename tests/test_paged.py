@@ -1,0 +1,167 @@
+"""Paged serving without a GPU: rotary frequencies, shape support and refusals of the C entries."""
+import ctypes
+import math
+import sys
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+HERE = Path(__file__).resolve().parent
+sys.path.insert(0, str(HERE))
+import conftest  # noqa: E402,F401
+import llm_inference_b200 as q3  # noqa: E402
+from llm_inference_b200 import _lib, build, paged  # noqa: E402
+
+
+@pytest.fixture(scope="module", autouse=True)
+def lib():
+    build.build()
+    return _lib.load()
+
+
+def plain(d, theta):
+    return theta ** (-np.arange(0, d, 2, dtype=np.float64) / d)
+
+
+def close(got, want):  # one fp32 rounding of a double
+    assert got.dtype == np.float32
+    assert np.all(np.abs(got - want) <= 2.0 ** -23 * np.abs(want))
+
+
+@pytest.mark.parametrize("d", [2, 20, 64, 128])
+@pytest.mark.parametrize("theta", [1e4, 1e6])
+def test_plain_and_linear_frequencies(d, theta):
+    f, a = q3.rope_inv_freq(d, theta)
+    close(f, plain(d, theta))
+    assert a == 1.0
+    f, a = q3.rope_inv_freq(d, theta, "linear", factor=4.0)
+    close(f, plain(d, theta) / 4)
+    assert a == 1.0
+
+
+def test_frequencies_by_parts():
+    f, a = q3.rope_inv_freq(128, 5e5, "by_parts", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
+                            original_max=8192)
+    want = []
+    for w in plain(128, 5e5):
+        wave = 2 * math.pi / w
+        if wave < 8192 / 4:
+            want.append(w)
+        elif wave > 8192:
+            want.append(w / 8)
+        else:
+            t = (8192 / wave - 1) / 3
+            want.append((1 - t) * w / 8 + t * w)
+    close(f, np.array(want))
+    assert a == 1.0 and want[0] == 1.0 and want[-1] < plain(128, 5e5)[-1]
+
+
+def test_yarn_frequencies():
+    d, theta, factor, orig = 128, 1e6, 4.0, 32768
+    f, a = q3.rope_inv_freq(d, theta, "yarn", factor=factor, beta_fast=32.0, beta_slow=1.0, original_max=orig)
+    w = plain(d, theta)
+    turns = orig * w / (2 * math.pi)
+    # pairs that turn more than beta_fast times keep their frequency, those below beta_slow are divided
+    low = math.floor(d * math.log(orig / (32 * 2 * math.pi)) / (2 * math.log(theta)))
+    high = math.ceil(d * math.log(orig / (2 * math.pi)) / (2 * math.log(theta)))
+    ramp = np.clip((np.arange(64) - low) / (high - low), 0, 1)
+    close(f, w * (1 - ramp) + w / factor * ramp)
+    assert turns[low] >= 32 and turns[min(high, 63)] <= 1
+    assert abs(a - (0.1 * math.log(factor) + 1)) < 1e-6
+    assert q3.rope_inv_freq(d, theta, "yarn", factor=factor, beta_fast=32.0, beta_slow=1.0, original_max=orig,
+                            attention_factor=1.25)[1] == 1.25
+
+
+@pytest.mark.parametrize("kw", [
+    dict(rope_dim=0), dict(rope_dim=7), dict(theta=1.0), dict(theta=float("nan")), dict(kind="linear", factor=0.5),
+    dict(kind="linear", factor=float("inf")), dict(kind="by_parts", factor=2.0, low_freq_factor=4.0, high_freq_factor=1.0,
+                                                   original_max=10),
+    dict(kind="yarn", factor=2.0, beta_fast=1.0, beta_slow=2.0, original_max=10),
+    dict(kind="yarn", factor=2.0, beta_fast=32.0, beta_slow=1.0, original_max=0)])
+def test_frequencies_refuse(kw):
+    kw = dict(dict(rope_dim=64, theta=1e4), **kw)
+    with pytest.raises(q3.Q3Error) as e:
+        q3.rope_inv_freq(kw.pop("rope_dim"), kw.pop("theta"), **kw)
+    assert e.value.status == 1
+    with pytest.raises(q3.Q3Error):
+        q3.rope_inv_freq(64, 1e4, "unknown")
+
+
+GOOD = dict(n_seqs=4, n_tokens=9, max_q_len=3, n_heads=32, n_kv_heads=8, head_dim=128, page_size=16, n_pages=100,
+            max_pages=20)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(head_dim=136), dict(head_dim=100), dict(head_dim=0), dict(n_kv_heads=5), dict(n_kv_heads=0), dict(n_heads=0),
+    dict(n_heads=129, n_kv_heads=1), dict(page_size=12), dict(page_size=0), dict(n_pages=0), dict(max_pages=0),
+    dict(n_seqs=-1), dict(n_seqs=4097), dict(n_tokens=-1), dict(max_q_len=-1), dict(max_pages=1 << 28)])
+def test_unsupported_shapes(lib, bad):
+    good = paged.Q3PagedShape(**GOOD)
+    assert lib.q3_paged_plan_bytes(ctypes.byref(good)) > 0
+    assert lib.q3_paged_attention_scratch_bytes(ctypes.byref(good)) > 0
+    s = paged.Q3PagedShape(**dict(GOOD, **bad))
+    assert lib.q3_paged_plan_bytes(ctypes.byref(s)) == 0
+    assert lib.q3_paged_attention_scratch_bytes(ctypes.byref(s)) == 0
+    fake = 4096  # never dereferenced: refused before any launch
+    assert lib.q3_paged_plan(fake, ctypes.byref(s), fake, fake, fake, None) == 1
+    c = paged.Q3PagedCache(fake, fake, 16 * 8 * 128, 16 * 128, 128)
+    assert lib.q3_paged_attention(fake, 1 << 20, fake, 1 << 20, ctypes.byref(c), 0.1, ctypes.byref(s), fake, fake, None) == 1
+
+
+def attention(lib, **kw):
+    fake = 4096
+    a = dict(out=fake, out_stride=4096, q=fake, q_stride=4096, kp=fake, vp=fake, page=16 * 8 * 128, head=16 * 128,
+             pos=128, plan=fake, scratch=fake)
+    a.update(kw)
+    c = paged.Q3PagedCache(a["kp"], a["vp"], a["page"], a["head"], a["pos"])
+    s = paged.Q3PagedShape(**GOOD)
+    return lib.q3_paged_attention(a["out"], a["out_stride"], a["q"], a["q_stride"], ctypes.byref(c), 0.1,
+                                  ctypes.byref(s), a["plan"], a["scratch"], None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(out=None), 5), (dict(q=None), 5), (dict(kp=None), 5), (dict(vp=None), 5), (dict(plan=None), 5),
+    (dict(scratch=None), 5), (dict(q_stride=4088), 1), (dict(out_stride=0), 1), (dict(page=0), 1), (dict(pos=-128), 1),
+    (dict(q=4098), 2), (dict(kp=4104), 2), (dict(head=4), 2), (dict(out_stride=4100), 2), (dict(plan=4097), 2)])
+def test_attention_refuses(lib, kw, status):
+    assert attention(lib, **kw) == status
+
+
+def append(lib, **kw):
+    fake = 4096
+    a = dict(q_out=8192, q_out_stride=4096, q=fake, q_stride=4096, k=fake, k_stride=1024, v=fake, v_stride=1024, qw=fake,
+             kw=fake, f=fake, rope=128, pos=128, plan=fake)
+    a.update(kw)
+    c = paged.Q3PagedCache(fake, fake, 16 * 8 * 128, 16 * 128, a["pos"])
+    s = paged.Q3PagedShape(**GOOD)
+    return lib.q3_paged_rope_append(a["q_out"], a["q_out_stride"], a["q"], a["q_stride"], a["k"], a["k_stride"], a["v"],
+                                    a["v_stride"], a["qw"], a["kw"], 1e-6, a["f"], a["rope"], 0, 1.0, ctypes.byref(c),
+                                    ctypes.byref(s), a["plan"], None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(q_out=None), 5), (dict(k=None), 5), (dict(v=None), 5), (dict(plan=None), 5), (dict(f=None), 5),
+    (dict(rope=130), 1), (dict(rope=-2), 1), (dict(rope=63), 1), (dict(k_stride=1016), 1), (dict(pos=0), 1),
+    (dict(q_out=4096, q_out_stride=8192), 1), (dict(qw=4100), 2), (dict(k_stride=1028), 2), (dict(v=4100), 2)])
+def test_append_refuses(lib, kw, status):
+    assert append(lib, **kw) == status
+
+
+def logits(lib, **kw):
+    fake = 4096
+    a = dict(out=fake, x=fake, dtype=0, rows=2, vocab=1000, out_stride=1000, stride=1000, hs=fake, hp=fake, hi=fake,
+             bs=fake, bi=fake, b=fake, mask=fake, ms=32)
+    a.update(kw)
+    return lib.q3_logits_process(a["out"], a["x"], a["dtype"], a["rows"], a["vocab"], a["out_stride"], a["stride"],
+                                 a["hs"], a["hp"], a["hi"], fake, fake, fake, a["bs"], a["bi"], a["b"], a["mask"],
+                                 a["ms"], None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(out=None), 5), (dict(x=None), 5), (dict(dtype=2), 5), (dict(hp=None), 5), (dict(hi=None), 5), (dict(bi=None), 5),
+    (dict(b=None), 5), (dict(rows=-1), 1), (dict(rows=65536), 1), (dict(vocab=0), 1), (dict(stride=999), 1),
+    (dict(out_stride=999), 1), (dict(out_stride=1001), 1), (dict(ms=31), 1), (dict(out=4097), 2),
+    (dict(x=4098, dtype=1, out=8192), 2)])
+def test_logits_refuse(lib, kw, status):
+    assert logits(lib, **kw) == status
