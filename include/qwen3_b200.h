@@ -409,7 +409,7 @@ int q3_paged_rope_append(q3_bf16 *q_out, long long q_out_stride, const q3_bf16 *
  * product as bf16. NaN or infinite values in the cache reach only the rows that attend to their
  * position. */
 int q3_paged_attention(q3_bf16 *out, long long out_stride, const q3_bf16 *q, long long q_stride,
-                       const q3_paged_cache *cache, float scale, const q3_paged_shape *shape, const void *plan,
+                       const q3_paged_cache *cache, float scale, const q3_paged_shape *shape, void *plan,
                        void *scratch, void *stream);
 
 /* How the rotation frequencies theta^(-2j/rope_dim) are changed for contexts longer than the

@@ -25,10 +25,77 @@ struct PlanArgs {
     PagedPlanLayout l;
     q3_paged_shape s;
     const int *q_start, *kv_len, *page_table;
+    int n_ctas;
 };
 
+// Costs, in sixteen-KB loads' worth of a CTA's time: a step of a small item is one (32 or 64 positions of
+// K and V), a 128-position step of one or two tensor-core tiles BIG_ONE or BIG_TWO; an item's start and
+// end (queries, merge, output) ITEM. Items are cut only while each CTA still gets MIN_SHARE.
+constexpr int COST_ITEM = 3, COST_BIG_ONE = 2, COST_BIG_TWO = 3, MIN_SHARE = 16;
+
+// The items of sequence q: a big one has n_q per kv head.
+struct SeqItems {
+    bool big;
+    int n_q, span;  // items per kv head, tokens of each
+};
+
+__device__ __forceinline__ SeqItems seq_items(const PagedSeq &q, int rep) {
+    SeqItems s;
+    s.big = (long long)q.q_len * rep > SMALL_ROWS;
+    s.span = s.big ? 2 * (BIG_TILE / rep) : q.q_len;
+    s.n_q = q.q_len == 0 ? 0 : (q.q_len + s.span - 1) / s.span;
+    return s;
+}
+
+// Item i's positions end here, it has this many steps, and each costs this much.
+__device__ __forceinline__ void item_steps(const PagedSeq &q, const SeqItems &s, int i, int rep, int step, int *end, int *n,
+                                           int *cost) {
+    const int last = min((i + 1) * s.span, q.q_len);
+    *end = max(0, q.kv_len - q.q_len + last);
+    *n = max(1, (*end + step - 1) / step);
+    *cost = !s.big ? 1 : last - i * s.span > s.span / 2 ? COST_BIG_TWO : COST_BIG_ONE;
+}
+
+// Steps of an item that lie before cost r of it.
+__device__ __forceinline__ int steps_before(long long r, int n, int cost) {
+    return (int)max(0ll, min((long long)n, (r - COST_ITEM + cost - 1) / cost));
+}
+
+// Exclusive prefix sum of v[0 .. n) in place by the whole CTA; returns the total.
+__device__ long long scan(long long *v, int n, long long *warp_sums) {
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    const int per = (n + PLAN_THREADS - 1) / PLAN_THREADS;
+    long long mine = 0;
+    for (int i = tid * per; i < min(n, (tid + 1) * per); i++) mine += v[i];
+    long long sum = mine;
+    for (int off = 1; off < 32; off *= 2) {
+        const long long o = __shfl_up_sync(0xffffffffu, sum, off);
+        if (lane >= off) sum += o;
+    }
+    if (lane == 31) warp_sums[warp] = sum;
+    __syncthreads();
+    long long before = 0, total = 0;
+    for (int w = 0; w < PLAN_THREADS / 32; w++) {
+        if (w < warp) before += warp_sums[w];
+        total += warp_sums[w];
+    }
+    before += sum - mine;
+    for (int i = tid * per; i < min(n, (tid + 1) * per); i++) {
+        const long long x = v[i];
+        v[i] = before;
+        before += x;
+    }
+    __syncthreads();
+    return total;
+}
+
 __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_constant__ PlanArgs a) {
-    __shared__ int start_s[PAGED_MAX_SEQS + 1];
+    extern __shared__ __align__(16) unsigned char plan_smem[];
+    long long *big_s = reinterpret_cast<long long *>(plan_smem);  // cost before each sequence's big items
+    long long *small_s = big_s + a.s.n_seqs + 1;                  // and before its small ones
+    long long *item_s = small_s + a.s.n_seqs + 1;                 // items before: big ones << 32 | small ones
+    int *start_s = reinterpret_cast<int *>(item_s + a.s.n_seqs + 1);
+    __shared__ long long sums_s[PLAN_THREADS / 32];
     pdl_trigger();
     pdl_wait();
     const int n = a.s.n_seqs, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -84,6 +151,106 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
             }
         }
         toks[t] = tok;
+    }
+
+    // ---- work: big items of all sequences, then small ones
+    const int rep = a.s.n_heads / a.s.n_kv_heads, kvh = a.s.n_kv_heads;
+    const int small_step = a.s.head_dim <= 64 ? 64 : 32;
+    for (int b = tid; b < n; b += PLAN_THREADS) {
+        const PagedSeq q = seqs[b];
+        const SeqItems s = seq_items(q, rep);
+        long long cost = 0;
+        for (int i = 0; i < s.n_q; i++) {
+            int end, steps, c;
+            item_steps(q, s, i, rep, s.big ? BIG_TILE : small_step, &end, &steps, &c);
+            cost += COST_ITEM + (long long)steps * c;
+        }
+        big_s[b] = s.big ? cost * kvh : 0;
+        small_s[b] = s.big ? 0 : cost * kvh;
+        item_s[b] = (long long)s.n_q * kvh << (s.big ? 32 : 0);
+    }
+    __syncthreads();
+    const long long items = scan(item_s, n, sums_s);
+    const int n_big = (int)(items >> 32), n_items = n_big + (int)(items & 0xffffffff);
+    const long long total_big = scan(big_s, n, sums_s), total = total_big + scan(small_s, n, sums_s);
+    if (tid == 0) {
+        big_s[n] = total_big;
+        small_s[n] = total - total_big;
+    }
+    __syncthreads();
+    const int used = (int)max(1ll, min((long long)a.n_ctas, max((long long)n_items, total / MIN_SHARE)));
+    int2 *ctas = reinterpret_cast<int2 *>(a.plan + a.l.ctas);
+    PagedPiece *pieces = reinterpret_cast<PagedPiece *>(a.plan + a.l.pieces);
+    PagedPiece *splits = reinterpret_cast<PagedPiece *>(a.plan + a.l.splits);
+    int *counters = reinterpret_cast<int *>(a.plan + a.l.counters);
+    // A CTA's pieces start at (items before its first) + (CTAs before it): every cut adds one piece at most.
+    for (int c = tid; c < a.n_ctas; c += PLAN_THREADS) {
+        auto bound = [&](int i) { return total * i / used; };
+        const long long u0 = c < used ? bound(c) : total, u1 = c < used ? bound(c + 1) : total;
+        int count = 0, first_piece = -1;
+        PagedPiece split = {};
+        long long u = u0;
+        while (u < u1) {
+            const bool big = u < total_big;
+            const long long *pre = big ? big_s : small_s;
+            const long long at = big ? u : u - total_big, origin = big ? 0 : total_big;
+            int lo = 0, hi = n - 1;  // the last sequence that starts at or before `at`
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (pre[mid] <= at) lo = mid;
+                else hi = mid - 1;
+            }
+            const PagedSeq q = seqs[lo];
+            const SeqItems s = seq_items(q, rep);
+            const long long per_head = (pre[lo + 1] - pre[lo]) / kvh;
+            const int head = (int)((at - pre[lo]) / per_head);
+            long long start = pre[lo] + head * per_head;
+            int i = 0, end, steps, cost;
+            long long len;
+            for (;; i++) {
+                item_steps(q, s, i, rep, big ? BIG_TILE : small_step, &end, &steps, &cost);
+                len = COST_ITEM + (long long)steps * cost;
+                if (at < start + len) break;
+                start += len;
+            }
+            start += origin;  // in the common line of costs
+            const int t0 = steps_before(u - start, steps, cost);
+            const int t1 = u1 >= start + len ? steps : steps_before(u1 - start, steps, cost);
+            if (t1 > t0) {
+                PagedPiece p;
+                const int step = big ? BIG_TILE : small_step;
+                p.seq = lo;
+                p.kvh = head;
+                p.tok0 = q.q0 + i * s.span;
+                p.n_tok = min(s.span, q.q_len - i * s.span);
+                p.kv0 = t0 * step;
+                p.kv1 = t1 == steps ? end : t1 * step;
+                p.kv_end = end;
+                p.pos0 = q.kv_len - q.q_len + i * s.span;
+                p.big = big;
+                p.part = -1;
+                p.first = c;
+                p.n_parts = 1;
+                if (t0 > 0 || t1 < steps) {
+                    int f = c;
+                    while (steps_before(bound(f) - start, steps, cost) > 0) f--;
+                    p.first = f;
+                    while (f + 1 < used && bound(f + 1) < start + len && steps_before(bound(f + 1) - start, steps, cost) < steps) f++;
+                    p.n_parts = f - p.first + 1;
+                    p.part = part_slot(p.first, c - p.first);
+                    if (t0 == 0 && big) split = p;
+                }
+                if (first_piece < 0)
+                    first_piece = (big ? (int)(item_s[lo] >> 32) : n_big + (int)(item_s[lo] & 0xffffffff)) +
+                                  head * s.n_q + i + c;
+                pieces[first_piece + count] = p;
+                count++;
+            }
+            u = start + len;
+        }
+        ctas[c] = make_int2(max(first_piece, 0), bad_starts ? -1 : count);
+        splits[c] = split;
+        counters[c] = 0;
     }
 }
 
@@ -276,65 +443,15 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_odd_kernel(const 
     }
 }
 
-// ------------------------------------------------------------------ attention
-struct PagedAttnArgs {
-    bf16 *out;
-    const bf16 *q, *key_pages, *value_pages;
-    long long out_stride, q_stride, page_stride, head_stride, pos_stride;
-    const int *table;
-    const int4 *toks;
-    int n_heads, rep, head_dim, page_size, max_pages;
-    float scale_log2;  // scale * log2(e)
-};
-
-// One warp per (token, query head), positions one after the other with the running maximum and sum.
-__global__ void __launch_bounds__(128) paged_attention_simple_kernel(const __grid_constant__ PagedAttnArgs a) {
-    pdl_trigger();
-    pdl_wait();
-    const int t = blockIdx.x, h = blockIdx.y * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int4 tok = a.toks[t];
-    if (h >= a.n_heads || tok.y == PAGED_OUTSIDE) return;
-    float q[4], o[4] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int d = lane + 32 * j;
-        q[j] = d < a.head_dim ? __bfloat162float(a.q[t * a.q_stride + (long long)h * a.head_dim + d]) * a.scale_log2 : 0.0f;
-    }
-    const int *pages = a.table + (size_t)max(tok.x, 0) * a.max_pages;
-    for (int p = 0; p <= tok.y; p++) {
-        const long long at = pages[p / a.page_size] * a.page_stride + h / a.rep * a.head_stride + p % a.page_size * a.pos_stride;
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int d = lane + 32 * j;
-            if (d < a.head_dim) s = __fmaf_rn(q[j], __bfloat162float(a.key_pages[at + d]), s);
-        }
-        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        const float m2 = fmaxf(m, s), base = m2 == -INFINITY ? 0.0f : m2;
-        const float c = exp2f(m - base), w = exp2f(s - base);
-        m = m2;
-        l = l * c + w;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int d = lane + 32 * j;
-            if (d < a.head_dim) o[j] = o[j] * c + w * __bfloat162float(a.value_pages[at + d]);
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int d = lane + 32 * j;
-        if (d < a.head_dim)
-            a.out[t * a.out_stride + (long long)h * a.head_dim + d] = __float2bfloat16(tok.y < 0 ? 0.0f : o[j] / l);
-    }
-}
-
 }  // namespace
+
+unsigned take_error_paged_attn();
 
 unsigned take_error_paged() {
     unsigned v = 0, zero = 0;
     if (cudaMemcpyFromSymbol(&v, g_dev_error, sizeof(v)) != cudaSuccess) return 0;
     if (v) cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(zero));
-    return v;
+    return v | take_error_paged_attn();
 }
 
 int paged_shape_check(const q3_paged_shape *s) {
@@ -384,7 +501,7 @@ size_t q3_paged_plan_bytes(const q3_paged_shape *shape) {
 }
 
 size_t q3_paged_attention_scratch_bytes(const q3_paged_shape *shape) {
-    return paged_shape_check(shape) == Q3_OK ? 256 : 0;
+    return paged_shape_check(shape) == Q3_OK ? paged_scratch_layout(*shape).bytes : 0;
 }
 
 int q3_paged_plan(void *plan, const q3_paged_shape *shape, const int *q_start, const int *kv_len,
@@ -393,8 +510,11 @@ int q3_paged_plan(void *plan, const q3_paged_shape *shape, const int *q_start, c
     if (!plan || !q_start || !kv_len || !page_table) return Q3_ERR_ARG;
     if (!aligned16(plan)) return Q3_ERR_ALIGN;
     TRY(check_device());
-    PlanArgs a = {static_cast<char *>(plan), paged_plan_layout(*shape), *shape, q_start, kv_len, page_table};
-    Q3_TRY_LAUNCH(launch(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, (cudaStream_t)stream, 1, a));
+    PlanArgs a = {static_cast<char *>(plan), paged_plan_layout(*shape), *shape, q_start, kv_len, page_table,
+                  paged_ctas()};
+    const size_t smem = (size_t)(shape->n_seqs + 1) * (3 * sizeof(long long) + sizeof(int));
+    Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_plan_kernel), smem));
+    Q3_TRY_LAUNCH(launch(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), smem, (cudaStream_t)stream, 1, a));
     return Q3_OK;
 }
 
@@ -454,7 +574,7 @@ int q3_paged_rope_append(q3_bf16 *q_out, long long q_out_stride, const q3_bf16 *
 }
 
 int q3_paged_attention(q3_bf16 *out, long long out_stride, const q3_bf16 *q, long long q_stride,
-                       const q3_paged_cache *cache, float scale, const q3_paged_shape *shape, const void *plan,
+                       const q3_paged_cache *cache, float scale, const q3_paged_shape *shape, void *plan,
                        void *scratch, void *stream) {
     TRY(paged_shape_check(shape));
     const q3_paged_shape &s = *shape;
@@ -465,29 +585,10 @@ int q3_paged_attention(q3_bf16 *out, long long out_stride, const q3_bf16 *q, lon
     TRY(cache_check(cache));
     if (!aligned16(plan) || !aligned16(scratch)) return Q3_ERR_ALIGN;
     TRY(check_device());
-    if (s.n_tokens == 0) return Q3_OK;
-    const PagedPlanLayout l = paged_plan_layout(s);
-    PagedAttnArgs a;
-    a.out = (bf16 *)out;
-    a.q = (const bf16 *)q;
-    a.key_pages = (const bf16 *)cache->key_pages;
-    a.value_pages = (const bf16 *)cache->value_pages;
-    a.out_stride = out_stride;
-    a.q_stride = q_stride;
-    a.page_stride = cache->page_stride;
-    a.head_stride = cache->head_stride;
-    a.pos_stride = cache->pos_stride;
-    a.table = reinterpret_cast<const int *>(static_cast<const char *>(plan) + l.table);
-    a.toks = reinterpret_cast<const int4 *>(static_cast<const char *>(plan) + l.toks);
-    a.n_heads = s.n_heads;
-    a.rep = s.n_heads / s.n_kv_heads;
-    a.head_dim = s.head_dim;
-    a.page_size = s.page_size;
-    a.max_pages = s.max_pages;
-    a.scale_log2 = scale * 1.4426950408889634f;
-    Q3_TRY_LAUNCH(launch(paged_attention_simple_kernel, dim3(s.n_tokens, (s.n_heads + 3) / 4), dim3(128), 0,
-                         (cudaStream_t)stream, 1, a));
-    return Q3_OK;
+    if (s.n_tokens == 0 || s.n_seqs == 0) return Q3_OK;
+    const PagedAttnCall c = {(bf16 *)out, (const bf16 *)q, out_stride, q_stride, *cache, scale, s,
+                             static_cast<char *>(plan), static_cast<char *>(scratch)};
+    return paged_attention(c, (cudaStream_t)stream);
 }
 
 int q3_rope_inv_freq(float *inv_freq, float *amplitude, int rope_dim, float theta, const q3_rope_scaling *scaling) {

@@ -16,13 +16,39 @@ struct PagedSeq {
     int q0, q_len, kv_len, pad;
 };
 
+// Attention work. An item is what one CTA could do alone: the query rows of a (sequence, kv head) that
+// attend together. Few rows (q_len * n_heads / n_kv_heads <= SMALL_ROWS) are one item, fed to warp-level
+// matrix instructions 16 rows high; more are cut into items of two 128-row tensor-core tiles. The plan lays
+// all items' costs end to end and gives each CTA an equal stretch, so an item may be cut along its
+// positions into pieces of neighbouring CTAs, which leave partial results in the scratch.
+constexpr int SMALL_ROWS = 16;
+constexpr int BIG_TILE = 128;       // rows of a tensor-core tile, and positions of one of its steps
+constexpr int PAGED_MAX_CTAS = 160; // persistent CTAs, one per SM
+
+struct alignas(16) PagedPiece {
+    int seq, kvh, tok0, n_tok;   // query rows: tokens tok0 .. tok0 + n_tok of the batch
+    int kv0, kv1, kv_end, pos0;  // this piece's positions, the item's end, the first token's position (< 0: padding)
+    int part, first, n_parts;    // scratch slot (-1: the item is whole), the item's first CTA, its pieces
+    int big;
+};
+
+// Where a piece of CTA c leaves its partial result: an item's first piece is its CTA's last (slot 2c + 1), the
+// later ones are the first of theirs (slot 2c).
+__host__ __device__ __forceinline__ int part_slot(int first, int i) { return i == 0 ? 2 * first + 1 : 2 * (first + i); }
+
 // Byte offsets of the plan's parts; the same arithmetic on host and device.
 struct PagedPlanLayout {
-    size_t seqs;   // PagedSeq [n_seqs]
-    size_t table;  // int [n_seqs][max_pages]: checked page ids, -1 past a sequence's last page
-    size_t toks;   // int4 [n_tokens]: sequence, position, page, slot
+    size_t seqs;      // PagedSeq [n_seqs]
+    size_t table;     // int [n_seqs][max_pages]: checked page ids, -1 past a sequence's last page
+    size_t toks;      // int4 [n_tokens]: sequence, position, page, slot
+    size_t ctas;      // int2 [PAGED_MAX_CTAS]: first piece, pieces (-1: zero every row)
+    size_t counters;  // int [PAGED_MAX_CTAS]: pieces done of the small item that starts in the CTA, zero at rest
+    size_t splits;    // PagedPiece [PAGED_MAX_CTAS]: the big item that is cut at the CTA's end (n_parts 0: none)
+    size_t pieces;    // PagedPiece []
     size_t bytes;
 };
+
+inline int paged_tile_tokens(const q3_paged_shape &s) { return BIG_TILE / (s.n_heads / s.n_kv_heads); }
 
 inline PagedPlanLayout paged_plan_layout(const q3_paged_shape &s) {
     PagedPlanLayout l = {};
@@ -32,14 +58,55 @@ inline PagedPlanLayout paged_plan_layout(const q3_paged_shape &s) {
         off += (bytes + 255) / 256 * 256;
         return o;
     };
+    const size_t items = (size_t)s.n_kv_heads * ((size_t)s.n_seqs + (size_t)s.n_tokens / (2 * paged_tile_tokens(s)));
     l.seqs = take((size_t)s.n_seqs * sizeof(PagedSeq));
     l.table = take((size_t)s.n_seqs * s.max_pages * 4);
     l.toks = take((size_t)s.n_tokens * 16);
+    l.ctas = take(PAGED_MAX_CTAS * sizeof(int2));
+    l.counters = take(PAGED_MAX_CTAS * sizeof(int));
+    l.splits = take(PAGED_MAX_CTAS * sizeof(PagedPiece));
+    l.pieces = take((items + PAGED_MAX_CTAS) * sizeof(PagedPiece));
     l.bytes = off;
     return l;
 }
 
+// Scratch of the attention: partial outputs, unnormalized fp32 rows with their maximum (in units of log2) and
+// sum, two slots per CTA.
+struct PagedScratchLayout {
+    size_t small_o, small_ml, big_o, big_ml, bytes;
+};
+
+inline bool paged_has_big(const q3_paged_shape &s) {
+    return (long long)s.max_q_len * (s.n_heads / s.n_kv_heads) > SMALL_ROWS;
+}
+
+inline PagedScratchLayout paged_scratch_layout(const q3_paged_shape &s) {
+    PagedScratchLayout l = {};
+    const size_t dp = s.head_dim <= 64 ? 64 : 128, slots = 2 * PAGED_MAX_CTAS;
+    const size_t big = paged_has_big(s) ? 2 * BIG_TILE : 0;
+    l.small_o = 0;
+    l.small_ml = l.small_o + slots * SMALL_ROWS * dp * 4;
+    l.big_o = l.small_ml + slots * SMALL_ROWS * 8;
+    l.big_ml = l.big_o + slots * big * dp * 4;
+    l.bytes = l.big_ml + slots * big * 8;
+    return l;
+}
+
+inline int paged_ctas() { return num_sms() < PAGED_MAX_CTAS ? num_sms() : PAGED_MAX_CTAS; }
+
 // Q3_OK, or why the shape is not supported.
 int paged_shape_check(const q3_paged_shape *s);
+
+// Attention over the pages (paged_attn.cu).
+struct PagedAttnCall {
+    bf16 *out;
+    const bf16 *q;
+    long long out_stride, q_stride;
+    q3_paged_cache cache;
+    float scale;
+    q3_paged_shape shape;
+    char *plan, *scratch;
+};
+int paged_attention(const PagedAttnCall &c, cudaStream_t s);
 
 }  // namespace q3

@@ -1,0 +1,1084 @@
+// Attention of each sequence's new tokens over its pages (q3_paged_attention).
+//
+//   o = sum_t p_t v_t / sum_t p_t,  p_t = 2^(c q.k_t - m),  c = scale * log2(e)
+//
+// in one pass over the positions, with a running reference m per row that the sums are rescaled to when it
+// grows. Partial results (o, m, l) of a row over disjoint positions combine as
+// m = max m_i, o = sum 2^(m_i - m) o_i, l = sum 2^(m_i - m) l_i.
+//
+// Persistent CTAs, one per SM, take the pieces the plan gave them (paged.cuh). A producer warp
+// streams K and V by TMA, one box per run of positions inside a page, into a ring of 16 KB stages; what
+// consumes them depends on the item's rows.
+//
+// Few rows (a decode step): bound by the bytes of K and V. Warp-level matrix instructions 16
+// rows high are enough for that: at 4 query heads per kv head an SM computes 16 x 32 x 128 x 2 products per 16 KB
+// stage, a small part of the time the stage takes to arrive. Each warp owns whole stages (32 positions at
+// head_dim 128) with its own running maximum, so warps meet only at the end of a piece.
+//
+// Many rows (a chunk of a prompt): bound by the tensor cores. 128 rows -- all query heads of a kv head side by
+// side, token after token -- make a tcgen05 tile; two tiles share each K and V tile and alternate, one
+// in its softmax while the other multiplies. S = Q K^T goes to tensor memory, a thread per row reads it, writes P
+// back over it as bf16, and P is the A operand of O += P V from tensor memory.
+//
+// Bad values behind the mask: a masked score is replaced, whatever it is, but a zero probability times a NaN
+// or infinite v would still be NaN. Rows of V past the item's end are zeroed in shared memory; the few
+// rows that some tokens of the item see and others do not are checked, and if one holds such a value that step's
+// second product runs on the CUDA cores, skipping what each row does not see.
+#include <math.h>
+
+#include <algorithm>
+
+#include "paged.cuh"
+#include "tc_common.cuh"
+
+namespace q3 {
+namespace {
+
+__device__ unsigned g_dev_error;
+
+constexpr int STAGE = 16384;        // bytes of a ring stage
+constexpr int SMALL_STAGES = 12;    // few-row kernel: 4 consumer warps
+constexpr int SMALL_WARPS = 4;
+constexpr int MIXED_STAGES = 10;    // kernel for both kinds: two softmax warpgroups
+constexpr int MIXED_WARPS = 8;
+constexpr float GROW = 8.0f;        // many rows: the reference follows the maximum in steps of 2^8
+
+struct PaArgs {
+    bf16 *out;
+    const bf16 *q;
+    long long out_stride, q_stride;
+    const int *table;
+    const int2 *ctas;
+    const PagedPiece *pieces, *splits;
+    int *counters;
+    float *small_o, *big_o;
+    float2 *small_ml, *big_ml;
+    int rep, tile_tok, head_dim, page_size, max_pages, n_tokens, row_elems;
+    int small_box, big_box;  // rows of a TMA box: the largest power of two that divides a page, at most a step
+    float scale_log2;
+    uint32_t idesc_qk, idesc_pv;
+};
+
+// ---------------------------------------------------------------- helpers
+
+// Waits until one has given up; from then on the role runs through its loop without waiting, so that every
+// barrier of the CTA still sees its arrivals and the kernel ends.
+struct Waiter {
+    bool dead = false;
+    __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) {
+        if (!dead) dead = !mbar_wait(bar, parity, &g_dev_error);
+    }
+};
+
+template <int N>
+struct Ring {
+    int s = 0;
+    uint32_t ph = 0;
+    __device__ __forceinline__ void next(int by = 1) {
+        s += by;
+        if (s >= N) {
+            s -= N;
+            ph ^= 1;
+        }
+    }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void tma_page(void *dst, const CUtensorMap *map, int x, int slot, int head, int page,
+                                         uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t *r, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t *r, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// one of two packed bf16 is NaN or infinite
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+__device__ __forceinline__ bool not_finite8(const uint4 &u) {
+    return not_finite2(u.x) || not_finite2(u.y) || not_finite2(u.z) || not_finite2(u.w);
+}
+
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// The step's description was refused as a whole (a negative piece count): every row is padding.
+__device__ __forceinline__ void zero_rows(const PaArgs &a) {
+    for (int t = blockIdx.x; t < a.n_tokens; t += gridDim.x)
+        for (int i = threadIdx.x; i < a.row_elems / 8; i += blockDim.x)
+            reinterpret_cast<uint4 *>(a.out + t * a.out_stride)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// The position from which on at least one row of the piece's item is masked.
+__device__ __forceinline__ int first_masked(const PagedPiece &p) { return p.pos0 + 1; }
+
+// ---------------------------------------------------------------- few rows: producer
+
+// One warp streams a piece's steps: K and V of UPOS positions, NB = DP / 64 halves of 64 columns each, in the
+// 128-byte swizzle. Each lane issues one box and looks up the next step's page while this one waits for room.
+template <int DP, int NST>
+__device__ void small_produce(const PaArgs &a, const CUtensorMap *mk, const CUtensorMap *mv, const PagedPiece &p,
+                              unsigned char *ring, uint64_t *full, uint64_t *empty, Ring<NST> &r, Waiter &wait) {
+    constexpr int NB = DP / 64, UPOS = 32 * 128 / DP;
+    const int lane = threadIdx.x % 32, box = a.small_box, nsub = UPOS / box;
+    const int sub = lane % nsub, part = lane / nsub, half = part % NB;
+    const bool active = part < 2 * NB, is_v = part >= NB;
+    const int *tab = a.table + (size_t)p.seq * a.max_pages;
+    const uint32_t off = (is_v ? NB : 0) * (UPOS * 128) + half * (UPOS * 128) + sub * box * 128;
+    int at = p.kv0 + sub * box;
+    int page = active && at < p.kv1 ? __ldg(tab + at / a.page_size) : 0;
+    int p0 = p.kv0;
+    do {
+        const int ahead = at + UPOS;
+        const int next_page = active && ahead < p.kv1 ? __ldg(tab + ahead / a.page_size) : 0;
+        wait(&empty[r.s], r.ph ^ 1);
+        __syncwarp();
+        if (lane == 0) {
+            const int n = min(nsub, max(0, (p.kv1 - p0 + box - 1) / box));
+            mbar_arrive_expect_tx(&full[r.s], (uint32_t)(n * box * 128 * NB * 2));
+        }
+        __syncwarp();
+        if (active && at < p.kv1)
+            tma_page(ring + (size_t)r.s * STAGE + off, is_v ? mv : mk, half * 64, at % a.page_size, p.kvh, page, &full[r.s]);
+        r.next();
+        at = ahead;
+        page = next_page;
+        p0 += UPOS;
+    } while (p0 < p.kv1);
+}
+
+// ---------------------------------------------------------------- few rows: consumers
+
+// merge buffer: [NW][16][DP] fp32 (columns rotated by row, so that a fragment's rows fall in
+// different banks), then [NW][16] (m, l).
+template <int DP, int NW, int NST>
+__device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned char *ring, uint64_t *full,
+                              uint64_t *empty, Ring<NST> &r, Waiter &wait, int cw, float *merge_o, float2 *merge_ml,
+                              int *flag_s) {
+    constexpr int NB = DP / 64, UPOS = 32 * 128 / DP, NT = UPOS / 8, KS = DP / 16, OT = DP / 8;
+    const int lane = threadIdx.x % 32, g = lane / 4, tq = lane % 4;
+    const int rows = p.n_tok * a.rep;
+    uint32_t qa[KS][4];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int row = g + 8 * i;
+        const bf16 *src = a.q + (p.tok0 + row / a.rep) * a.q_stride + (long long)(p.kvh * a.rep + row % a.rep) * a.head_dim;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int col = 16 * k + 8 * j + 2 * tq;
+                qa[k][2 * j + i] = row < rows && col < a.head_dim ? *reinterpret_cast<const uint32_t *>(src + col) : 0u;
+            }
+    }
+    const int lim0 = p.pos0 + g / a.rep + 1, lim1 = p.pos0 + (g + 8) / a.rep + 1, lim_min = first_masked(p);
+    float o[OT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < OT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+
+    int p0 = p.kv0;
+    do {
+        if (r.s % NW == cw) {
+            unsigned char *stage = ring + (size_t)r.s * STAGE;
+            const uint32_t kb = smem_u32(stage), vb = kb + NB * UPOS * 128;
+            wait(&full[r.s], r.ph);
+            __syncwarp();
+            float s[NT][4];
+#pragma unroll
+            for (int i = 0; i < NT; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+            const int mi = lane / 8, l7 = lane % 8;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const int c = 2 * k + (mi & 1);
+                const uint32_t col = (c / 8) * (UPOS * 128) + (((c % 8) ^ l7) << 4);
+#pragma unroll
+                for (int t = 0; t < NT / 2; t++) {
+                    uint32_t b[4];
+                    ldsm4(b, kb + col + (t * 16 + (mi >> 1) * 8 + l7) * 128);
+                    mma16816(s[2 * t], qa[k], b[0], b[1]);
+                    mma16816(s[2 * t + 1], qa[k], b[2], b[3]);
+                }
+            }
+            const bool masked = p0 + UPOS > lim_min;
+            float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float &u = s[i][j], &w = s[i][2 + j];
+                    u *= a.scale_log2;
+                    w *= a.scale_log2;
+                    if (masked) {
+                        const int t = p0 + i * 8 + 2 * tq + j;
+                        if (t >= lim0) u = -INFINITY;
+                        if (t >= lim1) w = -INFINITY;
+                    }
+                    x0 = fmaxf(x0, u);
+                    x1 = fmaxf(x1, w);
+                }
+#pragma unroll
+            for (int off = 1; off < 4; off *= 2) {
+                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
+                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
+            }
+            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+                const float f0 = n0 == -INFINITY ? 1.0f : ex2(m0 - n0), f1 = n1 == -INFINITY ? 1.0f : ex2(m1 - n1);
+                m0 = n0;
+                m1 = n1;
+                l0 *= f0;
+                l1 *= f1;
+#pragma unroll
+                for (int i = 0; i < OT; i++) {
+                    o[i][0] *= f0;
+                    o[i][1] *= f0;
+                    o[i][2] *= f1;
+                    o[i][3] *= f1;
+                }
+            }
+            const float base0 = m0 == -INFINITY ? 0.0f : m0, base1 = m1 == -INFINITY ? 0.0f : m1;
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    s[i][j] = ex2(s[i][j] - base0);
+                    s[i][2 + j] = ex2(s[i][2 + j] - base1);
+                    l0 += s[i][j];
+                    l1 += s[i][2 + j];
+                }
+            bool touched = false, slow = false;
+            if (p0 + UPOS > p.kv_end) {  // rows past the item's end: zero
+                const int t0 = max(0, p.kv_end - p0), n = (UPOS - t0) * 8;
+                for (int h = 0; h < NB; h++)
+                    for (int i = lane; i < n; i += 32)
+                        reinterpret_cast<uint4 *>(stage + (NB + h) * (UPOS * 128) + t0 * 128)[i] = make_uint4(0, 0, 0, 0);
+                touched = true;
+                __syncwarp();
+            }
+            if (masked && p.n_tok > 1) {  // rows that only some tokens see
+                const int t0 = max(0, lim_min - p0), n = (min(UPOS, p.kv_end - p0) - t0) * 8;
+                for (int h = 0; h < NB; h++)
+                    for (int i = lane; i < n; i += 32)
+                        slow |= not_finite8(reinterpret_cast<const uint4 *>(stage + (NB + h) * (UPOS * 128) + t0 * 128)[i]);
+                slow = __any_sync(0xffffffffu, slow);
+            }
+            if (!slow) {
+#pragma unroll
+                for (int t = 0; t < NT / 2; t++) {
+                    const uint32_t pa[4] = {pack_bf16(s[2 * t][0], s[2 * t][1]), pack_bf16(s[2 * t][2], s[2 * t][3]),
+                                            pack_bf16(s[2 * t + 1][0], s[2 * t + 1][1]),
+                                            pack_bf16(s[2 * t + 1][2], s[2 * t + 1][3])};
+                    const uint32_t row = vb + (t * 16 + (mi & 1) * 8 + l7) * 128;
+#pragma unroll
+                    for (int i = 0; i < OT / 2; i++) {
+                        const int c = 2 * i + (mi >> 1);
+                        uint32_t b[4];
+                        ldsm4_t(b, row + (c / 8) * (UPOS * 128) + (((c % 8) ^ l7) << 4));
+                        mma16816(o[2 * i], pa, b[0], b[1]);
+                        mma16816(o[2 * i + 1], pa, b[2], b[3]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+                    for (int e = 0; e < 8; e++) {
+                        const int from = (lane & ~3) | (e >> 1), t = i * 8 + e;
+                        const float w0 = __shfl_sync(0xffffffffu, e & 1 ? s[i][1] : s[i][0], from);
+                        const float w1 = __shfl_sync(0xffffffffu, e & 1 ? s[i][3] : s[i][2], from);
+                        const bool see0 = p0 + t < lim0 && p0 + t < p.kv_end, see1 = p0 + t < lim1 && p0 + t < p.kv_end;
+#pragma unroll
+                        for (int c = 0; c < OT; c++) {
+                            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(
+                                stage + (NB + c / 8) * (UPOS * 128) + t * 128 + (((c % 8) ^ (t & 7)) << 4) + 4 * tq));
+                            if (see0) {
+                                o[c][0] += w0 * v.x;
+                                o[c][1] += w0 * v.y;
+                            }
+                            if (see1) {
+                                o[c][2] += w1 * v.x;
+                                o[c][3] += w1 * v.y;
+                            }
+                        }
+                    }
+            }
+            if (touched) fence_proxy_async();  // the zeros, before the next TMA write of the stage
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[r.s]);
+        }
+        r.next();
+        p0 += UPOS;
+    } while (p0 < p.kv1);
+
+    // ---- merge the warps
+#pragma unroll
+    for (int off = 1; off < 4; off *= 2) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int row = g + 8 * i;
+        if (row < rows) {
+            float *dst = merge_o + (cw * SMALL_ROWS + row) * DP;
+#pragma unroll
+            for (int c = 0; c < OT; c++)
+                *reinterpret_cast<float2 *>(dst + ((c * 8 + 2 * tq) ^ (g * 8))) = make_float2(o[c][2 * i], o[c][2 * i + 1]);
+            if (tq == 0) merge_ml[cw * SMALL_ROWS + row] = i == 0 ? make_float2(m0, l0) : make_float2(m1, l1);
+        }
+    }
+    bar_sync(1, NW * 32);
+    const int tid = cw * 32 + lane;
+    for (int i = tid; i < rows * (DP / 4); i += NW * 32) {
+        const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+        float m = -INFINITY, l = 0.0f, acc[4] = {};
+#pragma unroll
+        for (int w = 0; w < NW; w++) m = fmaxf(m, merge_ml[w * SMALL_ROWS + row].x);
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float2 ml = merge_ml[w * SMALL_ROWS + row];
+            const float f = ex2(ml.x - base);
+            const float4 v = *reinterpret_cast<const float4 *>(merge_o + (w * SMALL_ROWS + row) * DP + (d ^ ((row & 7) * 8)));
+            l += f * ml.y;
+            acc[0] += f * v.x;
+            acc[1] += f * v.y;
+            acc[2] += f * v.z;
+            acc[3] += f * v.w;
+        }
+        if (p.part < 0) {
+            const float inv = p.pos0 + row / a.rep < 0 ? 0.0f : 1.0f / l;  // a row without positions is zero
+            if (d < a.head_dim) {
+                bf16 *dst = a.out + (p.tok0 + row / a.rep) * a.out_stride + (long long)(p.kvh * a.rep + row % a.rep) * a.head_dim + d;
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+            }
+        } else {
+            const size_t at = (size_t)p.part * SMALL_ROWS + row;
+            __stcg(reinterpret_cast<float4 *>(a.small_o + at * DP + d), make_float4(acc[0], acc[1], acc[2], acc[3]));
+            if (d == 0) __stcg(a.small_ml + at, make_float2(m, l));
+        }
+    }
+    if (p.part >= 0) {  // the item's last piece to finish adds the parts up, in their order
+        __threadfence();
+        bar_sync(1, NW * 32);
+        if (tid == 0) *flag_s = atomicAdd(a.counters + p.first, 1) == p.n_parts - 1;
+        bar_sync(1, NW * 32);
+        if (*flag_s) {
+            __threadfence();
+            for (int i = tid; i < rows * (DP / 4); i += NW * 32) {
+                const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+                float m = -INFINITY, l = 0.0f, acc[4] = {};
+                for (int w = 0; w < p.n_parts; w++)
+                    m = fmaxf(m, __ldcg(a.small_ml + (size_t)part_slot(p.first, w) * SMALL_ROWS + row).x);
+                const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll 4
+                for (int w = 0; w < p.n_parts; w++) {
+                    const size_t at = (size_t)part_slot(p.first, w) * SMALL_ROWS + row;
+                    const float2 ml = __ldcg(a.small_ml + at);
+                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.small_o + at * DP + d));
+                    const float f = ex2(ml.x - base);
+                    l += f * ml.y;
+                    acc[0] += f * v.x;
+                    acc[1] += f * v.y;
+                    acc[2] += f * v.z;
+                    acc[3] += f * v.w;
+                }
+                const float inv = p.pos0 + row / a.rep < 0 ? 0.0f : 1.0f / l;
+                if (d < a.head_dim) {
+                    bf16 *dst = a.out + (p.tok0 + row / a.rep) * a.out_stride + (long long)(p.kvh * a.rep + row % a.rep) * a.head_dim + d;
+                    *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+                }
+            }
+            if (tid == 0) a.counters[p.first] = 0;
+        }
+    }
+    bar_sync(1, NW * 32);  // the merge buffer is free again
+}
+
+// ---------------------------------------------------------------- kernel for few rows alone
+
+template <int DP>
+struct SmallSmem {
+    alignas(1024) unsigned char ring[SMALL_STAGES * STAGE];
+    float merge_o[SMALL_WARPS * SMALL_ROWS * DP];
+    float2 merge_ml[SMALL_WARPS * SMALL_ROWS];
+    uint64_t full[SMALL_STAGES], empty[SMALL_STAGES];
+    int flag;
+};
+
+template <int DP>
+__global__ void __launch_bounds__((1 + SMALL_WARPS) * 32, 1)
+    paged_small_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                       const __grid_constant__ PaArgs a) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    SmallSmem<DP> &sm = *reinterpret_cast<SmallSmem<DP> *>(align_shared<1024>(smem_raw));
+    const int warp = threadIdx.x / 32;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < SMALL_STAGES; i++) {
+            mbar_init(&sm.full[i], 1);
+            mbar_init(&sm.empty[i], 1);
+        }
+        fence_barrier_init();
+        prefetch_tmap(&mk);
+        prefetch_tmap(&mv);
+    }
+    __syncthreads();
+    pdl_trigger();
+    pdl_wait();
+    const int2 work = a.ctas[blockIdx.x];
+    if (work.y < 0) zero_rows(a);
+    Ring<SMALL_STAGES> r;
+    Waiter wait;
+    if (warp == SMALL_WARPS) {
+        for (int i = 0; i < work.y; i++)
+            small_produce<DP, SMALL_STAGES>(a, &mk, &mv, a.pieces[work.x + i], sm.ring, sm.full, sm.empty, r, wait);
+        // every load is waited for by a consumer before the CTA ends
+    } else {
+        for (int i = 0; i < work.y; i++)
+            small_consume<DP, SMALL_WARPS, SMALL_STAGES>(a, a.pieces[work.x + i], sm.ring, sm.full, sm.empty, r, wait, warp,
+                                                        sm.merge_o, sm.merge_ml, &sm.flag);
+    }
+}
+
+// ---------------------------------------------------------------- many rows
+
+// D[tmem] (+)= A[tmem] B[smem], bf16
+__device__ __forceinline__ void mma_bf16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+#define Q3_R16(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), \
+    "=r"(r[o + 6]), "=r"(r[o + 7]), "=r"(r[o + 8]), "=r"(r[o + 9]), "=r"(r[o + 10]), "=r"(r[o + 11]), \
+    "=r"(r[o + 12]), "=r"(r[o + 13]), "=r"(r[o + 14]), "=r"(r[o + 15])
+
+// 32 columns of this thread's tensor-memory lane
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : Q3_R16(r, 0), Q3_R16(r, 16)
+        : "r"(taddr)
+        : "memory");
+}
+#undef Q3_R16
+
+#define Q3_W16(r) "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), \
+    "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16};" ::"r"(taddr),
+        Q3_W16(r)
+        : "memory");
+}
+#undef Q3_W16
+
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int DP>
+struct MixedSmem {
+    static constexpr int NB = DP / 64;
+    union {
+        alignas(1024) unsigned char q[2 * NB * STAGE];            // two query tiles
+        float merge_o[MIXED_WARPS * SMALL_ROWS * DP];             // few rows: the warps' partial results
+    };
+    alignas(1024) unsigned char ring[MIXED_STAGES * STAGE];
+    float2 merge_ml[MIXED_WARPS * SMALL_ROWS];
+    uint64_t full[MIXED_STAGES], empty[MIXED_STAGES], q_full, q_empty, s_full[2], p_full[2], v_ready[2];
+    uint32_t tmem;
+    int flag;
+    int v_bad[2][4];  // by v_ready, per warp: the step's V holds a NaN or infinity that some row must not see
+};
+
+// Tensor memory: S (and P over it) of tile x at column 128 x, O at 256 + DP x.
+__device__ __forceinline__ uint32_t tmem_s(uint32_t base, int x) { return base + 128 * x; }
+template <int DP>
+__device__ __forceinline__ uint32_t tmem_o(uint32_t base, int x) {
+    return base + 256 + DP * x;
+}
+
+__device__ __forceinline__ int big_steps(const PagedPiece &p) { return max(1, (p.kv1 - p.kv0 + BIG_TILE - 1) / BIG_TILE); }
+
+// One warp loads a piece's queries, then K and V of each 128-position step.
+template <int DP>
+__device__ void big_produce(const PaArgs &a, const CUtensorMap *mq, const CUtensorMap *mk, const CUtensorMap *mv,
+                            const PagedPiece &p, MixedSmem<DP> &sm, Ring<MIXED_STAGES> &r, uint32_t &q_ph, Waiter &wait) {
+    constexpr int NB = DP / 64;
+    const int lane = threadIdx.x % 32, tiles = p.n_tok > a.tile_tok ? 2 : 1;
+    wait(&sm.q_empty, q_ph ^ 1);
+    q_ph ^= 1;
+    __syncwarp();
+    if (lane == 0) mbar_arrive_expect_tx(&sm.q_full, (uint32_t)(tiles * NB * a.tile_tok * a.rep * 128));
+    __syncwarp();
+    if (lane < tiles * NB)
+        tma_load_3d(sm.q + lane * STAGE, mq, lane % NB * 64, p.kvh * a.rep, p.tok0 + lane / NB * a.tile_tok, &sm.q_full);
+    const int box = a.big_box, nsub = BIG_TILE / box, sub = lane % nsub, half = lane / nsub;
+    const bool active = half < NB;
+    const int *tab = a.table + (size_t)p.seq * a.max_pages;
+    int at = p.kv0 + sub * box;
+    int page = active && at < p.kv1 ? __ldg(tab + at / a.page_size) : 0;
+    int p0 = p.kv0;
+    do {
+        const int ahead = at + BIG_TILE;
+        const int next_page = active && ahead < p.kv1 ? __ldg(tab + ahead / a.page_size) : 0;
+        const uint32_t bytes = (uint32_t)(min(nsub, max(0, (p.kv1 - p0 + box - 1) / box)) * box * 128);
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+#pragma unroll
+            for (int h = 0; h < NB; h++) {
+                wait(&sm.empty[r.s], r.ph ^ 1);
+                __syncwarp();
+                if (lane == 0) mbar_arrive_expect_tx(&sm.full[r.s], bytes);
+                __syncwarp();
+                if (active && half == h && at < p.kv1)
+                    tma_page(sm.ring + (size_t)r.s * STAGE + sub * box * 128, kv ? mv : mk, h * 64, at % a.page_size, p.kvh, page,
+                             &sm.full[r.s]);
+                r.next();
+            }
+        }
+        at = ahead;
+        page = next_page;
+        p0 += BIG_TILE;
+    } while (p0 < p.kv1);
+}
+
+// One thread issues the products. Per step and tile: O += P V of this step, then S = Q K^T of the next one
+// into the columns P was read from (the tensor core takes a CTA's products in order).
+template <int DP>
+__device__ void big_multiply(const PaArgs &a, const PagedPiece &p, MixedSmem<DP> &sm, uint32_t tmem,
+                             Ring<MIXED_STAGES> &r, uint32_t &q_ph, uint32_t &p_ph, int &n_masked, Waiter &wait) {
+    constexpr int NB = DP / 64;
+    const int tiles = p.n_tok > a.tile_tok ? 2 : 1, steps = big_steps(p), lim_min = first_masked(p);
+    const uint32_t qb = smem_u32(sm.q), ring = smem_u32(sm.ring);
+    auto scores = [&](int x, int k_stage) {
+#pragma unroll
+        for (int k = 0; k < DP / 16; k++)
+            mma_bf16(tmem_s(tmem, x), smem_desc_sw128(qb + (x * NB + k / 4) * STAGE + k % 4 * 32),
+                     smem_desc_sw128(ring + (k_stage + k / 4) * STAGE + k % 4 * 32), a.idesc_qk, k > 0);
+        mma_commit(&sm.s_full[x]);
+    };
+    auto wait_stages = [&](const Ring<MIXED_STAGES> &at) {  // a tile's halves never wrap: the ring is a multiple of NB
+        for (int h = 0; h < NB; h++) wait(&sm.full[at.s + h], at.ph);
+        tc_fence_after();
+    };
+    auto release = [&](const Ring<MIXED_STAGES> &at) {
+        for (int h = 0; h < NB; h++) mma_commit(&sm.empty[at.s + h]);
+    };
+    wait(&sm.q_full, q_ph);
+    q_ph ^= 1;
+    wait_stages(r);
+    for (int x = 0; x < tiles; x++) scores(x, r.s);
+    release(r);
+    if (steps == 1) mma_commit(&sm.q_empty);
+    r.next(NB);
+    for (int j = 0; j < steps; j++) {
+        const Ring<MIXED_STAGES> rv = r;
+        r.next(NB);
+        const Ring<MIXED_STAGES> rk = r;  // the next step's K
+        const bool more = j + 1 < steps;
+        if (more) r.next(NB);
+        wait_stages(rv);
+        bool slow = false;
+        if (p.kv0 + (j + 1) * BIG_TILE > lim_min) {
+            const int b = n_masked & 1;
+            wait(&sm.v_ready[b], n_masked >> 1 & 1);
+            n_masked++;
+            const volatile int *bad = sm.v_bad[b];
+            slow = bad[0] | bad[1] | bad[2] | bad[3];
+        }
+        for (int x = 0; x < tiles; x++) {
+            wait(&sm.p_full[x], p_ph >> x & 1);
+            p_ph ^= 1u << x;
+            tc_fence_after();
+            if (!slow) {
+#pragma unroll
+                for (int k = 0; k < BIG_TILE / 16; k++)
+                    mma_bf16_ta(tmem_o<DP>(tmem, x), tmem_s(tmem, x) + k * 8,
+                                smem_desc_sw128(ring + rv.s * STAGE + k * 2048, STAGE, 1024), a.idesc_pv, j > 0 || k > 0);
+            }
+            if (more) {
+                if (x == 0) wait_stages(rk);
+                scores(x, rk.s);
+            } else {
+                mma_commit(&sm.s_full[x]);  // the tile's last product
+            }
+        }
+        release(rv);
+        if (more) release(rk);
+        if (j + 2 == steps) mma_commit(&sm.q_empty);
+    }
+}
+
+// A warpgroup per tile, a thread per row.
+template <int DP>
+__device__ void big_softmax(const PaArgs &a, const PagedPiece &p, MixedSmem<DP> &sm, uint32_t tmem, int x,
+                            Ring<MIXED_STAGES> &r, uint32_t &s_ph, int &n_masked, Waiter &wait) {
+    constexpr int NB = DP / 64;
+    const int steps = big_steps(p), lim_min = first_masked(p);
+    if (x == 1 && p.n_tok <= a.tile_tok) {  // this tile is empty
+        r.next(2 * NB * steps % MIXED_STAGES);
+        // keep the phase: 2 * NB * steps stages are passed in whole laps, too
+        if (2 * NB * steps / MIXED_STAGES & 1) r.ph ^= 1;
+        for (int j = 0; j < steps; j++) n_masked += p.kv0 + (j + 1) * BIG_TILE > lim_min;
+        return;
+    }
+    const int quarter = threadIdx.x / 32 % 4, lane = threadIdx.x % 32, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t ts = tmem_s(tmem, x) + lanes, to = tmem_o<DP>(tmem, x) + lanes;
+    const int tt = x * a.tile_tok + row / a.rep, lim = p.pos0 + tt + 1;
+    // a negative scale negates Q in the first product; a zero one must still leave masked scores at -infinity
+    const float c = fmaxf(fabsf(a.scale_log2), 1e-30f);
+    float m = -INFINITY, l = 0.0f;
+    for (int j = 0; j < steps; j++) {
+        r.next(NB);
+        const Ring<MIXED_STAGES> rv = r;
+        r.next(NB);
+        const int t0 = p.kv0 + j * BIG_TILE;
+        const bool masked = t0 + BIG_TILE > lim_min;
+        wait(&sm.s_full[x], s_ph);
+        s_ph ^= 1;
+        __syncwarp();
+        tc_fence_after();
+        uint32_t su[128];
+#pragma unroll
+        for (int i = 0; i < 4; i++) tmem_ld32(ts + 32 * i, su + 32 * i);
+        bool slow = false;
+        if (masked) {
+            const int b = n_masked & 1;
+            if (x == 0) {  // V past the item's end becomes zero; rows only some tokens see are checked
+                for (int h = 0; h < NB; h++) wait(&sm.full[rv.s + h], rv.ph);
+                __syncwarp();
+                bool bad = false;
+                unsigned char *v = sm.ring + (size_t)rv.s * STAGE;
+                const int end = min(BIG_TILE, p.kv_end - t0), check = max(0, lim_min - t0);
+                for (int i = row; i < NB * 128 * 8; i += 128) {
+                    uint4 *chunk = reinterpret_cast<uint4 *>(v) + i;
+                    const int t = i / 8 % 128;
+                    if (t >= end) *chunk = make_uint4(0, 0, 0, 0);
+                    else if (t >= check) bad |= not_finite8(*chunk);
+                }
+                fence_proxy_async();
+                bad = __any_sync(0xffffffffu, bad);
+                if (lane == 0) {
+                    sm.v_bad[b][quarter] = bad;
+                    mbar_arrive(&sm.v_ready[b]);
+                }
+            }
+            wait(&sm.v_ready[b], n_masked >> 1 & 1);
+            __syncwarp();
+            n_masked++;
+            const volatile int *flags = sm.v_bad[b];
+            slow = flags[0] | flags[1] | flags[2] | flags[3];
+        }
+        tmem_wait_ld();
+        float s[128];
+#pragma unroll
+        for (int i = 0; i < 128; i++) s[i] = __uint_as_float(su[i]);
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < 128; i++)
+                if (t0 + i >= lim) s[i] = -INFINITY;
+        }
+        float x0 = fmaxf(s[0], s[1]), x1 = fmaxf(s[2], s[3]);
+#pragma unroll
+        for (int i = 4; i < 128; i += 4) {
+            x0 = fmaxf(x0, fmaxf(s[i], s[i + 1]));
+            x1 = fmaxf(x1, fmaxf(s[i + 2], s[i + 3]));
+        }
+        const float top = fmaxf(x0, x1) * c;
+        const bool grow = top > m + GROW || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, grow)) {
+            const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
+            if (grow) m = top;
+            l *= f;
+            if (j > 0) {  // the previous product has finished: s_full was committed after it
+                for (int i = 0; i < DP / 16; i++) {
+                    uint32_t o[16];
+                    tmem_ld8(to + 16 * i, reinterpret_cast<float *>(o));
+                    tmem_ld8(to + 16 * i + 8, reinterpret_cast<float *>(o) + 8);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    tmem_st16(to + 16 * i, o);
+                }
+                tmem_wait_st();
+            }
+        }
+        const float base = m == -INFINITY ? 0.0f : -m;
+        if (!slow) {
+            float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const float a0 = ex2(__fmaf_rn(s[32 * i + 2 * e], c, base));
+                    const float a1 = ex2(__fmaf_rn(s[32 * i + 2 * e + 1], c, base));
+                    sum0 += a0;
+                    sum1 += a1;
+                    pk[e] = pack_bf16(a0, a1);
+                }
+                tmem_st16(ts + 16 * i, pk);
+            }
+            l += sum0 + sum1;
+            tmem_wait_st();
+        } else {
+            // on the CUDA cores, 16 columns of O at a time, over the positions this row sees
+            const unsigned char *v = sm.ring + (size_t)rv.s * STAGE;
+            for (int d = 0; d < DP / 16; d++) {
+                float acc[16];
+                if (j > 0) {
+                    tmem_ld8(to + 16 * d, acc);
+                    tmem_ld8(to + 16 * d + 8, acc + 8);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) acc[e] = 0.0f;
+                }
+                for (int t8 = 0; t8 < BIG_TILE; t8 += 8) {
+                    float sc[8];
+                    __syncwarp();
+                    tmem_ld8(ts + t8, sc);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int t = t8 + e;
+                        if (t0 + t >= lim || t0 + t >= p.kv_end) continue;
+                        const float w = ex2(__fmaf_rn(sc[e], c, base));
+                        if (d == 0) l += w;
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint4 u = *reinterpret_cast<const uint4 *>(v + d / 4 * STAGE + t * 128 + (((d % 4 * 2 + h) ^ (t & 7)) << 4));
+                            const __nv_bfloat162 *w2 = reinterpret_cast<const __nv_bfloat162 *>(&u);
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const float2 vv = __bfloat1622float2(w2[q]);
+                                acc[8 * h + 2 * q] += w * vv.x;
+                                acc[8 * h + 2 * q + 1] += w * vv.y;
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+                tmem_st16(to + 16 * d, reinterpret_cast<const uint32_t *>(acc));
+            }
+            tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[x]);
+    }
+    wait(&sm.s_full[x], s_ph);
+    s_ph ^= 1;
+    __syncwarp();
+    tc_fence_after();
+    const bool valid = row / a.rep < a.tile_tok && tt < p.n_tok;
+    const int head = p.kvh * a.rep + row % a.rep;
+    if (p.part < 0) {
+        const float inv = lim <= 0 ? 0.0f : 1.0f / l;
+        bf16 *dst = a.out + (p.tok0 + tt) * a.out_stride + (long long)head * a.head_dim;
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++) {
+            uint32_t o[32];
+            tmem_ld32(to + 32 * i, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                uint32_t w[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const float lo = __uint_as_float(o[8 * e + 2 * q]), hi = __uint_as_float(o[8 * e + 2 * q + 1]);
+                    w[q] = pack_bf16(lo * inv, hi * inv);
+                }
+                const int d = 32 * i + 8 * e;
+                if (valid && d < a.head_dim)
+                    *reinterpret_cast<uint4 *>(dst + d) = lim <= 0 ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    } else {
+        const size_t at = (size_t)p.part * (2 * BIG_TILE) + x * BIG_TILE + row;
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++) {
+            uint32_t o[32];
+            tmem_ld32(to + 32 * i, o);
+            tmem_wait_ld();
+            if (valid) {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    __stcg(reinterpret_cast<uint4 *>(a.big_o + at * DP + 32 * i) + e, make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
+            }
+        }
+        if (valid) __stcg(a.big_ml + at, make_float2(m, l));
+    }
+    tc_fence_before();
+}
+
+template <int DP>
+__global__ void __launch_bounds__((4 + MIXED_WARPS) * 32, 1)
+    paged_mixed_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk_small,
+                       const __grid_constant__ CUtensorMap mv_small, const __grid_constant__ CUtensorMap mk_big,
+                       const __grid_constant__ CUtensorMap mv_big, const __grid_constant__ PaArgs a) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    MixedSmem<DP> &sm = *reinterpret_cast<MixedSmem<DP> *>(align_shared<1024>(smem_raw));
+    const int warp = threadIdx.x / 32;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < MIXED_STAGES; i++) {
+            mbar_init(&sm.full[i], 1);
+            mbar_init(&sm.empty[i], 1);
+        }
+        mbar_init(&sm.q_full, 1);
+        mbar_init(&sm.q_empty, 1);
+        for (int x = 0; x < 2; x++) {
+            mbar_init(&sm.s_full[x], 1);
+            mbar_init(&sm.p_full[x], 4);
+            mbar_init(&sm.v_ready[x], 4);
+        }
+        fence_barrier_init();
+        prefetch_tmap(&mq);
+        prefetch_tmap(&mk_small);
+        prefetch_tmap(&mv_small);
+        prefetch_tmap(&mk_big);
+        prefetch_tmap(&mv_big);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    // after the allocation: a dependent kernel's CTA that took this SM's tensor memory first would wait for this
+    // kernel while this CTA waits for its memory
+    pdl_trigger();
+    pdl_wait();
+    const int2 work = a.ctas[blockIdx.x];
+    if (work.y < 0) zero_rows(a);
+    Ring<MIXED_STAGES> r;
+    Waiter wait;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        uint32_t q_ph = 0, p_ph = 0;
+        int n_masked = 0;
+        for (int i = 0; i < work.y && warp < 2; i++) {
+            const PagedPiece p = a.pieces[work.x + i];
+            if (warp == 0) {
+                if (p.big) big_produce<DP>(a, &mq, &mk_big, &mv_big, p, sm, r, q_ph, wait);
+                else small_produce<DP, MIXED_STAGES>(a, &mk_small, &mv_small, p, sm.ring, sm.full, sm.empty, r, wait);
+            } else if (p.big) {
+                if (threadIdx.x % 32 == 0) big_multiply<DP>(a, p, sm, tmem, r, q_ph, p_ph, n_masked, wait);
+                __syncwarp();
+            }
+        }
+        if (warp == 0) {  // the products' release of the ring arrives asynchronously: before the CTA ends
+            for (int i = 0; i < MIXED_STAGES; i++) {
+                wait(&sm.empty[r.s], r.ph ^ 1);
+                r.next();
+            }
+            wait(&sm.q_empty, q_ph ^ 1);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const int x = warp >= 8;
+        uint32_t s_ph = 0;
+        int n_masked = 0;
+        bool big = false;
+        for (int i = 0; i < work.y; i++) {
+            const PagedPiece p = a.pieces[work.x + i];
+            // from the last big piece to the small ones together: a warpgroup whose tile was empty came here early, while
+            // the ring and the queries, whose memory the merge uses, still belonged to the big piece
+            if (big && !p.big) bar_sync(1, MIXED_WARPS * 32);
+            big = p.big;
+            if (p.big) big_softmax<DP>(a, p, sm, tmem, x, r, s_ph, n_masked, wait);
+            else small_consume<DP, MIXED_WARPS, MIXED_STAGES>(a, p, sm.ring, sm.full, sm.empty, r, wait, warp - 4, sm.merge_o,
+                                                            sm.merge_ml, &sm.flag);
+        }
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// Adds up the parts of the big items that were cut: a CTA per (item, 32 rows), a warp per row.
+template <int DP>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ PaArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const PagedPiece p = a.splits[blockIdx.x];
+    if (p.n_parts < 2) return;
+    const int lane = threadIdx.x % 32, d = lane * (DP / 32);
+    for (int i = 0; i < 4; i++) {
+        const int row = blockIdx.y * 32 + i * 8 + threadIdx.x / 32, x = row / BIG_TILE, rr = row % BIG_TILE;
+        const int tt = x * a.tile_tok + rr / a.rep;
+        if (rr / a.rep >= a.tile_tok || tt >= p.n_tok) continue;
+        float m = -INFINITY, l = 0.0f, acc[DP / 32] = {};
+        for (int w = 0; w < p.n_parts; w++)
+            m = fmaxf(m, __ldcg(a.big_ml + (size_t)part_slot(p.first, w) * (2 * BIG_TILE) + row).x);
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll 4
+        for (int w = 0; w < p.n_parts; w++) {
+            const size_t at = (size_t)part_slot(p.first, w) * (2 * BIG_TILE) + row;
+            const float2 ml = __ldcg(a.big_ml + at);
+            const float f = ex2(ml.x - base);
+            l += f * ml.y;
+#pragma unroll
+            for (int e = 0; e < DP / 32; e += 2) {
+                const float2 v = __ldcg(reinterpret_cast<const float2 *>(a.big_o + at * DP + d + e));
+                acc[e] += f * v.x;
+                acc[e + 1] += f * v.y;
+            }
+        }
+        const float inv = 1.0f / l;
+        bf16 *dst = a.out + (p.tok0 + tt) * a.out_stride + (long long)(p.kvh * a.rep + rr % a.rep) * a.head_dim + d;
+#pragma unroll
+        for (int e = 0; e < DP / 32; e += 2)
+            if (d + e < a.head_dim)
+                *reinterpret_cast<uint32_t *>(dst + e) = p.pos0 + tt < 0 ? 0u : pack_bf16(acc[e] * inv, acc[e + 1] * inv);
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+// K or V pages as a 4-D map (column, slot, kv head, page) with a box of `rows` slots of 64 columns.
+bool make_page_map(CUtensorMap *map, const void *base, const PagedAttnCall &c, int rows) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)c.shape.head_dim, (cuuint64_t)c.shape.page_size, (cuuint64_t)c.shape.n_kv_heads,
+                                (cuuint64_t)c.shape.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.cache.pos_stride * 2, (cuuint64_t)c.cache.head_stride * 2,
+                                   (cuuint64_t)c.cache.page_stride * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Query rows as a 3-D map (column, head, token): a box is all heads of a kv head for a tile's tokens.
+bool make_query_map(CUtensorMap *map, const PagedAttnCall &c, const PaArgs &a) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)c.shape.head_dim, (cuuint64_t)c.shape.n_heads, (cuuint64_t)c.shape.n_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)c.shape.head_dim * 2, (cuuint64_t)c.q_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)a.rep, (cuuint32_t)a.tile_tok}, estr[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16 *>(c.q), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DP>
+int run(const PagedAttnCall &c, PaArgs &a, cudaStream_t s) {
+    CUtensorMap mk, mv;
+    a.small_box = std::min(a.small_box, 32 * 128 / DP);
+    if (!make_page_map(&mk, c.cache.key_pages, c, a.small_box) || !make_page_map(&mv, c.cache.value_pages, c, a.small_box))
+        return Q3_ERR_SHAPE;
+    if (!paged_has_big(c.shape)) {
+        const size_t smem = sizeof(SmallSmem<DP>) + 1024;
+        Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_small_kernel<DP>), smem));
+        Q3_TRY_LAUNCH(launch(paged_small_kernel<DP>, dim3(paged_ctas()), dim3((1 + SMALL_WARPS) * 32), smem, s, 1, mk, mv, a));
+        return Q3_OK;
+    }
+    CUtensorMap mq, mk_big, mv_big;
+    if (!make_page_map(&mk_big, c.cache.key_pages, c, a.big_box) || !make_page_map(&mv_big, c.cache.value_pages, c, a.big_box) ||
+        !make_query_map(&mq, c, a))
+        return Q3_ERR_SHAPE;
+    // f32 accumulator, bf16 operands; second product: B = V with its columns contiguous
+    const uint32_t kinds = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BIG_TILE >> 4) << 24);
+    a.idesc_qk = kinds | ((uint32_t)(BIG_TILE >> 3) << 17) | (c.scale < 0.0f ? 1u << 13 : 0u);
+    a.idesc_pv = kinds | ((uint32_t)(DP >> 3) << 17) | (1u << 16);
+    const size_t smem = sizeof(MixedSmem<DP>) + 1024;
+    Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_mixed_kernel<DP>), smem));
+    Q3_TRY_LAUNCH(launch(paged_mixed_kernel<DP>, dim3(paged_ctas()), dim3((4 + MIXED_WARPS) * 32), smem, s, 1, mq, mk, mv,
+                         mk_big, mv_big, a));
+    Q3_TRY_LAUNCH(launch(paged_combine_kernel<DP>, dim3(paged_ctas(), 2 * BIG_TILE / 32), dim3(256), 0, s, 1, a));
+    return Q3_OK;
+}
+
+}  // namespace
+
+unsigned take_error_paged_attn() {
+    unsigned v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_dev_error, sizeof(v)) != cudaSuccess) return 0;
+    if (v) cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(zero));
+    return v;
+}
+
+int paged_attention(const PagedAttnCall &c, cudaStream_t s) {
+    const PagedPlanLayout l = paged_plan_layout(c.shape);
+    const PagedScratchLayout x = paged_scratch_layout(c.shape);
+    PaArgs a = {};
+    a.out = c.out;
+    a.q = c.q;
+    a.out_stride = c.out_stride;
+    a.q_stride = c.q_stride;
+    a.table = reinterpret_cast<const int *>(c.plan + l.table);
+    a.ctas = reinterpret_cast<const int2 *>(c.plan + l.ctas);
+    a.pieces = reinterpret_cast<const PagedPiece *>(c.plan + l.pieces);
+    a.splits = reinterpret_cast<const PagedPiece *>(c.plan + l.splits);
+    a.counters = reinterpret_cast<int *>(c.plan + l.counters);
+    a.small_o = reinterpret_cast<float *>(c.scratch + x.small_o);
+    a.small_ml = reinterpret_cast<float2 *>(c.scratch + x.small_ml);
+    a.big_o = reinterpret_cast<float *>(c.scratch + x.big_o);
+    a.big_ml = reinterpret_cast<float2 *>(c.scratch + x.big_ml);
+    a.rep = c.shape.n_heads / c.shape.n_kv_heads;
+    a.tile_tok = BIG_TILE / a.rep;
+    a.head_dim = c.shape.head_dim;
+    a.page_size = c.shape.page_size;
+    a.max_pages = c.shape.max_pages;
+    a.n_tokens = c.shape.n_tokens;
+    a.row_elems = c.shape.n_heads * c.shape.head_dim;
+    a.small_box = a.big_box = std::min(c.shape.page_size & -c.shape.page_size, BIG_TILE);
+    a.scale_log2 = c.scale * 1.4426950408889634f;
+    return a.head_dim <= 64 ? run<64>(c, a, s) : run<128>(c, a, s);
+}
+
+}  // namespace q3
