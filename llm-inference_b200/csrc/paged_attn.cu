@@ -37,8 +37,6 @@ namespace {
 __device__ unsigned g_dev_error;
 
 constexpr int STAGE = 16384;        // bytes of a ring stage
-constexpr int SMALL_STAGES = 12;    // few-row kernel: 4 consumer warps
-constexpr int SMALL_WARPS = 4;
 constexpr int MIXED_STAGES = 10;    // kernel for both kinds: two softmax warpgroups
 constexpr int MIXED_WARPS = 8;
 constexpr float GROW = 8.0f;        // many rows: the reference follows the maximum in steps of 2^8
@@ -55,6 +53,7 @@ struct PaArgs {
     float2 *small_ml, *big_ml;
     int rep, tile_tok, head_dim, page_size, max_pages, n_tokens, row_elems;
     int small_box, big_box;  // rows of a TMA box: the largest power of two that divides a page, at most a step
+    int small_step_pages, small_step_slots, big_step_pages, big_step_slots;  // a producer's step in pages and slots
     float scale_log2;
     uint32_t idesc_qk, idesc_pv;
 };
@@ -80,6 +79,10 @@ struct Ring {
             s -= N;
             ph ^= 1;
         }
+    }
+    __device__ __forceinline__ void advance(int by) {  // any number of stages
+        next(by % N);
+        ph ^= by / N & 1;
     }
 };
 
@@ -131,6 +134,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return r;
 }
 
+// the 8 x 8 matrix of 16-bit values that a warp holds as a fragment, transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // one of two packed bf16 is NaN or infinite
 __device__ __forceinline__ bool not_finite2(uint32_t w) {
     return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
@@ -155,67 +165,104 @@ __device__ __forceinline__ int first_masked(const PagedPiece &p) { return p.pos0
 
 // ---------------------------------------------------------------- few rows: producer
 
-// One warp streams a piece's steps: K and V of UPOS positions, NB = DP / 64 halves of 64 columns each, in the
-// 128-byte swizzle. Each lane issues one box and looks up the next step's page while this one waits for room.
-template <int DP, int NST>
+// A position's page-table index and slot, stepped without dividing.
+struct PageWalk {
+    int idx, slot;
+    __device__ __forceinline__ PageWalk(int at, int page_size) : idx(at / page_size), slot(at % page_size) {}
+    __device__ __forceinline__ void step(int pages, int slots, int page_size) {
+        idx += pages;
+        slot += slots;
+        if (slot >= page_size) {
+            slot -= page_size;
+            idx++;
+        }
+    }
+};
+
+// NP warps stream a piece's steps: K and V of UPOS positions, NB = DP / 64 halves of 64 columns each, in the
+// 128-byte swizzle. A warp fills every NP-th stage; each lane issues one box and looks up its page of the
+// warp's next step before this one waits for room. The loop's length bounds the kernel: with one
+// warp that divided by the page size it took 1360 cycles a stage, half of the time at which HBM delivers.
+template <int DP, int NST, int NP>
 __device__ void small_produce(const PaArgs &a, const CUtensorMap *mk, const CUtensorMap *mv, const PagedPiece &p,
-                              unsigned char *ring, uint64_t *full, uint64_t *empty, Ring<NST> &r, Waiter &wait) {
+                              unsigned char *ring, uint64_t *full, uint64_t *empty, Ring<NST> &r, int pid, Waiter &wait) {
     constexpr int NB = DP / 64, UPOS = 32 * 128 / DP;
+    static_assert(NST % NP == 0, "a stage belongs to one producer");
     const int lane = threadIdx.x % 32, box = a.small_box, nsub = UPOS / box;
     const int sub = lane % nsub, part = lane / nsub, half = part % NB;
     const bool active = part < 2 * NB, is_v = part >= NB;
     const int *tab = a.table + (size_t)p.seq * a.max_pages;
     const uint32_t off = (is_v ? NB : 0) * (UPOS * 128) + half * (UPOS * 128) + sub * box * 128;
-    int at = p.kv0 + sub * box;
-    int page = active && at < p.kv1 ? __ldg(tab + at / a.page_size) : 0;
-    int p0 = p.kv0;
-    do {
-        const int ahead = at + UPOS;
-        const int next_page = active && ahead < p.kv1 ? __ldg(tab + ahead / a.page_size) : 0;
-        wait(&empty[r.s], r.ph ^ 1);
+    const CUtensorMap *map = is_v ? mv : mk;
+    const int skip = (pid - r.s % NP + NP) % NP;  // steps of this piece before this warp's first
+    const int units = max(1, (p.kv1 - p.kv0 + UPOS - 1) / UPOS);
+    int at = p.kv0 + skip * UPOS + sub * box, p0 = p.kv0 + skip * UPOS;
+    PageWalk w(at, a.page_size);
+    Ring<NST> mine = r;
+    mine.next(skip);
+    int page = active && at < p.kv1 ? __ldg(tab + w.idx) : 0, slot = w.slot;
+    for (int u = skip; u < units; u += NP) {
+        w.step(a.small_step_pages, a.small_step_slots, a.page_size);
+        const bool on = active && at < p.kv1;
+        at += NP * UPOS;
+        const int next_page = active && at < p.kv1 ? __ldg(tab + w.idx) : 0;
+        wait(&empty[mine.s], mine.ph ^ 1);
         __syncwarp();
         if (lane == 0) {
-            const int n = min(nsub, max(0, (p.kv1 - p0 + box - 1) / box));
-            mbar_arrive_expect_tx(&full[r.s], (uint32_t)(n * box * 128 * NB * 2));
+            const int n = min(UPOS, max(0, p.kv1 - p0) + box - 1) & -box;
+            mbar_arrive_expect_tx(&full[mine.s], (uint32_t)(n * 128 * NB * 2));
         }
         __syncwarp();
-        if (active && at < p.kv1)
-            tma_page(ring + (size_t)r.s * STAGE + off, is_v ? mv : mk, half * 64, at % a.page_size, p.kvh, page, &full[r.s]);
-        r.next();
-        at = ahead;
+        if (on) tma_page(ring + (size_t)mine.s * STAGE + off, map, half * 64, slot, p.kvh, page, &full[mine.s]);
+        mine.next(NP);
+        p0 += NP * UPOS;
         page = next_page;
-        p0 += UPOS;
-    } while (p0 < p.kv1);
+        slot = w.slot;
+    }
+    r.advance(units);
 }
 
 // ---------------------------------------------------------------- few rows: consumers
 
-// merge buffer: [NW][16][DP] fp32 (columns rotated by row, so that a fragment's rows fall in
-// different banks), then [NW][16] (m, l).
-template <int DP, int NW, int NST>
+// The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that positions and head columns fill the
+// instruction's 16 rows and query rows its 8 columns: NQ = 1 for up to 8 rows, 2 for 16. Against queries as
+// the 16 rows (most of them padding at 4 query heads per kv head) this halves products, exponentials
+// and accumulators; P^T moves from accumulator to operand layout by an 8 x 8 transpose in registers.
+// merge buffer: [NW][8 NQ][DP] fp32 (columns permuted by row against bank conflicts), then (m, l).
+template <int DP, int NW, int NST, int NQ>
 __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned char *ring, uint64_t *full,
                               uint64_t *empty, Ring<NST> &r, Waiter &wait, int cw, float *merge_o, float2 *merge_ml,
                               int *flag_s) {
-    constexpr int NB = DP / 64, UPOS = 32 * 128 / DP, NT = UPOS / 8, KS = DP / 16, OT = DP / 8;
-    const int lane = threadIdx.x % 32, g = lane / 4, tq = lane % 4;
+    constexpr int NB = DP / 64, UPOS = 32 * 128 / DP, MT = UPOS / 16, KS = DP / 16, ROWS = 8 * NQ;
+    const int lane = threadIdx.x % 32, g = lane / 4, tq = lane % 4, l7 = lane % 8, mi = lane / 8;
     const int rows = p.n_tok * a.rep;
-    uint32_t qa[KS][4];
+    uint32_t qb[NQ][KS][2];
+    int lim[NQ][2];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int row = g + 8 * i;
+    for (int n = 0; n < NQ; n++) {
+        const int row = 8 * n + g;
         const bf16 *src = a.q + (p.tok0 + row / a.rep) * a.q_stride + (long long)(p.kvh * a.rep + row % a.rep) * a.head_dim;
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int col = 16 * k + 8 * j + 2 * tq;
-                qa[k][2 * j + i] = row < rows && col < a.head_dim ? *reinterpret_cast<const uint32_t *>(src + col) : 0u;
+                qb[n][k][j] = row < rows && col < a.head_dim ? *reinterpret_cast<const uint32_t *>(src + col) : 0u;
             }
-    }
-    const int lim0 = p.pos0 + g / a.rep + 1, lim1 = p.pos0 + (g + 8) / a.rep + 1, lim_min = first_masked(p);
-    float o[OT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
-    for (int i = 0; i < OT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        for (int e = 0; e < 2; e++) lim[n][e] = p.pos0 + (8 * n + 2 * tq + e) / a.rep + 1;
+    }
+    const int lim_min = first_masked(p);
+    float o[NQ][KS][4], m[NQ][2], l[NQ][2];  // o: columns 16 i + g and + 8 of rows 2 tq, 2 tq + 1
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+#pragma unroll
+        for (int i = 0; i < KS; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.0f;
+    }
+    // ldmatrix rows of this lane: K as [position][column] (operand rows = positions), V transposed
+    const uint32_t k_row = ((mi & 1) * 8 + l7) * 128, v_row = ((mi >> 1) * 8 + l7) * 128;
 
     int p0 = p.kv0;
     do {
@@ -224,69 +271,63 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
             const uint32_t kb = smem_u32(stage), vb = kb + NB * UPOS * 128;
             wait(&full[r.s], r.ph);
             __syncwarp();
-            float s[NT][4];
+            float s[NQ][MT][4];
 #pragma unroll
-            for (int i = 0; i < NT; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
-            const int mi = lane / 8, l7 = lane % 8;
+            for (int n = 0; n < NQ; n++)
+#pragma unroll
+                for (int i = 0; i < MT; i++) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                const int c = 2 * k + (mi & 1);
-                const uint32_t col = (c / 8) * (UPOS * 128) + (((c % 8) ^ l7) << 4);
+                const int c = 2 * k + (mi >> 1);
+                const uint32_t at = kb + k_row + (k / 4) * (UPOS * 128) + (((c % 8) ^ l7) << 4);
 #pragma unroll
-                for (int t = 0; t < NT / 2; t++) {
-                    uint32_t b[4];
-                    ldsm4(b, kb + col + (t * 16 + (mi >> 1) * 8 + l7) * 128);
-                    mma16816(s[2 * t], qa[k], b[0], b[1]);
-                    mma16816(s[2 * t + 1], qa[k], b[2], b[3]);
+                for (int i = 0; i < MT; i++) {
+                    uint32_t ka[4];
+                    ldsm4(ka, at + i * 16 * 128);
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) mma16816(s[n][i], ka, qb[n][k][0], qb[n][k][1]);
                 }
             }
             const bool masked = p0 + UPOS > lim_min;
-            float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < NT; i++)
+            for (int n = 0; n < NQ; n++) {
+                float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    float &u = s[i][j], &w = s[i][2 + j];
-                    u *= a.scale_log2;
-                    w *= a.scale_log2;
-                    if (masked) {
-                        const int t = p0 + i * 8 + 2 * tq + j;
-                        if (t >= lim0) u = -INFINITY;
-                        if (t >= lim1) w = -INFINITY;
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        s[n][i][j] *= a.scale_log2;
+                        if (masked && p0 + 16 * i + 8 * (j >> 1) + g >= lim[n][j & 1]) s[n][i][j] = -INFINITY;
+                        x[j & 1] = fmaxf(x[j & 1], s[n][i][j]);
                     }
-                    x0 = fmaxf(x0, u);
-                    x1 = fmaxf(x1, w);
-                }
 #pragma unroll
-            for (int off = 1; off < 4; off *= 2) {
-                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
-                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
+                for (int off = 4; off < 32; off *= 2) {
+                    x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], off));
+                    x[1] = fmaxf(x[1], __shfl_xor_sync(0xffffffffu, x[1], off));
+                }
+                if (__any_sync(0xffffffffu, x[0] > m[n][0] || x[1] > m[n][1])) {
+                    float f[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float top = fmaxf(m[n][e], x[e]);
+                        f[e] = top == -INFINITY ? 1.0f : ex2(m[n][e] - top);
+                        m[n][e] = top;
+                        l[n][e] *= f[e];
+                    }
+#pragma unroll
+                    for (int i = 0; i < KS; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) o[n][i][j] *= f[j & 1];
+                }
+                const float base[2] = {m[n][0] == -INFINITY ? 0.0f : m[n][0], m[n][1] == -INFINITY ? 0.0f : m[n][1]};
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        s[n][i][j] = ex2(s[n][i][j] - base[j & 1]);
+                        l[n][j & 1] += s[n][i][j];
+                    }
             }
-            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
-                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-                const float f0 = n0 == -INFINITY ? 1.0f : ex2(m0 - n0), f1 = n1 == -INFINITY ? 1.0f : ex2(m1 - n1);
-                m0 = n0;
-                m1 = n1;
-                l0 *= f0;
-                l1 *= f1;
-#pragma unroll
-                for (int i = 0; i < OT; i++) {
-                    o[i][0] *= f0;
-                    o[i][1] *= f0;
-                    o[i][2] *= f1;
-                    o[i][3] *= f1;
-                }
-            }
-            const float base0 = m0 == -INFINITY ? 0.0f : m0, base1 = m1 == -INFINITY ? 0.0f : m1;
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    s[i][j] = ex2(s[i][j] - base0);
-                    s[i][2 + j] = ex2(s[i][2 + j] - base1);
-                    l0 += s[i][j];
-                    l1 += s[i][2 + j];
-                }
             bool touched = false, slow = false;
             if (p0 + UPOS > p.kv_end) {  // rows past the item's end: zero
                 const int t0 = max(0, p.kv_end - p0), n = (UPOS - t0) * 8;
@@ -305,44 +346,53 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
             }
             if (!slow) {
 #pragma unroll
-                for (int t = 0; t < NT / 2; t++) {
-                    const uint32_t pa[4] = {pack_bf16(s[2 * t][0], s[2 * t][1]), pack_bf16(s[2 * t][2], s[2 * t][3]),
-                                            pack_bf16(s[2 * t + 1][0], s[2 * t + 1][1]),
-                                            pack_bf16(s[2 * t + 1][2], s[2 * t + 1][3])};
-                    const uint32_t row = vb + (t * 16 + (mi & 1) * 8 + l7) * 128;
+                for (int t = 0; t < MT; t++) {
+                    uint32_t pb[NQ][2];
 #pragma unroll
-                    for (int i = 0; i < OT / 2; i++) {
-                        const int c = 2 * i + (mi >> 1);
-                        uint32_t b[4];
-                        ldsm4_t(b, row + (c / 8) * (UPOS * 128) + (((c % 8) ^ l7) << 4));
-                        mma16816(o[2 * i], pa, b[0], b[1]);
-                        mma16816(o[2 * i + 1], pa, b[2], b[3]);
+                    for (int n = 0; n < NQ; n++) {
+                        pb[n][0] = transpose8(pack_bf16(s[n][t][0], s[n][t][1]));
+                        pb[n][1] = transpose8(pack_bf16(s[n][t][2], s[n][t][3]));
+                    }
+#pragma unroll
+                    for (int i = 0; i < KS; i++) {
+                        const int c = 2 * i + (mi & 1);
+                        uint32_t va[4];
+                        ldsm4_t(va, vb + v_row + t * 16 * 128 + (i / 4) * (UPOS * 128) + (((c % 8) ^ l7) << 4));
+#pragma unroll
+                        for (int n = 0; n < NQ; n++) mma16816(o[n][i], va, pb[n][0], pb[n][1]);
                     }
                 }
-            } else {
+            } else {  // the probabilities take K's place in the stage; then position by position
+                float *ps = reinterpret_cast<float *>(stage);
 #pragma unroll
-                for (int i = 0; i < NT; i++)
-                    for (int e = 0; e < 8; e++) {
-                        const int from = (lane & ~3) | (e >> 1), t = i * 8 + e;
-                        const float w0 = __shfl_sync(0xffffffffu, e & 1 ? s[i][1] : s[i][0], from);
-                        const float w1 = __shfl_sync(0xffffffffu, e & 1 ? s[i][3] : s[i][2], from);
-                        const bool see0 = p0 + t < lim0 && p0 + t < p.kv_end, see1 = p0 + t < lim1 && p0 + t < p.kv_end;
+                for (int n = 0; n < NQ; n++)
 #pragma unroll
-                        for (int c = 0; c < OT; c++) {
-                            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(
-                                stage + (NB + c / 8) * (UPOS * 128) + t * 128 + (((c % 8) ^ (t & 7)) << 4) + 4 * tq));
-                            if (see0) {
-                                o[c][0] += w0 * v.x;
-                                o[c][1] += w0 * v.y;
-                            }
-                            if (see1) {
-                                o[c][2] += w1 * v.x;
-                                o[c][3] += w1 * v.y;
-                            }
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            ps[(16 * i + 8 * (j >> 1) + g) * ROWS + 8 * n + 2 * tq + (j & 1)] = s[n][i][j];
+                touched = true;
+                __syncwarp();
+#pragma unroll 1
+                for (int t = 0; t < min(UPOS, p.kv_end - p0); t++) {
+                    float v[2 * KS];  // columns 8 c + g
+#pragma unroll
+                    for (int c = 0; c < 2 * KS; c++)
+                        v[c] = __bfloat162float(*reinterpret_cast<const bf16 *>(
+                            stage + (NB + c / 8) * (UPOS * 128) + t * 128 + (((c % 8) ^ (t & 7)) << 4) + 2 * g));
+#pragma unroll
+                    for (int n = 0; n < NQ; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            if (p0 + t >= lim[n][e]) continue;
+                            const float w = ps[t * ROWS + 8 * n + 2 * tq + e];
+#pragma unroll
+                            for (int c = 0; c < 2 * KS; c++) o[n][c / 2][c % 2 * 2 + e] += w * v[c];
                         }
-                    }
+                }
+                __syncwarp();
             }
-            if (touched) fence_proxy_async();  // the zeros, before the next TMA write of the stage
+            if (touched) fence_proxy_async();  // these writes, before the next TMA write of the stage
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[r.s]);
         }
@@ -352,19 +402,24 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
 
     // ---- merge the warps
 #pragma unroll
-    for (int off = 1; off < 4; off *= 2) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, off);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, off);
-    }
+    for (int n = 0; n < NQ; n++) {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int row = g + 8 * i;
-        if (row < rows) {
-            float *dst = merge_o + (cw * SMALL_ROWS + row) * DP;
+        for (int off = 4; off < 32; off *= 2) {
+            l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], off);
+            l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], off);
+        }
 #pragma unroll
-            for (int c = 0; c < OT; c++)
-                *reinterpret_cast<float2 *>(dst + ((c * 8 + 2 * tq) ^ (g * 8))) = make_float2(o[c][2 * i], o[c][2 * i + 1]);
-            if (tq == 0) merge_ml[cw * SMALL_ROWS + row] = i == 0 ? make_float2(m0, l0) : make_float2(m1, l1);
+        for (int e = 0; e < 2; e++) {
+            const int row = 8 * n + 2 * tq + e;
+            if (row < rows) {
+                float *dst = merge_o + (cw * ROWS + row) * DP;
+#pragma unroll
+                for (int i = 0; i < KS; i++) {
+                    dst[(16 * i + g) ^ (tq * 8)] = o[n][i][e];
+                    dst[(16 * i + 8 + g) ^ (tq * 8)] = o[n][i][2 + e];
+                }
+                if (g == 0) merge_ml[cw * ROWS + row] = make_float2(m[n][e], l[n][e]);
+            }
         }
     }
     bar_sync(1, NW * 32);
@@ -373,13 +428,13 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
         const int row = i / (DP / 4), d = i % (DP / 4) * 4;
         float m = -INFINITY, l = 0.0f, acc[4] = {};
 #pragma unroll
-        for (int w = 0; w < NW; w++) m = fmaxf(m, merge_ml[w * SMALL_ROWS + row].x);
+        for (int w = 0; w < NW; w++) m = fmaxf(m, merge_ml[w * ROWS + row].x);
         const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float2 ml = merge_ml[w * SMALL_ROWS + row];
+            const float2 ml = merge_ml[w * ROWS + row];
             const float f = ex2(ml.x - base);
-            const float4 v = *reinterpret_cast<const float4 *>(merge_o + (w * SMALL_ROWS + row) * DP + (d ^ ((row & 7) * 8)));
+            const float4 v = *reinterpret_cast<const float4 *>(merge_o + (w * ROWS + row) * DP + (d ^ ((row >> 1 & 3) * 8)));
             l += f * ml.y;
             acc[0] += f * v.x;
             acc[1] += f * v.y;
@@ -437,24 +492,34 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
 
 // ---------------------------------------------------------------- kernel for few rows alone
 
-template <int DP>
+constexpr int SMALL_PRODUCERS = 2;
+
+// NQ: query rows in eights. Warps and stages share the SM's registers and shared memory.
+template <int NQ>
+struct SmallShape {
+    static constexpr int WARPS = NQ == 1 ? 10 : 8, STAGES = NQ == 1 ? 10 : 8;
+};
+
+template <int DP, int NQ>
 struct SmallSmem {
-    alignas(1024) unsigned char ring[SMALL_STAGES * STAGE];
-    float merge_o[SMALL_WARPS * SMALL_ROWS * DP];
-    float2 merge_ml[SMALL_WARPS * SMALL_ROWS];
-    uint64_t full[SMALL_STAGES], empty[SMALL_STAGES];
+    static constexpr int NW = SmallShape<NQ>::WARPS, NST = SmallShape<NQ>::STAGES;
+    alignas(1024) unsigned char ring[NST * STAGE];
+    float merge_o[NW * 8 * NQ * DP];
+    float2 merge_ml[NW * 8 * NQ];
+    uint64_t full[NST], empty[NST];
     int flag;
 };
 
-template <int DP>
-__global__ void __launch_bounds__((1 + SMALL_WARPS) * 32, 1)
+template <int DP, int NQ>
+__global__ void __launch_bounds__((SMALL_PRODUCERS + SmallShape<NQ>::WARPS) * 32, 1)
     paged_small_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                        const __grid_constant__ PaArgs a) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    SmallSmem<DP> &sm = *reinterpret_cast<SmallSmem<DP> *>(align_shared<1024>(smem_raw));
+    constexpr int NW = SmallShape<NQ>::WARPS, NST = SmallShape<NQ>::STAGES;
+    SmallSmem<DP, NQ> &sm = *reinterpret_cast<SmallSmem<DP, NQ> *>(align_shared<1024>(smem_raw));
     const int warp = threadIdx.x / 32;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < SMALL_STAGES; i++) {
+        for (int i = 0; i < NST; i++) {
             mbar_init(&sm.full[i], 1);
             mbar_init(&sm.empty[i], 1);
         }
@@ -467,16 +532,17 @@ __global__ void __launch_bounds__((1 + SMALL_WARPS) * 32, 1)
     pdl_wait();
     const int2 work = a.ctas[blockIdx.x];
     if (work.y < 0) zero_rows(a);
-    Ring<SMALL_STAGES> r;
+    Ring<NST> r;
     Waiter wait;
-    if (warp == SMALL_WARPS) {
+    if (warp >= NW) {
         for (int i = 0; i < work.y; i++)
-            small_produce<DP, SMALL_STAGES>(a, &mk, &mv, a.pieces[work.x + i], sm.ring, sm.full, sm.empty, r, wait);
+            small_produce<DP, NST, SMALL_PRODUCERS>(a, &mk, &mv, a.pieces[work.x + i], sm.ring, sm.full, sm.empty, r, warp - NW,
+                                                    wait);
         // every load is waited for by a consumer before the CTA ends
     } else {
         for (int i = 0; i < work.y; i++)
-            small_consume<DP, SMALL_WARPS, SMALL_STAGES>(a, a.pieces[work.x + i], sm.ring, sm.full, sm.empty, r, wait, warp,
-                                                        sm.merge_o, sm.merge_ml, &sm.flag);
+            small_consume<DP, NW, NST, NQ>(a, a.pieces[work.x + i], sm.ring, sm.full, sm.empty, r, wait, warp, sm.merge_o,
+                                           sm.merge_ml, &sm.flag);
     }
 }
 
@@ -562,13 +628,15 @@ __device__ void big_produce(const PaArgs &a, const CUtensorMap *mq, const CUtens
     const int box = a.big_box, nsub = BIG_TILE / box, sub = lane % nsub, half = lane / nsub;
     const bool active = half < NB;
     const int *tab = a.table + (size_t)p.seq * a.max_pages;
-    int at = p.kv0 + sub * box;
-    int page = active && at < p.kv1 ? __ldg(tab + at / a.page_size) : 0;
-    int p0 = p.kv0;
+    int at = p.kv0 + sub * box, p0 = p.kv0;
+    PageWalk w(at, a.page_size);
+    int page = active && at < p.kv1 ? __ldg(tab + w.idx) : 0, slot = w.slot;
     do {
-        const int ahead = at + BIG_TILE;
-        const int next_page = active && ahead < p.kv1 ? __ldg(tab + ahead / a.page_size) : 0;
-        const uint32_t bytes = (uint32_t)(min(nsub, max(0, (p.kv1 - p0 + box - 1) / box)) * box * 128);
+        w.step(a.big_step_pages, a.big_step_slots, a.page_size);
+        const bool on = active && at < p.kv1;
+        at += BIG_TILE;
+        const int next_page = active && at < p.kv1 ? __ldg(tab + w.idx) : 0;
+        const uint32_t bytes = (uint32_t)((min(BIG_TILE, max(0, p.kv1 - p0) + box - 1) & -box) * 128);
 #pragma unroll
         for (int kv = 0; kv < 2; kv++) {
 #pragma unroll
@@ -577,14 +645,13 @@ __device__ void big_produce(const PaArgs &a, const CUtensorMap *mq, const CUtens
                 __syncwarp();
                 if (lane == 0) mbar_arrive_expect_tx(&sm.full[r.s], bytes);
                 __syncwarp();
-                if (active && half == h && at < p.kv1)
-                    tma_page(sm.ring + (size_t)r.s * STAGE + sub * box * 128, kv ? mv : mk, h * 64, at % a.page_size, p.kvh, page,
-                             &sm.full[r.s]);
+                if (on && half == h)
+                    tma_page(sm.ring + (size_t)r.s * STAGE + sub * box * 128, kv ? mv : mk, h * 64, slot, p.kvh, page, &sm.full[r.s]);
                 r.next();
             }
         }
-        at = ahead;
         page = next_page;
+        slot = w.slot;
         p0 += BIG_TILE;
     } while (p0 < p.kv1);
 }
@@ -663,9 +730,7 @@ __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, MixedSmem<DP> 
     constexpr int NB = DP / 64;
     const int steps = big_steps(p), lim_min = first_masked(p);
     if (x == 1 && p.n_tok <= a.tile_tok) {  // this tile is empty
-        r.next(2 * NB * steps % MIXED_STAGES);
-        // keep the phase: 2 * NB * steps stages are passed in whole laps, too
-        if (2 * NB * steps / MIXED_STAGES & 1) r.ph ^= 1;
+        r.advance(2 * NB * steps);
         for (int j = 0; j < steps; j++) n_masked += p.kv0 + (j + 1) * BIG_TILE > lim_min;
         return;
     }
@@ -912,7 +977,7 @@ __global__ void __launch_bounds__((4 + MIXED_WARPS) * 32, 1)
             const PagedPiece p = a.pieces[work.x + i];
             if (warp == 0) {
                 if (p.big) big_produce<DP>(a, &mq, &mk_big, &mv_big, p, sm, r, q_ph, wait);
-                else small_produce<DP, MIXED_STAGES>(a, &mk_small, &mv_small, p, sm.ring, sm.full, sm.empty, r, wait);
+                else small_produce<DP, MIXED_STAGES, 1>(a, &mk_small, &mv_small, p, sm.ring, sm.full, sm.empty, r, 0, wait);
             } else if (p.big) {
                 if (threadIdx.x % 32 == 0) big_multiply<DP>(a, p, sm, tmem, r, q_ph, p_ph, n_masked, wait);
                 __syncwarp();
@@ -938,7 +1003,7 @@ __global__ void __launch_bounds__((4 + MIXED_WARPS) * 32, 1)
             if (big && !p.big) bar_sync(1, MIXED_WARPS * 32);
             big = p.big;
             if (p.big) big_softmax<DP>(a, p, sm, tmem, x, r, s_ph, n_masked, wait);
-            else small_consume<DP, MIXED_WARPS, MIXED_STAGES>(a, p, sm.ring, sm.full, sm.empty, r, wait, warp - 4, sm.merge_o,
+            else small_consume<DP, MIXED_WARPS, MIXED_STAGES, 2>(a, p, sm.ring, sm.full, sm.empty, r, wait, warp - 4, sm.merge_o,
                                                             sm.merge_ml, &sm.flag);
         }
     }
@@ -1015,18 +1080,28 @@ bool make_query_map(CUtensorMap *map, const PagedAttnCall &c, const PaArgs &a) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <int DP, int NQ>
+int run_small(const CUtensorMap &mk, const CUtensorMap &mv, const PaArgs &a, cudaStream_t s) {
+    const size_t smem = sizeof(SmallSmem<DP, NQ>) + 1024;
+    auto kernel = paged_small_kernel<DP, NQ>;
+    Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(kernel), smem));
+    Q3_TRY_LAUNCH(launch(kernel, dim3(paged_ctas()), dim3((SMALL_PRODUCERS + SmallShape<NQ>::WARPS) * 32), smem, s, 1, mk, mv, a));
+    return Q3_OK;
+}
+
 template <int DP>
 int run(const PagedAttnCall &c, PaArgs &a, cudaStream_t s) {
     CUtensorMap mk, mv;
     a.small_box = std::min(a.small_box, 32 * 128 / DP);
     if (!make_page_map(&mk, c.cache.key_pages, c, a.small_box) || !make_page_map(&mv, c.cache.value_pages, c, a.small_box))
         return Q3_ERR_SHAPE;
-    if (!paged_has_big(c.shape)) {
-        const size_t smem = sizeof(SmallSmem<DP>) + 1024;
-        Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_small_kernel<DP>), smem));
-        Q3_TRY_LAUNCH(launch(paged_small_kernel<DP>, dim3(paged_ctas()), dim3((1 + SMALL_WARPS) * 32), smem, s, 1, mk, mv, a));
-        return Q3_OK;
-    }
+    const int small_step = 32 * 128 / DP * (paged_has_big(c.shape) ? 1 : SMALL_PRODUCERS);
+    a.small_step_pages = small_step / a.page_size;
+    a.small_step_slots = small_step % a.page_size;
+    a.big_step_pages = BIG_TILE / a.page_size;
+    a.big_step_slots = BIG_TILE % a.page_size;
+    if (c.shape.max_q_len * a.rep <= 8 && !paged_has_big(c.shape)) return run_small<DP, 1>(mk, mv, a, s);
+    if (!paged_has_big(c.shape)) return run_small<DP, 2>(mk, mv, a, s);
     CUtensorMap mq, mk_big, mv_big;
     if (!make_page_map(&mk_big, c.cache.key_pages, c, a.big_box) || !make_page_map(&mv_big, c.cache.value_pages, c, a.big_box) ||
         !make_query_map(&mq, c, a))
