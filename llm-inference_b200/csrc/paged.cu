@@ -25,12 +25,12 @@ struct PlanArgs {
     PagedPlanLayout l;
     q3_paged_shape s;
     const int *q_start, *kv_len, *page_table;
-    int n_ctas;
+    int n_ctas, small_step;
 };
 
-// Costs, in sixteen-KB loads' worth of a CTA's time: a step of a small item is one (32 or 64 positions of
-// K and V), a 128-position step of one or two tensor-core tiles BIG_ONE or BIG_TWO; an item's start and
-// end (queries, merge, output) ITEM. Items are cut only while each CTA still gets MIN_SHARE.
+// Costs, in 16 KB loads' worth of a CTA's time: a step of a small item is one, a 128-position step of one or two
+// tensor-core tiles BIG_ONE or BIG_TWO; an item's start and end (queries, merge, output) ITEM. Items are
+// cut only while each CTA still gets MIN_SHARE.
 constexpr int COST_ITEM = 3, COST_BIG_ONE = 2, COST_BIG_TWO = 3, MIN_SHARE = 16;
 
 // The items of sequence q: a big one has n_q per kv head.
@@ -48,8 +48,7 @@ __device__ __forceinline__ SeqItems seq_items(const PagedSeq &q, int rep) {
 }
 
 // Item i's positions end here, it has this many steps, and each costs this much.
-__device__ __forceinline__ void item_steps(const PagedSeq &q, const SeqItems &s, int i, int rep, int step, int *end, int *n,
-                                           int *cost) {
+__device__ __forceinline__ void item_steps(const PagedSeq &q, const SeqItems &s, int i, int step, int *end, int *n, int *cost) {
     const int last = min((i + 1) * s.span, q.q_len);
     *end = max(0, q.kv_len - q.q_len + last);
     *n = max(1, (*end + step - 1) / step);
@@ -153,16 +152,16 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
         toks[t] = tok;
     }
 
-    // ---- work: big items of all sequences, then small ones
+    // ---- work
     const int rep = a.s.n_heads / a.s.n_kv_heads, kvh = a.s.n_kv_heads;
-    const int small_step = a.s.head_dim <= 64 ? 64 : 32;
+    const int small_step = a.small_step;
     for (int b = tid; b < n; b += PLAN_THREADS) {
         const PagedSeq q = seqs[b];
         const SeqItems s = seq_items(q, rep);
         long long cost = 0;
         for (int i = 0; i < s.n_q; i++) {
             int end, steps, c;
-            item_steps(q, s, i, rep, s.big ? BIG_TILE : small_step, &end, &steps, &c);
+            item_steps(q, s, i, s.big ? BIG_TILE : small_step, &end, &steps, &c);
             cost += COST_ITEM + (long long)steps * c;
         }
         big_s[b] = s.big ? cost * kvh : 0;
@@ -171,54 +170,53 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     }
     __syncthreads();
     const long long items = scan(item_s, n, sums_s);
-    const int n_big = (int)(items >> 32), n_items = n_big + (int)(items & 0xffffffff);
-    const long long total_big = scan(big_s, n, sums_s), total = total_big + scan(small_s, n, sums_s);
+    const int n_items[2] = {(int)(items & 0xffffffff), (int)(items >> 32)};
+    const long long total_big = scan(big_s, n, sums_s), total_small = scan(small_s, n, sums_s);
     if (tid == 0) {
         big_s[n] = total_big;
-        small_s[n] = total - total_big;
+        small_s[n] = total_small;
     }
     __syncthreads();
-    const int used = (int)max(1ll, min((long long)a.n_ctas, max((long long)n_items, total / MIN_SHARE)));
     int2 *ctas = reinterpret_cast<int2 *>(a.plan + a.l.ctas);
     PagedPiece *pieces = reinterpret_cast<PagedPiece *>(a.plan + a.l.pieces);
     PagedPiece *splits = reinterpret_cast<PagedPiece *>(a.plan + a.l.splits);
     int *counters = reinterpret_cast<int *>(a.plan + a.l.counters);
     // A CTA's pieces start at (items before its first) + (CTAs before it): every cut adds one piece at most.
-    for (int c = tid; c < a.n_ctas; c += PLAN_THREADS) {
+    for (int id = tid; id < 2 * a.n_ctas; id += PLAN_THREADS) {
+        const bool big = id >= a.n_ctas;
+        const int c = big ? id - a.n_ctas : id, step = big ? BIG_TILE : small_step;
+        const long long total = big ? total_big : total_small;
+        const long long *pre = big ? big_s : small_s;
+        const int used = (int)max(1ll, min((long long)a.n_ctas, max((long long)n_items[big], total / MIN_SHARE)));
         auto bound = [&](int i) { return total * i / used; };
         const long long u0 = c < used ? bound(c) : total, u1 = c < used ? bound(c + 1) : total;
         int count = 0, first_piece = -1;
         PagedPiece split = {};
         long long u = u0;
         while (u < u1) {
-            const bool big = u < total_big;
-            const long long *pre = big ? big_s : small_s;
-            const long long at = big ? u : u - total_big, origin = big ? 0 : total_big;
-            int lo = 0, hi = n - 1;  // the last sequence that starts at or before `at`
+            int lo = 0, hi = n - 1;  // the last sequence that starts at or before u
             while (lo < hi) {
                 const int mid = (lo + hi + 1) / 2;
-                if (pre[mid] <= at) lo = mid;
+                if (pre[mid] <= u) lo = mid;
                 else hi = mid - 1;
             }
             const PagedSeq q = seqs[lo];
             const SeqItems s = seq_items(q, rep);
             const long long per_head = (pre[lo + 1] - pre[lo]) / kvh;
-            const int head = (int)((at - pre[lo]) / per_head);
+            const int head = (int)((u - pre[lo]) / per_head);
             long long start = pre[lo] + head * per_head;
             int i = 0, end, steps, cost;
             long long len;
             for (;; i++) {
-                item_steps(q, s, i, rep, big ? BIG_TILE : small_step, &end, &steps, &cost);
+                item_steps(q, s, i, step, &end, &steps, &cost);
                 len = COST_ITEM + (long long)steps * cost;
-                if (at < start + len) break;
+                if (u < start + len) break;
                 start += len;
             }
-            start += origin;  // in the common line of costs
             const int t0 = steps_before(u - start, steps, cost);
             const int t1 = u1 >= start + len ? steps : steps_before(u1 - start, steps, cost);
             if (t1 > t0) {
                 PagedPiece p;
-                const int step = big ? BIG_TILE : small_step;
                 p.seq = lo;
                 p.kvh = head;
                 p.tok0 = q.q0 + i * s.span;
@@ -241,16 +239,16 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
                     if (t0 == 0 && big) split = p;
                 }
                 if (first_piece < 0)
-                    first_piece = (big ? (int)(item_s[lo] >> 32) : n_big + (int)(item_s[lo] & 0xffffffff)) +
+                    first_piece = (big ? n_items[0] + a.n_ctas + (int)(item_s[lo] >> 32) : (int)(item_s[lo] & 0xffffffff)) +
                                   head * s.n_q + i + c;
                 pieces[first_piece + count] = p;
                 count++;
             }
             u = start + len;
         }
-        ctas[c] = make_int2(max(first_piece, 0), bad_starts ? -1 : count);
-        splits[c] = split;
-        counters[c] = 0;
+        ctas[(big ? PAGED_MAX_CTAS : 0) + c] = make_int2(max(first_piece, 0), bad_starts ? -1 : count);
+        if (big) splits[c] = split;
+        else counters[c] = 0;
     }
 }
 
@@ -511,7 +509,7 @@ int q3_paged_plan(void *plan, const q3_paged_shape *shape, const int *q_start, c
     if (!aligned16(plan)) return Q3_ERR_ALIGN;
     TRY(check_device());
     PlanArgs a = {static_cast<char *>(plan), paged_plan_layout(*shape), *shape, q_start, kv_len, page_table,
-                  paged_ctas()};
+                  paged_ctas(), paged_small_step(*shape)};
     const size_t smem = (size_t)(shape->n_seqs + 1) * (3 * sizeof(long long) + sizeof(int));
     Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_plan_kernel), smem));
     Q3_TRY_LAUNCH(launch(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), smem, (cudaStream_t)stream, 1, a));

@@ -18,8 +18,8 @@ struct PagedSeq {
 
 // Attention work. An item is what one CTA could do alone: the query rows of a (sequence, kv head) that
 // attend together. Few rows (q_len * n_heads / n_kv_heads <= SMALL_ROWS) are one item, fed to warp-level
-// matrix instructions 16 rows high; more are cut into items of two 128-row tensor-core tiles. The plan lays
-// all items' costs end to end and gives each CTA an equal stretch, so an item may be cut along its
+// matrix instructions; more are cut into items of two 128-row tensor-core tiles. Each kind has its kernel.
+// The plan lays a kind's costs end to end and gives each CTA an equal stretch, so an item may be cut along its
 // positions into pieces of neighbouring CTAs, which leave partial results in the scratch.
 constexpr int SMALL_ROWS = 16;
 constexpr int BIG_TILE = 128;       // rows of a tensor-core tile, and positions of one of its steps
@@ -41,7 +41,7 @@ struct PagedPlanLayout {
     size_t seqs;      // PagedSeq [n_seqs]
     size_t table;     // int [n_seqs][max_pages]: checked page ids, -1 past a sequence's last page
     size_t toks;      // int4 [n_tokens]: sequence, position, page, slot
-    size_t ctas;      // int2 [PAGED_MAX_CTAS]: first piece, pieces (-1: zero every row)
+    size_t ctas;      // int2 [2][PAGED_MAX_CTAS], small items' CTAs and big ones': first piece, pieces (-1: zero every row)
     size_t counters;  // int [PAGED_MAX_CTAS]: pieces done of the small item that starts in the CTA, zero at rest
     size_t splits;    // PagedPiece [PAGED_MAX_CTAS]: the big item that is cut at the CTA's end (n_parts 0: none)
     size_t pieces;    // PagedPiece []
@@ -62,10 +62,10 @@ inline PagedPlanLayout paged_plan_layout(const q3_paged_shape &s) {
     l.seqs = take((size_t)s.n_seqs * sizeof(PagedSeq));
     l.table = take((size_t)s.n_seqs * s.max_pages * 4);
     l.toks = take((size_t)s.n_tokens * 16);
-    l.ctas = take(PAGED_MAX_CTAS * sizeof(int2));
+    l.ctas = take(2 * PAGED_MAX_CTAS * sizeof(int2));
     l.counters = take(PAGED_MAX_CTAS * sizeof(int));
     l.splits = take(PAGED_MAX_CTAS * sizeof(PagedPiece));
-    l.pieces = take((items + PAGED_MAX_CTAS) * sizeof(PagedPiece));
+    l.pieces = take((items + 2 * PAGED_MAX_CTAS) * sizeof(PagedPiece));
     l.bytes = off;
     return l;
 }
@@ -79,6 +79,10 @@ struct PagedScratchLayout {
 inline bool paged_has_big(const q3_paged_shape &s) {
     return (long long)s.max_q_len * (s.n_heads / s.n_kv_heads) > SMALL_ROWS;
 }
+
+// A step of a small item is one ring stage of K and V; pieces are cut at multiples of it.
+constexpr int SMALL_STAGE = 16384;  // bytes
+inline int paged_small_step(const q3_paged_shape &s) { return SMALL_STAGE / (4 * (s.head_dim <= 64 ? 64 : 128)); }
 
 inline PagedScratchLayout paged_scratch_layout(const q3_paged_shape &s) {
     PagedScratchLayout l = {};

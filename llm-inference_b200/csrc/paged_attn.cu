@@ -36,9 +36,11 @@ namespace {
 
 __device__ unsigned g_dev_error;
 
-constexpr int STAGE = 16384;        // bytes of a ring stage
-constexpr int MIXED_STAGES = 10;    // kernel for both kinds: two softmax warpgroups
-constexpr int MIXED_WARPS = 8;
+constexpr int BOX64 = 16384;        // bytes of 128 rows x 64 columns, half a tile of K or V at head_dim 128
+constexpr int BIG_STAGE = 32768;    // a ring stage in the kernel for many rows: one such tile
+constexpr int BIG_STAGES = 5;
+constexpr int SMALL_PRODUCERS = 2;  // warps that load, in the kernel for few rows
+constexpr int BIG_THREADS = 128 + 512;  // loads, products; four softmax warpgroups, two threads a row
 constexpr float GROW = 8.0f;        // many rows: the reference follows the maximum in steps of 2^8
 
 struct PaArgs {
@@ -56,16 +58,39 @@ struct PaArgs {
     int small_step_pages, small_step_slots, big_step_pages, big_step_slots;  // a producer's step in pages and slots
     float scale_log2;
     uint32_t idesc_qk, idesc_pv;
+    bool after_big;  // few rows: launched behind the kernel for many rows, whose results are not needed
 };
 
 // ---------------------------------------------------------------- helpers
+
+// Polls a barrier a few thousand times. The loop is four instructions, and what follows a wait that gives up is out
+// of line: the roles' loops compete for the instruction cache.
+__device__ __forceinline__ bool poll(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+        "mov.u32 n, 4096;\n\t"
+        "again:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra done;\n\t"
+        "sub.u32 n, n, 1;\n\t"
+        "setp.ne.u32 q, n, 0;\n\t"
+        "@q bra again;\n\t"
+        "done:\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+__device__ __noinline__ bool wait_clocked(uint64_t *bar, uint32_t parity) { return mbar_wait(bar, parity, &g_dev_error); }
 
 // Waits until one has given up; from then on the role runs through its loop without waiting, so that every
 // barrier of the CTA still sees its arrivals and the kernel ends.
 struct Waiter {
     bool dead = false;
     __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) {
-        if (!dead) dead = !mbar_wait(bar, parity, &g_dev_error);
+        if (!dead && !poll(bar, parity)) dead = !wait_clocked(bar, parity);
     }
 };
 
@@ -92,6 +117,48 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// the disjunction over the N threads that meet at barrier `id`
+template <int N>
+__device__ __forceinline__ bool any_at(int id, bool x) {
+    int y;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.s32 p, %2, 0;\n\t"
+        "barrier.cta.red.or.pred.aligned q, %1, %3, p;\n\t"
+        "selp.s32 %0, 1, 0, q;\n\t}"
+        : "=r"(y)
+        : "r"(id), "r"((int)x), "n"(N)
+        : "memory");
+    return y != 0;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+// two floats as one operand of the packed fp32 instructions
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+    float2 y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+    return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
 __device__ __forceinline__ void tma_page(void *dst, const CUtensorMap *map, int x, int slot, int head, int page,
                                          uint64_t *bar) {
     asm volatile(
@@ -185,8 +252,9 @@ struct PageWalk {
 // warp that divided by the page size it took 1360 cycles a stage, half of the time at which HBM delivers.
 template <int DP, int NST, int NP>
 __device__ void small_produce(const PaArgs &a, const CUtensorMap *mk, const CUtensorMap *mv, const PagedPiece &p,
-                              unsigned char *ring, uint64_t *full, uint64_t *empty, Ring<NST> &r, int pid, Waiter &wait) {
-    constexpr int NB = DP / 64, UPOS = 32 * 128 / DP;
+                              unsigned char *ring, uint64_t *full, uint64_t *empty, Ring<NST> &r, int pid, Waiter &wait,
+                              int step_pages, int step_slots) {
+    constexpr int NB = DP / 64, UPOS = SMALL_STAGE / (4 * DP);
     static_assert(NST % NP == 0, "a stage belongs to one producer");
     const int lane = threadIdx.x % 32, box = a.small_box, nsub = UPOS / box;
     const int sub = lane % nsub, part = lane / nsub, half = part % NB;
@@ -202,18 +270,18 @@ __device__ void small_produce(const PaArgs &a, const CUtensorMap *mk, const CUte
     mine.next(skip);
     int page = active && at < p.kv1 ? __ldg(tab + w.idx) : 0, slot = w.slot;
     for (int u = skip; u < units; u += NP) {
-        w.step(a.small_step_pages, a.small_step_slots, a.page_size);
+        w.step(step_pages, step_slots, a.page_size);
         const bool on = active && at < p.kv1;
         at += NP * UPOS;
         const int next_page = active && at < p.kv1 ? __ldg(tab + w.idx) : 0;
         wait(&empty[mine.s], mine.ph ^ 1);
         __syncwarp();
-        if (lane == 0) {
+        if (lane == 0 && !wait.dead) {
             const int n = min(UPOS, max(0, p.kv1 - p0) + box - 1) & -box;
             mbar_arrive_expect_tx(&full[mine.s], (uint32_t)(n * 128 * NB * 2));
         }
         __syncwarp();
-        if (on) tma_page(ring + (size_t)mine.s * STAGE + off, map, half * 64, slot, p.kvh, page, &full[mine.s]);
+        if (on && !wait.dead) tma_page(ring + (size_t)mine.s * SMALL_STAGE + off, map, half * 64, slot, p.kvh, page, &full[mine.s]);
         mine.next(NP);
         p0 += NP * UPOS;
         page = next_page;
@@ -233,7 +301,7 @@ template <int DP, int NW, int NST, int NQ>
 __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned char *ring, uint64_t *full,
                               uint64_t *empty, Ring<NST> &r, Waiter &wait, int cw, float *merge_o, float2 *merge_ml,
                               int *flag_s) {
-    constexpr int NB = DP / 64, UPOS = 32 * 128 / DP, MT = UPOS / 16, KS = DP / 16, ROWS = 8 * NQ;
+    constexpr int NB = DP / 64, UPOS = SMALL_STAGE / (4 * DP), MT = UPOS / 16, KS = DP / 16, ROWS = 8 * NQ;
     const int lane = threadIdx.x % 32, g = lane / 4, tq = lane % 4, l7 = lane % 8, mi = lane / 8;
     const int rows = p.n_tok * a.rep;
     uint32_t qb[NQ][KS][2];
@@ -250,9 +318,9 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
                 qb[n][k][j] = row < rows && col < a.head_dim ? *reinterpret_cast<const uint32_t *>(src + col) : 0u;
             }
 #pragma unroll
-        for (int e = 0; e < 2; e++) lim[n][e] = p.pos0 + (8 * n + 2 * tq + e) / a.rep + 1;
+        for (int e = 0; e < 2; e++) lim[n][e] = min(p.pos0 + (8 * n + 2 * tq + e) / a.rep + 1, p.kv1);
     }
-    const int lim_min = first_masked(p);
+    const int lim_min = min(first_masked(p), p.kv1);  // a step may reach past the piece, where nothing was loaded
     float o[NQ][KS][4], m[NQ][2], l[NQ][2];  // o: columns 16 i + g and + 8 of rows 2 tq, 2 tq + 1
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
@@ -267,7 +335,7 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
     int p0 = p.kv0;
     do {
         if (r.s % NW == cw) {
-            unsigned char *stage = ring + (size_t)r.s * STAGE;
+            unsigned char *stage = ring + (size_t)r.s * SMALL_STAGE;
             const uint32_t kb = smem_u32(stage), vb = kb + NB * UPOS * 128;
             wait(&full[r.s], r.ph);
             __syncwarp();
@@ -329,8 +397,8 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
                     }
             }
             bool touched = false, slow = false;
-            if (p0 + UPOS > p.kv_end) {  // rows past the item's end: zero
-                const int t0 = max(0, p.kv_end - p0), n = (UPOS - t0) * 8;
+            if (p0 + UPOS > p.kv1) {  // rows past the end: zero
+                const int t0 = max(0, p.kv1 - p0), n = (UPOS - t0) * 8;
                 for (int h = 0; h < NB; h++)
                     for (int i = lane; i < n; i += 32)
                         reinterpret_cast<uint4 *>(stage + (NB + h) * (UPOS * 128) + t0 * 128)[i] = make_uint4(0, 0, 0, 0);
@@ -338,7 +406,7 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
                 __syncwarp();
             }
             if (masked && p.n_tok > 1) {  // rows that only some tokens see
-                const int t0 = max(0, lim_min - p0), n = (min(UPOS, p.kv_end - p0) - t0) * 8;
+                const int t0 = max(0, lim_min - p0), n = (min(UPOS, p.kv1 - p0) - t0) * 8;
                 for (int h = 0; h < NB; h++)
                     for (int i = lane; i < n; i += 32)
                         slow |= not_finite8(reinterpret_cast<const uint4 *>(stage + (NB + h) * (UPOS * 128) + t0 * 128)[i]);
@@ -374,7 +442,7 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
                 touched = true;
                 __syncwarp();
 #pragma unroll 1
-                for (int t = 0; t < min(UPOS, p.kv_end - p0); t++) {
+                for (int t = 0; t < min(UPOS, p.kv1 - p0); t++) {
                     float v[2 * KS];  // columns 8 c + g
 #pragma unroll
                     for (int c = 0; c < 2 * KS; c++)
@@ -492,8 +560,6 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
 
 // ---------------------------------------------------------------- kernel for few rows alone
 
-constexpr int SMALL_PRODUCERS = 2;
-
 // NQ: query rows in eights. Warps and stages share the SM's registers and shared memory.
 template <int NQ>
 struct SmallShape {
@@ -503,7 +569,7 @@ struct SmallShape {
 template <int DP, int NQ>
 struct SmallSmem {
     static constexpr int NW = SmallShape<NQ>::WARPS, NST = SmallShape<NQ>::STAGES;
-    alignas(1024) unsigned char ring[NST * STAGE];
+    alignas(1024) unsigned char ring[NST * SMALL_STAGE];
     float merge_o[NW * 8 * NQ * DP];
     float2 merge_ml[NW * 8 * NQ];
     uint64_t full[NST], empty[NST];
@@ -529,21 +595,24 @@ __global__ void __launch_bounds__((SMALL_PRODUCERS + SmallShape<NQ>::WARPS) * 32
     }
     __syncthreads();
     pdl_trigger();
-    pdl_wait();
+    // The kernel before is the plan or whatever wrote q, K and V; or it is the kernel for many rows, which let this one
+    // start only after it had itself waited for those: then there is nothing to wait for until the end.
+    if (!a.after_big) pdl_wait();
     const int2 work = a.ctas[blockIdx.x];
     if (work.y < 0) zero_rows(a);
     Ring<NST> r;
     Waiter wait;
     if (warp >= NW) {
         for (int i = 0; i < work.y; i++)
-            small_produce<DP, NST, SMALL_PRODUCERS>(a, &mk, &mv, a.pieces[work.x + i], sm.ring, sm.full, sm.empty, r, warp - NW,
-                                                    wait);
+            small_produce<DP, NST, SMALL_PRODUCERS>(a, &mk, &mv, a.pieces[work.x + i], sm.ring, sm.full, sm.empty, r,
+                                                                 warp - NW, wait, a.small_step_pages, a.small_step_slots);
         // every load is waited for by a consumer before the CTA ends
     } else {
         for (int i = 0; i < work.y; i++)
             small_consume<DP, NW, NST, NQ>(a, a.pieces[work.x + i], sm.ring, sm.full, sm.empty, r, wait, warp, sm.merge_o,
                                            sm.merge_ml, &sm.flag);
     }
+    if (a.after_big) pdl_wait();  // whoever waits for this kernel waits for that one, too
 }
 
 // ---------------------------------------------------------------- many rows
@@ -589,21 +658,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <int DP>
-struct MixedSmem {
-    static constexpr int NB = DP / 64;
-    union {
-        alignas(1024) unsigned char q[2 * NB * STAGE];            // two query tiles
-        float merge_o[MIXED_WARPS * SMALL_ROWS * DP];             // few rows: the warps' partial results
-    };
-    alignas(1024) unsigned char ring[MIXED_STAGES * STAGE];
-    float2 merge_ml[MIXED_WARPS * SMALL_ROWS];
-    uint64_t full[MIXED_STAGES], empty[MIXED_STAGES], q_full, q_empty, s_full[2], p_full[2], v_ready[2];
+struct BigSmem {
+    alignas(1024) unsigned char q[DP / 64 * 2 * BOX64];  // two query tiles
+    alignas(1024) unsigned char ring[BIG_STAGES * BIG_STAGE];
+    float stat[2][2][BIG_TILE];  // by tile and half of the columns: a row's maximum, at the end its sum
+    uint64_t full[BIG_STAGES], empty[BIG_STAGES], q_full, q_empty, s_full[2], p_full[2], o_full[2];
     uint32_t tmem;
-    int flag;
-    int v_bad[2][4];  // by v_ready, per warp: the step's V holds a NaN or infinity that some row must not see
+    int slow[2];  // by tile: this step's second product is not the tensor core's
 };
 
-// Tensor memory: S (and P over it) of tile x at column 128 x, O at 256 + DP x.
+// Tensor memory: S of tile x at column 128 x, O at 256 + DP x. P of positions 0 .. 63 lies over the first 32 columns of
+// their scores, P of 64 .. 127 over the first 32 of theirs.
 __device__ __forceinline__ uint32_t tmem_s(uint32_t base, int x) { return base + 128 * x; }
 template <int DP>
 __device__ __forceinline__ uint32_t tmem_o(uint32_t base, int x) {
@@ -612,199 +677,258 @@ __device__ __forceinline__ uint32_t tmem_o(uint32_t base, int x) {
 
 __device__ __forceinline__ int big_steps(const PagedPiece &p) { return max(1, (p.kv1 - p.kv0 + BIG_TILE - 1) / BIG_TILE); }
 
-// One warp loads a piece's queries, then K and V of each 128-position step.
+// One warp loads a piece's queries, then K of each 128-position step, another one V; each lane issues one box.
 template <int DP>
 __device__ void big_produce(const PaArgs &a, const CUtensorMap *mq, const CUtensorMap *mk, const CUtensorMap *mv,
-                            const PagedPiece &p, MixedSmem<DP> &sm, Ring<MIXED_STAGES> &r, uint32_t &q_ph, Waiter &wait) {
+                            const PagedPiece &p, BigSmem<DP> &sm, Ring<BIG_STAGES> &r, uint32_t &q_ph, int pid, Waiter &wait) {
     constexpr int NB = DP / 64;
-    const int lane = threadIdx.x % 32, tiles = p.n_tok > a.tile_tok ? 2 : 1;
-    wait(&sm.q_empty, q_ph ^ 1);
-    q_ph ^= 1;
-    __syncwarp();
-    if (lane == 0) mbar_arrive_expect_tx(&sm.q_full, (uint32_t)(tiles * NB * a.tile_tok * a.rep * 128));
-    __syncwarp();
-    if (lane < tiles * NB)
-        tma_load_3d(sm.q + lane * STAGE, mq, lane % NB * 64, p.kvh * a.rep, p.tok0 + lane / NB * a.tile_tok, &sm.q_full);
+    const int lane = threadIdx.x % 32, tiles = p.n_tok > a.tile_tok ? 2 : 1, n = big_steps(p);
+    Ring<BIG_STAGES> mine = r;
+    r.advance(2 * n);
+    if (pid == 0) {
+        wait(&sm.q_empty, q_ph ^ 1);
+        q_ph ^= 1;
+        __syncwarp();
+        if (lane == 0 && !wait.dead) mbar_arrive_expect_tx(&sm.q_full, (uint32_t)(tiles * NB * a.tile_tok * a.rep * 128));
+        __syncwarp();
+        if (lane < tiles * NB && !wait.dead)
+            tma_load_3d(sm.q + lane * BOX64, mq, lane % NB * 64, p.kvh * a.rep, p.tok0 + lane / NB * a.tile_tok, &sm.q_full);
+    } else {
+        mine.next();
+    }
+    const CUtensorMap *map = pid == 0 ? mk : mv;
     const int box = a.big_box, nsub = BIG_TILE / box, sub = lane % nsub, half = lane / nsub;
     const bool active = half < NB;
     const int *tab = a.table + (size_t)p.seq * a.max_pages;
     int at = p.kv0 + sub * box, p0 = p.kv0;
     PageWalk w(at, a.page_size);
     int page = active && at < p.kv1 ? __ldg(tab + w.idx) : 0, slot = w.slot;
-    do {
+    for (int j = 0; j < n; j++) {
         w.step(a.big_step_pages, a.big_step_slots, a.page_size);
         const bool on = active && at < p.kv1;
         at += BIG_TILE;
         const int next_page = active && at < p.kv1 ? __ldg(tab + w.idx) : 0;
-        const uint32_t bytes = (uint32_t)((min(BIG_TILE, max(0, p.kv1 - p0) + box - 1) & -box) * 128);
-#pragma unroll
-        for (int kv = 0; kv < 2; kv++) {
-#pragma unroll
-            for (int h = 0; h < NB; h++) {
-                wait(&sm.empty[r.s], r.ph ^ 1);
-                __syncwarp();
-                if (lane == 0) mbar_arrive_expect_tx(&sm.full[r.s], bytes);
-                __syncwarp();
-                if (on && half == h)
-                    tma_page(sm.ring + (size_t)r.s * STAGE + sub * box * 128, kv ? mv : mk, h * 64, slot, p.kvh, page, &sm.full[r.s]);
-                r.next();
-            }
-        }
+        const uint32_t bytes = (uint32_t)((min(BIG_TILE, max(0, p.kv1 - p0) + box - 1) & -box) * 128 * NB);
+        wait(&sm.empty[mine.s], mine.ph ^ 1);
+        __syncwarp();
+        if (lane == 0 && !wait.dead) mbar_arrive_expect_tx(&sm.full[mine.s], bytes);
+        __syncwarp();
+        if (on && !wait.dead)
+            tma_page(sm.ring + (size_t)mine.s * BIG_STAGE + half * BOX64 + sub * box * 128, map, half * 64, slot, p.kvh, page,
+                     &sm.full[mine.s]);
+        mine.next(2);
         page = next_page;
         slot = w.slot;
         p0 += BIG_TILE;
-    } while (p0 < p.kv1);
-}
-
-// One thread issues the products. Per step and tile: O += P V of this step, then S = Q K^T of the next one
-// into the columns P was read from (the tensor core takes a CTA's products in order).
-template <int DP>
-__device__ void big_multiply(const PaArgs &a, const PagedPiece &p, MixedSmem<DP> &sm, uint32_t tmem,
-                             Ring<MIXED_STAGES> &r, uint32_t &q_ph, uint32_t &p_ph, int &n_masked, Waiter &wait) {
-    constexpr int NB = DP / 64;
-    const int tiles = p.n_tok > a.tile_tok ? 2 : 1, steps = big_steps(p), lim_min = first_masked(p);
-    const uint32_t qb = smem_u32(sm.q), ring = smem_u32(sm.ring);
-    auto scores = [&](int x, int k_stage) {
-#pragma unroll
-        for (int k = 0; k < DP / 16; k++)
-            mma_bf16(tmem_s(tmem, x), smem_desc_sw128(qb + (x * NB + k / 4) * STAGE + k % 4 * 32),
-                     smem_desc_sw128(ring + (k_stage + k / 4) * STAGE + k % 4 * 32), a.idesc_qk, k > 0);
-        mma_commit(&sm.s_full[x]);
-    };
-    auto wait_stages = [&](const Ring<MIXED_STAGES> &at) {  // a tile's halves never wrap: the ring is a multiple of NB
-        for (int h = 0; h < NB; h++) wait(&sm.full[at.s + h], at.ph);
-        tc_fence_after();
-    };
-    auto release = [&](const Ring<MIXED_STAGES> &at) {
-        for (int h = 0; h < NB; h++) mma_commit(&sm.empty[at.s + h]);
-    };
-    wait(&sm.q_full, q_ph);
-    q_ph ^= 1;
-    wait_stages(r);
-    for (int x = 0; x < tiles; x++) scores(x, r.s);
-    release(r);
-    if (steps == 1) mma_commit(&sm.q_empty);
-    r.next(NB);
-    for (int j = 0; j < steps; j++) {
-        const Ring<MIXED_STAGES> rv = r;
-        r.next(NB);
-        const Ring<MIXED_STAGES> rk = r;  // the next step's K
-        const bool more = j + 1 < steps;
-        if (more) r.next(NB);
-        wait_stages(rv);
-        bool slow = false;
-        if (p.kv0 + (j + 1) * BIG_TILE > lim_min) {
-            const int b = n_masked & 1;
-            wait(&sm.v_ready[b], n_masked >> 1 & 1);
-            n_masked++;
-            const volatile int *bad = sm.v_bad[b];
-            slow = bad[0] | bad[1] | bad[2] | bad[3];
-        }
-        for (int x = 0; x < tiles; x++) {
-            wait(&sm.p_full[x], p_ph >> x & 1);
-            p_ph ^= 1u << x;
-            tc_fence_after();
-            if (!slow) {
-#pragma unroll
-                for (int k = 0; k < BIG_TILE / 16; k++)
-                    mma_bf16_ta(tmem_o<DP>(tmem, x), tmem_s(tmem, x) + k * 8,
-                                smem_desc_sw128(ring + rv.s * STAGE + k * 2048, STAGE, 1024), a.idesc_pv, j > 0 || k > 0);
-            }
-            if (more) {
-                if (x == 0) wait_stages(rk);
-                scores(x, rk.s);
-            } else {
-                mma_commit(&sm.s_full[x]);  // the tile's last product
-            }
-        }
-        release(rv);
-        if (more) release(rk);
-        if (j + 2 == steps) mma_commit(&sm.q_empty);
     }
 }
 
-// A warpgroup per tile, a thread per row.
+// one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t y;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(y));
+    return y != 0;
+}
+// a value that is the same in every lane, in a way that the compiler sees it
+template <typename T>
+__device__ __forceinline__ T uniform(T x) {
+    return __shfl_sync(0xffffffffu, x, 0);
+}
+
+// One thread of a warp issues the products of both tiles in turn: O += P V of this step, then S = Q K^T of the next one
+// over the columns that P was read from (the tensor core takes one thread's products in order). A tile's
+// two products run back to back while the other tile is in its softmax. s_full of a step says, too, that the
+// product of the step before has finished; o_full says it of the last one. Neither can move on
+// twice before its softmax has seen the first time.
+//
+// This warp's own instructions are what the tensor core idles for, so they are few: one wait per step and tile, for P,
+// with another warp's arrival on the same barrier (big_ready) saying that V and the next K have landed; control
+// flow that is the same for all lanes, with what it depends on broadcast, so that operands of the products are made
+// in uniform registers (as one lane's code, a product took up to 95 cycles to issue instead of 56).
 template <int DP>
-__device__ void big_softmax(const PaArgs &a, const PagedPiece &p, MixedSmem<DP> &sm, uint32_t tmem, int x,
-                            Ring<MIXED_STAGES> &r, uint32_t &s_ph, int &n_masked, Waiter &wait) {
-    constexpr int NB = DP / 64;
-    const int steps = big_steps(p), lim_min = first_masked(p);
+__device__ void big_multiply(const PaArgs &a, const PagedPiece &p, BigSmem<DP> &sm, uint32_t tmem_any, Ring<BIG_STAGES> &r,
+                             uint32_t &q_ph, uint32_t &p_ph, Waiter &wait) {
+    const int tiles = uniform(p.n_tok > a.tile_tok ? 2 : 1), n = uniform(big_steps(p));
+    const int first = uniform((first_masked(p) - p.kv0) / BIG_TILE);  // rows are masked from this step on
+    const uint32_t tmem = uniform(tmem_any), ring = smem_u32(sm.ring);
+    const uint64_t q_desc = smem_desc_sw128(smem_u32(sm.q)), k_desc = smem_desc_sw128(ring),
+                   v_desc = smem_desc_sw128(ring, BOX64, 1024);  // descriptors count in 16 bytes
+    auto scores = [&](int x, int stage) {
+        const uint64_t qd = q_desc + x * (DP / 64 * BOX64 >> 4), kd = k_desc + stage * (BIG_STAGE >> 4);
+#pragma unroll
+        for (int k = 0; k < DP / 16; k++)
+            mma_bf16(tmem_s(tmem, x), qd + k / 4 * (BOX64 >> 4) + k % 4 * 2, kd + k / 4 * (BOX64 >> 4) + k % 4 * 2, a.idesc_qk, k > 0);
+        mma_commit(&sm.s_full[x]);
+    };
+    wait(&sm.q_full, q_ph);
+    q_ph ^= 1;
+    wait(&sm.full[r.s], r.ph);
+    if (__any_sync(0xffffffffu, wait.dead)) return;
+    tc_fence_after();
+    int stage = uniform(r.s);
+    r.advance(2 * n);
+    if (elect_one()) {
+        scores(0, stage);
+        if (tiles > 1) scores(1, stage);
+        mma_commit(&sm.empty[stage]);
+        if (n == 1) mma_commit(&sm.q_empty);
+    }
+    __syncwarp();
+    stage = stage + 1 == BIG_STAGES ? 0 : stage + 1;
+#pragma unroll 1
+    for (int j = 0; j < n; j++) {
+        const bool more = j + 1 < n;
+        const int v_stage = stage, k_stage = stage + 1 == BIG_STAGES ? 0 : stage + 1;
+        stage = k_stage + 1 == BIG_STAGES ? 0 : k_stage + 1;
+        const uint64_t vd = v_desc + v_stage * (BIG_STAGE >> 4);
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            if (x == 1 && tiles == 1) break;
+            wait(&sm.p_full[x], p_ph >> x & 1);
+            p_ph ^= 1u << x;
+            tc_fence_after();
+            const bool slow = j >= first && *(const volatile int *)&sm.slow[x];
+            if (elect_one()) {
+                if (!slow) {
+#pragma unroll
+                    for (int k = 0; k < BIG_TILE / 16; k++)
+                        mma_bf16_ta(tmem_o<DP>(tmem, x), tmem_s(tmem, x) + k / 4 * 64 + k % 4 * 8, vd + k * (2048 >> 4), a.idesc_pv, j > 0 || k > 0);
+                }
+                if (more) scores(x, k_stage);
+                else mma_commit(&sm.o_full[x]);
+                if (x == tiles - 1) {
+                    mma_commit(&sm.empty[v_stage]);
+                    if (more) mma_commit(&sm.empty[k_stage]);
+                    if (j + 2 == n) mma_commit(&sm.q_empty);
+                }
+            }
+            __syncwarp();
+        }
+    }
+}
+
+// One thread waits for V of each step and K of the next, and passes that on with P's arrivals.
+template <int DP>
+__device__ void big_ready(const PaArgs &a, const PagedPiece &p, BigSmem<DP> &sm, Ring<BIG_STAGES> &r, uint32_t &p_ph,
+                          Waiter &wait) {
+    const int tiles = p.n_tok > a.tile_tok ? 2 : 1, n = big_steps(p);
+    wait(&sm.full[r.s], r.ph);  // the first K
+    r.next();
+    for (int j = 0; j < n; j++) {
+        wait(&sm.full[r.s], r.ph);
+        r.next();
+        if (j + 1 < n) {
+            wait(&sm.full[r.s], r.ph);
+            r.next();
+        }
+        for (int x = 0; x < tiles; x++) {
+            wait(&sm.p_full[x], p_ph >> x & 1 ^ 1);  // the step before has its P: this arrival counts for this one
+            p_ph ^= 1u << x;
+            if (wait.dead) return;
+            mbar_arrive(&sm.p_full[x]);
+        }
+    }
+}
+
+// 64 scores of a row: their largest (in `top`), P against the row's reference as bf16, and P's sum. Columns at or past
+// `seen` are left out.
+template <bool MASKED>
+__device__ __forceinline__ float exp64(uint32_t ts, int seen, uint64_t c2, uint64_t base2, uint32_t *pk, float &top) {
+    uint32_t u[64];
+    tmem_ld32(ts, u);
+    tmem_ld32(ts + 32, u + 32);
+    tmem_wait_ld();
+    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    uint64_t sum[2] = {};
+#pragma unroll
+    for (int e = 0; e < 32; e++) {
+        float s0 = __uint_as_float(u[2 * e]), s1 = __uint_as_float(u[2 * e + 1]);
+        if (MASKED && 2 * e >= seen) s0 = -INFINITY;
+        if (MASKED && 2 * e + 1 >= seen) s1 = -INFINITY;
+        x[e & 3] = max3(x[e & 3], s0, s1);
+        const uint64_t y = fma2(pair(s0, s1), c2, base2);
+        const float2 w = unpair(y);
+        const float p0 = ex2(w.x), p1 = ex2(w.y);
+        sum[e & 1] = add2(sum[e & 1], pair(p0, p1));
+        pk[e] = pack_bf16(p0, p1);
+    }
+    top = fmaxf(max3(x[0], x[1], x[2]), x[3]);
+    const float2 w = unpair(add2(sum[0], sum[1]));
+    return w.x + w.y;
+}
+
+// Two warpgroups per tile, two threads per row: each takes 64 of a step's columns and half of the output's.
+template <int DP>
+__device__ void big_softmax(const PaArgs &a, const PagedPiece &p, BigSmem<DP> &sm, uint32_t tmem, int x, int part,
+                            Ring<BIG_STAGES> &r, uint32_t &s_ph, Waiter &wait) {
+    constexpr int NB = DP / 64, HALF = BIG_TILE / 2;
+    const int n = big_steps(p), lim_min = first_masked(p);
     if (x == 1 && p.n_tok <= a.tile_tok) {  // this tile is empty
-        r.advance(2 * NB * steps);
-        for (int j = 0; j < steps; j++) n_masked += p.kv0 + (j + 1) * BIG_TILE > lim_min;
+        r.advance(2 * n);
         return;
     }
     const int quarter = threadIdx.x / 32 % 4, lane = threadIdx.x % 32, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t ts = tmem_s(tmem, x) + lanes, to = tmem_o<DP>(tmem, x) + lanes;
+    const uint32_t ts = tmem_s(tmem, x) + lanes, to = tmem_o<DP>(tmem, x) + lanes + part * (DP / 2);
     const int tt = x * a.tile_tok + row / a.rep, lim = p.pos0 + tt + 1;
     // a negative scale negates Q in the first product; a zero one must still leave masked scores at -infinity
     const float c = fmaxf(fabsf(a.scale_log2), 1e-30f);
     float m = -INFINITY, l = 0.0f;
-    for (int j = 0; j < steps; j++) {
-        r.next(NB);
-        const Ring<MIXED_STAGES> rv = r;
-        r.next(NB);
+#pragma unroll 1
+    for (int j = 0; j < n; j++) {
+        r.next();
+        const Ring<BIG_STAGES> rv = r;
+        r.next();
         const int t0 = p.kv0 + j * BIG_TILE;
         const bool masked = t0 + BIG_TILE > lim_min;
-        wait(&sm.s_full[x], s_ph);
+        wait(&sm.s_full[x], s_ph & 1);
         s_ph ^= 1;
         __syncwarp();
         tc_fence_after();
-        uint32_t su[128];
-#pragma unroll
-        for (int i = 0; i < 4; i++) tmem_ld32(ts + 32 * i, su + 32 * i);
         bool slow = false;
-        if (masked) {
-            const int b = n_masked & 1;
-            if (x == 0) {  // V past the item's end becomes zero; rows only some tokens see are checked
-                for (int h = 0; h < NB; h++) wait(&sm.full[rv.s + h], rv.ph);
-                __syncwarp();
-                bool bad = false;
-                unsigned char *v = sm.ring + (size_t)rv.s * STAGE;
-                const int end = min(BIG_TILE, p.kv_end - t0), check = max(0, lim_min - t0);
-                for (int i = row; i < NB * 128 * 8; i += 128) {
-                    uint4 *chunk = reinterpret_cast<uint4 *>(v) + i;
-                    const int t = i / 8 % 128;
-                    if (t >= end) *chunk = make_uint4(0, 0, 0, 0);
-                    else if (t >= check) bad |= not_finite8(*chunk);
-                }
-                fence_proxy_async();
-                bad = __any_sync(0xffffffffu, bad);
-                if (lane == 0) {
-                    sm.v_bad[b][quarter] = bad;
-                    mbar_arrive(&sm.v_ready[b]);
-                }
-            }
-            wait(&sm.v_ready[b], n_masked >> 1 & 1);
+        unsigned char *v = sm.ring + (size_t)rv.s * BIG_STAGE;
+        if (masked) {  // V past the item's end becomes zero; rows only some tokens see are checked
+            wait(&sm.full[rv.s], rv.ph);
             __syncwarp();
-            n_masked++;
-            const volatile int *flags = sm.v_bad[b];
-            slow = flags[0] | flags[1] | flags[2] | flags[3];
+            const int end = min(BIG_TILE, p.kv_end - t0), check = max(0, lim_min - t0);
+            for (int i = row + part * 128; i < NB * BIG_TILE * 8; i += 256) {
+                uint4 *chunk = reinterpret_cast<uint4 *>(v) + i;
+                const int t = i / 8 % BIG_TILE;
+                if (t >= end) *chunk = make_uint4(0, 0, 0, 0);
+                else if (t >= check) slow |= not_finite8(*chunk);
+            }
+            fence_proxy_async();
+            slow = any_at<256>(9 + x, slow);
         }
-        tmem_wait_ld();
-        float s[128];
-#pragma unroll
-        for (int i = 0; i < 128; i++) s[i] = __uint_as_float(su[i]);
-        if (masked) {
-#pragma unroll
-            for (int i = 0; i < 128; i++)
-                if (t0 + i >= lim) s[i] = -INFINITY;
-        }
-        float x0 = fmaxf(s[0], s[1]), x1 = fmaxf(s[2], s[3]);
-#pragma unroll
-        for (int i = 4; i < 128; i += 4) {
-            x0 = fmaxf(x0, fmaxf(s[i], s[i + 1]));
-            x1 = fmaxf(x1, fmaxf(s[i + 2], s[i + 3]));
-        }
-        const float top = fmaxf(x0, x1) * c;
-        const bool grow = top > m + GROW || (m == -INFINITY && top > m);
-        if (__any_sync(0xffffffffu, grow)) {
-            const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
-            if (grow) m = top;
+        if (masked && row == 0 && part == 0) sm.slow[x] = slow;
+        // P is taken against the reference as it stands, its maximum found on the way. Only if a row outgrew its
+        // reference (always in the first step) is the reference moved, what was summed against it rescaled, and P
+        // taken again; S is still in tensor memory, for P is stored after the row's two threads have agreed.
+        const uint32_t sv = ts + HALF * part;
+        const int seen = lim - t0 - HALF * part, pairs = 1 + x * 4 + quarter;
+        uint32_t pk[32];
+        float top, more;
+        auto take = [&]() {
+            const float base = m == -INFINITY ? 0.0f : -m;
+            more = masked ? exp64<true>(sv, seen, pair(c, c), pair(base, base), pk, top)
+                          : exp64<false>(sv, 0, pair(c, c), pair(base, base), pk, top);
+        };
+        take();
+        if (any_at<64>(pairs, top * c > m + GROW || (m == -INFINITY && top > m))) {
+            sm.stat[x][part][row] = top;
+            bar_sync(pairs, 64);
+            const float both = fmaxf(top, sm.stat[x][part ^ 1][row]) * c;
+            const bool grow = both > m + GROW || (m == -INFINITY && both > m);
+            const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - both);
+            if (grow) m = both;
             l *= f;
-            if (j > 0) {  // the previous product has finished: s_full was committed after it
-                for (int i = 0; i < DP / 16; i++) {
+            if (j > 0) {  // O is at rest: the product of j - 1 came before these scores
+#pragma unroll 1
+                for (int i = 0; i < DP / 32; i++) {
                     uint32_t o[16];
                     tmem_ld8(to + 16 * i, reinterpret_cast<float *>(o));
                     tmem_ld8(to + 16 * i + 8, reinterpret_cast<float *>(o) + 8);
@@ -815,30 +939,21 @@ __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, MixedSmem<DP> 
                 }
                 tmem_wait_st();
             }
+            bar_sync(pairs, 64);  // both have read the maxima
+            take();
         }
-        const float base = m == -INFINITY ? 0.0f : -m;
         if (!slow) {
-            float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                uint32_t pk[16];
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const float a0 = ex2(__fmaf_rn(s[32 * i + 2 * e], c, base));
-                    const float a1 = ex2(__fmaf_rn(s[32 * i + 2 * e + 1], c, base));
-                    sum0 += a0;
-                    sum1 += a1;
-                    pk[e] = pack_bf16(a0, a1);
-                }
-                tmem_st16(ts + 16 * i, pk);
-            }
-            l += sum0 + sum1;
+            l += more;
+            tmem_st16(sv, pk);
+            tmem_st16(sv + 16, pk + 16);
             tmem_wait_st();
         } else {
             // on the CUDA cores, 16 columns of O at a time, over the positions this row sees
-            const unsigned char *v = sm.ring + (size_t)rv.s * STAGE;
-            for (int d = 0; d < DP / 16; d++) {
+#pragma unroll 1
+            for (int d = 0; d < DP / 32; d++) {
+                const int dd = part * (DP / 32) + d;
                 float acc[16];
+                const float base = m == -INFINITY ? 0.0f : -m;
                 if (j > 0) {
                     tmem_ld8(to + 16 * d, acc);
                     tmem_ld8(to + 16 * d + 8, acc + 8);
@@ -847,6 +962,7 @@ __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, MixedSmem<DP> 
 #pragma unroll
                     for (int e = 0; e < 16; e++) acc[e] = 0.0f;
                 }
+#pragma unroll 1
                 for (int t8 = 0; t8 < BIG_TILE; t8 += 8) {
                     float sc[8];
                     __syncwarp();
@@ -857,16 +973,16 @@ __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, MixedSmem<DP> 
                         const int t = t8 + e;
                         if (t0 + t >= lim || t0 + t >= p.kv_end) continue;
                         const float w = ex2(__fmaf_rn(sc[e], c, base));
-                        if (d == 0) l += w;
+                        if (d == 0 && t / HALF == part) l += w;
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const uint4 u = *reinterpret_cast<const uint4 *>(v + d / 4 * STAGE + t * 128 + (((d % 4 * 2 + h) ^ (t & 7)) << 4));
-                            const __nv_bfloat162 *w2 = reinterpret_cast<const __nv_bfloat162 *>(&u);
+                        for (int g = 0; g < 2; g++) {
+                            const uint4 q4 = *reinterpret_cast<const uint4 *>(v + dd / 4 * BOX64 + t * 128 + (((dd % 4 * 2 + g) ^ (t & 7)) << 4));
+                            const __nv_bfloat162 *w2 = reinterpret_cast<const __nv_bfloat162 *>(&q4);
 #pragma unroll
                             for (int q = 0; q < 4; q++) {
                                 const float2 vv = __bfloat1622float2(w2[q]);
-                                acc[8 * h + 2 * q] += w * vv.x;
-                                acc[8 * h + 2 * q + 1] += w * vv.y;
+                                acc[8 * g + 2 * q] += w * vv.x;
+                                acc[8 * g + 2 * q + 1] += w * vv.y;
                             }
                         }
                     }
@@ -880,17 +996,20 @@ __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, MixedSmem<DP> 
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.p_full[x]);
     }
-    wait(&sm.s_full[x], s_ph);
-    s_ph ^= 1;
+    sm.stat[x][part][row] = l;
+    bar_sync(1 + x * 4 + quarter, 64);
+    l += sm.stat[x][part ^ 1][row];
+    wait(&sm.o_full[x], s_ph >> 1);
+    s_ph ^= 2;
     __syncwarp();
     tc_fence_after();
     const bool valid = row / a.rep < a.tile_tok && tt < p.n_tok;
     const int head = p.kvh * a.rep + row % a.rep;
     if (p.part < 0) {
-        const float inv = lim <= 0 ? 0.0f : 1.0f / l;
+        const float inv = 1.0f / l;
         bf16 *dst = a.out + (p.tok0 + tt) * a.out_stride + (long long)head * a.head_dim;
 #pragma unroll
-        for (int i = 0; i < DP / 32; i++) {
+        for (int i = 0; i < DP / 64; i++) {
             uint32_t o[32];
             tmem_ld32(to + 32 * i, o);
             tmem_wait_ld();
@@ -898,43 +1017,47 @@ __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, MixedSmem<DP> 
             for (int e = 0; e < 4; e++) {
                 uint32_t w[4];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const float lo = __uint_as_float(o[8 * e + 2 * q]), hi = __uint_as_float(o[8 * e + 2 * q + 1]);
-                    w[q] = pack_bf16(lo * inv, hi * inv);
-                }
-                const int d = 32 * i + 8 * e;
-                if (valid && d < a.head_dim)
+                for (int q = 0; q < 4; q++)
+                    w[q] = pack_bf16(__uint_as_float(o[8 * e + 2 * q]) * inv, __uint_as_float(o[8 * e + 2 * q + 1]) * inv);
+                const int d = part * (DP / 2) + 32 * i + 8 * e;
+                if (valid && d < a.head_dim)  // a row without positions is zero
                     *reinterpret_cast<uint4 *>(dst + d) = lim <= 0 ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
     } else {
         const size_t at = (size_t)p.part * (2 * BIG_TILE) + x * BIG_TILE + row;
 #pragma unroll
-        for (int i = 0; i < DP / 32; i++) {
+        for (int i = 0; i < DP / 64; i++) {
             uint32_t o[32];
             tmem_ld32(to + 32 * i, o);
             tmem_wait_ld();
             if (valid) {
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                    __stcg(reinterpret_cast<uint4 *>(a.big_o + at * DP + 32 * i) + e, make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
+                    __stcg(reinterpret_cast<uint4 *>(a.big_o + at * DP + part * (DP / 2) + 32 * i) + e,
+                           make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
             }
         }
-        if (valid) __stcg(a.big_ml + at, make_float2(m, l));
+        if (valid && part == 0) __stcg(a.big_ml + at, make_float2(m, l));
     }
     tc_fence_before();
+    bar_sync(1 + x * 4 + quarter, 64);  // the sums have been read
 }
 
 template <int DP>
-__global__ void __launch_bounds__((4 + MIXED_WARPS) * 32, 1)
-    paged_mixed_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk_small,
-                       const __grid_constant__ CUtensorMap mv_small, const __grid_constant__ CUtensorMap mk_big,
-                       const __grid_constant__ CUtensorMap mv_big, const __grid_constant__ PaArgs a) {
+__global__ void __launch_bounds__(BIG_THREADS, 1)
+    paged_big_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                     const __grid_constant__ CUtensorMap mv, const __grid_constant__ PaArgs a) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    MixedSmem<DP> &sm = *reinterpret_cast<MixedSmem<DP> *>(align_shared<1024>(smem_raw));
+    // no room to align by hand; the declaration's alignment holds for the shared window
+    BigSmem<DP> &sm = *reinterpret_cast<BigSmem<DP> *>(smem_raw);
+    if (smem_u32(smem_raw) % 1024 != 0) {
+        if (threadIdx.x == 0) atomicOr(&g_dev_error, DEV_ERR_TMEM);
+        return;
+    }
     const int warp = threadIdx.x / 32;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < MIXED_STAGES; i++) {
+        for (int i = 0; i < BIG_STAGES; i++) {
             mbar_init(&sm.full[i], 1);
             mbar_init(&sm.empty[i], 1);
         }
@@ -942,15 +1065,13 @@ __global__ void __launch_bounds__((4 + MIXED_WARPS) * 32, 1)
         mbar_init(&sm.q_empty, 1);
         for (int x = 0; x < 2; x++) {
             mbar_init(&sm.s_full[x], 1);
-            mbar_init(&sm.p_full[x], 4);
-            mbar_init(&sm.v_ready[x], 4);
+            mbar_init(&sm.o_full[x], 1);
+            mbar_init(&sm.p_full[x], 9);
         }
         fence_barrier_init();
         prefetch_tmap(&mq);
-        prefetch_tmap(&mk_small);
-        prefetch_tmap(&mv_small);
-        prefetch_tmap(&mk_big);
-        prefetch_tmap(&mv_big);
+        prefetch_tmap(&mk);
+        prefetch_tmap(&mv);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512)
@@ -961,50 +1082,43 @@ __global__ void __launch_bounds__((4 + MIXED_WARPS) * 32, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
-    // after the allocation: a dependent kernel's CTA that took this SM's tensor memory first would wait for this
-    // kernel while this CTA waits for its memory
-    pdl_trigger();
+    // The next kernel may start once this one's predecessors are done (the kernel for few rows relies on it) and
+    // every CTA has its tensor memory: a dependent's CTA that took it first would wait for this kernel while
+    // this CTA waits for its memory.
     pdl_wait();
-    const int2 work = a.ctas[blockIdx.x];
+    pdl_trigger();
+    const int2 work = a.ctas[PAGED_MAX_CTAS + blockIdx.x];
     if (work.y < 0) zero_rows(a);
-    Ring<MIXED_STAGES> r;
+    Ring<BIG_STAGES> r;
     Waiter wait;
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         uint32_t q_ph = 0, p_ph = 0;
-        int n_masked = 0;
-        for (int i = 0; i < work.y && warp < 2; i++) {
+        const bool first = threadIdx.x % 32 == 0;
+        for (int i = 0; i < work.y; i++) {
             const PagedPiece p = a.pieces[work.x + i];
-            if (warp == 0) {
-                if (p.big) big_produce<DP>(a, &mq, &mk_big, &mv_big, p, sm, r, q_ph, wait);
-                else small_produce<DP, MIXED_STAGES, 1>(a, &mk_small, &mv_small, p, sm.ring, sm.full, sm.empty, r, 0, wait);
-            } else if (p.big) {
-                if (threadIdx.x % 32 == 0) big_multiply<DP>(a, p, sm, tmem, r, q_ph, p_ph, n_masked, wait);
-                __syncwarp();
-            }
+            if (warp % 2 == 0) big_produce<DP>(a, &mq, &mk, &mv, p, sm, r, q_ph, warp / 2, wait);
+            else if (warp == 1) big_multiply<DP>(a, p, sm, tmem, r, q_ph, p_ph, wait);
+            else if (first) big_ready<DP>(a, p, sm, r, p_ph, wait);
         }
+        __syncwarp();
         if (warp == 0) {  // the products' release of the ring arrives asynchronously: before the CTA ends
-            for (int i = 0; i < MIXED_STAGES; i++) {
+            for (int i = 0; i < BIG_STAGES; i++) {
                 wait(&sm.empty[r.s], r.ph ^ 1);
                 r.next();
             }
             wait(&sm.q_empty, q_ph ^ 1);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-        const int x = warp >= 8;
+        const int group = warp / 4 - 1;
         uint32_t s_ph = 0;
-        int n_masked = 0;
-        bool big = false;
         for (int i = 0; i < work.y; i++) {
             const PagedPiece p = a.pieces[work.x + i];
-            // from the last big piece to the small ones together: a warpgroup whose tile was empty came here early, while
-            // the ring and the queries, whose memory the merge uses, still belonged to the big piece
-            if (big && !p.big) bar_sync(1, MIXED_WARPS * 32);
-            big = p.big;
-            if (p.big) big_softmax<DP>(a, p, sm, tmem, x, r, s_ph, n_masked, wait);
-            else small_consume<DP, MIXED_WARPS, MIXED_STAGES, 2>(a, p, sm.ring, sm.full, sm.empty, r, wait, warp - 4, sm.merge_o,
-                                                            sm.merge_ml, &sm.flag);
+            big_softmax<DP>(a, p, sm, tmem, group / 2, group % 2, r, s_ph, wait);
+        }
+    }
+    if (wait.dead) {  // a wait gave up: what was issued before it, or without it since, ends well within this time
+        const uint64_t t = globaltimer();
+        while (globaltimer() - t < 1000000) {
         }
     }
     __syncthreads();
@@ -1092,28 +1206,30 @@ int run_small(const CUtensorMap &mk, const CUtensorMap &mv, const PaArgs &a, cud
 template <int DP>
 int run(const PagedAttnCall &c, PaArgs &a, cudaStream_t s) {
     CUtensorMap mk, mv;
-    a.small_box = std::min(a.small_box, 32 * 128 / DP);
-    if (!make_page_map(&mk, c.cache.key_pages, c, a.small_box) || !make_page_map(&mv, c.cache.value_pages, c, a.small_box))
-        return Q3_ERR_SHAPE;
-    const int small_step = 32 * 128 / DP * (paged_has_big(c.shape) ? 1 : SMALL_PRODUCERS);
-    a.small_step_pages = small_step / a.page_size;
-    a.small_step_slots = small_step % a.page_size;
+    const int small_step = paged_small_step(c.shape), loads = small_step * SMALL_PRODUCERS;
+    a.small_box = std::min(a.small_box, small_step);
+    a.small_step_pages = loads / a.page_size;
+    a.small_step_slots = loads % a.page_size;
     a.big_step_pages = BIG_TILE / a.page_size;
     a.big_step_slots = BIG_TILE % a.page_size;
-    if (c.shape.max_q_len * a.rep <= 8 && !paged_has_big(c.shape)) return run_small<DP, 1>(mk, mv, a, s);
-    if (!paged_has_big(c.shape)) return run_small<DP, 2>(mk, mv, a, s);
-    CUtensorMap mq, mk_big, mv_big;
-    if (!make_page_map(&mk_big, c.cache.key_pages, c, a.big_box) || !make_page_map(&mv_big, c.cache.value_pages, c, a.big_box) ||
-        !make_query_map(&mq, c, a))
+    if (!make_page_map(&mk, c.cache.key_pages, c, a.small_box) || !make_page_map(&mv, c.cache.value_pages, c, a.small_box))
         return Q3_ERR_SHAPE;
-    // f32 accumulator, bf16 operands; second product: B = V with its columns contiguous
-    const uint32_t kinds = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BIG_TILE >> 4) << 24);
-    a.idesc_qk = kinds | ((uint32_t)(BIG_TILE >> 3) << 17) | (c.scale < 0.0f ? 1u << 13 : 0u);
-    a.idesc_pv = kinds | ((uint32_t)(DP >> 3) << 17) | (1u << 16);
-    const size_t smem = sizeof(MixedSmem<DP>) + 1024;
-    Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_mixed_kernel<DP>), smem));
-    Q3_TRY_LAUNCH(launch(paged_mixed_kernel<DP>, dim3(paged_ctas()), dim3((4 + MIXED_WARPS) * 32), smem, s, 1, mq, mk, mv,
-                         mk_big, mv_big, a));
+    a.after_big = paged_has_big(c.shape);
+    if (a.after_big) {
+        CUtensorMap mq, mk_big, mv_big;
+        if (!make_page_map(&mk_big, c.cache.key_pages, c, a.big_box) || !make_page_map(&mv_big, c.cache.value_pages, c, a.big_box) ||
+            !make_query_map(&mq, c, a))
+            return Q3_ERR_SHAPE;
+        // f32 accumulator, bf16 operands; second product: B = V with its columns contiguous
+        const uint32_t kinds = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BIG_TILE >> 4) << 24);
+        a.idesc_qk = kinds | ((uint32_t)(BIG_TILE >> 3) << 17) | (c.scale < 0.0f ? 1u << 13 : 0u);
+        a.idesc_pv = kinds | ((uint32_t)(DP >> 3) << 17) | (1u << 16);
+        const size_t smem = sizeof(BigSmem<DP>);
+        Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_big_kernel<DP>), smem));
+        Q3_TRY_LAUNCH(launch(paged_big_kernel<DP>, dim3(paged_ctas()), dim3(BIG_THREADS), smem, s, 1, mq, mk_big, mv_big, a));
+    }
+    const int st = std::min(c.shape.max_q_len * a.rep, SMALL_ROWS) <= 8 ? run_small<DP, 1>(mk, mv, a, s) : run_small<DP, 2>(mk, mv, a, s);
+    if (st != Q3_OK || !a.after_big) return st;
     Q3_TRY_LAUNCH(launch(paged_combine_kernel<DP>, dim3(paged_ctas(), 2 * BIG_TILE / 32), dim3(256), 0, s, 1, a));
     return Q3_OK;
 }
