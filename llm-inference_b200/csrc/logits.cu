@@ -1,9 +1,12 @@
 // Penalties, biases and grammar masks on a step's logits (q3_logits_process).
 //
-// A CTA owns a slice of one row's vocabulary. It counts the row's history into shared memory (bit
-// 31: the token occurs, low bits: how often it was generated; integer adds, so the order of the
-// atomics does not matter), notes for each biased token the largest index of its entries, and
-// then makes one pass over its slice.
+// A CTA owns a slice of one row's vocabulary, eight tokens a thread, whose logits it asks for first. Meanwhile
+// it counts the row's history into shared memory (bit 31: the token occurs, low bits: how often it was
+// generated; integer adds, so the order of the atomics does not matter) and notes for each biased token the
+// largest index of its entries; then one pass over the slice.
+//
+// Bound by the logits' bytes, in and out, for a batch, and by latency for one row. Each slice reads the
+// row's whole history, from L2 after the first, so slices are as large as still leaves two per SM.
 #include <math.h>
 
 #include <algorithm>
@@ -17,14 +20,13 @@ namespace {
 
 __device__ unsigned g_dev_error;
 
-constexpr int LP_THREADS = 512;
-constexpr int LP_SLICE = 8192;  // tokens per CTA
+constexpr int LP_EACH = 8;  // tokens per thread
 constexpr unsigned LP_SEEN = 1u << 31;
 
 struct LogitsArgs {
     void *out;
     const void *in;
-    int vocab;
+    int vocab, vec;
     long long out_stride, stride, mask_stride;
     const int *hist_start, *hist_split, *hist_ids;
     const float *repetition, *frequency, *presence;
@@ -38,17 +40,76 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ void from_f32(float f, bf16 *o) { *o = __float2bfloat16(f); }
 __device__ __forceinline__ void from_f32(float f, float *o) { *o = f; }
 
+__device__ __forceinline__ void unpack(const uint4 *u, float *x, bf16) {
+    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __bfloat1622float2(h[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void unpack(const uint4 *u, float *x, float) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = __uint_as_float(reinterpret_cast<const uint32_t *>(u)[i]);
+}
+__device__ __forceinline__ void pack(const float *x, uint4 *u, bf16) {
+    __nv_bfloat162 *h = reinterpret_cast<__nv_bfloat162 *>(u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+}
+__device__ __forceinline__ void pack(const float *x, uint4 *u, float) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) reinterpret_cast<uint32_t *>(u)[i] = __float_as_uint(x[i]);
+}
+
+// f(index, id) for ids[i0 .. i1) by the CTA, four at a time where they are aligned.
+template <typename F>
+__device__ __forceinline__ void each_id(const int *ids, int i0, int i1, F f) {
+    const int lead = min(i1 - i0, (int)((16 - (reinterpret_cast<uintptr_t>(ids + i0) & 15)) & 15) / 4);
+    const int quads = (i1 - i0 - lead) / 4, tail = i0 + lead + 4 * quads;
+    if ((int)threadIdx.x < lead) f(i0 + threadIdx.x, ids[i0 + threadIdx.x]);
+    for (int q = threadIdx.x; q < quads; q += blockDim.x) {
+        const int i = i0 + lead + 4 * q;
+        const int4 v = __ldg(reinterpret_cast<const int4 *>(ids + i));
+        f(i, v.x);
+        f(i + 1, v.y);
+        f(i + 2, v.z);
+        f(i + 3, v.w);
+    }
+    if (tail + (int)threadIdx.x < i1) f(tail + threadIdx.x, ids[tail + threadIdx.x]);
+}
+
+// A slice starts `shift` tokens early, so that a row whose first logit is not 16-byte aligned is still read in whole
+// vectors; a.vec says that input and output rows are aligned alike.
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logits_process_kernel(const __grid_constant__ LogitsArgs a) {
+__global__ void __launch_bounds__(512) logits_process_kernel(const __grid_constant__ LogitsArgs a) {
     extern __shared__ __align__(16) unsigned lp_smem[];
-    unsigned *count_s = lp_smem;                             // [LP_SLICE] if there is a history
-    int *bias_s = reinterpret_cast<int *>(lp_smem + (a.hist_start ? LP_SLICE : 0));  // [LP_SLICE] if there are biases
+    constexpr int VECS = LP_EACH * sizeof(T) / 16;
+    const int slice = LP_EACH * blockDim.x, r = blockIdx.y, tid = threadIdx.x;
+    unsigned *count_s = lp_smem;                                                  // [slice] if there is a history
+    int *bias_s = reinterpret_cast<int *>(lp_smem + (a.hist_start ? slice : 0));  // [slice] if there are biases
     pdl_trigger();
     pdl_wait();
-    const int r = blockIdx.y, s0 = blockIdx.x * LP_SLICE, n = min(LP_SLICE, a.vocab - s0), tid = threadIdx.x;
-    bool hist = a.hist_start != nullptr, biased = a.bias_start != nullptr;
+    const T *in = static_cast<const T *>(a.in) + r * a.stride;
+    T *out = static_cast<T *>(a.out) + r * a.out_stride;
+    const int shift = a.vec ? (int)((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T)) : 0;
+    const int s0 = (int)(blockIdx.x * slice) - shift, i0 = s0 + LP_EACH * tid;
+    const bool whole = a.vec && i0 >= 0 && i0 + LP_EACH <= a.vocab;
+    uint4 raw[VECS];
+    if (whole) {
+#pragma unroll
+        for (int v = 0; v < VECS; v++) raw[v] = reinterpret_cast<const uint4 *>(in + i0)[v];
+    }
+    uint32_t allowed = 0xff;  // by token, bit 0 first
+    if (a.mask && i0 < a.vocab) {
+        const unsigned *mask = a.mask + r * a.mask_stride;
+        const int from = max(i0, 0), word = from / 32, lastw = (a.vocab - 1) / 32;
+        const unsigned bits = __funnelshift_r(mask[word], mask[min(word + 1, lastw)], from % 32);
+        allowed = bits << (from - i0);
+    }
     int h0 = 0, h1 = 0, hs = 0, b0 = 0, b1 = 0;
-    if (hist) {
+    if (a.hist_start) {
         h0 = a.hist_start[r];
         h1 = a.hist_start[r + 1];
         hs = a.hist_split[r];
@@ -56,50 +117,75 @@ __global__ void __launch_bounds__(LP_THREADS) logits_process_kernel(const __grid
             if (tid == 0) atomicOr(&g_dev_error, DEV_ERR_POS_RANGE);
             h1 = h0;
         }
-        hist = h1 > h0;
     }
-    if (biased) {
+    if (a.bias_start) {
         b0 = a.bias_start[r];
         b1 = a.bias_start[r + 1];
         if (b0 < 0 || b1 < b0) {
             if (tid == 0) atomicOr(&g_dev_error, DEV_ERR_POS_RANGE);
             b1 = b0;
         }
-        biased = b1 > b0;
     }
-    for (int i = tid; i < n; i += LP_THREADS) {
-        if (hist) count_s[i] = 0;
-        if (biased) bias_s[i] = -1;
+    const bool hist = h1 > h0, biased = b1 > b0;
+    if (hist || biased) {
+#pragma unroll
+        for (int v = 0; v < LP_EACH / 4; v++) {
+            if (hist) reinterpret_cast<uint4 *>(count_s)[tid * (LP_EACH / 4) + v] = make_uint4(0, 0, 0, 0);
+            if (biased) reinterpret_cast<int4 *>(bias_s)[tid * (LP_EACH / 4) + v] = make_int4(-1, -1, -1, -1);
+        }
+        __syncthreads();
+        const int first = max(s0, 0), n = max(0, min(s0 + slice, a.vocab) - first);  // this slice's ids
+        if (hist)
+            each_id(a.hist_ids, h0, h1, [&](int i, int id) {
+                if ((unsigned)(id - first) < (unsigned)n) {
+                    if (i < hs) atomicOr(&count_s[id - s0], LP_SEEN);
+                    else atomicAdd(&count_s[id - s0], 1u);
+                }
+            });
+        if (biased)
+            each_id(a.bias_ids, b0, b1, [&](int i, int id) {
+                if ((unsigned)(id - first) < (unsigned)n) atomicMax(&bias_s[id - s0], i);
+            });
+        __syncthreads();
     }
-    __syncthreads();
-    for (int i = h0 + tid; i < h1; i += LP_THREADS) {
-        const int t = a.hist_ids[i] - s0;
-        if (t >= 0 && t < n) {
-            if (i < hs) atomicOr(&count_s[t], LP_SEEN);
-            else atomicAdd(&count_s[t], 1);
+    float x[LP_EACH];
+    if (whole) {
+        unpack(raw, x, T());
+    } else {
+#pragma unroll
+        for (int e = 0; e < LP_EACH; e++) x[e] = i0 + e >= 0 && i0 + e < a.vocab ? to_f32(in[i0 + e]) : 0.0f;
+    }
+    if (hist) {
+        const float rep = a.repetition ? a.repetition[r] : 1.0f, freq = a.frequency ? a.frequency[r] : 0.0f,
+                    pres = a.presence ? a.presence[r] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < LP_EACH; e++) {
+            const unsigned c = count_s[LP_EACH * tid + e];
+            if (c != 0) {
+                if (a.repetition) x[e] = x[e] > 0.0f ? x[e] / rep : x[e] * rep;
+                const unsigned times = c & ~LP_SEEN;
+                if (times != 0) x[e] -= freq * (float)times + pres;
+            }
         }
     }
-    for (int i = b0 + tid; i < b1; i += LP_THREADS) {
-        const int t = a.bias_ids[i] - s0;
-        if (t >= 0 && t < n) atomicMax(&bias_s[t], i);
-    }
-    __syncthreads();
-    const float rep = a.repetition ? a.repetition[r] : 1.0f;
-    const float freq = a.frequency ? a.frequency[r] : 0.0f, pres = a.presence ? a.presence[r] : 0.0f;
-    const T *in = static_cast<const T *>(a.in) + r * a.stride + s0;
-    T *out = static_cast<T *>(a.out) + r * a.out_stride + s0;
-    const unsigned *mask = a.mask ? a.mask + r * a.mask_stride : nullptr;
-    for (int i = tid; i < n; i += LP_THREADS) {
-        float x = to_f32(in[i]);
-        const unsigned c = hist ? count_s[i] : 0u;
-        if (c != 0) {
-            if (a.repetition) x = x > 0.0f ? x / rep : x * rep;
-            const unsigned times = c & ~LP_SEEN;
-            if (times != 0) x -= freq * (float)times + pres;
+    if (biased) {
+#pragma unroll
+        for (int e = 0; e < LP_EACH; e++) {
+            const int i = bias_s[LP_EACH * tid + e];
+            if (i >= 0) x[e] += a.bias[i];
         }
-        if (biased && bias_s[i] >= 0) x += a.bias[bias_s[i]];
-        if (mask && !(mask[(s0 + i) / 32] >> ((s0 + i) % 32) & 1)) x = -INFINITY;
-        from_f32(x, &out[i]);
+    }
+#pragma unroll
+    for (int e = 0; e < LP_EACH; e++)
+        if (!(allowed >> e & 1)) x[e] = -INFINITY;
+    if (whole) {
+        pack(x, raw, T());
+#pragma unroll
+        for (int v = 0; v < VECS; v++) reinterpret_cast<uint4 *>(out + i0)[v] = raw[v];
+    } else {
+#pragma unroll
+        for (int e = 0; e < LP_EACH; e++)
+            if (i0 + e >= 0 && i0 + e < a.vocab) from_f32(x[e], &out[i0 + e]);
     }
 }
 
@@ -131,14 +217,22 @@ extern "C" int q3_logits_process(void *out, const void *logits, int dtype, int r
     const int st = check_device();
     if (st != Q3_OK) return st;
     if (rows == 0) return Q3_OK;
-    LogitsArgs a = {out,       logits,     vocab,    out_stride, stride,   mask_stride, hist_start, hist_split,
-                    hist_ids,  repetition, frequency, presence,  bias_start, bias_ids,  bias,       mask};
+    const int elt = dtype ? 4 : 2;
+    // the same place in a 16-byte line for each row's input and output, and whole lines between places of a row
+    const bool vec = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(logits)) & 15) == 0 &&
+                     (out_stride - stride) * elt % 16 == 0;
+    LogitsArgs a = {out,        logits,    vocab,    vec,        out_stride, stride, mask_stride, hist_start, hist_split, hist_ids,
+                    repetition, frequency, presence, bias_start, bias_ids,   bias,   mask};
     if (!repetition && !frequency && !presence) a.hist_start = nullptr;
-    const size_t smem = (size_t)LP_SLICE * 4 * ((a.hist_start ? 1 : 0) + (a.bias_start ? 1 : 0));
-    const dim3 grid((vocab + LP_SLICE - 1) / LP_SLICE, rows);
+    // two slices an SM at least; 128 threads are the smallest that make whole warps busy
+    int threads = 512;
+    auto slices = [&](int t) { return (vocab + 7 + LP_EACH * t - 1) / (LP_EACH * t); };
+    while (threads > 128 && (long long)slices(threads) * rows < 2 * num_sms()) threads /= 2;
+    const size_t smem = (size_t)LP_EACH * threads * 4 * ((a.hist_start ? 1 : 0) + (a.bias_start ? 1 : 0));
+    const dim3 grid(slices(threads), rows);
     auto kernel = dtype == 0 ? logits_process_kernel<bf16> : logits_process_kernel<float>;
     cudaError_t e = allow_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return record_cuda_error(e);
-    Q3_TRY_LAUNCH(launch(kernel, grid, dim3(LP_THREADS), smem, (cudaStream_t)stream, 1, a));
+    Q3_TRY_LAUNCH(launch(kernel, grid, dim3(threads), smem, (cudaStream_t)stream, 1, a));
     return Q3_OK;
 }

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
                     while (f + 1 < used && bound(f + 1) < start + len && steps_before(bound(f + 1) - start, steps, cost) < steps) f++;
                     p.n_parts = f - p.first + 1;
                     p.part = part_slot(p.first, c - p.first);
-                    if (t0 == 0 && big) split = p;
+                    if (t0 == 0 && p.n_parts > MERGE_PARTS) split = p;
                 }
                 if (first_piece < 0)
                     first_piece = (big ? n_items[0] + a.n_ctas + (int)(item_s[lo] >> 32) : (int)(item_s[lo] & 0xffffffff)) +
@@ -248,21 +248,24 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
         }
         ctas[(big ? PAGED_MAX_CTAS : 0) + c] = make_int2(max(first_piece, 0), bad_starts ? -1 : count);
         if (big) splits[c] = split;
-        else counters[c] = 0;
+        counters[(big ? PAGED_MAX_CTAS : 0) + c] = 0;
+        if (big) counters[2 * PAGED_MAX_CTAS + c] = 0;
     }
 }
 
 // ------------------------------------------------------------------ append
-// One CTA per token. A unit is two 8-element chunks of a head that one lane holds in registers: for
+// One CTA per token, with a group of lanes for every head where 512 threads are enough for that. A unit is two 8-element chunks of a head that one lane holds in registers: for
 // half-split pairs chunk u and its partner u + rope_dim/16, so a pair's two elements sit in one lane;
 // otherwise neighbours. A head is a group of `lph` lanes (a power of two), so the sum of squares
 // is a few shuffles. The angles depend on the token alone: the CTA computes them once, then every
-// head reads them from shared memory.
+// head reads them from shared memory; what the heads hold is asked for before. Bound by the rows' bytes, and for
+// few tokens by the chain plan -> angle -> heads.
 //
 // The angle is reduced in fp64: pos * inv_freq reaches 10^5 rad and more, where an fp32 product is
 // off by up to 2^-25 of itself, more than a bf16 result may be. turns = pos * inv_freq / 2 pi, its
 // nearest integer dropped, goes to sincospif.
-constexpr int APPEND_THREADS = 128;
+constexpr int APPEND_MAX_THREADS = 512;
+constexpr int APPEND_ODD_THREADS = 128;
 
 struct AppendArgs {
     bf16 *q_out;
@@ -303,46 +306,46 @@ __device__ __forceinline__ void rope_angle(int pos, float inv_freq, float amplit
 }
 
 template <bool INTERLEAVED>
-__global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(APPEND_MAX_THREADS) paged_append_kernel(const __grid_constant__ AppendArgs a) {
     __shared__ float cos_s[PAGED_MAX_HEAD_DIM / 2], sin_s[PAGED_MAX_HEAD_DIM / 2];
     pdl_trigger();
     pdl_wait();
-    const int t = blockIdx.x;
-    const int4 tok = a.toks[t];
-    const int pos = tok.y;
-    if (pos == PAGED_OUTSIDE) return;
-    const int half = a.rope_dim / 2;
-    for (int j = threadIdx.x; j < half; j += APPEND_THREADS)
-        if (pos >= 0) rope_angle(pos, a.inv_freq[j], a.amplitude, &cos_s[j], &sin_s[j]);
-    __syncthreads();
-    const int u = threadIdx.x % a.lph, nc = a.head_dim / 8, hc = INTERLEAVED ? 0 : half / 8;
+    const int t = blockIdx.x, heads = a.n_heads + 2 * a.n_kv_heads, groups = blockDim.x / a.lph;
+    const int u = threadIdx.x % a.lph, half = a.rope_dim / 2, nc = a.head_dim / 8, hc = INTERLEAVED ? 0 : half / 8;
     const int c0 = INTERLEAVED ? 2 * u : u < hc ? u : 2 * u;  // units past the rotated pairs: chunks 2u, 2u + 1
     const int c1 = !INTERLEAVED && u < hc ? u + hc : c0 + 1;
     const bool in0 = c0 < nc, in1 = c1 < nc;
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int h = threadIdx.x / a.lph; h < a.n_heads + 2 * a.n_kv_heads; h += APPEND_THREADS / a.lph) {
+    auto source = [&](int h) {
         const int kh = h - a.n_heads, vh = kh - a.n_kv_heads;
-        const bf16 *src;
-        bf16 *dst;
-        const bf16 *w = nullptr;
-        if (kh < 0) {
-            src = a.q + t * a.q_stride + (long long)h * a.head_dim;
-            dst = a.q_out + t * a.q_out_stride + (long long)h * a.head_dim;
-            w = a.q_norm_w;
-        } else {
-            const long long slot = tok.z * a.page_stride + tok.w * a.pos_stride;
-            src = vh < 0 ? a.k + t * a.k_stride + (long long)kh * a.head_dim
-                         : a.v + t * a.v_stride + (long long)vh * a.head_dim;
-            dst = vh < 0 ? a.key_pages + slot + kh * a.head_stride : a.value_pages + slot + vh * a.head_stride;
-            w = a.k_norm_w;
-        }
+        return kh < 0 ? a.q + t * a.q_stride + (long long)h * a.head_dim
+                      : vh < 0 ? a.k + t * a.k_stride + (long long)kh * a.head_dim
+                               : a.v + t * a.v_stride + (long long)vh * a.head_dim;
+    };
+    int h = threadIdx.x / a.lph;
+    uint4 r0 = zero, r1 = zero;
+    if (h < heads) {
+        const uint4 *src = reinterpret_cast<const uint4 *>(source(h));
+        if (in0) r0 = src[c0];
+        if (in1) r1 = src[c1];
+    }
+    const int4 tok = a.toks[t];
+    const int pos = tok.y;
+    if (pos == PAGED_OUTSIDE) return;
+    for (int j = threadIdx.x; j < half; j += blockDim.x)
+        if (pos >= 0) rope_angle(pos, a.inv_freq[j], a.amplitude, &cos_s[j], &sin_s[j]);
+    __syncthreads();
+    for (; h < heads; h += groups) {
+        const int kh = h - a.n_heads, vh = kh - a.n_kv_heads;
+        const long long slot = tok.z * a.page_stride + tok.w * a.pos_stride;
+        bf16 *dst = kh < 0 ? a.q_out + t * a.q_out_stride + (long long)h * a.head_dim
+                           : vh < 0 ? a.key_pages + slot + kh * a.head_stride : a.value_pages + slot + vh * a.head_stride;
+        const bf16 *w = kh < 0 ? a.q_norm_w : a.k_norm_w;
         if (pos < 0) {  // padding: zero query rows, nothing stored
             if (kh < 0 && in0) reinterpret_cast<uint4 *>(dst)[c0] = zero;
             if (kh < 0 && in1) reinterpret_cast<uint4 *>(dst)[c1] = zero;
             continue;
         }
-        const uint4 r0 = in0 ? reinterpret_cast<const uint4 *>(src)[c0] : zero;
-        const uint4 r1 = in1 ? reinterpret_cast<const uint4 *>(src)[c1] : zero;
         uint4 o0 = r0, o1 = r1;
         if (vh < 0) {
             float x[16];
@@ -384,25 +387,30 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __gr
         }
         if (in0) reinterpret_cast<uint4 *>(dst)[c0] = o0;
         if (in1) reinterpret_cast<uint4 *>(dst)[c1] = o1;
+        if (h + groups < heads) {
+            const uint4 *src = reinterpret_cast<const uint4 *>(source(h + groups));
+            if (in0) r0 = src[c0];
+            if (in1) r1 = src[c1];
+        }
     }
 }
 
 // Half-split pairs whose distance is not a multiple of 8 elements: one warp per head, the head's
 // fp32 values in the warp's shared memory.
-__global__ void __launch_bounds__(APPEND_THREADS) paged_append_odd_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(APPEND_ODD_THREADS) paged_append_odd_kernel(const __grid_constant__ AppendArgs a) {
     __shared__ float cos_s[PAGED_MAX_HEAD_DIM / 2], sin_s[PAGED_MAX_HEAD_DIM / 2];
-    __shared__ float head_s[APPEND_THREADS / 32][PAGED_MAX_HEAD_DIM];
+    __shared__ float head_s[APPEND_ODD_THREADS / 32][PAGED_MAX_HEAD_DIM];
     pdl_trigger();
     pdl_wait();
     const int t = blockIdx.x, lane = threadIdx.x % 32;
     const int4 tok = a.toks[t];
     const int pos = tok.y, D = a.head_dim, half = a.rope_dim / 2;
     if (pos == PAGED_OUTSIDE) return;
-    for (int j = threadIdx.x; j < half; j += APPEND_THREADS)
+    for (int j = threadIdx.x; j < half; j += APPEND_ODD_THREADS)
         if (pos >= 0) rope_angle(pos, a.inv_freq[j], a.amplitude, &cos_s[j], &sin_s[j]);
     __syncthreads();
     float *x = head_s[threadIdx.x / 32];
-    for (int h = threadIdx.x / 32; h < a.n_heads + 2 * a.n_kv_heads; h += APPEND_THREADS / 32) {
+    for (int h = threadIdx.x / 32; h < a.n_heads + 2 * a.n_kv_heads; h += APPEND_ODD_THREADS / 32) {
         const int kh = h - a.n_heads, vh = kh - a.n_kv_heads;
         if (pos < 0) {
             if (kh < 0)
@@ -564,10 +572,11 @@ int q3_paged_rope_append(q3_bf16 *q_out, long long q_out_stride, const q3_bf16 *
     const int units = hc + (chunks - 2 * hc + 1) / 2;
     for (a.lph = 1; a.lph < units;) a.lph *= 2;
     cudaStream_t st = (cudaStream_t)stream;
-    const dim3 grid(s.n_tokens), block(APPEND_THREADS);
+    const int heads = s.n_heads + 2 * s.n_kv_heads, rounds = (heads * a.lph + APPEND_MAX_THREADS - 1) / APPEND_MAX_THREADS;
+    const dim3 grid(s.n_tokens), block(((heads + rounds - 1) / rounds * a.lph + 31) / 32 * 32);
     if (interleaved) Q3_TRY_LAUNCH(launch(paged_append_kernel<true>, grid, block, 0, st, 1, a));
     else if (rope_dim % 16 == 0) Q3_TRY_LAUNCH(launch(paged_append_kernel<false>, grid, block, 0, st, 1, a));
-    else Q3_TRY_LAUNCH(launch(paged_append_odd_kernel, grid, block, 0, st, 1, a));
+    else Q3_TRY_LAUNCH(launch(paged_append_odd_kernel, grid, dim3(APPEND_ODD_THREADS), 0, st, 1, a));
     return Q3_OK;
 }
 

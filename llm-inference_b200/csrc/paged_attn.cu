@@ -292,43 +292,36 @@ __device__ void small_produce(const PaArgs &a, const CUtensorMap *mk, const CUte
 
 // ---------------------------------------------------------------- few rows: consumers
 
-// The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that positions and head columns fill the
-// instruction's 16 rows and query rows its 8 columns: NQ = 1 for up to 8 rows, 2 for 16. Against queries as
-// the 16 rows (most of them padding at 4 query heads per kv head) this halves products, exponentials
-// and accumulators; P^T moves from accumulator to operand layout by an 8 x 8 transpose in registers.
-// merge buffer: [NW][8 NQ][DP] fp32 (columns permuted by row against bank conflicts), then (m, l).
-template <int DP, int NW, int NST, int NQ>
+// Each warp owns whole stages. The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that positions
+// and head columns fill the instruction's 16 rows and the query rows its 8 columns. Against queries as the 16
+// rows (most of them padding at 4 query heads per kv head) this halves products, exponentials and
+// accumulators; P^T moves from accumulator to operand layout by an 8 x 8 transpose in registers.
+// merge_o is [NW][8][DP] fp32, columns permuted by row against bank conflicts; merge_ml (m, l).
+template <int DP, int NW, int NST>
 __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned char *ring, uint64_t *full,
                               uint64_t *empty, Ring<NST> &r, Waiter &wait, int cw, float *merge_o, float2 *merge_ml,
                               int *flag_s) {
-    constexpr int NB = DP / 64, UPOS = SMALL_STAGE / (4 * DP), MT = UPOS / 16, KS = DP / 16, ROWS = 8 * NQ;
+    constexpr int NB = DP / 64, UPOS = SMALL_STAGE / (4 * DP), MT = UPOS / 16, KS = DP / 16;
     const int lane = threadIdx.x % 32, g = lane / 4, tq = lane % 4, l7 = lane % 8, mi = lane / 8;
     const int rows = p.n_tok * a.rep;
-    uint32_t qb[NQ][KS][2];
-    int lim[NQ][2];
-#pragma unroll
-    for (int n = 0; n < NQ; n++) {
-        const int row = 8 * n + g;
-        const bf16 *src = a.q + (p.tok0 + row / a.rep) * a.q_stride + (long long)(p.kvh * a.rep + row % a.rep) * a.head_dim;
+    uint32_t qb[KS][2];
+    {
+        const bf16 *src = a.q + (p.tok0 + g / a.rep) * a.q_stride + (long long)(p.kvh * a.rep + g % a.rep) * a.head_dim;
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int col = 16 * k + 8 * j + 2 * tq;
-                qb[n][k][j] = row < rows && col < a.head_dim ? *reinterpret_cast<const uint32_t *>(src + col) : 0u;
+                qb[k][j] = g < rows && col < a.head_dim ? *reinterpret_cast<const uint32_t *>(src + col) : 0u;
             }
-#pragma unroll
-        for (int e = 0; e < 2; e++) lim[n][e] = min(p.pos0 + (8 * n + 2 * tq + e) / a.rep + 1, p.kv1);
     }
-    const int lim_min = min(first_masked(p), p.kv1);  // a step may reach past the piece, where nothing was loaded
-    float o[NQ][KS][4], m[NQ][2], l[NQ][2];  // o: columns 16 i + g and + 8 of rows 2 tq, 2 tq + 1
+    // rows 2 tq and 2 tq + 1 are this thread's columns of S^T and O^T; the last step may reach past the piece, where
+    // nothing was loaded
+    const int lim[2] = {min(p.pos0 + 2 * tq / a.rep + 1, p.kv1), min(p.pos0 + (2 * tq + 1) / a.rep + 1, p.kv1)};
+    const int lim_min = min(first_masked(p), p.kv1);
+    float o[KS][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // o: head columns 16 i + g and + 8
 #pragma unroll
-    for (int n = 0; n < NQ; n++) {
-#pragma unroll
-        for (int i = 0; i < KS; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
-        m[n][0] = m[n][1] = -INFINITY;
-        l[n][0] = l[n][1] = 0.0f;
-    }
+    for (int i = 0; i < KS; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
     // ldmatrix rows of this lane: K as [position][column] (operand rows = positions), V transposed
     const uint32_t k_row = ((mi & 1) * 8 + l7) * 128, v_row = ((mi >> 1) * 8 + l7) * 128;
 
@@ -339,11 +332,9 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
             const uint32_t kb = smem_u32(stage), vb = kb + NB * UPOS * 128;
             wait(&full[r.s], r.ph);
             __syncwarp();
-            float s[NQ][MT][4];
+            float s[MT][4];
 #pragma unroll
-            for (int n = 0; n < NQ; n++)
-#pragma unroll
-                for (int i = 0; i < MT; i++) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0.0f;
+            for (int i = 0; i < MT; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 const int c = 2 * k + (mi >> 1);
@@ -352,50 +343,46 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
                 for (int i = 0; i < MT; i++) {
                     uint32_t ka[4];
                     ldsm4(ka, at + i * 16 * 128);
-#pragma unroll
-                    for (int n = 0; n < NQ; n++) mma16816(s[n][i], ka, qb[n][k][0], qb[n][k][1]);
+                    mma16816(s[i], ka, qb[k][0], qb[k][1]);
                 }
             }
             const bool masked = p0 + UPOS > lim_min;
+            float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int n = 0; n < NQ; n++) {
-                float x[2] = {-INFINITY, -INFINITY};
+            for (int i = 0; i < MT; i++)
 #pragma unroll
-                for (int i = 0; i < MT; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        s[n][i][j] *= a.scale_log2;
-                        if (masked && p0 + 16 * i + 8 * (j >> 1) + g >= lim[n][j & 1]) s[n][i][j] = -INFINITY;
-                        x[j & 1] = fmaxf(x[j & 1], s[n][i][j]);
-                    }
-#pragma unroll
-                for (int off = 4; off < 32; off *= 2) {
-                    x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], off));
-                    x[1] = fmaxf(x[1], __shfl_xor_sync(0xffffffffu, x[1], off));
+                for (int j = 0; j < 4; j++) {
+                    s[i][j] *= a.scale_log2;
+                    if (masked && p0 + 16 * i + 8 * (j >> 1) + g >= lim[j & 1]) s[i][j] = -INFINITY;
+                    x[j & 1] = fmaxf(x[j & 1], s[i][j]);
                 }
-                if (__any_sync(0xffffffffu, x[0] > m[n][0] || x[1] > m[n][1])) {
-                    float f[2];
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const float top = fmaxf(m[n][e], x[e]);
-                        f[e] = top == -INFINITY ? 1.0f : ex2(m[n][e] - top);
-                        m[n][e] = top;
-                        l[n][e] *= f[e];
-                    }
-#pragma unroll
-                    for (int i = 0; i < KS; i++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) o[n][i][j] *= f[j & 1];
-                }
-                const float base[2] = {m[n][0] == -INFINITY ? 0.0f : m[n][0], m[n][1] == -INFINITY ? 0.0f : m[n][1]};
-#pragma unroll
-                for (int i = 0; i < MT; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        s[n][i][j] = ex2(s[n][i][j] - base[j & 1]);
-                        l[n][j & 1] += s[n][i][j];
-                    }
+            for (int off = 4; off < 32; off *= 2) {
+                x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], off));
+                x[1] = fmaxf(x[1], __shfl_xor_sync(0xffffffffu, x[1], off));
             }
+            if (__any_sync(0xffffffffu, x[0] > m[0] || x[1] > m[1])) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float top = fmaxf(m[e], x[e]);
+                    f[e] = top == -INFINITY ? 1.0f : ex2(m[e] - top);
+                    m[e] = top;
+                    l[e] *= f[e];
+                }
+#pragma unroll
+                for (int i = 0; i < KS; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[i][j] *= f[j & 1];
+            }
+            const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    s[i][j] = ex2(s[i][j] - base[j & 1]);
+                    l[j & 1] += s[i][j];
+                }
             bool touched = false, slow = false;
             if (p0 + UPOS > p.kv1) {  // rows past the end: zero
                 const int t0 = max(0, p.kv1 - p0), n = (UPOS - t0) * 8;
@@ -415,30 +402,21 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
             if (!slow) {
 #pragma unroll
                 for (int t = 0; t < MT; t++) {
-                    uint32_t pb[NQ][2];
-#pragma unroll
-                    for (int n = 0; n < NQ; n++) {
-                        pb[n][0] = transpose8(pack_bf16(s[n][t][0], s[n][t][1]));
-                        pb[n][1] = transpose8(pack_bf16(s[n][t][2], s[n][t][3]));
-                    }
+                    const uint32_t pb0 = transpose8(pack_bf16(s[t][0], s[t][1])), pb1 = transpose8(pack_bf16(s[t][2], s[t][3]));
 #pragma unroll
                     for (int i = 0; i < KS; i++) {
                         const int c = 2 * i + (mi & 1);
                         uint32_t va[4];
                         ldsm4_t(va, vb + v_row + t * 16 * 128 + (i / 4) * (UPOS * 128) + (((c % 8) ^ l7) << 4));
-#pragma unroll
-                        for (int n = 0; n < NQ; n++) mma16816(o[n][i], va, pb[n][0], pb[n][1]);
+                        mma16816(o[i], va, pb0, pb1);
                     }
                 }
             } else {  // the probabilities take K's place in the stage; then position by position
                 float *ps = reinterpret_cast<float *>(stage);
 #pragma unroll
-                for (int n = 0; n < NQ; n++)
+                for (int i = 0; i < MT; i++)
 #pragma unroll
-                    for (int i = 0; i < MT; i++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            ps[(16 * i + 8 * (j >> 1) + g) * ROWS + 8 * n + 2 * tq + (j & 1)] = s[n][i][j];
+                    for (int j = 0; j < 4; j++) ps[(16 * i + 8 * (j >> 1) + g) * SMALL_ROWS + 2 * tq + (j & 1)] = s[i][j];
                 touched = true;
                 __syncwarp();
 #pragma unroll 1
@@ -449,14 +427,12 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
                         v[c] = __bfloat162float(*reinterpret_cast<const bf16 *>(
                             stage + (NB + c / 8) * (UPOS * 128) + t * 128 + (((c % 8) ^ (t & 7)) << 4) + 2 * g));
 #pragma unroll
-                    for (int n = 0; n < NQ; n++)
+                    for (int e = 0; e < 2; e++) {
+                        if (p0 + t >= lim[e]) continue;
+                        const float w = ps[t * SMALL_ROWS + 2 * tq + e];
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            if (p0 + t >= lim[n][e]) continue;
-                            const float w = ps[t * ROWS + 8 * n + 2 * tq + e];
-#pragma unroll
-                            for (int c = 0; c < 2 * KS; c++) o[n][c / 2][c % 2 * 2 + e] += w * v[c];
-                        }
+                        for (int c = 0; c < 2 * KS; c++) o[c / 2][c % 2 * 2 + e] += w * v[c];
+                    }
                 }
                 __syncwarp();
             }
@@ -470,55 +446,57 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
 
     // ---- merge the warps
 #pragma unroll
-    for (int n = 0; n < NQ; n++) {
+    for (int off = 4; off < 32; off *= 2) {
+        l[0] += __shfl_xor_sync(0xffffffffu, l[0], off);
+        l[1] += __shfl_xor_sync(0xffffffffu, l[1], off);
+    }
 #pragma unroll
-        for (int off = 4; off < 32; off *= 2) {
-            l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], off);
-            l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], off);
-        }
+    for (int e = 0; e < 2; e++) {
+        const int row = 2 * tq + e;
+        if (row < rows) {
+            float *dst = merge_o + (cw * SMALL_ROWS + row) * DP;
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int row = 8 * n + 2 * tq + e;
-            if (row < rows) {
-                float *dst = merge_o + (cw * ROWS + row) * DP;
-#pragma unroll
-                for (int i = 0; i < KS; i++) {
-                    dst[(16 * i + g) ^ (tq * 8)] = o[n][i][e];
-                    dst[(16 * i + 8 + g) ^ (tq * 8)] = o[n][i][2 + e];
-                }
-                if (g == 0) merge_ml[cw * ROWS + row] = make_float2(m[n][e], l[n][e]);
+            for (int i = 0; i < KS; i++) {
+                dst[(16 * i + g) ^ (tq * 8)] = o[i][e];
+                dst[(16 * i + 8 + g) ^ (tq * 8)] = o[i][2 + e];
             }
+            if (g == 0) merge_ml[cw * SMALL_ROWS + row] = make_float2(m[e], l[e]);
         }
     }
     bar_sync(1, NW * 32);
     const int tid = cw * 32 + lane;
+    // four columns of a row of the output; a row without positions is zero
+    auto put = [&](int row, int d, const float *acc, float sum) {
+        const float inv = 1.0f / sum;
+        bf16 *dst = a.out + (p.tok0 + row / a.rep) * a.out_stride + (long long)(p.kvh * a.rep + row % a.rep) * a.head_dim + d;
+        if (d < a.head_dim)
+            *reinterpret_cast<uint2 *>(dst) =
+                p.pos0 + row / a.rep < 0 ? make_uint2(0u, 0u)
+                                         : make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+    };
     for (int i = tid; i < rows * (DP / 4); i += NW * 32) {
         const int row = i / (DP / 4), d = i % (DP / 4) * 4;
-        float m = -INFINITY, l = 0.0f, acc[4] = {};
+        float top = -INFINITY, sum = 0.0f, acc[4] = {};
 #pragma unroll
-        for (int w = 0; w < NW; w++) m = fmaxf(m, merge_ml[w * ROWS + row].x);
-        const float base = m == -INFINITY ? 0.0f : m;
+        for (int w = 0; w < NW; w++) top = fmaxf(top, merge_ml[w * SMALL_ROWS + row].x);
+        const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float2 ml = merge_ml[w * ROWS + row];
+            const float2 ml = merge_ml[w * SMALL_ROWS + row];
             const float f = ex2(ml.x - base);
-            const float4 v = *reinterpret_cast<const float4 *>(merge_o + (w * ROWS + row) * DP + (d ^ ((row >> 1 & 3) * 8)));
-            l += f * ml.y;
+            const float4 v = *reinterpret_cast<const float4 *>(merge_o + (w * SMALL_ROWS + row) * DP + (d ^ ((row >> 1 & 3) * 8)));
+            sum += f * ml.y;
             acc[0] += f * v.x;
             acc[1] += f * v.y;
             acc[2] += f * v.z;
             acc[3] += f * v.w;
         }
         if (p.part < 0) {
-            const float inv = p.pos0 + row / a.rep < 0 ? 0.0f : 1.0f / l;  // a row without positions is zero
-            if (d < a.head_dim) {
-                bf16 *dst = a.out + (p.tok0 + row / a.rep) * a.out_stride + (long long)(p.kvh * a.rep + row % a.rep) * a.head_dim + d;
-                *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
-            }
+            put(row, d, acc, sum);
         } else {
             const size_t at = (size_t)p.part * SMALL_ROWS + row;
             __stcg(reinterpret_cast<float4 *>(a.small_o + at * DP + d), make_float4(acc[0], acc[1], acc[2], acc[3]));
-            if (d == 0) __stcg(a.small_ml + at, make_float2(m, l));
+            if (d == 0) __stcg(a.small_ml + at, make_float2(top, sum));
         }
     }
     if (p.part >= 0) {  // the item's last piece to finish adds the parts up, in their order
@@ -530,27 +508,23 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
             __threadfence();
             for (int i = tid; i < rows * (DP / 4); i += NW * 32) {
                 const int row = i / (DP / 4), d = i % (DP / 4) * 4;
-                float m = -INFINITY, l = 0.0f, acc[4] = {};
+                float top = -INFINITY, sum = 0.0f, acc[4] = {};
                 for (int w = 0; w < p.n_parts; w++)
-                    m = fmaxf(m, __ldcg(a.small_ml + (size_t)part_slot(p.first, w) * SMALL_ROWS + row).x);
-                const float base = m == -INFINITY ? 0.0f : m;
+                    top = fmaxf(top, __ldcg(a.small_ml + (size_t)part_slot(p.first, w) * SMALL_ROWS + row).x);
+                const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll 4
                 for (int w = 0; w < p.n_parts; w++) {
                     const size_t at = (size_t)part_slot(p.first, w) * SMALL_ROWS + row;
                     const float2 ml = __ldcg(a.small_ml + at);
                     const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.small_o + at * DP + d));
                     const float f = ex2(ml.x - base);
-                    l += f * ml.y;
+                    sum += f * ml.y;
                     acc[0] += f * v.x;
                     acc[1] += f * v.y;
                     acc[2] += f * v.z;
                     acc[3] += f * v.w;
                 }
-                const float inv = p.pos0 + row / a.rep < 0 ? 0.0f : 1.0f / l;
-                if (d < a.head_dim) {
-                    bf16 *dst = a.out + (p.tok0 + row / a.rep) * a.out_stride + (long long)(p.kvh * a.rep + row % a.rep) * a.head_dim + d;
-                    *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
-                }
+                put(row, d, acc, sum);
             }
             if (tid == 0) a.counters[p.first] = 0;
         }
@@ -560,32 +534,26 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
 
 // ---------------------------------------------------------------- kernel for few rows alone
 
-// NQ: query rows in eights. Warps and stages share the SM's registers and shared memory.
-template <int NQ>
-struct SmallShape {
-    static constexpr int WARPS = NQ == 1 ? 10 : 8, STAGES = NQ == 1 ? 10 : 8;
-};
+constexpr int SMALL_WARPS = 10, SMALL_STAGES = 10;
 
-template <int DP, int NQ>
+template <int DP>
 struct SmallSmem {
-    static constexpr int NW = SmallShape<NQ>::WARPS, NST = SmallShape<NQ>::STAGES;
-    alignas(1024) unsigned char ring[NST * SMALL_STAGE];
-    float merge_o[NW * 8 * NQ * DP];
-    float2 merge_ml[NW * 8 * NQ];
-    uint64_t full[NST], empty[NST];
+    alignas(1024) unsigned char ring[SMALL_STAGES * SMALL_STAGE];
+    float merge_o[SMALL_WARPS * SMALL_ROWS * DP];
+    float2 merge_ml[SMALL_WARPS * SMALL_ROWS];
+    uint64_t full[SMALL_STAGES], empty[SMALL_STAGES];
     int flag;
 };
 
-template <int DP, int NQ>
-__global__ void __launch_bounds__((SMALL_PRODUCERS + SmallShape<NQ>::WARPS) * 32, 1)
+template <int DP>
+__global__ void __launch_bounds__((SMALL_PRODUCERS + SMALL_WARPS) * 32, 1)
     paged_small_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                        const __grid_constant__ PaArgs a) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    constexpr int NW = SmallShape<NQ>::WARPS, NST = SmallShape<NQ>::STAGES;
-    SmallSmem<DP, NQ> &sm = *reinterpret_cast<SmallSmem<DP, NQ> *>(align_shared<1024>(smem_raw));
+    SmallSmem<DP> &sm = *reinterpret_cast<SmallSmem<DP> *>(align_shared<1024>(smem_raw));
     const int warp = threadIdx.x / 32;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < NST; i++) {
+        for (int i = 0; i < SMALL_STAGES; i++) {
             mbar_init(&sm.full[i], 1);
             mbar_init(&sm.empty[i], 1);
         }
@@ -600,17 +568,17 @@ __global__ void __launch_bounds__((SMALL_PRODUCERS + SmallShape<NQ>::WARPS) * 32
     if (!a.after_big) pdl_wait();
     const int2 work = a.ctas[blockIdx.x];
     if (work.y < 0) zero_rows(a);
-    Ring<NST> r;
+    Ring<SMALL_STAGES> r;
     Waiter wait;
-    if (warp >= NW) {
-        for (int i = 0; i < work.y; i++)
-            small_produce<DP, NST, SMALL_PRODUCERS>(a, &mk, &mv, a.pieces[work.x + i], sm.ring, sm.full, sm.empty, r,
-                                                                 warp - NW, wait, a.small_step_pages, a.small_step_slots);
+    for (int i = 0; i < work.y; i++) {
+        const PagedPiece p = a.pieces[work.x + i];
         // every load is waited for by a consumer before the CTA ends
-    } else {
-        for (int i = 0; i < work.y; i++)
-            small_consume<DP, NW, NST, NQ>(a, a.pieces[work.x + i], sm.ring, sm.full, sm.empty, r, wait, warp, sm.merge_o,
-                                           sm.merge_ml, &sm.flag);
+        if (warp >= SMALL_WARPS)
+            small_produce<DP, SMALL_STAGES, SMALL_PRODUCERS>(a, &mk, &mv, p, sm.ring, sm.full, sm.empty, r, warp - SMALL_WARPS, wait,
+                                                             a.small_step_pages, a.small_step_slots);
+        else
+            small_consume<DP, SMALL_WARPS, SMALL_STAGES>(a, p, sm.ring, sm.full, sm.empty, r, wait, warp, sm.merge_o, sm.merge_ml,
+                                                         &sm.flag);
     }
     if (a.after_big) pdl_wait();  // whoever waits for this kernel waits for that one, too
 }
@@ -861,6 +829,13 @@ __device__ __forceinline__ float exp64(uint32_t ts, int seen, uint64_t c2, uint6
     return w.x + w.y;
 }
 
+// Where a partial result keeps columns d .. d + 3 of a row, in scratch slot `slot`: four columns of all rows side by
+// side, so that a warp's 32 rows are one run of memory (row by row, its accesses took a sector each, and 20 us a piece).
+template <int DP>
+__device__ __forceinline__ float4 *big_part(const PaArgs &a, int slot, int d, size_t row) {
+    return reinterpret_cast<float4 *>(a.big_o + (size_t)slot * (2 * BIG_TILE) * DP) + (size_t)(d / 4) * (2 * BIG_TILE) + row;
+}
+
 // Two warpgroups per tile, two threads per row: each takes 64 of a step's columns and half of the output's.
 template <int DP>
 __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, BigSmem<DP> &sm, uint32_t tmem, int x, int part,
@@ -1005,40 +980,99 @@ __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, BigSmem<DP> &s
     tc_fence_after();
     const bool valid = row / a.rep < a.tile_tok && tt < p.n_tok;
     const int head = p.kvh * a.rep + row % a.rep;
-    if (p.part < 0) {
-        const float inv = 1.0f / l;
-        bf16 *dst = a.out + (p.tok0 + tt) * a.out_stride + (long long)head * a.head_dim;
-#pragma unroll
-        for (int i = 0; i < DP / 64; i++) {
-            uint32_t o[32];
-            tmem_ld32(to + 32 * i, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                uint32_t w[4];
-#pragma unroll
-                for (int q = 0; q < 4; q++)
-                    w[q] = pack_bf16(__uint_as_float(o[8 * e + 2 * q]) * inv, __uint_as_float(o[8 * e + 2 * q + 1]) * inv);
-                const int d = part * (DP / 2) + 32 * i + 8 * e;
-                if (valid && d < a.head_dim)  // a row without positions is zero
-                    *reinterpret_cast<uint4 *>(dst + d) = lim <= 0 ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-    } else {
-        const size_t at = (size_t)p.part * (2 * BIG_TILE) + x * BIG_TILE + row;
+    const size_t at = (size_t)x * BIG_TILE + row;  // this row in a scratch slot
+    bool last = p.part < 0;
+    if (p.part >= 0) {
 #pragma unroll
         for (int i = 0; i < DP / 64; i++) {
             uint32_t o[32];
             tmem_ld32(to + 32 * i, o);
             tmem_wait_ld();
             if (valid) {
+                uint4 *dst = reinterpret_cast<uint4 *>(big_part<DP>(a, p.part, part * (DP / 2) + 32 * i, at));
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                    __stcg(reinterpret_cast<uint4 *>(a.big_o + at * DP + part * (DP / 2) + 32 * i) + e,
-                           make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
+                    __stcg(dst + e * (2 * BIG_TILE), make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
             }
         }
-        if (valid && part == 0) __stcg(a.big_ml + at, make_float2(m, l));
+        if (valid && part == 0) __stcg(a.big_ml + (size_t)p.part * (2 * BIG_TILE) + at, make_float2(m, l));
+        if (p.n_parts <= MERGE_PARTS) {  // the tile's last piece to finish adds the parts up; of more, the combine kernel does
+            __threadfence();
+            bar_sync(9 + x, 256);
+            if (row == 0 && part == 0) {
+                int *done = a.counters + (1 + x) * PAGED_MAX_CTAS + p.first;
+                const bool all = atomicAdd(done, 1) == p.n_parts - 1;
+                if (all) *done = 0;
+                sm.slow[x] = all;
+            }
+            bar_sync(9 + x, 256);
+            last = *(const volatile int *)&sm.slow[x];
+            __threadfence();
+        }
+    }
+    if (last) {
+        // weights of the parts, in their order; a whole item is its only part
+        const int parts = p.part < 0 ? 1 : p.n_parts, own = p.part < 0 ? 0 : p.part == part_slot(p.first, 0) ? 0 : p.part / 2 - p.first;
+        float weight[MERGE_PARTS] = {1.0f, 0.0f};
+        float sum = l;
+        if (parts > 1) {
+            float2 ml[MERGE_PARTS];
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < MERGE_PARTS; w++) {
+                ml[w] = make_float2(-INFINITY, 0.0f);
+                if (w == own) ml[w] = make_float2(m, l);
+                else if (w < parts && valid) ml[w] = __ldcg(a.big_ml + (size_t)part_slot(p.first, w) * (2 * BIG_TILE) + at);
+                top = fmaxf(top, ml[w].x);
+            }
+            const float base = top == -INFINITY ? 0.0f : top;
+            sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < MERGE_PARTS; w++) {
+                weight[w] = ex2(ml[w].x - base);
+                sum += weight[w] * ml[w].y;
+            }
+        }
+        const float inv = 1.0f / sum;
+        bf16 *dst = a.out + (p.tok0 + tt) * a.out_stride + (long long)head * a.head_dim;
+#pragma unroll 1
+        for (int i = 0; i < DP / 32; i++) {
+            float mine[16], acc[16];
+            __syncwarp();
+            tmem_ld8(to + 16 * i, mine);
+            tmem_ld8(to + 16 * i + 8, mine + 8);
+            tmem_wait_ld();
+            if (parts == 1) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[e] = mine[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[e] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < MERGE_PARTS; w++) {
+                    if (w >= parts) continue;
+                    const float4 *src = big_part<DP>(a, part_slot(p.first, w), part * (DP / 2) + 16 * i, at);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        float4 v = make_float4(mine[4 * q], mine[4 * q + 1], mine[4 * q + 2], mine[4 * q + 3]);
+                        if (w != own && valid) v = __ldcg(src + q * (2 * BIG_TILE));
+                        acc[4 * q] += weight[w] * v.x;
+                        acc[4 * q + 1] += weight[w] * v.y;
+                        acc[4 * q + 2] += weight[w] * v.z;
+                        acc[4 * q + 3] += weight[w] * v.w;
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                uint32_t w[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) w[q] = pack_bf16(acc[8 * e + 2 * q] * inv, acc[8 * e + 2 * q + 1] * inv);
+                const int d = part * (DP / 2) + 16 * i + 8 * e;
+                if (valid && d < a.head_dim)  // a row without positions is zero
+                    *reinterpret_cast<uint4 *>(dst + d) = lim <= 0 ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
     }
     tc_fence_before();
     bar_sync(1 + x * 4 + quarter, 64);  // the sums have been read
@@ -1128,41 +1162,45 @@ __global__ void __launch_bounds__(BIG_THREADS, 1)
     }
 }
 
-// Adds up the parts of the big items that were cut: a CTA per (item, 32 rows), a warp per row.
+// Adds up the parts of big items that were cut into many: a CTA per item and 16 columns, a thread per row.
 template <int DP>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ PaArgs a) {
+__global__ void __launch_bounds__(2 * BIG_TILE) paged_combine_kernel(const __grid_constant__ PaArgs a) {
     pdl_trigger();
     pdl_wait();
     const PagedPiece p = a.splits[blockIdx.x];
     if (p.n_parts < 2) return;
-    const int lane = threadIdx.x % 32, d = lane * (DP / 32);
-    for (int i = 0; i < 4; i++) {
-        const int row = blockIdx.y * 32 + i * 8 + threadIdx.x / 32, x = row / BIG_TILE, rr = row % BIG_TILE;
-        const int tt = x * a.tile_tok + rr / a.rep;
-        if (rr / a.rep >= a.tile_tok || tt >= p.n_tok) continue;
-        float m = -INFINITY, l = 0.0f, acc[DP / 32] = {};
-        for (int w = 0; w < p.n_parts; w++)
-            m = fmaxf(m, __ldcg(a.big_ml + (size_t)part_slot(p.first, w) * (2 * BIG_TILE) + row).x);
-        const float base = m == -INFINITY ? 0.0f : m;
+    const int row = threadIdx.x, x = row / BIG_TILE, rr = row % BIG_TILE, d = blockIdx.y * 16;
+    const int tt = x * a.tile_tok + rr / a.rep;
+    if (rr / a.rep >= a.tile_tok || tt >= p.n_tok || d >= a.head_dim) return;
+    float m = -INFINITY;
 #pragma unroll 4
-        for (int w = 0; w < p.n_parts; w++) {
-            const size_t at = (size_t)part_slot(p.first, w) * (2 * BIG_TILE) + row;
-            const float2 ml = __ldcg(a.big_ml + at);
-            const float f = ex2(ml.x - base);
-            l += f * ml.y;
+    for (int w = 0; w < p.n_parts; w++) m = fmaxf(m, __ldcg(a.big_ml + (size_t)part_slot(p.first, w) * (2 * BIG_TILE) + row).x);
+    float l = 0.0f, acc[16] = {};
+    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll 4
+    for (int w = 0; w < p.n_parts; w++) {
+        const float2 ml = __ldcg(a.big_ml + (size_t)part_slot(p.first, w) * (2 * BIG_TILE) + row);
+        const float4 *src = big_part<DP>(a, part_slot(p.first, w), d, row);
+        const float f = ex2(ml.x - base);
+        l += f * ml.y;
 #pragma unroll
-            for (int e = 0; e < DP / 32; e += 2) {
-                const float2 v = __ldcg(reinterpret_cast<const float2 *>(a.big_o + at * DP + d + e));
-                acc[e] += f * v.x;
-                acc[e + 1] += f * v.y;
-            }
+        for (int q = 0; q < 4; q++) {
+            const float4 v = __ldcg(src + q * (2 * BIG_TILE));
+            acc[4 * q] += f * v.x;
+            acc[4 * q + 1] += f * v.y;
+            acc[4 * q + 2] += f * v.z;
+            acc[4 * q + 3] += f * v.w;
         }
-        const float inv = 1.0f / l;
-        bf16 *dst = a.out + (p.tok0 + tt) * a.out_stride + (long long)(p.kvh * a.rep + rr % a.rep) * a.head_dim + d;
+    }
+    const float inv = 1.0f / l;
+    bf16 *dst = a.out + (p.tok0 + tt) * a.out_stride + (long long)(p.kvh * a.rep + rr % a.rep) * a.head_dim + d;
 #pragma unroll
-        for (int e = 0; e < DP / 32; e += 2)
-            if (d + e < a.head_dim)
-                *reinterpret_cast<uint32_t *>(dst + e) = p.pos0 + tt < 0 ? 0u : pack_bf16(acc[e] * inv, acc[e + 1] * inv);
+    for (int e = 0; e < 2; e++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) w[q] = pack_bf16(acc[8 * e + 2 * q] * inv, acc[8 * e + 2 * q + 1] * inv);
+        if (d + 8 * e < a.head_dim)  // a row without positions is zero
+            reinterpret_cast<uint4 *>(dst)[e] = p.pos0 + tt < 0 ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -1194,15 +1232,6 @@ bool make_query_map(CUtensorMap *map, const PagedAttnCall &c, const PaArgs &a) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DP, int NQ>
-int run_small(const CUtensorMap &mk, const CUtensorMap &mv, const PaArgs &a, cudaStream_t s) {
-    const size_t smem = sizeof(SmallSmem<DP, NQ>) + 1024;
-    auto kernel = paged_small_kernel<DP, NQ>;
-    Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(kernel), smem));
-    Q3_TRY_LAUNCH(launch(kernel, dim3(paged_ctas()), dim3((SMALL_PRODUCERS + SmallShape<NQ>::WARPS) * 32), smem, s, 1, mk, mv, a));
-    return Q3_OK;
-}
-
 template <int DP>
 int run(const PagedAttnCall &c, PaArgs &a, cudaStream_t s) {
     CUtensorMap mk, mv;
@@ -1224,13 +1253,16 @@ int run(const PagedAttnCall &c, PaArgs &a, cudaStream_t s) {
         const uint32_t kinds = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BIG_TILE >> 4) << 24);
         a.idesc_qk = kinds | ((uint32_t)(BIG_TILE >> 3) << 17) | (c.scale < 0.0f ? 1u << 13 : 0u);
         a.idesc_pv = kinds | ((uint32_t)(DP >> 3) << 17) | (1u << 16);
-        const size_t smem = sizeof(BigSmem<DP>);
-        Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_big_kernel<DP>), smem));
-        Q3_TRY_LAUNCH(launch(paged_big_kernel<DP>, dim3(paged_ctas()), dim3(BIG_THREADS), smem, s, 1, mq, mk_big, mv_big, a));
+        const size_t big_smem = sizeof(BigSmem<DP>);
+        Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_big_kernel<DP>), big_smem));
+        Q3_TRY_LAUNCH(launch(paged_big_kernel<DP>, dim3(paged_ctas()), dim3(BIG_THREADS), big_smem, s, 1, mq, mk_big, mv_big, a));
     }
-    const int st = std::min(c.shape.max_q_len * a.rep, SMALL_ROWS) <= 8 ? run_small<DP, 1>(mk, mv, a, s) : run_small<DP, 2>(mk, mv, a, s);
-    if (st != Q3_OK || !a.after_big) return st;
-    Q3_TRY_LAUNCH(launch(paged_combine_kernel<DP>, dim3(paged_ctas(), 2 * BIG_TILE / 32), dim3(256), 0, s, 1, a));
+    const size_t smem = sizeof(SmallSmem<DP>) + 1024;
+    Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_small_kernel<DP>), smem));
+    Q3_TRY_LAUNCH(launch(paged_small_kernel<DP>, dim3(paged_ctas()), dim3((SMALL_PRODUCERS + SMALL_WARPS) * 32), smem, s, 1, mk,
+                         mv, a));
+    if (!a.after_big) return Q3_OK;
+    Q3_TRY_LAUNCH(launch(paged_combine_kernel<DP>, dim3(paged_ctas(), DP / 16), dim3(2 * BIG_TILE), 0, s, 1, a));
     return Q3_OK;
 }
 

@@ -10,9 +10,19 @@ import ctypes
 
 import numpy as np
 
-from ._lib import Q3Error, call, load
+from ._lib import Q3Error, call, check, load
 
 _SHAPE, _ARG = 1, 5
+_torch = None
+
+
+def _t():
+    """torch, imported when the first tensor arrives."""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch
 
 
 class Q3PagedShape(ctypes.Structure):
@@ -37,18 +47,26 @@ ROPE_KINDS = {"plain": 0, "linear": 1, "by_parts": 2, "yarn": 3}
 def _stream(stream):
     if stream is not None:
         return stream
-    import torch
-    return torch.cuda.current_stream().cuda_stream
+    raw = getattr(_t()._C, "_cuda_getCurrentRawStream", None)  # the stream's handle without an object around it
+    if raw is None:
+        return _torch.cuda.current_stream().cuda_stream
+    return raw(_torch.cuda.current_device())
 
 
 def _refuse(name, what, status=_ARG):
     raise Q3Error(name, status, what)
 
 
-def _rows(name, t, what, width, dtype):
+# These calls run once per layer of every step, so the checks read as few tensor attributes as they can.
+
+def _rows(name, t, what, rows, width, dtype):
     """Row stride of a [rows, ...] tensor whose rows are `width` contiguous elements."""
-    if t.dtype != dtype or not t.is_cuda:
+    if t.dtype is not dtype or not t.is_cuda:
         _refuse(name, f"{what} must be a CUDA tensor of {dtype}")
+    if t.is_contiguous() and t.numel() == rows * width and len(t) == rows:
+        return width
+    if t.dim() == 0 or len(t) != rows:
+        _refuse(name, f"{what}: {tuple(t.shape)}, expected {rows} rows", _SHAPE)
     n = 1
     for size, step in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
         if size != 1 and step != n:
@@ -56,13 +74,13 @@ def _rows(name, t, what, width, dtype):
         n *= size
     if n != width:
         _refuse(name, f"{what}: {n} elements a row, expected {width}", _SHAPE)
-    return t.stride(0) if t.shape[0] > 1 else width
+    return t.stride(0) if rows > 1 else width
 
 
 def _vector(name, t, what, size, dtype):
     if t is None:
         return None
-    if t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
+    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
         _refuse(name, f"{what} must be a contiguous CUDA tensor of {dtype}")
     if size is not None and t.numel() != size:
         _refuse(name, f"{what}: {t.numel()} elements, expected {size}", _SHAPE)
@@ -76,7 +94,7 @@ class PagedPlan:
 
     def __init__(self, n_seqs: int, n_tokens: int, max_q_len: int, n_heads: int, n_kv_heads: int, head_dim: int,
                  page_size: int, n_pages: int, max_pages: int, device="cuda"):
-        import torch
+        torch = _t()
         self.shape = Q3PagedShape(n_seqs, n_tokens, max_q_len, n_heads, n_kv_heads, head_dim, page_size, n_pages,
                                   max_pages)
         self._shape = ctypes.byref(self.shape)
@@ -86,64 +104,61 @@ class PagedPlan:
         self.plan = torch.empty(n, dtype=torch.uint8, device=device)
         self.scratch = torch.empty(load().q3_paged_attention_scratch_bytes(self._shape), dtype=torch.uint8,
                                    device=device)
-        self._caches = {}
+        self.n_tokens, self.head_dim, self.scale = n_tokens, head_dim, head_dim ** -0.5
+        self.q_width, self.kv_width = n_heads * head_dim, n_kv_heads * head_dim
+        self._pages = (n_pages, n_kv_heads, page_size, head_dim)
+        self._ptr, self._scratch_ptr = self.plan.data_ptr(), self.scratch.data_ptr()
+        self._cache = Q3PagedCache()  # filled anew for every call, which reads it before it returns
+        self._cache_ref = ctypes.byref(self._cache)
 
     def update(self, q_start, kv_len, page_table, stream=None):
-        import torch
-        s, name = self.shape, "q3_paged_plan"
-        call(name, self.plan.data_ptr(), self._shape, _vector(name, q_start, "q_start", s.n_seqs + 1, torch.int32),
-             _vector(name, kv_len, "kv_len", s.n_seqs, torch.int32),
-             _vector(name, page_table, "page_table", s.n_seqs * s.max_pages, torch.int32), _stream(stream))
+        s, name, i32 = self.shape, "q3_paged_plan", _t().int32
+        call(name, self._ptr, self._shape, _vector(name, q_start, "q_start", s.n_seqs + 1, i32),
+             _vector(name, kv_len, "kv_len", s.n_seqs, i32),
+             _vector(name, page_table, "page_table", s.n_seqs * s.max_pages, i32), _stream(stream))
 
-    def cache(self, name, key_pages, value_pages) -> Q3PagedCache:
-        import torch
-        s = self.shape
-        want = (s.n_pages, s.n_kv_heads, s.page_size, s.head_dim)
-        for t in (key_pages, value_pages):
-            if t.dtype != torch.bfloat16 or not t.is_cuda:
-                _refuse(name, "pages must be CUDA tensors of torch.bfloat16")
-            if tuple(t.shape) != want:
-                _refuse(name, f"pages {tuple(t.shape)}, expected {want}", _SHAPE)
-            if t.stride(3) != 1:
-                _refuse(name, "pages: the last dimension must be contiguous")
-        if key_pages.stride() != value_pages.stride():
+    def _bind(self, name, key_pages, value_pages):
+        """The pages as the C struct."""
+        bf16, c = _t().bfloat16, self._cache
+        if key_pages.dtype is not bf16 or value_pages.dtype is not bf16 or not (key_pages.is_cuda and value_pages.is_cuda):
+            _refuse(name, "pages must be CUDA tensors of torch.bfloat16")
+        if key_pages.shape != self._pages or value_pages.shape != self._pages:
+            _refuse(name, f"pages {tuple(key_pages.shape)} and {tuple(value_pages.shape)}, expected {self._pages}", _SHAPE)
+        strides = key_pages.stride()
+        if strides != value_pages.stride():
             _refuse(name, "key and value pages must have the same strides", _SHAPE)
-        return Q3PagedCache(key_pages.data_ptr(), value_pages.data_ptr(), key_pages.stride(0), key_pages.stride(1),
-                            key_pages.stride(2))
-
-
-def _tokens(name, plan, **tensors):
-    for what, t in tensors.items():
-        if t.shape[0] != plan.shape.n_tokens:
-            _refuse(name, f"{what}: {t.shape[0]} rows, the plan has {plan.shape.n_tokens}", _SHAPE)
+        if strides[3] != 1:
+            _refuse(name, "pages: the last dimension must be contiguous")
+        c.key_pages, c.value_pages = key_pages.data_ptr(), value_pages.data_ptr()
+        c.page_stride, c.head_stride, c.pos_stride = strides[0], strides[1], strides[2]
+        return self._cache_ref
 
 
 def paged_rope_append(q_out, q, k, v, key_pages, value_pages, plan: PagedPlan, inv_freq=None, q_norm_w=None,
                       k_norm_w=None, eps: float = 1e-6, interleaved: bool = False, amplitude: float = 1.0, stream=None):
     """Norms, rotary positions and the write into the pages (q3_paged_rope_append). inv_freq holds
     rope_dim / 2 fp32 frequencies on the device (`rope_inv_freq`); None rotates nothing."""
-    import torch
-    name, s, bf = "q3_paged_rope_append", plan.shape, torch.bfloat16
-    qd, kd = s.n_heads * s.head_dim, s.n_kv_heads * s.head_dim
-    _tokens(name, plan, q_out=q_out, q=q, k=k, v=v)
-    call(name, q_out.data_ptr(), _rows(name, q_out, "q_out", qd, bf), q.data_ptr(), _rows(name, q, "q", qd, bf),
-         k.data_ptr(), _rows(name, k, "k", kd, bf), v.data_ptr(), _rows(name, v, "v", kd, bf),
-         _vector(name, q_norm_w, "q_norm_w", s.head_dim, bf), _vector(name, k_norm_w, "k_norm_w", s.head_dim, bf), eps,
-         _vector(name, inv_freq, "inv_freq", None, torch.float32), 0 if inv_freq is None else 2 * inv_freq.numel(),
-         int(interleaved), amplitude, ctypes.byref(plan.cache(name, key_pages, value_pages)), plan._shape,
-         plan.plan.data_ptr(), _stream(stream))
+    name, bf, n, qw, kw = "q3_paged_rope_append", _t().bfloat16, plan.n_tokens, plan.q_width, plan.kv_width
+    status = load().q3_paged_rope_append(
+        q_out.data_ptr(), _rows(name, q_out, "q_out", n, qw, bf), q.data_ptr(), _rows(name, q, "q", n, qw, bf),
+        k.data_ptr(), _rows(name, k, "k", n, kw, bf), v.data_ptr(), _rows(name, v, "v", n, kw, bf),
+        _vector(name, q_norm_w, "q_norm_w", plan.head_dim, bf), _vector(name, k_norm_w, "k_norm_w", plan.head_dim, bf),
+        eps, _vector(name, inv_freq, "inv_freq", None, _torch.float32), 0 if inv_freq is None else 2 * inv_freq.numel(),
+        interleaved, amplitude, plan._bind(name, key_pages, value_pages), plan._shape, plan._ptr, _stream(stream))
+    if status:
+        check(name, status)
 
 
 def paged_attention(out, q, key_pages, value_pages, plan: PagedPlan, scale: float | None = None, stream=None):
     """Attention of the step's new tokens over the pages (q3_paged_attention); scale defaults to
     1 / sqrt(head_dim)."""
-    import torch
-    name, s, bf = "q3_paged_attention", plan.shape, torch.bfloat16
-    qd = s.n_heads * s.head_dim
-    _tokens(name, plan, out=out, q=q)
-    call(name, out.data_ptr(), _rows(name, out, "out", qd, bf), q.data_ptr(), _rows(name, q, "q", qd, bf),
-         ctypes.byref(plan.cache(name, key_pages, value_pages)), s.head_dim ** -0.5 if scale is None else scale,
-         plan._shape, plan.plan.data_ptr(), plan.scratch.data_ptr(), _stream(stream))
+    name, bf, n, qw = "q3_paged_attention", _t().bfloat16, plan.n_tokens, plan.q_width
+    status = load().q3_paged_attention(
+        out.data_ptr(), _rows(name, out, "out", n, qw, bf), q.data_ptr(), _rows(name, q, "q", n, qw, bf),
+        plan._bind(name, key_pages, value_pages), plan.scale if scale is None else scale, plan._shape, plan._ptr,
+        plan._scratch_ptr, _stream(stream))
+    if status:
+        check(name, status)
 
 
 def rope_inv_freq(rope_dim: int, theta: float, kind: str = "plain", **scaling) -> tuple[np.ndarray, float]:
@@ -162,32 +177,33 @@ def logits_process(out, logits, hist_start=None, hist_split=None, hist_ids=None,
                    presence=None, bias_start=None, bias_ids=None, bias=None, mask=None, stream=None):
     """Penalties, biases and grammar masks on [rows, vocab] logits, bf16 or fp32 (q3_logits_process);
     out may be logits. mask is int32 [rows, >= ceil(vocab / 32)], one bit per allowed token."""
-    import torch
-    name = "q3_logits_process"
-    if logits.dim() != 2 or out.shape != logits.shape:
-        _refuse(name, "logits and out must both be [rows, vocab]", _SHAPE)
-    if logits.dtype not in (torch.bfloat16, torch.float32):
+    torch = _t()
+    name, dtype, i32, f32 = "q3_logits_process", logits.dtype, torch.int32, torch.float32
+    if dtype is not torch.bfloat16 and dtype is not f32:
         _refuse(name, "logits must be bfloat16 or float32")
-    rows, vocab = logits.shape
-    i32, f32 = torch.int32, torch.float32
-    mask_stride = 0
+    shape = logits.shape
+    if len(shape) != 2 or out.shape != shape:
+        _refuse(name, "logits and out must both be [rows, vocab]", _SHAPE)
+    rows, vocab = shape
+    mask_ptr, mask_stride = None, 0
     if mask is not None:
-        if mask.dim() != 2 or mask.shape[0] != rows:
-            _refuse(name, "mask must be [rows, words]", _SHAPE)
-        mask_stride = _rows(name, mask, "mask", mask.shape[1], i32)
-        if mask.shape[1] * 32 < vocab:
-            _refuse(name, "mask: too few words a row", _SHAPE)
-    if bias is not None and bias_ids is not None and bias.numel() != bias_ids.numel():
-        _refuse(name, "bias and bias_ids differ in length", _SHAPE)
+        if mask.dim() != 2 or mask.shape[1] * 32 < vocab:
+            _refuse(name, "mask must be [rows, at least vocab / 32 words]", _SHAPE)
+        mask_ptr, mask_stride = mask.data_ptr(), _rows(name, mask, "mask", rows, mask.shape[1], i32)
     if hist_ids is not None and hist_ids.numel() == 0:  # an empty tensor has no address to pass
         hist_start = hist_split = hist_ids = None
-    if bias_ids is not None and bias_ids.numel() == 0:
-        bias_start = bias_ids = bias = None
-    call(name, out.data_ptr(), logits.data_ptr(), int(logits.dtype == f32), rows, vocab,
-         _rows(name, out, "out", vocab, logits.dtype), _rows(name, logits, "logits", vocab, logits.dtype),
-         _vector(name, hist_start, "hist_start", rows + 1, i32), _vector(name, hist_split, "hist_split", rows, i32),
-         _vector(name, hist_ids, "hist_ids", None, i32), _vector(name, repetition, "repetition", rows, f32),
-         _vector(name, frequency, "frequency", rows, f32), _vector(name, presence, "presence", rows, f32),
-         _vector(name, bias_start, "bias_start", rows + 1, i32), _vector(name, bias_ids, "bias_ids", None, i32),
-         _vector(name, bias, "bias", None, f32), None if mask is None else mask.data_ptr(), mask_stride,
-         _stream(stream))
+    if bias_ids is not None:
+        if bias is not None and bias.numel() != bias_ids.numel():
+            _refuse(name, "bias and bias_ids differ in length", _SHAPE)
+        if bias_ids.numel() == 0:
+            bias_start = bias_ids = bias = None
+    status = load().q3_logits_process(
+        out.data_ptr(), logits.data_ptr(), dtype is f32, rows, vocab, _rows(name, out, "out", rows, vocab, dtype),
+        _rows(name, logits, "logits", rows, vocab, dtype), _vector(name, hist_start, "hist_start", rows + 1, i32),
+        _vector(name, hist_split, "hist_split", rows, i32), _vector(name, hist_ids, "hist_ids", None, i32),
+        _vector(name, repetition, "repetition", rows, f32), _vector(name, frequency, "frequency", rows, f32),
+        _vector(name, presence, "presence", rows, f32), _vector(name, bias_start, "bias_start", rows + 1, i32),
+        _vector(name, bias_ids, "bias_ids", None, i32), _vector(name, bias, "bias", None, f32), mask_ptr, mask_stride,
+        _stream(stream))
+    if status:
+        check(name, status)
