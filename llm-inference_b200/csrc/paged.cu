@@ -254,17 +254,20 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
 }
 
 // ------------------------------------------------------------------ append
-// One CTA per token, with a group of lanes for every head where 512 threads are enough for that. A unit is two 8-element chunks of a head that one lane holds in registers: for
-// half-split pairs chunk u and its partner u + rope_dim/16, so a pair's two elements sit in one lane;
-// otherwise neighbours. A head is a group of `lph` lanes (a power of two), so the sum of squares
-// is a few shuffles. The angles depend on the token alone: the CTA computes them once, then every
-// head reads them from shared memory; what the heads hold is asked for before. Bound by the rows' bytes, and for
-// few tokens by the chain plan -> angle -> heads.
+// One CTA per token: 128 threads that take the heads in rounds where tokens are many, a group of lanes for every head
+// (up to 512 threads) where they are few. A unit is two 8-element chunks of a head that one lane holds in
+// registers: for half-split pairs chunk u and its partner u + rope_dim/16, so a pair's two elements sit in one
+// lane; otherwise neighbours. A head is a group of `lph` lanes (a power of two), so the sum of squares is a few
+// shuffles. The angles depend on the token alone: the CTA computes them once, then every lane keeps its pairs' in
+// registers. A lane's first query head and first key or value head are asked for before that.
+//
+// With many tokens the instructions bound it before the bytes do (360 a warp and four heads, 44 us for 8192 tokens of 48
+// heads, before the packed arithmetic and one loop per kind of head); with few, the chain plan -> angle -> heads.
 //
 // The angle is reduced in fp64: pos * inv_freq reaches 10^5 rad and more, where an fp32 product is
 // off by up to 2^-25 of itself, more than a bf16 result may be. turns = pos * inv_freq / 2 pi, its
 // nearest integer dropped, goes to sincospif.
-constexpr int APPEND_MAX_THREADS = 512;
+constexpr int APPEND_MAX_THREADS = 512, APPEND_THREADS = 128;
 constexpr int APPEND_ODD_THREADS = 128;
 
 struct AppendArgs {
@@ -279,21 +282,21 @@ struct AppendArgs {
     float eps, amplitude;
 };
 
-__device__ __forceinline__ void unpack8(const uint4 &u, float *f) {
-    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&u);
+// eight bf16 as four pairs of floats, and back
+__device__ __forceinline__ void unpack8(const uint4 &u, uint64_t *f) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&u);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 p = __bfloat1622float2(h[i]);
-        f[2 * i] = p.x;
-        f[2 * i + 1] = p.y;
-    }
+    for (int i = 0; i < 4; i++) f[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
 
-__device__ __forceinline__ uint4 pack8(const float *f) {
+__device__ __forceinline__ uint4 pack8(const uint64_t *f) {
     uint4 u;
     __nv_bfloat162 *h = reinterpret_cast<__nv_bfloat162 *>(&u);
 #pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    for (int i = 0; i < 4; i++) {
+        const float2 v = unpair(f[i]);
+        h[i] = __floats2bfloat162_rn(v.x, v.y);
+    }
     return u;
 }
 
@@ -307,90 +310,117 @@ __device__ __forceinline__ void rope_angle(int pos, float inv_freq, float amplit
 
 template <bool INTERLEAVED>
 __global__ void __launch_bounds__(APPEND_MAX_THREADS) paged_append_kernel(const __grid_constant__ AppendArgs a) {
-    __shared__ float cos_s[PAGED_MAX_HEAD_DIM / 2], sin_s[PAGED_MAX_HEAD_DIM / 2];
+    // cos and sin of pair j: (cos, cos) and (-sin, sin) interleaved; half split cos, sin and -sin, for two pairs at a time
+    __shared__ __align__(16) float cos_s[PAGED_MAX_HEAD_DIM], sin_s[PAGED_MAX_HEAD_DIM], neg_s[PAGED_MAX_HEAD_DIM / 2];
     pdl_trigger();
     pdl_wait();
-    const int t = blockIdx.x, heads = a.n_heads + 2 * a.n_kv_heads, groups = blockDim.x / a.lph;
+    const int t = blockIdx.x, groups = blockDim.x / a.lph, first = threadIdx.x / a.lph, step = groups * a.head_dim;
     const int u = threadIdx.x % a.lph, half = a.rope_dim / 2, nc = a.head_dim / 8, hc = INTERLEAVED ? 0 : half / 8;
     const int c0 = INTERLEAVED ? 2 * u : u < hc ? u : 2 * u;  // units past the rotated pairs: chunks 2u, 2u + 1
     const int c1 = !INTERLEAVED && u < hc ? u + hc : c0 + 1;
     const bool in0 = c0 < nc, in1 = c1 < nc;
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    auto source = [&](int h) {
-        const int kh = h - a.n_heads, vh = kh - a.n_kv_heads;
-        return kh < 0 ? a.q + t * a.q_stride + (long long)h * a.head_dim
-                      : vh < 0 ? a.k + t * a.k_stride + (long long)kh * a.head_dim
-                               : a.v + t * a.v_stride + (long long)vh * a.head_dim;
+    auto load = [&](const bf16 *src, bool on, uint4 &r0, uint4 &r1) {
+        r0 = on && in0 ? reinterpret_cast<const uint4 *>(src)[c0] : zero;
+        r1 = on && in1 ? reinterpret_cast<const uint4 *>(src)[c1] : zero;
     };
-    int h = threadIdx.x / a.lph;
-    uint4 r0 = zero, r1 = zero;
-    if (h < heads) {
-        const uint4 *src = reinterpret_cast<const uint4 *>(source(h));
-        if (in0) r0 = src[c0];
-        if (in1) r1 = src[c1];
-    }
+    auto store = [&](bf16 *dst, const uint4 &r0, const uint4 &r1) {
+        if (in0) reinterpret_cast<uint4 *>(dst)[c0] = r0;
+        if (in1) reinterpret_cast<uint4 *>(dst)[c1] = r1;
+    };
+    const bf16 *src = a.q + t * a.q_stride + first * a.head_dim;
+    uint4 n0, n1;
+    load(src, first < a.n_heads, n0, n1);
     const int4 tok = a.toks[t];
     const int pos = tok.y;
     if (pos == PAGED_OUTSIDE) return;
-    for (int j = threadIdx.x; j < half; j += blockDim.x)
-        if (pos >= 0) rope_angle(pos, a.inv_freq[j], a.amplitude, &cos_s[j], &sin_s[j]);
+    bf16 *dst = a.q_out + t * a.q_out_stride + first * a.head_dim;
+    if (pos < 0) {  // padding: zero query rows, nothing stored
+        for (int h = first; h < a.n_heads; h += groups, dst += step) store(dst, zero, zero);
+        return;
+    }
+    for (int j = threadIdx.x; j < (INTERLEAVED ? a.head_dim / 2 : half); j += blockDim.x) {
+        float cs = 1.0f, sn = 0.0f;
+        if (j < half) rope_angle(pos, a.inv_freq[j], a.amplitude, &cs, &sn);
+        if (INTERLEAVED) {
+            reinterpret_cast<float2 *>(cos_s)[j] = make_float2(cs, cs);
+            reinterpret_cast<float2 *>(sin_s)[j] = make_float2(-sn, sn);
+        } else {
+            cos_s[j] = cs;
+            sin_s[j] = sn;
+            neg_s[j] = -sn;
+        }
+    }
     __syncthreads();
-    for (; h < heads; h += groups) {
-        const int kh = h - a.n_heads, vh = kh - a.n_kv_heads;
-        const long long slot = tok.z * a.page_stride + tok.w * a.pos_stride;
-        bf16 *dst = kh < 0 ? a.q_out + t * a.q_out_stride + (long long)h * a.head_dim
-                           : vh < 0 ? a.key_pages + slot + kh * a.head_stride : a.value_pages + slot + vh * a.head_stride;
-        const bf16 *w = kh < 0 ? a.q_norm_w : a.k_norm_w;
-        if (pos < 0) {  // padding: zero query rows, nothing stored
-            if (kh < 0 && in0) reinterpret_cast<uint4 *>(dst)[c0] = zero;
-            if (kh < 0 && in1) reinterpret_cast<uint4 *>(dst)[c1] = zero;
-            continue;
+    const unsigned group = ((1u << a.lph) - 1) << (threadIdx.x % 32 / a.lph * a.lph);
+    const float inv_dim = 1.0f / a.head_dim;
+    // one head: norm with weights w (if there are any), rotation, one rounding
+    auto turn = [&](uint4 &r0, uint4 &r1, const bf16 *w) {
+        uint64_t x[8];
+        unpack8(r0, x);
+        unpack8(r1, x + 4);
+        if (w != nullptr) {  // uniform over q heads and over k heads, whose groups of lanes may share a warp
+            uint64_t sq = mul2(x[0], x[0]);
+#pragma unroll
+            for (int i = 1; i < 8; i++) sq = fma2(x[i], x[i], sq);
+            float sum = unpair(sq).x + unpair(sq).y;
+            for (int off = a.lph / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(group, sum, off);
+            const float inv = rsqrtf(sum * inv_dim + a.eps);
+            uint4 g0, g1;
+            load(w, true, g0, g1);
+            uint64_t g[4];
+            unpack8(g0, g);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = mul2(mul2(x[i], pair(inv, inv)), g[i]);
+            unpack8(g1, g);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[4 + i] = mul2(mul2(x[4 + i], pair(inv, inv)), g[i]);
         }
-        uint4 o0 = r0, o1 = r1;
-        if (vh < 0) {
-            float x[16];
-            unpack8(r0, x);
-            unpack8(r1, x + 8);
-            if (w != nullptr) {  // uniform over q heads and over k heads, whose groups of lanes may share a warp
-                float sum = 0.0f;
+        if (INTERLEAVED) {
+            const uint64_t *c = reinterpret_cast<const uint64_t *>(cos_s) + 8 * u, *s = reinterpret_cast<const uint64_t *>(sin_s) + 8 * u;
 #pragma unroll
-                for (int i = 0; i < 16; i++) sum = __fmaf_rn(x[i], x[i], sum);
-                const unsigned group = (a.lph == 32 ? 0xffffffffu : (1u << a.lph) - 1) << (threadIdx.x % 32 / a.lph * a.lph);
-                for (int off = a.lph / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(group, sum, off);
-                const float inv = rsqrtf(sum / a.head_dim + a.eps);
-                float g[16];
-                unpack8(in0 ? reinterpret_cast<const uint4 *>(w)[c0] : zero, g);
-                unpack8(in1 ? reinterpret_cast<const uint4 *>(w)[c1] : zero, g + 8);
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[i] = x[i] * inv * g[i];
+            for (int i = 0; i < 8; i++) {
+                const float2 v = unpair(x[i]);
+                if (in1 || i < 4) x[i] = fma2(pair(v.y, v.x), s[i], mul2(x[i], c[i]));
             }
-            if constexpr (INTERLEAVED) {
+        } else if (u < hc) {
+            const uint64_t *c = reinterpret_cast<const uint64_t *>(cos_s) + 4 * u, *s = reinterpret_cast<const uint64_t *>(sin_s) + 4 * u,
+                           *ns = reinterpret_cast<const uint64_t *>(neg_s) + 4 * u;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int j = 8 * u + i;  // pair (2j, 2j + 1)
-                    if (j < half) {
-                        const float e = x[2 * i], o = x[2 * i + 1], c = cos_s[j], s = sin_s[j];
-                        x[2 * i] = e * c - o * s;
-                        x[2 * i + 1] = o * c + e * s;
-                    }
-                }
-            } else if (u < hc) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float e = x[i], o = x[8 + i], c = cos_s[8 * u + i], s = sin_s[8 * u + i];
-                    x[i] = e * c - o * s;
-                    x[8 + i] = o * c + e * s;
-                }
+            for (int i = 0; i < 4; i++) {
+                const uint64_t e = x[i], o = x[4 + i];
+                x[i] = fma2(o, ns[i], mul2(e, c[i]));
+                x[4 + i] = fma2(e, s[i], mul2(o, c[i]));
             }
-            o0 = pack8(x);
-            o1 = pack8(x + 8);
         }
-        if (in0) reinterpret_cast<uint4 *>(dst)[c0] = o0;
-        if (in1) reinterpret_cast<uint4 *>(dst)[c1] = o1;
-        if (h + groups < heads) {
-            const uint4 *src = reinterpret_cast<const uint4 *>(source(h + groups));
-            if (in0) r0 = src[c0];
-            if (in1) r1 = src[c1];
+        r0 = pack8(x);
+        r1 = pack8(x + 4);
+    };
+    // key and value heads go to the groups from the other end, so that none has two heads more than another
+    int kv = groups - 1 - first;
+    auto kv_load = [&](int i) {
+        load(i < a.n_kv_heads ? a.k + t * a.k_stride + i * a.head_dim : a.v + t * a.v_stride + (i - a.n_kv_heads) * a.head_dim,
+             i < 2 * a.n_kv_heads, n0, n1);
+    };
+    if (first >= a.n_heads) kv_load(kv);
+    for (int h = first; h < a.n_heads; h += groups) {
+        uint4 r0 = n0, r1 = n1;
+        src += step;
+        if (h + groups < a.n_heads) load(src, true, n0, n1);
+        else kv_load(kv);
+        turn(r0, r1, a.q_norm_w);
+        store(dst, r0, r1);
+        dst += step;
+    }
+    const long long slot = tok.z * a.page_stride + tok.w * a.pos_stride;
+    for (; kv < 2 * a.n_kv_heads; kv += groups) {
+        uint4 r0 = n0, r1 = n1;
+        if (kv + groups < 2 * a.n_kv_heads) kv_load(kv + groups);
+        if (kv < a.n_kv_heads) {
+            turn(r0, r1, a.k_norm_w);
+            store(a.key_pages + slot + kv * a.head_stride, r0, r1);
+        } else {
+            store(a.value_pages + slot + (kv - a.n_kv_heads) * a.head_stride, r0, r1);
         }
     }
 }
@@ -572,11 +602,12 @@ int q3_paged_rope_append(q3_bf16 *q_out, long long q_out_stride, const q3_bf16 *
     const int units = hc + (chunks - 2 * hc + 1) / 2;
     for (a.lph = 1; a.lph < units;) a.lph *= 2;
     cudaStream_t st = (cudaStream_t)stream;
-    const int heads = s.n_heads + 2 * s.n_kv_heads, rounds = (heads * a.lph + APPEND_MAX_THREADS - 1) / APPEND_MAX_THREADS;
+    const int most = s.n_tokens >= 2 * num_sms() ? APPEND_THREADS : APPEND_MAX_THREADS;
+    const int heads = s.n_heads + 2 * s.n_kv_heads, rounds = (heads * a.lph + most - 1) / most;
     const dim3 grid(s.n_tokens), block(((heads + rounds - 1) / rounds * a.lph + 31) / 32 * 32);
     if (interleaved) Q3_TRY_LAUNCH(launch(paged_append_kernel<true>, grid, block, 0, st, 1, a));
     else if (rope_dim % 16 == 0) Q3_TRY_LAUNCH(launch(paged_append_kernel<false>, grid, block, 0, st, 1, a));
-    else Q3_TRY_LAUNCH(launch(paged_append_odd_kernel, grid, dim3(APPEND_ODD_THREADS), 0, st, 1, a));
+    else Q3_TRY_LAUNCH(launch(paged_append_odd_kernel, dim3(s.n_tokens), dim3(APPEND_ODD_THREADS), 0, st, 1, a));
     return Q3_OK;
 }
 

@@ -101,6 +101,33 @@ inline PagedScratchLayout paged_scratch_layout(const q3_paged_shape &s) {
 
 inline int paged_ctas() { return num_sms() < PAGED_MAX_CTAS ? num_sms() : PAGED_MAX_CTAS; }
 
+// two floats as one operand of the packed fp32 instructions
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+    float2 y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+    return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t y;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+
 // Q3_OK, or why the shape is not supported.
 int paged_shape_check(const q3_paged_shape *s);
 

@@ -138,27 +138,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return y;
 }
 
-// two floats as one operand of the packed fp32 instructions
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t y;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
-    return y;
-}
-__device__ __forceinline__ float2 unpair(uint64_t x) {
-    float2 y;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
-    return y;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t y;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
-    return y;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t y;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
-    return y;
-}
 __device__ __forceinline__ void tma_page(void *dst, const CUtensorMap *map, int x, int slot, int head, int page,
                                          uint64_t *bar) {
     asm volatile(
