@@ -69,6 +69,8 @@ __device__ __forceinline__ void each_id(const int *ids, int i0, int i1, F f) {
     const int lead = min(i1 - i0, (int)((16 - (reinterpret_cast<uintptr_t>(ids + i0) & 15)) & 15) / 4);
     const int quads = (i1 - i0 - lead) / 4, tail = i0 + lead + 4 * quads;
     if ((int)threadIdx.x < lead) f(i0 + threadIdx.x, ids[i0 + threadIdx.x]);
+    // one load in flight: with four, the unrolled body's registers cost more than the loads' latency (14.3 -> 18 us
+    // for 32 rows of 151936)
     for (int q = threadIdx.x; q < quads; q += blockDim.x) {
         const int i = i0 + lead + 4 * q;
         const int4 v = __ldg(reinterpret_cast<const int4 *>(ids + i));
@@ -155,24 +157,30 @@ __global__ void __launch_bounds__(512) logits_process_kernel(const __grid_consta
 #pragma unroll
         for (int e = 0; e < LP_EACH; e++) x[e] = i0 + e >= 0 && i0 + e < a.vocab ? to_f32(in[i0 + e]) : 0.0f;
     }
-    if (hist) {
-        const float rep = a.repetition ? a.repetition[r] : 1.0f, freq = a.frequency ? a.frequency[r] : 0.0f,
-                    pres = a.presence ? a.presence[r] : 0.0f;
+    if (hist) {  // most threads own no token of the history
+        const uint4 *own = reinterpret_cast<const uint4 *>(count_s) + tid * (LP_EACH / 4);
+        const uint4 ca = own[0], cb = own[1];
+        if ((ca.x | ca.y | ca.z | ca.w | cb.x | cb.y | cb.z | cb.w) != 0) {
+            const float rep = a.repetition ? a.repetition[r] : 1.0f, freq = a.frequency ? a.frequency[r] : 0.0f,
+                        pres = a.presence ? a.presence[r] : 0.0f;
+            const unsigned c[LP_EACH] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
 #pragma unroll
-        for (int e = 0; e < LP_EACH; e++) {
-            const unsigned c = count_s[LP_EACH * tid + e];
-            if (c != 0) {
+            for (int e = 0; e < LP_EACH; e++) {
+                if (c[e] == 0) continue;
                 if (a.repetition) x[e] = x[e] > 0.0f ? x[e] / rep : x[e] * rep;
-                const unsigned times = c & ~LP_SEEN;
+                const unsigned times = c[e] & ~LP_SEEN;
                 if (times != 0) x[e] -= freq * (float)times + pres;
             }
         }
     }
     if (biased) {
+        const int4 *own = reinterpret_cast<const int4 *>(bias_s) + tid * (LP_EACH / 4);
+        const int4 ba = own[0], bb = own[1];
+        if ((ba.x & ba.y & ba.z & ba.w & bb.x & bb.y & bb.z & bb.w) != -1) {
+            const int i[LP_EACH] = {ba.x, ba.y, ba.z, ba.w, bb.x, bb.y, bb.z, bb.w};
 #pragma unroll
-        for (int e = 0; e < LP_EACH; e++) {
-            const int i = bias_s[LP_EACH * tid + e];
-            if (i >= 0) x[e] += a.bias[i];
+            for (int e = 0; e < LP_EACH; e++)
+                if (i[e] >= 0) x[e] += a.bias[i[e]];
         }
     }
 #pragma unroll
