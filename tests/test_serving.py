@@ -1,0 +1,71 @@
+"""The server's host side: pages, and which tokens each step takes."""
+import sys
+from pathlib import Path
+
+import pytest
+
+HERE = Path(__file__).resolve().parent
+sys.path.insert(0, str(HERE))
+import conftest  # noqa: E402,F401
+from llm_inference_b200.serving import Sequence, Sequences  # noqa: E402
+
+
+def run(s, n, token=7):
+    steps = []
+    for _ in range(n):
+        st = s.step()
+        steps.append((list(zip(st.ids, st.counts)), [i for _, i in st.outputs]))
+        s.commit(st, [token] * len(st.outputs))
+    return steps
+
+
+def test_decodes_run_beside_one_chunk():
+    s = Sequences(n_pages=100, page_size=8, max_seqs=4, max_pages=10, chunk=16)
+    a = s.add(Sequence([1]))
+    b = s.add(Sequence(list(range(40))))
+    c = s.add(Sequence(list(range(20))))
+    got = run(s, 6)
+    assert got[0] == ([(a, 1), (b, 16)], [a])
+    assert got[1] == ([(a, 1), (b, 16)], [a])
+    assert got[2] == ([(a, 1), (b, 8)], [a, b])       # b's last chunk: its first token
+    assert got[3] == ([(a, 1), (b, 1), (c, 16)], [a, b])
+    assert got[4] == ([(a, 1), (b, 1), (c, 4)], [a, b, c])
+    assert got[5][1] == [a, b, c]
+    assert s.live[b].generated == [7] * 4 and s.live[b].cached == 43
+    assert len(s.live[b].pages) == 6 and len(set(s.live[a].pages + s.live[b].pages + s.live[c].pages)) == 10
+
+
+def test_tokens_and_rows_of_a_step():
+    s = Sequences(10, 8, 4, 10, 16)
+    a = s.add(Sequence([5]))
+    b = s.add(Sequence([9, 8, 7]))
+    st = s.step()
+    assert st.tokens == [5, 9, 8, 7] and st.outputs == [(0, a), (3, b)]
+    s.commit(st, [50, 90])
+    assert s.step().tokens == [50, 90]
+
+
+def test_pages_run_out_and_come_back():
+    s = Sequences(n_pages=3, page_size=8, max_seqs=4, max_pages=3, chunk=16)
+    a = s.add(Sequence(list(range(16))))
+    b = s.add(Sequence(list(range(16))))
+    assert run(s, 1)[0][0] == [(a, 16)]               # two of three pages
+    assert run(s, 1)[0][0] == [(a, 1)]                # the third; b finds none
+    assert run(s, 1)[0][0] == [(a, 1)]
+    s.remove(a)
+    assert sorted(s.free) == [0, 1, 2]
+    assert run(s, 1)[0][0] == [(b, 16)]
+    for _ in range(20):                               # b's page table ends at 24 positions
+        run(s, 1)
+    assert s.live[b].cached == 24 and s.step().ids == []
+
+
+def test_refusals():
+    s = Sequences(10, 8, 1, 2, 16)
+    with pytest.raises(ValueError):
+        s.add(Sequence([]))
+    with pytest.raises(ValueError):
+        s.add(Sequence([1] * 17))
+    s.add(Sequence([1]))
+    with pytest.raises(RuntimeError):
+        s.add(Sequence([1]))
