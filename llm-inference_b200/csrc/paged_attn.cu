@@ -758,12 +758,13 @@ __device__ void big_multiply(const PaArgs &a, const PagedPiece &p, BigSmem<DP> &
     }
 }
 
-// One thread waits for V of each step and K of the next, and passes that on with P's arrivals.
+// One thread waits for V of each step and K of the next, and passes that on with P's arrivals. Their stages are not
+// released before it has arrived. A piece's first K is not waited for here: the products release it without asking
+// this thread, which could come so late that its stage has been filled once more, a phase it would wait for in vain.
 template <int DP>
 __device__ void big_ready(const PaArgs &a, const PagedPiece &p, BigSmem<DP> &sm, Ring<BIG_STAGES> &r, uint32_t &p_ph,
                           Waiter &wait) {
     const int tiles = p.n_tok > a.tile_tok ? 2 : 1, n = big_steps(p);
-    wait(&sm.full[r.s], r.ph);  // the first K
     r.next();
     for (int j = 0; j < n; j++) {
         wait(&sm.full[r.s], r.ph);

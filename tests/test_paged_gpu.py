@@ -451,3 +451,19 @@ def test_sequences_without_new_tokens():
     out = torch.full((4, 8, 64), 7.0, dtype=BF, device="cuda")
     q3.paged_attention(out, torch.zeros_like(out), pages, pages, plan)
     assert (out == 7.0).all() and q3.device_error() == 0
+
+
+def test_many_short_chunks_beside_long_decodes():
+    # CTAs that take many items of one or two steps each while the decodes keep memory busy: no wait may miss its phase
+    g = np.random.default_rng(9)
+    lens = [(1, 4096)] * 24 + [(int(n), int(n) + int(c)) for n, c in zip(g.integers(9, 200, 48), g.integers(0, 150, 48))]
+    b = Batch(lens, 32, 8, 128, 32, seed=31, fill=NAN)
+    q = rn(b.g, b.tokens, 32, 128)
+    out = attend(b, q)
+    again = [torch.empty_like(out) for _ in range(2)]
+    for i in range(60):
+        q3.paged_attention(again[i % 2], q, b.kp, b.vp, b.plan)
+    torch.cuda.synchronize()
+    assert q3.device_error() == 0
+    assert torch.equal(out, again[0]) and torch.equal(out, again[1])
+    check_attention(out, *b.attention_exact(q, 128 ** -0.5), "short chunks and long decodes")
