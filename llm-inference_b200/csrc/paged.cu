@@ -28,15 +28,18 @@ struct PlanArgs {
     int n_ctas, small_step;
 };
 
-// Costs, in 16 KB loads' worth of a CTA's time: a step of a small item is one, a 128-position step of one or two
-// tensor-core tiles BIG_ONE or BIG_TWO; an item's start and end (queries, merge, output) ITEM. Items are
-// cut only while each CTA still gets MIN_SHARE.
-constexpr int COST_ITEM = 3, COST_BIG_ONE = 2, COST_BIG_TWO = 3, MIN_SHARE = 16;
+// Costs, in units of a kind's own: a step of a small item is one, the 16 KB load that it waits for; a 128-position step of
+// one or two tensor-core tiles BIG_ONE or BIG_TWO; an item's start and end (queries, merge, output) ITEM or BIG_ITEM.
+// Items are cut only while each CTA still gets MIN_SHARE. A unit of the big kind takes BIG_WEIGHT / 2 of the small one's
+// time where the two share the SMs: with 31 decodes and a chunk of 333 tokens, 1 to 4 and 5.5 gave 178, 107, 89, 88, 96 us
+// (105 one after the other), with 32 decodes at 4096 and a chunk of 2048 at 8192 425, 370, 334, 400, 480 (376).
+constexpr int COST_ITEM = 3, COST_BIG_ITEM = 6, COST_BIG_ONE = 2, COST_BIG_TWO = 3, MIN_SHARE = 16, BIG_WEIGHT = 6;
 
 // The items of sequence q: a big one has n_q per kv head.
 struct SeqItems {
     bool big;
     int n_q, span;  // items per kv head, tokens of each
+    __device__ __forceinline__ int ends() const { return big ? COST_BIG_ITEM : COST_ITEM; }
 };
 
 __device__ __forceinline__ SeqItems seq_items(const PagedSeq &q, int rep) {
@@ -55,9 +58,9 @@ __device__ __forceinline__ void item_steps(const PagedSeq &q, const SeqItems &s,
     *cost = !s.big ? 1 : last - i * s.span > s.span / 2 ? COST_BIG_TWO : COST_BIG_ONE;
 }
 
-// Steps of an item that lie before cost r of it.
-__device__ __forceinline__ int steps_before(long long r, int n, int cost) {
-    return (int)max(0ll, min((long long)n, (r - COST_ITEM + cost - 1) / cost));
+// Steps of an item that lie before cost r of it; its ends come first.
+__device__ __forceinline__ int steps_before(long long r, int ends, int n, int cost) {
+    return (int)max(0ll, min((long long)n, (r - ends + cost - 1) / cost));
 }
 
 // Exclusive prefix sum of v[0 .. n) in place by the whole CTA; returns the total.
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
         for (int i = 0; i < s.n_q; i++) {
             int end, steps, c;
             item_steps(q, s, i, s.big ? BIG_TILE : small_step, &end, &steps, &c);
-            cost += COST_ITEM + (long long)steps * c;
+            cost += s.ends() + (long long)steps * c;
         }
         big_s[b] = s.big ? cost * kvh : 0;
         small_s[b] = s.big ? 0 : cost * kvh;
@@ -181,13 +184,24 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     PagedPiece *pieces = reinterpret_cast<PagedPiece *>(a.plan + a.l.pieces);
     PagedPiece *splits = reinterpret_cast<PagedPiece *>(a.plan + a.l.splits);
     int *counters = reinterpret_cast<int *>(a.plan + a.l.counters);
+    // The two kernels of a step with items of both kinds run side by side: the big one's CTAs first, the small
+    // one's on the SMs that those leave: tensor-core work beside loads, and memory bandwidth is not for want of SMs.
+    const long long weight = total_big * BIG_WEIGHT / 2;
+    const int share = total_big > 0 && total_small > 0
+                          ? (int)max(1ll, min((long long)a.n_ctas - 1, a.n_ctas * weight / (weight + total_small)))
+                          : a.n_ctas;
+    auto ctas_used = [&](long long most, bool big) {
+        return (int)max(1ll, min(most, max((long long)n_items[big], (big ? total_big : total_small) / MIN_SHARE)));
+    };
+    const int used_big = ctas_used(share, true);
+    const int used_small = ctas_used(total_big > 0 ? max(1, a.n_ctas - used_big) : a.n_ctas, false);
     // A CTA's pieces start at (items before its first) + (CTAs before it): every cut adds one piece at most.
     for (int id = tid; id < 2 * a.n_ctas; id += PLAN_THREADS) {
         const bool big = id >= a.n_ctas;
         const int c = big ? id - a.n_ctas : id, step = big ? BIG_TILE : small_step;
         const long long total = big ? total_big : total_small;
         const long long *pre = big ? big_s : small_s;
-        const int used = (int)max(1ll, min((long long)a.n_ctas, max((long long)n_items[big], total / MIN_SHARE)));
+        const int used = big ? used_big : used_small;
         auto bound = [&](int i) { return total * i / used; };
         const long long u0 = c < used ? bound(c) : total, u1 = c < used ? bound(c + 1) : total;
         int count = 0, first_piece = -1;
@@ -209,12 +223,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
             long long len;
             for (;; i++) {
                 item_steps(q, s, i, step, &end, &steps, &cost);
-                len = COST_ITEM + (long long)steps * cost;
+                len = s.ends() + (long long)steps * cost;
                 if (u < start + len) break;
                 start += len;
             }
-            const int t0 = steps_before(u - start, steps, cost);
-            const int t1 = u1 >= start + len ? steps : steps_before(u1 - start, steps, cost);
+            const int t0 = steps_before(u - start, s.ends(), steps, cost);
+            const int t1 = u1 >= start + len ? steps : steps_before(u1 - start, s.ends(), steps, cost);
             if (t1 > t0) {
                 PagedPiece p;
                 p.seq = lo;
@@ -231,9 +245,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
                 p.n_parts = 1;
                 if (t0 > 0 || t1 < steps) {
                     int f = c;
-                    while (steps_before(bound(f) - start, steps, cost) > 0) f--;
+                    while (steps_before(bound(f) - start, s.ends(), steps, cost) > 0) f--;
                     p.first = f;
-                    while (f + 1 < used && bound(f + 1) < start + len && steps_before(bound(f + 1) - start, steps, cost) < steps) f++;
+                    while (f + 1 < used && bound(f + 1) < start + len && steps_before(bound(f + 1) - start, s.ends(), steps, cost) < steps) f++;
                     p.n_parts = f - p.first + 1;
                     p.part = part_slot(p.first, c - p.first);
                     if (t0 == 0 && p.n_parts > MERGE_PARTS) split = p;
