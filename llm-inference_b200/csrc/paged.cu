@@ -25,7 +25,7 @@ struct PlanArgs {
     PagedPlanLayout l;
     q3_paged_shape s;
     const int *q_start, *kv_len, *page_table;
-    int n_ctas, small_step;
+    int n_ctas, small_step, small_rows;
 };
 
 // Costs, in units of a kind's own: a step of a small item is one, the 16 KB load that it waits for; a 128-position step of
@@ -42,9 +42,9 @@ struct SeqItems {
     __device__ __forceinline__ int ends() const { return big ? COST_BIG_ITEM : COST_ITEM; }
 };
 
-__device__ __forceinline__ SeqItems seq_items(const PagedSeq &q, int rep) {
+__device__ __forceinline__ SeqItems seq_items(const PagedSeq &q, int rep, int small_rows) {
     SeqItems s;
-    s.big = (long long)q.q_len * rep > SMALL_ROWS;
+    s.big = (long long)q.q_len * rep > small_rows;
     s.span = s.big ? 2 * (BIG_TILE / rep) : q.q_len;
     s.n_q = q.q_len == 0 ? 0 : (q.q_len + s.span - 1) / s.span;
     return s;
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     const int small_step = a.small_step;
     for (int b = tid; b < n; b += PLAN_THREADS) {
         const PagedSeq q = seqs[b];
-        const SeqItems s = seq_items(q, rep);
+        const SeqItems s = seq_items(q, rep, a.small_rows);
         long long cost = 0;
         for (int i = 0; i < s.n_q; i++) {
             int end, steps, c;
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
                 else hi = mid - 1;
             }
             const PagedSeq q = seqs[lo];
-            const SeqItems s = seq_items(q, rep);
+            const SeqItems s = seq_items(q, rep, a.small_rows);
             const long long per_head = (pre[lo + 1] - pre[lo]) / kvh;
             const int head = (int)((u - pre[lo]) / per_head);
             long long start = pre[lo] + head * per_head;
@@ -561,7 +561,7 @@ int q3_paged_plan(void *plan, const q3_paged_shape *shape, const int *q_start, c
     if (!aligned16(plan)) return Q3_ERR_ALIGN;
     TRY(check_device());
     PlanArgs a = {static_cast<char *>(plan), paged_plan_layout(*shape), *shape, q_start, kv_len, page_table,
-                  paged_ctas(), paged_small_step(*shape)};
+                  paged_ctas(), paged_small_step(*shape), paged_small_rows(*shape)};
     const size_t smem = (size_t)(shape->n_seqs + 1) * (3 * sizeof(long long) + sizeof(int));
     Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_plan_kernel), smem));
     Q3_TRY_LAUNCH(launch(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), smem, (cudaStream_t)stream, 1, a));

@@ -17,11 +17,10 @@ struct PagedSeq {
 };
 
 // Attention work. An item is what one CTA could do alone: the query rows of a (sequence, kv head) that
-// attend together. Few rows (q_len * n_heads / n_kv_heads <= SMALL_ROWS) are one item, fed to warp-level
+// attend together. Few rows (q_len * n_heads / n_kv_heads <= paged_small_rows) are one item, fed to warp-level
 // matrix instructions; more are cut into items of two 128-row tensor-core tiles. Each kind has its kernel.
 // The plan lays a kind's costs end to end and gives each CTA an equal stretch, so an item may be cut along its
 // positions into pieces of neighbouring CTAs, which leave partial results in the scratch.
-constexpr int SMALL_ROWS = 8;
 constexpr int BIG_TILE = 128;       // rows of a tensor-core tile, and positions of one of its steps
 constexpr int PAGED_MAX_CTAS = 160; // persistent CTAs, one per SM
 constexpr int MERGE_PARTS = 2;      // a big item of up to this many pieces is merged by the last of them to finish
@@ -79,8 +78,18 @@ struct PagedScratchLayout {
     size_t small_o, small_ml, big_o, big_ml, bytes;
 };
 
+// Rows of the kernel for few rows: eight for each 8-column tile of its products. Where every sequence fits into a
+// few tiles (draft tokens being verified) the step needs no other kernel; where some do not, it is the one for single
+// tokens, and all longer sequences go to the kernel for many rows. 32 sequences at 4096, 8 kv heads of 128: 16 rows take
+// 90 us here and 120 there, 24 rows 152 and 120 (their accumulators spill); 4 kv heads of 64: 16 rows 31 and 59,
+// 24 rows 38 and 60, 40 rows 64 and 59.
+inline int paged_small_rows(const q3_paged_shape &s) {
+    const long long most = (long long)s.max_q_len * (s.n_heads / s.n_kv_heads);
+    if (most > (s.head_dim <= 64 ? 24 : 16) || most <= 8) return 8;
+    return most <= 16 ? 16 : 24;
+}
 inline bool paged_has_big(const q3_paged_shape &s) {
-    return (long long)s.max_q_len * (s.n_heads / s.n_kv_heads) > SMALL_ROWS;
+    return (long long)s.max_q_len * (s.n_heads / s.n_kv_heads) > paged_small_rows(s);
 }
 
 // A step of a small item is one ring stage of K and V; pieces are cut at multiples of it.
@@ -92,8 +101,8 @@ inline PagedScratchLayout paged_scratch_layout(const q3_paged_shape &s) {
     const size_t dp = s.head_dim <= 64 ? 64 : 128, slots = 2 * PAGED_MAX_CTAS;
     const size_t big = paged_has_big(s) ? 2 * BIG_TILE : 0;
     l.small_o = 0;
-    l.small_ml = l.small_o + slots * SMALL_ROWS * dp * 4;
-    l.big_o = l.small_ml + slots * SMALL_ROWS * 8;
+    l.small_ml = l.small_o + slots * paged_small_rows(s) * dp * 4;
+    l.big_o = l.small_ml + slots * paged_small_rows(s) * 8;
     l.big_ml = l.big_o + slots * big * dp * 4;
     l.bytes = l.big_ml + slots * big * 8;
     return l;

@@ -24,6 +24,7 @@
 // or infinite v would still be NaN. Rows of V past the item's end are zeroed in shared memory; the few
 // rows that some tokens of the item see and others do not are checked, and if one holds such a value that step's
 // second product runs on the CUDA cores, skipping what each row does not see.
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -272,35 +273,50 @@ __device__ void small_produce(const PaArgs &a, const CUtensorMap *mk, const CUte
 // ---------------------------------------------------------------- few rows: consumers
 
 // Each warp owns whole stages. The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that positions
-// and head columns fill the instruction's 16 rows and the query rows its 8 columns. Against queries as the 16
-// rows (most of them padding at 4 query heads per kv head) this halves products, exponentials and
+// and head columns fill the instruction's 16 rows and the query rows its 8 columns, in NQ tiles of them. Against queries
+// as the 16 rows (most of them padding at 4 query heads per kv head) this halves products, exponentials and
 // accumulators; P^T moves from accumulator to operand layout by an 8 x 8 transpose in registers.
-// merge_o is [NW][8][DP] fp32, columns permuted by row against bank conflicts; merge_ml (m, l).
-template <int DP, int NW, int NST>
+// One tile keeps its queries in registers; more read them from q_s, laid out as the instruction's operand, and take
+// a stage 32 positions at a time.
+// merge_o is [NW][8][DP] fp32, columns permuted by row against bank conflicts; merge_ml (m, l); one tile at a time.
+template <int DP, int NQ, int NW, int NST>
 __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned char *ring, uint64_t *full,
-                              uint64_t *empty, Ring<NST> &r, Waiter &wait, int cw, float *merge_o, float2 *merge_ml,
-                              int *flag_s) {
-    constexpr int NB = DP / 64, UPOS = SMALL_STAGE / (4 * DP), MT = UPOS / 16, KS = DP / 16;
+                              uint64_t *empty, Ring<NST> &r, Waiter &wait, int cw, uint2 *q_s, int2 *lim_s, float *merge_o,
+                              float2 *merge_ml, int *flag_s) {
+    constexpr int NB = DP / 64, UPOS = SMALL_STAGE / (4 * DP), MT = NQ == 1 ? UPOS / 16 : 2, KS = DP / 16;
     const int lane = threadIdx.x % 32, g = lane / 4, tq = lane % 4, l7 = lane % 8, mi = lane / 8;
-    const int rows = p.n_tok * a.rep;
-    uint32_t qb[KS][2];
-    {
-        const bf16 *src = a.q + (p.tok0 + g / a.rep) * a.q_stride + (long long)(p.kvh * a.rep + g % a.rep) * a.head_dim;
+    const int rows = p.n_tok * a.rep, tid = cw * 32 + lane;
+    // operand words of lane `ln`: queries of row 8 nq + ln / 4, columns 16 k + 8 j + 2 (ln % 4) and the one after
+    auto queries = [&](int ln, int nq, int k) {
+        const int row = 8 * nq + ln / 4, col = 16 * k + 2 * (ln % 4);
+        const bf16 *src = a.q + (p.tok0 + row / a.rep) * a.q_stride + (long long)(p.kvh * a.rep + row % a.rep) * a.head_dim + col;
+        return make_uint2(row < rows && col < a.head_dim ? *reinterpret_cast<const uint32_t *>(src) : 0u,
+                          row < rows && col + 8 < a.head_dim ? *reinterpret_cast<const uint32_t *>(src + 8) : 0u);
+    };
+    // rows 8 nq + 2 tq and the next are this thread's columns of S^T and O^T, and see the positions before these; the last
+    // step may reach past the piece, where nothing was loaded
+    auto limit = [&](int row) { return min(p.pos0 + row / a.rep + 1, p.kv1); };
+    uint2 qb[NQ == 1 ? KS : 1];
+    int2 lim1;
+    if (NQ == 1) {
 #pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int col = 16 * k + 8 * j + 2 * tq;
-                qb[k][j] = g < rows && col < a.head_dim ? *reinterpret_cast<const uint32_t *>(src + col) : 0u;
-            }
+        for (int k = 0; k < KS; k++) qb[k] = queries(lane, 0, k);
+        lim1 = make_int2(limit(2 * tq), limit(2 * tq + 1));
+    } else {
+        for (int i = tid; i < KS * NQ * 32; i += NW * 32) q_s[i] = queries(i % 32, i / 32 % NQ, i / 32 / NQ);
+        if (tid < 4 * NQ) lim_s[tid] = make_int2(limit(2 * tid), limit(2 * tid + 1));
+        bar_sync(1, NW * 32);
     }
-    // rows 2 tq and 2 tq + 1 are this thread's columns of S^T and O^T; the last step may reach past the piece, where
-    // nothing was loaded
-    const int lim[2] = {min(p.pos0 + 2 * tq / a.rep + 1, p.kv1), min(p.pos0 + (2 * tq + 1) / a.rep + 1, p.kv1)};
+    auto limits = [&](int nq) { return NQ == 1 ? lim1 : lim_s[4 * nq + tq]; };
     const int lim_min = min(first_masked(p), p.kv1);
-    float o[KS][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // o: head columns 16 i + g and + 8
+    float o[NQ][KS][4], m[NQ][2], l[NQ][2];  // o: head columns 16 i + g and + 8
 #pragma unroll
-    for (int i = 0; i < KS; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    for (int nq = 0; nq < NQ; nq++) {
+        m[nq][0] = m[nq][1] = -INFINITY;
+        l[nq][0] = l[nq][1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KS; i++) o[nq][i][0] = o[nq][i][1] = o[nq][i][2] = o[nq][i][3] = 0.0f;
+    }
     // ldmatrix rows of this lane: K as [position][column] (operand rows = positions), V transposed
     const uint32_t k_row = ((mi & 1) * 8 + l7) * 128, v_row = ((mi >> 1) * 8 + l7) * 128;
 
@@ -311,64 +327,14 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
             const uint32_t kb = smem_u32(stage), vb = kb + NB * UPOS * 128;
             wait(&full[r.s], r.ph);
             __syncwarp();
-            float s[MT][4];
-#pragma unroll
-            for (int i = 0; i < MT; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const int c = 2 * k + (mi >> 1);
-                const uint32_t at = kb + k_row + (k / 4) * (UPOS * 128) + (((c % 8) ^ l7) << 4);
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    uint32_t ka[4];
-                    ldsm4(ka, at + i * 16 * 128);
-                    mma16816(s[i], ka, qb[k][0], qb[k][1]);
-                }
-            }
             const bool masked = p0 + UPOS > lim_min;
-            float x[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int i = 0; i < MT; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    s[i][j] *= a.scale_log2;
-                    if (masked && p0 + 16 * i + 8 * (j >> 1) + g >= lim[j & 1]) s[i][j] = -INFINITY;
-                    x[j & 1] = fmaxf(x[j & 1], s[i][j]);
-                }
-#pragma unroll
-            for (int off = 4; off < 32; off *= 2) {
-                x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], off));
-                x[1] = fmaxf(x[1], __shfl_xor_sync(0xffffffffu, x[1], off));
-            }
-            if (__any_sync(0xffffffffu, x[0] > m[0] || x[1] > m[1])) {
-                float f[2];
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const float top = fmaxf(m[e], x[e]);
-                    f[e] = top == -INFINITY ? 1.0f : ex2(m[e] - top);
-                    m[e] = top;
-                    l[e] *= f[e];
-                }
-#pragma unroll
-                for (int i = 0; i < KS; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) o[i][j] *= f[j & 1];
-            }
-            const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-#pragma unroll
-            for (int i = 0; i < MT; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    s[i][j] = ex2(s[i][j] - base[j & 1]);
-                    l[j & 1] += s[i][j];
-                }
-            bool touched = false, slow = false;
+            bool slow = false;
             if (p0 + UPOS > p.kv1) {  // rows past the end: zero
                 const int t0 = max(0, p.kv1 - p0), n = (UPOS - t0) * 8;
                 for (int h = 0; h < NB; h++)
                     for (int i = lane; i < n; i += 32)
                         reinterpret_cast<uint4 *>(stage + (NB + h) * (UPOS * 128) + t0 * 128)[i] = make_uint4(0, 0, 0, 0);
-                touched = true;
+                fence_proxy_async();  // these writes, before the next TMA write of the stage
                 __syncwarp();
             }
             if (masked && p.n_tok > 1) {  // rows that only some tokens see
@@ -378,44 +344,114 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
                         slow |= not_finite8(reinterpret_cast<const uint4 *>(stage + (NB + h) * (UPOS * 128) + t0 * 128)[i]);
                 slow = __any_sync(0xffffffffu, slow);
             }
-            if (!slow) {
-#pragma unroll
-                for (int t = 0; t < MT; t++) {
-                    const uint32_t pb0 = transpose8(pack_bf16(s[t][0], s[t][1])), pb1 = transpose8(pack_bf16(s[t][2], s[t][3]));
-#pragma unroll
-                    for (int i = 0; i < KS; i++) {
-                        const int c = 2 * i + (mi & 1);
-                        uint32_t va[4];
-                        ldsm4_t(va, vb + v_row + t * 16 * 128 + (i / 4) * (UPOS * 128) + (((c % 8) ^ l7) << 4));
-                        mma16816(o[i], va, pb0, pb1);
-                    }
-                }
-            } else {  // the probabilities take K's place in the stage; then position by position
-                float *ps = reinterpret_cast<float *>(stage);
-#pragma unroll
-                for (int i = 0; i < MT; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) ps[(16 * i + 8 * (j >> 1) + g) * SMALL_ROWS + 2 * tq + (j & 1)] = s[i][j];
-                touched = true;
-                __syncwarp();
 #pragma unroll 1
-                for (int t = 0; t < min(UPOS, p.kv1 - p0); t++) {
-                    float v[2 * KS];  // columns 8 c + g
+            for (int h0 = 0; h0 < UPOS; h0 += 16 * MT) {  // 16 MT positions
+                float s[NQ][MT][4];
 #pragma unroll
-                    for (int c = 0; c < 2 * KS; c++)
-                        v[c] = __bfloat162float(*reinterpret_cast<const bf16 *>(
-                            stage + (NB + c / 8) * (UPOS * 128) + t * 128 + (((c % 8) ^ (t & 7)) << 4) + 2 * g));
+                for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        if (p0 + t >= lim[e]) continue;
-                        const float w = ps[t * SMALL_ROWS + 2 * tq + e];
+                    for (int i = 0; i < MT; i++) s[nq][i][0] = s[nq][i][1] = s[nq][i][2] = s[nq][i][3] = 0.0f;
 #pragma unroll
-                        for (int c = 0; c < 2 * KS; c++) o[c / 2][c % 2 * 2 + e] += w * v[c];
+                for (int k = 0; k < KS; k++) {
+                    const int c = 2 * k + (mi >> 1);
+                    const uint32_t at = kb + h0 * 128 + k_row + (k / 4) * (UPOS * 128) + (((c % 8) ^ l7) << 4);
+                    uint2 q[NQ];
+#pragma unroll
+                    for (int nq = 0; nq < NQ; nq++) q[nq] = NQ == 1 ? qb[k] : q_s[(k * NQ + nq) * 32 + lane];
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        uint32_t ka[4];
+                        ldsm4(ka, at + i * 16 * 128);
+#pragma unroll
+                        for (int nq = 0; nq < NQ; nq++) mma16816(s[nq][i], ka, q[nq].x, q[nq].y);
                     }
                 }
-                __syncwarp();
+#pragma unroll
+                for (int nq = 0; nq < NQ; nq++) {
+                    float x[2] = {-INFINITY, -INFINITY};
+                    const int2 lim = masked ? limits(nq) : make_int2(INT_MAX, INT_MAX);
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            s[nq][i][j] *= a.scale_log2;
+                            if (p0 + h0 + 16 * i + 8 * (j >> 1) + g >= (j & 1 ? lim.y : lim.x)) s[nq][i][j] = -INFINITY;
+                            x[j & 1] = fmaxf(x[j & 1], s[nq][i][j]);
+                        }
+#pragma unroll
+                    for (int off = 4; off < 32; off *= 2) {
+                        x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], off));
+                        x[1] = fmaxf(x[1], __shfl_xor_sync(0xffffffffu, x[1], off));
+                    }
+                    if (__any_sync(0xffffffffu, x[0] > m[nq][0] || x[1] > m[nq][1])) {
+                        float f[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float top = fmaxf(m[nq][e], x[e]);
+                            f[e] = top == -INFINITY ? 1.0f : ex2(m[nq][e] - top);
+                            m[nq][e] = top;
+                            l[nq][e] *= f[e];
+                        }
+#pragma unroll
+                        for (int i = 0; i < KS; i++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) o[nq][i][j] *= f[j & 1];
+                    }
+                    const float base[2] = {m[nq][0] == -INFINITY ? 0.0f : m[nq][0], m[nq][1] == -INFINITY ? 0.0f : m[nq][1]};
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            s[nq][i][j] = ex2(s[nq][i][j] - base[j & 1]);
+                            l[nq][j & 1] += s[nq][i][j];
+                        }
+                }
+                if (!slow) {
+#pragma unroll
+                    for (int t = 0; t < MT; t++) {
+                        uint32_t pb[NQ][2];
+#pragma unroll
+                        for (int nq = 0; nq < NQ; nq++) {
+                            pb[nq][0] = transpose8(pack_bf16(s[nq][t][0], s[nq][t][1]));
+                            pb[nq][1] = transpose8(pack_bf16(s[nq][t][2], s[nq][t][3]));
+                        }
+#pragma unroll
+                        for (int i = 0; i < KS; i++) {
+                            const int c = 2 * i + (mi & 1);
+                            uint32_t va[4];
+                            ldsm4_t(va, vb + h0 * 128 + v_row + t * 16 * 128 + (i / 4) * (UPOS * 128) + (((c % 8) ^ l7) << 4));
+#pragma unroll
+                            for (int nq = 0; nq < NQ; nq++) mma16816(o[nq][i], va, pb[nq][0], pb[nq][1]);
+                        }
+                    }
+                } else {  // position by position, skipping what each row does not see; the probabilities by way of this
+                          // warp's part of the merge buffer, [16 MT][8]
+                    float *ps = merge_o + cw * 8 * DP;
+#pragma unroll
+                    for (int nq = 0; nq < NQ; nq++) {
+                        const int2 lim = limits(nq);
+#pragma unroll
+                        for (int i = 0; i < MT; i++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) ps[(16 * i + 8 * (j >> 1) + g) * 8 + 2 * tq + (j & 1)] = s[nq][i][j];
+                        __syncwarp();
+#pragma unroll 1
+                        for (int t = h0; t < h0 + 16 * MT; t++) {
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                if (p0 + t >= (e ? lim.y : lim.x)) continue;
+                                const float w = ps[(t - h0) * 8 + 2 * tq + e];
+#pragma unroll
+                                for (int c = 0; c < 2 * KS; c++)  // columns 8 c + g
+                                    o[nq][c / 2][c % 2 * 2 + e] +=
+                                        w * __bfloat162float(*reinterpret_cast<const bf16 *>(
+                                                stage + (NB + c / 8) * (UPOS * 128) + t * 128 + (((c % 8) ^ (t & 7)) << 4) + 2 * g));
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
             }
-            if (touched) fence_proxy_async();  // these writes, before the next TMA write of the stage
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[r.s]);
         }
@@ -424,26 +460,6 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
     } while (p0 < p.kv1);
 
     // ---- merge the warps
-#pragma unroll
-    for (int off = 4; off < 32; off *= 2) {
-        l[0] += __shfl_xor_sync(0xffffffffu, l[0], off);
-        l[1] += __shfl_xor_sync(0xffffffffu, l[1], off);
-    }
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-        const int row = 2 * tq + e;
-        if (row < rows) {
-            float *dst = merge_o + (cw * SMALL_ROWS + row) * DP;
-#pragma unroll
-            for (int i = 0; i < KS; i++) {
-                dst[(16 * i + g) ^ (tq * 8)] = o[i][e];
-                dst[(16 * i + 8 + g) ^ (tq * 8)] = o[i][2 + e];
-            }
-            if (g == 0) merge_ml[cw * SMALL_ROWS + row] = make_float2(m[e], l[e]);
-        }
-    }
-    bar_sync(1, NW * 32);
-    const int tid = cw * 32 + lane;
     // four columns of a row of the output; a row without positions is zero
     auto put = [&](int row, int d, const float *acc, float sum) {
         const float inv = 1.0f / sum;
@@ -453,29 +469,60 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
                 p.pos0 + row / a.rep < 0 ? make_uint2(0u, 0u)
                                          : make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
     };
-    for (int i = tid; i < rows * (DP / 4); i += NW * 32) {
-        const int row = i / (DP / 4), d = i % (DP / 4) * 4;
-        float top = -INFINITY, sum = 0.0f, acc[4] = {};
 #pragma unroll
-        for (int w = 0; w < NW; w++) top = fmaxf(top, merge_ml[w * SMALL_ROWS + row].x);
-        const float base = top == -INFINITY ? 0.0f : top;
+    for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
-        for (int w = 0; w < NW; w++) {
-            const float2 ml = merge_ml[w * SMALL_ROWS + row];
-            const float f = ex2(ml.x - base);
-            const float4 v = *reinterpret_cast<const float4 *>(merge_o + (w * SMALL_ROWS + row) * DP + (d ^ ((row >> 1 & 3) * 8)));
-            sum += f * ml.y;
-            acc[0] += f * v.x;
-            acc[1] += f * v.y;
-            acc[2] += f * v.z;
-            acc[3] += f * v.w;
+        for (int off = 4; off < 32; off *= 2) {
+            l[nq][0] += __shfl_xor_sync(0xffffffffu, l[nq][0], off);
+            l[nq][1] += __shfl_xor_sync(0xffffffffu, l[nq][1], off);
         }
-        if (p.part < 0) {
-            put(row, d, acc, sum);
-        } else {
-            const size_t at = (size_t)p.part * SMALL_ROWS + row;
-            __stcg(reinterpret_cast<float4 *>(a.small_o + at * DP + d), make_float4(acc[0], acc[1], acc[2], acc[3]));
-            if (d == 0) __stcg(a.small_ml + at, make_float2(top, sum));
+#pragma unroll 1
+    for (int at = 0; at < NQ; at++) {
+        const int here = min(8, rows - 8 * at);
+        if (here <= 0) break;
+        if (at > 0) bar_sync(1, NW * 32);  // the tile before has been read
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) {
+            if (nq != at) continue;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int row = 2 * tq + e;
+                if (row < here) {
+                    float *dst = merge_o + (cw * 8 + row) * DP;
+#pragma unroll
+                    for (int i = 0; i < KS; i++) {
+                        dst[(16 * i + g) ^ (tq * 8)] = o[nq][i][e];
+                        dst[(16 * i + 8 + g) ^ (tq * 8)] = o[nq][i][2 + e];
+                    }
+                    if (g == 0) merge_ml[cw * 8 + row] = make_float2(m[nq][e], l[nq][e]);
+                }
+            }
+        }
+        bar_sync(1, NW * 32);
+        for (int i = tid; i < here * (DP / 4); i += NW * 32) {
+            const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+            float top = -INFINITY, sum = 0.0f, acc[4] = {};
+#pragma unroll
+            for (int w = 0; w < NW; w++) top = fmaxf(top, merge_ml[w * 8 + row].x);
+            const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const float2 ml = merge_ml[w * 8 + row];
+                const float f = ex2(ml.x - base);
+                const float4 v = *reinterpret_cast<const float4 *>(merge_o + (w * 8 + row) * DP + (d ^ ((row >> 1 & 3) * 8)));
+                sum += f * ml.y;
+                acc[0] += f * v.x;
+                acc[1] += f * v.y;
+                acc[2] += f * v.z;
+                acc[3] += f * v.w;
+            }
+            if (p.part < 0) {
+                put(8 * at + row, d, acc, sum);
+            } else {
+                const size_t to = (size_t)p.part * (8 * NQ) + 8 * at + row;
+                __stcg(reinterpret_cast<float4 *>(a.small_o + to * DP + d), make_float4(acc[0], acc[1], acc[2], acc[3]));
+                if (d == 0) __stcg(a.small_ml + to, make_float2(top, sum));
+            }
         }
     }
     if (p.part >= 0) {  // the item's last piece to finish adds the parts up, in their order
@@ -489,11 +536,11 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
                 const int row = i / (DP / 4), d = i % (DP / 4) * 4;
                 float top = -INFINITY, sum = 0.0f, acc[4] = {};
                 for (int w = 0; w < p.n_parts; w++)
-                    top = fmaxf(top, __ldcg(a.small_ml + (size_t)part_slot(p.first, w) * SMALL_ROWS + row).x);
+                    top = fmaxf(top, __ldcg(a.small_ml + (size_t)part_slot(p.first, w) * (8 * NQ) + row).x);
                 const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll 4
                 for (int w = 0; w < p.n_parts; w++) {
-                    const size_t at = (size_t)part_slot(p.first, w) * SMALL_ROWS + row;
+                    const size_t at = (size_t)part_slot(p.first, w) * (8 * NQ) + row;
                     const float2 ml = __ldcg(a.small_ml + at);
                     const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.small_o + at * DP + d));
                     const float f = ex2(ml.x - base);
@@ -513,26 +560,28 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
 
 // ---------------------------------------------------------------- kernel for few rows alone
 
-constexpr int SMALL_WARPS = 10, SMALL_STAGES = 10;
+constexpr int SMALL_WARPS = 10;  // consumers, each with a stage of its own
 
-template <int DP>
+template <int DP, int NQ>
 struct SmallSmem {
-    alignas(1024) unsigned char ring[SMALL_STAGES * SMALL_STAGE];
-    float merge_o[SMALL_WARPS * SMALL_ROWS * DP];
-    float2 merge_ml[SMALL_WARPS * SMALL_ROWS];
-    uint64_t full[SMALL_STAGES], empty[SMALL_STAGES];
+    alignas(1024) unsigned char ring[SMALL_WARPS * SMALL_STAGE];
+    float merge_o[SMALL_WARPS * 8 * DP];
+    float2 merge_ml[SMALL_WARPS * 8];
+    uint2 q[NQ == 1 ? 1 : DP / 16 * NQ * 32];
+    int2 lim[4 * NQ];
+    uint64_t full[SMALL_WARPS], empty[SMALL_WARPS];
     int flag;
 };
 
-template <int DP>
+template <int DP, int NQ>
 __global__ void __launch_bounds__((SMALL_PRODUCERS + SMALL_WARPS) * 32, 1)
     paged_small_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                        const __grid_constant__ PaArgs a) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    SmallSmem<DP> &sm = *reinterpret_cast<SmallSmem<DP> *>(align_shared<1024>(smem_raw));
+    SmallSmem<DP, NQ> &sm = *reinterpret_cast<SmallSmem<DP, NQ> *>(align_shared<1024>(smem_raw));
     const int warp = threadIdx.x / 32;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < SMALL_STAGES; i++) {
+        for (int i = 0; i < SMALL_WARPS; i++) {
             mbar_init(&sm.full[i], 1);
             mbar_init(&sm.empty[i], 1);
         }
@@ -547,16 +596,16 @@ __global__ void __launch_bounds__((SMALL_PRODUCERS + SMALL_WARPS) * 32, 1)
     if (!a.after_big) pdl_wait();
     const int2 work = a.ctas[blockIdx.x];
     if (work.y < 0) zero_rows(a);
-    Ring<SMALL_STAGES> r;
+    Ring<SMALL_WARPS> r;
     Waiter wait;
     for (int i = 0; i < work.y; i++) {
         const PagedPiece p = a.pieces[work.x + i];
         // every load is waited for by a consumer before the CTA ends
         if (warp >= SMALL_WARPS)
-            small_produce<DP, SMALL_STAGES, SMALL_PRODUCERS>(a, &mk, &mv, p, sm.ring, sm.full, sm.empty, r, warp - SMALL_WARPS, wait,
+            small_produce<DP, SMALL_WARPS, SMALL_PRODUCERS>(a, &mk, &mv, p, sm.ring, sm.full, sm.empty, r, warp - SMALL_WARPS, wait,
                                                              a.small_step_pages, a.small_step_slots);
         else
-            small_consume<DP, SMALL_WARPS, SMALL_STAGES>(a, p, sm.ring, sm.full, sm.empty, r, wait, warp, sm.merge_o, sm.merge_ml,
+            small_consume<DP, NQ, SMALL_WARPS, SMALL_WARPS>(a, p, sm.ring, sm.full, sm.empty, r, wait, warp, sm.q, sm.lim, sm.merge_o, sm.merge_ml,
                                                          &sm.flag);
     }
     if (a.after_big) pdl_wait();  // whoever waits for this kernel waits for that one, too
@@ -1212,6 +1261,14 @@ bool make_query_map(CUtensorMap *map, const PagedAttnCall &c, const PaArgs &a) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <int DP, int NQ>
+cudaError_t launch_small(const CUtensorMap &mk, const CUtensorMap &mv, const PaArgs &a, cudaStream_t s) {
+    const size_t smem = sizeof(SmallSmem<DP, NQ>) + 1024;
+    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(paged_small_kernel<DP, NQ>), smem);
+    if (e != cudaSuccess) return e;
+    return launch(paged_small_kernel<DP, NQ>, dim3(paged_ctas()), dim3((SMALL_PRODUCERS + SMALL_WARPS) * 32), smem, s, 1, mk, mv, a);
+}
+
 template <int DP>
 int run(const PagedAttnCall &c, PaArgs &a, cudaStream_t s) {
     CUtensorMap mk, mv;
@@ -1237,10 +1294,11 @@ int run(const PagedAttnCall &c, PaArgs &a, cudaStream_t s) {
         Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_big_kernel<DP>), big_smem));
         Q3_TRY_LAUNCH(launch(paged_big_kernel<DP>, dim3(paged_ctas()), dim3(BIG_THREADS), big_smem, s, 1, mq, mk_big, mv_big, a));
     }
-    const size_t smem = sizeof(SmallSmem<DP>) + 1024;
-    Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_small_kernel<DP>), smem));
-    Q3_TRY_LAUNCH(launch(paged_small_kernel<DP>, dim3(paged_ctas()), dim3((SMALL_PRODUCERS + SMALL_WARPS) * 32), smem, s, 1, mk,
-                         mv, a));
+    const int tiles = paged_small_rows(c.shape) / 8;
+    if (tiles == 1) Q3_TRY_LAUNCH((launch_small<DP, 1>(mk, mv, a, s)));
+    if (tiles == 2) Q3_TRY_LAUNCH((launch_small<DP, 2>(mk, mv, a, s)));
+    if constexpr (DP == 64)
+        if (tiles == 3) Q3_TRY_LAUNCH((launch_small<DP, 3>(mk, mv, a, s)));
     if (!a.after_big) return Q3_OK;
     Q3_TRY_LAUNCH(launch(paged_combine_kernel<DP>, dim3(paged_ctas(), DP / 16), dim3(2 * BIG_TILE), 0, s, 1, a));
     return Q3_OK;

@@ -467,3 +467,32 @@ def test_many_short_chunks_beside_long_decodes():
     assert q3.device_error() == 0
     assert torch.equal(out, again[0]) and torch.equal(out, again[1])
     check_attention(out, *b.attention_exact(q, 128 ** -0.5), "short chunks and long decodes")
+
+
+# draft tokens being verified: a few rows per kv head, in one to three tiles of the kernel for few rows
+@pytest.mark.parametrize("heads,kvh,dim,most", [(32, 8, 128, 4), (16, 8, 128, 8), (8, 8, 128, 11), (12, 2, 96, 2), (6, 2, 40, 7),
+                                                (32, 4, 64, 3), (4, 2, 64, 12), (64, 8, 128, 2), (40, 2, 64, 1)])
+@pytest.mark.parametrize("page", [8, 48])
+def test_draft_tokens_match_definition(heads, kvh, dim, most, page):
+    kv = (1, 2, 31, 32, 33, 64, 65, 127, 320, 1500, 4097)
+    lens = [(min(1 + i * most // 8, most), max(n, i % 3)) for i, n in enumerate(kv)] + [(most, most - 1), (most, 0), (0, 50)]
+    b = Batch(lens, heads, kvh, dim, page, seed=heads + page + most, fill=NAN)
+    q = rn(b.g, b.tokens, heads, dim, std=1.5)
+    out = attend(b, q)
+    check_attention(out, *b.attention_exact(q, dim ** -0.5), f"drafts {heads}/{kvh}x{dim} page {page}")
+    assert torch.equal(out, attend(b, q))
+    assert q3.device_error() == 0
+
+
+@pytest.mark.parametrize("heads,kvh,dim,n", [(32, 8, 128, 4), (8, 8, 128, 13), (32, 4, 64, 3), (4, 2, 64, 9)])
+def test_bad_values_stay_behind_the_mask_of_drafts(heads, kvh, dim, n):
+    for kv in (n, 40, 96, 97, 700):
+        for value in (NAN, float("inf")):
+            b = Batch([(n, kv), (1, 30)], heads, kvh, dim, 16, seed=n + kv, fill=NAN)
+            q = rn(b.g, b.tokens, heads, dim)
+            where = kv - n + n // 2
+            page, slot = b.table[0, where // 16].item(), where % 16
+            b.vp[page, 0, slot, 5] = value
+            b.vp[page, 1, slot, dim - 1] = -value
+            exact, mag = b.attention_exact(q, dim ** -0.5)
+            check_attention(attend(b, q), exact, mag, f"value {value} at {where} of {kv}")
