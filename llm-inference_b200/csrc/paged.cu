@@ -25,7 +25,7 @@ struct PlanArgs {
     PagedPlanLayout l;
     q3_paged_shape s;
     const int *q_start, *kv_len, *page_table;
-    int n_ctas, small_step, small_rows;
+    int n_ctas, small_shift, small_rows;  // a small item's step is 1 << small_shift positions
 };
 
 // Costs, in units of a kind's own: a step of a small item is one, the 16 KB load that it waits for; a 128-position step of
@@ -51,10 +51,10 @@ __device__ __forceinline__ SeqItems seq_items(const PagedSeq &q, int rep, int sm
 }
 
 // Item i's positions end here, it has this many steps, and each costs this much.
-__device__ __forceinline__ void item_steps(const PagedSeq &q, const SeqItems &s, int i, int step, int *end, int *n, int *cost) {
+__device__ __forceinline__ void item_steps(const PagedSeq &q, const SeqItems &s, int i, int shift, int *end, int *n, int *cost) {
     const int last = min((i + 1) * s.span, q.q_len);
     *end = max(0, q.kv_len - q.q_len + last);
-    *n = max(1, (*end + step - 1) / step);
+    *n = max(1, (*end + (1 << shift) - 1) >> shift);
     *cost = !s.big ? 1 : last - i * s.span > s.span / 2 ? COST_BIG_TWO : COST_BIG_ONE;
 }
 
@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     long long *small_s = big_s + a.s.n_seqs + 1;                  // and before its small ones
     long long *item_s = small_s + a.s.n_seqs + 1;                 // items before: big ones << 32 | small ones
     int *start_s = reinterpret_cast<int *>(item_s + a.s.n_seqs + 1);
+    int *kv_s = start_s + a.s.n_seqs + 1;
     __shared__ long long sums_s[PLAN_THREADS / 32];
     pdl_trigger();
     pdl_wait();
@@ -130,10 +131,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
         bad = __any_sync(0xffffffffu, bad);
         if (lane == 0) {
             if (bad) atomicOr(&g_dev_error, DEV_ERR_POS_RANGE);
+            kv_s[b] = bad ? 0 : kv;
             seqs[b] = {bad_starts ? 0 : q0, bad_starts ? 0 : q_len, bad ? 0 : kv, 0};
         }
     }
     __syncthreads();
+    auto seq = [&](int b) -> PagedSeq {
+        return bad_starts ? PagedSeq{0, 0, 0, 0} : PagedSeq{start_s[b], start_s[b + 1] - start_s[b], kv_s[b], 0};
+    };
     for (int t = tid; t < a.s.n_tokens; t += PLAN_THREADS) {
         int4 tok = make_int4(-1, bad_starts ? -1 : PAGED_OUTSIDE, -1, -1);
         if (!bad_starts && n > 0 && t >= start_s[0] && t < start_s[n]) {
@@ -143,7 +148,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
                 if (start_s[mid] <= t) lo = mid;
                 else hi = mid - 1;
             }
-            const PagedSeq q = seqs[lo];
+            const PagedSeq q = seq(lo);
             const int pos = q.kv_len - q.q_len + (t - q.q0);
             tok.x = lo;
             tok.y = pos < 0 ? -1 : pos;
@@ -157,14 +162,15 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
 
     // ---- work
     const int rep = a.s.n_heads / a.s.n_kv_heads, kvh = a.s.n_kv_heads;
-    const int small_step = a.small_step;
+    constexpr int BIG_SHIFT = 7;
+    static_assert(1 << BIG_SHIFT == BIG_TILE, "a step of a big item");
     for (int b = tid; b < n; b += PLAN_THREADS) {
-        const PagedSeq q = seqs[b];
+        const PagedSeq q = seq(b);
         const SeqItems s = seq_items(q, rep, a.small_rows);
         long long cost = 0;
         for (int i = 0; i < s.n_q; i++) {
             int end, steps, c;
-            item_steps(q, s, i, s.big ? BIG_TILE : small_step, &end, &steps, &c);
+            item_steps(q, s, i, s.big ? BIG_SHIFT : a.small_shift, &end, &steps, &c);
             cost += s.ends() + (long long)steps * c;
         }
         big_s[b] = s.big ? cost * kvh : 0;
@@ -198,7 +204,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     // A CTA's pieces start at (items before its first) + (CTAs before it): every cut adds one piece at most.
     for (int id = tid; id < 2 * a.n_ctas; id += PLAN_THREADS) {
         const bool big = id >= a.n_ctas;
-        const int c = big ? id - a.n_ctas : id, step = big ? BIG_TILE : small_step;
+        const int c = big ? id - a.n_ctas : id, shift = big ? BIG_SHIFT : a.small_shift;
         const long long total = big ? total_big : total_small;
         const long long *pre = big ? big_s : small_s;
         const int used = big ? used_big : used_small;
@@ -206,26 +212,39 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
         const long long u0 = c < used ? bound(c) : total, u1 = c < used ? bound(c + 1) : total;
         int count = 0, first_piece = -1;
         PagedPiece split = {};
-        long long u = u0;
-        while (u < u1) {
-            int lo = 0, hi = n - 1;  // the last sequence that starts at or before u
+        long long u = u0, start = u0;  // of the item
+        int lo = 0, head = 0, i = 0;
+        PagedSeq q = {};
+        SeqItems s = {};
+        if (u < u1) {  // the item that holds u0; then one after the other
+            int hi = n - 1;  // the last sequence that starts at or before u
             while (lo < hi) {
                 const int mid = (lo + hi + 1) / 2;
                 if (pre[mid] <= u) lo = mid;
                 else hi = mid - 1;
             }
-            const PagedSeq q = seqs[lo];
-            const SeqItems s = seq_items(q, rep, a.small_rows);
+            q = seq(lo);
+            s = seq_items(q, rep, a.small_rows);
             const long long per_head = (pre[lo + 1] - pre[lo]) / kvh;
-            const int head = (int)((u - pre[lo]) / per_head);
-            long long start = pre[lo] + head * per_head;
-            int i = 0, end, steps, cost;
+            head = (int)((u - pre[lo]) / per_head);
+            start = pre[lo] + head * per_head;
+        }
+        while (u < u1) {
+            int end, steps, cost;
             long long len;
-            for (;; i++) {
-                item_steps(q, s, i, step, &end, &steps, &cost);
+            for (;;) {  // all lanes look first, then all write
+                item_steps(q, s, i, shift, &end, &steps, &cost);
                 len = s.ends() + (long long)steps * cost;
                 if (u < start + len) break;
                 start += len;
+                if (++i < s.n_q) continue;
+                i = 0;
+                if (++head < kvh) continue;
+                head = 0;
+                do lo++;
+                while (pre[lo + 1] == pre[lo]);  // u < total: there is one
+                q = seq(lo);
+                s = seq_items(q, rep, a.small_rows);
             }
             const int t0 = steps_before(u - start, s.ends(), steps, cost);
             const int t1 = u1 >= start + len ? steps : steps_before(u1 - start, s.ends(), steps, cost);
@@ -235,8 +254,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
                 p.kvh = head;
                 p.tok0 = q.q0 + i * s.span;
                 p.n_tok = min(s.span, q.q_len - i * s.span);
-                p.kv0 = t0 * step;
-                p.kv1 = t1 == steps ? end : t1 * step;
+                p.kv0 = t0 << shift;
+                p.kv1 = t1 == steps ? end : t1 << shift;
                 p.kv_end = end;
                 p.pos0 = q.kv_len - q.q_len + i * s.span;
                 p.big = big;
@@ -561,8 +580,8 @@ int q3_paged_plan(void *plan, const q3_paged_shape *shape, const int *q_start, c
     if (!aligned16(plan)) return Q3_ERR_ALIGN;
     TRY(check_device());
     PlanArgs a = {static_cast<char *>(plan), paged_plan_layout(*shape), *shape, q_start, kv_len, page_table,
-                  paged_ctas(), paged_small_step(*shape), paged_small_rows(*shape)};
-    const size_t smem = (size_t)(shape->n_seqs + 1) * (3 * sizeof(long long) + sizeof(int));
+                  paged_ctas(), __builtin_ctz(paged_small_step(*shape)), paged_small_rows(*shape)};
+    const size_t smem = (size_t)(shape->n_seqs + 1) * (3 * sizeof(long long) + 2 * sizeof(int));
     Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_plan_kernel), smem));
     Q3_TRY_LAUNCH(launch(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), smem, (cudaStream_t)stream, 1, a));
     return Q3_OK;
