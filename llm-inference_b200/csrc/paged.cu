@@ -17,7 +17,8 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 // ------------------------------------------------------------------ plan
 // One CTA. The description is checked here once, so that the kernels of every layer can use the
-// plan's copy of the page table and the token map without checks of their own.
+// plan's copy of the page table and the token map without checks of their own. Latency bounds it: 10 us for one sequence,
+// 16 for 32 of 64 pages, 27 for four chunks of 2048 tokens, once per step.
 constexpr int PLAN_THREADS = 1024;
 
 struct PlanArgs {
@@ -26,6 +27,7 @@ struct PlanArgs {
     q3_paged_shape s;
     const int *q_start, *kv_len, *page_table;
     int n_ctas, small_shift, small_rows;  // a small item's step is 1 << small_shift positions
+    bool has_big;
 };
 
 // Costs, in units of a kind's own: a step of a small item is one, the 16 KB load that it waits for; a 128-position step of
@@ -42,10 +44,12 @@ struct SeqItems {
     __device__ __forceinline__ int ends() const { return big ? COST_BIG_ITEM : COST_ITEM; }
 };
 
-__device__ __forceinline__ SeqItems seq_items(const PagedSeq &q, int rep, int small_rows) {
+// A step without the kernel for many rows may still describe a sequence with more of them than it may have. It
+// has no positions then, but its rows are written: as items of what a small one holds.
+__device__ __forceinline__ SeqItems seq_items(const PagedSeq &q, int rep, const PlanArgs &a) {
     SeqItems s;
-    s.big = (long long)q.q_len * rep > small_rows;
-    s.span = s.big ? 2 * (BIG_TILE / rep) : q.q_len;
+    s.big = a.has_big && (long long)q.q_len * rep > a.small_rows;
+    s.span = s.big ? 2 * (BIG_TILE / rep) : max(1, a.small_rows / rep);
     s.n_q = q.q_len == 0 ? 0 : (q.q_len + s.span - 1) / s.span;
     return s;
 }
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     static_assert(1 << BIG_SHIFT == BIG_TILE, "a step of a big item");
     for (int b = tid; b < n; b += PLAN_THREADS) {
         const PagedSeq q = seq(b);
-        const SeqItems s = seq_items(q, rep, a.small_rows);
+        const SeqItems s = seq_items(q, rep, a);
         long long cost = 0;
         for (int i = 0; i < s.n_q; i++) {
             int end, steps, c;
@@ -224,7 +228,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
                 else hi = mid - 1;
             }
             q = seq(lo);
-            s = seq_items(q, rep, a.small_rows);
+            s = seq_items(q, rep, a);
             const long long per_head = (pre[lo + 1] - pre[lo]) / kvh;
             head = (int)((u - pre[lo]) / per_head);
             start = pre[lo] + head * per_head;
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
                 do lo++;
                 while (pre[lo + 1] == pre[lo]);  // u < total: there is one
                 q = seq(lo);
-                s = seq_items(q, rep, a.small_rows);
+                s = seq_items(q, rep, a);
             }
             const int t0 = steps_before(u - start, s.ends(), steps, cost);
             const int t1 = u1 >= start + len ? steps : steps_before(u1 - start, s.ends(), steps, cost);
@@ -291,11 +295,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
 // (up to 512 threads) where they are few. A unit is two 8-element chunks of a head that one lane holds in
 // registers: for half-split pairs chunk u and its partner u + rope_dim/16, so a pair's two elements sit in one
 // lane; otherwise neighbours. A head is a group of `lph` lanes (a power of two), so the sum of squares is a few
-// shuffles. The angles depend on the token alone: the CTA computes them once, then every lane keeps its pairs' in
-// registers. A lane's first query head and first key or value head are asked for before that.
+// shuffles. The angles depend on the token alone: the CTA computes them once, into shared memory, where lanes read
+// theirs for every head (held in registers they cost occupancy: 44 us against 40.5 below). A lane's first query head is
+// asked for before that.
 //
-// With many tokens the instructions bound it before the bytes do (360 a warp and four heads, 44 us for 8192 tokens of 48
-// heads, before the packed arithmetic and one loop per kind of head); with few, the chain plan -> angle -> heads.
+// With many tokens the instructions bound it about as much as the bytes: 8192 tokens of 48 heads of 128 take 40.5 us
+// (5.0 TB/s, 0.77 of the measured copy bandwidth) with packed arithmetic and a loop per kind of head, 43 without. With
+// few, the chain plan -> angle -> heads: 2.5 us for one token.
 //
 // The angle is reduced in fp64: pos * inv_freq reaches 10^5 rad and more, where an fp32 product is
 // off by up to 2^-25 of itself, more than a bf16 result may be. turns = pos * inv_freq / 2 pi, its
@@ -580,7 +586,7 @@ int q3_paged_plan(void *plan, const q3_paged_shape *shape, const int *q_start, c
     if (!aligned16(plan)) return Q3_ERR_ALIGN;
     TRY(check_device());
     PlanArgs a = {static_cast<char *>(plan), paged_plan_layout(*shape), *shape, q_start, kv_len, page_table,
-                  paged_ctas(), __builtin_ctz(paged_small_step(*shape)), paged_small_rows(*shape)};
+                  paged_ctas(), __builtin_ctz(paged_small_step(*shape)), paged_small_rows(*shape), paged_has_big(*shape)};
     const size_t smem = (size_t)(shape->n_seqs + 1) * (3 * sizeof(long long) + 2 * sizeof(int));
     Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_plan_kernel), smem));
     Q3_TRY_LAUNCH(launch(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), smem, (cudaStream_t)stream, 1, a));

@@ -1,6 +1,8 @@
 // Layout of a paged step's plan (paged.cu writes it, the append and attention kernels read it).
 #pragma once
 
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace q3 {
@@ -36,6 +38,21 @@ struct alignas(16) PagedPiece {
 // later ones are the first of theirs (slot 2c).
 __host__ __device__ __forceinline__ int part_slot(int first, int i) { return i == 0 ? 2 * first + 1 : 2 * (first + i); }
 
+// Rows of the kernel for few rows: eight for each 8-column tile of its products. Where every sequence fits into a
+// few tiles (draft tokens being verified) the step needs no other kernel; where some do not, it is the one for single
+// tokens, and all longer sequences go to the kernel for many rows. 32 sequences at 4096, 8 kv heads of 128: 16 rows take
+// 90 us here and 120 there, 24 rows 152 and 120 (their accumulators spill); 4 kv heads of 64: 16 rows 31 and 59,
+// 24 rows 38 and 60, 40 rows 64 and 59.
+inline int paged_small_rows(const q3_paged_shape &s) {
+    const long long most = (long long)s.max_q_len * (s.n_heads / s.n_kv_heads);
+    if (most > (s.head_dim <= 64 ? 24 : 16) || most <= 8) return 8;
+    return most <= 16 ? 16 : 24;
+}
+// One query head group alone may be too many; a batch that may bring no tokens at all counts as bringing one.
+inline bool paged_has_big(const q3_paged_shape &s) {
+    return (long long)std::max(s.max_q_len, 1) * (s.n_heads / s.n_kv_heads) > paged_small_rows(s);
+}
+
 // Byte offsets of the plan's parts; the same arithmetic on host and device.
 struct PagedPlanLayout {
     size_t seqs;      // PagedSeq [n_seqs]
@@ -50,8 +67,6 @@ struct PagedPlanLayout {
     size_t bytes;
 };
 
-inline int paged_tile_tokens(const q3_paged_shape &s) { return BIG_TILE / (s.n_heads / s.n_kv_heads); }
-
 inline PagedPlanLayout paged_plan_layout(const q3_paged_shape &s) {
     PagedPlanLayout l = {};
     size_t off = 0;
@@ -60,7 +75,8 @@ inline PagedPlanLayout paged_plan_layout(const q3_paged_shape &s) {
         off += (bytes + 255) / 256 * 256;
         return o;
     };
-    const size_t items = (size_t)s.n_kv_heads * ((size_t)s.n_seqs + (size_t)s.n_tokens / (2 * paged_tile_tokens(s)));
+    const int rep = s.n_heads / s.n_kv_heads, span = paged_has_big(s) ? 2 * (BIG_TILE / rep) : paged_small_rows(s) / rep;
+    const size_t items = (size_t)s.n_kv_heads * ((size_t)s.n_seqs + (size_t)s.n_tokens / span);
     l.seqs = take((size_t)s.n_seqs * sizeof(PagedSeq));
     l.table = take((size_t)s.n_seqs * s.max_pages * 4);
     l.toks = take((size_t)s.n_tokens * 16);
@@ -77,20 +93,6 @@ inline PagedPlanLayout paged_plan_layout(const q3_paged_shape &s) {
 struct PagedScratchLayout {
     size_t small_o, small_ml, big_o, big_ml, bytes;
 };
-
-// Rows of the kernel for few rows: eight for each 8-column tile of its products. Where every sequence fits into a
-// few tiles (draft tokens being verified) the step needs no other kernel; where some do not, it is the one for single
-// tokens, and all longer sequences go to the kernel for many rows. 32 sequences at 4096, 8 kv heads of 128: 16 rows take
-// 90 us here and 120 there, 24 rows 152 and 120 (their accumulators spill); 4 kv heads of 64: 16 rows 31 and 59,
-// 24 rows 38 and 60, 40 rows 64 and 59.
-inline int paged_small_rows(const q3_paged_shape &s) {
-    const long long most = (long long)s.max_q_len * (s.n_heads / s.n_kv_heads);
-    if (most > (s.head_dim <= 64 ? 24 : 16) || most <= 8) return 8;
-    return most <= 16 ? 16 : 24;
-}
-inline bool paged_has_big(const q3_paged_shape &s) {
-    return (long long)s.max_q_len * (s.n_heads / s.n_kv_heads) > paged_small_rows(s);
-}
 
 // A step of a small item is one ring stage of K and V; pieces are cut at multiples of it.
 constexpr int SMALL_STAGE = 16384;  // bytes

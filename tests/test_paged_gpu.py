@@ -496,3 +496,16 @@ def test_bad_values_stay_behind_the_mask_of_drafts(heads, kvh, dim, n):
             b.vp[page, 1, slot, dim - 1] = -value
             exact, mag = b.attention_exact(q, dim ** -0.5)
             check_attention(attend(b, q), exact, mag, f"value {value} at {where} of {kv}")
+
+
+# more tokens than the shape allows, in a step whose shape needs no kernel for many rows
+@pytest.mark.parametrize("heads,kvh,most", [(8, 2, 1), (8, 2, 4), (8, 8, 1), (32, 2, 0), (4, 2, 0)])
+def test_too_many_tokens_are_padding(heads, kvh, most):
+    b = Batch([(most, 40), (37, 50), (0, 9), (most, 7)], heads, kvh, 64, 16, seed=heads, max_q=most)
+    b.bad = [False, True, False, False]
+    q = rn(b.g, b.tokens, heads, 64)
+    out = attend(b, q)
+    assert q3.device_error() == 4
+    b.lens[1] = (37, 0)
+    check_attention(out, *b.attention_exact(q, 0.125), "too many tokens")
+    assert not out[b.rows(1)].any()
