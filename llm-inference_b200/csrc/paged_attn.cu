@@ -6,19 +6,23 @@
 // grows. Partial results (o, m, l) of a row over disjoint positions combine as
 // m = max m_i, o = sum 2^(m_i - m) o_i, l = sum 2^(m_i - m) l_i.
 //
-// Persistent CTAs, one per SM, take the pieces the plan gave them (paged.cuh). A producer warp
-// streams K and V by TMA, one box per run of positions inside a page, into a ring of 16 KB stages; what
-// consumes them depends on the item's rows.
+// Persistent CTAs, one per SM, take the pieces the plan gave them (paged.cuh). Two producer warps stream K and V
+// by TMA, one box per run of positions inside a page, into a ring of stages. There are two kernels, by the rows of the
+// items; in a step that has both, they run side by side on SMs that the plan has shared out.
 //
-// Few rows (a decode step): bound by the bytes of K and V. Warp-level matrix instructions 16
-// rows high are enough for that: at 4 query heads per kv head an SM computes 16 x 32 x 128 x 2 products per 16 KB
-// stage, a small part of the time the stage takes to arrive. Each warp owns whole stages (32 positions at
-// head_dim 128) with its own running maximum, so warps meet only at the end of a piece.
+// Few rows (a decode step): bound by the bytes of K and V, with 160 KB of loads in flight on each SM. Warp-level matrix
+// instructions are enough for that; each warp owns whole 16 KB stages (32 positions at head_dim 128) with its own
+// running maximum, so warps meet only at the end of a piece. 32 sequences at 4096, 32 query heads on 8: 85 us,
+// 0.96 of the measured copy bandwidth; one sequence at 256: 5.5 us in a graph.
 //
-// Many rows (a chunk of a prompt): bound by the tensor cores. 128 rows -- all query heads of a kv head side by
-// side, token after token -- make a tcgen05 tile; two tiles share each K and V tile and alternate, one
-// in its softmax while the other multiplies. S = Q K^T goes to tensor memory, a thread per row reads it, writes P
-// back over it as bf16, and P is the A operand of O += P V from tensor memory.
+// Many rows (a chunk of a prompt): bound by the tensor cores and the chain between their products. 128 rows -- all
+// query heads of a kv head side by side, token after token -- make a tcgen05 tile; two tiles share each K and V
+// tile and alternate, one in its softmax while the other multiplies. S = Q K^T goes to tensor memory, two threads
+// per row read it, write P back over it as bf16, and P is the A operand of O += P V from tensor memory. A step of two
+// tiles takes 3550 cycles: per tile 2000 of softmax and 1400 of products (1024 of them multiplying), of which only the
+// two tiles' overlap hides any. 2048 tokens at 8192, 32 query heads on 8: 310 us, 1.0 PFLOP/s, 0.61 of the measured
+// matrix rate. What did not help: exponentials partly by polynomial (411 us at a quarter against 391), half-steps
+// of 64 columns (390), one thread a row (385), a product thread per tile (460).
 //
 // Bad values behind the mask: a masked score is replaced, whatever it is, but a zero probability times a NaN
 // or infinite v would still be NaN. Rows of V past the item's end are zeroed in shared memory; the few
@@ -1191,7 +1195,8 @@ __global__ void __launch_bounds__(BIG_THREADS, 1)
     }
 }
 
-// Adds up the parts of big items that were cut into many: a CTA per item and 16 columns, a thread per row.
+// Adds up the parts of big items that were cut into more than MERGE_PARTS: a CTA per item and 16 columns, a thread per
+// row. The last of an item's CTAs would read them all alone; with three parts or more this launch is the faster.
 template <int DP>
 __global__ void __launch_bounds__(2 * BIG_TILE) paged_combine_kernel(const __grid_constant__ PaArgs a) {
     pdl_trigger();
