@@ -562,6 +562,87 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
     bar_sync(1, NW * 32);  // the merge buffer is free again
 }
 
+// ---------------------------------------------------------------- partial results of many rows
+
+// Where a partial result keeps columns d .. d + 3 of a row, in scratch slot `slot`: four columns of all rows side by
+// side, so that a warp's 32 rows are one run of memory (row by row, its accesses took a sector each, and 20 us a piece).
+template <int DP>
+__device__ __forceinline__ float4 *big_part(const PaArgs &a, int slot, int d, size_t row) {
+    return reinterpret_cast<float4 *>(a.big_o + (size_t)slot * (2 * BIG_TILE) * DP) + (size_t)(d / 4) * (2 * BIG_TILE) + row;
+}
+
+// Adds up the parts of big items that were cut into more than MERGE_PARTS. The kernel for few rows ends with it, once the
+// other one has finished; as a launch of its own it cost 2 to 3 us more. A CTA takes 16 columns each of GROUPS items, a
+// different GROUPS-th of all items for each group of columns, and their rows one after the other, a thread per row.
+template <int DP>
+__device__ void combine_big(const PaArgs &a) {
+    constexpr int GROUPS = DP / 16;
+    auto item = [&](int i) { return a.splits + (blockIdx.x + i * (gridDim.x / GROUPS)) % gridDim.x; };
+    int rows[GROUPS], total = 0;
+#pragma unroll
+    for (int i = 0; i < GROUPS; i++) rows[i] = item(i)->n_parts > 1 ? item(i)->n_tok * a.rep : 0;
+#pragma unroll
+    for (int i = 0; i < GROUPS; i++) total += rows[i];
+#pragma unroll 1
+    for (int at = threadIdx.x; at < total; at += blockDim.x) {
+        int g = 0, r = at;
+#pragma unroll
+        for (int i = 0; i < GROUPS - 1; i++)
+            if (g == i && r >= rows[i]) {
+                r -= rows[i];
+                g++;
+            }
+        const int d = g * 16;
+        if (d >= a.head_dim) continue;
+        const PagedPiece p = *item(g);
+        const int tt = r / a.rep, x = tt / a.tile_tok, row = x * BIG_TILE + (tt - x * a.tile_tok) * a.rep + r % a.rep;
+        float m = -INFINITY, l = 0.0f, acc[16] = {};
+#pragma unroll 1
+        for (int w0 = 0; w0 < p.n_parts; w0 += 4) {  // four parts' loads in flight
+            float2 ml[4];
+            float4 v[4][4];
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                ml[w] = make_float2(-INFINITY, 0.0f);
+                if (w0 + w >= p.n_parts) continue;
+                const int slot = part_slot(p.first, w0 + w);
+                ml[w] = __ldcg(a.big_ml + (size_t)slot * (2 * BIG_TILE) + row);
+#pragma unroll
+                for (int q = 0; q < 4; q++) v[w][q] = __ldcg(big_part<DP>(a, slot, d, row) + q * (2 * BIG_TILE));
+            }
+            const float top = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+            const float base = top == -INFINITY ? 0.0f : top, f0 = ex2(m - base);
+            m = top;
+            l *= f0;
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[e] *= f0;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                if (w0 + w >= p.n_parts) continue;
+                const float f = ex2(ml[w].x - base);
+                l += f * ml[w].y;
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    acc[4 * q] += f * v[w][q].x;
+                    acc[4 * q + 1] += f * v[w][q].y;
+                    acc[4 * q + 2] += f * v[w][q].z;
+                    acc[4 * q + 3] += f * v[w][q].w;
+                }
+            }
+        }
+        const float inv = 1.0f / l;
+        bf16 *dst = a.out + (p.tok0 + tt) * a.out_stride + (long long)(p.kvh * a.rep + r % a.rep) * a.head_dim + d;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) w[q] = pack_bf16(acc[8 * e + 2 * q] * inv, acc[8 * e + 2 * q + 1] * inv);
+            if (d + 8 * e < a.head_dim)  // a row without positions is zero
+                reinterpret_cast<uint4 *>(dst)[e] = p.pos0 + tt < 0 ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
 // ---------------------------------------------------------------- kernel for few rows alone
 
 constexpr int SMALL_WARPS = 10;  // consumers, each with a stage of its own
@@ -612,7 +693,11 @@ __global__ void __launch_bounds__((SMALL_PRODUCERS + SMALL_WARPS) * 32, 1)
             small_consume<DP, NQ, SMALL_WARPS, SMALL_WARPS>(a, p, sm.ring, sm.full, sm.empty, r, wait, warp, sm.q, sm.lim, sm.merge_o, sm.merge_ml,
                                                          &sm.flag);
     }
-    if (a.after_big) pdl_wait();  // whoever waits for this kernel waits for that one, too
+    if constexpr (NQ == 1)
+        if (a.after_big) {  // whoever waits for this kernel waits for that one, too
+            pdl_wait();
+            combine_big<DP>(a);
+        }
 }
 
 // ---------------------------------------------------------------- many rows
@@ -862,13 +947,6 @@ __device__ __forceinline__ float exp64(uint32_t ts, int seen, uint64_t c2, uint6
     return w.x + w.y;
 }
 
-// Where a partial result keeps columns d .. d + 3 of a row, in scratch slot `slot`: four columns of all rows side by
-// side, so that a warp's 32 rows are one run of memory (row by row, its accesses took a sector each, and 20 us a piece).
-template <int DP>
-__device__ __forceinline__ float4 *big_part(const PaArgs &a, int slot, int d, size_t row) {
-    return reinterpret_cast<float4 *>(a.big_o + (size_t)slot * (2 * BIG_TILE) * DP) + (size_t)(d / 4) * (2 * BIG_TILE) + row;
-}
-
 // Two warpgroups per tile, two threads per row: each takes 64 of a step's columns and half of the output's.
 template <int DP>
 __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, BigSmem<DP> &sm, uint32_t tmem, int x, int part,
@@ -1029,7 +1107,7 @@ __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, BigSmem<DP> &s
             }
         }
         if (valid && part == 0) __stcg(a.big_ml + (size_t)p.part * (2 * BIG_TILE) + at, make_float2(m, l));
-        if (p.n_parts <= MERGE_PARTS) {  // the tile's last piece to finish adds the parts up; of more, the combine kernel does
+        if (p.n_parts <= MERGE_PARTS) {  // the tile's last piece to finish adds the parts up; of more, combine_big does
             __threadfence();
             bar_sync(9 + x, 256);
             if (row == 0 && part == 0) {
@@ -1195,49 +1273,6 @@ __global__ void __launch_bounds__(BIG_THREADS, 1)
     }
 }
 
-// Adds up the parts of big items that were cut into more than MERGE_PARTS: a CTA per item and 16 columns, a thread per
-// row. The last of an item's CTAs would read them all alone; with three parts or more this launch is the faster.
-template <int DP>
-__global__ void __launch_bounds__(2 * BIG_TILE) paged_combine_kernel(const __grid_constant__ PaArgs a) {
-    pdl_trigger();
-    pdl_wait();
-    const PagedPiece p = a.splits[blockIdx.x];
-    if (p.n_parts < 2) return;
-    const int row = threadIdx.x, x = row / BIG_TILE, rr = row % BIG_TILE, d = blockIdx.y * 16;
-    const int tt = x * a.tile_tok + rr / a.rep;
-    if (rr / a.rep >= a.tile_tok || tt >= p.n_tok || d >= a.head_dim) return;
-    float m = -INFINITY;
-#pragma unroll 4
-    for (int w = 0; w < p.n_parts; w++) m = fmaxf(m, __ldcg(a.big_ml + (size_t)part_slot(p.first, w) * (2 * BIG_TILE) + row).x);
-    float l = 0.0f, acc[16] = {};
-    const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll 4
-    for (int w = 0; w < p.n_parts; w++) {
-        const float2 ml = __ldcg(a.big_ml + (size_t)part_slot(p.first, w) * (2 * BIG_TILE) + row);
-        const float4 *src = big_part<DP>(a, part_slot(p.first, w), d, row);
-        const float f = ex2(ml.x - base);
-        l += f * ml.y;
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const float4 v = __ldcg(src + q * (2 * BIG_TILE));
-            acc[4 * q] += f * v.x;
-            acc[4 * q + 1] += f * v.y;
-            acc[4 * q + 2] += f * v.z;
-            acc[4 * q + 3] += f * v.w;
-        }
-    }
-    const float inv = 1.0f / l;
-    bf16 *dst = a.out + (p.tok0 + tt) * a.out_stride + (long long)(p.kvh * a.rep + rr % a.rep) * a.head_dim + d;
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-        uint32_t w[4];
-#pragma unroll
-        for (int q = 0; q < 4; q++) w[q] = pack_bf16(acc[8 * e + 2 * q] * inv, acc[8 * e + 2 * q + 1] * inv);
-        if (d + 8 * e < a.head_dim)  // a row without positions is zero
-            reinterpret_cast<uint4 *>(dst)[e] = p.pos0 + tt < 0 ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
-    }
-}
-
 // ---------------------------------------------------------------- host
 
 // K or V pages as a 4-D map (column, slot, kv head, page) with a box of `rows` slots of 64 columns.
@@ -1304,8 +1339,6 @@ int run(const PagedAttnCall &c, PaArgs &a, cudaStream_t s) {
     if (tiles == 2) Q3_TRY_LAUNCH((launch_small<DP, 2>(mk, mv, a, s)));
     if constexpr (DP == 64)
         if (tiles == 3) Q3_TRY_LAUNCH((launch_small<DP, 3>(mk, mv, a, s)));
-    if (!a.after_big) return Q3_OK;
-    Q3_TRY_LAUNCH(launch(paged_combine_kernel<DP>, dim3(paged_ctas(), DP / 16), dim3(2 * BIG_TILE), 0, s, 1, a));
     return Q3_OK;
 }
 
