@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
                     while (f + 1 < used && bound(f + 1) < start + len && steps_before(bound(f + 1) - start, s.ends(), steps, cost) < steps) f++;
                     p.n_parts = f - p.first + 1;
                     p.part = part_slot(p.first, c - p.first);
-                    if (t0 == 0 && p.n_parts > MERGE_PARTS) split = p;
+                    if (t0 == 0 && p.n_parts > 1) split = p;
                 }
                 if (first_piece < 0)
                     first_piece = (big ? n_items[0] + a.n_ctas + (int)(item_s[lo] >> 32) : (int)(item_s[lo] & 0xffffffff)) +
@@ -285,8 +285,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
         }
         ctas[(big ? PAGED_MAX_CTAS : 0) + c] = make_int2(max(first_piece, 0), bad_starts ? -1 : count);
         if (big) splits[c] = split;
-        counters[(big ? PAGED_MAX_CTAS : 0) + c] = 0;
-        if (big) counters[2 * PAGED_MAX_CTAS + c] = 0;
+        else counters[c] = 0;
     }
 }
 

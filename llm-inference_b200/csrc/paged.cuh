@@ -25,7 +25,6 @@ struct PagedSeq {
 // positions into pieces of neighbouring CTAs, which leave partial results in the scratch.
 constexpr int BIG_TILE = 128;       // rows of a tensor-core tile, and positions of one of its steps
 constexpr int PAGED_MAX_CTAS = 160; // persistent CTAs, one per SM
-constexpr int MERGE_PARTS = 2;      // a big item of up to this many pieces is merged by the last of them to finish
 
 struct alignas(16) PagedPiece {
     int seq, kvh, tok0, n_tok;   // query rows: tokens tok0 .. tok0 + n_tok of the batch
@@ -59,10 +58,8 @@ struct PagedPlanLayout {
     size_t table;     // int [n_seqs][max_pages]: checked page ids, -1 past a sequence's last page
     size_t toks;      // int4 [n_tokens]: sequence, position, page, slot
     size_t ctas;      // int2 [2][PAGED_MAX_CTAS], small items' CTAs and big ones': first piece, pieces (-1: zero every row)
-    size_t counters;  // int [3][PAGED_MAX_CTAS]: pieces done of the small item that starts in the CTA, of the big one's two
-                      // tiles; zero at rest
-    size_t splits;    // PagedPiece [PAGED_MAX_CTAS]: the big item of more than MERGE_PARTS pieces that starts
-                      // in the CTA (n_parts 0: none)
+    size_t counters;  // int [PAGED_MAX_CTAS]: pieces done of the small item that starts in the CTA; zero at rest
+    size_t splits;    // PagedPiece [PAGED_MAX_CTAS]: the cut big item that starts in the CTA (n_parts 0: none)
     size_t pieces;    // PagedPiece []
     size_t bytes;
 };
@@ -81,7 +78,7 @@ inline PagedPlanLayout paged_plan_layout(const q3_paged_shape &s) {
     l.table = take((size_t)s.n_seqs * s.max_pages * 4);
     l.toks = take((size_t)s.n_tokens * 16);
     l.ctas = take(2 * PAGED_MAX_CTAS * sizeof(int2));
-    l.counters = take(3 * PAGED_MAX_CTAS * sizeof(int));
+    l.counters = take(PAGED_MAX_CTAS * sizeof(int));
     l.splits = take(PAGED_MAX_CTAS * sizeof(PagedPiece));
     l.pieces = take((items + 2 * PAGED_MAX_CTAS) * sizeof(PagedPiece));
     l.bytes = off;

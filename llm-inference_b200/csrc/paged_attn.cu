@@ -571,7 +571,7 @@ __device__ __forceinline__ float4 *big_part(const PaArgs &a, int slot, int d, si
     return reinterpret_cast<float4 *>(a.big_o + (size_t)slot * (2 * BIG_TILE) * DP) + (size_t)(d / 4) * (2 * BIG_TILE) + row;
 }
 
-// Adds up the parts of big items that were cut into more than MERGE_PARTS. The kernel for few rows ends with it, once the
+// Adds up the parts of big items that were cut. The kernel for few rows ends with it, once the
 // other one has finished; as a launch of its own it cost 2 to 3 us more. A CTA takes 16 columns each of GROUPS items, a
 // different GROUPS-th of all items for each group of columns, and their rows one after the other, a thread per row.
 template <int DP>
@@ -1092,7 +1092,6 @@ __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, BigSmem<DP> &s
     const bool valid = row / a.rep < a.tile_tok && tt < p.n_tok;
     const int head = p.kvh * a.rep + row % a.rep;
     const size_t at = (size_t)x * BIG_TILE + row;  // this row in a scratch slot
-    bool last = p.part < 0;
     if (p.part >= 0) {
 #pragma unroll
         for (int i = 0; i < DP / 64; i++) {
@@ -1107,79 +1106,21 @@ __device__ void big_softmax(const PaArgs &a, const PagedPiece &p, BigSmem<DP> &s
             }
         }
         if (valid && part == 0) __stcg(a.big_ml + (size_t)p.part * (2 * BIG_TILE) + at, make_float2(m, l));
-        if (p.n_parts <= MERGE_PARTS) {  // the tile's last piece to finish adds the parts up; of more, combine_big does
-            __threadfence();
-            bar_sync(9 + x, 256);
-            if (row == 0 && part == 0) {
-                int *done = a.counters + (1 + x) * PAGED_MAX_CTAS + p.first;
-                const bool all = atomicAdd(done, 1) == p.n_parts - 1;
-                if (all) *done = 0;
-                sm.slow[x] = all;
-            }
-            bar_sync(9 + x, 256);
-            last = *(const volatile int *)&sm.slow[x];
-            __threadfence();
-        }
-    }
-    if (last) {
-        // weights of the parts, in their order; a whole item is its only part
-        const int parts = p.part < 0 ? 1 : p.n_parts, own = p.part < 0 ? 0 : p.part == part_slot(p.first, 0) ? 0 : p.part / 2 - p.first;
-        float weight[MERGE_PARTS] = {1.0f, 0.0f};
-        float sum = l;
-        if (parts > 1) {
-            float2 ml[MERGE_PARTS];
-            float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < MERGE_PARTS; w++) {
-                ml[w] = make_float2(-INFINITY, 0.0f);
-                if (w == own) ml[w] = make_float2(m, l);
-                else if (w < parts && valid) ml[w] = __ldcg(a.big_ml + (size_t)part_slot(p.first, w) * (2 * BIG_TILE) + at);
-                top = fmaxf(top, ml[w].x);
-            }
-            const float base = top == -INFINITY ? 0.0f : top;
-            sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < MERGE_PARTS; w++) {
-                weight[w] = ex2(ml[w].x - base);
-                sum += weight[w] * ml[w].y;
-            }
-        }
-        const float inv = 1.0f / sum;
+    } else {
+        const float inv = 1.0f / l;
         bf16 *dst = a.out + (p.tok0 + tt) * a.out_stride + (long long)head * a.head_dim;
-#pragma unroll 1
-        for (int i = 0; i < DP / 32; i++) {
-            float mine[16], acc[16];
-            __syncwarp();
-            tmem_ld8(to + 16 * i, mine);
-            tmem_ld8(to + 16 * i + 8, mine + 8);
+#pragma unroll
+        for (int i = 0; i < DP / 64; i++) {
+            uint32_t o[32];
+            tmem_ld32(to + 32 * i, o);
             tmem_wait_ld();
-            if (parts == 1) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) acc[e] = mine[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc[e] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < MERGE_PARTS; w++) {
-                    if (w >= parts) continue;
-                    const float4 *src = big_part<DP>(a, part_slot(p.first, w), part * (DP / 2) + 16 * i, at);
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        float4 v = make_float4(mine[4 * q], mine[4 * q + 1], mine[4 * q + 2], mine[4 * q + 3]);
-                        if (w != own && valid) v = __ldcg(src + q * (2 * BIG_TILE));
-                        acc[4 * q] += weight[w] * v.x;
-                        acc[4 * q + 1] += weight[w] * v.y;
-                        acc[4 * q + 2] += weight[w] * v.z;
-                        acc[4 * q + 3] += weight[w] * v.w;
-                    }
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
+            for (int e = 0; e < 4; e++) {
                 uint32_t w[4];
 #pragma unroll
-                for (int q = 0; q < 4; q++) w[q] = pack_bf16(acc[8 * e + 2 * q] * inv, acc[8 * e + 2 * q + 1] * inv);
-                const int d = part * (DP / 2) + 16 * i + 8 * e;
+                for (int q = 0; q < 4; q++)
+                    w[q] = pack_bf16(__uint_as_float(o[8 * e + 2 * q]) * inv, __uint_as_float(o[8 * e + 2 * q + 1]) * inv);
+                const int d = part * (DP / 2) + 32 * i + 8 * e;
                 if (valid && d < a.head_dim)  // a row without positions is zero
                     *reinterpret_cast<uint4 *>(dst + d) = lim <= 0 ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
             }
