@@ -13,15 +13,18 @@ import numpy as np
 from ._lib import Q3Error, call, check, load
 
 _SHAPE, _ARG = 1, 5
-_torch = None
+_torch = _device = _raw_stream = None
 
 
 def _t():
     """torch, imported when the first tensor arrives."""
-    global _torch
+    global _torch, _device, _raw_stream
     if _torch is None:
         import torch
         _torch = torch
+        # the current device's index and its stream's handle without objects around them, where torch has these
+        _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda _: torch.cuda.current_stream().cuda_stream)
     return _torch
 
 
@@ -45,12 +48,7 @@ ROPE_KINDS = {"plain": 0, "linear": 1, "by_parts": 2, "yarn": 3}
 
 
 def _stream(stream):
-    if stream is not None:
-        return stream
-    raw = getattr(_t()._C, "_cuda_getCurrentRawStream", None)  # the stream's handle without an object around it
-    if raw is None:
-        return _torch.cuda.current_stream().cuda_stream
-    return raw(_torch.cuda.current_device())
+    return _raw_stream(_device()) if stream is None else stream
 
 
 def _refuse(name, what, status=_ARG):
@@ -63,12 +61,13 @@ def _rows(name, t, what, rows, width, dtype):
     """Row stride of a [rows, ...] tensor whose rows are `width` contiguous elements."""
     if t.dtype is not dtype or not t.is_cuda:
         _refuse(name, f"{what} must be a CUDA tensor of {dtype}")
-    if t.is_contiguous() and t.numel() == rows * width and len(t) == rows:
+    shape = t.shape
+    if not shape or shape[0] != rows:
+        _refuse(name, f"{what}: {tuple(shape)}, expected {rows} rows", _SHAPE)
+    if t.is_contiguous() and t.numel() == rows * width:
         return width
-    if t.dim() == 0 or len(t) != rows:
-        _refuse(name, f"{what}: {tuple(t.shape)}, expected {rows} rows", _SHAPE)
     n = 1
-    for size, step in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+    for size, step in zip(reversed(shape[1:]), reversed(t.stride()[1:])):
         if size != 1 and step != n:
             _refuse(name, f"{what}: a row's elements must be contiguous")
         n *= size
@@ -110,6 +109,7 @@ class PagedPlan:
         self._ptr, self._scratch_ptr = self.plan.data_ptr(), self.scratch.data_ptr()
         self._cache = Q3PagedCache()  # filled anew for every call, which reads it before it returns
         self._cache_ref = ctypes.byref(self._cache)
+        self._strides = None  # of the pages that _cache describes
 
     def update(self, q_start, kv_len, page_table, stream=None):
         s, name, i32 = self.shape, "q3_paged_plan", _t().int32
@@ -130,7 +130,9 @@ class PagedPlan:
         if strides[3] != 1:
             _refuse(name, "pages: the last dimension must be contiguous")
         c.key_pages, c.value_pages = key_pages.data_ptr(), value_pages.data_ptr()
-        c.page_stride, c.head_stride, c.pos_stride = strides[0], strides[1], strides[2]
+        if strides != self._strides:
+            self._strides = strides
+            c.page_stride, c.head_stride, c.pos_stride = strides[0], strides[1], strides[2]
         return self._cache_ref
 
 
