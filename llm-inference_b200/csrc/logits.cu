@@ -8,9 +8,9 @@
 // Bound by latency: one row by the chain lengths -> ids -> logits, a batch by that chain once for each of the two or
 // three CTAs that an SM runs after one another. Each slice reads the row's whole history, from L2 after the
 // first, so slices are as large as still leaves two per SM. 32 rows of 151936 bf16 with masks and 2000 ids of history
-// each take 13.8 us in a graph (10.7 without the histories: 1.8 TB/s), 100 rows of 32003 floats with 8000 ids 19.6 (10.6).
+// each take 13.4 us in a graph (10.5 without the histories: 1.9 TB/s), 100 rows of 32003 floats with 8000 ids 18.3 (10.5).
 // Clusters of 8 slices that share the scan and count in one another's shared memory took 22 and 49 us; they
-// gain only for a single row of 16000 ids (16.1 -> 6.9).
+// gain only for a single row of 16000 ids (13.2 -> 6.9).
 #include <math.h>
 
 #include <algorithm>
@@ -73,11 +73,15 @@ __device__ __forceinline__ void each_id(const int *ids, int i0, int i1, F f) {
     const int lead = min(i1 - i0, (int)((16 - (reinterpret_cast<uintptr_t>(ids + i0) & 15)) & 15) / 4);
     const int quads = (i1 - i0 - lead) / 4, tail = i0 + lead + 4 * quads;
     if ((int)threadIdx.x < lead) f(i0 + threadIdx.x, ids[i0 + threadIdx.x]);
-    // one load in flight: with four, the unrolled body's registers cost more than the loads' latency (14.3 -> 18 us
-    // for 32 rows of 151936)
+    // the next load is asked for before this one's ids are looked at (100 rows of 8000 ids: 19.5 -> 18.3 us); with three
+    // or four in flight, or the first before the caller's barrier, their registers cost an SM its third CTA (20.5 us)
+    const int4 *src = reinterpret_cast<const int4 *>(ids + i0 + lead);
+    int4 next = threadIdx.x < quads ? __ldg(src + threadIdx.x) : make_int4(0, 0, 0, 0);
+#pragma unroll 1
     for (int q = threadIdx.x; q < quads; q += blockDim.x) {
         const int i = i0 + lead + 4 * q;
-        const int4 v = __ldg(reinterpret_cast<const int4 *>(ids + i));
+        const int4 v = next;
+        if (q + (int)blockDim.x < quads) next = __ldg(src + q + blockDim.x);
         f(i, v.x);
         f(i + 1, v.y);
         f(i + 2, v.z);
