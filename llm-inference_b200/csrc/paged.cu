@@ -293,14 +293,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
 // One CTA per token: 128 threads that take the heads in rounds where tokens are many, a group of lanes for every head
 // (up to 512 threads) where they are few. A unit is two 8-element chunks of a head that one lane holds in
 // registers: for half-split pairs chunk u and its partner u + rope_dim/16, so a pair's two elements sit in one
-// lane; otherwise neighbours. A head is a group of `lph` lanes (a power of two), so the sum of squares is a few
+// lane; otherwise u and u + lph. A head is a group of `lph` lanes (a power of two), so the sum of squares is a few
 // shuffles. The angles depend on the token alone: the CTA computes them once, into shared memory, where lanes read
-// theirs for every head (held in registers they cost occupancy: 44 us against 40.5 below). A lane's first query head is
+// theirs for every head (held in registers they cost occupancy: 44 us against 40.5). A lane's first query head is
 // asked for before that.
 //
-// With many tokens the instructions bound it about as much as the bytes: 8192 tokens of 48 heads of 128 take 40.5 us
-// (5.0 TB/s, 0.77 of the measured copy bandwidth) with packed arithmetic and a loop per kind of head, 43 without. With
-// few, the chain plan -> angle -> heads: 2.5 us for one token.
+// With many tokens the instructions bound it about as much as the bytes: 8192 tokens of 48 heads of 128 take 37.5 us
+// (5.4 TB/s, 0.83 of the measured copy bandwidth), interleaved 38.7 (61 with angles in the pairs' order, whose reads
+// met in a few banks); without packed arithmetic and a loop per kind of head it was 43. With few, the chain plan -> angle -> heads: 2.5 us for one token.
 //
 // The angle is reduced in fp64: pos * inv_freq reaches 10^5 rad and more, where an fp32 product is
 // off by up to 2^-25 of itself, more than a bf16 result may be. turns = pos * inv_freq / 2 pi, its
@@ -347,15 +347,17 @@ __device__ __forceinline__ void rope_angle(int pos, float inv_freq, float amplit
 }
 
 template <bool INTERLEAVED>
-__global__ void __launch_bounds__(APPEND_MAX_THREADS) paged_append_kernel(const __grid_constant__ AppendArgs a) {
-    // cos and sin of pair j: (cos, cos) and (-sin, sin) interleaved; half split cos, sin and -sin, for two pairs at a time
-    __shared__ __align__(16) float cos_s[PAGED_MAX_HEAD_DIM], sin_s[PAGED_MAX_HEAD_DIM], neg_s[PAGED_MAX_HEAD_DIM / 2];
+__global__ void __launch_bounds__(APPEND_MAX_THREADS, 2) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+    // cos and sin of pair j: (cos, cos) and (-sin, sin) interleaved; half split cos and sin, for two pairs at a time.
+    // Laid out so that the lanes of a group read 16 bytes each side by side: a lane's first 16 bytes of all lanes,
+    // then the second ones.
+    __shared__ __align__(16) float cos_s[PAGED_MAX_HEAD_DIM], sin_s[PAGED_MAX_HEAD_DIM];
     pdl_trigger();
     pdl_wait();
     const int t = blockIdx.x, groups = blockDim.x / a.lph, first = threadIdx.x / a.lph, step = groups * a.head_dim;
     const int u = threadIdx.x % a.lph, half = a.rope_dim / 2, nc = a.head_dim / 8, hc = INTERLEAVED ? 0 : half / 8;
-    const int c0 = INTERLEAVED ? 2 * u : u < hc ? u : 2 * u;  // units past the rotated pairs: chunks 2u, 2u + 1
-    const int c1 = !INTERLEAVED && u < hc ? u + hc : c0 + 1;
+    const int c0 = INTERLEAVED || u < hc ? u : 2 * u;  // half split, units past the rotated pairs: chunks 2u, 2u + 1
+    const int c1 = INTERLEAVED ? u + a.lph : u < hc ? u + hc : c0 + 1;
     const bool in0 = c0 < nc, in1 = c1 < nc;
     const uint4 zero = make_uint4(0, 0, 0, 0);
     auto load = [&](const bf16 *src, bool on, uint4 &r0, uint4 &r1) {
@@ -381,12 +383,13 @@ __global__ void __launch_bounds__(APPEND_MAX_THREADS) paged_append_kernel(const 
         float cs = 1.0f, sn = 0.0f;
         if (j < half) rope_angle(pos, a.inv_freq[j], a.amplitude, &cs, &sn);
         if (INTERLEAVED) {
-            reinterpret_cast<float2 *>(cos_s)[j] = make_float2(cs, cs);
-            reinterpret_cast<float2 *>(sin_s)[j] = make_float2(-sn, sn);
+            const int at = (j % 4 / 2 * 16 + j / 4) * 2 + j % 2;
+            reinterpret_cast<float2 *>(cos_s)[at] = make_float2(cs, cs);
+            reinterpret_cast<float2 *>(sin_s)[at] = make_float2(-sn, sn);
         } else {
-            cos_s[j] = cs;
-            sin_s[j] = sn;
-            neg_s[j] = -sn;
+            const int at = (j % 8 / 4 * 8 + j / 8) * 4 + j % 4;
+            cos_s[at] = cs;
+            sin_s[at] = sn;
         }
     }
     __syncthreads();
@@ -415,20 +418,28 @@ __global__ void __launch_bounds__(APPEND_MAX_THREADS) paged_append_kernel(const 
             for (int i = 0; i < 4; i++) x[4 + i] = mul2(mul2(x[4 + i], pair(inv, inv)), g[i]);
         }
         if (INTERLEAVED) {
-            const uint64_t *c = reinterpret_cast<const uint64_t *>(cos_s) + 8 * u, *s = reinterpret_cast<const uint64_t *>(sin_s) + 8 * u;
+            const ulonglong2 *c = reinterpret_cast<const ulonglong2 *>(cos_s), *s = reinterpret_cast<const ulonglong2 *>(sin_s);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float2 v = unpair(x[i]);
-                if (in1 || i < 4) x[i] = fma2(pair(v.y, v.x), s[i], mul2(x[i], c[i]));
+            for (int i = 0; i < 4; i++) {  // chunk c0's two pairs of pairs, then c1's
+                const int at = i % 2 * 16 + (i < 2 ? c0 : c1);
+                if (i < 2 ? !in0 : !in1) continue;
+                const ulonglong2 cc = c[at], ss = s[at];
+                const float2 v = unpair(x[2 * i]), w = unpair(x[2 * i + 1]);
+                x[2 * i] = fma2(pair(v.y, v.x), ss.x, mul2(x[2 * i], cc.x));
+                x[2 * i + 1] = fma2(pair(w.y, w.x), ss.y, mul2(x[2 * i + 1], cc.y));
             }
         } else if (u < hc) {
-            const uint64_t *c = reinterpret_cast<const uint64_t *>(cos_s) + 4 * u, *s = reinterpret_cast<const uint64_t *>(sin_s) + 4 * u,
-                           *ns = reinterpret_cast<const uint64_t *>(neg_s) + 4 * u;
+            const ulonglong2 *c = reinterpret_cast<const ulonglong2 *>(cos_s) + u, *s = reinterpret_cast<const ulonglong2 *>(sin_s) + u;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint64_t e = x[i], o = x[4 + i];
-                x[i] = fma2(o, ns[i], mul2(e, c[i]));
-                x[4 + i] = fma2(e, s[i], mul2(o, c[i]));
+            for (int i = 0; i < 2; i++) {
+                const ulonglong2 cc = c[8 * i], ss = s[8 * i];
+                constexpr unsigned long long SIGNS = 0x8000000080000000ull;
+                const ulonglong2 nn = make_ulonglong2(ss.x ^ SIGNS, ss.y ^ SIGNS);
+                const uint64_t e0 = x[2 * i], o0 = x[4 + 2 * i], e1 = x[2 * i + 1], o1 = x[5 + 2 * i];
+                x[2 * i] = fma2(o0, nn.x, mul2(e0, cc.x));
+                x[4 + 2 * i] = fma2(e0, ss.x, mul2(o0, cc.x));
+                x[2 * i + 1] = fma2(o1, nn.y, mul2(e1, cc.y));
+                x[5 + 2 * i] = fma2(e1, ss.y, mul2(o1, cc.y));
             }
         }
         r0 = pack8(x);
