@@ -379,9 +379,9 @@ __global__ void __launch_bounds__(APPEND_MAX_THREADS, 2) paged_append_kernel(con
         for (int h = first; h < a.n_heads; h += groups, dst += step) store(dst, zero, zero);
         return;
     }
-    for (int j = threadIdx.x; j < (INTERLEAVED ? a.head_dim / 2 : half); j += blockDim.x) {
-        float cs = 1.0f, sn = 0.0f;
-        if (j < half) rope_angle(pos, a.inv_freq[j], a.amplitude, &cs, &sn);
+    for (int j = threadIdx.x; j < half; j += blockDim.x) {
+        float cs, sn;
+        rope_angle(pos, a.inv_freq[j], a.amplitude, &cs, &sn);
         if (INTERLEAVED) {
             const int at = (j % 4 / 2 * 16 + j / 4) * 2 + j % 2;
             reinterpret_cast<float2 *>(cos_s)[at] = make_float2(cs, cs);
@@ -425,8 +425,9 @@ __global__ void __launch_bounds__(APPEND_MAX_THREADS, 2) paged_append_kernel(con
                 if (i < 2 ? !in0 : !in1) continue;
                 const ulonglong2 cc = c[at], ss = s[at];
                 const float2 v = unpair(x[2 * i]), w = unpair(x[2 * i + 1]);
-                x[2 * i] = fma2(pair(v.y, v.x), ss.x, mul2(x[2 * i], cc.x));
-                x[2 * i + 1] = fma2(pair(w.y, w.x), ss.y, mul2(x[2 * i + 1], cc.y));
+                const int at_pair = 4 * (i < 2 ? c0 : c1) + i % 2 * 2;  // pairs from `half` on stay as they are, NaN or not
+                if (at_pair < half) x[2 * i] = fma2(pair(v.y, v.x), ss.x, mul2(x[2 * i], cc.x));
+                if (at_pair + 1 < half) x[2 * i + 1] = fma2(pair(w.y, w.x), ss.y, mul2(x[2 * i + 1], cc.y));
             }
         } else if (u < hc) {
             const ulonglong2 *c = reinterpret_cast<const ulonglong2 *>(cos_s) + u, *s = reinterpret_cast<const ulonglong2 *>(sin_s) + u;

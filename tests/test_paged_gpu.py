@@ -509,3 +509,21 @@ def test_too_many_tokens_are_padding(heads, kvh, most):
     b.lens[1] = (37, 0)
     check_attention(out, *b.attention_exact(q, 0.125), "too many tokens")
     assert not out[b.rows(1)].any()
+
+
+# what lies past rope_dim passes through: an infinity there reaches nothing else
+@pytest.mark.parametrize("dim,rope,interleaved", [(128, 64, True), (128, 20, True), (64, 32, False), (64, 20, False), (96, 48, True)])
+def test_append_keeps_values_past_the_rotated_ones_apart(dim, rope, interleaved):
+    b = Batch([(3, 9)], 4, 2, dim, 8, seed=dim + rope)
+    b.update()
+    q, k, v = rn(b.g, 3, 4, dim), rn(b.g, 3, 2, dim), rn(b.g, 3, 2, dim)
+    freq = torch.from_numpy(q3.rope_inv_freq(rope, 1e4)[0]).cuda()
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    q3.paged_rope_append(clean, q, k, v, b.kp, b.vp, b.plan, freq, interleaved=interleaved)
+    q[1, 2, rope + 2] = float("inf")
+    q[2, 0, dim - 1] = NAN
+    q3.paged_rope_append(out, q, k, v, b.kp, b.vp, b.plan, freq, interleaved=interleaved)
+    assert torch.equal(clean[..., rope:], torch.where(torch.isfinite(q[..., rope:]), q[..., rope:], clean[..., rope:]))
+    changed = (out != clean).nonzero().tolist()
+    assert changed == [[1, 2, rope + 2], [2, 0, dim - 1]]
+    assert torch.isinf(out[1, 2, rope + 2]) and torch.isnan(out[2, 0, dim - 1])
