@@ -35,7 +35,7 @@ struct PlanArgs {
 // Items are cut only while each CTA still gets MIN_SHARE or BIG_MIN_SHARE. A unit of the big kind takes BIG_WEIGHT / 2 of the small one's
 // time where the two share the SMs: with 31 decodes and a chunk of 333 tokens, 1 to 4 and 5.5 gave 178, 107, 89, 88, 96 us
 // (105 one after the other), with 32 decodes at 4096 and a chunk of 2048 at 8192 425, 370, 334, 400, 480 (376).
-constexpr int COST_ITEM = 3, COST_BIG_ITEM = 6, COST_BIG_ONE = 2, COST_BIG_TWO = 3, MIN_SHARE = 16, BIG_MIN_SHARE = 8, BIG_WEIGHT = 6;
+constexpr int COST_ITEM = 3, COST_BIG_ITEM = 6, COST_BIG_ONE = 2, COST_BIG_TWO = 3, MIN_SHARE = 10, BIG_MIN_SHARE = 6, BIG_WEIGHT = 6;
 
 // The items of sequence q: a big one has n_q per kv head.
 struct SeqItems {
@@ -202,8 +202,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
                           : a.n_ctas;
     // Items are cut where there are CTAs to spare and every piece still gets its least share; in equal numbers of pieces, if
     // that leaves no more than a tenth of the CTAs without work (32 sequences' decodes with 532 tokens at 1389: 28 us, 39
-    // otherwise; the geometric mean of 36 random batches is 1 % less). Least shares of 8, 10, 12 and 16 for big items: 18,
-    // 18.7, 20 and 21 us for 14 decodes with 31 tokens at 3995.
+    // otherwise; the geometric mean of 36 random batches is 1 % less). Least shares of 6, 8, 10, 12 and 16 for big items: 17.2,
+    // 18.2, 18.7, 20 and 21 us for 14 decodes with 31 tokens at 3995; of 8, 10 and 16 for small ones: 16.2, 11.5 and 11.7 us
+    // for 3 draft tokens of 4 sequences at 1000, 10.1, 9.7 and 11.5 for one token of one sequence in the thousands.
     auto ctas_used = [&](int most, bool big) {
         const int n_of = max(1, n_items[big]);
         const long long shares = big ? total_big / BIG_MIN_SHARE : total_small / MIN_SHARE;
