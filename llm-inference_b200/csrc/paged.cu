@@ -309,7 +309,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
 //
 // With many tokens the instructions bound it about as much as the bytes: 8192 tokens of 48 heads of 128 take 37.5 us
 // (5.4 TB/s, 0.83 of the measured copy bandwidth), interleaved 38.7 (61 with angles in the pairs' order, whose reads
-// met in a few banks); without packed arithmetic and a loop per kind of head it was 43. With few, the chain plan -> angle -> heads: 2.5 us for one token.
+// met in a few banks); without packed arithmetic and a loop per kind of head it was 43. With few, the chain plan ->
+// angle -> heads: 2.4 us for one token.
 //
 // The angle is reduced in fp64: pos * inv_freq reaches 10^5 rad and more, where an fp32 product is
 // off by up to 2^-25 of itself, more than a bf16 result may be. turns = pos * inv_freq / 2 pi, its

@@ -21,8 +21,9 @@
 // per row read it, write P back over it as bf16, and P is the A operand of O += P V from tensor memory. A step of two
 // tiles takes 3550 cycles: per tile 2000 of softmax and 1400 of products (1024 of them multiplying), of which only the
 // two tiles' overlap hides any. 2048 tokens at 8192, 32 query heads on 8: 310 us, 1.0 PFLOP/s, 0.61 of the measured
-// matrix rate. What did not help: exponentials partly by polynomial (411 us at a quarter against 391), half-steps
-// of 64 columns (390), one thread a row (385), a product thread per tile (460).
+// matrix rate. What did not help: a quarter of the exponentials by polynomial
+// (275 to 296 us against 266 on one set of inputs), half-steps of 64 columns (390 where whole ones took 363), one
+// thread a row (385), a product thread per tile (460).
 //
 // Bad values behind the mask: a masked score is replaced, whatever it is, but a zero probability times a NaN
 // or infinite v would still be NaN. Rows of V past the item's end are zeroed in shared memory; the few
