@@ -58,7 +58,8 @@ __device__ __forceinline__ uint64_t globaltimer() {
 // A kernel launched with programmatic stream serialization may start while its predecessor
 // still runs. Every kernel here touches activations only after pdl_wait(), which returns once
 // the predecessor grid has completed and its writes are visible; loads of constant weights
-// may be issued before it. pdl_trigger() lets the successor be scheduled early.
+// may be issued before it. The one exception takes an acquire in its place (take_ready in paged_attn.cu).
+// pdl_trigger() lets the successor be scheduled early.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

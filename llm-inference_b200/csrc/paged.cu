@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     int2 *ctas = reinterpret_cast<int2 *>(a.plan + a.l.ctas);
     PagedPiece *pieces = reinterpret_cast<PagedPiece *>(a.plan + a.l.pieces);
     PagedPiece *splits = reinterpret_cast<PagedPiece *>(a.plan + a.l.splits);
-    int *counters = reinterpret_cast<int *>(a.plan + a.l.counters);
+    int *counters = reinterpret_cast<int *>(a.plan + a.l.counters), *ready = reinterpret_cast<int *>(a.plan + a.l.ready);
     // The two kernels of a step with items of both kinds run side by side: the big one's CTAs first, the small
     // one's on the SMs that those leave: tensor-core work beside loads, and memory bandwidth is not for want of SMs.
     const long long weight = total_big * BIG_WEIGHT / 2;
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
         }
         ctas[(big ? PAGED_MAX_CTAS : 0) + c] = make_int2(max(first_piece, 0), bad_starts ? -1 : count);
         if (big) splits[c] = split;
-        else counters[c] = 0;
+        else counters[c] = ready[c] = 0;
     }
 }
 

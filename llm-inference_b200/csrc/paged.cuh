@@ -59,6 +59,7 @@ struct PagedPlanLayout {
     size_t toks;      // int4 [n_tokens]: sequence, position, page, slot
     size_t ctas;      // int2 [2][PAGED_MAX_CTAS], small items' CTAs and big ones': first piece, pieces (-1: zero every row)
     size_t counters;  // int [PAGED_MAX_CTAS]: pieces done of the small item that starts in the CTA; zero at rest
+    size_t ready;     // int [PAGED_MAX_CTAS]: the CTA of the kernel for many rows has waited for what came before; zero at rest
     size_t splits;    // PagedPiece [PAGED_MAX_CTAS]: the cut big item that starts in the CTA (n_parts 0: none)
     size_t pieces;    // PagedPiece []
     size_t bytes;
@@ -79,6 +80,7 @@ inline PagedPlanLayout paged_plan_layout(const q3_paged_shape &s) {
     l.toks = take((size_t)s.n_tokens * 16);
     l.ctas = take(2 * PAGED_MAX_CTAS * sizeof(int2));
     l.counters = take(PAGED_MAX_CTAS * sizeof(int));
+    l.ready = take(PAGED_MAX_CTAS * sizeof(int));
     l.splits = take(PAGED_MAX_CTAS * sizeof(PagedPiece));
     l.pieces = take((items + 2 * PAGED_MAX_CTAS) * sizeof(PagedPiece));
     l.bytes = off;

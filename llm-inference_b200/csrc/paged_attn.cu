@@ -56,7 +56,7 @@ struct PaArgs {
     const int *table;
     const int2 *ctas;
     const PagedPiece *pieces, *splits;
-    int *counters;
+    int *counters, *ready;
     float *small_o, *big_o;
     float2 *small_ml, *big_ml;
     int rep, tile_tok, head_dim, page_size, max_pages, n_tokens, row_elems;
@@ -64,7 +64,7 @@ struct PaArgs {
     int small_step_pages, small_step_slots, big_step_pages, big_step_slots;  // a producer's step in pages and slots
     float scale_log2;
     uint32_t idesc_qk, idesc_pv;
-    bool after_big;  // few rows: launched behind the kernel for many rows, whose results are not needed
+    bool after_big;  // few rows: launched behind the kernel for many rows, whose results are needed at the end only
 };
 
 // ---------------------------------------------------------------- helpers
@@ -99,6 +99,29 @@ struct Waiter {
         if (!dead && !poll(bar, parity)) dead = !wait_clocked(bar, parity);
     }
 };
+
+// The kernel for few rows, launched behind the one for many, starts while that still runs, so its own
+// griddepcontrol.wait would come too late, and what the other grid's wait made visible it did so to that grid alone.
+// So CTA i of the kernel for many rows, after its wait, passes that on to CTA i of this one: a release, taken here
+// by an acquire that also puts the flag back to rest. Every CTA of the other kernel has released before this one can
+// start (it triggers after that), so the loop hardly ever turns.
+__device__ __forceinline__ void give_ready(int *flag) {
+    asm volatile("st.release.gpu.global.b32 [%0], 1;" ::"l"(flag) : "memory");
+}
+__device__ bool take_ready(int *flag) {
+    const uint64_t start = globaltimer();
+    for (;;) {
+        int seen;
+        asm volatile("atom.acquire.gpu.global.exch.b32 %0, [%1], 0;" : "=r"(seen) : "l"(flag) : "memory");
+        if (seen != 0) return true;
+        if (globaltimer() - start > WAIT_LIMIT_NS) {
+            atomicOr(&g_dev_error, DEV_ERR_WAIT_TIMEOUT);
+            return false;
+        }
+    }
+}
+// Orders what was written before by plain stores and is visible to this thread before its later TMA loads.
+__device__ __forceinline__ void fence_proxy_async_global() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
 
 template <int N>
 struct Ring {
@@ -656,7 +679,7 @@ struct SmallSmem {
     uint2 q[NQ == 1 ? 1 : DP / 16 * NQ * 32];
     int2 lim[4 * NQ];
     uint64_t full[SMALL_WARPS], empty[SMALL_WARPS];
-    int flag;
+    int flag, go;
 };
 
 template <int DP, int NQ>
@@ -675,12 +698,15 @@ __global__ void __launch_bounds__((SMALL_PRODUCERS + SMALL_WARPS) * 32, 1)
         prefetch_tmap(&mk);
         prefetch_tmap(&mv);
     }
+    // The kernel before is the plan or whatever wrote q, K and V; or it is the kernel for many rows, whose CTA says when
+    // it has waited for those.
+    if (a.after_big && threadIdx.x == 32) sm.go = take_ready(a.ready + blockIdx.x);
     __syncthreads();
     pdl_trigger();
-    // The kernel before is the plan or whatever wrote q, K and V; or it is the kernel for many rows, which let this one
-    // start only after it had itself waited for those: then there is nothing to wait for until the end.
+    int2 work = make_int2(0, 0);
     if (!a.after_big) pdl_wait();
-    const int2 work = a.ctas[blockIdx.x];
+    else fence_proxy_async_global();
+    if (!a.after_big || sm.go) work = a.ctas[blockIdx.x];
     if (work.y < 0) zero_rows(a);
     Ring<SMALL_WARPS> r;
     Waiter wait;
@@ -1139,7 +1165,11 @@ __global__ void __launch_bounds__(BIG_THREADS, 1)
     // no room to align by hand; the declaration's alignment holds for the shared window
     BigSmem<DP> &sm = *reinterpret_cast<BigSmem<DP> *>(smem_raw);
     if (smem_u32(smem_raw) % 1024 != 0) {
-        if (threadIdx.x == 0) atomicOr(&g_dev_error, DEV_ERR_TMEM);
+        pdl_wait();
+        if (threadIdx.x == 0) {
+            atomicOr(&g_dev_error, DEV_ERR_TMEM);
+            give_ready(a.ready + blockIdx.x);
+        }
         return;
     }
     const int warp = threadIdx.x / 32;
@@ -1169,10 +1199,11 @@ __global__ void __launch_bounds__(BIG_THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
-    // The next kernel may start once this one's predecessors are done (the kernel for few rows relies on it) and
+    // The next kernel may start once this one's predecessors are done (the kernel for few rows takes that over) and
     // every CTA has its tensor memory: a dependent's CTA that took it first would wait for this kernel while
     // this CTA waits for its memory.
     pdl_wait();
+    if (threadIdx.x == 0) give_ready(a.ready + blockIdx.x);
     pdl_trigger();
     const int2 work = a.ctas[PAGED_MAX_CTAS + blockIdx.x];
     if (work.y < 0) zero_rows(a);
@@ -1306,6 +1337,7 @@ int paged_attention(const PagedAttnCall &c, cudaStream_t s) {
     a.pieces = reinterpret_cast<const PagedPiece *>(c.plan + l.pieces);
     a.splits = reinterpret_cast<const PagedPiece *>(c.plan + l.splits);
     a.counters = reinterpret_cast<int *>(c.plan + l.counters);
+    a.ready = reinterpret_cast<int *>(c.plan + l.ready);
     a.small_o = reinterpret_cast<float *>(c.scratch + x.small_o);
     a.small_ml = reinterpret_cast<float2 *>(c.scratch + x.small_ml);
     a.big_o = reinterpret_cast<float *>(c.scratch + x.big_o);

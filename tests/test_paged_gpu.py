@@ -527,3 +527,50 @@ def test_append_keeps_values_past_the_rotated_ones_apart(dim, rope, interleaved)
     changed = (out != clean).nonzero().tolist()
     assert changed == [[1, 2, rope + 2], [2, 0, dim - 1]]
     assert torch.isinf(out[1, 2, rope + 2]) and torch.isnan(out[2, 0, dim - 1])
+
+
+# A captured step with decodes and a chunk, whose two kernels run side by side: what the step before it left in the plan,
+# the queries and the pages is overwritten between replays, and neither kernel may still see it.
+def test_a_captured_mixed_step_follows_its_inputs():
+    heads, kvh, dim, page, most = 32, 8, 128, 16, 120
+    b = Batch([(1, 900)] * 6 + [(most, 900)], heads, kvh, dim, page, seed=12, max_q=most)
+    freq = torch.from_numpy(q3.rope_inv_freq(dim, 1e6)[0]).cuda()
+    layers = [(b.kp, b.vp), (b.vp.clone(), b.kp.clone())]
+    x = [[rn(b.g, b.tokens, n, dim) for n in (heads, kvh, kvh)] for _ in layers]
+    qs = [torch.empty_like(x[0][0]) for _ in layers]
+    outs = [torch.empty_like(x[0][0]) for _ in layers]
+
+    def step():
+        b.update()
+        for (kp, vp), (q, k, v), q_out, out in zip(layers, x, qs, outs):
+            q3.paged_rope_append(q_out, q, k, v, kp, vp, b.plan, freq)
+            q3.paged_attention(out, q_out, kp, vp, b.plan)
+
+    step()  # kernel attributes are set before the capture
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    first = b.table.clone()
+    for i, (chunk, kv) in enumerate([(most, [900, 17, 1, 640, 33, 128, 900]), (40, [1, 2, 899, 5, 900, 0, 40]), (most, [64] * 6 + [most]),
+                                     (1, [900] * 7), (77, [300, 900, 31, 32, 33, 34, 800])]):
+        b.lens = [(1, n) for n in kv[:6]] + [(chunk, kv[6])]
+        b.starts = [0, 1, 2, 3, 4, 5, 6, 6 + chunk]
+        b.q_start.copy_(torch.tensor(b.starts, dtype=torch.int32))
+        b.kv_len.copy_(torch.tensor(kv, dtype=torch.int32))
+        b.table.copy_(first.roll(i, 0))
+        for rows in x:
+            for t in rows:
+                t.normal_(generator=b.g)
+        for out in outs:
+            out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert q3.device_error() == 0
+        n = b.starts[-1]
+        for (b.kp, b.vp), (_, _, v), q, out in zip(layers, x, qs, outs):
+            exact, mag = b.attention_exact(q, dim ** -0.5)
+            check_attention(out[:n], exact[:n], mag[:n], f"replay {i}")
+            assert (out[n:] == 7.0).all()
+            for s, (m, kv_s) in enumerate(b.lens):
+                assert torch.equal(b.cached(b.vp, s)[max(0, kv_s - m):], v[b.rows(s)][max(0, m - kv_s):])
