@@ -36,6 +36,7 @@
 
 #include "paged.cuh"
 #include "tc_common.cuh"
+#include "waiter.cuh"
 
 namespace q3 {
 namespace {
@@ -68,37 +69,6 @@ struct PaArgs {
 };
 
 // ---------------------------------------------------------------- helpers
-
-// Polls a barrier a few thousand times. The loop is four instructions, and what follows a wait that gives up is out
-// of line: the roles' loops compete for the instruction cache.
-__device__ __forceinline__ bool poll(uint64_t *bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
-        "mov.u32 n, 4096;\n\t"
-        "again:\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "@p bra done;\n\t"
-        "sub.u32 n, n, 1;\n\t"
-        "setp.ne.u32 q, n, 0;\n\t"
-        "@q bra again;\n\t"
-        "done:\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-__device__ __noinline__ bool wait_clocked(uint64_t *bar, uint32_t parity) { return mbar_wait(bar, parity, &g_dev_error); }
-
-// Waits until one has given up; from then on the role runs through its loop without waiting, so that every
-// barrier of the CTA still sees its arrivals and the kernel ends.
-struct Waiter {
-    bool dead = false;
-    __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) {
-        if (!dead && !poll(bar, parity)) dead = !wait_clocked(bar, parity);
-    }
-};
 
 // The kernel for few rows, launched behind the one for many, starts while that still runs, so its own
 // griddepcontrol.wait would come too late, and what the other grid's wait made visible it did so to that grid alone.
@@ -283,13 +253,13 @@ __device__ void small_produce(const PaArgs &a, const CUtensorMap *mk, const CUte
         at += NP * UPOS;
         const int next_page = active && at < p.kv1 ? __ldg(tab + w.idx) : 0;
         wait(&empty[mine.s], mine.ph ^ 1);
-        __syncwarp();
-        if (lane == 0 && !wait.dead) {
+        if (wait.stopped()) break;
+        if (lane == 0) {
             const int n = min(UPOS, max(0, p.kv1 - p0) + box - 1) & -box;
             mbar_arrive_expect_tx(&full[mine.s], (uint32_t)(n * 128 * NB * 2));
         }
         __syncwarp();
-        if (on && !wait.dead) tma_page(ring + (size_t)mine.s * SMALL_STAGE + off, map, half * 64, slot, p.kvh, page, &full[mine.s]);
+        if (on) tma_page(ring + (size_t)mine.s * SMALL_STAGE + off, map, half * 64, slot, p.kvh, page, &full[mine.s]);
         mine.next(NP);
         p0 += NP * UPOS;
         page = next_page;
@@ -679,7 +649,7 @@ struct SmallSmem {
     uint2 q[NQ == 1 ? 1 : DP / 16 * NQ * 32];
     int2 lim[4 * NQ];
     uint64_t full[SMALL_WARPS], empty[SMALL_WARPS];
-    int flag, go;
+    int flag, go, down;
 };
 
 template <int DP, int NQ>
@@ -695,6 +665,7 @@ __global__ void __launch_bounds__((SMALL_PRODUCERS + SMALL_WARPS) * 32, 1)
             mbar_init(&sm.empty[i], 1);
         }
         fence_barrier_init();
+        sm.down = 0;
         prefetch_tmap(&mk);
         prefetch_tmap(&mv);
     }
@@ -709,10 +680,10 @@ __global__ void __launch_bounds__((SMALL_PRODUCERS + SMALL_WARPS) * 32, 1)
     if (!a.after_big || sm.go) work = a.ctas[blockIdx.x];
     if (work.y < 0) zero_rows(a);
     Ring<SMALL_WARPS> r;
-    Waiter wait;
+    Waiter wait(&g_dev_error, &sm.down);
     for (int i = 0; i < work.y; i++) {
         const PagedPiece p = a.pieces[work.x + i];
-        // every load is waited for by a consumer before the CTA ends
+        // every load is waited for by a consumer before the CTA ends, or by settle
         if (warp >= SMALL_WARPS)
             small_produce<DP, SMALL_WARPS, SMALL_PRODUCERS>(a, &mk, &mv, p, sm.ring, sm.full, sm.empty, r, warp - SMALL_WARPS, wait,
                                                              a.small_step_pages, a.small_step_slots);
@@ -720,6 +691,7 @@ __global__ void __launch_bounds__((SMALL_PRODUCERS + SMALL_WARPS) * 32, 1)
             small_consume<DP, NQ, SMALL_WARPS, SMALL_WARPS>(a, p, sm.ring, sm.full, sm.empty, r, wait, warp, sm.q, sm.lim, sm.merge_o, sm.merge_ml,
                                                          &sm.flag);
     }
+    settle(wait);
     if constexpr (NQ == 1)
         if (a.after_big) {  // whoever waits for this kernel waits for that one, too
             pdl_wait();
@@ -777,6 +749,7 @@ struct BigSmem {
     uint64_t full[BIG_STAGES], empty[BIG_STAGES], q_full, q_empty, s_full[2], p_full[2], o_full[2];
     uint32_t tmem;
     int slow[2];  // by tile: this step's second product is not the tensor core's
+    int down;
 };
 
 // Tensor memory: S of tile x at column 128 x, O at 256 + DP x. P of positions 0 .. 63 lies over the first 32 columns of
@@ -800,10 +773,10 @@ __device__ void big_produce(const PaArgs &a, const CUtensorMap *mq, const CUtens
     if (pid == 0) {
         wait(&sm.q_empty, q_ph ^ 1);
         q_ph ^= 1;
+        if (wait.stopped()) return;
+        if (lane == 0) mbar_arrive_expect_tx(&sm.q_full, (uint32_t)(tiles * NB * a.tile_tok * a.rep * 128));
         __syncwarp();
-        if (lane == 0 && !wait.dead) mbar_arrive_expect_tx(&sm.q_full, (uint32_t)(tiles * NB * a.tile_tok * a.rep * 128));
-        __syncwarp();
-        if (lane < tiles * NB && !wait.dead)
+        if (lane < tiles * NB)
             tma_load_3d(sm.q + lane * BOX64, mq, lane % NB * 64, p.kvh * a.rep, p.tok0 + lane / NB * a.tile_tok, &sm.q_full);
     } else {
         mine.next();
@@ -822,10 +795,10 @@ __device__ void big_produce(const PaArgs &a, const CUtensorMap *mq, const CUtens
         const int next_page = active && at < p.kv1 ? __ldg(tab + w.idx) : 0;
         const uint32_t bytes = (uint32_t)((min(BIG_TILE, max(0, p.kv1 - p0) + box - 1) & -box) * 128 * NB);
         wait(&sm.empty[mine.s], mine.ph ^ 1);
+        if (wait.stopped()) return;
+        if (lane == 0) mbar_arrive_expect_tx(&sm.full[mine.s], bytes);
         __syncwarp();
-        if (lane == 0 && !wait.dead) mbar_arrive_expect_tx(&sm.full[mine.s], bytes);
-        __syncwarp();
-        if (on && !wait.dead)
+        if (on)
             tma_page(sm.ring + (size_t)mine.s * BIG_STAGE + half * BOX64 + sub * box * 128, map, half * 64, slot, p.kvh, page,
                      &sm.full[mine.s]);
         mine.next(2);
@@ -1186,6 +1159,7 @@ __global__ void __launch_bounds__(BIG_THREADS, 1)
             mbar_init(&sm.p_full[x], 9);
         }
         fence_barrier_init();
+        sm.down = 0;
         prefetch_tmap(&mq);
         prefetch_tmap(&mk);
         prefetch_tmap(&mv);
@@ -1208,7 +1182,7 @@ __global__ void __launch_bounds__(BIG_THREADS, 1)
     const int2 work = a.ctas[PAGED_MAX_CTAS + blockIdx.x];
     if (work.y < 0) zero_rows(a);
     Ring<BIG_STAGES> r;
-    Waiter wait;
+    Waiter wait(&g_dev_error, &sm.down);
     if (warp < 4) {
         uint32_t q_ph = 0, p_ph = 0;
         const bool first = threadIdx.x % 32 == 0;
@@ -1234,12 +1208,7 @@ __global__ void __launch_bounds__(BIG_THREADS, 1)
             big_softmax<DP>(a, p, sm, tmem, group / 2, group % 2, r, s_ph, wait);
         }
     }
-    if (wait.dead) {  // a wait gave up: what was issued before it, or without it since, ends well within this time
-        const uint64_t t = globaltimer();
-        while (globaltimer() - t < 1000000) {
-        }
-    }
-    __syncthreads();
+    settle(wait);
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");

@@ -93,3 +93,25 @@ def test_rank_exit_ends_peer_collective_with_error():
     assert got[1] == "left"
     assert got[0].startswith("error after"), got[0]
     assert float(got[0].split()[2].rstrip("s:")) < 60
+
+
+@pytest.mark.gpu
+def test_a_ring_stops_loading_after_a_wait_gave_up():
+    import llm_inference_b200 as q3
+    from llm_inference_b200 import _lib
+    src = torch.arange(256, dtype=torch.int32, device="cuda")
+    out = torch.zeros(4, dtype=torch.int32, device="cuda")
+    _lib.call("q3_selftest_ring_timeout", out.data_ptr(), src.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert q3.device_error() == 1, "expected the wait-timeout bit alone"
+    # steps 0 to 3 were loaded before the reader gave up at step 2; both stages hold their latest ones
+    assert out.tolist() == [2, 4, 4 * 2 + 3, 4 * 3 + 3]
+    assert q3.device_error() == 0
+
+
+def test_ring_selftest_refuses():
+    from llm_inference_b200 import _lib, build
+    build.build()
+    lib = _lib.load()
+    assert lib.q3_selftest_ring_timeout(None, 4096, None) == 5
+    assert lib.q3_selftest_ring_timeout(4096, None, None) == 5
+    assert lib.q3_selftest_ring_timeout(4096, 4100, None) == 2
