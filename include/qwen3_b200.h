@@ -388,8 +388,9 @@ typedef struct q3_paged_cache {
 
 /* Bytes of a plan, and of the scratch q3_paged_attention needs, for a shape (0 if the shape is
  * not supported: head_dim not a multiple of 8 up to 128, n_heads not a multiple of n_kv_heads or
- * more than 128 query heads per kv head). Neither needs initialization. Calls that share a plan's
- * scratch must not overlap on the GPU. */
+ * more than 128 query heads per kv head). Neither needs initialization, but q3_paged_plan must have written
+ * a plan before the other calls read it; zeroed memory is a plan without any tokens. Calls that share
+ * a plan's scratch must not overlap on the GPU. */
 size_t q3_paged_plan_bytes(const q3_paged_shape *shape);
 size_t q3_paged_attention_scratch_bytes(const q3_paged_shape *shape);
 

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
         return bad_starts ? PagedSeq{0, 0, 0, 0} : PagedSeq{start_s[b], start_s[b + 1] - start_s[b], kv_s[b], 0};
     };
     for (int t = tid; t < a.s.n_tokens; t += PLAN_THREADS) {
-        int4 tok = make_int4(-1, bad_starts ? -1 : PAGED_OUTSIDE, -1, -1);
+        int4 tok = make_int4(-1, bad_starts ? PAGED_PADDING : PAGED_OUTSIDE, -1, -1);
         if (!bad_starts && n > 0 && t >= start_s[0] && t < start_s[n]) {
             int lo = 0, hi = n - 1;  // the last sequence that starts at or before t and is not empty there
             while (lo < hi) {
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
             const PagedSeq q = seq(lo);
             const int pos = q.kv_len - q.q_len + (t - q.q0);
             tok.x = lo;
-            tok.y = pos < 0 ? -1 : pos;
+            tok.y = pos < 0 ? PAGED_PADDING : pos + 1;
             if (pos >= 0) {
                 tok.z = table[(size_t)lo * a.s.max_pages + pos / a.s.page_size];
                 tok.w = pos % a.s.page_size;
@@ -382,8 +382,8 @@ __global__ void __launch_bounds__(APPEND_MAX_THREADS, 2) paged_append_kernel(con
     uint4 n0, n1;
     load(src, first < a.n_heads, n0, n1);
     const int4 tok = a.toks[t];
-    const int pos = tok.y;
-    if (pos == PAGED_OUTSIDE) return;
+    const int pos = tok.y - 1;
+    if (tok.y == PAGED_OUTSIDE) return;
     bf16 *dst = a.q_out + t * a.q_out_stride + first * a.head_dim;
     if (pos < 0) {  // padding: zero query rows, nothing stored
         for (int h = first; h < a.n_heads; h += groups, dst += step) store(dst, zero, zero);
@@ -494,8 +494,8 @@ __global__ void __launch_bounds__(APPEND_ODD_THREADS) paged_append_odd_kernel(co
     pdl_wait();
     const int t = blockIdx.x, lane = threadIdx.x % 32;
     const int4 tok = a.toks[t];
-    const int pos = tok.y, D = a.head_dim, half = a.rope_dim / 2;
-    if (pos == PAGED_OUTSIDE) return;
+    const int pos = tok.y - 1, D = a.head_dim, half = a.rope_dim / 2;
+    if (tok.y == PAGED_OUTSIDE) return;
     for (int j = threadIdx.x; j < half; j += APPEND_ODD_THREADS)
         if (pos >= 0) rope_angle(pos, a.inv_freq[j], a.amplitude, &cos_s[j], &sin_s[j]);
     __syncthreads();

@@ -10,9 +10,9 @@ namespace q3 {
 constexpr int PAGED_MAX_SEQS = 4096;
 constexpr int PAGED_MAX_HEAD_DIM = 128;
 
-// A token's sequence and position. pos -1: padding (its rows are written as zeros); PAGED_OUTSIDE:
-// a row of the batch outside every sequence (never written).
-constexpr int PAGED_OUTSIDE = -2;
+// A token's place is its position + 1, or one of these: a row of the batch outside every sequence (never written), or
+// padding (its rows are written as zeros). A plan of zeroed memory has neither tokens nor pieces.
+constexpr int PAGED_OUTSIDE = 0, PAGED_PADDING = -1;
 
 struct PagedSeq {
     int q0, q_len, kv_len, pad;
@@ -56,7 +56,7 @@ inline bool paged_has_big(const q3_paged_shape &s) {
 struct PagedPlanLayout {
     size_t seqs;      // PagedSeq [n_seqs]
     size_t table;     // int [n_seqs][max_pages]: checked page ids, -1 past a sequence's last page
-    size_t toks;      // int4 [n_tokens]: sequence, position, page, slot
+    size_t toks;      // int4 [n_tokens]: sequence, place, page, slot
     size_t ctas;      // int2 [2][PAGED_MAX_CTAS], small items' CTAs and big ones': first piece, pieces (-1: zero every row)
     size_t counters;  // int [PAGED_MAX_CTAS]: pieces done of the small item that starts in the CTA; zero at rest
     size_t ready;     // int [PAGED_MAX_CTAS]: the CTA of the kernel for many rows has waited for what came before; zero at rest

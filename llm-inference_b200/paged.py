@@ -13,6 +13,7 @@ import numpy as np
 from ._lib import Q3Error, call, check, load
 
 _SHAPE, _ARG = 1, 5
+_NO_PLAN = "the plan has not been updated"
 _torch = _device = _raw_stream = None
 
 
@@ -89,7 +90,8 @@ def _vector(name, t, what, size, dtype):
 class PagedPlan:
     """Device work list of a step (q3_paged_plan): make one for the step's shape, `update` it once
     per step, use it in every layer. Owns the attention's scratch too, so calls that share a plan
-    must follow each other on one stream (or be ordered by the caller)."""
+    must follow each other on one stream (or be ordered by the caller). Calls that need the plan are
+    refused before its first `update`."""
 
     def __init__(self, n_seqs: int, n_tokens: int, max_q_len: int, n_heads: int, n_kv_heads: int, head_dim: int,
                  page_size: int, n_pages: int, max_pages: int, device="cuda"):
@@ -100,7 +102,12 @@ class PagedPlan:
         n = load().q3_paged_plan_bytes(self._shape)
         if n == 0:
             _refuse("q3_paged_plan", "the shape is not supported", _SHAPE)
-        self.plan = torch.empty(n, dtype=torch.uint8, device=device)
+        # zeros are a plan without any work, for the time between a captured first update and its replay
+        self.plan = torch.zeros(n, dtype=torch.uint8, device=device)
+        self._updated, self._zeroed = False, None
+        if self.plan.is_cuda and not torch.cuda.is_current_stream_capturing():
+            made_on = torch.cuda.current_stream(self.plan.device)
+            self._zeroed = made_on.cuda_stream, made_on.record_event()
         self.scratch = torch.empty(load().q3_paged_attention_scratch_bytes(self._shape), dtype=torch.uint8,
                                    device=device)
         self.n_tokens, self.head_dim, self.scale = n_tokens, head_dim, head_dim ** -0.5
@@ -112,10 +119,17 @@ class PagedPlan:
         self._strides = None  # of the pages that _cache describes
 
     def update(self, q_start, kv_len, page_table, stream=None):
-        s, name, i32 = self.shape, "q3_paged_plan", _t().int32
+        torch, s, name, stream = _t(), self.shape, "q3_paged_plan", _stream(stream)
+        i32 = torch.int32
+        if self._zeroed is not None and not torch.cuda.is_current_stream_capturing():  # a capture began after a wait for all
+            made_on, zeroed = self._zeroed
+            if stream != made_on:
+                torch.cuda.ExternalStream(stream, self.plan.device).wait_event(zeroed)
+            self._zeroed = None
         call(name, self._ptr, self._shape, _vector(name, q_start, "q_start", s.n_seqs + 1, i32),
              _vector(name, kv_len, "kv_len", s.n_seqs, i32),
-             _vector(name, page_table, "page_table", s.n_seqs * s.max_pages, i32), _stream(stream))
+             _vector(name, page_table, "page_table", s.n_seqs * s.max_pages, i32), stream)
+        self._updated = True
 
     def _bind(self, name, key_pages, value_pages):
         """The pages as the C struct."""
@@ -141,6 +155,8 @@ def paged_rope_append(q_out, q, k, v, key_pages, value_pages, plan: PagedPlan, i
     """Norms, rotary positions and the write into the pages (q3_paged_rope_append). inv_freq holds
     rope_dim / 2 fp32 frequencies on the device (`rope_inv_freq`); None rotates nothing."""
     name, bf, n, qw, kw = "q3_paged_rope_append", _t().bfloat16, plan.n_tokens, plan.q_width, plan.kv_width
+    if not plan._updated:
+        _refuse(name, _NO_PLAN)
     status = load().q3_paged_rope_append(
         q_out.data_ptr(), _rows(name, q_out, "q_out", n, qw, bf), q.data_ptr(), _rows(name, q, "q", n, qw, bf),
         k.data_ptr(), _rows(name, k, "k", n, kw, bf), v.data_ptr(), _rows(name, v, "v", n, kw, bf),
@@ -155,6 +171,8 @@ def paged_attention(out, q, key_pages, value_pages, plan: PagedPlan, scale: floa
     """Attention of the step's new tokens over the pages (q3_paged_attention); scale defaults to
     1 / sqrt(head_dim)."""
     name, bf, n, qw = "q3_paged_attention", _t().bfloat16, plan.n_tokens, plan.q_width
+    if not plan._updated:
+        _refuse(name, _NO_PLAN)
     status = load().q3_paged_attention(
         out.data_ptr(), _rows(name, out, "out", n, qw, bf), q.data_ptr(), _rows(name, q, "q", n, qw, bf),
         plan._bind(name, key_pages, value_pages), plan.scale if scale is None else scale, plan._shape, plan._ptr,

@@ -165,3 +165,13 @@ def logits(lib, **kw):
     (dict(x=4098, dtype=1, out=8192), 2)])
 def test_logits_refuse(lib, kw, status):
     assert logits(lib, **kw) == status
+
+
+def test_a_plan_is_refused_before_its_first_update():
+    plan = q3.PagedPlan(*GOOD.values(), device="cpu")
+    assert not plan.plan.any()
+    for call in (lambda: q3.paged_attention(None, None, None, None, plan),
+                 lambda: q3.paged_rope_append(None, None, None, None, None, None, plan)):
+        with pytest.raises(q3.Q3Error, match="has not been updated") as e:
+            call()
+        assert e.value.status == 5

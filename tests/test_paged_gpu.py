@@ -574,3 +574,42 @@ def test_a_captured_mixed_step_follows_its_inputs():
             assert (out[n:] == 7.0).all()
             for s, (m, kv_s) in enumerate(b.lens):
                 assert torch.equal(b.cached(b.vp, s)[max(0, kv_s - m):], v[b.rows(s)][max(0, m - kv_s):])
+
+
+# a plan whose first update has only been captured describes nothing yet
+@pytest.mark.parametrize("most", [1, 40])
+def test_a_plan_that_was_only_captured_does_nothing(most):
+    b = Batch([(1, 20), (most, 60)], 8, 2, 64, 16, seed=3)
+    q, k, v = rn(b.g, b.tokens, 8, 64), rn(b.g, b.tokens, 2, 64), rn(b.g, b.tokens, 2, 64)
+    out, q_out = torch.full_like(q, 7.0), torch.full_like(q, 7.0)
+    kp, vp = b.kp.clone(), b.vp.clone()
+    with pytest.raises(q3.Q3Error):
+        q3.paged_attention(out, q, b.kp, b.vp, b.plan)
+    warm = Batch(b.lens, 8, 2, 64, 16, seed=3)
+    attend(warm, q)  # kernel attributes are set before the capture
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.update()
+    for interleaved in (False, True):
+        q3.paged_rope_append(q_out, q, k, v, b.kp, b.vp, b.plan, interleaved=interleaved)
+    q3.paged_rope_append(q_out, q, k, v, b.kp, b.vp, b.plan, torch.ones(10, device="cuda"))
+    q3.paged_attention(out, q, b.kp, b.vp, b.plan)
+    torch.cuda.synchronize()
+    assert torch.equal(b.kp, kp) and torch.equal(b.vp, vp)
+    assert (out == 7.0).all() and (q_out == 7.0).all() and q3.device_error() == 0
+    graph.replay()
+    q3.paged_attention(out, q, b.kp, b.vp, b.plan)
+    check_attention(out, *b.attention_exact(q, 0.125), "after the replay")
+
+
+def test_a_first_update_on_another_stream():
+    side = torch.cuda.Stream()
+    b = Batch([(1, 20), (30, 60)], 8, 2, 64, 16, seed=3)
+    q = rn(b.g, b.tokens, 8, 64)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        torch.cuda._sleep(1000000)  # the zeros of a new plan come late on this stream
+        b.plan = q3.PagedPlan(2, b.tokens, 30, 8, 2, 64, 16, b.n_pages, b.max_pages)
+        with torch.cuda.stream(side):
+            out = attend(b, q)
+        check_attention(out, *b.attention_exact(q, 0.125), "updated on another stream")
