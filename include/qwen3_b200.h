@@ -457,12 +457,20 @@ int q3_rope_inv_freq(float *inv_freq, float *amplitude, int rope_dim, float thet
  * [0, vocab) are ignored (negative ids can pad). hist_start and bias_start must not fall; a row for
  * which one does, or whose split is outside its history, sets device error bit 2 and is treated
  * as having none. Strides are elements between rows (mask_stride: words); out may be logits (same
- * stride). */
+ * stride). hist_ids, bias_ids and bias must reach as far as the last entries of their starts say. */
 int q3_logits_process(void *out, const void *logits, int dtype, int rows, int vocab, long long out_stride,
                       long long stride, const int *hist_start, const int *hist_split, const int *hist_ids,
                       const float *repetition, const float *frequency, const float *presence, const int *bias_start,
                       const int *bias_ids, const float *bias, const unsigned *mask, long long mask_stride,
                       void *stream);
+
+/* The same for arrays whose lengths are known: hist_ids has n_hist entries, bias_ids and bias n_bias. A row whose
+ * range goes past them sets device error bit 2 and is treated as having none; nothing past them is read. */
+int q3_logits_process_bounded(void *out, const void *logits, int dtype, int rows, int vocab, long long out_stride,
+                              long long stride, const int *hist_start, const int *hist_split, const int *hist_ids,
+                              long long n_hist, const float *repetition, const float *frequency, const float *presence,
+                              const int *bias_start, const int *bias_ids, const float *bias, long long n_bias,
+                              const unsigned *mask, long long mask_stride, void *stream);
 
 #ifdef __cplusplus
 }

@@ -74,6 +74,7 @@ SIGNATURES: dict[str, list] = {
     "q3_paged_attention": [_P, _LL, _P, _LL, _P, _F, _P, _P, _P, _P],
     "q3_rope_inv_freq": [_P, _P, _I, _F, _P],
     "q3_logits_process": [_P, _P, _I, _I, _I, _LL, _LL, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _LL, _P],
+    "q3_logits_process_bounded": [_P, _P, _I, _I, _I, _LL, _LL, _P, _P, _P, _LL, _P, _P, _P, _P, _P, _P, _LL, _P, _LL, _P],
 }
 RESTYPES = {"q3_status_string": ctypes.c_char_p, "q3_attention_scratch_bytes": ctypes.c_size_t,
             "q3_paged_plan_bytes": ctypes.c_size_t, "q3_paged_attention_scratch_bytes": ctypes.c_size_t,

@@ -1,4 +1,4 @@
-// Penalties, biases and grammar masks on a step's logits (q3_logits_process).
+// Penalties, biases and grammar masks on a step's logits (q3_logits_process, q3_logits_process_bounded).
 //
 // A CTA owns a slice of one row's vocabulary, eight tokens a thread, whose logits it asks for first. Meanwhile
 // it counts the row's history into shared memory (bit 31: the token occurs, low bits: how often it was
@@ -14,6 +14,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <limits>
 
 #include "common.cuh"
 
@@ -30,7 +31,7 @@ constexpr unsigned LP_SEEN = 1u << 31;
 struct LogitsArgs {
     void *out;
     const void *in;
-    int vocab, vec;
+    int vocab, vec, n_hist, n_bias;  // n_: entries of hist_ids, and of bias_ids and bias
     long long out_stride, stride, mask_stride;
     const int *hist_start, *hist_split, *hist_ids;
     const float *repetition, *frequency, *presence;
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(512) logits_process_kernel(const __grid_consta
         h0 = a.hist_start[r];
         h1 = a.hist_start[r + 1];
         hs = a.hist_split[r];
-        if (h0 < 0 || h1 < h0 || hs < h0 || hs > h1) {
+        if (h0 < 0 || h1 < h0 || hs < h0 || hs > h1 || h1 > a.n_hist) {
             if (tid == 0) atomicOr(&g_dev_error, DEV_ERR_POS_RANGE);
             h1 = h0;
         }
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(512) logits_process_kernel(const __grid_consta
     if (a.bias_start) {
         b0 = a.bias_start[r];
         b1 = a.bias_start[r + 1];
-        if (b0 < 0 || b1 < b0) {
+        if (b0 < 0 || b1 < b0 || b1 > a.n_bias) {
             if (tid == 0) atomicOr(&g_dev_error, DEV_ERR_POS_RANGE);
             b1 = b0;
         }
@@ -218,16 +219,19 @@ unsigned take_error_logits() {
 
 using namespace q3;
 
-extern "C" int q3_logits_process(void *out, const void *logits, int dtype, int rows, int vocab, long long out_stride,
-                                 long long stride, const int *hist_start, const int *hist_split, const int *hist_ids,
-                                 const float *repetition, const float *frequency, const float *presence,
-                                 const int *bias_start, const int *bias_ids, const float *bias, const unsigned *mask,
-                                 long long mask_stride, void *stream) {
+extern "C" {
+
+int q3_logits_process_bounded(void *out, const void *logits, int dtype, int rows, int vocab, long long out_stride,
+                              long long stride, const int *hist_start, const int *hist_split, const int *hist_ids,
+                              long long n_hist, const float *repetition, const float *frequency, const float *presence,
+                              const int *bias_start, const int *bias_ids, const float *bias, long long n_bias,
+                              const unsigned *mask, long long mask_stride, void *stream) {
     if (!out || !logits || (dtype != 0 && dtype != 1)) return Q3_ERR_ARG;
     if (rows < 0 || rows > 65535 || vocab <= 0 || stride < vocab || out_stride < vocab) return Q3_ERR_SHAPE;
     if (out == logits && out_stride != stride) return Q3_ERR_SHAPE;
     if (hist_start && (!hist_split || !hist_ids)) return Q3_ERR_ARG;
     if (bias_start && (!bias_ids || !bias)) return Q3_ERR_ARG;
+    if ((hist_start && n_hist < 0) || (bias_start && n_bias < 0)) return Q3_ERR_SHAPE;
     if (mask && mask_stride < ((long long)vocab + 31) / 32) return Q3_ERR_SHAPE;
     if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(logits)) & (dtype ? 3 : 1)) return Q3_ERR_ALIGN;
     const int st = check_device();
@@ -237,8 +241,9 @@ extern "C" int q3_logits_process(void *out, const void *logits, int dtype, int r
     // the same place in a 16-byte line for each row's input and output, and whole lines between places of a row
     const bool vec = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(logits)) & 15) == 0 &&
                      (out_stride - stride) * elt % 16 == 0;
-    LogitsArgs a = {out,        logits,    vocab,    vec,        out_stride, stride, mask_stride, hist_start, hist_split, hist_ids,
-                    repetition, frequency, presence, bias_start, bias_ids,   bias,   mask};
+    const long long most = std::numeric_limits<int>::max();  // what a start can say
+    LogitsArgs a = {out, logits, vocab, vec, (int)std::min(n_hist, most), (int)std::min(n_bias, most), out_stride, stride,
+                    mask_stride, hist_start, hist_split, hist_ids, repetition, frequency, presence, bias_start, bias_ids, bias, mask};
     if (!repetition && !frequency && !presence) a.hist_start = nullptr;
     // two slices an SM at least; 128 threads are the smallest that make whole warps busy
     int threads = 512;
@@ -252,3 +257,14 @@ extern "C" int q3_logits_process(void *out, const void *logits, int dtype, int r
     Q3_TRY_LAUNCH(launch(kernel, grid, dim3(threads), smem, (cudaStream_t)stream, 1, a));
     return Q3_OK;
 }
+
+int q3_logits_process(void *out, const void *logits, int dtype, int rows, int vocab, long long out_stride, long long stride,
+                      const int *hist_start, const int *hist_split, const int *hist_ids, const float *repetition,
+                      const float *frequency, const float *presence, const int *bias_start, const int *bias_ids,
+                      const float *bias, const unsigned *mask, long long mask_stride, void *stream) {
+    const long long any = std::numeric_limits<int>::max();
+    return q3_logits_process_bounded(out, logits, dtype, rows, vocab, out_stride, stride, hist_start, hist_split, hist_ids, any,
+                                     repetition, frequency, presence, bias_start, bias_ids, bias, any, mask, mask_stride, stream);
+}
+
+}  // extern "C"

@@ -195,7 +195,7 @@ def rope_inv_freq(rope_dim: int, theta: float, kind: str = "plain", **scaling) -
 
 def logits_process(out, logits, hist_start=None, hist_split=None, hist_ids=None, repetition=None, frequency=None,
                    presence=None, bias_start=None, bias_ids=None, bias=None, mask=None, stream=None):
-    """Penalties, biases and grammar masks on [rows, vocab] logits, bf16 or fp32 (q3_logits_process);
+    """Penalties, biases and grammar masks on [rows, vocab] logits, bf16 or fp32 (q3_logits_process_bounded);
     out may be logits. mask is int32 [rows, >= ceil(vocab / 32)], one bit per allowed token."""
     torch = _t()
     name, dtype, i32, f32 = "q3_logits_process", logits.dtype, torch.int32, torch.float32
@@ -210,20 +210,21 @@ def logits_process(out, logits, hist_start=None, hist_split=None, hist_ids=None,
         if mask.dim() != 2 or mask.shape[1] * 32 < vocab:
             _refuse(name, "mask must be [rows, at least vocab / 32 words]", _SHAPE)
         mask_ptr, mask_stride = mask.data_ptr(), _rows(name, mask, "mask", rows, mask.shape[1], i32)
-    if hist_ids is not None and hist_ids.numel() == 0:  # an empty tensor has no address to pass
-        hist_start = hist_split = hist_ids = None
+    hist, history, n_hist = _vector(name, hist_start, "hist_start", rows + 1, i32), None, 0
+    if hist_ids is not None:  # an empty tensor has no address to pass; of none, nothing is read at another one
+        n_hist = hist_ids.numel()
+        history = _vector(name, hist_ids, "hist_ids", None, i32) if n_hist else hist
+    bias_at, biased, added, n_bias = _vector(name, bias_start, "bias_start", rows + 1, i32), None, None, 0
     if bias_ids is not None:
-        if bias is not None and bias.numel() != bias_ids.numel():
+        n_bias = bias_ids.numel()
+        if bias is not None and bias.numel() != n_bias:
             _refuse(name, "bias and bias_ids differ in length", _SHAPE)
-        if bias_ids.numel() == 0:
-            bias_start = bias_ids = bias = None
-    status = load().q3_logits_process(
+        biased = _vector(name, bias_ids, "bias_ids", None, i32) if n_bias else bias_at
+        added = _vector(name, bias, "bias", None, f32) if n_bias else bias_at
+    status = load().q3_logits_process_bounded(
         out.data_ptr(), logits.data_ptr(), dtype is f32, rows, vocab, _rows(name, out, "out", rows, vocab, dtype),
-        _rows(name, logits, "logits", rows, vocab, dtype), _vector(name, hist_start, "hist_start", rows + 1, i32),
-        _vector(name, hist_split, "hist_split", rows, i32), _vector(name, hist_ids, "hist_ids", None, i32),
-        _vector(name, repetition, "repetition", rows, f32), _vector(name, frequency, "frequency", rows, f32),
-        _vector(name, presence, "presence", rows, f32), _vector(name, bias_start, "bias_start", rows + 1, i32),
-        _vector(name, bias_ids, "bias_ids", None, i32), _vector(name, bias, "bias", None, f32), mask_ptr, mask_stride,
-        _stream(stream))
+        _rows(name, logits, "logits", rows, vocab, dtype), hist, _vector(name, hist_split, "hist_split", rows, i32), history,
+        n_hist, _vector(name, repetition, "repetition", rows, f32), _vector(name, frequency, "frequency", rows, f32),
+        _vector(name, presence, "presence", rows, f32), bias_at, biased, added, n_bias, mask_ptr, mask_stride, _stream(stream))
     if status:
         check(name, status)

@@ -221,3 +221,35 @@ def test_refusals():
     refuses(5, x, x, mask=torch.zeros(2, 2, dtype=torch.int64, device="cuda"))
     refuses(5, x, x, hist_start=torch.zeros(3, dtype=torch.int32, device="cuda"), repetition=torch.ones(2, device="cuda"))
     refuses(1, x, x, hist_start=torch.zeros(2, dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("vocab", [64, 5001])
+@pytest.mark.parametrize("have,hist,bias", [(4, 5, 3), (4, 2 ** 31 - 1, 4), (4, 4, 5), (4, 3, 2 ** 31 - 1), (0, 1, 0), (0, 0, 1)])
+def test_ranges_past_their_arrays_are_flagged(vocab, have, hist, bias):
+    # the second row's history or biases end past the arrays: it has none then, the first row has what it says
+    i32 = dict(dtype=torch.int32, device="cuda")
+    x = torch.randn(2, vocab, device="cuda")
+    ids = torch.tensor([1, 2, 3, 4], **i32)[:have]
+    own = min(have, 2)
+    out = torch.empty_like(x)
+    q3.logits_process(out, x, torch.tensor([0, own, hist], **i32), torch.tensor([0, own], **i32), ids,
+                      frequency=torch.full((2,), 2.0, device="cuda"), bias_start=torch.tensor([0, own, bias], **i32), bias_ids=ids,
+                      bias=torch.full((have,), 8.0, device="cuda"))
+    assert q3.device_error() == 4
+    want = x.clone()
+    for row, (h, b) in enumerate([(own, own), (hist, bias)]):
+        lo = [0, own][row]
+        if h <= have:
+            want[row, ids[lo:h].long()] -= 2.0
+        if b <= have:
+            want[row, ids[lo:b].long()] += 8.0
+    assert torch.equal(out, want)
+
+
+def test_empty_histories_and_biases():
+    i32 = dict(dtype=torch.int32, device="cuda")
+    x = torch.randn(3, 100, device="cuda")
+    out, zero = torch.empty_like(x), torch.zeros(4, **i32)
+    none, two = torch.zeros(0, **i32), torch.full((3,), 2.0, device="cuda")
+    q3.logits_process(out, x, zero, zero[:3], none, repetition=two, bias_start=zero, bias_ids=none)
+    assert torch.equal(out, x) and q3.device_error() == 0

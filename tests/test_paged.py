@@ -175,3 +175,10 @@ def test_a_plan_is_refused_before_its_first_update():
         with pytest.raises(q3.Q3Error, match="has not been updated") as e:
             call()
         assert e.value.status == 5
+
+
+@pytest.mark.parametrize("n_hist,n_bias,status", [(-1, 5, 1), (5, -1, 1), (-1, -1, 1)])
+def test_logits_refuse_negative_lengths(lib, n_hist, n_bias, status):
+    fake = 4096
+    assert lib.q3_logits_process_bounded(fake, fake, 0, 2, 1000, 1000, 1000, fake, fake, fake, n_hist, fake, fake, fake, fake,
+                                         fake, fake, n_bias, None, 0, None) == status
