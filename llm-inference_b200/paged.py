@@ -2,7 +2,8 @@
 
 Page tensors are [n_pages, n_kv_heads, page_size, head_dim] torch views with a contiguous last
 dimension; a pool laid out [n_pages, page_size, n_kv_heads, head_dim] is passed as
-``pool.transpose(1, 2)``. Launches go to torch's current stream unless one is given.
+``pool.transpose(1, 2)``. Launches go to torch's current stream unless one is given; all tensors must be on
+the current device, and so must the plan.
 """
 from __future__ import annotations
 
@@ -13,7 +14,9 @@ import numpy as np
 from ._lib import Q3Error, call, check, load
 
 _SHAPE, _ARG = 1, 5
+_NO_DEVICE = -2  # no tensor's device: the CPU's is -1
 _NO_PLAN = "the plan has not been updated"
+_ELSEWHERE = "the plan is on another device"
 _torch = _device = _raw_stream = None
 
 
@@ -24,7 +27,7 @@ def _t():
         import torch
         _torch = torch
         # the current device's index and its stream's handle without objects around them, where torch has these
-        _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device) if torch.cuda.is_available() else lambda: _NO_DEVICE
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda _: torch.cuda.current_stream().cuda_stream)
     return _torch
 
@@ -58,10 +61,10 @@ def _refuse(name, what, status=_ARG):
 
 # These calls run once per layer of every step, so the checks read as few tensor attributes as they can.
 
-def _rows(name, t, what, rows, width, dtype):
+def _rows(name, t, what, rows, width, dtype, dev):
     """Row stride of a [rows, ...] tensor whose rows are `width` contiguous elements."""
-    if t.dtype is not dtype or not t.is_cuda:
-        _refuse(name, f"{what} must be a CUDA tensor of {dtype}")
+    if t.dtype is not dtype or t.get_device() != dev:
+        _refuse(name, f"{what} must be a tensor of {dtype} on the current CUDA device")
     shape = t.shape
     if not shape or shape[0] != rows:
         _refuse(name, f"{what}: {tuple(shape)}, expected {rows} rows", _SHAPE)
@@ -77,11 +80,11 @@ def _rows(name, t, what, rows, width, dtype):
     return t.stride(0) if rows > 1 else width
 
 
-def _vector(name, t, what, size, dtype):
+def _vector(name, t, what, size, dtype, dev):
     if t is None:
         return None
-    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
-        _refuse(name, f"{what} must be a contiguous CUDA tensor of {dtype}")
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+        _refuse(name, f"{what} must be a contiguous tensor of {dtype} on the current CUDA device")
     if size is not None and t.numel() != size:
         _refuse(name, f"{what}: {t.numel()} elements, expected {size}", _SHAPE)
     return t.data_ptr()
@@ -104,7 +107,7 @@ class PagedPlan:
             _refuse("q3_paged_plan", "the shape is not supported", _SHAPE)
         # zeros are a plan without any work, for the time between a captured first update and its replay
         self.plan = torch.zeros(n, dtype=torch.uint8, device=device)
-        self._updated, self._zeroed = False, None
+        self._updated, self._zeroed, self._on = False, None, self.plan.get_device()
         if self.plan.is_cuda and not torch.cuda.is_current_stream_capturing():
             made_on = torch.cuda.current_stream(self.plan.device)
             self._zeroed = made_on.cuda_stream, made_on.record_event()
@@ -120,22 +123,24 @@ class PagedPlan:
 
     def update(self, q_start, kv_len, page_table, stream=None):
         torch, s, name, stream = _t(), self.shape, "q3_paged_plan", _stream(stream)
-        i32 = torch.int32
+        i32, dev = torch.int32, _device()
+        if self._on != dev:
+            _refuse(name, _ELSEWHERE)
         if self._zeroed is not None and not torch.cuda.is_current_stream_capturing():  # a capture began after a wait for all
             made_on, zeroed = self._zeroed
             if stream != made_on:
                 torch.cuda.ExternalStream(stream, self.plan.device).wait_event(zeroed)
             self._zeroed = None
-        call(name, self._ptr, self._shape, _vector(name, q_start, "q_start", s.n_seqs + 1, i32),
-             _vector(name, kv_len, "kv_len", s.n_seqs, i32),
-             _vector(name, page_table, "page_table", s.n_seqs * s.max_pages, i32), stream)
+        call(name, self._ptr, self._shape, _vector(name, q_start, "q_start", s.n_seqs + 1, i32, dev),
+             _vector(name, kv_len, "kv_len", s.n_seqs, i32, dev),
+             _vector(name, page_table, "page_table", s.n_seqs * s.max_pages, i32, dev), stream)
         self._updated = True
 
-    def _bind(self, name, key_pages, value_pages):
+    def _bind(self, name, key_pages, value_pages, dev):
         """The pages as the C struct."""
         bf16, c = _t().bfloat16, self._cache
-        if key_pages.dtype is not bf16 or value_pages.dtype is not bf16 or not (key_pages.is_cuda and value_pages.is_cuda):
-            _refuse(name, "pages must be CUDA tensors of torch.bfloat16")
+        if key_pages.dtype is not bf16 or value_pages.dtype is not bf16 or not key_pages.get_device() == value_pages.get_device() == dev:
+            _refuse(name, "pages must be tensors of torch.bfloat16 on the current CUDA device")
         if key_pages.shape != self._pages or value_pages.shape != self._pages:
             _refuse(name, f"pages {tuple(key_pages.shape)} and {tuple(value_pages.shape)}, expected {self._pages}", _SHAPE)
         strides = key_pages.stride()
@@ -157,12 +162,15 @@ def paged_rope_append(q_out, q, k, v, key_pages, value_pages, plan: PagedPlan, i
     name, bf, n, qw, kw = "q3_paged_rope_append", _t().bfloat16, plan.n_tokens, plan.q_width, plan.kv_width
     if not plan._updated:
         _refuse(name, _NO_PLAN)
+    dev = _device()
+    if plan._on != dev:
+        _refuse(name, _ELSEWHERE)
     status = load().q3_paged_rope_append(
-        q_out.data_ptr(), _rows(name, q_out, "q_out", n, qw, bf), q.data_ptr(), _rows(name, q, "q", n, qw, bf),
-        k.data_ptr(), _rows(name, k, "k", n, kw, bf), v.data_ptr(), _rows(name, v, "v", n, kw, bf),
-        _vector(name, q_norm_w, "q_norm_w", plan.head_dim, bf), _vector(name, k_norm_w, "k_norm_w", plan.head_dim, bf),
-        eps, _vector(name, inv_freq, "inv_freq", None, _torch.float32), 0 if inv_freq is None else 2 * inv_freq.numel(),
-        interleaved, amplitude, plan._bind(name, key_pages, value_pages), plan._shape, plan._ptr, _stream(stream))
+        q_out.data_ptr(), _rows(name, q_out, "q_out", n, qw, bf, dev), q.data_ptr(), _rows(name, q, "q", n, qw, bf, dev),
+        k.data_ptr(), _rows(name, k, "k", n, kw, bf, dev), v.data_ptr(), _rows(name, v, "v", n, kw, bf, dev),
+        _vector(name, q_norm_w, "q_norm_w", plan.head_dim, bf, dev), _vector(name, k_norm_w, "k_norm_w", plan.head_dim, bf, dev),
+        eps, _vector(name, inv_freq, "inv_freq", None, _torch.float32, dev), 0 if inv_freq is None else 2 * inv_freq.numel(),
+        interleaved, amplitude, plan._bind(name, key_pages, value_pages, dev), plan._shape, plan._ptr, _stream(stream))
     if status:
         check(name, status)
 
@@ -173,9 +181,12 @@ def paged_attention(out, q, key_pages, value_pages, plan: PagedPlan, scale: floa
     name, bf, n, qw = "q3_paged_attention", _t().bfloat16, plan.n_tokens, plan.q_width
     if not plan._updated:
         _refuse(name, _NO_PLAN)
+    dev = _device()
+    if plan._on != dev:
+        _refuse(name, _ELSEWHERE)
     status = load().q3_paged_attention(
-        out.data_ptr(), _rows(name, out, "out", n, qw, bf), q.data_ptr(), _rows(name, q, "q", n, qw, bf),
-        plan._bind(name, key_pages, value_pages), plan.scale if scale is None else scale, plan._shape, plan._ptr,
+        out.data_ptr(), _rows(name, out, "out", n, qw, bf, dev), q.data_ptr(), _rows(name, q, "q", n, qw, bf, dev),
+        plan._bind(name, key_pages, value_pages, dev), plan.scale if scale is None else scale, plan._shape, plan._ptr,
         plan._scratch_ptr, _stream(stream))
     if status:
         check(name, status)
@@ -204,27 +215,27 @@ def logits_process(out, logits, hist_start=None, hist_split=None, hist_ids=None,
     shape = logits.shape
     if len(shape) != 2 or out.shape != shape:
         _refuse(name, "logits and out must both be [rows, vocab]", _SHAPE)
-    rows, vocab = shape
+    (rows, vocab), dev = shape, _device()
     mask_ptr, mask_stride = None, 0
     if mask is not None:
         if mask.dim() != 2 or mask.shape[1] * 32 < vocab:
             _refuse(name, "mask must be [rows, at least vocab / 32 words]", _SHAPE)
-        mask_ptr, mask_stride = mask.data_ptr(), _rows(name, mask, "mask", rows, mask.shape[1], i32)
-    hist, history, n_hist = _vector(name, hist_start, "hist_start", rows + 1, i32), None, 0
+        mask_ptr, mask_stride = mask.data_ptr(), _rows(name, mask, "mask", rows, mask.shape[1], i32, dev)
+    hist, history, n_hist = _vector(name, hist_start, "hist_start", rows + 1, i32, dev), None, 0
     if hist_ids is not None:  # an empty tensor has no address to pass; of none, nothing is read at another one
         n_hist = hist_ids.numel()
-        history = _vector(name, hist_ids, "hist_ids", None, i32) if n_hist else hist
-    bias_at, biased, added, n_bias = _vector(name, bias_start, "bias_start", rows + 1, i32), None, None, 0
+        history = _vector(name, hist_ids, "hist_ids", None, i32, dev) if n_hist else hist
+    bias_at, biased, added, n_bias = _vector(name, bias_start, "bias_start", rows + 1, i32, dev), None, None, 0
     if bias_ids is not None:
         n_bias = bias_ids.numel()
         if bias is not None and bias.numel() != n_bias:
             _refuse(name, "bias and bias_ids differ in length", _SHAPE)
-        biased = _vector(name, bias_ids, "bias_ids", None, i32) if n_bias else bias_at
-        added = _vector(name, bias, "bias", None, f32) if n_bias else bias_at
+        biased = _vector(name, bias_ids, "bias_ids", None, i32, dev) if n_bias else bias_at
+        added = _vector(name, bias, "bias", None, f32, dev) if n_bias else bias_at
     status = load().q3_logits_process_bounded(
-        out.data_ptr(), logits.data_ptr(), dtype is f32, rows, vocab, _rows(name, out, "out", rows, vocab, dtype),
-        _rows(name, logits, "logits", rows, vocab, dtype), hist, _vector(name, hist_split, "hist_split", rows, i32), history,
-        n_hist, _vector(name, repetition, "repetition", rows, f32), _vector(name, frequency, "frequency", rows, f32),
-        _vector(name, presence, "presence", rows, f32), bias_at, biased, added, n_bias, mask_ptr, mask_stride, _stream(stream))
+        out.data_ptr(), logits.data_ptr(), dtype is f32, rows, vocab, _rows(name, out, "out", rows, vocab, dtype, dev),
+        _rows(name, logits, "logits", rows, vocab, dtype, dev), hist, _vector(name, hist_split, "hist_split", rows, i32, dev), history,
+        n_hist, _vector(name, repetition, "repetition", rows, f32, dev), _vector(name, frequency, "frequency", rows, f32, dev),
+        _vector(name, presence, "presence", rows, f32, dev), bias_at, biased, added, n_bias, mask_ptr, mask_stride, _stream(stream))
     if status:
         check(name, status)

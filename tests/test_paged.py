@@ -182,3 +182,77 @@ def test_logits_refuse_negative_lengths(lib, n_hist, n_bias, status):
     fake = 4096
     assert lib.q3_logits_process_bounded(fake, fake, 0, 2, 1000, 1000, 1000, fake, fake, fake, n_hist, fake, fake, fake, fake,
                                          fake, fake, n_bias, None, 0, None) == status
+
+
+class Elsewhere:
+    """As much of a tensor as the checks look at; on GPU `device`, and without any memory."""
+
+    def __init__(self, shape, dtype, device):
+        self.shape, self.dtype, self.device, self.is_cuda = shape, dtype, device, True
+
+    def get_device(self):
+        return self.device
+
+    def numel(self):
+        return math.prod(self.shape)
+
+    def dim(self):
+        return len(self.shape)
+
+    def is_contiguous(self):
+        return True
+
+    def stride(self, i=None):
+        steps = tuple(math.prod(self.shape[j + 1:]) for j in range(len(self.shape)))
+        return steps if i is None else steps[i]
+
+    def data_ptr(self):
+        return 4096  # never dereferenced: refused before any launch
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    import torch
+    paged._t()
+    monkeypatch.setattr(paged, "_device", lambda: 0)
+    monkeypatch.setattr(paged, "_raw_stream", lambda device: 0)
+    bf, i32, f32 = torch.bfloat16, torch.int32, torch.float32
+    plan = q3.PagedPlan(*GOOD.values(), device="cpu")
+    plan._on, plan._updated = 0, True
+    launched = []
+    monkeypatch.setattr(paged, "call", lambda *a: launched.append(a[0]))
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: launched.append(name)
+
+    monkeypatch.setattr(paged, "load", Lib)
+
+    def tensors(which, away):
+        return {k: Elsewhere(shape, dtype, 1 if k == away else 0) for k, (shape, dtype) in which.items()}
+
+    pages, q, kv = ((100, 8, 16, 128), bf), ((9, 4096), bf), ((9, 1024), bf)
+    calls = [
+        (lambda t: plan.update(*t.values()), dict(q_start=((5,), i32), kv_len=((4,), i32), table=((4, 20), i32))),
+        (lambda t: q3.paged_attention(*t.values(), plan), dict(out=q, q=q, key_pages=pages, value_pages=pages)),
+        (lambda t: q3.paged_rope_append(*[t[k] for k in ("q_out", "q", "k", "v", "key_pages", "value_pages")], plan, t["inv_freq"],
+                                        t["q_norm_w"], t["k_norm_w"]),
+         dict(q_out=q, q=q, k=kv, v=kv, key_pages=pages, value_pages=pages, inv_freq=((64,), f32), q_norm_w=((128,), bf),
+              k_norm_w=((128,), bf))),
+        (lambda t: q3.logits_process(**t),
+         dict(out=((3, 64), f32), logits=((3, 64), f32), hist_start=((4,), i32), hist_split=((3,), i32), hist_ids=((9,), i32),
+              repetition=((3,), f32), frequency=((3,), f32), presence=((3,), f32), bias_start=((4,), i32), bias_ids=((5,), i32),
+              bias=((5,), f32), mask=((3, 2), i32)))]
+    for go, which in calls:
+        launched.clear()
+        go(tensors(which, None))
+        assert len(launched) == 1
+        for away in which:
+            with pytest.raises(q3.Q3Error) as e:
+                go(tensors(which, away))
+            assert e.value.status == 5, away
+        assert len(launched) == 1
+    plan._on = 1
+    for go, which in calls[:3]:
+        with pytest.raises(q3.Q3Error, match="another device") as e:
+            go(tensors(which, None))
+        assert e.value.status == 5
