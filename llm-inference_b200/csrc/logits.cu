@@ -226,8 +226,10 @@ int q3_logits_process_bounded(void *out, const void *logits, int dtype, int rows
                               long long n_hist, const float *repetition, const float *frequency, const float *presence,
                               const int *bias_start, const int *bias_ids, const float *bias, long long n_bias,
                               const unsigned *mask, long long mask_stride, void *stream) {
-    if (!out || !logits || (dtype != 0 && dtype != 1)) return Q3_ERR_ARG;
+    if (dtype != 0 && dtype != 1) return Q3_ERR_ARG;
     if (rows < 0 || rows > 65535 || vocab <= 0 || stride < vocab || out_stride < vocab) return Q3_ERR_SHAPE;
+    if (rows == 0) return Q3_OK;  // before the pointers: tensors of no elements have none
+    if (!out || !logits) return Q3_ERR_ARG;
     if (out == logits && out_stride != stride) return Q3_ERR_SHAPE;
     if (hist_start && (!hist_split || !hist_ids)) return Q3_ERR_ARG;
     if (bias_start && (!bias_ids || !bias)) return Q3_ERR_ARG;
@@ -236,7 +238,6 @@ int q3_logits_process_bounded(void *out, const void *logits, int dtype, int rows
     if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(logits)) & (dtype ? 3 : 1)) return Q3_ERR_ALIGN;
     const int st = check_device();
     if (st != Q3_OK) return st;
-    if (rows == 0) return Q3_OK;
     const int elt = dtype ? 4 : 2;
     // the same place in a 16-byte line for each row's input and output, and whole lines between places of a row
     const bool vec = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(logits)) & 15) == 0 &&

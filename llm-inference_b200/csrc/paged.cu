@@ -603,7 +603,7 @@ size_t q3_paged_attention_scratch_bytes(const q3_paged_shape *shape) {
 int q3_paged_plan(void *plan, const q3_paged_shape *shape, const int *q_start, const int *kv_len,
                   const int *page_table, void *stream) {
     TRY(paged_shape_check(shape));
-    if (!plan || !q_start || !kv_len || !page_table) return Q3_ERR_ARG;
+    if (!plan || !q_start || (shape->n_seqs > 0 && (!kv_len || !page_table))) return Q3_ERR_ARG;
     if (!aligned16(plan)) return Q3_ERR_ALIGN;
     TRY(check_device());
     PlanArgs a = {static_cast<char *>(plan), paged_plan_layout(*shape), *shape, q_start, kv_len, page_table,
@@ -622,6 +622,7 @@ int q3_paged_rope_append(q3_bf16 *q_out, long long q_out_stride, const q3_bf16 *
     TRY(paged_shape_check(shape));
     const q3_paged_shape &s = *shape;
     const long long qd = (long long)s.n_heads * s.head_dim, kd = (long long)s.n_kv_heads * s.head_dim;
+    if (s.n_tokens == 0) return Q3_OK;  // before the pointers: tensors of no elements have none
     if (!plan) return Q3_ERR_ARG;
     TRY(rows_check(q_out, q_out_stride, qd));
     TRY(rows_check(q, q_stride, qd));
@@ -633,7 +634,6 @@ int q3_paged_rope_append(q3_bf16 *q_out, long long q_out_stride, const q3_bf16 *
     if (q_out == q && q_out_stride != q_stride) return Q3_ERR_SHAPE;
     if (!aligned16(q_norm_w) || !aligned16(k_norm_w) || !aligned16(plan)) return Q3_ERR_ALIGN;
     TRY(check_device());
-    if (s.n_tokens == 0) return Q3_OK;
     AppendArgs a;
     a.q_out = (bf16 *)q_out;
     a.q = (const bf16 *)q;
@@ -677,13 +677,13 @@ int q3_paged_attention(q3_bf16 *out, long long out_stride, const q3_bf16 *q, lon
     TRY(paged_shape_check(shape));
     const q3_paged_shape &s = *shape;
     const long long qd = (long long)s.n_heads * s.head_dim;
+    if (s.n_tokens == 0 || s.n_seqs == 0) return Q3_OK;  // before the pointers: tensors of no elements have none
     if (!plan || !scratch) return Q3_ERR_ARG;
     TRY(rows_check(out, out_stride, qd));
     TRY(rows_check(q, q_stride, qd));
     TRY(cache_check(cache));
     if (!aligned16(plan) || !aligned16(scratch)) return Q3_ERR_ALIGN;
     TRY(check_device());
-    if (s.n_tokens == 0 || s.n_seqs == 0) return Q3_OK;
     const PagedAttnCall c = {(bf16 *)out, (const bf16 *)q, out_stride, q_stride, *cache, scale, s,
                              static_cast<char *>(plan), static_cast<char *>(scratch)};
     return paged_attention(c, (cudaStream_t)stream);

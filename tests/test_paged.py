@@ -256,3 +256,20 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
         with pytest.raises(q3.Q3Error, match="another device") as e:
             go(tensors(which, None))
         assert e.value.status == 5
+
+
+# tensors of no elements have no address
+def test_calls_without_rows_do_nothing(lib):
+    fake = 4096
+    c = paged.Q3PagedCache(fake, fake, 16 * 8 * 128, 16 * 128, 128)
+    s = paged.Q3PagedShape(**dict(GOOD, n_tokens=0))
+    assert lib.q3_paged_attention(None, 4096, None, 4096, ctypes.byref(c), 0.1, ctypes.byref(s), fake, fake, None) == 0
+    assert lib.q3_paged_rope_append(None, 4096, None, 4096, None, 1024, None, 1024, None, None, 1e-6, fake, 128, 0, 1.0,
+                                    ctypes.byref(c), ctypes.byref(s), fake, None) == 0
+    assert logits(lib, rows=0, out=None, x=None) == 0
+    # without sequences, a plan is not refused for its null lengths and page table (but for its alignment), and still is
+    # for a null start
+    none = paged.Q3PagedShape(**dict(GOOD, n_seqs=0, n_tokens=0))
+    assert lib.q3_paged_plan(4097, ctypes.byref(none), fake, None, None, None) == 2
+    assert lib.q3_paged_plan(fake, ctypes.byref(none), None, None, None, None) == 5
+    assert lib.q3_paged_plan(fake, ctypes.byref(s), fake, None, fake, None) == 5

@@ -613,3 +613,21 @@ def test_a_first_update_on_another_stream():
         with torch.cuda.stream(side):
             out = attend(b, q)
         check_attention(out, *b.attention_exact(q, 0.125), "updated on another stream")
+
+
+@pytest.mark.parametrize("n_seqs,max_q", [(0, 0), (0, 40), (3, 1), (3, 40)])
+@pytest.mark.parametrize("tokens", [0, 2])
+def test_steps_without_tokens_or_sequences(n_seqs, max_q, tokens):
+    i32 = dict(dtype=torch.int32, device="cuda")
+    plan = q3.PagedPlan(n_seqs, tokens, max_q, 8, 2, 64, 16, 4, 2)
+    plan.update(torch.zeros(n_seqs + 1, **i32), torch.full((n_seqs,), 20, **i32), torch.zeros(n_seqs, 2, **i32))
+    pages = torch.ones(4, 2, 16, 64, dtype=BF, device="cuda")
+    q, kv = torch.ones(tokens, 8, 64, dtype=BF, device="cuda"), torch.ones(tokens, 2, 64, dtype=BF, device="cuda")
+    out = torch.full_like(q, 7.0)
+    q3.paged_rope_append(out, q, 2 * kv, 2 * kv, pages, pages, plan, torch.ones(32, device="cuda"))
+    q3.paged_attention(out, q, pages, pages, plan)
+    assert (out == 7.0).all() and (pages == 1.0).all()
+    x = torch.ones(0, 50, device="cuda")
+    q3.logits_process(x, x, torch.zeros(1, **i32), torch.zeros(0, **i32), torch.zeros(0, **i32), torch.ones(0, device="cuda"),
+                      mask=torch.zeros(0, 2, **i32))
+    assert q3.device_error() == 0
