@@ -56,6 +56,7 @@ class Sequences:
 
     def __init__(self, n_pages: int, page_size: int, max_seqs: int, max_pages: int, chunk: int):
         self.page_size, self.max_seqs, self.max_pages, self.chunk = page_size, max_seqs, max_pages, chunk
+        self.most = min(max_pages, n_pages) * page_size  # positions that one sequence can have
         self.free = list(range(n_pages - 1, -1, -1))
         self.live: dict[int, Sequence] = {}
         self._next = 0
@@ -65,8 +66,8 @@ class Sequences:
             raise ValueError("an empty prompt")
         if len(self.live) == self.max_seqs:
             raise RuntimeError("every sequence slot is taken")
-        if len(seq.prompt) > self.max_pages * self.page_size:
-            raise ValueError("the prompt is longer than a page table")
+        if len(seq.prompt) > self.most:
+            raise ValueError("the prompt is longer than a page table or the pool")
         self._next += 1
         self.live[self._next] = seq
         return self._next

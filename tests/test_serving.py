@@ -69,3 +69,12 @@ def test_refusals():
     s.add(Sequence([1]))
     with pytest.raises(RuntimeError):
         s.add(Sequence([1]))
+
+
+def test_a_prompt_longer_than_the_pool_is_refused():
+    s = Sequences(n_pages=2, page_size=8, max_seqs=4, max_pages=8, chunk=16)
+    with pytest.raises(ValueError, match="pool"):
+        s.add(Sequence(list(range(17))))
+    assert not s.live
+    a = s.add(Sequence(list(range(16))))
+    assert run(s, 1) == [([(a, 16)], [a])]
