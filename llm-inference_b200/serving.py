@@ -8,10 +8,13 @@ model: the projections of the batched ABI, and per layer ``paged_rope_append`` a
 
     server = PagedServer(DeviceWeights.load(model_dir), n_pages=4096)
     a = server.add(prompt, repetition=1.1)
-    while not done:
+    while server.running():
         for seq, token in server.step().items():
-            ...
+            ...  # server.remove(seq) once it has said what it had to
     server.remove(a)
+
+A sequence runs until its page table (or the whole pool) is full; it then keeps its tokens, gives its pages back and
+gets no more tokens. A step in which only prompts are taken in returns no tokens.
 """
 from __future__ import annotations
 
@@ -72,8 +75,16 @@ class Sequences:
         self.live[self._next] = seq
         return self._next
 
+    def _release(self, seq: Sequence) -> None:
+        self.free += reversed(seq.pages)
+        seq.pages = []
+
     def remove(self, i: int) -> None:
-        self.free += reversed(self.live.pop(i).pages)
+        self._release(self.live.pop(i))
+
+    def running(self) -> list[int]:
+        """The sequences that will still get tokens: those whose next position has a place."""
+        return [i for i, seq in self.live.items() if seq.cached < self.most]
 
     def _grow(self, seq: Sequence, positions: int) -> bool:
         """Pages for this many positions, or no change and False."""
@@ -99,17 +110,21 @@ class Sequences:
                 out.outputs.append((len(out.tokens) - 1, i))
             return True
 
-        for i, seq in self.live.items():
+        running = [(i, self.live[i]) for i in self.running()]
+        for i, seq in running:
             if seq.pending() == 1:
                 take(i, 1)
-        for i, seq in self.live.items():
+        for i, seq in running:
             if seq.pending() > 1 and take(i, min(seq.pending(), self.chunk)):
                 break
         return out
 
     def commit(self, step: Step, tokens: list[int]) -> dict[int, int]:
         for i, n in zip(step.ids, step.counts):
-            self.live[i].cached += n
+            seq = self.live[i]
+            seq.cached += n
+            if seq.cached == self.most:  # at its end
+                self._release(seq)
         done = {}
         for (_, i), t in zip(step.outputs, tokens):
             self.live[i].generated.append(t)
@@ -155,6 +170,10 @@ class PagedServer:
 
     def remove(self, i: int) -> None:
         self.seqs.remove(i)
+
+    def running(self) -> list[int]:
+        """The sequences that will still get tokens."""
+        return self.seqs.running()
 
     def step(self) -> dict[int, int]:
         """Runs one step; the next token of every sequence that got one."""

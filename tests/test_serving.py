@@ -78,3 +78,24 @@ def test_a_prompt_longer_than_the_pool_is_refused():
     assert not s.live
     a = s.add(Sequence(list(range(16))))
     assert run(s, 1) == [([(a, 16)], [a])]
+
+
+@pytest.mark.parametrize("max_pages,n_pages", [(3, 3), (2, 9), (8, 2)])
+def test_sequences_at_their_end_are_reported_and_give_their_pages_back(max_pages, n_pages):
+    s = Sequences(n_pages=n_pages, page_size=8, max_seqs=4, max_pages=max_pages, chunk=16)
+    most = 8 * min(max_pages, n_pages)
+    a = s.add(Sequence([1, 2, 3]))
+    assert s.running() == [a]
+    steps = 0
+    while s.running():
+        run(s, 1)
+        steps += 1
+        assert steps <= most
+    # its last token comes from its last position
+    assert s.live[a].cached == most and len(s.live[a].generated) == most - 2
+    assert sorted(s.free) == list(range(n_pages)) and s.step().ids == []
+    b = s.add(Sequence(list(range(9))))  # room again, beside the one that has ended
+    assert s.running() == [b] and run(s, 2) == [([(b, 9)], [b]), ([(b, 1)], [b])]
+    s.remove(a)
+    s.remove(b)
+    assert sorted(s.free) == list(range(n_pages)) and s.running() == []
