@@ -14,7 +14,8 @@ model: the projections of the batched ABI, and per layer ``paged_rope_append`` a
     server.remove(a)
 
 A sequence runs until its page table (or the whole pool) is full; it then keeps its tokens, gives its pages back and
-gets no more tokens. A step in which only prompts are taken in returns no tokens.
+gets no more tokens. A step in which only prompts are taken in returns no tokens. When no sequence finds a page for its next
+token, the youngest give theirs back, and are taken in again later, prompt and tokens.
 """
 from __future__ import annotations
 
@@ -96,7 +97,23 @@ class Sequences:
         return True
 
     def step(self) -> Step:
-        """The next batch. A sequence that finds no page sits the step out."""
+        """The next batch, not empty while a sequence is running. A sequence that finds no page sits the step out; if all
+        would, the youngest lose theirs. The oldest alone always finds some, so that it comes to its end."""
+        while True:
+            out = self._choose()
+            if out.ids or not self._preempt():
+                return out
+
+    def _preempt(self) -> bool:
+        """Takes the pages of the youngest running sequence that has any, the oldest aside."""
+        for i in reversed(self.running()[1:]):
+            if self.live[i].pages:
+                self._release(self.live[i])
+                self.live[i].cached = 0
+                return True
+        return False
+
+    def _choose(self) -> Step:
         out = Step([], [], [], [])
 
         def take(i, n):

@@ -99,3 +99,52 @@ def test_sequences_at_their_end_are_reported_and_give_their_pages_back(max_pages
     s.remove(a)
     s.remove(b)
     assert sorted(s.free) == list(range(n_pages)) and s.running() == []
+
+
+def test_two_half_loaded_prompts_do_not_block_each_other():
+    s = Sequences(n_pages=4, page_size=8, max_seqs=4, max_pages=4, chunk=8)
+    a = s.add(Sequence(list(range(24))))
+    b = s.add(Sequence(list(range(24))))
+    s.live[b].pages, s.live[b].cached = [s.free.pop(), s.free.pop()], 16  # both have two of the four pages
+    s.live[a].pages, s.live[a].cached = [s.free.pop(), s.free.pop()], 16
+    assert run(s, 2) == [([(a, 8)], [a]), ([(a, 1)], [a])]
+    assert s.live[b].cached == 0 and s.live[b].pages == []
+
+
+# what a sequence says depends on its own tokens alone, however often it loses its pages on the way
+@pytest.mark.parametrize("seed", range(12))
+def test_a_small_pool_stops_nobody(seed):
+    import random
+    rng = random.Random(seed)
+    page, pool, chunk = 4, rng.randint(5, 12), rng.choice([1, 3, 8, 16])
+    prompts = [[rng.randrange(97) for _ in range(rng.randint(1, 4 * pool // 2))] for _ in range(5)]
+
+    def next_token(tokens):
+        return (31 * sum(tokens) + 7 * tokens[-1] + len(tokens)) % 97
+
+    s = Sequences(n_pages=pool, page_size=page, max_seqs=5, max_pages=pool, chunk=chunk)
+    ids = [s.add(Sequence(list(p))) for p in prompts]
+    lost = 0
+    for _ in range(20000):
+        if not s.running():
+            break
+        before = {i: s.live[i].cached for i in ids}
+        st = s.step()
+        lost += sum(s.live[i].cached < before[i] for i in ids)
+        assert st.ids and len(set(st.ids)) == len(st.ids), "a step without work"
+        held = [q for i in ids for q in s.live[i].pages]
+        assert sorted(held + s.free) == list(range(pool))
+        at = 0
+        for i, n in zip(st.ids, st.counts):  # a step's tokens follow on what is in the cache
+            seq = s.live[i]
+            whole = seq.prompt + seq.generated
+            assert st.tokens[at:at + n] == whole[seq.cached:seq.cached + n]
+            assert len(seq.pages) * page >= seq.cached + n
+            at += n
+        s.commit(st, [next_token(s.live[i].prompt + s.live[i].generated) for _, i in st.outputs])
+    assert not s.running() and lost > 0
+    for i, p in zip(ids, prompts):
+        want = list(p)
+        while len(want) <= pool * page:
+            want.append(next_token(want))
+        assert s.live[i].prompt + s.live[i].generated == want

@@ -115,3 +115,29 @@ def test_sampling_rules_reach_the_tokens():
     for i in (a, b, c):
         server.remove(i)
     assert sorted(server.seqs.free) == list(range(32)) and server.step() == {}
+
+
+def test_sequences_that_lost_their_pages_go_on_as_before():
+    shape = SHAPES["tiny"]
+    w = DeviceWeights.random(shape, seed=4)
+    server = PagedServer(w, n_pages=9, page_size=16, max_seqs=4, max_positions=100, chunk=40)
+    rng = np.random.default_rng(2)
+    prompts = {server.add(p): p for p in (rng.integers(0, shape.vocab_size, n).tolist() for n in (40, 30, 50))}
+    said, lost, steps = {i: [] for i in prompts}, 0, 0
+    while server.running():
+        before = {i: server.seqs.live[i].cached for i in prompts}
+        for i, token in server.step().items():
+            said[i].append(token)
+        lost += sum(server.seqs.live[i].cached < before[i] for i in prompts)
+        steps += 1
+        assert steps < 1000
+    assert q3.device_error() == 0 and lost > 0
+    for i, prompt in prompts.items():
+        most = 112  # seven pages hold the 100 positions
+        assert len(prompt) + len(said[i]) == most + 1
+        ref = plain_logits(w, prompt + said[i])[len(prompt) - 1:-1]
+        top = ref.topk(2)
+        clear = top.values[:, 0] - top.values[:, 1] > 2.0 ** -4
+        assert clear.any()
+        token = torch.tensor(said[i], device="cuda")
+        assert torch.equal(token[clear], top.indices[clear, 0])
