@@ -181,9 +181,10 @@ class PagedServer:
 
     def add(self, prompt, **sampling) -> int:
         """Takes a prompt in; sampling holds repetition, frequency, presence, bias and mask."""
+        prompt = [int(t) for t in prompt]
         if any(t < 0 or t >= self.shape.vocab_size for t in prompt):
             raise ValueError("a token id outside the vocabulary")
-        return self.seqs.add(Sequence([int(t) for t in prompt], **sampling))
+        return self.seqs.add(Sequence(prompt, **sampling))
 
     def remove(self, i: int) -> None:
         self.seqs.remove(i)

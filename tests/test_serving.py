@@ -7,7 +7,8 @@ import pytest
 HERE = Path(__file__).resolve().parent
 sys.path.insert(0, str(HERE))
 import conftest  # noqa: E402,F401
-from llm_inference_b200.serving import Sequence, Sequences  # noqa: E402
+from llm_inference_b200.checkpoint import PRESETS  # noqa: E402
+from llm_inference_b200.serving import PagedServer, Sequence, Sequences  # noqa: E402
 
 
 def run(s, n, token=7):
@@ -148,3 +149,20 @@ def test_a_small_pool_stops_nobody(seed):
         while len(want) <= pool * page:
             want.append(next_token(want))
         assert s.live[i].prompt + s.live[i].generated == want
+
+
+def server():
+    """A server without its device side."""
+    s = PagedServer.__new__(PagedServer)
+    s.shape, s.seqs = PRESETS["tiny"], Sequences(n_pages=8, page_size=8, max_seqs=4, max_pages=8, chunk=16)
+    return s
+
+
+def test_a_prompt_may_be_an_iterator():
+    s = server()
+    a = s.add(t for t in (5, 6, 7))
+    assert s.seqs.live[a].prompt == [5, 6, 7]
+    for prompt in ([1, -1], [s.shape.vocab_size], iter([2, s.shape.vocab_size])):
+        with pytest.raises(ValueError, match="vocabulary"):
+            s.add(prompt)
+    assert list(s.seqs.live) == [a]
