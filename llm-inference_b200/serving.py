@@ -184,6 +184,12 @@ class PagedServer:
         prompt = [int(t) for t in prompt]
         if any(t < 0 or t >= self.shape.vocab_size for t in prompt):
             raise ValueError("a token id outside the vocabulary")
+        mask, words = sampling.get("mask"), (self.shape.vocab_size + 31) // 32
+        if mask is not None:
+            mask = np.asarray(mask)
+            if mask.ndim != 1 or len(mask) < words or mask.dtype.kind not in "iu":
+                raise ValueError(f"the mask must be {words} words of 32 bits")
+            sampling["mask"] = mask[:words].astype(np.uint32).view(np.int32)
         return self.seqs.add(Sequence(prompt, **sampling))
 
     def remove(self, i: int) -> None:

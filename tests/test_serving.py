@@ -2,6 +2,7 @@
 import sys
 from pathlib import Path
 
+import numpy as np
 import pytest
 
 HERE = Path(__file__).resolve().parent
@@ -166,3 +167,17 @@ def test_a_prompt_may_be_an_iterator():
         with pytest.raises(ValueError, match="vocabulary"):
             s.add(prompt)
     assert list(s.seqs.live) == [a]
+
+
+def test_masks_are_checked_when_a_sequence_is_added():
+    s = server()
+    words = (s.shape.vocab_size + 31) // 32
+    bits = np.arange(words, dtype=np.uint32) * np.uint32(0x90000001)
+    for mask in (bits, bits.view(np.int32), bits.astype(np.int64), np.append(bits, bits[:3]), bits.tolist()):
+        m = s.seqs.live[s.add([1], mask=mask)].mask
+        assert m.dtype == np.int32 and np.array_equal(m.view(np.uint32), bits)
+        s.seqs.live.clear()
+    for mask in (bits[:-1], bits[None], bits.astype(np.float32), []):
+        with pytest.raises(ValueError, match="mask"):
+            s.add([1], mask=mask)
+    assert not s.seqs.live
