@@ -362,7 +362,8 @@ int q3_engine_info(const q3_engine *e, q3_engine_buffers *out);
  * Padding and bad descriptions:
  *   - tokens at negative positions (q_len > kv_len) are padding: nothing is stored for them and
  *     their q_out and attention rows are zero;
- *   - rows of the batch outside [q_start[0], q_start[n_seqs]) are neither read nor written;
+ *   - for rows of the batch outside [q_start[0], q_start[n_seqs]) nothing is written, and what q, k and v hold
+ *     there does not matter (q may be read);
  *   - a step may have no tokens or no sequences, logits no rows: such a call does nothing, and arrays of no
  *     elements may be null;
  *   - q_start not rising within [0, n_tokens], q_len above max_q_len, kv_len outside

@@ -1,5 +1,5 @@
-// Paged serving: the step plan, the append of new tokens with rotary positions, and attention over
-// the pages (include/qwen3_b200.h, "Paged serving").
+// Paged serving (include/qwen3_b200.h): the step plan, the append of new tokens with rotary positions, the rotary
+// frequencies, and the C entries of these and of the attention over the pages, whose kernels are in paged_attn.cu.
 #include <math.h>
 
 #include <algorithm>
@@ -31,7 +31,8 @@ struct PlanArgs {
 };
 
 // Costs, in units of a kind's own: a step of a small item is one, the 16 KB load that it waits for; a 128-position step of
-// one or two tensor-core tiles BIG_ONE or BIG_TWO; an item's start and end (queries, merge, output) ITEM or BIG_ITEM.
+// one or two tensor-core tiles COST_BIG_ONE or COST_BIG_TWO; an item's start and end (queries, merge, output) COST_ITEM or
+// COST_BIG_ITEM.
 // Items are cut only while each CTA still gets MIN_SHARE or BIG_MIN_SHARE. A unit of the big kind takes BIG_WEIGHT / 2 of the small one's
 // time where the two share the SMs: with 31 decodes and a chunk of 333 tokens, 1 to 4 and 5.5 gave 178, 107, 89, 88, 96 us
 // (105 one after the other), with 32 decodes at 4096 and a chunk of 2048 at 8192 425, 370, 334, 400, 480 (376).
@@ -106,7 +107,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     pdl_trigger();
     pdl_wait();
     const int n = a.s.n_seqs, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    PagedSeq *seqs = reinterpret_cast<PagedSeq *>(a.plan + a.l.seqs);
     int *table = reinterpret_cast<int *>(a.plan + a.l.table);
     int4 *toks = reinterpret_cast<int4 *>(a.plan + a.l.toks);
 
@@ -136,12 +136,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
         if (lane == 0) {
             if (bad) atomicOr(&g_dev_error, DEV_ERR_POS_RANGE);
             kv_s[b] = bad ? 0 : kv;
-            seqs[b] = {bad_starts ? 0 : q0, bad_starts ? 0 : q_len, bad ? 0 : kv, 0};
         }
     }
     __syncthreads();
     auto seq = [&](int b) -> PagedSeq {
-        return bad_starts ? PagedSeq{0, 0, 0, 0} : PagedSeq{start_s[b], start_s[b + 1] - start_s[b], kv_s[b], 0};
+        return bad_starts ? PagedSeq{0, 0, 0} : PagedSeq{start_s[b], start_s[b + 1] - start_s[b], kv_s[b]};
     };
     for (int t = tid; t < a.s.n_tokens; t += PLAN_THREADS) {
         int4 tok = make_int4(-1, bad_starts ? PAGED_PADDING : PAGED_OUTSIDE, -1, -1);
@@ -271,7 +270,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
                 p.kv1 = t1 == steps ? end : t1 << shift;
                 p.kv_end = end;
                 p.pos0 = q.kv_len - q.q_len + i * s.span;
-                p.big = big;
                 p.part = -1;
                 p.first = c;
                 p.n_parts = 1;

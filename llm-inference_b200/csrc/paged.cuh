@@ -15,7 +15,7 @@ constexpr int PAGED_MAX_HEAD_DIM = 128;
 constexpr int PAGED_OUTSIDE = 0, PAGED_PADDING = -1;
 
 struct PagedSeq {
-    int q0, q_len, kv_len, pad;
+    int q0, q_len, kv_len;
 };
 
 // Attention work. An item is what one CTA could do alone: the query rows of a (sequence, kv head) that
@@ -30,7 +30,6 @@ struct alignas(16) PagedPiece {
     int seq, kvh, tok0, n_tok;   // query rows: tokens tok0 .. tok0 + n_tok of the batch
     int kv0, kv1, kv_end, pos0;  // this piece's positions, the item's end, the first token's position (< 0: padding)
     int part, first, n_parts;    // scratch slot (-1: the item is whole), the item's first CTA, its pieces
-    int big;
 };
 
 // Where a piece of CTA c leaves its partial result: an item's first piece is its CTA's last (slot 2c + 1), the
@@ -54,7 +53,6 @@ inline bool paged_has_big(const q3_paged_shape &s) {
 
 // Byte offsets of the plan's parts; the same arithmetic on host and device.
 struct PagedPlanLayout {
-    size_t seqs;      // PagedSeq [n_seqs]
     size_t table;     // int [n_seqs][max_pages]: checked page ids, -1 past a sequence's last page
     size_t toks;      // int4 [n_tokens]: sequence, place, page, slot
     size_t ctas;      // int2 [2][PAGED_MAX_CTAS], small items' CTAs and big ones': first piece, pieces (-1: zero every row)
@@ -75,7 +73,6 @@ inline PagedPlanLayout paged_plan_layout(const q3_paged_shape &s) {
     };
     const int rep = s.n_heads / s.n_kv_heads, span = paged_has_big(s) ? 2 * (BIG_TILE / rep) : paged_small_rows(s) / rep;
     const size_t items = (size_t)s.n_kv_heads * ((size_t)s.n_seqs + (size_t)s.n_tokens / span);
-    l.seqs = take((size_t)s.n_seqs * sizeof(PagedSeq));
     l.table = take((size_t)s.n_seqs * s.max_pages * 4);
     l.toks = take((size_t)s.n_tokens * 16);
     l.ctas = take(2 * PAGED_MAX_CTAS * sizeof(int2));
