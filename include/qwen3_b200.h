@@ -67,10 +67,11 @@ int q3_selftest_wait_timeout(int *done, void *stream);
 
 /* The same in the middle of a ring of two shared-memory stages between a warp that loads and one that
  * reads: the reader's wait for the third of 64 steps gives up; the loading warp must then stop, and what it
- * had loaded must have arrived before the kernel ends. src: 256 device ints, 16-byte aligned; step u loads
- * src[4u .. 4u+3]. out (4 device ints): 2 if the loading warp stopped, the loads it had issued, and
- * each stage's last word. */
-int q3_selftest_ring_timeout(int *out, const int *src, void *stream);
+ * had loaded must have arrived before the kernel ends. With `starve` the reader keeps its stage, and the
+ * loading warp's own wait gives up; else it sees that the reader has. src: 256 device ints, 16-byte
+ * aligned; step u loads src[4u .. 4u+3]. out (4 device ints): 2 if the loading warp stopped, the loads it
+ * had issued, and each stage's last word. */
+int q3_selftest_ring_timeout(int *out, const int *src, int starve, void *stream);
 
 /* ---------------------------------------------------------------------------------------
  * Drop-in launchers (batch 1). Each replaces the launcher of the same name without the

@@ -65,7 +65,6 @@ struct PaArgs {
     int small_step_pages, small_step_slots, big_step_pages, big_step_slots;  // a producer's step in pages and slots
     float scale_log2;
     uint32_t idesc_qk, idesc_pv;
-    bool after_big;  // few rows: launched behind the kernel for many rows, whose results are needed at the end only
 };
 
 // ---------------------------------------------------------------- helpers
@@ -253,13 +252,13 @@ __device__ void small_produce(const PaArgs &a, const CUtensorMap *mk, const CUte
         at += NP * UPOS;
         const int next_page = active && at < p.kv1 ? __ldg(tab + w.idx) : 0;
         wait(&empty[mine.s], mine.ph ^ 1);
-        if (wait.stopped()) break;
-        if (lane == 0) {
+        __syncwarp();
+        if (lane == 0 && !wait.dead) {
             const int n = min(UPOS, max(0, p.kv1 - p0) + box - 1) & -box;
             mbar_arrive_expect_tx(&full[mine.s], (uint32_t)(n * 128 * NB * 2));
         }
         __syncwarp();
-        if (on) tma_page(ring + (size_t)mine.s * SMALL_STAGE + off, map, half * 64, slot, p.kvh, page, &full[mine.s]);
+        if (on && !wait.dead) tma_page(ring + (size_t)mine.s * SMALL_STAGE + off, map, half * 64, slot, p.kvh, page, &full[mine.s]);
         mine.next(NP);
         p0 += NP * UPOS;
         page = next_page;
@@ -451,7 +450,7 @@ __device__ void small_consume(const PaArgs &a, const PagedPiece &p, unsigned cha
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[r.s]);
+            if (lane == 0 && !wait.dead) mbar_arrive(&empty[r.s]);  // a load that never came may still be owed to this stage
         }
         r.next();
         p0 += UPOS;
@@ -652,7 +651,8 @@ struct SmallSmem {
     int flag, go, down;
 };
 
-template <int DP, int NQ>
+// AFTER_BIG: launched behind the kernel for many rows, whose results are needed at the end only.
+template <int DP, int NQ, bool AFTER_BIG>
 __global__ void __launch_bounds__((SMALL_PRODUCERS + SMALL_WARPS) * 32, 1)
     paged_small_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                        const __grid_constant__ PaArgs a) {
@@ -671,19 +671,19 @@ __global__ void __launch_bounds__((SMALL_PRODUCERS + SMALL_WARPS) * 32, 1)
     }
     // The kernel before is the plan or whatever wrote q, K and V; or it is the kernel for many rows, whose CTA says when
     // it has waited for those.
-    if (a.after_big && threadIdx.x == 32) sm.go = take_ready(a.ready + blockIdx.x);
+    if (AFTER_BIG && threadIdx.x == 32) sm.go = take_ready(a.ready + blockIdx.x);
     __syncthreads();
     pdl_trigger();
     int2 work = make_int2(0, 0);
-    if (!a.after_big) pdl_wait();
+    if (!AFTER_BIG) pdl_wait();
     else fence_proxy_async_global();
-    if (!a.after_big || sm.go) work = a.ctas[blockIdx.x];
+    if (!AFTER_BIG || sm.go) work = a.ctas[blockIdx.x];
     if (work.y < 0) zero_rows(a);
     Ring<SMALL_WARPS> r;
     Waiter wait(&g_dev_error, &sm.down);
     for (int i = 0; i < work.y; i++) {
         const PagedPiece p = a.pieces[work.x + i];
-        // every load is waited for by a consumer before the CTA ends, or by settle
+        // every load is waited for by a consumer before the CTA ends; one that has given up gets no more
         if (warp >= SMALL_WARPS)
             small_produce<DP, SMALL_WARPS, SMALL_PRODUCERS>(a, &mk, &mv, p, sm.ring, sm.full, sm.empty, r, warp - SMALL_WARPS, wait,
                                                              a.small_step_pages, a.small_step_slots);
@@ -691,12 +691,11 @@ __global__ void __launch_bounds__((SMALL_PRODUCERS + SMALL_WARPS) * 32, 1)
             small_consume<DP, NQ, SMALL_WARPS, SMALL_WARPS>(a, p, sm.ring, sm.full, sm.empty, r, wait, warp, sm.q, sm.lim, sm.merge_o, sm.merge_ml,
                                                          &sm.flag);
     }
-    settle(wait);
-    if constexpr (NQ == 1)
-        if (a.after_big) {  // whoever waits for this kernel waits for that one, too
-            pdl_wait();
-            combine_big<DP>(a);
-        }
+    if (wait.dead) settle();
+    if constexpr (AFTER_BIG) {  // whoever waits for this kernel waits for that one, too
+        pdl_wait();
+        combine_big<DP>(a);
+    }
 }
 
 // ---------------------------------------------------------------- many rows
@@ -1208,7 +1207,7 @@ __global__ void __launch_bounds__(BIG_THREADS, 1)
             big_softmax<DP>(a, p, sm, tmem, group / 2, group % 2, r, s_ph, wait);
         }
     }
-    settle(wait);
+    if (__syncthreads_or(wait.dead)) settle();
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
@@ -1243,12 +1242,12 @@ bool make_query_map(CUtensorMap *map, const PagedAttnCall &c, const PaArgs &a) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DP, int NQ>
+template <int DP, int NQ, bool AFTER_BIG = false>
 cudaError_t launch_small(const CUtensorMap &mk, const CUtensorMap &mv, const PaArgs &a, cudaStream_t s) {
     const size_t smem = sizeof(SmallSmem<DP, NQ>) + 1024;
-    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(paged_small_kernel<DP, NQ>), smem);
+    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(paged_small_kernel<DP, NQ, AFTER_BIG>), smem);
     if (e != cudaSuccess) return e;
-    return launch(paged_small_kernel<DP, NQ>, dim3(paged_ctas()), dim3((SMALL_PRODUCERS + SMALL_WARPS) * 32), smem, s, 1, mk, mv, a);
+    return launch(paged_small_kernel<DP, NQ, AFTER_BIG>, dim3(paged_ctas()), dim3((SMALL_PRODUCERS + SMALL_WARPS) * 32), smem, s, 1, mk, mv, a);
 }
 
 template <int DP>
@@ -1262,8 +1261,7 @@ int run(const PagedAttnCall &c, PaArgs &a, cudaStream_t s) {
     a.big_step_slots = BIG_TILE % a.page_size;
     if (!make_page_map(&mk, c.cache.key_pages, c, a.small_box) || !make_page_map(&mv, c.cache.value_pages, c, a.small_box))
         return Q3_ERR_SHAPE;
-    a.after_big = paged_has_big(c.shape);
-    if (a.after_big) {
+    if (paged_has_big(c.shape)) {
         CUtensorMap mq, mk_big, mv_big;
         if (!make_page_map(&mk_big, c.cache.key_pages, c, a.big_box) || !make_page_map(&mv_big, c.cache.value_pages, c, a.big_box) ||
             !make_query_map(&mq, c, a))
@@ -1275,6 +1273,8 @@ int run(const PagedAttnCall &c, PaArgs &a, cudaStream_t s) {
         const size_t big_smem = sizeof(BigSmem<DP>);
         Q3_TRY_LAUNCH(allow_smem(reinterpret_cast<const void *>(paged_big_kernel<DP>), big_smem));
         Q3_TRY_LAUNCH(launch(paged_big_kernel<DP>, dim3(paged_ctas()), dim3(BIG_THREADS), big_smem, s, 1, mq, mk_big, mv_big, a));
+        Q3_TRY_LAUNCH((launch_small<DP, 1, true>(mk, mv, a, s)));  // eight rows (paged_small_rows)
+        return Q3_OK;
     }
     const int tiles = paged_small_rows(c.shape) / 8;
     if (tiles == 1) Q3_TRY_LAUNCH((launch_small<DP, 1>(mk, mv, a, s)));

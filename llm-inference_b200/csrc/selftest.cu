@@ -6,7 +6,8 @@
 // the wait ends at WAIT_LIMIT_NS.
 //
 // The second kernel does the same in the middle of a ring between a warp that loads and one that reads (waiter.cuh): once
-// the reader has given up, the loading warp must stop, and all that it had loaded must have arrived before the end.
+// the reader has given up, the loading warp must stop, and all that it had loaded must have arrived before the end: in
+// either of the ways that are in use.
 #include "waiter.cuh"
 
 namespace q3 {
@@ -26,7 +27,7 @@ __global__ void wait_timeout_kernel(int *done) {
 
 constexpr int RING_STAGES = 2, RING_STEPS = 64, RING_STUCK = 2;
 
-__global__ void ring_timeout_kernel(int *out, const int *src) {
+__global__ void ring_timeout_kernel(int *out, const int *src, bool starve) {
     __shared__ __align__(16) int ring[RING_STAGES][4];
     __shared__ __align__(8) uint64_t full[RING_STAGES], empty[RING_STAGES];
     __shared__ int down;
@@ -54,7 +55,7 @@ __global__ void ring_timeout_kernel(int *out, const int *src) {
                 }
             }
             wait(&empty[s], ph ^ 1);
-            if (wait.stopped()) break;
+            if (starve ? __any_sync(0xffffffffu, wait.dead) : wait.stopped()) break;
             if (lane == 0) {
                 // one step expects 16 bytes more than come: its phase never completes
                 mbar_arrive_expect_tx(&full[s], u == RING_STUCK ? 32 : 16);
@@ -64,10 +65,10 @@ __global__ void ring_timeout_kernel(int *out, const int *src) {
         } else {
             wait(&full[s], ph);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[s]);
+            if (lane == 0 && !(starve && wait.dead)) mbar_arrive(&empty[s]);
         }
     }
-    settle(wait);
+    if (__syncthreads_or(wait.dead)) settle();
     if (threadIdx.x == 32) {
         out[0] = wait.dead ? 2 : 1;
         out[1] = loaded;
@@ -96,11 +97,11 @@ extern "C" int q3_selftest_wait_timeout(int *done, void *stream) {
 }
 
 // The same for a ring of two stages between a loading and a reading warp, 64 steps of 16 bytes of `src` (256 ints of device
-// memory). The reader gives up at the third; out (four ints): 2 if the loading warp saw that, the loads that it issued,
+// memory). The reader gives up at the third; out (four ints): 2 if the loading warp stopped, the loads that it issued,
 // and the last word of either stage.
-extern "C" int q3_selftest_ring_timeout(int *out, const int *src, void *stream) {
+extern "C" int q3_selftest_ring_timeout(int *out, const int *src, int starve, void *stream) {
     if (!out || !src) return Q3_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(src) % 16 != 0) return Q3_ERR_ALIGN;
-    q3::ring_timeout_kernel<<<1, 64, 0, reinterpret_cast<cudaStream_t>(stream)>>>(out, src);
+    q3::ring_timeout_kernel<<<1, 64, 0, reinterpret_cast<cudaStream_t>(stream)>>>(out, src, starve != 0);
     return q3::record_cuda_error(cudaGetLastError());
 }

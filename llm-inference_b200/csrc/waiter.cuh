@@ -1,8 +1,10 @@
 // Bounded waits of kernels whose warps hand ring stages to one another.
 //
-// A wait that gives up must not leave anything behind: the roles go on without waiting, so that every barrier of the
-// CTA still sees its arrivals; what loads stops loading, because a stage may still be owed to a load before; and
-// the CTA ends only when all copies and products that it has started have ended, too.
+// A wait that gives up must not leave anything behind. The roles go on without waiting, so that the CTA comes to its end.
+// Loading stops, because a load that never came may still be owed to a stage: either who has given up releases no more
+// stages, so that the loading warps starve and give up in turn (that costs their loop nothing), or, where the tensor
+// core releases them, the loading warps look at a shared word. And the CTA ends only when the copies and products that it
+// has started have ended, too.
 #pragma once
 
 #include "common.cuh"
@@ -54,9 +56,8 @@ struct Waiter {
     }
 };
 
-// The end of the CTA's work, all threads. After a wait that gave up: what was issued until then ends well within this time.
-__device__ __forceinline__ void settle(const Waiter &wait) {
-    if (!__syncthreads_or(wait.dead)) return;
+// After a wait that gave up, at the end: what was issued until then ends well within this time.
+static __device__ __noinline__ void settle() {
     const uint64_t t = globaltimer();
     while (globaltimer() - t < 1000000) {
     }

@@ -96,12 +96,13 @@ def test_rank_exit_ends_peer_collective_with_error():
 
 
 @pytest.mark.gpu
-def test_a_ring_stops_loading_after_a_wait_gave_up():
+@pytest.mark.parametrize("starve", [0, 1])
+def test_a_ring_stops_loading_after_a_wait_gave_up(starve):
     import llm_inference_b200 as q3
     from llm_inference_b200 import _lib
     src = torch.arange(256, dtype=torch.int32, device="cuda")
     out = torch.zeros(4, dtype=torch.int32, device="cuda")
-    _lib.call("q3_selftest_ring_timeout", out.data_ptr(), src.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    _lib.call("q3_selftest_ring_timeout", out.data_ptr(), src.data_ptr(), starve, torch.cuda.current_stream().cuda_stream)
     assert q3.device_error() == 1, "expected the wait-timeout bit alone"
     # steps 0 to 3 were loaded before the reader gave up at step 2; both stages hold their latest ones
     assert out.tolist() == [2, 4, 4 * 2 + 3, 4 * 3 + 3]
@@ -112,6 +113,6 @@ def test_ring_selftest_refuses():
     from llm_inference_b200 import _lib, build
     build.build()
     lib = _lib.load()
-    assert lib.q3_selftest_ring_timeout(None, 4096, None) == 5
-    assert lib.q3_selftest_ring_timeout(4096, None, None) == 5
-    assert lib.q3_selftest_ring_timeout(4096, 4100, None) == 2
+    assert lib.q3_selftest_ring_timeout(None, 4096, 0, None) == 5
+    assert lib.q3_selftest_ring_timeout(4096, None, 0, None) == 5
+    assert lib.q3_selftest_ring_timeout(4096, 4100, 0, None) == 2
