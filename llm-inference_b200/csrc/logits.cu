@@ -8,7 +8,7 @@
 // Bound by latency: one row by the chain lengths -> ids -> logits, a batch by that chain once for each of the two or
 // three CTAs that an SM runs after one another. Each slice reads the row's whole history, from L2 after the
 // first, so slices are as large as still leaves two per SM. 32 rows of 151936 bf16 with masks and 2000 ids of history
-// each take 13.4 us in a graph (10.5 without the histories: 1.9 TB/s), 100 rows of 32003 floats with 8000 ids 18.3 (10.5).
+// each take 13.5 us in a graph (9.0 without the histories: 2.2 TB/s), 100 rows of 32003 floats with 8000 ids 18.5 (8.4).
 // Clusters of 8 slices that share the scan and count in one another's shared memory took 22 and 49 us; they
 // gain only for a single row of 16000 ids (13.2 -> 6.9).
 #include <math.h>

@@ -18,7 +18,7 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 // ------------------------------------------------------------------ plan
 // One CTA. The description is checked here once, so that the kernels of every layer can use the
 // plan's copy of the page table and the token map without checks of their own. Latency bounds it: 10 us for one sequence,
-// 16 for 32 of 64 pages, 27 for four chunks of 2048 tokens, once per step.
+// 17 for 32 of 64 pages, 28 for four chunks of 2048 tokens, 83 for 256 sequences with tables of 2560 pages, once per step.
 constexpr int PLAN_THREADS = 1024;
 
 struct PlanArgs {
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
 // asked for before that.
 //
 // With many tokens the instructions bound it about as much as the bytes: 8192 tokens of 48 heads of 128 take 37.5 us
-// (5.4 TB/s, 0.83 of the measured copy bandwidth), interleaved 38.7 (61 with angles in the pairs' order, whose reads
+// (5.4 TB/s, 0.83 of the measured copy bandwidth), interleaved 39 to 40 (61 with angles in the pairs' order, whose reads
 // met in a few banks); without packed arithmetic and a loop per kind of head it was 43. With few, the chain plan ->
 // angle -> heads: 2.4 us for one token.
 //
@@ -484,7 +484,8 @@ __global__ void __launch_bounds__(APPEND_MAX_THREADS, 2) paged_append_kernel(con
 }
 
 // Half-split pairs whose distance is not a multiple of 8 elements: one warp per head, the head's
-// fp32 values in the warp's shared memory.
+// fp32 values in the warp's shared memory. Two-byte accesses, and no head's loads ahead of the one before: 8192 tokens
+// of 48 heads of 128, 40 elements rotated, take 107 us where the kernel above takes 39 with 48 of them.
 __global__ void __launch_bounds__(APPEND_ODD_THREADS) paged_append_odd_kernel(const __grid_constant__ AppendArgs a) {
     __shared__ float cos_s[PAGED_MAX_HEAD_DIM / 2], sin_s[PAGED_MAX_HEAD_DIM / 2];
     __shared__ float head_s[APPEND_ODD_THREADS / 32][PAGED_MAX_HEAD_DIM];

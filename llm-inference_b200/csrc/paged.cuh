@@ -39,8 +39,8 @@ __host__ __device__ __forceinline__ int part_slot(int first, int i) { return i =
 // Rows of the kernel for few rows: eight for each 8-column tile of its products. Where every sequence fits into a
 // few tiles (draft tokens being verified) the step needs no other kernel; where some do not, it is the one for single
 // tokens, and all longer sequences go to the kernel for many rows. 32 sequences at 4096, 8 kv heads of 128: 16 rows take
-// 90 us here and 120 there, 24 rows 152 and 120 (their accumulators spill); 4 kv heads of 64: 16 rows 31 and 59,
-// 24 rows 38 and 60, 40 rows 64 and 59.
+// 92 us here and 128 there (at 1.7 GHz), 24 rows 152 and 128 to 133 (their accumulators spill); 4 kv heads of 64: 16 rows 31
+// and 52, 24 rows 37 and 52, 40 rows 64 and 52.
 inline int paged_small_rows(const q3_paged_shape &s) {
     const long long most = (long long)s.max_q_len * (s.n_heads / s.n_kv_heads);
     if (most > (s.head_dim <= 64 ? 24 : 16) || most <= 8) return 8;

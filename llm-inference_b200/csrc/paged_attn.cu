@@ -13,17 +13,18 @@
 // Few rows (a decode step): bound by the bytes of K and V, with 160 KB of loads in flight on each SM. Warp-level matrix
 // instructions are enough for that; each warp owns whole 16 KB stages (32 positions at head_dim 128) with its own
 // running maximum, so warps meet only at the end of a piece. 32 sequences at 4096, 32 query heads on 8: 85 us,
-// 0.96 of the measured copy bandwidth; one sequence at 256: 5.5 us in a graph.
+// 0.96 of the measured copy bandwidth; one sequence at 256: 5.4 us in a graph.
 //
 // Many rows (a chunk of a prompt): bound by the tensor cores and the chain between their products. 128 rows -- all
 // query heads of a kv head side by side, token after token -- make a tcgen05 tile; two tiles share each K and V
 // tile and alternate, one in its softmax while the other multiplies. S = Q K^T goes to tensor memory, two threads
 // per row read it, write P back over it as bf16, and P is the A operand of O += P V from tensor memory. A step of two
 // tiles takes 3550 cycles: per tile 2000 of softmax and 1400 of products (1024 of them multiplying), of which only the
-// two tiles' overlap hides any. 2048 tokens at 8192, 32 query heads on 8: 310 us, 1.0 PFLOP/s, 0.61 of the measured
-// matrix rate. What did not help: a quarter of the exponentials by polynomial
-// (275 to 296 us against 266 on one set of inputs), half-steps of 64 columns (390 where whole ones took 363), one
-// thread a row (385), a product thread per tile (460).
+// two tiles' overlap hides any. 2048 tokens at 8192, 32 query heads on 8: 310 to 320 us in a row, when the power limit
+// holds the SMs near 1.67 GHz (1.0 PFLOP/s, 0.60 of the measured matrix rate), 270 in the first calls, at 1.97 GHz, with one
+// set of inputs as with three. What did not help this kernel: 12 to 50 % of the exponentials by polynomial (272 to 307 us
+// against 266, all in short runs). What did not help the forms before it: half-steps of 64 columns (388 to 397 us against
+// 391, later 390 against 363), a product thread per tile (460, it spilled).
 //
 // Bad values behind the mask: a masked score is replaced, whatever it is, but a zero probability times a NaN
 // or infinite v would still be NaN. Rows of V past the item's end are zeroed in shared memory; the few
