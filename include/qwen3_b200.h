@@ -476,6 +476,25 @@ int q3_logits_process_bounded(void *out, const void *logits, int dtype, int rows
                               const int *bias_start, const int *bias_ids, const float *bias, long long n_bias,
                               const unsigned *mask, long long mask_stride, void *stream);
 
+/* The next token of `rows` rows of logits (0: bf16, 1: fp32) from given random numbers u[r] in [0, 1). Per row the tokens
+ * are ordered by logit, largest first, equal ones by index, and weigh w = exp((x - largest) / temperature[r]).
+ *   1. top_k[r] > 0: the first top_k of the order are kept
+ *   2. top_p[r] < 1: of those the fewest first ones that have at least top_p of their weight
+ *   3. min_p[r] > 0: of those the ones with w >= min_p (above 1 counts as 1)
+ * The first token always stays. With W the weight that is left, out[r] is the first kept token at which the
+ * running sum of the weights passes u W, and prob[r] (if not null) its w / W. draft[r] names a token that has been
+ * guessed: if it is kept, the running sum begins with it, so that out[r] == draft[r] with exactly the probability the
+ * row gives the draft, and the distribution of out[r] is the same as without one; a chain of drafts holds up to the first
+ * row that says otherwise. A draft outside [0, vocab) is none. Null arrays leave their part out; null temperature is 1.
+ * temperature[r] not above 0 takes the first token. NaN logits and those of -inf are never taken; with an infinite
+ * logit only its equals weigh. A row without any token gets -1 and prob 0. u below 0 or NaN counts as 0, from 1 on as
+ * the largest below 1. Weights are exact to 2^-43 of the largest and their sums independent of order, so a row's result does
+ * not depend on its neighbours. rows at most 2^24; vocab at most 655296 (bf16) or 327648 (fp32). stride: elements
+ * between rows. */
+int q3_sample_logits(int *out, float *prob, const void *logits, int dtype, int rows, int vocab, long long stride,
+                     const float *u, const float *temperature, const int *top_k, const float *top_p, const float *min_p,
+                     const int *draft, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

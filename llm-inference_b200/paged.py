@@ -239,3 +239,24 @@ def logits_process(out, logits, hist_start=None, hist_split=None, hist_ids=None,
         _vector(name, presence, "presence", rows, f32, dev), bias_at, biased, added, n_bias, mask_ptr, mask_stride, _stream(stream))
     if status:
         check(name, status)
+
+
+def sample_logits(out, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, draft=None, prob=None, stream=None):
+    """The next token of each row of [rows, vocab] logits, bf16 or fp32, from random numbers u in [0, 1) (q3_sample_logits):
+    int32 tokens to out and, if given, their fp32 probabilities to prob. temperature, top_p, min_p: fp32, top_k and draft:
+    int32, one entry a row, or None. A row's draft token comes out with the probability that the row gives it."""
+    torch = _t()
+    name, dtype, i32, f32 = "q3_sample_logits", logits.dtype, torch.int32, torch.float32
+    if dtype is not torch.bfloat16 and dtype is not f32:
+        _refuse(name, "logits must be bfloat16 or float32")
+    if logits.dim() != 2:
+        _refuse(name, "logits must be [rows, vocab]", _SHAPE)
+    (rows, vocab), dev = logits.shape, _device()
+    status = load().q3_sample_logits(
+        _vector(name, out, "out", rows, i32, dev), _vector(name, prob, "prob", rows, f32, dev), logits.data_ptr(), dtype is f32, rows,
+        vocab, _rows(name, logits, "logits", rows, vocab, dtype, dev), _vector(name, u, "u", rows, f32, dev),
+        _vector(name, temperature, "temperature", rows, f32, dev), _vector(name, top_k, "top_k", rows, i32, dev),
+        _vector(name, top_p, "top_p", rows, f32, dev), _vector(name, min_p, "min_p", rows, f32, dev),
+        _vector(name, draft, "draft", rows, i32, dev), _stream(stream))
+    if status:
+        check(name, status)
