@@ -294,8 +294,8 @@ def test_refusals():
     refuses(5, out, x, u, None, u)
     refuses(1, out, x, u, draft=out[:1])
     refuses(1, out, x, u, prob=u[:1])
-    refuses(1, out, torch.zeros(2, 700000, device="cuda", dtype=torch.bfloat16), u)
-    refuses(1, out, torch.zeros(2, 350000, device="cuda"), u)
+    refuses(1, out, torch.zeros(2, 1048065, device="cuda", dtype=torch.bfloat16), u)
+    refuses(1, out, torch.zeros(2, 1048065, device="cuda"), u)
     refuses(5, out, x.cpu(), u)
     refuses(5, out, x, u.cpu())
     none = torch.zeros(0, dtype=torch.int32, device="cuda")
@@ -303,7 +303,7 @@ def test_refusals():
 
 
 def test_the_largest_vocabularies():
-    for vocab, dtype in ((655296, torch.bfloat16), (327648, torch.float32)):
+    for vocab, dtype in ((1048064, torch.bfloat16), (1048064, torch.float32)):
         g = np.random.default_rng(vocab)
         x = torch.from_numpy(g.normal(0, 2, (2, vocab)).astype(np.float32)).cuda().to(dtype)
         run(x, f32(0.3, 0.9))
