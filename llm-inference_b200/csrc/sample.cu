@@ -8,7 +8,7 @@
 // A draft token takes the first place of the order for the draw: it comes out with its own probability, the
 // others with theirs.
 //
-// Weights are whole numbers, round(2^bits w), from exponentials in fp64: their sums are the same in any order, so neither the
+// Weights are whole numbers, round(2^41 w), from exponentials in fp64: their sums are the same in any order, so neither the
 // atomics below nor the way the row is cut change a result, and a draw is decided as in 64 bits.
 //
 // A cluster of CTAs shares a row. Two ways to find a crossing:
@@ -19,8 +19,9 @@
 //     histogram of mass and count over the logits, and per crossing one that gathers the tokens of its bin, which are ranked by
 //     comparing each with each. A bin of too many tokens is cut finer by the bits of its logits; as many equal ones are
 //     told apart by counting them in the order of their index.
-// CTAs write what all of a cluster need into each other's shared memory before a cluster barrier (reading it after one, C
-// loads that wait for one another, cost more than all the arithmetic).
+// CTAs write what others need into their shared memory before a cluster barrier (reading it after one, C loads that wait for
+// one another, cost more than all the arithmetic). The counts of values all go to the first CTA, which then needs no more
+// barriers.
 #include <math.h>
 
 #include <algorithm>
@@ -39,9 +40,9 @@ namespace {
 constexpr int SL_THREADS = 512;
 constexpr int SL_WARPS = SL_THREADS / 32;
 constexpr int SL_MAX_CLUSTER = 8;
-constexpr int SL_SLICE = 1 << 17;  // tokens of a CTA at most: 15-bit parts of their weights add up within 32 bits
-constexpr int SL_VOCAB = SL_MAX_CLUSTER * (SL_SLICE - 64);
-constexpr int SL_LOADS = 4;  // 16-byte loads that a thread has in flight
+constexpr int SL_BITS = 41;        // the largest weight is 2^41: those of a whole row add up to less than 2^62
+constexpr int SL_SLICE = 1 << 18;  // tokens of a CTA at most: 14-bit parts of their weights add up within 32 bits
+constexpr int SL_VOCAB = 1 << 20;
 
 typedef unsigned long long u64;
 
@@ -50,24 +51,24 @@ struct SampleArgs {
     float *prob;
     const void *logits;
     long long stride;
-    int vocab, slice, bits;  // slice: tokens of a CTA, a multiple of 8
+    int vocab, slice;  // slice: tokens of a CTA, a multiple of 8
     const float *u, *temperature, *top_p, *min_p;
     const int *top_k, *draft;
 };
 
 // What a CTA tells the others.
 struct Told {
-    u64 mass, above, before_draft;  // of its share of the bins; its mass above min-p's limit and before the draft
-    u64 first;                      // its largest token: key in the upper half, complement of the index below
+    u64 above, before_draft;  // its mass above min-p's limit and before the draft
+    u64 first;                // its largest token: key in the upper half, complement of the index below
     unsigned count, low, high;
 };
 
 // Where a running sum passes a target: the token's weight, what comes before it, and which token it is.
 struct Crossing {
     u64 before, w;
-    int index;  // of the token; of a value: -1
-    int pos, owner;
-    unsigned nth;  // the value's place, the CTA that has the token and which of its tokens of that value it is
+    int index;     // of the token
+    int pos;       // or its value's place, and which token of that value it is
+    unsigned nth;
 };
 
 __device__ __forceinline__ float to_f32(bf16 v) { return __bfloat162float(v); }
@@ -84,8 +85,7 @@ __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k &
 struct Weigher {
     float peak;
     double c;  // log2 e / T
-    int bits;
-    // round(2^bits * 2^((x - peak) c)): the power's whole part goes to the exponent, the rest f in [-1/2, 1/2] through the
+    // round(2^SL_BITS * 2^((x - peak) c)): the power's whole part goes to the exponent, the rest f in [-1/2, 1/2] through the
     // Taylor polynomial of e^(f ln 2) (the first term left out is below 3e-13). No branches, so that a thread's
     // weights overlap: one chain of these operations is 200 cycles.
     __device__ __forceinline__ u64 operator()(float x) const {
@@ -105,9 +105,9 @@ struct Weigher {
         y = fma(y, f, 0.2402265069591007);
         y = fma(y, f, 0.6931471805599453);
         y = fma(y, f, 1.0);
-        y = __hiloint2double(__double2hiint(y) + ((n + bits) << 20), __double2loint(y));
+        y = __hiloint2double(__double2hiint(y) + ((n + SL_BITS) << 20), __double2loint(y));
         const u64 w = (u64)__double_as_longlong(y + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52: the sum's fraction bits
-        return x == peak ? 1ull << bits : t > -46.0 ? w : 0;
+        return x == peak ? 1ull << SL_BITS : t > -44.0 ? w : 0;
     }
 };
 
@@ -122,26 +122,53 @@ __device__ __forceinline__ u64 warp_max(u64 v) {
     return v;
 }
 
-// Exclusive running sum over the CTA's threads; `total` is everyone's sum.
-__device__ __forceinline__ u64 block_scan(u64 v, u64 *scan, u64 *total) {
+struct ScanShared {
+    u64 mass[SL_WARPS];
+    unsigned count[SL_WARPS];
+};
+
+// Exclusive running sums over the CTA's threads in place of m and n; the CTA's sums go to mass and count.
+__device__ void block_scan(ScanShared &s, u64 &m, unsigned &n, u64 &mass, unsigned &count) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    u64 run = v;
+    auto scan = [&](u64 &rm, unsigned &rn) {  // inclusive, over the lanes
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += y;
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 ym = __shfl_up_sync(0xffffffffu, rm, o);
+            const unsigned yn = __shfl_up_sync(0xffffffffu, rn, o);
+            rm += lane >= o ? ym : 0;
+            rn += lane >= o ? yn : 0;
+        }
+    };
+    u64 rm = m;
+    unsigned rn = n;
+    scan(rm, rn);
+    __syncthreads();  // earlier readers of s
+    if (lane == 31) {
+        s.mass[warp] = rm;
+        s.count[warp] = rn;
     }
-    __syncthreads();  // earlier readers of scan
-    if (lane == 31) scan[warp] = run;
     __syncthreads();
-    u64 before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < SL_WARPS; w++) {
-        if (w < warp) before += scan[w];
-        all += scan[w];
-    }
-    *total = all;
-    return before + run - v;
+    u64 wm = lane < SL_WARPS ? s.mass[lane] : 0;
+    unsigned wn = lane < SL_WARPS ? s.count[lane] : 0;
+    scan(wm, wn);
+    mass = __shfl_sync(0xffffffffu, wm, SL_WARPS - 1);
+    count = __shfl_sync(0xffffffffu, wn, SL_WARPS - 1);
+    wm = __shfl_sync(0xffffffffu, wm, max(warp - 1, 0));
+    wn = __shfl_sync(0xffffffffu, wn, max(warp - 1, 0));
+    m = rm - m + (warp ? wm : 0);
+    n = rn - n + (warp ? wn : 0);
+}
+
+// The last of N entries whose running sum (what comes before it) is not above the target, by all lanes of a warp. Entries of
+// no weight begin where the next one does, so the target lies in the entry that is found.
+template <int N>
+__device__ __forceinline__ int search(const u64 *mass, const unsigned *count, u64 target, bool by_count) {
+    constexpr int EACH = N / 32;
+    const int lane = threadIdx.x % 32;
+    auto before = [&](int e) { return by_count ? (u64)count[e] : mass[e]; };
+    int e = EACH * (31 - __clz(__ballot_sync(0xffffffffu, before(lane * EACH) <= target)));
+    e += 31 - __clz(__ballot_sync(0xffffffffu, lane < EACH && before(e + lane % EACH) <= target));
+    return e;
 }
 
 // A row as the CTAs of a cluster see it.
@@ -154,7 +181,15 @@ struct Row {
     int vocab, i0, slice;  // i0: index of the slice's first place, where a 16-byte line begins; it may lie before the row
 
     __device__ __forceinline__ void sync() {
-        if (C > 1) cluster.sync();
+        arrive();
+        wait();
+    }
+    // the two halves of a barrier
+    __device__ __forceinline__ void arrive() {
+        if (C > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    }
+    __device__ __forceinline__ void wait() {
+        if (C > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
         else __syncthreads();
     }
     template <typename V>
@@ -163,29 +198,37 @@ struct Row {
     // A line of the row; places outside it hold -infinity.
     __device__ __forceinline__ uint4 line(int i) const {
         if (i >= 0 && i + PER <= vocab) return __ldg(reinterpret_cast<const uint4 *>(in + i));
-        uint4 raw;
-        T *x = reinterpret_cast<T *>(&raw);
-#pragma unroll
-        for (int e = 0; e < PER; e++) x[e] = i + e >= 0 && i + e < vocab ? in[i + e] : T(-INFINITY);
-        return raw;
+        return edge(in, vocab, i);
     }
-    // f(line, index of its first place) over the slice, several loads in flight
-    template <typename F>
+    static __device__ __noinline__ uint4 edge(const T *in, int vocab, int i) {
+        alignas(16) T x[PER];
+#pragma unroll 1
+        for (int e = 0; e < PER; e++) x[e] = i + e >= 0 && i + e < vocab ? in[i + e] : T(-INFINITY);
+        return *reinterpret_cast<const uint4 *>(x);
+    }
+    // f(line, index of its first place) over the slice, with LOADS loads in flight and f's code only once: most of these
+    // kernels' code runs once or a few times, and waiting for it is what costs
+    template <int LOADS, typename F>
     __device__ __forceinline__ void each_line(F f) const {
-        for (int v = threadIdx.x * PER; v < slice; v += SL_LOADS * SL_THREADS * PER) {
-            uint4 raw[SL_LOADS];
+        constexpr int STEP = SL_THREADS * PER;
+        uint4 next[LOADS];
+        int v = threadIdx.x * PER;
 #pragma unroll
-            for (int l = 0; l < SL_LOADS; l++)
-                if (v + l * SL_THREADS * PER < slice) raw[l] = line(i0 + v + l * SL_THREADS * PER);
+        for (int l = 0; l < LOADS; l++)
+            if (v + l * STEP < slice) next[l] = line(i0 + v + l * STEP);
+#pragma unroll 1
+        for (; v < slice; v += STEP) {
+            const uint4 raw = next[0];
 #pragma unroll
-            for (int l = 0; l < SL_LOADS; l++)
-                if (v + l * SL_THREADS * PER < slice) f(raw[l], i0 + v + l * SL_THREADS * PER);
+            for (int l = 1; l < LOADS; l++) next[l - 1] = next[l];
+            if (v + LOADS * STEP < slice) next[LOADS - 1] = line(i0 + v + LOADS * STEP);
+            f(raw, i0 + v);
         }
     }
     // f(x, index); NaN comes as -infinity
-    template <typename F>
+    template <int LOADS, typename F>
     __device__ __forceinline__ void each(F f) const {
-        each_line([&](const uint4 &raw, int i) {
+        each_line<LOADS>([&](const uint4 &raw, int i) {
             const T *x = reinterpret_cast<const T *>(&raw);
 #pragma unroll
             for (int e = 0; e < PER; e++) {
@@ -207,19 +250,16 @@ struct Candidate {
 };
 
 struct BinsShared {
-    unsigned part[3][SL_BINS];  // this CTA's histogram: 15-bit parts of the weights
-    unsigned count[SL_BINS];
-    u64 sum_mass[2][SL_BINS];   // the cluster's, this CTA's share of the bins; [1]: of a bin that was cut finer
+    alignas(16) unsigned part[4][SL_BINS];  // this CTA's histogram: 14-bit parts of the weights, and counts
+    u64 sum_mass[2][SL_BINS];   // what comes before each bin in the row; [1]: of a bin that was cut finer
     unsigned sum_count[2][SL_BINS];
     Candidate list[2][SL_CAND];  // this CTA's tokens of the bin in question; finds take turns
     Candidate all[SL_CAND];      // and the cluster's
     unsigned n_list, key_lo, key_hi;
-    Told told[4][SL_MAX_CLUSTER];  // level 0's totals, a cut bin's, and the lists' (by turns)
-    u64 bin_mass;                  // before the bin where a find's target lies
-    unsigned bin_count;
+    Told told[4][SL_MAX_CLUSTER];  // the first pass's, the second's, and the lists' (by turns)
     int bin, tie;
     Crossing found;
-    u64 scan[SL_WARPS];
+    ScanShared scan;
 };
 
 template <typename T>
@@ -228,6 +268,7 @@ struct Bins {
     Row<T> &row;
     Weigher weigh;
     float per_bin;
+    unsigned least_key;  // no logit below it weighs anything
     int turn = 0;
 
     // by adding 2^23, which leaves the nearest whole number in the low bits
@@ -236,101 +277,69 @@ struct Bins {
     }
 
     __device__ __forceinline__ void zero() {
-        for (int b = threadIdx.x; b < SL_BINS; b += SL_THREADS) s.part[0][b] = s.part[1][b] = s.part[2][b] = s.count[b] = 0;
+        for (int b = threadIdx.x; b < SL_BINS; b += SL_THREADS) s.part[0][b] = s.part[1][b] = s.part[2][b] = s.part[3][b] = 0;
     }
     // 64-bit atomics in shared memory are loops; most weights have few parts
     __device__ __forceinline__ void add(int b, u64 w) {
-        const unsigned p0 = (unsigned)w & 0x7fff, p1 = (unsigned)(w >> 15) & 0x7fff, p2 = (unsigned)(w >> 30);
+        const unsigned p0 = (unsigned)w & 0x3fff, p1 = (unsigned)(w >> 14) & 0x3fff, p2 = (unsigned)(w >> 28);
         if (p0) atomicAdd(&s.part[0][b], p0);
         if (p1) atomicAdd(&s.part[1][b], p1);
         if (p2) atomicAdd(&s.part[2][b], p2);
-        if (w) atomicAdd(&s.count[b], 1u);
+        if (w) atomicAdd(&s.part[3][b], 1u);
     }
 
-    // The CTAs' histograms into sum_*[level], each CTA its share of the bins; everyone learns the shares' totals, and what
-    // else each CTA has to tell.
-    __device__ void merge(int level, u64 above, u64 before_draft) {
+    // Running sums of the CTAs' histograms into sum_*[level]; each CTA adds up a share of the bins for all.
+    __device__ void merge(int level, u64 base_mass, unsigned base_count, u64 &mass, unsigned &count) {
         row.sync();
-        const int share = (SL_BINS + row.C - 1) / row.C, first = row.rank * share, n_own = min(share, SL_BINS - first);
-        u64 m = 0, n = 0;
-        for (int b = threadIdx.x; b < n_own; b += SL_THREADS) {
-            u64 mass = 0;
-            unsigned count = 0;
+        // four bins a thread: remote shared memory gives and takes 16 bytes as fast as 4
+        const int share = (SL_BINS / 4 + row.C - 1) / row.C, b = 4 * (row.rank * share + threadIdx.x);
+        if (threadIdx.x < share && b < SL_BINS) {
+            u64 m[4] = {};
+            uint4 n = {};
+#pragma unroll 1
+            for (int r = 0; r < row.C; r++) {
+                uint4 p[4];
 #pragma unroll
-            for (int r = 0; r < SL_MAX_CLUSTER; r++)
-                if (r < row.C) {
-                    const unsigned p0 = row.of(s.part[0], r)[first + b], p1 = row.of(s.part[1], r)[first + b],
-                                   p2 = row.of(s.part[2], r)[first + b];
-                    mass += p0 + ((u64)p1 << 15) + ((u64)p2 << 30);
-                    count += row.of(s.count, r)[first + b];
-                }
-            s.sum_mass[level][b] = mass;
-            s.sum_count[level][b] = count;
-            m += mass;
-            n += count;
-        }
-        u64 mass, count;
-        block_scan(m, s.scan, &mass);
-        block_scan(n, s.scan, &count);
-        if (threadIdx.x < row.C) {
-            Told *t = row.of(&s.told[level][row.rank], threadIdx.x);
-            t->mass = mass;
-            t->count = (unsigned)count;
-            t->above = above;
-            t->before_draft = before_draft;
-        }
-        row.sync();
-    }
-
-    // The bin where the running mass (or count) passes `target`, and mass and count before it; the target lies in a bin.
-    __device__ void find_bin(int level, u64 target, bool by_count, u64 &mass, unsigned &count, int &bin) {
-        int owner = 0;
-        for (; owner < row.C - 1; owner++) {
-            const u64 m = s.told[level][owner].mass;
-            const unsigned n = s.told[level][owner].count;
-            if ((by_count ? count + n : mass + m) > target) break;
-            mass += m;
-            count += n;
-        }
-        const int share = (SL_BINS + row.C - 1) / row.C, first = owner * share, n_own = min(share, SL_BINS - first);
-        if (row.rank == owner) {
-            constexpr int EACH = SL_BINS / SL_THREADS;
-            u64 m[EACH], n[EACH], tm = 0, tn = 0, total;
-            const int b0 = threadIdx.x * EACH;
-#pragma unroll
-            for (int e = 0; e < EACH; e++) {
-                m[e] = b0 + e < n_own ? s.sum_mass[level][b0 + e] : 0;
-                n[e] = b0 + e < n_own ? s.sum_count[level][b0 + e] : 0;
-                tm += m[e];
-                tn += n[e];
+                for (int k = 0; k < 4; k++) p[k] = *reinterpret_cast<const uint4 *>(row.of(s.part[k], r) + b);
+                m[0] += p[0].x + ((u64)p[1].x << 14) + ((u64)p[2].x << 28);
+                m[1] += p[0].y + ((u64)p[1].y << 14) + ((u64)p[2].y << 28);
+                m[2] += p[0].z + ((u64)p[1].z << 14) + ((u64)p[2].z << 28);
+                m[3] += p[0].w + ((u64)p[1].w << 14) + ((u64)p[2].w << 28);
+                n.x += p[3].x;
+                n.y += p[3].y;
+                n.z += p[3].z;
+                n.w += p[3].w;
             }
-            u64 bm = mass + block_scan(tm, s.scan, &total), bn = count + block_scan(tn, s.scan, &total);
-#pragma unroll
-            for (int e = 0; e < EACH; e++) {
-                const u64 lo = by_count ? bn : bm, hi = lo + (by_count ? n[e] : m[e]);
-                if (lo <= target && target < hi)
-                    for (int r = 0; r < row.C; r++) {
-                        *row.of(&s.bin, r) = first + b0 + e;
-                        *row.of(&s.bin_mass, r) = bm;
-                        *row.of(&s.bin_count, r) = (unsigned)bn;
-                    }
-                bm += m[e];
-                bn += n[e];
+#pragma unroll 1
+            for (int r = 0; r < row.C; r++) {
+                ulonglong2 *to = reinterpret_cast<ulonglong2 *>(row.of(s.sum_mass[level], r) + b);
+                to[0] = make_ulonglong2(m[0], m[1]);
+                to[1] = make_ulonglong2(m[2], m[3]);
+                *reinterpret_cast<uint4 *>(row.of(s.sum_count[level], r) + b) = n;
             }
         }
         row.sync();
-        bin = s.bin;
-        mass = s.bin_mass;
-        count = s.bin_count;
+        static_assert(SL_BINS == 2 * SL_THREADS, "two bins a thread");
+        const int at = 2 * threadIdx.x;
+        const u64 m0 = s.sum_mass[level][at];
+        const unsigned n0 = s.sum_count[level][at];
+        u64 sm = m0 + s.sum_mass[level][at + 1];
+        unsigned sn = n0 + s.sum_count[level][at + 1];
+        block_scan(s.scan, sm, sn, mass, count);
+        s.sum_mass[level][at] = base_mass + sm;
+        s.sum_mass[level][at + 1] = base_mass + sm + m0;
+        s.sum_count[level][at] = base_count + sn;
+        s.sum_count[level][at + 1] = base_count + sn + n0;
+        __syncthreads();
     }
 
     // The token where the running mass (or count) of the row passes `target`, which lies in the row.
     __device__ Crossing find(u64 target, bool by_count) {
-        u64 mass = 0;
-        unsigned count = 0, lo = 0, hi = 0;  // lo, hi: keys of the tokens in question, once the first bin is cut
-        int bin = 0;
+        unsigned lo = 0, hi = 0;  // keys of the tokens in question, once the first bin is cut
         bool cut = false;
-        find_bin(0, target, by_count, mass, count, bin);
+        int bin = search<SL_BINS>(s.sum_mass[0], s.sum_count[0], target, by_count);
+        u64 mass = s.sum_mass[0][bin];
+        unsigned count = s.sum_count[0][bin];
         while (true) {
             // this CTA's tokens of the bin
             const int at_turn = turn;
@@ -342,17 +351,16 @@ struct Bins {
                 s.key_hi = 0;
             }
             __syncthreads();
-            row.each([&](float x, int i) {
+            row.template each<4>([&](float x, int i) {
                 const unsigned key = key_of(x);
-                if (cut ? key < lo || key > hi : bin_of(x) != bin) return;
-                const u64 w = weigh(x);
-                if (w == 0) return;
+                if (key < least_key || (cut ? key < lo || key > hi : bin_of(x) != bin)) return;
                 const unsigned at = atomicAdd(&s.n_list, 1u);
-                if (at < SL_CAND) list[at] = {(u64)key << 32 | (unsigned)~i, w};
+                if (at < SL_CAND) list[at].order = (u64)key << 32 | (unsigned)~i;
                 atomicMin(&s.key_lo, key);
                 atomicMax(&s.key_hi, key);
             });
             __syncthreads();
+            if (threadIdx.x < SL_CAND && threadIdx.x < s.n_list) list[threadIdx.x].w = weigh(of_key((unsigned)(list[threadIdx.x].order >> 32)));
             if (threadIdx.x < row.C) {
                 Told *t = row.of(&s.told[2 + at_turn][row.rank], threadIdx.x);
                 t->count = s.n_list;
@@ -376,12 +384,16 @@ struct Bins {
             const int shift = 32 - __clz((hi - lo) / SL_BINS);
             zero();
             __syncthreads();
-            row.each([&](float x, int) {
+            row.template each<1>([&](float x, int) {
                 const unsigned key = key_of(x);
                 if (key >= lo && key <= hi) add((hi - key) >> shift, weigh(x));
             });
-            merge(1, 0, 0);
-            find_bin(1, target, by_count, mass, count, bin);
+            u64 all_mass;
+            unsigned all_count;
+            merge(1, mass, count, all_mass, all_count);
+            bin = search<SL_BINS>(s.sum_mass[1], s.sum_count[1], target, by_count);
+            mass = s.sum_mass[1][bin];
+            count = s.sum_count[1][bin];
             const unsigned span = (1u << shift) - 1;
             hi -= (unsigned)bin << shift;
             lo = hi - lo > span ? hi - span : lo;
@@ -417,7 +429,7 @@ struct Bins {
         before += mass;
         places += count;
         if (mine < n && from == 0 && (by_count ? places == target : before <= target && target < before + own.w))
-            s.found = {before, own.w, (int)~(unsigned)own.order, 0, 0, 0};
+            s.found = {before, own.w, (int)~(unsigned)own.order, 0, 0};
         __syncthreads();
         const Crossing f = s.found;
         __syncthreads();  // all, found: read
@@ -438,8 +450,9 @@ struct Bins {
             for (int v0 = 0; v0 < row.slice; v0 += SL_THREADS) {
                 const int i = row.i0 + v0 + threadIdx.x;
                 const bool is = v0 + (int)threadIdx.x < row.slice && i >= 0 && i < row.vocab && key_of(to_f32(row.in[i])) == key;
-                u64 here;
-                const u64 before = block_scan(is, s.scan, &here);
+                u64 none = 0, sum;
+                unsigned before = is, here;
+                block_scan(s.scan, none, before, sum, here);
                 if (is && before == left)
                     for (int r = 0; r < row.C; r++) *row.of(&s.tie, r) = i;
                 if (left < here) break;
@@ -447,7 +460,7 @@ struct Bins {
             }
         }
         row.sync();
-        return {mass + nth * w, w, s.tie, 0, 0, 0};
+        return {mass + nth * w, w, s.tie, 0, 0};
     }
 
     __device__ __forceinline__ int index(const Crossing &f) { return f.index; }
@@ -455,21 +468,34 @@ struct Bins {
 
 // ------------------------------------------------------------------ bf16 logits: counts of their values
 
-constexpr int SL_LOW = (127 - 24) << 7, SL_HIGH = (127 + 8) << 7;  // magnitudes that are counted, from 2^-24 to below 2^8
+// Magnitudes that are counted, from 2^-32 to below 2^8. From 2^-24 on, one row in 300 of 151936 normal logits had one below
+// and went the other way, which its whole batch waited for.
+constexpr int SL_LOW = (127 - 32) << 7, SL_HIGH = (127 + 8) << 7;
+constexpr float SL_TINY = 0x1p-32f;
 constexpr int SL_SIGN = SL_HIGH - SL_LOW;
 constexpr int SL_VALUES = 2 * SL_SIGN + 1;  // in the order of the values: positive ones, zero, negative ones
+constexpr int SL_GROUP = 24;                // neighbouring values, which a warp takes side by side
+constexpr int SL_GROUPS = SL_THREADS;       // searched before the values themselves; the last ones are empty
+constexpr int SL_PADDED = (SL_VALUES + SL_GROUP - 1) / SL_GROUP * SL_GROUP;
+static_assert(SL_PADDED <= SL_GROUPS * SL_GROUP && SL_GROUP % 8 == 0, "whole groups, of 16-byte lines");
 
 struct ValuesShared {
-    unsigned count[SL_VALUES + 3];  // this CTA's
-    Told told[SL_MAX_CLUSTER], told_first[SL_MAX_CLUSTER];
-    Crossing found[2];  // finds take turns, so that the next one's writer does not meet the readers of this one
-    unsigned tiny, zeros, equal;  // low magnitudes but zero; the draft's equals before it in its CTA
+    alignas(16) unsigned count[SL_PADDED];  // this CTA's
+    Told told[SL_MAX_CLUSTER];
+    int n_list;  // groups of its share that are not empty
+    unsigned short list[SL_GROUPS];
+    unsigned tiny, equal;  // a low magnitude but zero; the draft's equals before it in its CTA
     unsigned outer;               // key of the largest of high magnitude, 0: none
-    int index;
-    u64 sums[2];
     unsigned top;
-    u64 scan[SL_WARPS];
-    unsigned warps[SL_WARPS];
+    // in the cluster's first CTA:
+    u64 group_mass[SL_GROUPS];  // then what comes before each group
+    unsigned group_count[SL_GROUPS];
+    unsigned equals[SL_MAX_CLUSTER];
+    Crossing at;
+    float prob;
+    bool is_draft;
+    ScanShared scan;
+    unsigned warps[2][2 * SL_WARPS];
 };
 
 __device__ __forceinline__ bf16 value_of(int pos) {
@@ -478,256 +504,274 @@ __device__ __forceinline__ bf16 value_of(int pos) {
 }
 // The value's place, -1 if it is not counted.
 __device__ __forceinline__ int pos_of(unsigned h) {
-    const unsigned m = h & 0x7fff;
+    const int m = h & 0x7fff;
     if (m == 0) return SL_SIGN;
-    if (m - SL_LOW >= SL_SIGN) return -1;
+    if (m < SL_LOW || m >= SL_HIGH) return -1;
     return h & 0x8000 ? SL_SIGN + 1 + (m - SL_LOW) : SL_HIGH - 1 - m;
+}
+// f(value) is true for the first values, down to some place: the number of them, by all lanes of a warp.
+template <typename F>
+__device__ __forceinline__ int first_values(F f) {
+    int lo = 0, hi = SL_VALUES;  // true before lo, false from hi on
+    const int lane = threadIdx.x % 32;
+    while (hi > lo) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const int n = __popc(__ballot_sync(0xffffffffu, at < hi && f(to_f32(value_of(at)))));
+        if (n == 0) return lo;
+        hi = min(hi, lo + n * step);
+        lo += (n - 1) * step + 1;
+    }
+    return lo;
 }
 
 struct Values {
     ValuesShared &s;
     Row<bf16> &row;
-    unsigned *sum;  // this CTA's share of the cluster's counts
+    unsigned *sum;  // the cluster's counts, in a CTA for its share of the groups, in the first one all
     Weigher weigh;
-    int share, each, base;  // values of a CTA's share and of a thread; the thread's first one
-    u64 before_mass, mass;  // of the thread's values
-    unsigned before_count, count;
-    int turn = 0;
 
-    // bits of a line's places that hold the value; zeros are one
-    static __device__ __forceinline__ unsigned equals(const uint4 &raw, unsigned value) {
+    // Bits of a line's places that hold the value; both zeros are one.
+    static __device__ __forceinline__ unsigned equals(const uint4 &raw, bf16 value) {
+        const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&raw), v = __halves2bfloat162(value, value);
         unsigned n = 0;
-        const unsigned *h = reinterpret_cast<const unsigned *>(&raw);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            unsigned a = h[e] & 0xffff, b = h[e] >> 16;
-            if (a == 0x8000) a = 0;
-            if (b == 0x8000) b = 0;
-            n |= (a == value ? 1u : 0u) << 2 * e | (b == value ? 2u : 0u) << 2 * e;
-        }
-        return n;
+        for (int e = 0; e < 4; e++) n |= (__heq2_mask(h[e], v) & 0x20001u) << 2 * e;
+        return (n | n >> 16) & 0xffu;
     }
 
     __device__ __forceinline__ void zero() {
-        for (int v = threadIdx.x; v < SL_VALUES; v += SL_THREADS) s.count[v] = 0;
-        if (threadIdx.x == 0) s.tiny = s.zeros = s.outer = s.equal = s.top = 0;
+        for (int v = 4 * threadIdx.x; v < SL_PADDED; v += 4 * SL_THREADS) *reinterpret_cast<uint4 *>(s.count + v) = make_uint4(0, 0, 0, 0);
+        if (threadIdx.x == 0) s.tiny = s.outer = s.equal = s.top = s.n_list = 0;
+    }
+
+    // A value that is not counted one by one, and not -infinity.
+    __device__ __noinline__ static void odd(ValuesShared &s, unsigned v) {
+        const unsigned m = v & 0x7fff;
+        if (m == 0) atomicAdd(&s.count[SL_SIGN], 1u);
+        else if (m < SL_LOW) s.tiny = 1;
+        else if (m <= 0x7f80) atomicMax(&s.outer, key_of(__uint_as_float(v << 16)));  // else NaN
     }
 
     // One pass over the slice: counts, and the largest value.
     __device__ void stream() {
         __nv_bfloat162 top = __floats2bfloat162_rn(-INFINITY, -INFINITY);
-        unsigned zeros = 0, tiny = 0, outer = 0;
-        row.each_line([&](const uint4 &raw, int) {
+        row.each_line<4>([&](const uint4 &raw, int) {
             const unsigned *h = reinterpret_cast<const unsigned *>(&raw);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 top = __hmax2(top, *reinterpret_cast<const __nv_bfloat162 *>(&h[e]));  // not NaN, if either is not
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    const unsigned v = k ? h[e] >> 16 : h[e] & 0xffff, m = v & 0x7fff, off = m - SL_LOW;
+                    const unsigned v = k ? h[e] >> 16 : h[e] & 0xffff, off = (v & 0x7fff) - SL_LOW;
                     if (off < (unsigned)SL_SIGN) atomicAdd(&s.count[v & 0x8000 ? SL_SIGN + 1 + off : SL_SIGN - 1 - off], 1u);
-                    else if (m == 0) zeros++;
-                    else if (m < SL_LOW) tiny = 1;
-                    else if (m <= 0x7f80 && v != 0xff80) outer = max(outer, key_of(__uint_as_float(v << 16)));
+                    else if (v != 0xff80) odd(s, v);
                 }
             }
         });
         float t = fmaxf(__low2float(top), __high2float(top));
         t = t == t ? t : -INFINITY;
         const unsigned best = __reduce_max_sync(0xffffffffu, t > -INFINITY ? key_of(t) : 0);
-        zeros = __reduce_add_sync(0xffffffffu, zeros);
-        tiny = __reduce_or_sync(0xffffffffu, tiny);
-        outer = __reduce_max_sync(0xffffffffu, outer);
-        if (threadIdx.x % 32 == 0) {
-            atomicMax(&s.top, best);
-            if (zeros) atomicAdd(&s.count[SL_SIGN], zeros);
-            if (tiny) s.tiny = 1;
-            if (outer) atomicMax(&s.outer, outer);
-        }
+        if (threadIdx.x % 32 == 0) atomicMax(&s.top, best);
         __syncthreads();
     }
 
-    // The CTAs' counts, each CTA its share; everyone learns the shares' totals. draft: index, or -1.
-    __device__ void merge(bool has_floor, double least_t, int draft, float xd) {
-        share = (SL_VALUES + row.C - 1) / row.C;
-        const int first = row.rank * share, n_own = max(0, min(share, SL_VALUES - first));
-        if (row.C > 1) {
-#pragma unroll 4
-            for (int b = threadIdx.x; b < n_own; b += SL_THREADS) {
-                unsigned n = 0;
+    // The CTAs' counts to the first one, each CTA the sums of its share of the groups. draft: index, or -1.
+    __device__ void merge(int draft, float xd) {
+        const int own = (SL_PADDED / SL_GROUP + row.C - 1) / row.C;
+        const int first = row.rank * own, last = min(first + own, SL_PADDED / SL_GROUP);
+        if (row.C > 1) {  // remote shared memory gives and takes 16 bytes as fast as 4
+#pragma unroll 1
+            for (int v = first * SL_GROUP + 4 * threadIdx.x; v < last * SL_GROUP; v += 4 * SL_THREADS) {
+                uint4 n = *reinterpret_cast<const uint4 *>(s.count + v);
+#pragma unroll 1
+                for (int r0 = 1; r0 < row.C; r0 += 4) {
+                    uint4 of[4];  // all loads before the first sum
 #pragma unroll
-                for (int r = 0; r < SL_MAX_CLUSTER; r++)
-                    if (r < row.C) n += row.of(s.count, r)[first + b];
-                sum[b] = n;
-            }
-            __syncthreads();
-        }
-        const unsigned value = draft < 0 || xd == 0.0f ? 0 : (unsigned)__bfloat16_as_ushort(__float2bfloat16(xd));
-        const int draft_pos = draft < 0 ? 0 : pos_of(value);  // -1: it weighs nothing
-        const u64 wd = draft < 0 ? 0 : weigh(xd);
-        each = (share + SL_THREADS - 1) / SL_THREADS;
-        base = threadIdx.x * each;
-        mass = 0;
-        count = 0;
-        u64 above = 0, ahead = 0;
-        for (int e = 0; e < each; e++) {
-            const unsigned n = base + e < n_own ? sum[base + e] : 0;
-            if (n == 0) continue;
-            const int pos = first + base + e;
-            const float x = to_f32(value_of(pos));
-            const u64 w = weigh(x);
-            if (w == 0) continue;
-            const u64 m = n * w;
-            mass += m;
-            count += n;
-            if (has_floor && (x == weigh.peak || ((double)x - (double)weigh.peak) * weigh.c >= least_t)) above += m;
-            if (wd > 0 && pos < draft_pos) ahead += m;
-        }
-        u64 all_mass, all_count;
-        before_mass = block_scan(mass, s.scan, &all_mass);
-        before_count = (unsigned)block_scan(count, s.scan, &all_count);
-        if (has_floor || wd > 0) {
-            above = warp_sum(above);
-            ahead = warp_sum(ahead);
-            if (threadIdx.x < 2) s.sums[threadIdx.x] = 0;
-            __syncthreads();
-            if (threadIdx.x % 32 == 0) {
-                atomicAdd(&s.sums[0], above);
-                atomicAdd(&s.sums[1], ahead);
-            }
-            if (wd > 0) {  // its equals with a smaller index
-                const unsigned here = s.count[draft_pos];
-                if (here > 0 && row.i0 + row.slice <= draft) {
-                    if (threadIdx.x == 0) s.equal = here;
-                } else if (here > 1 && row.i0 < draft) {
-                    unsigned n = 0;
-                    row.each_line([&](const uint4 &raw, int i) {
-                        const unsigned is = equals(raw, value);
-                        n += __popc(i + Row<bf16>::PER <= draft ? is : i < draft ? is & ((1u << (draft - i)) - 1) : 0);
-                    });
-                    n = __reduce_add_sync(0xffffffffu, n);
-                    if (threadIdx.x % 32 == 0) atomicAdd(&s.equal, n);
+                    for (int r = 0; r < 4; r++) {
+                        const int rank = row.rank + r0 + r;
+                        of[r] = r0 + r < row.C ? *reinterpret_cast<const uint4 *>(row.of(s.count, rank < row.C ? rank : rank - row.C) + v)
+                                               : make_uint4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        n.x += of[r].x;
+                        n.y += of[r].y;
+                        n.z += of[r].z;
+                        n.w += of[r].w;
+                    }
                 }
+                *reinterpret_cast<uint4 *>(sum + v) = n;
+                if (row.rank != 0) *reinterpret_cast<uint4 *>(row.of(sum, 0) + v) = n;
             }
             __syncthreads();
-            above = s.sums[0];
-            ahead = s.sums[1] + s.equal * wd;
         }
-        if (threadIdx.x < row.C) {
-            Told *t = row.of(&s.told[row.rank], threadIdx.x);
-            t->mass = all_mass;
-            t->count = (unsigned)all_count;
-            t->above = above;
-            t->before_draft = ahead;
+        // Two thirds of the groups are empty in a row of normal logits; the others are listed, in any order, and shared out.
+        {
+            const int g = first + threadIdx.x;
+            unsigned any = 0;
+            if (g < last) {
+#pragma unroll
+                for (int k = 0; k < SL_GROUP / 4; k++) {
+                    const uint4 n = *reinterpret_cast<const uint4 *>(sum + g * SL_GROUP + 4 * k);
+                    any |= n.x | n.y | n.z | n.w;
+                }
+                if (any) s.list[atomicAdd(&s.n_list, 1)] = (unsigned short)g;
+            }
+            if (!any && (g < last || (row.rank == row.C - 1 && g < SL_GROUPS))) *row.of(&s.group_mass[g], 0) = *row.of(&s.group_count[g], 0) = 0;
+            __syncthreads();
+        }
+        const int n_list = s.n_list, sub = n_list <= SL_THREADS / 8 ? 8 : n_list <= SL_THREADS / 4 ? 4 : n_list <= SL_THREADS / 2 ? 2 : 1;
+        const bool mine = (int)threadIdx.x / sub < n_list;  // `sub` neighbouring threads share a group
+        const int g = mine ? s.list[threadIdx.x / sub] : 0;
+        u64 mass = 0;
+        unsigned count = 0;
+        // a warp's lanes stay together
+#pragma unroll 1
+        for (int e = 0; e < SL_GROUP; e += sub) {
+            const int pos = g * SL_GROUP + e + threadIdx.x % sub;
+            const unsigned n = mine ? sum[pos] : 0;
+            if (__any_sync(0xffffffffu, n != 0)) {
+                const u64 w = weigh(to_f32(value_of(n ? pos : 0)));
+                mass += n * w;
+                count += w ? n : 0;
+            }
+        }
+        for (int o = sub / 2; o > 0; o /= 2) {
+            mass += __shfl_xor_sync(0xffffffffu, mass, o);
+            count += __shfl_xor_sync(0xffffffffu, count, o);
+        }
+        if (mine && threadIdx.x % sub == 0) {
+            *row.of(&s.group_mass[g], 0) = mass;
+            *row.of(&s.group_count[g], 0) = count;
+        }
+        if (draft >= 0) {  // the draft's equals with a smaller index
+            const bf16 value = __float2bfloat16(xd);
+            const int pos = pos_of(__bfloat16_as_ushort(value));
+            const unsigned here = pos < 0 ? 0 : s.count[pos];
+            if (here > 0 && row.i0 + row.slice <= draft) {
+                if (threadIdx.x == 0) s.equal = here;
+            } else if (here > 1 && row.i0 < draft) {
+                unsigned n = 0;
+                row.each_line<2>([&](const uint4 &raw, int i) {
+                    const unsigned is = equals(raw, value);
+                    n += __popc(i + Row<bf16>::PER <= draft ? is : i < draft ? is & ((1u << (draft - i)) - 1) : 0);
+                });
+                n = __reduce_add_sync(0xffffffffu, n);
+                if (threadIdx.x % 32 == 0) atomicAdd(&s.equal, n);
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) *row.of(&s.equals[row.rank], 0) = s.equal;
         }
         row.sync();
+    }
+
+    // What follows is the first CTA's. Running sums of the groups, and the row's.
+    __device__ void scan(u64 &mass, unsigned &count) {
+        const int g = threadIdx.x;
+        u64 m = s.group_mass[g];
+        unsigned n = s.group_count[g];
+        block_scan(s.scan, m, n, mass, count);
+        s.group_mass[g] = m;
+        s.group_count[g] = n;
+        __syncthreads();
     }
 
     // The token where the running mass (or count) of the row passes `target`, which lies in the row: which one of which value.
+    // By all lanes of a warp.
     __device__ Crossing find(u64 target, bool by_count) {
-        u64 m0 = 0, n0 = 0;
-        int owner = 0;
-        for (; owner < row.C - 1; owner++) {
-            const u64 m = s.told[owner].mass, n = s.told[owner].count;
-            if ((by_count ? n0 + n : m0 + m) > target) break;
-            m0 += m;
-            n0 += n;
-        }
-        if (row.rank == owner) {
-            const u64 lo = by_count ? n0 + before_count : m0 + before_mass, hi = lo + (by_count ? count : mass);
-            const bool mine = lo <= target && target < hi;
-            const unsigned who = __ballot_sync(0xffffffffu, mine);
-            if (who) {  // the warp where it lies takes the thread's values side by side
-                const int src = __ffs(who) - 1, lane = threadIdx.x % 32;
-                const int first = owner * share, n_own = min(share, SL_VALUES - first);
-                const int b = __shfl_sync(0xffffffffu, base, src) + lane;
-                const bool is = lane < each && b < n_own;
-                const unsigned n = is ? sum[b] : 0;
-                const u64 w = is ? weigh(to_f32(value_of(first + b))) : 0, m = n * w;
-                const unsigned k = w ? n : 0;
-                u64 bm = m;
-                unsigned bn = k;
+        __syncwarp();
+        const int lane = threadIdx.x % 32;
+        const int g = search<SL_GROUPS>(s.group_mass, s.group_count, target, by_count);
+        const int pos = g * SL_GROUP + lane;
+        const bool is = lane < SL_GROUP && pos < SL_VALUES;
+        const u64 w = is ? weigh(to_f32(value_of(pos))) : 0;
+        const unsigned n = is && w ? sum[pos] : 0;
+        const u64 m = n * w;
+        u64 bm = m;
+        unsigned bn = n;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 ym = __shfl_up_sync(0xffffffffu, bm, o);
-                    const unsigned yn = __shfl_up_sync(0xffffffffu, bn, o);
-                    if (lane >= o) {
-                        bm += ym;
-                        bn += yn;
-                    }
-                }
-                bm += m0 + __shfl_sync(0xffffffffu, before_mass, src) - m;
-                bn += (unsigned)n0 + __shfl_sync(0xffffffffu, before_count, src) - k;
-                if (k > 0 && (by_count ? bn <= target && target < bn + k : bm <= target && target < bm + m)) {
-                    const unsigned nth = by_count ? (unsigned)target - bn : (unsigned)((target - bm) / w);
-                    const Crossing f = {bm + nth * w, w, -1, first + b, 0, nth};
-                    for (int r = 0; r < row.C; r++) *row.of(&s.found[turn], r) = f;
-                }
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 ym = __shfl_up_sync(0xffffffffu, bm, o);
+            const unsigned yn = __shfl_up_sync(0xffffffffu, bn, o);
+            if (lane >= o) {
+                bm += ym;
+                bn += yn;
             }
         }
-        row.sync();
-        const Crossing f = s.found[turn];
-        turn ^= 1;
-        return f;
+        bm += s.group_mass[g] - m;
+        bn += s.group_count[g] - n;
+        const int src = 31 - __clz(__ballot_sync(0xffffffffu, n > 0 && (by_count ? bn <= target : bm <= target)));
+        bm = __shfl_sync(0xffffffffu, bm, src);
+        bn = __shfl_sync(0xffffffffu, bn, src);
+        const u64 ws = __shfl_sync(0xffffffffu, w, src);
+        const unsigned nth = by_count ? (unsigned)target - bn : (unsigned)((target - bm) / ws);
+        return {bm + nth * ws, ws, -1, g * SL_GROUP + src, nth};
+    }
+    // The mass before a value, by all lanes of a warp.
+    __device__ u64 before(int pos) {
+        if (pos >= SL_VALUES) pos = SL_VALUES;
+        const int g = min(pos / SL_GROUP, SL_GROUPS - 1), at = g * SL_GROUP + threadIdx.x % 32;
+        return s.group_mass[g] + warp_sum(at < pos ? sum[at] * weigh(to_f32(value_of(at))) : 0);
     }
 
-    // The index of a value's nth token in the CTA that has it, -1 in the others.
+    // The index of a value's nth token.
     __device__ int index(const Crossing &f) {
         const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-        unsigned n = lane < row.C ? row.of(s.count, lane)[f.pos] : 0, run = n;
+        const unsigned here = lane < row.C ? row.of(s.count, lane)[f.pos] : 0;
+        unsigned run = here;
 #pragma unroll
         for (int o = 1; o < SL_MAX_CLUSTER; o <<= 1) {
             const unsigned y = __shfl_up_sync(0xffffffffu, run, o);
             if (lane >= o) run += y;
         }
-        const unsigned before = __shfl_sync(0xffffffffu, run - n, row.rank), here = __shfl_sync(0xffffffffu, n, row.rank);
-        if (f.nth < before || f.nth >= before + here) return -1;
-        const unsigned left = f.nth - before;
-        // each warp a part of the slice; lane j keeps the count of its j-th 32 lines
-        const unsigned value = __bfloat16_as_ushort(value_of(f.pos));
-        const int lines = row.slice / 8, per_warp = (lines + SL_WARPS - 1) / SL_WARPS;
-        const int first = warp * per_warp, last = min(lines, first + per_warp);
-        unsigned mine = 0;
-        for (int l0 = first, it = 0; l0 < last; l0 += 32 * SL_LOADS, it += SL_LOADS) {
-            unsigned is[SL_LOADS];
-#pragma unroll
-            for (int l = 0; l < SL_LOADS; l++)
-                is[l] = l0 + 32 * l + lane < last ? __popc(equals(row.line(row.i0 + 8 * (l0 + 32 * l + lane)), value)) : 0;
-#pragma unroll
-            for (int l = 0; l < SL_LOADS; l++) {
-                const unsigned all = __reduce_add_sync(0xffffffffu, is[l]);
-                if (lane == it + l) mine = all;
+        const int owner = __popc(__ballot_sync(0xffffffffu, lane < row.C && run <= f.nth));
+        unsigned left = f.nth - __shfl_sync(0xffffffffu, run - here, owner);
+        const int i0 = row.i0 + owner * row.slice;
+        // 1024 lines a step, until the step that has it; the next step's lines are on their way meanwhile
+        const bf16 value = value_of(f.pos);
+        const int lines = row.slice / 8;
+        const uint4 none = make_uint4(0x7fff7fff, 0x7fff7fff, 0x7fff7fff, 0x7fff7fff);  // NaN equals nothing
+        auto load = [&](int l) { return l < lines ? row.line(i0 + 8 * l) : none; };
+        uint4 next[2] = {load(threadIdx.x), load(SL_THREADS + threadIdx.x)};
+#pragma unroll 1
+        for (int l0 = 0, odd = 0; l0 < lines; l0 += 2 * SL_THREADS, odd ^= 1) {
+            const unsigned is[2] = {equals(next[0], value), equals(next[1], value)};
+            next[0] = load(l0 + 2 * SL_THREADS + threadIdx.x);
+            next[1] = load(l0 + 3 * SL_THREADS + threadIdx.x);
+            // counts of the warps for the first 512 lines, then for the others: an entry a lane
+            static_assert(2 * SL_WARPS == 32, "an entry a lane");
+            const unsigned n0 = __reduce_add_sync(0xffffffffu, __popc(is[0])), n1 = __reduce_add_sync(0xffffffffu, __popc(is[1]));
+            if (lane < 2) s.warps[odd][lane * SL_WARPS + warp] = lane ? n1 : n0;
+            __syncthreads();
+            const unsigned n = s.warps[odd][lane], all = __reduce_add_sync(0xffffffffu, n);
+            if (left >= all) {
+                left -= all;
+                continue;
             }
-        }
-        const unsigned all = __reduce_add_sync(0xffffffffu, mine);
-        if (lane == 0) s.warps[warp] = all;
-        __syncthreads();
-        unsigned ahead = 0;
-        for (int w = 0; w < warp; w++) ahead += s.warps[w];
-        if (left >= ahead && left < ahead + all) {
             auto scan = [&](unsigned v) {
                 unsigned r = v;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const unsigned y = __shfl_up_sync(0xffffffffu, r, o);
-                    if (lane >= o) r += y;
+                    r += lane >= o ? y : 0;
                 }
                 return r - v;
             };
-            unsigned b = ahead + scan(mine);
-            unsigned who = __ballot_sync(0xffffffffu, left >= b && left < b + mine);
-            const int it = __ffs(who) - 1;
-            ahead = __shfl_sync(0xffffffffu, b, it);
-            const int line = first + 32 * it + lane;
-            unsigned is = line < last ? equals(row.line(row.i0 + 8 * line), value) : 0;
-            b = ahead + scan(__popc(is));
-            if (left >= b && left < b + __popc(is)) {
-                for (unsigned k = left - b; k > 0; k--) is &= is - 1;
-                s.index = row.i0 + 8 * line + __ffs(is) - 1;
+            const unsigned b = scan(n);
+            const int e = __ffs(__ballot_sync(0xffffffffu, left >= b && left < b + n)) - 1;
+            left -= __shfl_sync(0xffffffffu, b, e);
+            if (e % SL_WARPS == warp) {
+                unsigned mine = e < SL_WARPS ? is[0] : is[1];
+                const unsigned before = scan(__popc(mine));
+                if (left >= before && left < before + __popc(mine)) {
+                    for (unsigned j = left - before; j > 0; j--) mine &= mine - 1;
+                    s.at.index = i0 + 8 * (l0 + e / SL_WARPS * SL_THREADS + (int)threadIdx.x) + __ffs(mine) - 1;
+                }
             }
+            break;
         }
         __syncthreads();
-        return s.index;
+        return s.at.index;
     }
 };
 
@@ -746,34 +790,37 @@ struct Draw {
 };
 template <typename Finder>
 __device__ Draw draw(Finder &finder, const Choice &o, const Weigher &weigh, u64 mass, unsigned count, u64 above, u64 before_draft) {
-    Draw d;
-    if (o.k > 0 && (unsigned)o.k < count) {
-        const Crossing f = finder.find((u64)(o.k - 1), true);
-        mass = f.before + f.w;
-    }
-    if (o.p < 1.0f) {  // the shortest beginning with at least p of the mass
-        const double want = ceil((double)fmaxf(o.p, 0.0f) * (double)mass);
-        const Crossing f = finder.find(want < 1.0 ? 0 : min((u64)want, mass) - 1, false);
-        mass = f.before + f.w;
-    }
-    if (o.floor > 0.0f) mass = min(mass, above);
-    d.mass = mass;
-    u64 target = min((u64)((double)o.u * (double)mass), mass - 1);
+    Draw d = {};
     const u64 wd = o.draft >= 0 ? weigh(o.xd) : 0;
-    const bool kept = wd > 0 && before_draft < mass;
-    d.draft = kept && target < wd;
-    d.w = wd;
-    if (!d.draft) {
-        if (kept && target - wd < before_draft) target -= wd;  // the draft's place in the order is empty
-        d.at = finder.find(target, false);
-        d.w = d.at.w;
+    int what = o.k > 0 && (unsigned)o.k < count ? 0 : o.p < 1.0f ? 1 : 2;  // top-k's end, top-p's, the token
+    while (true) {
+        u64 target = o.k - 1;
+        if (what == 1) {  // the shortest beginning with at least p of the mass
+            const double want = ceil((double)fmaxf(o.p, 0.0f) * (double)mass);
+            target = want < 1.0 ? 0 : min((u64)want, mass) - 1;
+        } else if (what == 2) {
+            if (o.floor > 0.0f) mass = min(mass, above);
+            d.mass = mass;
+            target = min((u64)((double)o.u * (double)mass), mass - 1);
+            if (wd > 0 && before_draft < mass) {
+                d.w = wd;
+                d.draft = target < wd;
+                if (d.draft) return d;
+                if (target - wd < before_draft) target -= wd;  // the draft's place in the order is empty
+            }
+        }
+        d.at = finder.find(target, what == 0);
+        if (what == 2) break;
+        mass = d.at.before + d.at.w;
+        what = what == 0 && o.p < 1.0f ? 1 : 2;
     }
+    d.w = d.at.w;
     return d;
 }
 
-__device__ __forceinline__ Weigher weigher(float peak, float temperature, int bits) {
+__device__ __forceinline__ Weigher weigher(float peak, float temperature) {
     // an infinite temperature makes all finite logits weigh the same, -infinity still nothing
-    return {peak, fmax(1.4426950408889634 / (double)temperature, 1e-300), bits};
+    return {peak, fmax(1.4426950408889634 / (double)temperature, 1e-300)};
 }
 
 template <typename T>
@@ -782,7 +829,7 @@ __device__ void sample_bins(BinsShared &s, Row<T> &row, const SampleArgs &a, con
     // the largest token, and the smallest finite logit
     float top = -INFINITY, low = INFINITY;
     int at = 0;
-    row.each([&](float x, int i) {
+    row.template each<4>([&](float x, int i) {
         if (x > top) {
             top = x;
             at = i;
@@ -791,20 +838,17 @@ __device__ void sample_bins(BinsShared &s, Row<T> &row, const SampleArgs &a, con
     });
     const u64 best = warp_max(top > -INFINITY ? (u64)key_of(top) << 32 | (unsigned)~at : 0);
     const unsigned least = __reduce_min_sync(0xffffffffu, key_of(low));
-    if (tid % 32 == 0) {
-        s.scan[tid / 32] = best;
-        s.all[tid / 32].order = least;
-    }
-    Bins<T> bins = {s, row, {}, 0.0f};
+    if (tid % 32 == 0) s.all[tid / 32] = {best, least};
+    Bins<T> bins = {s, row, {}, 0.0f, 0};
     bins.zero();
     __syncthreads();
     if (tid < row.C) {
         u64 f = 0, l = 0xffffffffu;
         for (int w = 0; w < SL_WARPS; w++) {
-            f = max(f, s.scan[w]);
-            l = min(l, s.all[w].order);
+            f = max(f, s.all[w].order);
+            l = min(l, s.all[w].w);
         }
-        Told *t = row.of(&s.told[1][row.rank], tid);
+        Told *t = row.of(&s.told[0][row.rank], tid);
         t->first = f;
         t->low = (unsigned)l;
     }
@@ -812,40 +856,45 @@ __device__ void sample_bins(BinsShared &s, Row<T> &row, const SampleArgs &a, con
     u64 first = 0;
     unsigned min_key = 0xffffffffu;
     for (int c = 0; c < row.C; c++) {
-        first = max(first, s.told[1][c].first);
-        min_key = min(min_key, s.told[1][c].low);
+        first = max(first, s.told[0][c].first);
+        min_key = min(min_key, s.told[0][c].low);
     }
     int token = first ? (int)~(unsigned)first : -1;
     float prob = first ? 1.0f : 0.0f;
     if (first && o.temperature > 0.0f) {
-        const Weigher weigh = weigher(of_key((unsigned)(first >> 32)), o.temperature, a.bits);
+        const Weigher weigh = weigher(of_key((unsigned)(first >> 32)), o.temperature);
         bins.weigh = weigh;
-        const float range = fminf((float)(46.0 / weigh.c), weigh.peak - of_key(min_key));
+        const float range = fminf((float)(44.0 / weigh.c), weigh.peak - of_key(min_key));
         bins.per_bin = range > 0.0f ? fminf(SL_BINS / range, 1e30f) : 0.0f;
+        // nothing below t = -44 weighs anything, and -infinity does not
+        bins.least_key = max(key_of(-3.4028234663852886e38f), key_of(__double2float_rd((double)weigh.peak - 44.0 / weigh.c)));
         const double least_t = o.floor > 0.0f ? log2((double)fminf(o.floor, 1.0f)) : 0.0;
         // the histogram, the mass above min-p's limit, the mass before the draft
         u64 above = 0, before = 0;
-        row.each([&](float x, int i) {
+        row.template each<1>([&](float x, int i) {
             const u64 w = weigh(x);
             bins.add(bins.bin_of(x), w);
             if (o.floor > 0.0f && w && (x == weigh.peak || ((double)x - (double)weigh.peak) * weigh.c >= least_t)) above += w;
             if (o.draft >= 0 && (x > o.xd || (x == o.xd && i < o.draft))) before += w;
         });
+        u64 mass, above_all = 0, before_all = 0;
+        unsigned count;
         if (o.floor > 0.0f || o.draft >= 0) {
-            u64 sum;
-            block_scan(above, s.scan, &sum);
-            above = sum;
-            block_scan(before, s.scan, &sum);
-            before = sum;
+            unsigned none = 0;
+            u64 sum = above;
+            block_scan(s.scan, sum, none, above, count);
+            sum = before;
+            block_scan(s.scan, sum, none, before, count);
+            if (tid < row.C) {
+                Told *t = row.of(&s.told[1][row.rank], tid);
+                t->above = above;
+                t->before_draft = before;
+            }
         }
-        bins.merge(0, above, before);
-        u64 mass = 0, above_all = 0, before_all = 0;
-        unsigned count = 0;
+        bins.merge(0, 0, 0, mass, count);
         for (int c = 0; c < row.C; c++) {
-            mass += s.told[0][c].mass;
-            count += s.told[0][c].count;
-            above_all += s.told[0][c].above;
-            before_all += s.told[0][c].before_draft;
+            above_all += s.told[1][c].above;
+            before_all += s.told[1][c].before_draft;
         }
         const Draw d = draw(bins, o, weigh, mass, count, above_all, before_all);
         token = d.draft ? o.draft : d.at.index;
@@ -863,18 +912,17 @@ __device__ bool sample_values(ValuesShared &s, unsigned *sum, Row<bf16> &row, co
     Values values = {s, row, row.C > 1 ? sum : s.count};
     values.stream();
     if (tid < row.C) {
-        Told *t = row.of(&s.told_first[row.rank], tid);
+        Told *t = row.of(&s.told[row.rank], tid);
         t->first = s.top;
         t->low = s.tiny;
         t->high = s.outer;
     }
-    row.sync();
-    unsigned top = 0, tiny = 0, outer = 0;
-    for (int c = 0; c < row.C; c++) {
-        top = max(top, (unsigned)s.told_first[c].first);
-        tiny |= s.told_first[c].low;
-        outer = max(outer, s.told_first[c].high);
-    }
+    row.arrive();
+    Weigher weigh = weigher(0.0f, o.temperature);
+    row.wait();
+    const Told &told = s.told[min(tid % 32, row.C - 1)];
+    const unsigned top = __reduce_max_sync(0xffffffffu, (unsigned)told.first), tiny = __reduce_max_sync(0xffffffffu, told.low),
+                   outer = __reduce_max_sync(0xffffffffu, told.high);
     if (top == 0) {  // no tokens
         if (row.rank == 0 && tid == 0) {
             a.out[r] = -1;
@@ -885,32 +933,54 @@ __device__ bool sample_values(ValuesShared &s, unsigned *sum, Row<bf16> &row, co
     const float peak = of_key(top);
     const int peak_pos = pos_of(__bfloat16_as_ushort(__float2bfloat16(peak)));
     if (peak_pos < 0) return false;
-    const bool greedy = !(o.temperature > 0.0f);
-    const Weigher weigh = weigher(peak, greedy ? 1.0f : o.temperature, a.bits);
-    values.weigh = weigh;
-    Crossing at = {0, 1, -1, peak_pos, 0, 0};
-    bool is_draft = false;
+    Crossing at = {0, 1, -1, peak_pos, 0};
     float prob = 1.0f;
-    if (!greedy) {
+    if (o.temperature > 0.0f) {
+        weigh.peak = peak;
         if (outer && weigh(of_key(outer)) > 0) return false;
-        if (tiny && (peak < 0x1p-24f || weigh(0x1p-24f) > 0)) return false;
-        const double least_t = o.floor > 0.0f ? log2((double)fminf(o.floor, 1.0f)) : 0.0;
-        values.merge(o.floor > 0.0f, least_t, o.draft, o.xd);
-        u64 mass = 0, above = 0, before = 0;
-        unsigned count = 0;
-        for (int c = 0; c < row.C; c++) {
-            mass += s.told[c].mass;
-            count += s.told[c].count;
-            above += s.told[c].above;
-            before += s.told[c].before_draft;
+        if (tiny && (peak < SL_TINY || weigh(SL_TINY) > 0)) return false;
+        values.weigh = weigh;
+        values.merge(o.draft, o.xd);
+        if (row.rank != 0) return true;
+        u64 mass;
+        unsigned count;
+        values.scan(mass, count);
+        if (tid < 32) {
+            __syncwarp();
+            u64 above = 0, before = 0;
+            if (o.floor > 0.0f) {
+                const double least_t = log2((double)fminf(o.floor, 1.0f));
+                above = values.before(first_values([&](float x) {
+                    return x >= peak || ((double)x - (double)peak) * weigh.c >= least_t;
+                }));
+            }
+            if (o.draft >= 0) {
+                const int pos = pos_of(__bfloat16_as_ushort(__float2bfloat16(o.xd)));
+                unsigned ahead = 0;
+                for (int c = 0; c < row.C; c++) ahead += s.equals[c];
+                if (pos >= 0) before = values.before(pos) + ahead * weigh(o.xd);  // else it weighs nothing
+            }
+            const Draw d = draw(values, o, weigh, mass, count, above, before);
+            if (tid == 0) {
+                s.at = d.at;
+                s.is_draft = d.draft;
+                s.prob = (float)((double)d.w / (double)d.mass);
+            }
         }
-        const Draw d = draw(values, o, weigh, mass, count, above, before);
-        prob = (float)((double)d.w / (double)d.mass);
-        is_draft = d.draft;
-        at = d.at;
+        __syncthreads();
+        at = s.at;
+        prob = s.prob;
+        if (s.is_draft) {
+            if (tid == 0) {
+                a.out[r] = o.draft;
+                if (a.prob) a.prob[r] = prob;
+            }
+            return true;
+        }
     }
-    const int token = is_draft ? (row.rank == 0 ? o.draft : -1) : values.index(at);
-    if (token >= 0 && tid == 0) {
+    if (row.rank != 0) return true;
+    const int token = values.index(at);
+    if (tid == 0) {
         a.out[r] = token;
         if (a.prob) a.prob[r] = prob;
     }
@@ -976,10 +1046,9 @@ int q3_sample_logits(int *out, float *prob, const void *logits, int dtype, int r
     int c = 1;
     while (c < SL_MAX_CLUSTER && (slice_of(c) > SL_SLICE || ((long long)(c + 1) * rows <= 2 * num_sms() && slice_of(c) > 8 * SL_THREADS)))
         c++;
-    const int bits = vocab <= (1 << 18) ? 44 : 42;  // the whole row's mass stays below 2^62
-    SampleArgs a = {out, prob, logits, stride, vocab, slice_of(c), bits, u, temperature, top_p, min_p, top_k, draft};
+    SampleArgs a = {out, prob, logits, stride, vocab, slice_of(c), u, temperature, top_p, min_p, top_k, draft};
     size_t smem = sizeof(BinsShared);
-    if (dtype == 0) smem = std::max(smem, (sizeof(ValuesShared) + 15) / 16 * 16 + (c > 1 ? ((SL_VALUES + c - 1) / c) * 4 : 0));
+    if (dtype == 0) smem = std::max(smem, (sizeof(ValuesShared) + 15) / 16 * 16 + (c > 1 ? SL_PADDED * sizeof(unsigned) : 0));
     auto kernel = dtype == 0 ? sample_logits_kernel<bf16> : sample_logits_kernel<float>;
     cudaError_t e = allow_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return record_cuda_error(e);

@@ -1,7 +1,7 @@
 """Sampling from given random numbers on a B200 against its definition in 64 bits.
 
-A token has to be the one whose interval of the running mass holds u M. Weights are off by 2^-43 of the largest at most
-(and 3e-13 of themselves), so borders of the running mass by vocab * 2^-43 + 3e-13 M: a target closer than that to a border may fall
+A token has to be the one whose interval of the running mass holds u M. Weights are off by 2^-42 of the largest at most
+(and 3e-13 of themselves), so borders of the running mass by vocab * 2^-42 + 3e-13 M: a target closer than that to a border may fall
 on either side of it. Probabilities: one fp32 rounding, 2^-24, and the weights' errors.
 """
 import sys
@@ -65,7 +65,7 @@ def check(x, out, prob, u, t=None, k=None, p=None, floor=None, draft=None):
         order, w, total, target = want
         assert token in order, f"row {r}: token {token} is cut off"
         at = order.tolist().index(token)
-        before, room = w[:at].sum(), vocab * 2.0 ** -43 + 3e-13 * total
+        before, room = w[:at].sum(), vocab * 2.0 ** -42 + 3e-13 * total
         assert before - room <= target <= before + w[at] + room, f"row {r}: token {token} has {before}, {w[at]} and u M is {target}"
         share = w[at] / total
         assert abs(got - share) <= 2.0 ** -24 * share + 2 * room / total, f"row {r}: probability {got}, not {share}"
@@ -294,8 +294,8 @@ def test_refusals():
     refuses(5, out, x, u, None, u)
     refuses(1, out, x, u, draft=out[:1])
     refuses(1, out, x, u, prob=u[:1])
-    refuses(1, out, torch.zeros(2, 1048065, device="cuda", dtype=torch.bfloat16), u)
-    refuses(1, out, torch.zeros(2, 1048065, device="cuda"), u)
+    refuses(1, out, torch.zeros(2, 1048577, device="cuda", dtype=torch.bfloat16), u)
+    refuses(1, out, torch.zeros(2, 1048577, device="cuda"), u)
     refuses(5, out, x.cpu(), u)
     refuses(5, out, x, u.cpu())
     none = torch.zeros(0, dtype=torch.int32, device="cuda")
@@ -303,7 +303,7 @@ def test_refusals():
 
 
 def test_the_largest_vocabularies():
-    for vocab, dtype in ((1048064, torch.bfloat16), (1048064, torch.float32)):
+    for vocab, dtype in ((1048576, torch.bfloat16), (1048576, torch.float32)):
         g = np.random.default_rng(vocab)
         x = torch.from_numpy(g.normal(0, 2, (2, vocab)).astype(np.float32)).cuda().to(dtype)
         run(x, f32(0.3, 0.9))
