@@ -495,6 +495,53 @@ int q3_sample_logits(int *out, float *prob, const void *logits, int dtype, int r
                      const float *u, const float *temperature, const int *top_k, const float *top_p, const float *min_p,
                      const int *draft, void *stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a shared projection. No counterpart in the reference.
+ * For row r of a step and i = index[r]:
+ *   out[r] = base[r] + scale[i] * B_i (A_i x[r])
+ * with A_i [rank, k] and B_i [n, rank] of adapter i, for up to three projections of the same x (q, k and v). Products and sums are
+ * fp32 (A x enters the second product with 16 bits of mantissa), rounded to bf16 once.
+ *
+ * q3_lora_plan sorts the step's rows by adapter, once per step, and all layers and projections use that plan. A plan is
+ * plain device memory that the other calls only read; index, too, so plan and layers can be captured in one CUDA graph
+ * whose index changes from replay to replay. A negative index is a row without an adapter; one past the last adapter sets device error
+ * bit 2 and is treated as none. A plan must have been written before it is used; zeroed memory is a plan without rows.
+ * ------------------------------------------------------------------------------------- */
+
+/* Bytes of a plan (0: more than 65536 rows or 8192 adapters, or none of these). */
+size_t q3_lora_plan_bytes(int n_rows, int n_adapters);
+int q3_lora_plan(void *plan, int n_rows, int n_adapters, const int *index, void *stream);
+
+/* One projection: a is [n_adapters][rank][k], b is [n_adapters][n][rank]. Strides are elements between rows. */
+typedef struct q3_lora_slice {
+    q3_bf16 *out;
+    const q3_bf16 *base;
+    long long out_stride, base_stride;
+    const q3_bf16 *a, *b;
+    int n;
+} q3_lora_slice;
+
+/* What the projections of one call share. k, n, rank and strides are multiples of 8, rank is at most 128, pointers are
+ * 16-byte aligned. Adapter i has ranks[i] <= rank (null: all have rank): what a and b hold past it does not matter.
+ * scale null is 1. */
+typedef struct q3_lora {
+    const q3_bf16 *x;
+    long long x_stride;
+    int k, rank, n_rows, n_adapters;
+    const int *ranks;
+    const float *scale;
+    const void *plan;
+} q3_lora;
+
+/* out may be base (same stride); no output may share elements with x, or with another base or output. Rows without an
+ * adapter: out = base. */
+int q3_lora_add(const q3_lora_slice *slices, int n_slices, const q3_lora *l, void *stream);
+
+/* act = silu(gate) * up with gate and up as above (slices 0 and 1, whose out is not used), for the rows that have an
+ * adapter; the others are left as they are: q3_gate_up_batched, whose taps are the two bases, has written them. act may be
+ * either base (same stride). */
+int q3_lora_gate_up(q3_bf16 *act, long long act_stride, const q3_lora_slice *gate_up, const q3_lora *l, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

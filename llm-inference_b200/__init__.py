@@ -12,6 +12,7 @@ token buffers torch.int32, and ``stream`` defaults to torch's current stream. Er
 from __future__ import annotations
 
 from ._lib import Q3Error, call, load  # noqa: F401
+from .lora import LoraPlan, LoraStack, lora_add, lora_gate_up  # noqa: F401
 from .paged import (PagedPlan, logits_process, paged_attention, paged_rope_append,  # noqa: F401
                     rope_inv_freq, sample_logits)
 
@@ -20,7 +21,7 @@ __all__ = [
     "gemv_residual_forward", "qkv_forward", "gate_up_forward", "qk_norm_rope_forward",
     "attention_forward", "argmax_forward", "sample_forward", "device_error",
     "PagedPlan", "paged_rope_append", "paged_attention", "rope_inv_freq", "logits_process",
-    "sample_logits",
+    "sample_logits", "LoraPlan", "LoraStack", "lora_add", "lora_gate_up",
 ]
 
 

@@ -76,9 +76,14 @@ SIGNATURES: dict[str, list] = {
     "q3_logits_process": [_P, _P, _I, _I, _I, _LL, _LL, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _LL, _P],
     "q3_logits_process_bounded": [_P, _P, _I, _I, _I, _LL, _LL, _P, _P, _P, _LL, _P, _P, _P, _P, _P, _P, _LL, _P, _LL, _P],
     "q3_sample_logits": [_P, _P, _P, _I, _I, _I, _LL, _P, _P, _P, _P, _P, _P, _P],
+    "q3_lora_plan_bytes": [_I, _I],
+    "q3_lora_plan": [_P, _I, _I, _P, _P],
+    "q3_lora_add": [_P, _I, _P, _P],
+    "q3_lora_gate_up": [_P, _LL, _P, _P, _P],
 }
 RESTYPES = {"q3_status_string": ctypes.c_char_p, "q3_attention_scratch_bytes": ctypes.c_size_t,
             "q3_paged_plan_bytes": ctypes.c_size_t, "q3_paged_attention_scratch_bytes": ctypes.c_size_t,
+            "q3_lora_plan_bytes": ctypes.c_size_t,
             "q3_weight_bytes_per_step": ctypes.c_size_t, "q3_kv_bytes_per_position": ctypes.c_size_t}
 
 _lib = None

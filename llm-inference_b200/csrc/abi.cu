@@ -37,6 +37,7 @@ unsigned take_error_attn_fused();
 unsigned take_error_selftest();
 unsigned take_error_paged();
 unsigned take_error_logits();
+unsigned take_error_lora();
 
 namespace {
 constexpr int MAX_DEVICES = 64;
@@ -142,7 +143,7 @@ int q3_device_error(void *stream, unsigned *flags) {
     if (e != cudaSuccess) return q3::record_cuda_error(e);
     *flags = q3::take_error_gemv() | q3::take_error_decode() | q3::take_error_attention() | q3::take_error_tc() |
              q3::take_error_stream() | q3::take_error_attn_fused() | q3::take_error_selftest() | q3::take_error_paged() |
-             q3::take_error_logits();
+             q3::take_error_logits() | q3::take_error_lora();
     return Q3_OK;
 }
 
