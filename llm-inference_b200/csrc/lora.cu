@@ -27,32 +27,30 @@ namespace {
 
 __device__ unsigned g_dev_error;
 
-constexpr int LA_THREADS = 256;
-constexpr int LA_WARPS = LA_THREADS / 32;
 constexpr int LA_MAX_ROWS = 1 << 16;
 constexpr int LA_MAX_ADAPTERS = 8192;
 constexpr int LA_MAX_RANK = 128;
 constexpr int LA_MAX_SLICES = 3;
+constexpr int LA_MAX_CLUSTER = 8;
 constexpr int LA_PASS = 8;  // eight-column tiles of A x at a time: their sums stay in registers
 
-struct LoraTile {
-    int adapter, first, rows, unused;  // adapter -1: rows without one
-};
+// A tile's record: the adapter (-1: rows without one), how many rows, two unused, and the rows.
+constexpr int LA_HEAD = 4;
 
-// Rows of a tile: of a step of few rows as many as one matrix instruction takes.
-__host__ __device__ constexpr int lora_tile_rows(int n_rows) { return n_rows <= 128 ? 16 : 64; }
+// Rows of a tile: of a step of few rows as many as one matrix instruction takes; more share an adapter's weights in
+// longer tiles, as long as there are tiles for all SMs.
+__host__ __device__ constexpr int lora_tile_rows(int n_rows) { return n_rows <= 128 ? 16 : n_rows <= 1024 ? 32 : 64; }
 
 struct LoraPlanLayout {
-    size_t tiles, order, bytes;  // after the number of tiles
-    int max_tiles;
+    int max_tiles, record;  // record: ints of a tile
+    size_t bytes;           // the number of tiles, then the records
 };
 __host__ __device__ inline LoraPlanLayout lora_plan_layout(int n_rows, int n_adapters) {
     LoraPlanLayout l = {};
-    const int kinds = n_rows < n_adapters + 1 ? n_rows : n_adapters + 1;
-    l.max_tiles = kinds + n_rows / lora_tile_rows(n_rows);
-    l.tiles = 16;
-    l.order = l.tiles + (size_t)l.max_tiles * sizeof(LoraTile);
-    l.bytes = l.order + ((size_t)n_rows * 4 + 15) / 16 * 16;
+    const int kinds = n_rows < n_adapters + 1 ? n_rows : n_adapters + 1, tile_rows = lora_tile_rows(n_rows);
+    l.max_tiles = kinds + n_rows / tile_rows;
+    l.record = LA_HEAD + tile_rows;
+    l.bytes = 16 + (size_t)l.max_tiles * l.record * 4;
     return l;
 }
 
@@ -60,14 +58,16 @@ __host__ __device__ inline LoraPlanLayout lora_plan_layout(int n_rows, int n_ada
 
 constexpr int LP_THREADS = 1024;
 
+// Counts, running sums and a stable placement: 10 us for 2079 rows, once per step.
 __global__ void __launch_bounds__(LP_THREADS, 1) lora_plan_kernel(char *plan, int n_rows, int n_adapters, const int *index) {
-    extern __shared__ int la_next[];  // [n_adapters + 1]: rows of each adapter, then where its next row goes; the last: none
-    __shared__ int sums[2][32];
+    extern __shared__ int la_smem_plan[];
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, tile_rows = lora_tile_rows(n_rows), kinds = n_adapters + 1;
+    int *next = la_smem_plan;       // [kinds]: rows of each adapter, then placed ones; the last: those without one
+    int *first = next + kinds;      // [kinds]: its first tile
+    int *sums = first + kinds;      // [32]
     const LoraPlanLayout l = lora_plan_layout(n_rows, n_adapters);
-    LoraTile *tiles = reinterpret_cast<LoraTile *>(plan + l.tiles);
-    int *order = reinterpret_cast<int *>(plan + l.order);
-    for (int i = tid; i < kinds; i += LP_THREADS) la_next[i] = 0;
+    int *tiles = reinterpret_cast<int *>(plan + 16);
+    for (int i = tid; i < kinds; i += LP_THREADS) next[i] = 0;
     pdl_trigger();
     pdl_wait();
     __syncthreads();
@@ -77,36 +77,33 @@ __global__ void __launch_bounds__(LP_THREADS, 1) lora_plan_kernel(char *plan, in
     };
     for (int row = tid; row < n_rows; row += LP_THREADS) {
         if (index[row] >= n_adapters) atomicOr(&g_dev_error, DEV_ERR_POS_RANGE);
-        atomicAdd(&la_next[kind(row)], 1);
+        atomicAdd(&next[kind(row)], 1);
     }
     __syncthreads();
-    // running sums of rows and tiles, 1024 adapters at a time
-    int row0 = 0, tile0 = 0;
+    // running sums of tiles, 1024 adapters at a time
+    int tile0 = 0;
     for (int i0 = 0; i0 < kinds; i0 += LP_THREADS) {
-        const int i = i0 + tid, n = i < kinds ? la_next[i] : 0, t = (n + tile_rows - 1) / tile_rows;
-        int rn = n, rt = t;
+        const int i = i0 + tid, n = i < kinds ? next[i] : 0, t = (n + tile_rows - 1) / tile_rows;
+        int run = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int yn = __shfl_up_sync(0xffffffffu, rn, o), yt = __shfl_up_sync(0xffffffffu, rt, o);
-            rn += lane >= o ? yn : 0;
-            rt += lane >= o ? yt : 0;
+            const int y = __shfl_up_sync(0xffffffffu, run, o);
+            run += lane >= o ? y : 0;
         }
-        if (lane == 31) {
-            sums[0][warp] = rn;
-            sums[1][warp] = rt;
-        }
+        if (lane == 31) sums[warp] = run;
         __syncthreads();
-        int all_n = 0, all_t = 0, before_n = 0, before_t = 0;
+        int all = 0, before = 0;
         for (int w = 0; w < 32; w++) {
-            if (w == warp) before_n = all_n, before_t = all_t;
-            all_n += sums[0][w];
-            all_t += sums[1][w];
+            before += w < warp ? sums[w] : 0;
+            all += sums[w];
         }
-        const int first = row0 + before_n + rn - n, tile = tile0 + before_t + rt - t;
-        if (i < kinds) la_next[i] = first;
-        for (int k = 0; k < t; k++) tiles[tile + k] = {i < n_adapters ? i : -1, first + k * tile_rows, min(tile_rows, n - k * tile_rows), 0};
-        row0 += all_n;
-        tile0 += all_t;
+        const int tile = tile0 + before + run - t;
+        if (i < kinds) {
+            first[i] = tile;
+            next[i] = 0;
+        }
+        for (int k = 0; k < t; k++) *reinterpret_cast<int4 *>(tiles + (tile + k) * l.record) = make_int4(i < n_adapters ? i : -1, min(tile_rows, n - k * tile_rows), 0, 0);
+        tile0 += all;
         __syncthreads();
     }
     if (tid == 0) *reinterpret_cast<int *>(plan) = tile0;
@@ -116,10 +113,10 @@ __global__ void __launch_bounds__(LP_THREADS, 1) lora_plan_kernel(char *plan, in
         const bool mine = k >= 0 && k % (LP_THREADS / 32) == warp;
         if (!__any_sync(0xffffffffu, mine)) continue;
         const unsigned peers = __match_any_sync(0xffffffffu, mine ? k : -1);
-        const int at = mine ? la_next[k] : 0;
+        const int at = mine ? next[k] + __popc(peers & ((1u << lane) - 1)) : 0;
         __syncwarp();
-        if (mine) order[at + __popc(peers & ((1u << lane) - 1))] = row;
-        if (mine && lane == __ffs(peers) - 1) la_next[k] = at + __popc(peers);
+        if (mine) tiles[(first[k] + at / tile_rows) * l.record + LA_HEAD + at % tile_rows] = row;
+        if (mine && lane == __ffs(peers) - 1) next[k] = at + __popc(peers);
         __syncwarp();
     }
 }
@@ -142,7 +139,7 @@ struct LoraArgs {
     bf16 *act;  // gate_up
     long long act_stride;
     int n_slices, k, rank, n_rows, n_adapters;
-    int wide;  // columns of A x in shared memory: each slice's rank rounded up to 16
+    int wide;  // columns of A x in shared memory: each slice's rank rounded up to 32
 };
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -156,214 +153,385 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// 16 bytes to shared memory, zeros if not `in`
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+
+// Threads of a CTA: a tile of 16 rows is a chain of loads, which more warps shorten.
+__host__ __device__ constexpr int lora_threads(int rows) { return rows == 16 ? 512 : 256; }
+
+// A x of a short tile, this CTA's part of k: each warp a part of that for all columns, operands from global memory straight into
+// registers, then the warps' parts added up in their order.
+template <int WARPS>
+__device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float *part, const int *row_s, int rows, int adapter, int r, int C, int rank_c) {
+    constexpr int COLS = 8 * LA_PASS;
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4, each = a.wide / a.n_slices;
+    const int steps = (a.k + 31) / 32, parts = C * WARPS, p = rank_c * WARPS + warp;
+    const int s0 = (int)((long long)steps * p / parts), s1 = (int)((long long)steps * (p + 1) / parts);
+    const bf16 *x0 = a.x + (long long)row_s[min(g, rows - 1)] * a.x_stride, *x1 = a.x + (long long)row_s[min(g + 8, rows - 1)] * a.x_stride;
+    const int tiles_each = (r + 7) / 8, n_tiles = tiles_each * a.n_slices;
+#pragma unroll 1
+    for (int n0 = 0; n0 < n_tiles; n0 += LA_PASS) {
+        float acc[LA_PASS][4] = {};
+        const bf16 *w[LA_PASS];
+#pragma unroll
+        for (int j = 0; j < LA_PASS; j++) {
+            const int nt = n0 + j, sl = nt / tiles_each, row = (nt - sl * tiles_each) * 8 + g;
+            w[j] = nt < n_tiles && row < r ? a.slice[sl].a + ((long long)adapter * a.rank + row) * a.k : nullptr;
+        }
+#pragma unroll 1
+        for (int s = s0; s < s1; s++) {
+            const int k = 32 * s + 8 * t;
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+            const bool in = k < a.k;
+            const uint4 u = in ? __ldg(reinterpret_cast<const uint4 *>(x0 + k)) : zero, v = in ? __ldg(reinterpret_cast<const uint4 *>(x1 + k)) : zero;
+            uint4 b[LA_PASS];
+#pragma unroll
+            for (int j = 0; j < LA_PASS; j++) b[j] = in && w[j] ? __ldg(reinterpret_cast<const uint4 *>(w[j] + k)) : zero;
+            const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
+#pragma unroll
+            for (int j = 0; j < LA_PASS; j++)
+                if (n0 + j < n_tiles) {
+                    mma(acc[j], a0, b[j].x, b[j].y);
+                    mma(acc[j], a1, b[j].z, b[j].w);
+                }
+        }
+        float *own = part + warp * 16 * COLS;
+#pragma unroll
+        for (int j = 0; j < LA_PASS; j++) {
+            *reinterpret_cast<float2 *>(own + g * COLS + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+            *reinterpret_cast<float2 *>(own + (g + 8) * COLS + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+        }
+        __syncthreads();
+        for (int i = tid; i < rows * COLS; i += 32 * WARPS) {
+            const int row = i / COLS, col = i % COLS, nt = n0 + col / 8;
+            if (nt >= n_tiles) continue;
+            float f[WARPS];
+#pragma unroll
+            for (int q = 0; q < WARPS; q++) f[q] = part[(q * 16 + row) * COLS + col];
+#pragma unroll
+            for (int q = 1; q < WARPS; q++) f[0] += f[q];
+            const int sl = nt / tiles_each;
+            h[row * a.wide + sl * each + (nt - sl * tiles_each) * 8 + col % 8] = f[0];
+        }
+        __syncthreads();
+    }
+}
+
+// A x of a long tile, this CTA's part of k: x and A come through shared memory in stages of 64 elements of k (a row is 128 bytes,
+// its 16-byte lines exchanged by the row's lowest bits, so that the eight rows of a matrix lie in different banks), so
+// that each is read once; a warp has 32 rows and its share of the columns. From registers alone, eight warps read A
+// eight times over and 2079 rows took 30 us here.
+constexpr int LA_STAGES = 3, LA_KC = 64, LA_COLS = 192;  // columns at a time
+template <int ROWS>
+__host__ __device__ constexpr int lora_stage_bytes() { return (ROWS + LA_COLS) * LA_KC * 2; }
+
+template <int ROWS>
+__device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigned char *ring, const int *row_s, int rows, int adapter, int r, int C,
+                                            int rank_c) {
+    constexpr int THREADS = lora_threads(ROWS), M_GROUPS = ROWS / 32, N_GROUPS = THREADS / 32 / M_GROUPS, PAIRS = (LA_COLS / 16 + N_GROUPS - 1) / N_GROUPS;
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, mg = warp % M_GROUPS, ng = warp / M_GROUPS, each = a.wide / a.n_slices;
+    const int k16 = (a.k + 15) / 16, k0 = 16 * (int)((long long)k16 * rank_c / C), k1 = min(a.k, 16 * (int)((long long)k16 * (rank_c + 1) / C));
+    const int chunks = (k1 - k0 + LA_KC - 1) / LA_KC;
+    const int tiles_each = (r + 7) / 8, n_tiles = tiles_each * a.n_slices;
+    const uint32_t ring_at = smem_u32(ring);
+#pragma unroll 1
+    for (int n0 = 0; n0 < n_tiles; n0 += LA_COLS / 8) {
+        const int cols = min(LA_COLS, (n_tiles - n0) * 8), lines = (ROWS + cols) * (LA_KC / 8);
+        auto stage = [&](int c) {
+            const uint32_t to = ring_at + c % LA_STAGES * lora_stage_bytes<ROWS>();
+            const int kc = k0 + c * LA_KC;
+            for (int i = tid; i < lines; i += THREADS) {
+                const int row = i / (LA_KC / 8), q = i % (LA_KC / 8), k = kc + 8 * q;
+                const bf16 *from;
+                bool in = c < chunks && k < k1;
+                if (row < ROWS) {
+                    in = in && row < rows;
+                    from = a.x + (long long)row_s[min(row, rows - 1)] * a.x_stride;
+                } else {
+                    const int nt = n0 + (row - ROWS) / 8, sl = nt / tiles_each, rr = (nt - sl * tiles_each) * 8 + (row - ROWS) % 8;
+                    in = in && rr < r;
+                    from = a.slice[sl].a + ((long long)adapter * a.rank + min(rr, r - 1)) * a.k;
+                }
+                copy16(to + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4), in ? from + k : from, in);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        float acc[2][2 * PAIRS][4] = {};
+        for (int c = 0; c < LA_STAGES - 1; c++) stage(c);
+#pragma unroll 1
+        for (int c = 0; c < chunks; c++) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(LA_STAGES - 2) : "memory");
+            __syncthreads();  // this chunk is there; the one before is read
+            stage(c + LA_STAGES - 1);
+            const uint32_t x_at = ring_at + c % LA_STAGES * lora_stage_bytes<ROWS>(), w_at = x_at + ROWS * LA_KC * 2;
+#pragma unroll
+            for (int s = 0; s < LA_KC / 16; s++) {
+                uint32_t am[2][4];
+#pragma unroll
+                for (int m = 0; m < 2; m++) {
+                    const int row = mg * 32 + m * 16 + lane % 16, q = 2 * s + lane / 16;
+                    load_matrices(am[m], x_at + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4));
+                }
+#pragma unroll
+                for (int j = 0; j < PAIRS; j++) {
+                    const int pair = ng + j * N_GROUPS;
+                    if (16 * pair < cols) {
+                        uint32_t bm[4];
+                        const int row = pair * 16 + lane / 16 * 8 + lane % 8, q = 2 * s + lane / 8 % 2;
+                        load_matrices(bm, w_at + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4));
+#pragma unroll
+                        for (int m = 0; m < 2; m++) {
+                            mma(acc[m][2 * j], am[m], bm[0], bm[1]);
+                            mma(acc[m][2 * j + 1], am[m], bm[2], bm[3]);
+                        }
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // the ring may be where h is
+        const int g = lane / 4, t = lane % 4;
+#pragma unroll
+        for (int j = 0; j < 2 * PAIRS; j++) {
+            const int nt = n0 + 2 * (ng + j / 2 * N_GROUPS) + j % 2, sl = nt / tiles_each;
+            if (8 * (nt - n0) >= cols) continue;
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                float *to = h + (mg * 32 + m * 16 + g) * a.wide + sl * each + (nt - sl * tiles_each) * 8 + 2 * t;
+                *reinterpret_cast<float2 *>(to) = make_float2(acc[m][j][0], acc[m][j][1]);
+                *reinterpret_cast<float2 *>(to + 8 * a.wide) = make_float2(acc[m][j][2], acc[m][j][3]);
+            }
+        }
+        __syncthreads();
+    }
+}
+
 // GATE_UP: slices 0 and 1 are gate and up, and what is written is silu(gate) * up.
 template <int ROWS, bool GATE_UP>
-__global__ void __launch_bounds__(LA_THREADS) lora_kernel(const __grid_constant__ LoraArgs a) {
-    constexpr int M_TILES = ROWS / 16, K_SPLITS = LA_WARPS / M_TILES;
+__global__ void __launch_bounds__(lora_threads(ROWS), 512 / lora_threads(ROWS)) lora_kernel(const __grid_constant__ LoraArgs a) {
+    constexpr int THREADS = lora_threads(ROWS), WARPS = THREADS / 32, MT = ROWS == 16 ? 1 : 2;  // MT: 16-row tiles of a warp in the second product
     extern __shared__ __align__(16) unsigned char la_smem[];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = cluster.num_blocks(), rank_c = cluster.block_rank(), tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const int g = lane / 4, t = lane % 4;
-    const int wide = a.wide;
-    float *part = reinterpret_cast<float *>(la_smem);              // [LA_WARPS][16][8 * LA_PASS]
-    float *h = part + LA_WARPS * 16 * 8 * LA_PASS;                 // [ROWS][wide]: this CTA's part of A x
-    bf16 *hi = reinterpret_cast<bf16 *>(h + ROWS * wide);          // [ROWS][wide + 8]: the whole, scaled, upper and lower bits
-    bf16 *lo = hi + ROWS * (wide + 8);
-    __shared__ int row_s[ROWS];
+    const int wide = a.wide, each = wide / a.n_slices;
+    int *row_s = reinterpret_cast<int *>(la_smem), *head_s = row_s + ROWS;  // [ROWS], [LA_HEAD]
+    float *h = reinterpret_cast<float *>(head_s + LA_HEAD);                 // [ROWS][wide]: this CTA's part of A x
+    // [ROWS][wide + 8]: A x, scaled, upper and lower bits; before that the first product's buffers, those of a long tile over h,
+    // too, if that is written once
+    unsigned char *rest = reinterpret_cast<unsigned char *>(h + ROWS * wide);
+    bf16 *hi = reinterpret_cast<bf16 *>(rest), *lo = hi + ROWS * (wide + 8);
 
     pdl_trigger();
     pdl_wait();
-    const LoraPlanLayout l = lora_plan_layout(a.n_rows, a.n_adapters);
     const int tile = blockIdx.x / C;
-    if (tile >= *reinterpret_cast<const int *>(a.plan)) return;  // the whole cluster
-    const LoraTile job = reinterpret_cast<const LoraTile *>(a.plan + l.tiles)[tile];
-    const int *order = reinterpret_cast<const int *>(a.plan + l.order) + job.first;
-    const int rows = job.rows, adapter = job.adapter;
-    if (tid < ROWS) row_s[tid] = order[min(tid, rows - 1)];  // past the last row: that row again, never written
+    const int *record = reinterpret_cast<const int *>(a.plan + 16) + tile * (LA_HEAD + ROWS);
+    const int n_plan = *reinterpret_cast<const int *>(a.plan);
+    const int mine = tid < LA_HEAD + ROWS ? record[tid] : 0;  // past the rows of a tile, or the tiles: anything
+    if (tile >= n_plan) return;  // the whole cluster
+    if (tid < LA_HEAD) head_s[tid] = mine;
     __syncthreads();
-
+    const int adapter = head_s[0], rows = head_s[1];
+    if (GATE_UP && adapter < 0) return;  // the whole cluster: act is right already
+    if (tid >= LA_HEAD && tid < LA_HEAD + rows) row_s[tid - LA_HEAD] = mine;
     int r = 0;
     float scale = 1.0f;
     if (adapter >= 0) {
         r = a.ranks ? max(0, min(a.ranks[adapter], a.rank)) : a.rank;
         if (a.scale) scale = a.scale[adapter];
-    } else if (GATE_UP) {
-        return;  // the whole cluster: act is right already
     }
+    __syncthreads();
 
-    // ---- A x: warp (m tile, part of k)
+    int units = 0;
+    for (int sl = 0; sl < (GATE_UP ? 1 : a.n_slices); sl++) units += (a.slice[sl].n + 31) / 32;
+    bool waiting = false;
     if (r > 0) {
-        const int mt = warp % M_TILES, ks = warp / M_TILES;
-        const int steps = (a.k + 31) / 32, parts = C * K_SPLITS, p = rank_c * K_SPLITS + ks;
-        const int s0 = (int)((long long)steps * p / parts), s1 = (int)((long long)steps * (p + 1) / parts);
-        const bool live = mt * 16 < rows;
-        const bf16 *x0 = a.x + row_s[mt * 16 + g] * a.x_stride, *x1 = a.x + row_s[mt * 16 + g + 8] * a.x_stride;
-        const int tiles_each = (r + 7) / 8, n_tiles = tiles_each * a.n_slices;
-        for (int n0 = 0; n0 < n_tiles; n0 += LA_PASS) {
-            float acc[LA_PASS][4] = {};
-            const bf16 *w[LA_PASS];
-#pragma unroll
-            for (int j = 0; j < LA_PASS; j++) {
-                const int nt = n0 + j, sl = nt / tiles_each, row = (nt - sl * tiles_each) * 8 + g;
-                w[j] = nt < n_tiles && row < r ? a.slice[sl].a + ((long long)adapter * a.rank + row) * a.k : nullptr;
+        if constexpr (ROWS == 16) {
+            // what the second product will read is asked for before the first
+            for (int u = rank_c * WARPS + warp; u < units; u += C * WARPS) {
+                int sl = 0, n0 = u;
+                if (!GATE_UP)
+                    while (n0 >= (a.slice[sl].n + 31) / 32) n0 -= (a.slice[sl++].n + 31) / 32;
+                n0 = 32 * n0 + lane;
+                for (int pr = 0; pr < (GATE_UP ? 2 : 1); pr++)
+                    if (n0 < a.slice[sl].n) prefetch_l2(a.slice[sl + pr].b + ((long long)adapter * a.slice[sl].n + n0) * a.rank);
             }
-            if (live) {
-#pragma unroll 2
-                for (int s = s0; s < s1; s++) {
-                    const int k = 32 * s + 8 * t;
-                    const uint4 zero = make_uint4(0, 0, 0, 0);
-                    const bool in = k < a.k;
-                    const uint4 u = in ? __ldg(reinterpret_cast<const uint4 *>(x0 + k)) : zero, v = in ? __ldg(reinterpret_cast<const uint4 *>(x1 + k)) : zero;
-                    uint4 b[LA_PASS];
+            shrink_short<WARPS>(a, h, reinterpret_cast<float *>(rest), row_s, rows, adapter, r, C, rank_c);
+        } else {
+            shrink_long<ROWS>(a, h, wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest, row_s, rows, adapter, r, C, rank_c);
+        }
+        // the CTAs' parts, in their order. Few: each CTA adds up all of them; more: each some of the columns for all.
+        if (C > 1) cluster.sync();
+        const int octets = rows * wide / 8;
+        const bool all = octets <= THREADS;
+        const int q0 = all ? 0 : (int)((long long)octets * rank_c / C), q1 = all ? octets : (int)((long long)octets * (rank_c + 1) / C);
+        for (int q = q0 + tid; q < q1; q += THREADS) {
+            const int row = 8 * q / wide, col = 8 * q % wide, left = r - col % each;  // of the adapter's rank from here
+            float v[8] = {};
+            if (left > 0) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < C; c0 += 4) {
+                    float4 f[4][2];  // all loads before the first sum
 #pragma unroll
-                    for (int j = 0; j < LA_PASS; j++) b[j] = in && w[j] ? __ldg(reinterpret_cast<const uint4 *>(w[j] + k)) : zero;
-                    const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
+                    for (int c = 0; c < 4; c++)
 #pragma unroll
-                    for (int j = 0; j < LA_PASS; j++)
-                        if (n0 + j < n_tiles) {
-                            mma(acc[j], a0, b[j].x, b[j].y);
-                            mma(acc[j], a1, b[j].z, b[j].w);
+                        for (int half = 0; half < 2; half++)
+                            f[c][half] = *reinterpret_cast<const float4 *>((C > 1 ? cluster.map_shared_rank(h, min(c0 + c, C - 1)) : h) + 8 * q + 4 * half);
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            const bool in = c0 + c < C;
+                            v[4 * half] += in ? f[c][half].x : 0.0f;
+                            v[4 * half + 1] += in ? f[c][half].y : 0.0f;
+                            v[4 * half + 2] += in ? f[c][half].z : 0.0f;
+                            v[4 * half + 3] += in ? f[c][half].w : 0.0f;
                         }
                 }
             }
-            float *mine = part + warp * 16 * 8 * LA_PASS;
-#pragma unroll
-            for (int j = 0; j < LA_PASS; j++) {
-                *reinterpret_cast<float2 *>(mine + g * 8 * LA_PASS + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
-                *reinterpret_cast<float2 *>(mine + (g + 8) * 8 * LA_PASS + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
-            }
-            __syncthreads();
-            // the warps' parts, in their order
-            for (int i = tid; i < rows * 8 * LA_PASS; i += LA_THREADS) {
-                const int row = i / (8 * LA_PASS), col = i % (8 * LA_PASS), nt = n0 + col / 8;
-                if (nt >= n_tiles) continue;
-                float sum = 0.0f;
-#pragma unroll
-                for (int q = 0; q < K_SPLITS; q++) sum += part[((q * M_TILES + row / 16) * 16 + row % 16) * 8 * LA_PASS + col];
-                const int sl = nt / tiles_each;
-                h[row * wide + sl * (wide / a.n_slices) + (nt - sl * tiles_each) * 8 + col % 8] = sum;
-            }
-            __syncthreads();
-        }
-    }
-    // ---- the CTAs' parts, in their order, each CTA some of the columns for all
-    if (r > 0) {
-        if (C > 1) cluster.sync();
-        const int each = wide / a.n_slices, quads = rows * wide / 4, q0 = (int)((long long)quads * rank_c / C), q1 = (int)((long long)quads * (rank_c + 1) / C);
-        for (int q = q0 + tid; q < q1; q += LA_THREADS) {
-            const int row = 4 * q / wide, col = 4 * q % wide;
-            float v[4] = {};
-            if (col % each < r) {
-                for (int c = 0; c < C; c++) {
-                    const float4 f = *reinterpret_cast<const float4 *>((C > 1 ? cluster.map_shared_rank(h, c) : h) + 4 * q);
-                    v[0] += f.x;
-                    v[1] += f.y;
-                    v[2] += f.z;
-                    v[3] += f.w;
-                }
-            }
-            float up[4], low[4];
+            uint32_t up[4], low[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float s = col % each + e < r ? scale * v[e] : 0.0f;
-                up[e] = round_bf16(s);
-                low[e] = isfinite(up[e]) ? s - up[e] : 0.0f;
+                float s[2], b[2], l[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    s[k] = 2 * e + k < left ? scale * v[2 * e + k] : 0.0f;
+                    b[k] = round_bf16(s[k]);
+                    l[k] = isfinite(b[k]) ? s[k] - b[k] : 0.0f;
+                }
+                up[e] = pack2(b[0], b[1]);
+                low[e] = pack2(l[0], l[1]);
             }
-            const uint2 uh = make_uint2(pack2(up[0], up[1]), pack2(up[2], up[3])), ul = make_uint2(pack2(low[0], low[1]), pack2(low[2], low[3]));
-            for (int c = 0; c < C; c++) {
-                *reinterpret_cast<uint2 *>((C > 1 ? cluster.map_shared_rank(hi, c) : hi) + row * (wide + 8) + col) = uh;
-                *reinterpret_cast<uint2 *>((C > 1 ? cluster.map_shared_rank(lo, c) : lo) + row * (wide + 8) + col) = ul;
+            const int at = row * (wide + 8) + col;
+            for (int c = all ? rank_c : 0; c < (all ? rank_c + 1 : C); c++) {
+                *reinterpret_cast<uint4 *>((C > 1 ? cluster.map_shared_rank(hi, c) : hi) + at) = make_uint4(up[0], up[1], up[2], up[3]);
+                *reinterpret_cast<uint4 *>((C > 1 ? cluster.map_shared_rank(lo, c) : lo) + at) = make_uint4(low[0], low[1], low[2], low[3]);
             }
         }
-        if (C > 1) cluster.sync();
-        else __syncthreads();
+        if (all || C == 1) {
+            __syncthreads();
+            if (C > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // has read the others' parts
+            waiting = C > 1;
+        } else {
+            cluster.sync();
+        }
     }
 
-    // ---- out: units of 32 columns, a warp each
+    // ---- out: units of 32 columns and MT row tiles, a warp each
     constexpr int PAIR = GATE_UP ? 2 : 1;
-    const int each = wide / a.n_slices, k_steps = (r + 15) / 16;
-    int units = 0;
-    for (int sl = 0; sl < (GATE_UP ? 1 : a.n_slices); sl++) units += (a.slice[sl].n + 31) / 32;
-    for (int u = rank_c * LA_WARPS + warp; u < units; u += C * LA_WARPS) {
-        int sl = 0, n0 = u;
+    const int k_steps = (r + 31) / 32, groups = (rows + 16 * MT - 1) / (16 * MT);
+    for (int i = rank_c * WARPS + warp; i < units * groups; i += C * WARPS) {
+        const int m0 = i % groups * MT;
+        int sl = 0, n0 = i / groups;
         if (!GATE_UP)
             while (n0 >= (a.slice[sl].n + 31) / 32) n0 -= (a.slice[sl++].n + 31) / 32;
         n0 *= 32;
         const int n = a.slice[sl].n;
         if (r == 0 && !GATE_UP && a.slice[sl].out == a.slice[sl].base) continue;
-        for (int m = 0; m * 16 < rows; m++) {
-            float acc[PAIR][4][4] = {};
-            for (int s = 0; s < k_steps; s++) {
+        uint4 b[PAIR][4];
+        auto load_b = [&](int s) {
 #pragma unroll
-                for (int pr = 0; pr < PAIR; pr++) {
-                    const LoraSlice &c = a.slice[sl + pr];
-                    const int col = (sl + pr) * each + 16 * s + 4 * t, at = (m * 16 + g) * (wide + 8) + col;
-                    uint2 q[4];
+            for (int pr = 0; pr < PAIR; pr++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int nn = n0 + 8 * (g / 2) + 2 * j + g % 2, left = r - (16 * s + 4 * t);
-                        q[j] = make_uint2(0, 0);
-                        if (nn < n && left > 0) {
-                            q[j] = __ldg(reinterpret_cast<const uint2 *>(c.b + ((long long)adapter * n + nn) * a.rank + 16 * s + 4 * t));
-                            if (left < 4) {  // what is past the adapter's rank may be anything
-                                q[j].x &= left == 1 ? 0xffffu : 0xffffffffu;
-                                q[j].y &= left == 3 ? 0xffffu : 0u;
-                            }
-                        }
-                    }
-                    const uint2 u0 = *reinterpret_cast<const uint2 *>(hi + at), u1 = *reinterpret_cast<const uint2 *>(hi + at + 8 * (wide + 8));
-                    const uint2 l0 = *reinterpret_cast<const uint2 *>(lo + at), l1 = *reinterpret_cast<const uint2 *>(lo + at + 8 * (wide + 8));
-                    const uint32_t ah[4] = {u0.x, u1.x, u0.y, u1.y}, al[4] = {l0.x, l1.x, l0.y, l1.y};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        mma(acc[pr][j], ah, q[j].x, q[j].y);
-                        mma(acc[pr][j], al, q[j].x, q[j].y);
-                    }
+                for (int j = 0; j < 4; j++) {
+                    const int nn = n0 + 8 * (g / 2) + 2 * j + g % 2;
+                    b[pr][j] = make_uint4(0, 0, 0, 0);
+                    if (nn < n && 32 * s + 8 * t < r)
+                        b[pr][j] = __ldg(reinterpret_cast<const uint4 *>(a.slice[sl + pr].b + ((long long)adapter * n + nn) * a.rank + 32 * s + 8 * t));
                 }
-            }
-            // a lane has eight neighbouring columns of rows g and g + 8
-            const int col = n0 + 8 * t;
+        };
+        load_b(0);
+        // a lane has eight neighbouring columns of rows g and g + 8 of each tile
+        const int col = n0 + 8 * t;
+        uint4 base[PAIR][MT][2];
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const int i = m * 16 + g + 8 * half;
-                if (i >= rows || col >= n) continue;
-                const long long row = row_s[i];
-                uint32_t y[4];
-                if constexpr (GATE_UP) {
-                    const uint4 bg = *reinterpret_cast<const uint4 *>(a.slice[0].base + row * a.slice[0].base_stride + col);
-                    const uint4 bu = *reinterpret_cast<const uint4 *>(a.slice[1].base + row * a.slice[1].base_stride + col);
-                    const __nv_bfloat162 *pg = reinterpret_cast<const __nv_bfloat162 *>(&bg), *pu = reinterpret_cast<const __nv_bfloat162 *>(&bu);
+        for (int pr = 0; pr < PAIR; pr++)
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    const int at = (m0 + m) * 16 + g + 8 * q;
+                    base[pr][m][q] = make_uint4(0, 0, 0, 0);
+                    if (at < rows && col < n) base[pr][m][q] = *reinterpret_cast<const uint4 *>(a.slice[sl + pr].base + row_s[at] * a.slice[sl + pr].base_stride + col);
+                }
+        float acc[PAIR][MT][4][4] = {};
+#pragma unroll 1
+        for (int s = 0; s < k_steps; s++) {
+            const int left = r - (32 * s + 8 * t);
+            if (left < 8) {  // what is past the adapter's rank may be anything
+                auto keep = [&](int e) { return left > e + 1 ? 0xffffffffu : left > e ? 0xffffu : 0u; };
+#pragma unroll
+                for (int pr = 0; pr < PAIR; pr++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const float2 fg = __bfloat1622float2(pg[j]), fu = __bfloat1622float2(pu[j]);
-                        const float g0 = fg.x + acc[0][j][2 * half], g1 = fg.y + acc[0][j][2 * half + 1];
-                        const float u0 = fu.x + acc[1][j][2 * half], u1 = fu.y + acc[1][j][2 * half + 1];
-                        y[j] = pack2(g0 / (1.0f + __expf(-g0)) * u0, g1 / (1.0f + __expf(-g1)) * u1);
+                        b[pr][j].x &= keep(0);
+                        b[pr][j].y &= keep(2);
+                        b[pr][j].z &= keep(4);
+                        b[pr][j].w &= keep(6);
                     }
-                    *reinterpret_cast<uint4 *>(a.act + row * a.act_stride + col) = make_uint4(y[0], y[1], y[2], y[3]);
-                } else {
-                    const LoraSlice &c = a.slice[sl];
-                    uint4 b = *reinterpret_cast<const uint4 *>(c.base + row * c.base_stride + col);
-                    if (r > 0) {
-                        const __nv_bfloat162 *pb = reinterpret_cast<const __nv_bfloat162 *>(&b);
+            }
+#pragma unroll
+            for (int pr = 0; pr < PAIR; pr++)
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    const int at = ((m0 + m) * 16 + g) * (wide + 8) + (sl + pr) * each + 32 * s + 8 * t;
+#pragma unroll
+                    for (int part = 0; part < 2; part++) {
+                        const bf16 *from = (part ? lo : hi) + at;
+                        const uint4 u = *reinterpret_cast<const uint4 *>(from), v = *reinterpret_cast<const uint4 *>(from + 8 * (wide + 8));
+                        const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            const float2 f = __bfloat1622float2(pb[j]);
-                            y[j] = pack2(f.x + acc[0][j][2 * half], f.y + acc[0][j][2 * half + 1]);
+                            mma(acc[pr][m][j], a0, b[pr][j].x, b[pr][j].y);
+                            mma(acc[pr][m][j], a1, b[pr][j].z, b[pr][j].w);
                         }
-                        b = make_uint4(y[0], y[1], y[2], y[3]);
                     }
-                    *reinterpret_cast<uint4 *>(c.out + row * c.out_stride + col) = b;
                 }
-            }
+            if (s + 1 < k_steps) load_b(s + 1);
         }
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const int at = (m0 + m) * 16 + g + 8 * q;
+                if (at >= rows || col >= n) continue;
+                const long long row = row_s[at];
+                uint32_t y[4];
+                const __nv_bfloat162 *p0 = reinterpret_cast<const __nv_bfloat162 *>(&base[0][m][q]), *p1 = reinterpret_cast<const __nv_bfloat162 *>(&base[PAIR - 1][m][q]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float2 f = __bfloat1622float2(p0[j]);
+                    const float v0 = f.x + acc[0][m][j][2 * q], v1 = f.y + acc[0][m][j][2 * q + 1];
+                    if constexpr (GATE_UP) {
+                        const float2 fu = __bfloat1622float2(p1[j]);
+                        const float u0 = fu.x + acc[1][m][j][2 * q], u1 = fu.y + acc[1][m][j][2 * q + 1];
+                        y[j] = pack2(v0 / (1.0f + __expf(-v0)) * u0, v1 / (1.0f + __expf(-v1)) * u1);
+                    } else {
+                        y[j] = pack2(v0, v1);
+                    }
+                }
+                const uint4 out = r > 0 || GATE_UP ? make_uint4(y[0], y[1], y[2], y[3]) : base[0][m][q];
+                if constexpr (GATE_UP) *reinterpret_cast<uint4 *>(a.act + row * a.act_stride + col) = out;
+                else *reinterpret_cast<uint4 *>(a.slice[sl].out + row * a.slice[sl].out_stride + col) = out;
+            }
     }
+    if (waiting) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // the others have read this one's part
 }
 
-int wide_of(int n_slices, int rank) { return n_slices * ((rank + 15) / 16 * 16); }
+int wide_of(int n_slices, int rank) { return n_slices * ((rank + 31) / 32 * 32); }
 
-size_t lora_smem(int rows, int wide) {
-    return (size_t)LA_WARPS * 16 * 8 * LA_PASS * 4 + (size_t)rows * wide * 4 + 2 * (size_t)rows * (wide + 8) * 2;
+template <int ROWS>
+size_t lora_smem(int wide) {
+    const size_t h = (size_t)ROWS * wide * 4, both = h + 2 * (size_t)ROWS * (wide + 8) * 2;
+    const size_t first = ROWS == 16 ? h + (size_t)lora_threads(ROWS) / 32 * 16 * 8 * LA_PASS * 4
+                                    : (wide <= LA_COLS ? 0 : h) + (size_t)LA_STAGES * lora_stage_bytes<ROWS>();
+    return (size_t)(ROWS + LA_HEAD) * 4 + std::max(first, both);
 }
 
 // Whether two matrices of as many rows share any element.
@@ -380,13 +548,19 @@ bool overlap(const void *a, long long a_stride, int a_width, const void *b, long
 }
 
 template <int ROWS, bool GATE_UP>
-int launch_lora(const LoraArgs &args, int tiles, int cluster, cudaStream_t s) {
+int launch_lora(const LoraArgs &args, int tiles, cudaStream_t s) {
     auto kernel = lora_kernel<ROWS, GATE_UP>;
-    const size_t smem = lora_smem(ROWS, args.wide);
+    const size_t smem = lora_smem<ROWS>(args.wide);
     cudaError_t e = allow_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return record_cuda_error(e);
-    Q3_TRY_LAUNCH(launch(kernel, dim3((unsigned)tiles * cluster), dim3(LA_THREADS), smem, s, cluster, args));
+    // CTAs of a tile: as many as are at work at once, if there are as many tiles as there may be
+    const int cluster = ROWS == 16 ? LA_MAX_CLUSTER : std::max(1, std::min(LA_MAX_CLUSTER, 2 * num_sms() / tiles));
+    Q3_TRY_LAUNCH(launch(kernel, dim3((unsigned)tiles * cluster), dim3(lora_threads(ROWS)), smem, s, cluster, args));
     return Q3_OK;
+}
+template <int ROWS>
+int launch_lora(const LoraArgs &args, int tiles, bool gate_up, cudaStream_t s) {
+    return gate_up ? launch_lora<ROWS, true>(args, tiles, s) : launch_lora<ROWS, false>(args, tiles, s);
 }
 
 int plan_check(int n_rows, int n_adapters) {
@@ -445,8 +619,11 @@ int lora(const q3_lora_slice *slices, int n_slices, const q3_lora *l, bool gate_
     a.wide = wide_of(n_slices, l->rank);
     const int tiles = lora_plan_layout(l->n_rows, l->n_adapters).max_tiles;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (lora_tile_rows(l->n_rows) == 16) return gate_up ? launch_lora<16, true>(a, tiles, 8, s) : launch_lora<16, false>(a, tiles, 8, s);
-    return gate_up ? launch_lora<64, true>(a, tiles, 4, s) : launch_lora<64, false>(a, tiles, 4, s);
+    switch (lora_tile_rows(l->n_rows)) {
+        case 16: return launch_lora<16>(a, tiles, gate_up, s);
+        case 32: return launch_lora<32>(a, tiles, gate_up, s);
+        default: return launch_lora<64>(a, tiles, gate_up, s);
+    }
 }
 
 }  // namespace
@@ -475,7 +652,10 @@ int q3_lora_plan(void *plan, int n_rows, int n_adapters, const int *index, void 
     if (reinterpret_cast<uintptr_t>(plan) & 15) return Q3_ERR_ALIGN;
     const int st = check_device();
     if (st != Q3_OK) return st;
-    Q3_TRY_LAUNCH(launch(lora_plan_kernel, dim3(1), dim3(LP_THREADS), (size_t)(n_adapters + 1) * 4, (cudaStream_t)stream, 1,
+    const size_t smem = (2 * (size_t)(n_adapters + 1) + 32) * 4;
+    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(lora_plan_kernel), smem);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    Q3_TRY_LAUNCH(launch(lora_plan_kernel, dim3(1), dim3(LP_THREADS), smem, (cudaStream_t)stream, 1,
                          static_cast<char *>(plan), n_rows, n_adapters, index));
     return Q3_OK;
 }
