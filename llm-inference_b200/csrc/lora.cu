@@ -12,6 +12,8 @@
 //
 // A x is held in 32 bits and enters the second product as two bf16 numbers, which together have 16 bits of it: its
 // rounding to one would be as large as the output's own.
+#include <math.h>
+
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -38,8 +40,8 @@ constexpr int LA_PASS = 8;  // eight-column tiles of A x at a time: their sums s
 constexpr int LA_HEAD = 4;
 
 // Rows of a tile: of a step of few rows as many as one matrix instruction takes; more share an adapter's weights in
-// longer tiles, as long as there are tiles for all SMs.
-__host__ __device__ constexpr int lora_tile_rows(int n_rows) { return n_rows <= 128 ? 16 : n_rows <= 1024 ? 32 : 64; }
+// longer tiles. 347 rows, 5 adapters of rank 24, gate and up: 20 us with tiles of 32, 33 with 64; 2079 rows, 8 of rank 64, q, k and v: 49 and 61.
+__host__ __device__ constexpr int lora_tile_rows(int n_rows) { return n_rows <= 128 ? 16 : 32; }
 
 struct LoraPlanLayout {
     int max_tiles, record;  // record: ints of a tile
@@ -139,7 +141,8 @@ struct LoraArgs {
     bf16 *act;  // gate_up
     long long act_stride;
     int n_slices, k, rank, n_rows, n_adapters;
-    int wide;  // columns of A x in shared memory: each slice's rank rounded up to 32
+    int wide;   // columns of A x in shared memory: each slice's rank rounded up to 32
+    int pitch;  // and of its bf16 parts: an odd number of 64 bytes, so that the two rows that eight lanes read lie in other banks
 };
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -162,16 +165,19 @@ __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 
-// Threads of a CTA: a tile of 16 rows is a chain of loads, which more warps shorten.
-__host__ __device__ constexpr int lora_threads(int rows) { return rows == 16 ? 512 : 256; }
+// Which slice an eight-column tile of A x belongs to (each has tiles_each), and where it begins.
+__device__ __forceinline__ int slice_of(int nt, int tiles_each) { return nt < tiles_each ? 0 : nt < 2 * tiles_each ? 1 : 2; }
+
+// One CTA an SM: all of it is chains of loads, which sixteen warps overlap.
+constexpr int LA_THREADS = 512;
+constexpr int LA_WARPS = LA_THREADS / 32;
 
 // A x of a short tile, this CTA's part of k: each warp a part of that for all columns, operands from global memory straight into
 // registers, then the warps' parts added up in their order.
-template <int WARPS>
 __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float *part, const int *row_s, int rows, int adapter, int r, int C, int rank_c) {
     constexpr int COLS = 8 * LA_PASS;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4, each = a.wide / a.n_slices;
-    const int steps = (a.k + 31) / 32, parts = C * WARPS, p = rank_c * WARPS + warp;
+    const int steps = (a.k + 31) / 32, parts = C * LA_WARPS, p = rank_c * LA_WARPS + warp;
     const int s0 = (int)((long long)steps * p / parts), s1 = (int)((long long)steps * (p + 1) / parts);
     const bf16 *x0 = a.x + (long long)row_s[min(g, rows - 1)] * a.x_stride, *x1 = a.x + (long long)row_s[min(g + 8, rows - 1)] * a.x_stride;
     const int tiles_each = (r + 7) / 8, n_tiles = tiles_each * a.n_slices;
@@ -181,7 +187,7 @@ __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float 
         const bf16 *w[LA_PASS];
 #pragma unroll
         for (int j = 0; j < LA_PASS; j++) {
-            const int nt = n0 + j, sl = nt / tiles_each, row = (nt - sl * tiles_each) * 8 + g;
+            const int nt = n0 + j, sl = slice_of(nt, tiles_each), row = (nt - sl * tiles_each) * 8 + g;
             w[j] = nt < n_tiles && row < r ? a.slice[sl].a + ((long long)adapter * a.rank + row) * a.k : nullptr;
         }
 #pragma unroll 1
@@ -208,15 +214,15 @@ __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float 
             *reinterpret_cast<float2 *>(own + (g + 8) * COLS + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
         }
         __syncthreads();
-        for (int i = tid; i < rows * COLS; i += 32 * WARPS) {
+        for (int i = tid; i < rows * COLS; i += LA_THREADS) {
             const int row = i / COLS, col = i % COLS, nt = n0 + col / 8;
             if (nt >= n_tiles) continue;
-            float f[WARPS];
+            float f[LA_WARPS];
 #pragma unroll
-            for (int q = 0; q < WARPS; q++) f[q] = part[(q * 16 + row) * COLS + col];
+            for (int q = 0; q < LA_WARPS; q++) f[q] = part[(q * 16 + row) * COLS + col];
 #pragma unroll
-            for (int q = 1; q < WARPS; q++) f[0] += f[q];
-            const int sl = nt / tiles_each;
+            for (int q = 1; q < LA_WARPS; q++) f[0] += f[q];
+            const int sl = slice_of(nt, tiles_each);
             h[row * a.wide + sl * each + (nt - sl * tiles_each) * 8 + col % 8] = f[0];
         }
         __syncthreads();
@@ -225,40 +231,44 @@ __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float 
 
 // A x of a long tile, this CTA's part of k: x and A come through shared memory in stages of 64 elements of k (a row is 128 bytes,
 // its 16-byte lines exchanged by the row's lowest bits, so that the eight rows of a matrix lie in different banks), so
-// that each is read once; a warp has 32 rows and its share of the columns. From registers alone, eight warps read A
-// eight times over and 2079 rows took 30 us here.
+// that each is read once; a warp has all rows and its share of the columns. From registers alone, with each
+// warp reading all of A for its rows, this part took 2079 rows of rank 64 three times as long.
 constexpr int LA_STAGES = 3, LA_KC = 64, LA_COLS = 192;  // columns at a time
-template <int ROWS>
-__host__ __device__ constexpr int lora_stage_bytes() { return (ROWS + LA_COLS) * LA_KC * 2; }
+constexpr int LA_STAGE_BYTES = (32 + LA_COLS) * LA_KC * 2;
 
-template <int ROWS>
 __device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigned char *ring, const int *row_s, int rows, int adapter, int r, int C,
                                             int rank_c) {
-    constexpr int THREADS = lora_threads(ROWS), M_GROUPS = ROWS / 32, N_GROUPS = THREADS / 32 / M_GROUPS, PAIRS = (LA_COLS / 16 + N_GROUPS - 1) / N_GROUPS;
-    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, mg = warp % M_GROUPS, ng = warp / M_GROUPS, each = a.wide / a.n_slices;
+    constexpr int ROWS = 32, PAIRS = (LA_COLS / 16 + LA_WARPS - 1) / LA_WARPS;  // pairs of eight-column tiles of a warp
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, each = a.wide / a.n_slices;
     const int k16 = (a.k + 15) / 16, k0 = 16 * (int)((long long)k16 * rank_c / C), k1 = min(a.k, 16 * (int)((long long)k16 * (rank_c + 1) / C));
     const int chunks = (k1 - k0 + LA_KC - 1) / LA_KC;
     const int tiles_each = (r + 7) / 8, n_tiles = tiles_each * a.n_slices;
     const uint32_t ring_at = smem_u32(ring);
 #pragma unroll 1
     for (int n0 = 0; n0 < n_tiles; n0 += LA_COLS / 8) {
-        const int cols = min(LA_COLS, (n_tiles - n0) * 8), lines = (ROWS + cols) * (LA_KC / 8);
+        const int cols = min(LA_COLS, (n_tiles - n0) * 8);
+        // a thread copies one line of each of these rows: of x, then of A; null: zeros
+        constexpr int EACH = (ROWS + LA_COLS + LA_THREADS / 8 - 1) / (LA_THREADS / 8);
+        const int q_own = tid % 8;
+        const bf16 *from[EACH];
+#pragma unroll
+        for (int j = 0; j < EACH; j++) {
+            const int row = tid / 8 + j * (LA_THREADS / 8);
+            if (row < ROWS) {
+                from[j] = row < rows ? a.x + (long long)row_s[row] * a.x_stride : nullptr;
+            } else {
+                const int nt = n0 + (row - ROWS) / 8, sl = slice_of(nt, tiles_each), rr = (nt - sl * tiles_each) * 8 + (row - ROWS) % 8;
+                from[j] = nt < n_tiles && rr < r ? a.slice[sl].a + ((long long)adapter * a.rank + rr) * a.k : nullptr;
+            }
+        }
         auto stage = [&](int c) {
-            const uint32_t to = ring_at + c % LA_STAGES * lora_stage_bytes<ROWS>();
-            const int kc = k0 + c * LA_KC;
-            for (int i = tid; i < lines; i += THREADS) {
-                const int row = i / (LA_KC / 8), q = i % (LA_KC / 8), k = kc + 8 * q;
-                const bf16 *from;
-                bool in = c < chunks && k < k1;
-                if (row < ROWS) {
-                    in = in && row < rows;
-                    from = a.x + (long long)row_s[min(row, rows - 1)] * a.x_stride;
-                } else {
-                    const int nt = n0 + (row - ROWS) / 8, sl = nt / tiles_each, rr = (nt - sl * tiles_each) * 8 + (row - ROWS) % 8;
-                    in = in && rr < r;
-                    from = a.slice[sl].a + ((long long)adapter * a.rank + min(rr, r - 1)) * a.k;
-                }
-                copy16(to + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4), in ? from + k : from, in);
+            const uint32_t to = ring_at + c % LA_STAGES * LA_STAGE_BYTES;
+            const int k = k0 + c * LA_KC + 8 * q_own;
+#pragma unroll
+            for (int j = 0; j < EACH; j++) {
+                const int row = tid / 8 + j * (LA_THREADS / 8);
+                const bool in = from[j] && c < chunks && k < k1;
+                if (row < ROWS + cols) copy16(to + row * (LA_KC * 2) + ((q_own ^ (row & 7)) << 4), in ? from[j] + k : a.x, in);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -269,18 +279,18 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigne
             asm volatile("cp.async.wait_group %0;" ::"n"(LA_STAGES - 2) : "memory");
             __syncthreads();  // this chunk is there; the one before is read
             stage(c + LA_STAGES - 1);
-            const uint32_t x_at = ring_at + c % LA_STAGES * lora_stage_bytes<ROWS>(), w_at = x_at + ROWS * LA_KC * 2;
+            const uint32_t x_at = ring_at + c % LA_STAGES * LA_STAGE_BYTES, w_at = x_at + ROWS * LA_KC * 2;
 #pragma unroll
             for (int s = 0; s < LA_KC / 16; s++) {
                 uint32_t am[2][4];
 #pragma unroll
                 for (int m = 0; m < 2; m++) {
-                    const int row = mg * 32 + m * 16 + lane % 16, q = 2 * s + lane / 16;
+                    const int row = m * 16 + lane % 16, q = 2 * s + lane / 16;
                     load_matrices(am[m], x_at + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4));
                 }
 #pragma unroll
                 for (int j = 0; j < PAIRS; j++) {
-                    const int pair = ng + j * N_GROUPS;
+                    const int pair = warp + j * LA_WARPS;
                     if (16 * pair < cols) {
                         uint32_t bm[4];
                         const int row = pair * 16 + lane / 16 * 8 + lane % 8, q = 2 * s + lane / 8 % 2;
@@ -299,11 +309,11 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigne
         const int g = lane / 4, t = lane % 4;
 #pragma unroll
         for (int j = 0; j < 2 * PAIRS; j++) {
-            const int nt = n0 + 2 * (ng + j / 2 * N_GROUPS) + j % 2, sl = nt / tiles_each;
+            const int nt = n0 + 2 * (warp + j / 2 * LA_WARPS) + j % 2, sl = slice_of(nt, tiles_each);
             if (8 * (nt - n0) >= cols) continue;
 #pragma unroll
             for (int m = 0; m < 2; m++) {
-                float *to = h + (mg * 32 + m * 16 + g) * a.wide + sl * each + (nt - sl * tiles_each) * 8 + 2 * t;
+                float *to = h + (m * 16 + g) * a.wide + sl * each + (nt - sl * tiles_each) * 8 + 2 * t;
                 *reinterpret_cast<float2 *>(to) = make_float2(acc[m][j][0], acc[m][j][1]);
                 *reinterpret_cast<float2 *>(to + 8 * a.wide) = make_float2(acc[m][j][2], acc[m][j][3]);
             }
@@ -314,19 +324,19 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigne
 
 // GATE_UP: slices 0 and 1 are gate and up, and what is written is silu(gate) * up.
 template <int ROWS, bool GATE_UP>
-__global__ void __launch_bounds__(lora_threads(ROWS), 512 / lora_threads(ROWS)) lora_kernel(const __grid_constant__ LoraArgs a) {
-    constexpr int THREADS = lora_threads(ROWS), WARPS = THREADS / 32, MT = ROWS == 16 ? 1 : 2;  // MT: 16-row tiles of a warp in the second product
+__global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_constant__ LoraArgs a) {
+    constexpr int THREADS = LA_THREADS, WARPS = LA_WARPS, MT = ROWS == 16 || GATE_UP ? 1 : 2;  // MT: 16-row tiles of a warp in the second product
     extern __shared__ __align__(16) unsigned char la_smem[];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = cluster.num_blocks(), rank_c = cluster.block_rank(), tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const int g = lane / 4, t = lane % 4;
-    const int wide = a.wide, each = wide / a.n_slices;
+    const int wide = a.wide, pitch = a.pitch, each = wide / a.n_slices;
     int *row_s = reinterpret_cast<int *>(la_smem), *head_s = row_s + ROWS;  // [ROWS], [LA_HEAD]
     float *h = reinterpret_cast<float *>(head_s + LA_HEAD);                 // [ROWS][wide]: this CTA's part of A x
-    // [ROWS][wide + 8]: A x, scaled, upper and lower bits; before that the first product's buffers, those of a long tile over h,
+    // [ROWS][pitch]: A x, scaled, upper and lower bits; before that the first product's buffers, those of a long tile over h,
     // too, if that is written once
     unsigned char *rest = reinterpret_cast<unsigned char *>(h + ROWS * wide);
-    bf16 *hi = reinterpret_cast<bf16 *>(rest), *lo = hi + ROWS * (wide + 8);
+    bf16 *hi = reinterpret_cast<bf16 *>(rest), *lo = hi + ROWS * pitch;
 
     pdl_trigger();
     pdl_wait();
@@ -348,6 +358,11 @@ __global__ void __launch_bounds__(lora_threads(ROWS), 512 / lora_threads(ROWS)) 
     }
     __syncthreads();
 
+    if (adapter < 0) {  // nothing to add; in place there is nothing to do at all
+        bool copies = false;
+        for (int sl = 0; sl < a.n_slices; sl++) copies |= a.slice[sl].out != a.slice[sl].base;
+        if (!copies) return;  // the whole cluster
+    }
     int units = 0;
     for (int sl = 0; sl < (GATE_UP ? 1 : a.n_slices); sl++) units += (a.slice[sl].n + 31) / 32;
     bool waiting = false;
@@ -362,9 +377,9 @@ __global__ void __launch_bounds__(lora_threads(ROWS), 512 / lora_threads(ROWS)) 
                 for (int pr = 0; pr < (GATE_UP ? 2 : 1); pr++)
                     if (n0 < a.slice[sl].n) prefetch_l2(a.slice[sl + pr].b + ((long long)adapter * a.slice[sl].n + n0) * a.rank);
             }
-            shrink_short<WARPS>(a, h, reinterpret_cast<float *>(rest), row_s, rows, adapter, r, C, rank_c);
+            shrink_short(a, h, reinterpret_cast<float *>(rest), row_s, rows, adapter, r, C, rank_c);
         } else {
-            shrink_long<ROWS>(a, h, wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest, row_s, rows, adapter, r, C, rank_c);
+            shrink_long(a, h, wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest, row_s, rows, adapter, r, C, rank_c);
         }
         // the CTAs' parts, in their order. Few: each CTA adds up all of them; more: each some of the columns for all.
         if (C > 1) cluster.sync();
@@ -408,7 +423,7 @@ __global__ void __launch_bounds__(lora_threads(ROWS), 512 / lora_threads(ROWS)) 
                 up[e] = pack2(b[0], b[1]);
                 low[e] = pack2(l[0], l[1]);
             }
-            const int at = row * (wide + 8) + col;
+            const int at = row * pitch + col;
             for (int c = all ? rank_c : 0; c < (all ? rank_c + 1 : C); c++) {
                 *reinterpret_cast<uint4 *>((C > 1 ? cluster.map_shared_rank(hi, c) : hi) + at) = make_uint4(up[0], up[1], up[2], up[3]);
                 *reinterpret_cast<uint4 *>((C > 1 ? cluster.map_shared_rank(lo, c) : lo) + at) = make_uint4(low[0], low[1], low[2], low[3]);
@@ -423,85 +438,92 @@ __global__ void __launch_bounds__(lora_threads(ROWS), 512 / lora_threads(ROWS)) 
         }
     }
 
-    // ---- out: units of 32 columns and MT row tiles, a warp each
+    // ---- out: units of 32 columns and MT row tiles, a warp each. While one step of 32 of the rank is multiplied, the next
+    // one's B is on its way, and after a unit the next unit's base.
     constexpr int PAIR = GATE_UP ? 2 : 1;
-    const int k_steps = (r + 31) / 32, groups = (rows + 16 * MT - 1) / (16 * MT);
-    for (int i = rank_c * WARPS + warp; i < units * groups; i += C * WARPS) {
-        const int m0 = i % groups * MT;
-        int sl = 0, n0 = i / groups;
+    const int k_steps = max(1, (r + 31) / 32), groups = (rows + 16 * MT - 1) / (16 * MT), items = units * groups;
+    struct Unit {
+        int sl, n0, m0;
+    };
+    auto unit = [&](int i) {
+        Unit u = {0, i / groups, i % groups * MT};
         if (!GATE_UP)
-            while (n0 >= (a.slice[sl].n + 31) / 32) n0 -= (a.slice[sl++].n + 31) / 32;
-        n0 *= 32;
-        const int n = a.slice[sl].n;
-        if (r == 0 && !GATE_UP && a.slice[sl].out == a.slice[sl].base) continue;
-        uint4 b[PAIR][4];
-        auto load_b = [&](int s) {
+            while (u.n0 >= (a.slice[u.sl].n + 31) / 32) u.n0 -= (a.slice[u.sl++].n + 31) / 32;
+        u.n0 *= 32;
+        return u;
+    };
+    uint4 b[4], base[PAIR][MT][2];
+    auto load_b = [&](const Unit &u, int pr, int s) {
+        const LoraSlice &c = a.slice[u.sl + pr];
+        const bf16 *from = c.b + (long long)adapter * c.n * a.rank + 32 * s + 8 * t;
 #pragma unroll
-            for (int pr = 0; pr < PAIR; pr++)
+        for (int j = 0; j < 4; j++) {
+            const int nn = u.n0 + 8 * (g / 2) + 2 * j + g % 2;
+            b[j] = make_uint4(0, 0, 0, 0);
+            if (nn < c.n && 32 * s + 8 * t < r) b[j] = __ldg(reinterpret_cast<const uint4 *>(from + (long long)nn * a.rank));
+        }
+    };
+    auto load_base = [&](const Unit &u) {  // a lane has eight neighbouring columns of rows g and g + 8 of each tile
+        const int col = u.n0 + 8 * t;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int nn = n0 + 8 * (g / 2) + 2 * j + g % 2;
-                    b[pr][j] = make_uint4(0, 0, 0, 0);
-                    if (nn < n && 32 * s + 8 * t < r)
-                        b[pr][j] = __ldg(reinterpret_cast<const uint4 *>(a.slice[sl + pr].b + ((long long)adapter * n + nn) * a.rank + 32 * s + 8 * t));
-                }
-        };
-        load_b(0);
-        // a lane has eight neighbouring columns of rows g and g + 8 of each tile
-        const int col = n0 + 8 * t;
-        uint4 base[PAIR][MT][2];
-#pragma unroll
-        for (int pr = 0; pr < PAIR; pr++)
+        for (int pr = 0; pr < PAIR; pr++) {
+            const LoraSlice &c = a.slice[u.sl + pr];
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
                 for (int q = 0; q < 2; q++) {
-                    const int at = (m0 + m) * 16 + g + 8 * q;
+                    const int at = (u.m0 + m) * 16 + g + 8 * q;
                     base[pr][m][q] = make_uint4(0, 0, 0, 0);
-                    if (at < rows && col < n) base[pr][m][q] = *reinterpret_cast<const uint4 *>(a.slice[sl + pr].base + row_s[at] * a.slice[sl + pr].base_stride + col);
+                    if (at < rows && col < c.n) base[pr][m][q] = *reinterpret_cast<const uint4 *>(c.base + row_s[at] * c.base_stride + col);
                 }
-        float acc[PAIR][MT][4][4] = {};
+        }
+    };
+    int i = rank_c * WARPS + warp;
+    Unit u = unit(min(i, items - 1));
+    if (i < items) {
+        load_b(u, 0, 0);
+        load_base(u);
+    }
 #pragma unroll 1
-        for (int s = 0; s < k_steps; s++) {
-            const int left = r - (32 * s + 8 * t);
-            if (left < 8) {  // what is past the adapter's rank may be anything
+    for (; i < items; i += C * WARPS) {
+        const Unit next = unit(min(i + C * WARPS, items - 1));
+        float acc[PAIR][MT][4][4] = {};
+#pragma unroll
+        for (int pr = 0; pr < PAIR; pr++)
+#pragma unroll 1
+            for (int s = 0; s < k_steps; s++) {
+                uint4 now[4];
+                const int left = r - (32 * s + 8 * t);  // what is past the adapter's rank may be anything
                 auto keep = [&](int e) { return left > e + 1 ? 0xffffffffu : left > e ? 0xffffu : 0u; };
+                const uint32_t k0 = keep(0), k1 = keep(2), k2 = keep(4), k3 = keep(6);
 #pragma unroll
-                for (int pr = 0; pr < PAIR; pr++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        b[pr][j].x &= keep(0);
-                        b[pr][j].y &= keep(2);
-                        b[pr][j].z &= keep(4);
-                        b[pr][j].w &= keep(6);
-                    }
-            }
-#pragma unroll
-            for (int pr = 0; pr < PAIR; pr++)
+                for (int j = 0; j < 4; j++) now[j] = make_uint4(b[j].x & k0, b[j].y & k1, b[j].z & k2, b[j].w & k3);
+                if (s + 1 < k_steps) load_b(u, pr, s + 1);
+                else if (pr + 1 < PAIR) load_b(u, pr + 1, 0);
+                else if (i + C * WARPS < items) load_b(next, 0, 0);
+                if (r == 0) break;
 #pragma unroll
                 for (int m = 0; m < MT; m++) {
-                    const int at = ((m0 + m) * 16 + g) * (wide + 8) + (sl + pr) * each + 32 * s + 8 * t;
+                    const int at = ((u.m0 + m) * 16 + g) * pitch + (u.sl + pr) * each + 32 * s + 8 * t;
 #pragma unroll
                     for (int part = 0; part < 2; part++) {
                         const bf16 *from = (part ? lo : hi) + at;
-                        const uint4 u = *reinterpret_cast<const uint4 *>(from), v = *reinterpret_cast<const uint4 *>(from + 8 * (wide + 8));
-                        const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
+                        const uint4 v = *reinterpret_cast<const uint4 *>(from), w = *reinterpret_cast<const uint4 *>(from + 8 * pitch);
+                        const uint32_t a0[4] = {v.x, w.x, v.y, w.y}, a1[4] = {v.z, w.z, v.w, w.w};
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            mma(acc[pr][m][j], a0, b[pr][j].x, b[pr][j].y);
-                            mma(acc[pr][m][j], a1, b[pr][j].z, b[pr][j].w);
+                            mma(acc[pr][m][j], a0, now[j].x, now[j].y);
+                            mma(acc[pr][m][j], a1, now[j].z, now[j].w);
                         }
                     }
                 }
-            if (s + 1 < k_steps) load_b(s + 1);
-        }
+            }
+        const int col = u.n0 + 8 * t;
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
             for (int q = 0; q < 2; q++) {
-                const int at = (m0 + m) * 16 + g + 8 * q;
-                if (at >= rows || col >= n) continue;
-                const long long row = row_s[at];
+                const int at = (u.m0 + m) * 16 + g + 8 * q;
                 uint32_t y[4];
                 const __nv_bfloat162 *p0 = reinterpret_cast<const __nv_bfloat162 *>(&base[0][m][q]), *p1 = reinterpret_cast<const __nv_bfloat162 *>(&base[PAIR - 1][m][q]);
 #pragma unroll
@@ -511,26 +533,33 @@ __global__ void __launch_bounds__(lora_threads(ROWS), 512 / lora_threads(ROWS)) 
                     if constexpr (GATE_UP) {
                         const float2 fu = __bfloat1622float2(p1[j]);
                         const float u0 = fu.x + acc[1][m][j][2 * q], u1 = fu.y + acc[1][m][j][2 * q + 1];
-                        y[j] = pack2(v0 / (1.0f + __expf(-v0)) * u0, v1 / (1.0f + __expf(-v1)) * u1);
+                        // (the compiler's own divide, with a branch for rare operands, costs the kernel registers and twice its time)
+                        y[j] = pack2(__fdividef(v0, 1.0f + __expf(-v0)) * u0, __fdividef(v1, 1.0f + __expf(-v1)) * u1);
                     } else {
                         y[j] = pack2(v0, v1);
                     }
                 }
                 const uint4 out = r > 0 || GATE_UP ? make_uint4(y[0], y[1], y[2], y[3]) : base[0][m][q];
-                if constexpr (GATE_UP) *reinterpret_cast<uint4 *>(a.act + row * a.act_stride + col) = out;
-                else *reinterpret_cast<uint4 *>(a.slice[sl].out + row * a.slice[sl].out_stride + col) = out;
+                if (at < rows && col < a.slice[u.sl].n) {
+                    if constexpr (GATE_UP) *reinterpret_cast<uint4 *>(a.act + row_s[at] * a.act_stride + col) = out;
+                    else *reinterpret_cast<uint4 *>(a.slice[u.sl].out + row_s[at] * a.slice[u.sl].out_stride + col) = out;
+                }
             }
+        u = next;
+        if (i + C * WARPS < items) load_base(u);
     }
     if (waiting) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // the others have read this one's part
 }
 
 int wide_of(int n_slices, int rank) { return n_slices * ((rank + 31) / 32 * 32); }
 
+int pitch_of(int wide) { return wide / 32 % 2 ? wide : wide + 32; }
+
 template <int ROWS>
 size_t lora_smem(int wide) {
-    const size_t h = (size_t)ROWS * wide * 4, both = h + 2 * (size_t)ROWS * (wide + 8) * 2;
-    const size_t first = ROWS == 16 ? h + (size_t)lora_threads(ROWS) / 32 * 16 * 8 * LA_PASS * 4
-                                    : (wide <= LA_COLS ? 0 : h) + (size_t)LA_STAGES * lora_stage_bytes<ROWS>();
+    const size_t h = (size_t)ROWS * wide * 4, both = h + 2 * (size_t)ROWS * pitch_of(wide) * 2;
+    const size_t first = ROWS == 16 ? h + (size_t)LA_WARPS * 16 * 8 * LA_PASS * 4
+                                    : (wide <= LA_COLS ? 0 : h) + (size_t)LA_STAGES * LA_STAGE_BYTES;
     return (size_t)(ROWS + LA_HEAD) * 4 + std::max(first, both);
 }
 
@@ -553,9 +582,12 @@ int launch_lora(const LoraArgs &args, int tiles, cudaStream_t s) {
     const size_t smem = lora_smem<ROWS>(args.wide);
     cudaError_t e = allow_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return record_cuda_error(e);
-    // CTAs of a tile: as many as are at work at once, if there are as many tiles as there may be
-    const int cluster = ROWS == 16 ? LA_MAX_CLUSTER : std::max(1, std::min(LA_MAX_CLUSTER, 2 * num_sms() / tiles));
-    Q3_TRY_LAUNCH(launch(kernel, dim3((unsigned)tiles * cluster), dim3(lora_threads(ROWS)), smem, s, cluster, args));
+    // CTAs of a tile: as many as the SMs hold at once for as many tiles as there would be if each row took an adapter at random
+    // (64 rows, 64 adapters, about 41 tiles: clusters of 2 take 16.1 us, of 3 12.9, of 4 21.1)
+    const int kinds = args.n_adapters + 1;
+    const double expected = kinds * (1.0 - exp(-(double)args.n_rows / kinds)) + args.n_rows / ROWS;
+    const int cluster = std::max(1, std::min(LA_MAX_CLUSTER, (int)(num_sms() / expected)));
+    Q3_TRY_LAUNCH(launch(kernel, dim3((unsigned)tiles * cluster), dim3(LA_THREADS), smem, s, cluster, args));
     return Q3_OK;
 }
 template <int ROWS>
@@ -617,13 +649,10 @@ int lora(const q3_lora_slice *slices, int n_slices, const q3_lora *l, bool gate_
     a.n_rows = l->n_rows;
     a.n_adapters = l->n_adapters;
     a.wide = wide_of(n_slices, l->rank);
+    a.pitch = pitch_of(a.wide);
     const int tiles = lora_plan_layout(l->n_rows, l->n_adapters).max_tiles;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    switch (lora_tile_rows(l->n_rows)) {
-        case 16: return launch_lora<16>(a, tiles, gate_up, s);
-        case 32: return launch_lora<32>(a, tiles, gate_up, s);
-        default: return launch_lora<64>(a, tiles, gate_up, s);
-    }
+    return lora_tile_rows(l->n_rows) == 16 ? launch_lora<16>(a, tiles, gate_up, s) : launch_lora<32>(a, tiles, gate_up, s);
 }
 
 }  // namespace

@@ -178,7 +178,7 @@ def test_in_place_and_strided():
 
 
 def test_rows_do_not_depend_on_their_neighbours():
-    # up to 128 rows a row's sums are cut alike, whatever shares its tile
+    # with so few adapters the calls have clusters of one size, so a row's sums are cut alike, whatever shares its tile
     c = Case(100, 1024, [256], 32, 5, some(100, 5))
     want = c.add()[0]
     for at in ([3], [7, 50, 51, 99], list(range(0, 100, 3))):
