@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
     }
     __syncthreads();
 
-    if (adapter < 0) {  // nothing to add; in place there is nothing to do at all
+    if (!GATE_UP && r == 0) {  // nothing to add; in place there is nothing to do at all
         bool copies = false;
         for (int sl = 0; sl < a.n_slices; sl++) copies |= a.slice[sl].out != a.slice[sl].base;
         if (!copies) return;  // the whole cluster

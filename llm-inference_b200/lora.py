@@ -47,10 +47,10 @@ class LoraPlan:
             self._zeroed = made_on.cuda_stream, made_on.record_event()
 
     def update(self, index, stream=None):
-        torch, name, stream, dev = _t(), "q3_lora_plan", _stream(stream), paged._device()
+        torch, name, dev = _t(), "q3_lora_plan", paged._device()
         if self._on != dev:
             _refuse(name, _ELSEWHERE)
-        at = _vector(name, index, "index", self.n_rows, torch.int32, dev)
+        at, stream = _vector(name, index, "index", self.n_rows, torch.int32, dev), _stream(stream)
         if self._zeroed is not None and not torch.cuda.is_current_stream_capturing():  # a capture began after a wait for all
             made_on, zeroed = self._zeroed
             if stream != made_on:

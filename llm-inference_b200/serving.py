@@ -4,10 +4,11 @@
 values go. Every step it gives each running sequence one token and, in what is left of the step's
 rows, one chunk of the oldest unfinished prompt. :class:`PagedServer` runs such a step through the
 model: the projections of the batched ABI, and per layer ``paged_rope_append`` and
-``paged_attention`` with the step's one plan; then ``logits_process`` and the argmax.
+``paged_attention`` with the step's one plan, and ``lora_add`` and ``lora_gate_up`` beside the projections of sequences with an
+adapter; then ``logits_process`` and the argmax, or ``sample_logits`` where a sequence has a temperature.
 
     server = PagedServer(DeviceWeights.load(model_dir), n_pages=4096)
-    a = server.add(prompt, repetition=1.1)
+    a = server.add(prompt, repetition=1.1, temperature=0.6, top_k=20, top_p=0.95, seed=7)
     while server.running():
         for seq, token in server.step().items():
             ...  # server.remove(seq) once it has said what it had to
@@ -24,7 +25,8 @@ from dataclasses import dataclass, field
 import numpy as np
 
 from ._lib import call
-from .paged import PagedPlan, logits_process, paged_attention, paged_rope_append, rope_inv_freq
+from .lora import LoraPlan, lora_add, lora_gate_up
+from .paged import PagedPlan, logits_process, paged_attention, paged_rope_append, rope_inv_freq, sample_logits
 
 
 @dataclass
@@ -35,9 +37,22 @@ class Sequence:
     presence: float = 0.0
     bias: dict[int, float] = field(default_factory=dict)
     mask: np.ndarray | None = None  # int32 words, one bit per allowed token
+    temperature: float = 0.0        # 0: the largest logit
+    top_k: int = 0                  # 0: all
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: int | None = None         # of its random numbers; None: any
+    adapter: int = -1               # -1: none
+    random: np.random.Generator | None = field(default=None, repr=False)
     generated: list[int] = field(default_factory=list)
     cached: int = 0                 # positions whose keys and values are in the cache
     pages: list[int] = field(default_factory=list)
+
+    def draw(self) -> float:
+        """The next of its random numbers in [0, 1), an fp32 value."""
+        if self.random is None:
+            self.random = np.random.default_rng(self.seed)
+        return self.random.random(dtype=np.float32)
 
     def pending(self) -> int:
         return len(self.prompt) + len(self.generated) - self.cached
@@ -150,11 +165,14 @@ class Sequences:
 
 
 class PagedServer:
-    """Greedy decoding of up to `max_seqs` sequences over a pool of `n_pages` pages per layer."""
+    """Decoding of up to `max_seqs` sequences, greedy or sampled, each with one of the `adapters` (:class:`AdapterSet`) or none, over
+    a pool of `n_pages` pages per layer."""
 
     def __init__(self, weights, n_pages: int, page_size: int = 64, max_seqs: int = 32, max_positions: int | None = None,
-                 chunk: int = 256, rope_kind: str = "plain", **rope):
+                 chunk: int = 256, rope_kind: str = "plain", adapters=None, **rope):
         import torch
+        if adapters is not None and adapters.shape != weights.shape:
+            raise ValueError("the adapters are for another model shape")
         self.torch, self.w, s = torch, weights, weights.shape
         self.shape = s
         max_pages = -(-(max_positions or s.max_position_embeddings) // page_size)
@@ -168,6 +186,9 @@ class PagedServer:
         # a step of decodes alone, and one with a chunk of a prompt: fixed numbers of rows, the last ones unused
         self.plans = {rows: PagedPlan(max_seqs, rows, q, *heads) for rows, q in ((max_seqs, 1), (max_seqs + chunk, chunk))}
         rows = max_seqs + chunk
+        self.adapters = adapters
+        if adapters is not None:
+            self.lora_plans = {n: LoraPlan(n, adapters.n_adapters) for n in self.plans}
 
         def rows_of(n, count=rows):
             return torch.zeros(count, n, dtype=torch.bfloat16, device="cuda")
@@ -175,12 +196,15 @@ class PagedServer:
         self.x, self.xb, self.act = rows_of(s.hidden_size), rows_of(s.hidden_size), rows_of(s.intermediate_size)
         self.q, self.att = rows_of(s.q_dim), rows_of(s.q_dim)
         self.k, self.v = rows_of(s.kv_dim), rows_of(s.kv_dim)
+        if adapters is not None:  # the feed-forward's taps, which the adapters change before the activation
+            self.gate, self.up = rows_of(s.intermediate_size), rows_of(s.intermediate_size)
         self.last = rows_of(s.hidden_size, max_seqs)
         self.logits = rows_of(s.vocab_size, max_seqs)
         self.out = torch.zeros(max_seqs, dtype=torch.int32, device="cuda")
 
     def add(self, prompt, **sampling) -> int:
-        """Takes a prompt in; sampling holds repetition, frequency, presence, bias and mask."""
+        """Takes a prompt in; sampling holds repetition, frequency, presence, bias and mask, temperature (0: the largest logit),
+        top_k, top_p, min_p and seed, and adapter."""
         prompt = [int(t) for t in prompt]
         if any(t < 0 or t >= self.shape.vocab_size for t in prompt):
             raise ValueError("a token id outside the vocabulary")
@@ -190,7 +214,14 @@ class PagedServer:
             if mask.ndim != 1 or len(mask) < words or mask.dtype.kind not in "iu":
                 raise ValueError(f"the mask must be {words} words of 32 bits")
             sampling["mask"] = mask[:words].astype(np.uint32).view(np.int32)
-        return self.seqs.add(Sequence(prompt, **sampling))
+        seq = Sequence(prompt, **sampling)
+        if not 0.0 <= seq.temperature < float("inf"):
+            raise ValueError("the temperature must be a finite number from 0 on")
+        if not 0 <= seq.top_k < 2 ** 31 or not 0.0 <= seq.top_p <= 1.0 or not 0.0 <= seq.min_p <= 1.0:
+            raise ValueError("top_k must be an int from 0 on, top_p and min_p within [0, 1]")
+        if seq.adapter != -1 and (self.adapters is None or seq.adapter not in self.adapters.loaded):
+            raise ValueError(f"there is no adapter {seq.adapter}")
+        return self.seqs.add(seq)
 
     def remove(self, i: int) -> None:
         self.seqs.remove(i)
@@ -208,7 +239,8 @@ class PagedServer:
         n = len(step.outputs)
         if n:
             self._pick([self.seqs.live[i] for _, i in step.outputs])
-        return self.seqs.commit(step, self.out[:n].tolist())
+        # where a mask leaves nothing the argmax takes token 0, and so does sampling
+        return self.seqs.commit(step, [max(t, 0) for t in self.out[:n].tolist()])
 
     def _device(self, values, dtype="int32"):
         return self.torch.from_numpy(np.asarray(values, dtype)).cuda(non_blocking=True)
@@ -233,6 +265,14 @@ class PagedServer:
         x, xb, q, k, v, att, act = (b[:rows] for b in (self.x, self.xb, self.q, self.k, self.v, self.att, self.act))
         px, pxb, pq, pk, pv, pa, pact = (b.data_ptr() for b in (x, xb, q, k, v, att, act))
         tokens = self._device(step.tokens + [0] * (rows - len(step.tokens)))
+        chosen = [seqs.live[i].adapter for i in step.ids]
+        lora = None
+        if any(a >= 0 for a in chosen):
+            lora, stacks = self.lora_plans[rows], self.adapters.stacks
+            index = np.full(rows, -1, np.int32)
+            index[:starts[-1]] = np.repeat(chosen, step.counts)
+            lora.update(self._device(index))
+            gate, up = self.gate[:rows], self.up[:rows]
         call("q3_embedding_batched", px, w.ptr["model.embed_tokens.weight"], tokens.data_ptr(), rows, H, s.vocab_size, stream)
         for l in range(s.num_hidden_layers):
             p = {n: w.ptr[f"model.layers.{l}.{n}.weight"] for n in (
@@ -242,13 +282,22 @@ class PagedServer:
             call("q3_rmsnorm_forward", pxb, px, p["input_layernorm"], rows, H, eps, stream)
             call("q3_qkv_batched", pq, pk, pv, p["self_attn.q_proj"], p["self_attn.k_proj"], p["self_attn.v_proj"], pxb,
                  rows, qd, kd, H, stream)
+            if lora:
+                lora_add([q, k, v], [q, k, v], xb, stacks["qkv"][l], lora)
             paged_rope_append(q, q, k, v, self.key_pages[l], self.value_pages[l], plan, self.inv_freq, norms[0], norms[1],
                               eps, amplitude=self.amplitude)
             paged_attention(att, q, self.key_pages[l], self.value_pages[l], plan)
             call("q3_gemv_residual_batched", px, p["self_attn.o_proj"], pa, rows, H, qd, None, stream)
+            if lora:
+                lora_add(x, x, att, stacks["o"][l], lora)
             call("q3_rmsnorm_forward", pxb, px, p["post_attention_layernorm"], rows, H, eps, stream)
-            call("q3_gate_up_batched", pact, p["mlp.gate_proj"], p["mlp.up_proj"], pxb, rows, I, H, None, None, stream)
+            taps = (gate.data_ptr(), up.data_ptr()) if lora else (None, None)
+            call("q3_gate_up_batched", pact, p["mlp.gate_proj"], p["mlp.up_proj"], pxb, rows, I, H, *taps, stream)
+            if lora:
+                lora_gate_up(act, gate, up, xb, stacks["gate_up"][l], lora)
             call("q3_gemv_residual_batched", px, p["mlp.down_proj"], pact, rows, H, I, None, stream)
+            if lora:
+                lora_add(x, x, act, stacks["down"][l], lora)
         n = len(step.outputs)
         if n:
             picked = self._device([row for row, _ in step.outputs])
@@ -259,7 +308,7 @@ class PagedServer:
             call("q3_gemv_batched", self.logits.data_ptr(), lm, last, n, s.vocab_size, H, stream)
 
     def _pick(self, seqs: list[Sequence]) -> None:
-        """Penalties, biases and masks on the logits, then the largest of each row into self.out."""
+        """Penalties, biases and masks on the logits, then each row's token into self.out."""
         n, words = len(seqs), (self.shape.vocab_size + 31) // 32
         start, split, ids, bias_start, bias_ids, bias = [0], [], [], [0], [], []
         for q in seqs:
@@ -283,5 +332,10 @@ class PagedServer:
         rows = self.logits[:n]
         if kw:
             logits_process(rows, rows, **kw)
-        call("q3_argmax_batched", self.out.data_ptr(), rows.data_ptr(), n, self.shape.vocab_size,
-             self.torch.cuda.current_stream().cuda_stream)
+        if any(q.temperature > 0.0 for q in seqs):
+            f32 = [self._device([getattr(q, name) for q in seqs], "float32") for name in ("temperature", "top_p", "min_p")]
+            u = self._device([q.draw() if q.temperature > 0.0 else 0.0 for q in seqs], "float32")
+            sample_logits(self.out[:n], rows, u, f32[0], self._device([q.top_k for q in seqs]), f32[1], f32[2])
+        else:
+            call("q3_argmax_batched", self.out.data_ptr(), rows.data_ptr(), n, self.shape.vocab_size,
+                 self.torch.cuda.current_stream().cuda_stream)
