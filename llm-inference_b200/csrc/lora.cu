@@ -179,7 +179,7 @@ __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float 
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4, each = a.wide / a.n_slices;
     const int steps = (a.k + 31) / 32, parts = C * LA_WARPS, p = rank_c * LA_WARPS + warp;
     const int s0 = (int)((long long)steps * p / parts), s1 = (int)((long long)steps * (p + 1) / parts);
-    const bf16 *x0 = a.x + (long long)row_s[min(g, rows - 1)] * a.x_stride, *x1 = a.x + (long long)row_s[min(g + 8, rows - 1)] * a.x_stride;
+    const bf16 *x0 = a.x + row_s[g] * a.x_stride, *x1 = a.x + row_s[g + 8] * a.x_stride;
     const int tiles_each = (r + 7) / 8, n_tiles = tiles_each * a.n_slices;
 #pragma unroll 1
     for (int n0 = 0; n0 < n_tiles; n0 += LA_PASS) {
@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
     const int adapter = head_s[0], rows = head_s[1];
     if (GATE_UP && adapter < 0) return;  // the whole cluster: act is right already
     if (tid >= LA_HEAD && tid < LA_HEAD + rows) row_s[tid - LA_HEAD] = mine;
+    if (tid >= LA_HEAD + rows && tid < LA_HEAD + ROWS) row_s[tid - LA_HEAD] = record[LA_HEAD + rows - 1];  // read there, never written
     int r = 0;
     float scale = 1.0f;
     if (adapter >= 0) {
@@ -438,50 +439,43 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
         }
     }
 
-    // ---- out: units of 32 columns and MT row tiles, a warp each. While one step of 32 of the rank is multiplied, the next
-    // one's B is on its way, and after a unit the next unit's base.
+    // ---- out: units of 32 columns, and of those MT row tiles, a warp each. While one step of 32 of the rank is multiplied, the
+    // next one's B is on its way, and after a unit the next unit's base. What lies past the columns or rows is loaded from the
+    // last ones and not written.
     constexpr int PAIR = GATE_UP ? 2 : 1;
-    const int k_steps = max(1, (r + 31) / 32), groups = (rows + 16 * MT - 1) / (16 * MT), items = units * groups;
+    const int k_steps = (r + 31) / 32, two = rows > 16 * MT, items = units << two;
+    const int end0 = (a.slice[0].n + 31) / 32, end1 = end0 + (a.slice[1].n + 31) / 32;
     struct Unit {
         int sl, n0, m0;
     };
     auto unit = [&](int i) {
-        Unit u = {0, i / groups, i % groups * MT};
-        if (!GATE_UP)
-            while (u.n0 >= (a.slice[u.sl].n + 31) / 32) u.n0 -= (a.slice[u.sl++].n + 31) / 32;
-        u.n0 *= 32;
-        return u;
+        const int at = i >> two, sl = GATE_UP ? 0 : (at >= end0) + (at >= end1);
+        return Unit{sl, 32 * (at - (sl == 0 ? 0 : sl == 1 ? end0 : end1)), two ? i % 2 * MT : 0};
     };
     uint4 b[4], base[PAIR][MT][2];
     auto load_b = [&](const Unit &u, int pr, int s) {
         const LoraSlice &c = a.slice[u.sl + pr];
-        const bf16 *from = c.b + (long long)adapter * c.n * a.rank + 32 * s + 8 * t;
+        const int k = 32 * s + 8 * t;
+        const bf16 *from = c.b + (long long)adapter * c.n * a.rank + (k < r ? k : 0);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int nn = u.n0 + 8 * (g / 2) + 2 * j + g % 2;
-            b[j] = make_uint4(0, 0, 0, 0);
-            if (nn < c.n && 32 * s + 8 * t < r) b[j] = __ldg(reinterpret_cast<const uint4 *>(from + (long long)nn * a.rank));
-        }
+        for (int j = 0; j < 4; j++)
+            b[j] = __ldg(reinterpret_cast<const uint4 *>(from + (long long)min(u.n0 + 8 * (g / 2) + 2 * j + g % 2, c.n - 1) * a.rank));
     };
     auto load_base = [&](const Unit &u) {  // a lane has eight neighbouring columns of rows g and g + 8 of each tile
-        const int col = u.n0 + 8 * t;
 #pragma unroll
         for (int pr = 0; pr < PAIR; pr++) {
             const LoraSlice &c = a.slice[u.sl + pr];
+            const bf16 *from = c.base + min(u.n0 + 8 * t, c.n - 8);
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    const int at = (u.m0 + m) * 16 + g + 8 * q;
-                    base[pr][m][q] = make_uint4(0, 0, 0, 0);
-                    if (at < rows && col < c.n) base[pr][m][q] = *reinterpret_cast<const uint4 *>(c.base + row_s[at] * c.base_stride + col);
-                }
+                for (int q = 0; q < 2; q++) base[pr][m][q] = *reinterpret_cast<const uint4 *>(from + row_s[(u.m0 + m) * 16 + g + 8 * q] * c.base_stride);
         }
     };
     int i = rank_c * WARPS + warp;
     Unit u = unit(min(i, items - 1));
     if (i < items) {
-        load_b(u, 0, 0);
+        if (r > 0) load_b(u, 0, 0);
         load_base(u);
     }
 #pragma unroll 1
@@ -492,33 +486,35 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
         for (int pr = 0; pr < PAIR; pr++)
 #pragma unroll 1
             for (int s = 0; s < k_steps; s++) {
-                uint4 now[4];
-                const int left = r - (32 * s + 8 * t);  // what is past the adapter's rank may be anything
-                auto keep = [&](int e) { return left > e + 1 ? 0xffffffffu : left > e ? 0xffffu : 0u; };
-                const uint32_t k0 = keep(0), k1 = keep(2), k2 = keep(4), k3 = keep(6);
+                uint4 now[4] = {b[0], b[1], b[2], b[3]};
+                const int left = r - (32 * s + 8 * t);
+                if (r - 32 * s < 32) {  // what is past the adapter's rank may be anything
+                    auto keep = [&](int e) { return left > e + 1 ? 0xffffffffu : left > e ? 0xffffu : 0u; };
 #pragma unroll
-                for (int j = 0; j < 4; j++) now[j] = make_uint4(b[j].x & k0, b[j].y & k1, b[j].z & k2, b[j].w & k3);
+                    for (int j = 0; j < 4; j++) now[j] = make_uint4(now[j].x & keep(0), now[j].y & keep(2), now[j].z & keep(4), now[j].w & keep(6));
+                }
                 if (s + 1 < k_steps) load_b(u, pr, s + 1);
                 else if (pr + 1 < PAIR) load_b(u, pr + 1, 0);
-                else if (i + C * WARPS < items) load_b(next, 0, 0);
-                if (r == 0) break;
+                else load_b(next, 0, 0);
+                const int at = (u.m0 * 16 + g) * pitch + (u.sl + pr) * each + 32 * s + 8 * t;
 #pragma unroll
                 for (int m = 0; m < MT; m++) {
-                    const int at = ((u.m0 + m) * 16 + g) * pitch + (u.sl + pr) * each + 32 * s + 8 * t;
 #pragma unroll
                     for (int part = 0; part < 2; part++) {
-                        const bf16 *from = (part ? lo : hi) + at;
+                        const bf16 *from = (part ? lo : hi) + at + m * 16 * pitch;
                         const uint4 v = *reinterpret_cast<const uint4 *>(from), w = *reinterpret_cast<const uint4 *>(from + 8 * pitch);
                         const uint32_t a0[4] = {v.x, w.x, v.y, w.y}, a1[4] = {v.z, w.z, v.w, w.w};
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            mma(acc[pr][m][j], a0, now[j].x, now[j].y);
-                            mma(acc[pr][m][j], a1, now[j].z, now[j].w);
-                        }
+                        for (int j = 0; j < 4; j++) mma(acc[pr][m][j], a0, now[j].x, now[j].y);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) mma(acc[pr][m][j], a1, now[j].z, now[j].w);
                     }
                 }
             }
         const int col = u.n0 + 8 * t;
+        const bool inside = col < a.slice[u.sl].n;
+        bf16 *to = (GATE_UP ? a.act : a.slice[u.sl].out) + col;
+        const long long to_stride = GATE_UP ? a.act_stride : a.slice[u.sl].out_stride;
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -540,10 +536,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
                     }
                 }
                 const uint4 out = r > 0 || GATE_UP ? make_uint4(y[0], y[1], y[2], y[3]) : base[0][m][q];
-                if (at < rows && col < a.slice[u.sl].n) {
-                    if constexpr (GATE_UP) *reinterpret_cast<uint4 *>(a.act + row_s[at] * a.act_stride + col) = out;
-                    else *reinterpret_cast<uint4 *>(a.slice[u.sl].out + row_s[at] * a.slice[u.sl].out_stride + col) = out;
-                }
+                if (inside && at < rows) *reinterpret_cast<uint4 *>(to + row_s[at] * to_stride) = out;
             }
         u = next;
         if (i + C * WARPS < items) load_base(u);
