@@ -231,95 +231,108 @@ __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float 
 
 // A x of a long tile, this CTA's part of k: x and A come through shared memory in stages of 64 elements of k (a row is 128 bytes,
 // its 16-byte lines exchanged by the row's lowest bits, so that the eight rows of a matrix lie in different banks), so
-// that each is read once; a warp has all rows and its share of the columns. From registers alone, with each
-// warp reading all of A for its rows, this part took 2079 rows of rank 64 three times as long.
-constexpr int LA_STAGES = 3, LA_KC = 64, LA_COLS = 192;  // columns at a time
+// that each is read once. Twelve warps have a pair of eight-column tiles each, for all rows; four load. From registers alone, with
+// each warp reading all of A for its rows, this part took 2079 rows of rank 64 three times as long, and with loads and products
+// taking turns in every warp, once and a half.
+constexpr int LA_STAGES = 4, LA_KC = 64, LA_COLS = 192;  // columns at a time
 constexpr int LA_STAGE_BYTES = (32 + LA_COLS) * LA_KC * 2;
+constexpr int LA_READERS = LA_COLS / 16, LA_LOADERS = LA_WARPS - LA_READERS;  // warps
 
-__device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigned char *ring, const int *row_s, int rows, int adapter, int r, int C,
-                                            int rank_c) {
-    constexpr int ROWS = 32, PAIRS = (LA_COLS / 16 + LA_WARPS - 1) / LA_WARPS;  // pairs of eight-column tiles of a warp
+// bars: full, then empty, of each stage
+__device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigned char *ring, uint64_t *bars, const int *row_s, int rows, int adapter,
+                                            int r, int C, int rank_c) {
+    constexpr int ROWS = 32;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, each = a.wide / a.n_slices;
     const int k16 = (a.k + 15) / 16, k0 = 16 * (int)((long long)k16 * rank_c / C), k1 = min(a.k, 16 * (int)((long long)k16 * (rank_c + 1) / C));
     const int chunks = (k1 - k0 + LA_KC - 1) / LA_KC;
     const int tiles_each = (r + 7) / 8, n_tiles = tiles_each * a.n_slices;
     const uint32_t ring_at = smem_u32(ring);
-#pragma unroll 1
-    for (int n0 = 0; n0 < n_tiles; n0 += LA_COLS / 8) {
-        const int cols = min(LA_COLS, (n_tiles - n0) * 8);
+    bool ok = true;  // no wait has given up: from then on nothing is loaded, nor waited for
+    int it = 0;      // chunks so far
+    if (warp >= LA_READERS) {
         // a thread copies one line of each of these rows: of x, then of A; null: zeros
-        constexpr int EACH = (ROWS + LA_COLS + LA_THREADS / 8 - 1) / (LA_THREADS / 8);
-        const int q_own = tid % 8;
-        const bf16 *from[EACH];
-#pragma unroll
-        for (int j = 0; j < EACH; j++) {
-            const int row = tid / 8 + j * (LA_THREADS / 8);
-            if (row < ROWS) {
-                from[j] = row < rows ? a.x + (long long)row_s[row] * a.x_stride : nullptr;
-            } else {
-                const int nt = n0 + (row - ROWS) / 8, sl = slice_of(nt, tiles_each), rr = (nt - sl * tiles_each) * 8 + (row - ROWS) % 8;
-                from[j] = nt < n_tiles && rr < r ? a.slice[sl].a + ((long long)adapter * a.rank + rr) * a.k : nullptr;
-            }
-        }
-        auto stage = [&](int c) {
-            const uint32_t to = ring_at + c % LA_STAGES * LA_STAGE_BYTES;
-            const int k = k0 + c * LA_KC + 8 * q_own;
+        constexpr int STEP = LA_LOADERS * 4, EACH = (ROWS + LA_COLS) / STEP;
+        const int row0 = (tid - 32 * LA_READERS) / 8, q = tid % 8;
+#pragma unroll 1
+        for (int n0 = 0; n0 < n_tiles; n0 += LA_COLS / 8) {
+            const int all = ROWS + min(LA_COLS, (n_tiles - n0) * 8);
+            const bf16 *from[EACH];
 #pragma unroll
             for (int j = 0; j < EACH; j++) {
-                const int row = tid / 8 + j * (LA_THREADS / 8);
-                const bool in = from[j] && c < chunks && k < k1;
-                if (row < ROWS + cols) copy16(to + row * (LA_KC * 2) + ((q_own ^ (row & 7)) << 4), in ? from[j] + k : a.x, in);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        float acc[2][2 * PAIRS][4] = {};
-        for (int c = 0; c < LA_STAGES - 1; c++) stage(c);
-#pragma unroll 1
-        for (int c = 0; c < chunks; c++) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(LA_STAGES - 2) : "memory");
-            __syncthreads();  // this chunk is there; the one before is read
-            stage(c + LA_STAGES - 1);
-            const uint32_t x_at = ring_at + c % LA_STAGES * LA_STAGE_BYTES, w_at = x_at + ROWS * LA_KC * 2;
-#pragma unroll
-            for (int s = 0; s < LA_KC / 16; s++) {
-                uint32_t am[2][4];
-#pragma unroll
-                for (int m = 0; m < 2; m++) {
-                    const int row = m * 16 + lane % 16, q = 2 * s + lane / 16;
-                    load_matrices(am[m], x_at + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4));
+                const int row = row0 + j * STEP;
+                if (row < ROWS) {
+                    from[j] = row < rows ? a.x + row_s[row] * a.x_stride : nullptr;
+                } else {
+                    const int nt = n0 + (row - ROWS) / 8, sl = slice_of(nt, tiles_each), rr = (nt - sl * tiles_each) * 8 + (row - ROWS) % 8;
+                    from[j] = nt < n_tiles && rr < r ? a.slice[sl].a + ((long long)adapter * a.rank + rr) * a.k : nullptr;
                 }
+            }
+#pragma unroll 1
+            for (int c = 0; c < chunks; c++, it++) {
+                const int st = it % LA_STAGES;
+                if (it >= LA_STAGES && ok) ok = mbar_wait(bars + LA_STAGES + st, (it / LA_STAGES - 1) & 1, &g_dev_error);
+                if (!ok) continue;
+                const uint32_t to = ring_at + st * LA_STAGE_BYTES;
+                const int k = k0 + c * LA_KC + 8 * q;
 #pragma unroll
-                for (int j = 0; j < PAIRS; j++) {
-                    const int pair = warp + j * LA_WARPS;
-                    if (16 * pair < cols) {
-                        uint32_t bm[4];
-                        const int row = pair * 16 + lane / 16 * 8 + lane % 8, q = 2 * s + lane / 8 % 2;
+                for (int j = 0; j < EACH; j++) {
+                    const int row = row0 + j * STEP;
+                    const bool in = from[j] && k < k1;
+                    if (row < all) copy16(to + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4), in ? from[j] + k : a.x, in);
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bars + st)) : "memory");
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+#pragma unroll 1
+        for (int n0 = 0; n0 < n_tiles; n0 += LA_COLS / 8) {
+            const int cols = min(LA_COLS, (n_tiles - n0) * 8);
+            float acc[2][2][4] = {};
+#pragma unroll 1
+            for (int c = 0; c < chunks; c++, it++) {
+                const int st = it % LA_STAGES;
+                if (ok) ok = mbar_wait(bars + st, it / LA_STAGES & 1, &g_dev_error);
+                if (16 * warp < cols) {
+                    const uint32_t x_at = ring_at + st * LA_STAGE_BYTES, w_at = x_at + ROWS * LA_KC * 2;
+#pragma unroll
+                    for (int s = 0; s < LA_KC / 16; s++) {
+                        uint32_t am[2][4], bm[4];
+#pragma unroll
+                        for (int m = 0; m < 2; m++) {
+                            const int row = m * 16 + lane % 16, q = 2 * s + lane / 16;
+                            load_matrices(am[m], x_at + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4));
+                        }
+                        const int row = warp * 16 + lane / 16 * 8 + lane % 8, q = 2 * s + lane / 8 % 2;
                         load_matrices(bm, w_at + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4));
 #pragma unroll
                         for (int m = 0; m < 2; m++) {
-                            mma(acc[m][2 * j], am[m], bm[0], bm[1]);
-                            mma(acc[m][2 * j + 1], am[m], bm[2], bm[3]);
+                            mma(acc[m][0], am[m], bm[0], bm[1]);
+                            mma(acc[m][1], am[m], bm[2], bm[3]);
                         }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0 && ok) mbar_arrive(bars + LA_STAGES + st);
+            }
+            // h may be where the ring is, if this is the only pass
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * LA_READERS) : "memory");
+            const int g = lane / 4, t = lane % 4;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int nt = n0 + 2 * warp + j, sl = slice_of(nt, tiles_each);
+                if (8 * (nt - n0) < cols) {
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        float *to = h + (m * 16 + g) * a.wide + sl * each + (nt - sl * tiles_each) * 8 + 2 * t;
+                        *reinterpret_cast<float2 *>(to) = make_float2(acc[m][j][0], acc[m][j][1]);
+                        *reinterpret_cast<float2 *>(to + 8 * a.wide) = make_float2(acc[m][j][2], acc[m][j][3]);
                     }
                 }
             }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncthreads();  // the ring may be where h is
-        const int g = lane / 4, t = lane % 4;
-#pragma unroll
-        for (int j = 0; j < 2 * PAIRS; j++) {
-            const int nt = n0 + 2 * (warp + j / 2 * LA_WARPS) + j % 2, sl = slice_of(nt, tiles_each);
-            if (8 * (nt - n0) >= cols) continue;
-#pragma unroll
-            for (int m = 0; m < 2; m++) {
-                float *to = h + (m * 16 + g) * a.wide + sl * each + (nt - sl * tiles_each) * 8 + 2 * t;
-                *reinterpret_cast<float2 *>(to) = make_float2(acc[m][j][0], acc[m][j][1]);
-                *reinterpret_cast<float2 *>(to + 8 * a.wide) = make_float2(acc[m][j][2], acc[m][j][3]);
-            }
-        }
-        __syncthreads();
     }
+    __syncthreads();
 }
 
 // GATE_UP: slices 0 and 1 are gate and up, and what is written is silu(gate) * up.
@@ -331,13 +344,21 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
     const int C = cluster.num_blocks(), rank_c = cluster.block_rank(), tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const int g = lane / 4, t = lane % 4;
     const int wide = a.wide, pitch = a.pitch, each = wide / a.n_slices;
-    int *row_s = reinterpret_cast<int *>(la_smem), *head_s = row_s + ROWS;  // [ROWS], [LA_HEAD]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(la_smem);                 // [2 LA_STAGES]
+    int *row_s = reinterpret_cast<int *>(bars + 2 * LA_STAGES), *head_s = row_s + ROWS;  // [ROWS], [LA_HEAD]
     float *h = reinterpret_cast<float *>(head_s + LA_HEAD);                 // [ROWS][wide]: this CTA's part of A x
     // [ROWS][pitch]: A x, scaled, upper and lower bits; before that the first product's buffers, those of a long tile over h,
     // too, if that is written once
     unsigned char *rest = reinterpret_cast<unsigned char *>(h + ROWS * wide);
     bf16 *hi = reinterpret_cast<bf16 *>(rest), *lo = hi + ROWS * pitch;
 
+    if (ROWS > 16 && tid == 0) {
+        for (int st = 0; st < LA_STAGES; st++) {
+            mbar_init(bars + st, 32 * LA_LOADERS);
+            mbar_init(bars + LA_STAGES + st, LA_READERS);
+        }
+        fence_barrier_init();
+    }
     pdl_trigger();
     pdl_wait();
     const int tile = blockIdx.x / C;
@@ -380,7 +401,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
             }
             shrink_short(a, h, reinterpret_cast<float *>(rest), row_s, rows, adapter, r, C, rank_c);
         } else {
-            shrink_long(a, h, wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest, row_s, rows, adapter, r, C, rank_c);
+            shrink_long(a, h, wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest, bars, row_s, rows, adapter, r, C, rank_c);
         }
         // the CTAs' parts, in their order. Few: each CTA adds up all of them; more: each some of the columns for all.
         if (C > 1) cluster.sync();
@@ -553,7 +574,7 @@ size_t lora_smem(int wide) {
     const size_t h = (size_t)ROWS * wide * 4, both = h + 2 * (size_t)ROWS * pitch_of(wide) * 2;
     const size_t first = ROWS == 16 ? h + (size_t)LA_WARPS * 16 * 8 * LA_PASS * 4
                                     : (wide <= LA_COLS ? 0 : h) + (size_t)LA_STAGES * LA_STAGE_BYTES;
-    return (size_t)(ROWS + LA_HEAD) * 4 + std::max(first, both);
+    return 2 * LA_STAGES * 8 + (size_t)(ROWS + LA_HEAD) * 4 + std::max(first, both);
 }
 
 // Whether two matrices of as many rows share any element.
