@@ -19,6 +19,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "waiter.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -238,17 +239,17 @@ constexpr int LA_STAGES = 4, LA_KC = 64, LA_COLS = 192;  // columns at a time
 constexpr int LA_STAGE_BYTES = (32 + LA_COLS) * LA_KC * 2;
 constexpr int LA_READERS = LA_COLS / 16, LA_LOADERS = LA_WARPS - LA_READERS;  // warps
 
-// bars: full, then empty, of each stage
-__device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigned char *ring, uint64_t *bars, const int *row_s, int rows, int adapter,
-                                            int r, int C, int rank_c) {
+// bars: full, then empty, of each stage; down: zero, set when a wait has given up
+__device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigned char *ring, uint64_t *bars, int *down, const int *row_s, int rows,
+                                            int adapter, int r, int C, int rank_c) {
     constexpr int ROWS = 32;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, each = a.wide / a.n_slices;
     const int k16 = (a.k + 15) / 16, k0 = 16 * (int)((long long)k16 * rank_c / C), k1 = min(a.k, 16 * (int)((long long)k16 * (rank_c + 1) / C));
     const int chunks = (k1 - k0 + LA_KC - 1) / LA_KC;
     const int tiles_each = (r + 7) / 8, n_tiles = tiles_each * a.n_slices;
     const uint32_t ring_at = smem_u32(ring);
-    bool ok = true;  // no wait has given up: from then on nothing is loaded, nor waited for
-    int it = 0;      // chunks so far
+    Waiter wait(&g_dev_error, down);
+    int it = 0;  // chunks so far
     if (warp >= LA_READERS) {
         // a thread copies one line of each of these rows: of x, then of A; null: zeros
         constexpr int STEP = LA_LOADERS * 4, EACH = (ROWS + LA_COLS) / STEP;
@@ -270,8 +271,8 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigne
 #pragma unroll 1
             for (int c = 0; c < chunks; c++, it++) {
                 const int st = it % LA_STAGES;
-                if (it >= LA_STAGES && ok) ok = mbar_wait(bars + LA_STAGES + st, (it / LA_STAGES - 1) & 1, &g_dev_error);
-                if (!ok) continue;
+                if (it >= LA_STAGES) wait(bars + LA_STAGES + st, (it / LA_STAGES - 1) & 1);
+                if (wait.dead) continue;  // readers that gave up release no stages, so that the loaders starve and give up in turn
                 const uint32_t to = ring_at + st * LA_STAGE_BYTES;
                 const int k = k0 + c * LA_KC + 8 * q;
 #pragma unroll
@@ -292,7 +293,7 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigne
 #pragma unroll 1
             for (int c = 0; c < chunks; c++, it++) {
                 const int st = it % LA_STAGES;
-                if (ok) ok = mbar_wait(bars + st, it / LA_STAGES & 1, &g_dev_error);
+                wait(bars + st, it / LA_STAGES & 1);
                 if (16 * warp < cols) {
                     const uint32_t x_at = ring_at + st * LA_STAGE_BYTES, w_at = x_at + ROWS * LA_KC * 2;
 #pragma unroll
@@ -313,7 +314,7 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigne
                     }
                 }
                 __syncwarp();
-                if (lane == 0 && ok) mbar_arrive(bars + LA_STAGES + st);
+                if (lane == 0 && !wait.dead) mbar_arrive(bars + LA_STAGES + st);
             }
             // h may be where the ring is, if this is the only pass
             asm volatile("bar.sync 1, %0;" ::"n"(32 * LA_READERS) : "memory");
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
     const int n_plan = *reinterpret_cast<const int *>(a.plan);
     const int mine = tid < LA_HEAD + ROWS ? record[tid] : 0;  // past the rows of a tile, or the tiles: anything
     if (tile >= n_plan) return;  // the whole cluster
-    if (tid < LA_HEAD) head_s[tid] = mine;
+    if (tid < LA_HEAD) head_s[tid] = tid < 2 ? mine : 0;
     __syncthreads();
     const int adapter = head_s[0], rows = head_s[1];
     if (GATE_UP && adapter < 0) return;  // the whole cluster: act is right already
@@ -401,12 +402,12 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
             }
             shrink_short(a, h, reinterpret_cast<float *>(rest), row_s, rows, adapter, r, C, rank_c);
         } else {
-            shrink_long(a, h, wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest, bars, row_s, rows, adapter, r, C, rank_c);
+            shrink_long(a, h, wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest, bars, head_s + LA_HEAD - 1, row_s, rows, adapter, r, C, rank_c);
         }
         // the CTAs' parts, in their order. Few: each CTA adds up all of them; more: each some of the columns for all.
         if (C > 1) cluster.sync();
         const int octets = rows * wide / 8;
-        const bool all = octets <= THREADS;
+        const bool all = octets * C <= 512;  // remote shared memory gives some 9 bytes a cycle: 2000 cycles
         const int q0 = all ? 0 : (int)((long long)octets * rank_c / C), q1 = all ? octets : (int)((long long)octets * (rank_c + 1) / C);
         for (int q = q0 + tid; q < q1; q += THREADS) {
             const int row = 8 * q / wide, col = 8 * q % wide, left = r - col % each;  // of the adapter's rank from here
@@ -418,17 +419,18 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
 #pragma unroll
                     for (int c = 0; c < 4; c++)
 #pragma unroll
-                        for (int half = 0; half < 2; half++)
-                            f[c][half] = *reinterpret_cast<const float4 *>((C > 1 ? cluster.map_shared_rank(h, min(c0 + c, C - 1)) : h) + 8 * q + 4 * half);
+                        for (int half = 0; half < 2; half++) {
+                            f[c][half] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (c0 + c < C) f[c][half] = *reinterpret_cast<const float4 *>((C > 1 ? cluster.map_shared_rank(h, c0 + c) : h) + 8 * q + 4 * half);
+                        }
 #pragma unroll
                     for (int c = 0; c < 4; c++)
 #pragma unroll
                         for (int half = 0; half < 2; half++) {
-                            const bool in = c0 + c < C;
-                            v[4 * half] += in ? f[c][half].x : 0.0f;
-                            v[4 * half + 1] += in ? f[c][half].y : 0.0f;
-                            v[4 * half + 2] += in ? f[c][half].z : 0.0f;
-                            v[4 * half + 3] += in ? f[c][half].w : 0.0f;
+                            v[4 * half] += f[c][half].x;
+                            v[4 * half + 1] += f[c][half].y;
+                            v[4 * half + 2] += f[c][half].z;
+                            v[4 * half + 3] += f[c][half].w;
                         }
                 }
             }
