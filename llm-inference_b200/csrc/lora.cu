@@ -35,7 +35,6 @@ constexpr int LA_MAX_ADAPTERS = 8192;
 constexpr int LA_MAX_RANK = 128;
 constexpr int LA_MAX_SLICES = 3;
 constexpr int LA_MAX_CLUSTER = 8;
-constexpr int LA_PASS = 8;  // eight-column tiles of A x at a time: their sums stay in registers
 
 // A tile's record: the adapter (-1: rows without one), how many rows, two unused, and the rows.
 constexpr int LA_HEAD = 4;
@@ -175,19 +174,23 @@ constexpr int LA_WARPS = LA_THREADS / 32;
 
 // A x of a short tile, this CTA's part of k: each warp a part of that for all columns, operands from global memory straight into
 // registers, then the warps' parts added up in their order.
+// PASS: eight-column tiles at a time, whose sums stay in registers; the kernel is built for 2, 4, 6 and 12, and takes the least that holds
+// all: code for more that is stepped over costs 64 rows through the down projection 12.7 -> 15.3 us, a second pass 32 rows through q, k
+// and v 11.9 -> 12.5.
+template <int PASS>
 __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float *part, const int *row_s, int rows, int adapter, int r, int C, int rank_c) {
-    constexpr int COLS = 8 * LA_PASS;
+    constexpr int COLS = 8 * PASS;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4, each = a.wide / a.n_slices;
     const int steps = (a.k + 31) / 32, parts = C * LA_WARPS, p = rank_c * LA_WARPS + warp;
     const int s0 = (int)((long long)steps * p / parts), s1 = (int)((long long)steps * (p + 1) / parts);
     const bf16 *x0 = a.x + row_s[g] * a.x_stride, *x1 = a.x + row_s[g + 8] * a.x_stride;
     const int tiles_each = (r + 7) / 8, n_tiles = tiles_each * a.n_slices;
 #pragma unroll 1
-    for (int n0 = 0; n0 < n_tiles; n0 += LA_PASS) {
-        float acc[LA_PASS][4] = {};
-        const bf16 *w[LA_PASS];
+    for (int n0 = 0; n0 < n_tiles; n0 += PASS) {
+        float acc[PASS][4] = {};
+        const bf16 *w[PASS];
 #pragma unroll
-        for (int j = 0; j < LA_PASS; j++) {
+        for (int j = 0; j < PASS; j++) {
             const int nt = n0 + j, sl = slice_of(nt, tiles_each), row = (nt - sl * tiles_each) * 8 + g;
             w[j] = nt < n_tiles && row < r ? a.slice[sl].a + ((long long)adapter * a.rank + row) * a.k : nullptr;
         }
@@ -197,12 +200,12 @@ __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float 
             const uint4 zero = make_uint4(0, 0, 0, 0);
             const bool in = k < a.k;
             const uint4 u = in ? __ldg(reinterpret_cast<const uint4 *>(x0 + k)) : zero, v = in ? __ldg(reinterpret_cast<const uint4 *>(x1 + k)) : zero;
-            uint4 b[LA_PASS];
+            uint4 b[PASS];
 #pragma unroll
-            for (int j = 0; j < LA_PASS; j++) b[j] = in && w[j] ? __ldg(reinterpret_cast<const uint4 *>(w[j] + k)) : zero;
+            for (int j = 0; j < PASS; j++) b[j] = in && w[j] ? __ldg(reinterpret_cast<const uint4 *>(w[j] + k)) : zero;
             const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
 #pragma unroll
-            for (int j = 0; j < LA_PASS; j++)
+            for (int j = 0; j < PASS; j++)
                 if (n0 + j < n_tiles) {
                     mma(acc[j], a0, b[j].x, b[j].y);
                     mma(acc[j], a1, b[j].z, b[j].w);
@@ -210,7 +213,7 @@ __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float 
         }
         float *own = part + warp * 16 * COLS;
 #pragma unroll
-        for (int j = 0; j < LA_PASS; j++) {
+        for (int j = 0; j < PASS; j++) {
             *reinterpret_cast<float2 *>(own + g * COLS + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
             *reinterpret_cast<float2 *>(own + (g + 8) * COLS + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
         }
@@ -336,8 +339,8 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigne
     __syncthreads();
 }
 
-// GATE_UP: slices 0 and 1 are gate and up, and what is written is silu(gate) * up.
-template <int ROWS, bool GATE_UP>
+// GATE_UP: slices 0 and 1 are gate and up, and what is written is silu(gate) * up. PASS: of a short tile.
+template <int ROWS, bool GATE_UP, int PASS>
 __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_constant__ LoraArgs a) {
     constexpr int THREADS = LA_THREADS, WARPS = LA_WARPS, MT = ROWS == 16 || GATE_UP ? 1 : 2;  // MT: 16-row tiles of a warp in the second product
     extern __shared__ __align__(16) unsigned char la_smem[];
@@ -400,7 +403,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
                 for (int pr = 0; pr < (GATE_UP ? 2 : 1); pr++)
                     if (n0 < a.slice[sl].n) prefetch_l2(a.slice[sl + pr].b + ((long long)adapter * a.slice[sl].n + n0) * a.rank);
             }
-            shrink_short(a, h, reinterpret_cast<float *>(rest), row_s, rows, adapter, r, C, rank_c);
+            shrink_short<PASS>(a, h, reinterpret_cast<float *>(rest), row_s, rows, adapter, r, C, rank_c);
         } else {
             shrink_long(a, h, wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest, bars, head_s + LA_HEAD - 1, row_s, rows, adapter, r, C, rank_c);
         }
@@ -571,10 +574,10 @@ int wide_of(int n_slices, int rank) { return n_slices * ((rank + 31) / 32 * 32);
 
 int pitch_of(int wide) { return wide / 32 % 2 ? wide : wide + 32; }
 
-template <int ROWS>
+template <int ROWS, int PASS>
 size_t lora_smem(int wide) {
     const size_t h = (size_t)ROWS * wide * 4, both = h + 2 * (size_t)ROWS * pitch_of(wide) * 2;
-    const size_t first = ROWS == 16 ? h + (size_t)LA_WARPS * 16 * 8 * LA_PASS * 4
+    const size_t first = ROWS == 16 ? h + (size_t)LA_WARPS * 16 * 8 * PASS * 4
                                     : (wide <= LA_COLS ? 0 : h) + (size_t)LA_STAGES * LA_STAGE_BYTES;
     return 2 * LA_STAGES * 8 + (size_t)(ROWS + LA_HEAD) * 4 + std::max(first, both);
 }
@@ -592,10 +595,10 @@ bool overlap(const void *a, long long a_stride, int a_width, const void *b, long
     return d < 2LL * a_width || d + 2LL * b_width > s;
 }
 
-template <int ROWS, bool GATE_UP>
+template <int ROWS, bool GATE_UP, int PASS>
 int launch_lora(const LoraArgs &args, int tiles, cudaStream_t s) {
-    auto kernel = lora_kernel<ROWS, GATE_UP>;
-    const size_t smem = lora_smem<ROWS>(args.wide);
+    auto kernel = lora_kernel<ROWS, GATE_UP, PASS>;
+    const size_t smem = lora_smem<ROWS, PASS>(args.wide);
     cudaError_t e = allow_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return record_cuda_error(e);
     // CTAs of a tile: as many as the SMs hold at once for as many tiles as there would be if each row took an adapter at random
@@ -606,9 +609,14 @@ int launch_lora(const LoraArgs &args, int tiles, cudaStream_t s) {
     Q3_TRY_LAUNCH(launch(kernel, dim3((unsigned)tiles * cluster), dim3(LA_THREADS), smem, s, cluster, args));
     return Q3_OK;
 }
-template <int ROWS>
-int launch_lora(const LoraArgs &args, int tiles, bool gate_up, cudaStream_t s) {
-    return gate_up ? launch_lora<ROWS, true>(args, tiles, s) : launch_lora<ROWS, false>(args, tiles, s);
+template <bool GATE_UP>
+int launch_lora(const LoraArgs &args, int tiles, cudaStream_t s) {
+    if (lora_tile_rows(args.n_rows) == 32) return launch_lora<32, GATE_UP, 0>(args, tiles, s);
+    const int columns = args.n_slices * args.rank;
+    if (columns <= 16) return launch_lora<16, GATE_UP, 2>(args, tiles, s);
+    if (columns <= 32) return launch_lora<16, GATE_UP, 4>(args, tiles, s);
+    if (columns <= 48) return launch_lora<16, GATE_UP, 6>(args, tiles, s);
+    return launch_lora<16, GATE_UP, 12>(args, tiles, s);
 }
 
 int plan_check(int n_rows, int n_adapters) {
@@ -668,7 +676,7 @@ int lora(const q3_lora_slice *slices, int n_slices, const q3_lora *l, bool gate_
     a.pitch = pitch_of(a.wide);
     const int tiles = lora_plan_layout(l->n_rows, l->n_adapters).max_tiles;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return lora_tile_rows(l->n_rows) == 16 ? launch_lora<16>(a, tiles, gate_up, s) : launch_lora<32>(a, tiles, gate_up, s);
+    return gate_up ? launch_lora<true>(a, tiles, s) : launch_lora<false>(a, tiles, s);
 }
 
 }  // namespace
