@@ -177,8 +177,10 @@ constexpr int LA_WARPS = LA_THREADS / 32;
 // PASS: eight-column tiles at a time, whose sums stay in registers; the kernel is built for 2, 4, 6 and 12, and takes the least that holds
 // all: code for more that is stepped over costs 64 rows through the down projection 12.7 -> 15.3 us, a second pass 32 rows through q, k
 // and v 11.9 -> 12.5.
-template <int PASS>
-__device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float *part, const int *row_s, int rows, int adapter, int r, int C, int rank_c) {
+// meanwhile() runs once, while the first loads are on their way.
+template <int PASS, typename F>
+__device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float *part, const int *row_s, int rows, int adapter, int r, int C, int rank_c,
+                                             F meanwhile) {
     constexpr int COLS = 8 * PASS;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4, each = a.wide / a.n_slices;
     const int steps = (a.k + 31) / 32, parts = C * LA_WARPS, p = rank_c * LA_WARPS + warp;
@@ -194,15 +196,20 @@ __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float 
             const int nt = n0 + j, sl = slice_of(nt, tiles_each), row = (nt - sl * tiles_each) * 8 + g;
             w[j] = nt < n_tiles && row < r ? a.slice[sl].a + ((long long)adapter * a.rank + row) * a.k : nullptr;
         }
-#pragma unroll 1
-        for (int s = s0; s < s1; s++) {
+        uint4 u, v, b[PASS];
+        auto load = [&](int s) {
             const int k = 32 * s + 8 * t;
             const uint4 zero = make_uint4(0, 0, 0, 0);
-            const bool in = k < a.k;
-            const uint4 u = in ? __ldg(reinterpret_cast<const uint4 *>(x0 + k)) : zero, v = in ? __ldg(reinterpret_cast<const uint4 *>(x1 + k)) : zero;
-            uint4 b[PASS];
+            const bool in = s < s1 && k < a.k;
+            u = in ? __ldg(reinterpret_cast<const uint4 *>(x0 + k)) : zero;
+            v = in ? __ldg(reinterpret_cast<const uint4 *>(x1 + k)) : zero;
 #pragma unroll
             for (int j = 0; j < PASS; j++) b[j] = in && w[j] ? __ldg(reinterpret_cast<const uint4 *>(w[j] + k)) : zero;
+        };
+        load(s0);
+        if (n0 == 0) meanwhile();
+#pragma unroll 1
+        for (int s = s0; s < s1; s++) {
             const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
 #pragma unroll
             for (int j = 0; j < PASS; j++)
@@ -210,6 +217,7 @@ __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float 
                     mma(acc[j], a0, b[j].x, b[j].y);
                     mma(acc[j], a1, b[j].z, b[j].w);
                 }
+            load(s + 1);
         }
         float *own = part + warp * 16 * COLS;
 #pragma unroll
@@ -394,16 +402,17 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
     bool waiting = false;
     if (r > 0) {
         if constexpr (ROWS == 16) {
-            // what the second product will read is asked for before the first
-            for (int u = rank_c * WARPS + warp; u < units; u += C * WARPS) {
-                int sl = 0, n0 = u;
-                if (!GATE_UP)
-                    while (n0 >= (a.slice[sl].n + 31) / 32) n0 -= (a.slice[sl++].n + 31) / 32;
-                n0 = 32 * n0 + lane;
-                for (int pr = 0; pr < (GATE_UP ? 2 : 1); pr++)
-                    if (n0 < a.slice[sl].n) prefetch_l2(a.slice[sl + pr].b + ((long long)adapter * a.slice[sl].n + n0) * a.rank);
-            }
-            shrink_short<PASS>(a, h, reinterpret_cast<float *>(rest), row_s, rows, adapter, r, C, rank_c);
+            auto ask = [&] {  // for what the second product will read
+                for (int u = rank_c * WARPS + warp; u < units; u += C * WARPS) {
+                    int sl = 0, n0 = u;
+                    if (!GATE_UP)
+                        while (n0 >= (a.slice[sl].n + 31) / 32) n0 -= (a.slice[sl++].n + 31) / 32;
+                    n0 = 32 * n0 + lane;
+                    for (int pr = 0; pr < (GATE_UP ? 2 : 1); pr++)
+                        if (n0 < a.slice[sl].n) prefetch_l2(a.slice[sl + pr].b + ((long long)adapter * a.slice[sl].n + n0) * a.rank);
+                }
+            };
+            shrink_short<PASS>(a, h, reinterpret_cast<float *>(rest), row_s, rows, adapter, r, C, rank_c, ask);
         } else {
             shrink_long(a, h, wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest, bars, head_s + LA_HEAD - 1, row_s, rows, adapter, r, C, rank_c);
         }
@@ -415,19 +424,20 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
         for (int q = q0 + tid; q < q1; q += THREADS) {
             const int row = 8 * q / wide, col = 8 * q % wide, left = r - col % each;  // of the adapter's rank from here
             float v[8] = {};
+            constexpr int AT_ONCE = ROWS == 16 ? LA_MAX_CLUSTER : 4;
             if (left > 0) {
 #pragma unroll 1
-                for (int c0 = 0; c0 < C; c0 += 4) {
-                    float4 f[4][2];  // all loads before the first sum
+                for (int c0 = 0; c0 < C; c0 += AT_ONCE) {
+                    float4 f[AT_ONCE][2];  // all loads before the first sum
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
+                    for (int c = 0; c < AT_ONCE; c++)
 #pragma unroll
                         for (int half = 0; half < 2; half++) {
                             f[c][half] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                             if (c0 + c < C) f[c][half] = *reinterpret_cast<const float4 *>((C > 1 ? cluster.map_shared_rank(h, c0 + c) : h) + 8 * q + 4 * half);
                         }
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
+                    for (int c = 0; c < AT_ONCE; c++)
 #pragma unroll
                         for (int half = 0; half < 2; half++) {
                             v[4 * half] += f[c][half].x;
