@@ -322,3 +322,38 @@ def test_no_rows():
     plan.update(torch.zeros(0, dtype=torch.int32, device="cuda"))
     none = torch.zeros(0, 8, dtype=BF16, device="cuda")
     q3.lora_add(none, none, c.x[:0], c.stack, plan)
+
+
+def test_two_calls_at_once():
+    c = Case(150, 512, [256, 128], 16, 6, some(150, 6))
+    want = c.add()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [[[torch.empty_like(t) for t in c.base] for _ in range(6)] for _ in streams]
+    torch.cuda.synchronize()
+    for n in range(6):
+        for s, out in zip(streams, outs):  # one plan and one stack, read by all
+            with torch.cuda.stream(s):
+                q3.lora_add(out[n], c.base, c.x, c.stack, c.plan)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for out in outs for o in out for a, b in zip(o, want))
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_rows_far_apart(rows):
+    # offsets past 32 bits: x and out are rows of a wide buffer
+    stride = (1 << 31) // rows // 8 * 8 + 64
+    c = Case(rows, 64, [32], 16, 3, some(rows, 3))
+    want = c.add()[0]
+    buf = torch.empty(rows * stride, dtype=BF16, device="cuda")
+    x = buf.as_strided((rows, 64), (stride, 1))
+    out = buf.as_strided((rows, 32), (stride, 1), 64)
+    x.copy_(c.x)
+    q3.lora_add(out, c.base[0], x, c.stack, c.plan)
+    assert torch.equal(out, want)
+
+
+def test_long_steps():
+    c = Case(65536, 16, [8], 8, 100, [int(v) for v in np.random.default_rng(2).integers(-1, 100, 65536)])
+    c.add()
+    one = Case(5000, 64, [72], 128, 2, [1] * 5000)
+    one.add()

@@ -308,3 +308,38 @@ def test_the_largest_vocabularies():
         x = torch.from_numpy(g.normal(0, 2, (2, vocab)).astype(np.float32)).cuda().to(dtype)
         run(x, f32(0.3, 0.9))
         run(x, f32(0.3, 0.9), k=i32(1000, 0), p=f32(0.5, 0.9))
+
+
+@pytest.mark.parametrize("scale,shift,t", [(200.0, 0.0, 40.0), (3.0, 500.0, 1.0), (3.0, -500.0, 0.8), (1e-11, 0.0, 1e-11), (1e-11, 3.0, 1.0),
+                                           (1e30, 0.0, 3e29), (1e-38, 0.0, 1e-38), (3.0, 0.0, 1.0)])
+def test_bf16_rows_of_any_magnitude(scale, shift, t):
+    # most rows' logits lie where bf16 values are counted one by one; these are beside it, around it and across its borders
+    g = np.random.default_rng(8)
+    vocab = 6007
+    x = torch.from_numpy((g.normal(0, 1, (12, vocab)) * scale + shift).astype(np.float32)).cuda()
+    x[1::3, ::7] = -3e38
+    x[2::3, ::5] = 0.0
+    x[3::4, 11] = 2.0 ** -32 * 0.75
+    x = x.to(torch.bfloat16)
+    _, k, p, m, d = settings(12, vocab, g)
+    for u in (f32(*g.random(12)), f32(*[0.0] * 12)):
+        run(x, u, f32(*[t] * 12))
+        run(x, u, f32(*[t] * 12), k, p, m, d)
+        run(x, u, f32(*[0.0] * 12))
+
+
+def test_two_calls_at_once():
+    g = np.random.default_rng(9)
+    x = torch.from_numpy(g.normal(0, 2, (6, 50021)).astype(np.float32)).cuda()
+    t, k, p, m, d = settings(6, 50021, g)
+    u = f32(*g.random(6))
+    want, _ = run(x, u, t, k, p, m, d)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [[torch.empty(6, dtype=torch.int32, device="cuda") for _ in range(8)] for _ in streams]
+    torch.cuda.synchronize()
+    for n in range(8):
+        for s, out in zip(streams, outs):
+            with torch.cuda.stream(s):
+                q3.sample_logits(out[n], x, u, t, k, p, m, draft=d)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for out in outs for o in out)
