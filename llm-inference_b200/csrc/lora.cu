@@ -19,6 +19,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "tc_common.cuh"
 #include "waiter.cuh"
 
 namespace cg = cooperative_groups;
@@ -243,59 +244,69 @@ __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float 
 
 // A x of a long tile, this CTA's part of k: x and A come through shared memory in stages of 64 elements of k (a row is 128 bytes,
 // its 16-byte lines exchanged by the row's lowest bits, so that the eight rows of a matrix lie in different banks), so
-// that each is read once. Twelve warps have a pair of eight-column tiles each, for all rows; four load. From registers alone, with
-// each warp reading all of A for its rows, this part took 2079 rows of rank 64 three times as long, and with loads and products
-// taking turns in every warp, once and a half.
+// that each is read once. Twelve warps have a pair of eight-column tiles each, for all rows. One asks for A, up to 64 rows a copy; two
+// copy the rows of x, which may lie anywhere. From registers alone, with each warp reading all of A for its rows, this part took
+// 2079 rows of rank 64 three times as long; with 16-byte copies for A, too, their number was the limit (44.6 us in all, now 36.7).
 constexpr int LA_STAGES = 4, LA_KC = 64, LA_COLS = 192;  // columns at a time
 constexpr int LA_STAGE_BYTES = (32 + LA_COLS) * LA_KC * 2;
-constexpr int LA_READERS = LA_COLS / 16, LA_LOADERS = LA_WARPS - LA_READERS;  // warps
+constexpr int LA_READERS = LA_COLS / 16;  // warps; then one for A
+constexpr int LA_X_THREADS = 64;
 
-// bars: full, then empty, of each stage; down: zero, set when a wait has given up
-__device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigned char *ring, uint64_t *bars, int *down, const int *row_s, int rows,
-                                            int adapter, int r, int C, int rank_c) {
+struct LoraMaps {
+    CUtensorMap a[LA_MAX_SLICES];  // of long tiles: [n_adapters * rank][k], boxes of `box` rows and 64 elements
+    int box;                       // a power of two up to 64 that divides rank
+};
+
+// ring: 1024-byte aligned; bars: full, then empty, of each stage; down: zero, set when a wait has given up
+__device__ __forceinline__ void shrink_long(const LoraArgs &a, const LoraMaps &maps, float *h, unsigned char *ring, uint64_t *bars, int *down,
+                                            const int *row_s, int rows, int adapter, int r, int C, int rank_c) {
     constexpr int ROWS = 32;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, each = a.wide / a.n_slices;
-    const int k16 = (a.k + 15) / 16, k0 = 16 * (int)((long long)k16 * rank_c / C), k1 = min(a.k, 16 * (int)((long long)k16 * (rank_c + 1) / C));
-    const int chunks = (k1 - k0 + LA_KC - 1) / LA_KC;
-    const int tiles_each = (r + 7) / 8, n_tiles = tiles_each * a.n_slices;
+    const int k64 = (a.k + LA_KC - 1) / LA_KC, c0 = (int)((long long)k64 * rank_c / C), chunks = (int)((long long)k64 * (rank_c + 1) / C) - c0;
+    const int tiles_each = (r + maps.box - 1) / maps.box * (maps.box / 8), n_tiles = tiles_each * a.n_slices;  // whole boxes
     const uint32_t ring_at = smem_u32(ring);
     Waiter wait(&g_dev_error, down);
     int it = 0;  // chunks so far
-    if (warp >= LA_READERS) {
-        // a thread copies one line of each of these rows: of x, then of A; null: zeros
-        constexpr int STEP = LA_LOADERS * 4, EACH = (ROWS + LA_COLS) / STEP;
-        const int row0 = (tid - 32 * LA_READERS) / 8, q = tid % 8;
+    // Readers that gave up release no stages, so that the loaders starve and give up in turn.
+    if (warp == LA_READERS) {
 #pragma unroll 1
         for (int n0 = 0; n0 < n_tiles; n0 += LA_COLS / 8) {
-            const int all = ROWS + min(LA_COLS, (n_tiles - n0) * 8);
-            const bf16 *from[EACH];
-#pragma unroll
-            for (int j = 0; j < EACH; j++) {
-                const int row = row0 + j * STEP;
-                if (row < ROWS) {
-                    from[j] = row < rows ? a.x + row_s[row] * a.x_stride : nullptr;
-                } else {
-                    const int nt = n0 + (row - ROWS) / 8, sl = slice_of(nt, tiles_each), rr = (nt - sl * tiles_each) * 8 + (row - ROWS) % 8;
-                    from[j] = nt < n_tiles && rr < r ? a.slice[sl].a + ((long long)adapter * a.rank + rr) * a.k : nullptr;
-                }
-            }
+            const int tiles = min(LA_COLS / 8, n_tiles - n0), nt = n0 + lane * (maps.box / 8), sl = slice_of(nt, tiles_each);
+            const int y = adapter * a.rank + 8 * (nt - sl * tiles_each);
 #pragma unroll 1
             for (int c = 0; c < chunks; c++, it++) {
                 const int st = it % LA_STAGES;
                 if (it >= LA_STAGES) wait(bars + LA_STAGES + st, (it / LA_STAGES - 1) & 1);
-                if (wait.dead) continue;  // readers that gave up release no stages, so that the loaders starve and give up in turn
-                const uint32_t to = ring_at + st * LA_STAGE_BYTES;
-                const int k = k0 + c * LA_KC + 8 * q;
-#pragma unroll
-                for (int j = 0; j < EACH; j++) {
-                    const int row = row0 + j * STEP;
-                    const bool in = from[j] && k < k1;
-                    if (row < all) copy16(to + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4), in ? from[j] + k : a.x, in);
-                }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bars + st)) : "memory");
+                if (wait.stopped()) continue;
+                if (lane == 0) mbar_arrive_expect_tx(bars + st, tiles * 8 * LA_KC * 2);
+                __syncwarp();
+                if (nt < n0 + tiles) tma_load_2d(ring + st * LA_STAGE_BYTES + (ROWS + maps.box * lane) * LA_KC * 2, &maps.a[sl], (c0 + c) * LA_KC, y, bars + st);
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp > LA_READERS) {
+        const int own = tid - 32 * (LA_READERS + 1), row0 = own / 8, q = own % 8;
+        if (own < LA_X_THREADS) {
+            constexpr int STEP = LA_X_THREADS / 8;
+            const bf16 *from[ROWS / STEP];
+#pragma unroll
+            for (int j = 0; j < ROWS / STEP; j++) from[j] = a.x + row_s[row0 + j * STEP] * a.x_stride + 8 * q;
+#pragma unroll 1
+            for (int n0 = 0; n0 < n_tiles; n0 += LA_COLS / 8)
+#pragma unroll 1
+                for (int c = 0; c < chunks; c++, it++) {
+                    const int st = it % LA_STAGES, k = (c0 + c) * LA_KC;
+                    if (it >= LA_STAGES) wait(bars + LA_STAGES + st, (it / LA_STAGES - 1) & 1);
+                    if (wait.dead) continue;
+#pragma unroll
+                    for (int j = 0; j < ROWS / STEP; j++) {
+                        const int row = row0 + j * STEP;
+                        const bool in = row < rows && k + 8 * q < a.k;
+                        copy16(ring_at + st * LA_STAGE_BYTES + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4), in ? from[j] + k : a.x, in);
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bars + st)) : "memory");
+                }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        }
     } else {
 #pragma unroll 1
         for (int n0 = 0; n0 < n_tiles; n0 += LA_COLS / 8) {
@@ -345,11 +356,13 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, float *h, unsigne
         }
     }
     __syncthreads();
+    if (*reinterpret_cast<volatile int *>(down)) settle();  // copies may still be on their way
+    __syncthreads();
 }
 
 // GATE_UP: slices 0 and 1 are gate and up, and what is written is silu(gate) * up. PASS: of a short tile.
 template <int ROWS, bool GATE_UP, int PASS>
-__global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_constant__ LoraArgs a) {
+__global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ LoraMaps maps) {
     constexpr int THREADS = LA_THREADS, WARPS = LA_WARPS, MT = ROWS == 16 || GATE_UP ? 1 : 2;  // MT: 16-row tiles of a warp in the second product
     extern __shared__ __align__(16) unsigned char la_smem[];
     cg::cluster_group cluster = cg::this_cluster();
@@ -366,7 +379,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
 
     if (ROWS > 16 && tid == 0) {
         for (int st = 0; st < LA_STAGES; st++) {
-            mbar_init(bars + st, 32 * LA_LOADERS);
+            mbar_init(bars + st, 1 + LA_X_THREADS);
             mbar_init(bars + LA_STAGES + st, LA_READERS);
         }
         fence_barrier_init();
@@ -414,7 +427,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
             };
             shrink_short<PASS>(a, h, reinterpret_cast<float *>(rest), row_s, rows, adapter, r, C, rank_c, ask);
         } else {
-            shrink_long(a, h, wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest, bars, head_s + LA_HEAD - 1, row_s, rows, adapter, r, C, rank_c);
+            shrink_long(a, maps, h, align_shared<1024>(wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest), bars, head_s + LA_HEAD - 1, row_s, rows, adapter, r, C, rank_c);
         }
         // the CTAs' parts, in their order. Few: each CTA adds up all of them; more: each some of the columns for all.
         if (C > 1) cluster.sync();
@@ -588,7 +601,7 @@ template <int ROWS, int PASS>
 size_t lora_smem(int wide) {
     const size_t h = (size_t)ROWS * wide * 4, both = h + 2 * (size_t)ROWS * pitch_of(wide) * 2;
     const size_t first = ROWS == 16 ? h + (size_t)LA_WARPS * 16 * 8 * PASS * 4
-                                    : (wide <= LA_COLS ? 0 : h) + (size_t)LA_STAGES * LA_STAGE_BYTES;
+                                    : (wide <= LA_COLS ? 0 : h) + 1024 + (size_t)LA_STAGES * LA_STAGE_BYTES;
     return 2 * LA_STAGES * 8 + (size_t)(ROWS + LA_HEAD) * 4 + std::max(first, both);
 }
 
@@ -616,7 +629,12 @@ int launch_lora(const LoraArgs &args, int tiles, cudaStream_t s) {
     const int kinds = args.n_adapters + 1;
     const double expected = kinds * (1.0 - exp(-(double)args.n_rows / kinds)) + args.n_rows / ROWS;
     const int cluster = std::max(1, std::min(LA_MAX_CLUSTER, (int)(num_sms() / expected)));
-    Q3_TRY_LAUNCH(launch(kernel, dim3((unsigned)tiles * cluster), dim3(LA_THREADS), smem, s, cluster, args));
+    LoraMaps maps = {};
+    maps.box = std::min(64, args.rank & -args.rank);
+    if (ROWS > 16)
+        for (int i = 0; i < args.n_slices; i++)
+            if (!make_map_strided(&maps.a[i], args.slice[i].a, (long long)args.n_adapters * args.rank, args.k, args.k, maps.box)) return Q3_ERR_ARG;
+    Q3_TRY_LAUNCH(launch(kernel, dim3((unsigned)tiles * cluster), dim3(LA_THREADS), smem, s, cluster, args, maps));
     return Q3_OK;
 }
 template <bool GATE_UP>
