@@ -523,7 +523,7 @@ typedef struct q3_lora_slice {
 
 /* What the projections of one call share. k, n, rank and strides are multiples of 8, rank is at most 128, pointers are
  * 16-byte aligned. Adapter i has ranks[i] <= rank (null: all have rank): what a and b hold past it does not matter.
- * scale null is 1. */
+ * scale null is 1. plan: written for these n_rows and n_adapters. */
 typedef struct q3_lora {
     const q3_bf16 *x;
     long long x_stride;
