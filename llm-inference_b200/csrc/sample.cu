@@ -482,8 +482,8 @@ static_assert(SL_PADDED <= SL_GROUPS * SL_GROUP && SL_GROUP % 8 == 0, "whole gro
 struct ValuesShared {
     alignas(16) unsigned count[SL_PADDED];  // this CTA's
     Told told[SL_MAX_CLUSTER];
-    int n_list;  // groups of its share that are not empty
-    unsigned short list[SL_GROUPS];
+    unsigned occupied[SL_MAX_CLUSTER][SL_WARPS];  // which groups each CTA has tokens of
+    unsigned short list[SL_GROUPS];               // its share of those that any has
     unsigned tiny, equal;  // a low magnitude but zero; the draft's equals before it in its CTA
     unsigned outer;               // key of the largest of high magnitude, 0: none
     unsigned top;
@@ -527,7 +527,7 @@ __device__ __forceinline__ int first_values(F f) {
 struct Values {
     ValuesShared &s;
     Row<bf16> &row;
-    unsigned *sum;  // the cluster's counts, in a CTA for its share of the groups, in the first one all
+    unsigned *sum;  // the cluster's counts, in a CTA for its share of the groups, in the first one all that are not empty
     Weigher weigh;
 
     // Bits of a line's places that hold the value; both zeros are one.
@@ -541,7 +541,7 @@ struct Values {
 
     __device__ __forceinline__ void zero() {
         for (int v = 4 * threadIdx.x; v < SL_PADDED; v += 4 * SL_THREADS) *reinterpret_cast<uint4 *>(s.count + v) = make_uint4(0, 0, 0, 0);
-        if (threadIdx.x == 0) s.tiny = s.outer = s.equal = s.top = s.n_list = 0;
+        if (threadIdx.x == 0) s.tiny = s.outer = s.equal = s.top = 0;
     }
 
     // A value that is not counted one by one, and not -infinity.
@@ -573,15 +573,44 @@ struct Values {
         const unsigned best = __reduce_max_sync(0xffffffffu, t > -INFINITY ? key_of(t) : 0);
         if (threadIdx.x % 32 == 0) atomicMax(&s.top, best);
         __syncthreads();
+        unsigned any = 0;
+        if (threadIdx.x < SL_PADDED / SL_GROUP) {
+#pragma unroll
+            for (int k = 0; k < SL_GROUP / 4; k++) {
+                const uint4 n = *reinterpret_cast<const uint4 *>(s.count + threadIdx.x * SL_GROUP + 4 * k);
+                any |= n.x | n.y | n.z | n.w;
+            }
+        }
+        any = __ballot_sync(0xffffffffu, any != 0);
+        if ((int)threadIdx.x % 32 < row.C) *row.of(&s.occupied[row.rank][threadIdx.x / 32], threadIdx.x % 32) = any;
     }
 
     // The CTAs' counts to the first one, each CTA the sums of its share of the groups. draft: index, or -1.
     __device__ void merge(int draft, float xd) {
-        const int own = (SL_PADDED / SL_GROUP + row.C - 1) / row.C;
-        const int first = row.rank * own, last = min(first + own, SL_PADDED / SL_GROUP);
+        // Two thirds of the groups are empty in a row of normal logits; the others are dealt out to the CTAs in turn.
+        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+        unsigned some = 0;  // lane j: the 32 groups of warp j that any CTA has tokens of
+        if (lane < SL_WARPS)
+            for (int r = 0; r < row.C; r++) some |= s.occupied[r][lane];
+        unsigned run = __popc(some);
+#pragma unroll
+        for (int o = 1; o < SL_WARPS; o <<= 1) {
+            const unsigned y = __shfl_up_sync(0xffffffffu, run, o);
+            run += lane >= o ? y : 0;
+        }
+        const unsigned own = __shfl_sync(0xffffffffu, some, warp), all = __shfl_sync(0xffffffffu, run, SL_WARPS - 1);
+        const unsigned before = __shfl_sync(0xffffffffu, run - __popc(some), warp) + __popc(own & ((1u << lane) - 1));
+        if (own >> lane & 1) {
+            if ((int)(before % row.C) == row.rank) s.list[before / row.C] = (unsigned short)threadIdx.x;
+        } else if (row.rank == 0) {
+            s.group_mass[threadIdx.x] = s.group_count[threadIdx.x] = 0;
+        }
+        const int n_list = ((int)all + row.C - 1 - row.rank) / row.C;
+        __syncthreads();
         if (row.C > 1) {  // remote shared memory gives and takes 16 bytes as fast as 4
 #pragma unroll 1
-            for (int v = first * SL_GROUP + 4 * threadIdx.x; v < last * SL_GROUP; v += 4 * SL_THREADS) {
+            for (int i = threadIdx.x; i < n_list * (SL_GROUP / 4); i += SL_THREADS) {
+                const int v = s.list[i / (SL_GROUP / 4)] * SL_GROUP + i % (SL_GROUP / 4) * 4;
                 uint4 n = *reinterpret_cast<const uint4 *>(s.count + v);
 #pragma unroll 1
                 for (int r0 = 1; r0 < row.C; r0 += 4) {
@@ -605,22 +634,7 @@ struct Values {
             }
             __syncthreads();
         }
-        // Two thirds of the groups are empty in a row of normal logits; the others are listed, in any order, and shared out.
-        {
-            const int g = first + threadIdx.x;
-            unsigned any = 0;
-            if (g < last) {
-#pragma unroll
-                for (int k = 0; k < SL_GROUP / 4; k++) {
-                    const uint4 n = *reinterpret_cast<const uint4 *>(sum + g * SL_GROUP + 4 * k);
-                    any |= n.x | n.y | n.z | n.w;
-                }
-                if (any) s.list[atomicAdd(&s.n_list, 1)] = (unsigned short)g;
-            }
-            if (!any && (g < last || (row.rank == row.C - 1 && g < SL_GROUPS))) *row.of(&s.group_mass[g], 0) = *row.of(&s.group_count[g], 0) = 0;
-            __syncthreads();
-        }
-        const int n_list = s.n_list, sub = n_list <= SL_THREADS / 8 ? 8 : n_list <= SL_THREADS / 4 ? 4 : n_list <= SL_THREADS / 2 ? 2 : 1;
+        const int sub = n_list <= SL_THREADS / 8 ? 8 : n_list <= SL_THREADS / 4 ? 4 : n_list <= SL_THREADS / 2 ? 2 : 1;
         const bool mine = (int)threadIdx.x / sub < n_list;  // `sub` neighbouring threads share a group
         const int g = mine ? s.list[threadIdx.x / sub] : 0;
         u64 mass = 0;
@@ -711,7 +725,8 @@ struct Values {
     __device__ u64 before(int pos) {
         if (pos >= SL_VALUES) pos = SL_VALUES;
         const int g = min(pos / SL_GROUP, SL_GROUPS - 1), at = g * SL_GROUP + threadIdx.x % 32;
-        return s.group_mass[g] + warp_sum(at < pos ? sum[at] * weigh(to_f32(value_of(at))) : 0);
+        const bool some = g + 1 < SL_GROUPS && s.group_count[g + 1] > s.group_count[g];  // of an empty group there are no sums
+        return s.group_mass[g] + warp_sum(some && at < pos ? sum[at] * weigh(to_f32(value_of(at))) : 0);
     }
 
     // The index of a value's nth token.
