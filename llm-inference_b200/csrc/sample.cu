@@ -473,14 +473,17 @@ struct Bins {
 constexpr int SL_LOW = (127 - 32) << 7, SL_HIGH = (127 + 8) << 7;
 constexpr float SL_TINY = 0x1p-32f;
 constexpr int SL_SIGN = SL_HIGH - SL_LOW;
-constexpr int SL_VALUES = 2 * SL_SIGN + 1;  // in the order of the values: positive ones, zero, negative ones
-constexpr int SL_GROUP = 24;                // neighbouring values, which a warp takes side by side
-constexpr int SL_GROUPS = SL_THREADS;       // searched before the values themselves; the last ones are empty
-constexpr int SL_PADDED = (SL_VALUES + SL_GROUP - 1) / SL_GROUP * SL_GROUP;
-static_assert(SL_PADDED <= SL_GROUPS * SL_GROUP && SL_GROUP % 8 == 0, "whole groups, of 16-byte lines");
+// Places in the order of the values: positive ones, zero, which has a group of its own, negative ones; in groups of neighbouring
+// ones, which a warp takes side by side. Counters lie in another order, that of the values' bits: positive ones, negative ones, zero,
+// so that a token's counter takes few instructions to find.
+constexpr int SL_GROUP = 32;
+constexpr int SL_PLACES = 2 * SL_SIGN + SL_GROUP;
+constexpr int SL_USED = SL_PLACES / SL_GROUP;
+constexpr int SL_GROUPS = SL_THREADS;  // searched before the values themselves; the last ones are empty
+static_assert(SL_SIGN % SL_GROUP == 0 && SL_USED <= SL_GROUPS, "whole groups");
 
 struct ValuesShared {
-    alignas(16) unsigned count[SL_PADDED];  // this CTA's
+    alignas(16) unsigned count[SL_PLACES];  // this CTA's
     Told told[SL_MAX_CLUSTER];
     unsigned occupied[SL_MAX_CLUSTER][SL_WARPS];  // which groups each CTA has tokens of
     unsigned short list[SL_GROUPS];               // its share of those that any has
@@ -499,7 +502,7 @@ struct ValuesShared {
 };
 
 __device__ __forceinline__ bf16 value_of(int pos) {
-    const int m = pos < SL_SIGN ? SL_HIGH - 1 - pos : pos == SL_SIGN ? 0 : SL_LOW + (pos - SL_SIGN - 1) + 0x8000;
+    const int m = pos < SL_SIGN ? SL_HIGH - 1 - pos : pos < SL_SIGN + SL_GROUP ? 0 : SL_LOW + (pos - SL_SIGN - SL_GROUP) + 0x8000;
     return __ushort_as_bfloat16((unsigned short)m);
 }
 // The value's place, -1 if it is not counted.
@@ -507,12 +510,17 @@ __device__ __forceinline__ int pos_of(unsigned h) {
     const int m = h & 0x7fff;
     if (m == 0) return SL_SIGN;
     if (m < SL_LOW || m >= SL_HIGH) return -1;
-    return h & 0x8000 ? SL_SIGN + 1 + (m - SL_LOW) : SL_HIGH - 1 - m;
+    return h & 0x8000 ? SL_SIGN + SL_GROUP + (m - SL_LOW) : SL_HIGH - 1 - m;
+}
+// The counter of a place, and the first of a group.
+__device__ __forceinline__ int counter_of(int pos) { return pos < SL_SIGN ? SL_SIGN - 1 - pos : pos < SL_SIGN + SL_GROUP ? pos + SL_SIGN : pos - SL_GROUP; }
+__device__ __forceinline__ int counters_of(int g) {
+    return SL_GROUP * (g < SL_SIGN / SL_GROUP ? SL_SIGN / SL_GROUP - 1 - g : g == SL_SIGN / SL_GROUP ? 2 * SL_SIGN / SL_GROUP : g - 1);
 }
 // f(value) is true for the first values, down to some place: the number of them, by all lanes of a warp.
 template <typename F>
 __device__ __forceinline__ int first_values(F f) {
-    int lo = 0, hi = SL_VALUES;  // true before lo, false from hi on
+    int lo = 0, hi = SL_PLACES;  // true before lo, false from hi on
     const int lane = threadIdx.x % 32;
     while (hi > lo) {
         const int step = (hi - lo + 31) / 32, at = lo + lane * step;
@@ -540,14 +548,14 @@ struct Values {
     }
 
     __device__ __forceinline__ void zero() {
-        for (int v = 4 * threadIdx.x; v < SL_PADDED; v += 4 * SL_THREADS) *reinterpret_cast<uint4 *>(s.count + v) = make_uint4(0, 0, 0, 0);
+        for (int v = 4 * threadIdx.x; v < SL_PLACES; v += 4 * SL_THREADS) *reinterpret_cast<uint4 *>(s.count + v) = make_uint4(0, 0, 0, 0);
         if (threadIdx.x == 0) s.tiny = s.outer = s.equal = s.top = 0;
     }
 
     // A value that is not counted one by one, and not -infinity.
     __device__ __noinline__ static void odd(ValuesShared &s, unsigned v) {
         const unsigned m = v & 0x7fff;
-        if (m == 0) atomicAdd(&s.count[SL_SIGN], 1u);
+        if (m == 0) atomicAdd(&s.count[2 * SL_SIGN], 1u);
         else if (m < SL_LOW) s.tiny = 1;
         else if (m <= 0x7f80) atomicMax(&s.outer, key_of(__uint_as_float(v << 16)));  // else NaN
     }
@@ -555,17 +563,31 @@ struct Values {
     // One pass over the slice: counts, and the largest value.
     __device__ void stream() {
         __nv_bfloat162 top = __floats2bfloat162_rn(-INFINITY, -INFINITY);
+        const __nv_bfloat162 least = __floats2bfloat162_rn(SL_TINY, SL_TINY), most = __floats2bfloat162_rn(256.0f, 256.0f);
         row.each_line<4>([&](const uint4 &raw, int) {
             const unsigned *h = reinterpret_cast<const unsigned *>(&raw);
+            unsigned m2[4];
+            bool all = true;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 top = __hmax2(top, *reinterpret_cast<const __nv_bfloat162 *>(&h[e]));  // not NaN, if either is not
+                m2[e] = h[e] & 0x7fff7fffu;
+                const __nv_bfloat162 mag = *reinterpret_cast<const __nv_bfloat162 *>(&m2[e]);
+                all = all && __hbge2(mag, least) && __hblt2(mag, most);
+            }
+            if (all) {
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const unsigned v = k ? h[e] >> 16 : h[e] & 0xffff, off = (v & 0x7fff) - SL_LOW;
-                    if (off < (unsigned)SL_SIGN) atomicAdd(&s.count[v & 0x8000 ? SL_SIGN + 1 + off : SL_SIGN - 1 - off], 1u);
-                    else if (v != 0xff80) odd(s, v);
+                for (int e = 0; e < 4; e++) {
+                    atomicAdd(&s.count[(m2[e] & 0xffffu) + ((unsigned)((int)(h[e] << 16) >> 31) & SL_SIGN) - SL_LOW], 1u);
+                    atomicAdd(&s.count[(m2[e] >> 16) + ((unsigned)((int)h[e] >> 31) & SL_SIGN) - SL_LOW], 1u);
                 }
+                return;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const unsigned v = e % 2 ? h[e / 2] >> 16 : h[e / 2] & 0xffff, off = (v & 0x7fff) - SL_LOW;
+                if (off < (unsigned)SL_SIGN) atomicAdd(&s.count[off + (v & 0x8000 ? SL_SIGN : 0)], 1u);
+                else if (v != 0xff80) odd(s, v);
             }
         });
         float t = fmaxf(__low2float(top), __high2float(top));
@@ -574,10 +596,10 @@ struct Values {
         if (threadIdx.x % 32 == 0) atomicMax(&s.top, best);
         __syncthreads();
         unsigned any = 0;
-        if (threadIdx.x < SL_PADDED / SL_GROUP) {
+        if (threadIdx.x < SL_USED) {
 #pragma unroll
-            for (int k = 0; k < SL_GROUP / 4; k++) {
-                const uint4 n = *reinterpret_cast<const uint4 *>(s.count + threadIdx.x * SL_GROUP + 4 * k);
+            for (int k = 0; k < SL_GROUP / 4; k++) {  // each lane from another bank on
+                const uint4 n = *reinterpret_cast<const uint4 *>(s.count + counters_of(threadIdx.x) + 4 * ((k + threadIdx.x) % (SL_GROUP / 4)));
                 any |= n.x | n.y | n.z | n.w;
             }
         }
@@ -610,7 +632,7 @@ struct Values {
         if (row.C > 1) {  // remote shared memory gives and takes 16 bytes as fast as 4
 #pragma unroll 1
             for (int i = threadIdx.x; i < n_list * (SL_GROUP / 4); i += SL_THREADS) {
-                const int v = s.list[i / (SL_GROUP / 4)] * SL_GROUP + i % (SL_GROUP / 4) * 4;
+                const int v = counters_of(s.list[i / (SL_GROUP / 4)]) + i % (SL_GROUP / 4) * 4;
                 uint4 n = *reinterpret_cast<const uint4 *>(s.count + v);
 #pragma unroll 1
                 for (int r0 = 1; r0 < row.C; r0 += 4) {
@@ -642,8 +664,8 @@ struct Values {
         // a warp's lanes stay together
 #pragma unroll 1
         for (int e = 0; e < SL_GROUP; e += sub) {
-            const int pos = g * SL_GROUP + e + threadIdx.x % sub;
-            const unsigned n = mine ? sum[pos] : 0;
+            const int pos = g * SL_GROUP + (e + threadIdx.x) % SL_GROUP;  // from another bank in each group
+            const unsigned n = mine ? sum[counter_of(pos)] : 0;
             if (__any_sync(0xffffffffu, n != 0)) {
                 const u64 w = weigh(to_f32(value_of(n ? pos : 0)));
                 mass += n * w;
@@ -661,7 +683,7 @@ struct Values {
         if (draft >= 0) {  // the draft's equals with a smaller index
             const bf16 value = __float2bfloat16(xd);
             const int pos = pos_of(__bfloat16_as_ushort(value));
-            const unsigned here = pos < 0 ? 0 : s.count[pos];
+            const unsigned here = pos < 0 ? 0 : s.count[counter_of(pos)];
             if (here > 0 && row.i0 + row.slice <= draft) {
                 if (threadIdx.x == 0) s.equal = here;
             } else if (here > 1 && row.i0 < draft) {
@@ -697,9 +719,8 @@ struct Values {
         const int lane = threadIdx.x % 32;
         const int g = search<SL_GROUPS>(s.group_mass, s.group_count, target, by_count);
         const int pos = g * SL_GROUP + lane;
-        const bool is = lane < SL_GROUP && pos < SL_VALUES;
-        const u64 w = is ? weigh(to_f32(value_of(pos))) : 0;
-        const unsigned n = is && w ? sum[pos] : 0;
+        const u64 w = weigh(to_f32(value_of(pos)));
+        const unsigned n = w ? sum[counter_of(pos)] : 0;
         const u64 m = n * w;
         u64 bm = m;
         unsigned bn = n;
@@ -723,16 +744,15 @@ struct Values {
     }
     // The mass before a value, by all lanes of a warp.
     __device__ u64 before(int pos) {
-        if (pos >= SL_VALUES) pos = SL_VALUES;
-        const int g = min(pos / SL_GROUP, SL_GROUPS - 1), at = g * SL_GROUP + threadIdx.x % 32;
+        const int g = pos / SL_GROUP, at = g * SL_GROUP + threadIdx.x % 32;
         const bool some = g + 1 < SL_GROUPS && s.group_count[g + 1] > s.group_count[g];  // of an empty group there are no sums
-        return s.group_mass[g] + warp_sum(some && at < pos ? sum[at] * weigh(to_f32(value_of(at))) : 0);
+        return s.group_mass[g] + warp_sum(some && at < pos ? sum[counter_of(at)] * weigh(to_f32(value_of(at))) : 0);
     }
 
     // The index of a value's nth token.
     __device__ int index(const Crossing &f) {
         const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-        const unsigned here = lane < row.C ? row.of(s.count, lane)[f.pos] : 0;
+        const unsigned here = lane < row.C ? row.of(s.count, lane)[counter_of(f.pos)] : 0;
         unsigned run = here;
 #pragma unroll
         for (int o = 1; o < SL_MAX_CLUSTER; o <<= 1) {
@@ -1063,7 +1083,7 @@ int q3_sample_logits(int *out, float *prob, const void *logits, int dtype, int r
         c++;
     SampleArgs a = {out, prob, logits, stride, vocab, slice_of(c), u, temperature, top_p, min_p, top_k, draft};
     size_t smem = sizeof(BinsShared);
-    if (dtype == 0) smem = std::max(smem, (sizeof(ValuesShared) + 15) / 16 * 16 + (c > 1 ? SL_PADDED * sizeof(unsigned) : 0));
+    if (dtype == 0) smem = std::max(smem, (sizeof(ValuesShared) + 15) / 16 * 16 + (c > 1 ? SL_PLACES * sizeof(unsigned) : 0));
     auto kernel = dtype == 0 ? sample_logits_kernel<bf16> : sample_logits_kernel<float>;
     cudaError_t e = allow_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return record_cuda_error(e);
