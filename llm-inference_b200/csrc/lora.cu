@@ -60,17 +60,28 @@ __host__ __device__ inline LoraPlanLayout lora_plan_layout(int n_rows, int n_ada
 // ------------------------------------------------------------------ plan
 
 constexpr int LP_THREADS = 1024;
+constexpr int LP_COUNTERS = 49152;  // 192 KB of them
 
-// Counts, running sums and a stable placement: 10 us for 2079 rows, once per step.
+// Parts that the rows are cut into: a warp each, as far as there are rows for them and room for their counters.
+__host__ __device__ inline int lora_plan_parts(int n_rows, int n_adapters) {
+    const int rows = (n_rows + 31) / 32, room = LP_COUNTERS / (n_adapters + 1) - 1;
+    return rows < room ? (rows < 32 ? rows : 32) : room < 32 ? room : 32;
+}
+
+// A stable sort: counts for each part of the rows and adapter, running sums over both, and each part placed by its warp.
+// A chain of loads and, in a part, of steps of 32 rows; with one part, whose rows all warps went through for adapters of their
+// own, 2079 rows took 20 us and 65536 559. Now 2.9 us for 32 rows, 4.7 for 2079 of 8 adapters, 40 for 65536 (199 if of 8192); once
+// per step.
 __global__ void __launch_bounds__(LP_THREADS, 1) lora_plan_kernel(char *plan, int n_rows, int n_adapters, const int *index) {
     extern __shared__ int la_smem_plan[];
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, tile_rows = lora_tile_rows(n_rows), kinds = n_adapters + 1;
-    int *next = la_smem_plan;       // [kinds]: rows of each adapter, then placed ones; the last: those without one
-    int *first = next + kinds;      // [kinds]: its first tile
-    int *sums = first + kinds;      // [32]
+    const int parts = lora_plan_parts(n_rows, n_adapters), part_rows = (n_rows + 32 * parts - 1) / (32 * parts) * 32;
+    int *next = la_smem_plan;           // [parts][kinds]: a part's rows of each adapter, then where the next of them goes; the last kind: without one
+    int *first = next + parts * kinds;  // [kinds]: its first tile
+    int *sums = first + kinds;          // [32]
     const LoraPlanLayout l = lora_plan_layout(n_rows, n_adapters);
     int *tiles = reinterpret_cast<int *>(plan + 16);
-    for (int i = tid; i < kinds; i += LP_THREADS) next[i] = 0;
+    for (int i = tid; i < parts * kinds; i += LP_THREADS) next[i] = 0;
     pdl_trigger();
     pdl_wait();
     __syncthreads();
@@ -80,13 +91,20 @@ __global__ void __launch_bounds__(LP_THREADS, 1) lora_plan_kernel(char *plan, in
     };
     for (int row = tid; row < n_rows; row += LP_THREADS) {
         if (index[row] >= n_adapters) atomicOr(&g_dev_error, DEV_ERR_POS_RANGE);
-        atomicAdd(&next[kind(row)], 1);
+        atomicAdd(&next[row / part_rows * kinds + kind(row)], 1);
     }
     __syncthreads();
-    // running sums of tiles, 1024 adapters at a time
+    // running sums: of an adapter's rows over the parts, of tiles over the adapters, 1024 of them at a time
     int tile0 = 0;
     for (int i0 = 0; i0 < kinds; i0 += LP_THREADS) {
-        const int i = i0 + tid, n = i < kinds ? next[i] : 0, t = (n + tile_rows - 1) / tile_rows;
+        const int i = i0 + tid;
+        int n = 0;
+        for (int p = 0; i < kinds && p < parts; p++) {
+            const int c = next[p * kinds + i];
+            next[p * kinds + i] = n;
+            n += c;
+        }
+        const int t = (n + tile_rows - 1) / tile_rows;
         int run = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -101,25 +119,26 @@ __global__ void __launch_bounds__(LP_THREADS, 1) lora_plan_kernel(char *plan, in
             all += sums[w];
         }
         const int tile = tile0 + before + run - t;
-        if (i < kinds) {
-            first[i] = tile;
-            next[i] = 0;
-        }
+        if (i < kinds) first[i] = tile;
         for (int k = 0; k < t; k++) *reinterpret_cast<int4 *>(tiles + (tile + k) * l.record) = make_int4(i < n_adapters ? i : -1, min(tile_rows, n - k * tile_rows), 0, 0);
         tile0 += all;
         __syncthreads();
     }
     if (tid == 0) *reinterpret_cast<int *>(plan) = tile0;
-    // each warp places the rows of its adapters, in their order
-    for (int r0 = 0; r0 < n_rows; r0 += 32) {
-        const int row = r0 + lane, k = row < n_rows ? kind(row) : -1;
-        const bool mine = k >= 0 && k % (LP_THREADS / 32) == warp;
-        if (!__any_sync(0xffffffffu, mine)) continue;
-        const unsigned peers = __match_any_sync(0xffffffffu, mine ? k : -1);
-        const int at = mine ? next[k] + __popc(peers & ((1u << lane) - 1)) : 0;
+    if (warp >= parts) return;
+    next += warp * kinds;
+    const int r1 = min(n_rows, (warp + 1) * part_rows), shift = __ffs(tile_rows) - 1;
+    int k_next = warp * part_rows + lane < r1 ? kind(warp * part_rows + lane) : -1;
+    for (int r0 = warp * part_rows; r0 < r1; r0 += 32) {
+        const int row = r0 + lane, k = k_next;
+        k_next = row + 32 < r1 ? kind(row + 32) : -1;
+        const unsigned peers = __match_any_sync(0xffffffffu, k);
+        if (k >= 0) {
+            const int at = next[k] + __popc(peers & ((1u << lane) - 1));
+            tiles[(first[k] + (at >> shift)) * l.record + LA_HEAD + (at & (tile_rows - 1))] = row;
+        }
         __syncwarp();
-        if (mine) tiles[(first[k] + at / tile_rows) * l.record + LA_HEAD + at % tile_rows] = row;
-        if (mine && lane == __ffs(peers) - 1) next[k] = at + __popc(peers);
+        if (k >= 0 && lane == __ffs(peers) - 1) next[k] += __popc(peers);
         __syncwarp();
     }
 }
@@ -733,7 +752,7 @@ int q3_lora_plan(void *plan, int n_rows, int n_adapters, const int *index, void 
     if (reinterpret_cast<uintptr_t>(plan) & 15) return Q3_ERR_ALIGN;
     const int st = check_device();
     if (st != Q3_OK) return st;
-    const size_t smem = (2 * (size_t)(n_adapters + 1) + 32) * 4;
+    const size_t smem = (size_t)((lora_plan_parts(n_rows, n_adapters) + 1) * (n_adapters + 1) + 32) * 4;
     const cudaError_t e = allow_smem(reinterpret_cast<const void *>(lora_plan_kernel), smem);
     if (e != cudaSuccess) return record_cuda_error(e);
     Q3_TRY_LAUNCH(launch(lora_plan_kernel, dim3(1), dim3(LP_THREADS), smem, (cudaStream_t)stream, 1,

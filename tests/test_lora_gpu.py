@@ -357,3 +357,24 @@ def test_long_steps():
     c.add()
     one = Case(5000, 64, [72], 128, 2, [1] * 5000)
     one.add()
+
+
+@pytest.mark.parametrize("rows,n", [(33, 8192), (64, 4095), (129, 1), (2079, 1000), (4097, 5000), (65536, 3), (65536, 8192)])
+def test_plans_of_any_size(rows, n):
+    # every part of the rows, and every number of counters around those that a block has without asking
+    g = torch.Generator().manual_seed(rows)
+    index = torch.randint(-1, n, (rows,), generator=g, dtype=torch.int32).cuda()
+    x, base = normal(g, rows, 8), normal(g, rows, 8)
+    a, b = normal(g, n, 8, 8, std=0.3), normal(g, n, 8, 8, std=0.3)
+    plan, out = q3.LoraPlan(rows, n), torch.full_like(base, NAN)
+    for chosen in (index, index.flip(0)):
+        plan.update(chosen)
+        q3.lora_add(out, base, x, q3.LoraStack([a], [b]), plan)
+        at, has = chosen.long().clamp(min=0), (chosen >= 0).double()[:, None]
+        h = torch.einsum("nrk,nk->nr", a[at].double(), x.double())
+        y = base.double() + has * torch.einsum("nor,nr->no", b[at].double(), h)
+        mag = torch.einsum("nrk,nk->nr", a[at].double().abs(), x.double().abs())
+        bound = (40 * 2.0 ** -24 + 2.0 ** -16) * has * torch.einsum("nor,nr->no", b[at].double().abs(), mag) + 2.0 ** -23 * base.double().abs()
+        assert ((out.double() - y).abs() <= bound + 2.0 ** -8 * y.abs() + 1e-37).all()
+        assert torch.equal(out[chosen < 0], base[chosen < 0])
+    assert q3.device_error() == 0
