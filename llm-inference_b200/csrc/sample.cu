@@ -41,7 +41,7 @@ constexpr int SL_THREADS = 512;
 constexpr int SL_WARPS = SL_THREADS / 32;
 constexpr int SL_MAX_CLUSTER = 8;
 constexpr int SL_BITS = 41;        // the largest weight is 2^41: those of a whole row add up to less than 2^62
-constexpr int SL_SLICE = 1 << 18;  // tokens of a CTA at most: 14-bit parts of their weights add up within 32 bits
+constexpr int SL_SLICE = 1 << 18;  // tokens of a CTA at most: the upper halves of their weights, up to 2^9 each, add up within 32 bits
 constexpr int SL_VOCAB = 1 << 20;
 
 typedef unsigned long long u64;
@@ -244,13 +244,13 @@ struct Row {
 constexpr int SL_BINS = 1024;
 constexpr int SL_CAND = 256;  // tokens of a bin that are ranked directly
 
-struct Candidate {
+struct alignas(16) Candidate {
     u64 order;  // key in the upper half, complement of the index below: larger comes earlier
     u64 w;
 };
 
 struct BinsShared {
-    alignas(16) unsigned part[4][SL_BINS];  // this CTA's histogram: 14-bit parts of the weights, and counts
+    alignas(16) unsigned part[3][SL_BINS];  // this CTA's histogram: lower and upper halves of the masses, and counts
     u64 sum_mass[2][SL_BINS];   // what comes before each bin in the row; [1]: of a bin that was cut finer
     unsigned sum_count[2][SL_BINS];
     Candidate list[2][SL_CAND];  // this CTA's tokens of the bin in question; finds take turns
@@ -269,6 +269,7 @@ struct Bins {
     Weigher weigh;
     float per_bin;
     unsigned least_key;  // no logit below it weighs anything
+    bool counting;       // tokens, too
     int turn = 0;
 
     // by adding 2^23, which leaves the nearest whole number in the low bits
@@ -277,15 +278,24 @@ struct Bins {
     }
 
     __device__ __forceinline__ void zero() {
-        for (int b = threadIdx.x; b < SL_BINS; b += SL_THREADS) s.part[0][b] = s.part[1][b] = s.part[2][b] = s.part[3][b] = 0;
+        for (int b = threadIdx.x; b < SL_BINS; b += SL_THREADS) s.part[0][b] = s.part[1][b] = s.part[2][b] = 0;
     }
-    // 64-bit atomics in shared memory are loops; most weights have few parts
-    __device__ __forceinline__ void add(int b, u64 w) {
-        const unsigned p0 = (unsigned)w & 0x3fff, p1 = (unsigned)(w >> 14) & 0x3fff, p2 = (unsigned)(w >> 28);
-        if (p0) atomicAdd(&s.part[0][b], p0);
-        if (p1) atomicAdd(&s.part[1][b], p1);
-        if (p2) atomicAdd(&s.part[2][b], p2);
-        if (w) atomicAdd(&s.part[3][b], 1u);
+    // N tokens. 64-bit atomics in shared memory are loops, so the lower halves' own overflow says what to carry to the upper ones;
+    // most weights have no upper half, and only top-k asks for counts.
+    template <int N>
+    __device__ __forceinline__ void add(const int (&b)[N], const u64 (&w)[N]) {
+        unsigned up[N];
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const unsigned low = (unsigned)w[e];
+            up[e] = (unsigned)(w[e] >> 32);
+            if (low) up[e] += atomicAdd(&s.part[0][b[e]], low) + low < low;
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            if (up[e]) atomicAdd(&s.part[1][b[e]], up[e]);
+            if (counting && w[e]) atomicAdd(&s.part[2][b[e]], 1u);
+        }
     }
 
     // Running sums of the CTAs' histograms into sum_*[level]; each CTA adds up a share of the bins for all.
@@ -298,17 +308,17 @@ struct Bins {
             uint4 n = {};
 #pragma unroll 1
             for (int r = 0; r < row.C; r++) {
-                uint4 p[4];
+                uint4 p[3];
 #pragma unroll
-                for (int k = 0; k < 4; k++) p[k] = *reinterpret_cast<const uint4 *>(row.of(s.part[k], r) + b);
-                m[0] += p[0].x + ((u64)p[1].x << 14) + ((u64)p[2].x << 28);
-                m[1] += p[0].y + ((u64)p[1].y << 14) + ((u64)p[2].y << 28);
-                m[2] += p[0].z + ((u64)p[1].z << 14) + ((u64)p[2].z << 28);
-                m[3] += p[0].w + ((u64)p[1].w << 14) + ((u64)p[2].w << 28);
-                n.x += p[3].x;
-                n.y += p[3].y;
-                n.z += p[3].z;
-                n.w += p[3].w;
+                for (int k = 0; k < 3; k++) p[k] = *reinterpret_cast<const uint4 *>(row.of(s.part[k], r) + b);
+                m[0] += p[0].x + ((u64)p[1].x << 32);
+                m[1] += p[0].y + ((u64)p[1].y << 32);
+                m[2] += p[0].z + ((u64)p[1].z << 32);
+                m[3] += p[0].w + ((u64)p[1].w << 32);
+                n.x += p[2].x;
+                n.y += p[2].y;
+                n.z += p[2].z;
+                n.w += p[2].w;
             }
 #pragma unroll 1
             for (int r = 0; r < row.C; r++) {
@@ -386,7 +396,7 @@ struct Bins {
             __syncthreads();
             row.template each<1>([&](float x, int) {
                 const unsigned key = key_of(x);
-                if (key >= lo && key <= hi) add((hi - key) >> shift, weigh(x));
+                if (key >= lo && key <= hi) add<1>({(int)((hi - key) >> shift)}, {weigh(x)});
             });
             u64 all_mass;
             unsigned all_count;
@@ -417,11 +427,13 @@ struct Bins {
         const Candidate own = mine < n ? s.all[mine] : Candidate{~0ull, 0};
         u64 before = 0;
         unsigned places = 0;
-        for (unsigned j = from; j < n; j += sub)
-            if (s.all[j].order > own.order) {
-                before += s.all[j].w;
-                places++;
-            }
+#pragma unroll 4
+        for (unsigned j = from; j < n; j += sub) {
+            const Candidate c = s.all[j];
+            const bool ahead = c.order > own.order;
+            before += ahead ? c.w : 0;
+            places += ahead;
+        }
         for (int o = sub / 2; o > 0; o /= 2) {
             before += __shfl_xor_sync(0xffffffffu, before, o);
             places += __shfl_xor_sync(0xffffffffu, places, o);
@@ -874,7 +886,7 @@ __device__ void sample_bins(BinsShared &s, Row<T> &row, const SampleArgs &a, con
     const u64 best = warp_max(top > -INFINITY ? (u64)key_of(top) << 32 | (unsigned)~at : 0);
     const unsigned least = __reduce_min_sync(0xffffffffu, key_of(low));
     if (tid % 32 == 0) s.all[tid / 32] = {best, least};
-    Bins<T> bins = {s, row, {}, 0.0f, 0};
+    Bins<T> bins = {s, row, {}, 0.0f, 0, o.k > 0};
     bins.zero();
     __syncthreads();
     if (tid < row.C) {
@@ -906,15 +918,33 @@ __device__ void sample_bins(BinsShared &s, Row<T> &row, const SampleArgs &a, con
         const double least_t = o.floor > 0.0f ? log2((double)fminf(o.floor, 1.0f)) : 0.0;
         // the histogram, the mass above min-p's limit, the mass before the draft
         u64 above = 0, before = 0;
-        row.template each<1>([&](float x, int i) {
-            const u64 w = weigh(x);
-            bins.add(bins.bin_of(x), w);
-            if (o.floor > 0.0f && w && (x == weigh.peak || ((double)x - (double)weigh.peak) * weigh.c >= least_t)) above += w;
-            if (o.draft >= 0 && (x > o.xd || (x == o.xd && i < o.draft))) before += w;
+        const bool extra = o.floor > 0.0f || o.draft >= 0;
+        row.template each_line<2>([&](const uint4 &raw, int i0) {
+            const T *in = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+            for (int e0 = 0; e0 < Row<T>::PER; e0 += 4) {
+                float x[4];
+                u64 w[4];
+                int b[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {  // side by side, before the branches
+                    const float v = to_f32(in[e0 + e]);
+                    x[e] = v == v ? v : -INFINITY;
+                    w[e] = weigh(x[e]);
+                    b[e] = bins.bin_of(x[e]);
+                }
+                bins.add(b, w);
+                if (!extra) continue;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (o.floor > 0.0f && w[e] && (x[e] == weigh.peak || ((double)x[e] - (double)weigh.peak) * weigh.c >= least_t)) above += w[e];
+                    if (o.draft >= 0 && (x[e] > o.xd || (x[e] == o.xd && i0 + e0 + e < o.draft))) before += w[e];
+                }
+            }
         });
         u64 mass, above_all = 0, before_all = 0;
         unsigned count;
-        if (o.floor > 0.0f || o.draft >= 0) {
+        if (extra) {
             unsigned none = 0;
             u64 sum = above;
             block_scan(s.scan, sum, none, above, count);
