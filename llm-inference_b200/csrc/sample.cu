@@ -59,7 +59,7 @@ struct SampleArgs {
 // What a CTA tells the others.
 struct Told {
     u64 above, before_draft;  // its mass above min-p's limit and before the draft
-    u64 first;                // its largest token: key in the upper half, complement of the index below
+    unsigned first;           // key of its largest logit, 0: none
     unsigned count, low, high;
 };
 
@@ -114,11 +114,6 @@ struct Weigher {
 __device__ __forceinline__ u64 warp_sum(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-__device__ __forceinline__ u64 warp_max(u64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
@@ -225,16 +220,13 @@ struct Row {
             f(raw, i0 + v);
         }
     }
-    // f(x, index); NaN comes as -infinity
+    // f(x, index)
     template <int LOADS, typename F>
     __device__ __forceinline__ void each(F f) const {
         each_line<LOADS>([&](const uint4 &raw, int i) {
             const T *x = reinterpret_cast<const T *>(&raw);
 #pragma unroll
-            for (int e = 0; e < PER; e++) {
-                const float v = to_f32(x[e]);
-                f(v == v ? v : -INFINITY, i + e);
-            }
+            for (int e = 0; e < PER; e++) f(to_f32(x[e]), i + e);
         });
     }
 };
@@ -273,9 +265,9 @@ struct Bins {
     int turn = 0;
 
     // by adding 2^23, which leaves the nearest whole number in the low bits
-    __device__ __forceinline__ int bin_of(float x) const {
-        return __float_as_int(fminf((weigh.peak - x) * per_bin, SL_BINS - 1.0f) + 8388608.0f) & (SL_BINS - 1);
-    }
+    __device__ __forceinline__ float place_of(float x) const { return fminf((weigh.peak - x) * per_bin, SL_BINS - 1.0f) + 8388608.0f; }
+    __device__ __forceinline__ int bin_of(float x) const { return __float_as_int(place_of(x)) & (SL_BINS - 1); }
+    static __device__ __forceinline__ float bin_place(int bin) { return 8388608.0f + bin; }
 
     __device__ __forceinline__ void zero() {
         for (int b = threadIdx.x; b < SL_BINS; b += SL_THREADS) s.part[0][b] = s.part[1][b] = s.part[2][b] = 0;
@@ -361,9 +353,10 @@ struct Bins {
                 s.key_hi = 0;
             }
             __syncthreads();
-            row.template each<4>([&](float x, int i) {
+            const float least = of_key(cut ? lo : least_key), most = cut ? of_key(hi) : INFINITY, its = bin_place(bin);
+            row.template each<2>([&](float x, int i) {
+                if (!(x >= least && x <= most && (cut || place_of(x) == its))) return;
                 const unsigned key = key_of(x);
-                if (key < least_key || (cut ? key < lo || key > hi : bin_of(x) != bin)) return;
                 const unsigned at = atomicAdd(&s.n_list, 1u);
                 if (at < SL_CAND) list[at].order = (u64)key << 32 | (unsigned)~i;
                 atomicMin(&s.key_lo, key);
@@ -396,7 +389,7 @@ struct Bins {
             __syncthreads();
             row.template each<1>([&](float x, int) {
                 const unsigned key = key_of(x);
-                if (key >= lo && key <= hi) add<1>({(int)((hi - key) >> shift)}, {weigh(x)});
+                if (x == x && key >= lo && key <= hi) add<1>({(int)((hi - key) >> shift)}, {weigh(x)});
             });
             u64 all_mass;
             unsigned all_count;
@@ -873,43 +866,63 @@ __device__ __forceinline__ Weigher weigher(float peak, float temperature) {
 template <typename T>
 __device__ void sample_bins(BinsShared &s, Row<T> &row, const SampleArgs &a, const Choice &o, int r) {
     const int tid = threadIdx.x;
-    // the largest token, and the smallest finite logit
+    // the largest logit, and the smallest finite one
     float top = -INFINITY, low = INFINITY;
-    int at = 0;
-    row.template each<4>([&](float x, int i) {
-        if (x > top) {
-            top = x;
-            at = i;
+    row.template each_line<4>([&](const uint4 &raw, int) {
+        const T *x = reinterpret_cast<const T *>(&raw);
+        float most = to_f32(x[0]), least = most;
+#pragma unroll
+        for (int e = 1; e < Row<T>::PER; e++) {  // not NaN, if any is not
+            most = fmaxf(most, to_f32(x[e]));
+            least = fminf(least, to_f32(x[e]));
         }
-        if (x > -INFINITY) low = fminf(low, x);
+        top = fmaxf(top, most);
+        if (!(least > -INFINITY)) {
+            least = INFINITY;
+#pragma unroll
+            for (int e = 0; e < Row<T>::PER; e++) least = to_f32(x[e]) > -INFINITY ? fminf(least, to_f32(x[e])) : least;
+        }
+        low = fminf(low, least);
     });
-    const u64 best = warp_max(top > -INFINITY ? (u64)key_of(top) << 32 | (unsigned)~at : 0);
+    const unsigned best = __reduce_max_sync(0xffffffffu, top > -INFINITY ? key_of(top) : 0);
     const unsigned least = __reduce_min_sync(0xffffffffu, key_of(low));
     if (tid % 32 == 0) s.all[tid / 32] = {best, least};
     Bins<T> bins = {s, row, {}, 0.0f, 0, o.k > 0};
     bins.zero();
+    if (tid == 0) s.tie = 0x7fffffff;
     __syncthreads();
     if (tid < row.C) {
-        u64 f = 0, l = 0xffffffffu;
+        unsigned f = 0, l = 0xffffffffu;
         for (int w = 0; w < SL_WARPS; w++) {
-            f = max(f, s.all[w].order);
-            l = min(l, s.all[w].w);
+            f = max(f, (unsigned)s.all[w].order);
+            l = min(l, (unsigned)s.all[w].w);
         }
         Told *t = row.of(&s.told[0][row.rank], tid);
         t->first = f;
-        t->low = (unsigned)l;
+        t->low = l;
     }
     row.sync();
-    u64 first = 0;
-    unsigned min_key = 0xffffffffu;
+    unsigned first = 0, min_key = 0xffffffffu;  // first: the largest one's key, 0: none
     for (int c = 0; c < row.C; c++) {
         first = max(first, s.told[0][c].first);
         min_key = min(min_key, s.told[0][c].low);
     }
-    int token = first ? (int)~(unsigned)first : -1;
+    int token = -1;
     float prob = first ? 1.0f : 0.0f;
+    if (first && !(o.temperature > 0.0f)) {  // the first of the largest ones
+        const float peak = of_key(first);
+        row.template each<1>([&](float x, int i) {
+            if (x == peak) atomicMin(&s.tie, i);
+        });
+        __syncthreads();
+        if (tid < row.C) row.of(&s.told[1][row.rank], tid)->count = s.tie;
+        row.sync();
+        unsigned at = 0x7fffffff;
+        for (int c = 0; c < row.C; c++) at = min(at, s.told[1][c].count);
+        token = (int)at;
+    }
     if (first && o.temperature > 0.0f) {
-        const Weigher weigh = weigher(of_key((unsigned)(first >> 32)), o.temperature);
+        const Weigher weigh = weigher(of_key(first), o.temperature);
         bins.weigh = weigh;
         const float range = fminf((float)(44.0 / weigh.c), weigh.peak - of_key(min_key));
         bins.per_bin = range > 0.0f ? fminf(SL_BINS / range, 1e30f) : 0.0f;
@@ -928,8 +941,7 @@ __device__ void sample_bins(BinsShared &s, Row<T> &row, const SampleArgs &a, con
                 int b[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {  // side by side, before the branches
-                    const float v = to_f32(in[e0 + e]);
-                    x[e] = v == v ? v : -INFINITY;
+                    x[e] = to_f32(in[e0 + e]);
                     w[e] = weigh(x[e]);
                     b[e] = bins.bin_of(x[e]);
                 }
@@ -986,7 +998,7 @@ __device__ bool sample_values(ValuesShared &s, unsigned *sum, Row<bf16> &row, co
     Weigher weigh = weigher(0.0f, o.temperature);
     row.wait();
     const Told &told = s.told[min(tid % 32, row.C - 1)];
-    const unsigned top = __reduce_max_sync(0xffffffffu, (unsigned)told.first), tiny = __reduce_max_sync(0xffffffffu, told.low),
+    const unsigned top = __reduce_max_sync(0xffffffffu, told.first), tiny = __reduce_max_sync(0xffffffffu, told.low),
                    outer = __reduce_max_sync(0xffffffffu, told.high);
     if (top == 0) {  // no tokens
         if (row.rank == 0 && tid == 0) {
