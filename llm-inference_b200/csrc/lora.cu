@@ -4,11 +4,14 @@
 // The plan sorts a step's rows by their adapter, once for all layers, and cuts them into tiles, so that rows of one adapter
 // anywhere in the batch share its weights. A cluster of CTAs takes a tile: each CTA multiplies its part of k, the partial
 // A x are added up through distributed shared memory, and each CTA expands its part of the columns; nothing goes through global
-// memory between the two products. Both run on warp-level matrix instructions with operands loaded straight into
-// registers: the contraction's order is free as long as both operands have the same, so a lane takes eight (A x) or four
+// memory between the two products. Both run on warp-level matrix instructions, with operands loaded straight into
+// registers but for the first product of long tiles, whose operands come through shared memory: the contraction's order is free as long as both operands have the same, so a lane takes eight (A x) or four
 // (B h) neighbouring elements of its row, and its four columns of eight-column tiles are dealt out so that a lane writes eight
-// neighbouring outputs. Bound by the bytes of x, base, out and the present adapters' weights (a rank of 64 is 64 products for each
-// element of x, a tenth of what the tensor cores could do meanwhile) and, for few rows, by the chain of loads.
+// neighbouring outputs. What cannot be done without is the bytes of x, base, out and the present adapters' weights (a rank of 64 is 64
+// products for each element of x, a tenth of what the tensor cores could do meanwhile). Few rows are bound by the chain of loads
+// and two cluster barriers (one row through q, k and v 8.5 us, 32 rows 11.7), long steps by that chain in each warp beside the
+// bytes (2079 rows 35 us, of which the first product alone 14, the second alone 26.6; without the bases' loads that is 20.8, without
+// the stores 22.2, without matrix instructions 23.5, without B's loads 24.9).
 //
 // A x is held in 32 bits and enters the second product as two bf16 numbers, which together have 16 bits of it: its
 // rounding to one would be as large as the output's own.
@@ -41,7 +44,8 @@ constexpr int LA_MAX_CLUSTER = 8;
 constexpr int LA_HEAD = 4;
 
 // Rows of a tile: of a step of few rows as many as one matrix instruction takes; more share an adapter's weights in
-// longer tiles. 347 rows, 5 adapters of rank 24, gate and up: 20 us with tiles of 32, 33 with 64; 2079 rows, 8 of rank 64, q, k and v: 49 and 61.
+// longer tiles. 2079 rows, 8 adapters of rank 64, q, k and v: 37 us with tiles of 32, 47 with tiles of 64, which halve the weights' traffic but
+// not the products, and fill fewer SMs.
 __host__ __device__ constexpr int lora_tile_rows(int n_rows) { return n_rows <= 128 ? 16 : 32; }
 
 struct LoraPlanLayout {

@@ -12,16 +12,20 @@
 // atomics below nor the way the row is cut change a result, and a draw is decided as in 64 bits.
 //
 // A cluster of CTAs shares a row. Two ways to find a crossing:
-//   - bf16 logits have few values: one pass counts each value between 2^-24 and 2^8 of either sign, and zeros (one shared-memory
+//   - bf16 logits have few values: one pass counts each value between 2^-32 and 2^8 of either sign, and zeros (one shared-memory
 //     atomic a token, the exponentials once per value that occurs). Equal tokens weigh the same, so a running sum over
 //     the values says which value and which of its tokens; one more pass, by the CTA that has it, finds its index.
 //   - fp32 logits, and bf16 rows in which a value outside those weighs anything: a pass for the largest, one for a
-//     histogram of mass and count over the logits, and per crossing one that gathers the tokens of its bin, which are ranked by
-//     comparing each with each. A bin of too many tokens is cut finer by the bits of its logits; as many equal ones are
+//     histogram of mass (and for top-k of count) over the logits, and per crossing one that gathers the tokens of its bin, which are
+//     ranked by comparing each with each. A bin of too many tokens is cut finer by the bits of its logits; as many equal ones are
 //     told apart by counting them in the order of their index.
-// CTAs write what others need into their shared memory before a cluster barrier (reading it after one, C loads that wait for
-// one another, cost more than all the arithmetic). The counts of values all go to the first CTA, which then needs no more
-// barriers.
+// CTAs write what others need into their shared memory before a cluster barrier: loads after it that wait for one another
+// cost more than all the arithmetic. The counts of values are added up by all CTAs, each for a share of the groups of values
+// that any has tokens of, and the sums go to the first CTA, which then needs no more barriers.
+//
+// Bound by the chain of these steps for few rows (one of 151936 bf16 12.5 us, 32 with all settings 17.7), by shared-memory
+// atomics for many (256 rows 45 us, 1.7 TB/s), and by instructions for fp32 rows (100 of 32003 35 us, the pass for the
+// histogram half of it).
 #include <math.h>
 
 #include <algorithm>

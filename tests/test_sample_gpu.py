@@ -343,3 +343,26 @@ def test_two_calls_at_once():
                 q3.sample_logits(out[n], x, u, t, k, p, m, draft=d)
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for out in outs for o in out)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [5, 40000, 151936])
+def test_greedy_rows_take_the_first_of_the_largest(vocab, dtype):
+    # wherever its equals lie among the parts of a row; rows of one sign of zero and the other; beside NaN and -infinity
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randn(8, vocab, generator=g).clamp(max=3.0)
+    want = torch.randint(0, vocab, (8,), generator=g)
+    for r in range(8):
+        x[r, want[r]:][torch.rand(vocab - want[r], generator=g) < 0.3] = 3.5
+        x[r, want[r]] = 3.5
+    x[5] = NAN
+    x[5, want[5]:] = -INF
+    x[5, want[5]] = -1e30
+    x[6] = -INF
+    x[6, want[6]:] = 0.0
+    x[6, want[6]] = -0.0
+    x[7] = -1000.0
+    want[7] = 0
+    x = x.cuda().to(dtype)
+    out, prob = run(x, f32(*[0.999] * 8), t=f32(*[0.0] * 8), k=i32(*[3] * 8), draft=i32(*[vocab - 1] * 8))
+    assert out.tolist() == want.tolist() and prob.tolist() == [1.0] * 8
