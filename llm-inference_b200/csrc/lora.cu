@@ -5,11 +5,11 @@
 // anywhere in the batch share its weights. A cluster of CTAs takes a tile: each CTA multiplies its part of k, the partial
 // A x are added up through distributed shared memory, and each CTA expands its part of the columns; nothing goes through global
 // memory between the two products. Both run on warp-level matrix instructions, with operands loaded straight into
-// registers but for the first product of long tiles, whose operands come through shared memory: the contraction's order is free as long as both operands have the same, so a lane takes eight (A x) or four
+// registers but for the first product of long or wide tiles, whose operands come through shared memory: the contraction's order is free as long as both operands have the same, so a lane takes eight (A x) or four
 // (B h) neighbouring elements of its row, and its four columns of eight-column tiles are dealt out so that a lane writes eight
 // neighbouring outputs. What cannot be done without is the bytes of x, base, out and the present adapters' weights (a rank of 64 is 64
 // products for each element of x, a tenth of what the tensor cores could do meanwhile). Few rows are bound by the chain of loads
-// and two cluster barriers (one row through q, k and v 8.5 us, 32 rows 11.7), long steps by that chain in each warp beside the
+// and two cluster barriers (one row through q, k and v 8.3 us, 32 rows 9.4), long steps by that chain in each warp beside the
 // bytes (2079 rows 35 us, of which the first product alone 14, the second alone 26.6; without the bases' loads that is 20.8, without
 // the stores 22.2, without matrix instructions 23.5, without B's loads 24.9).
 //
@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include <cooperative_groups.h>
 
@@ -198,11 +199,11 @@ __device__ __forceinline__ int slice_of(int nt, int tiles_each) { return nt < ti
 constexpr int LA_THREADS = 512;
 constexpr int LA_WARPS = LA_THREADS / 32;
 
-// A x of a short tile, this CTA's part of k: each warp a part of that for all columns, operands from global memory straight into
-// registers, then the warps' parts added up in their order.
-// PASS: eight-column tiles at a time, whose sums stay in registers; the kernel is built for 2, 4, 6 and 12, and takes the least that holds
-// all: code for more that is stepped over costs 64 rows through the down projection 12.7 -> 15.3 us, a second pass 32 rows through q, k
-// and v 11.9 -> 12.5.
+// A x of a short tile of up to 48 columns, this CTA's part of k: each warp a part of that for all columns, operands from global memory straight
+// into registers, then the warps' parts added up in their order.
+// PASS: its eight-column tiles, whose sums stay in registers; the kernel is built for 2, 4 and 6, and takes the least that holds
+// all: code for more that is stepped over costs 64 rows through the down projection 12.7 -> 15.3 us. Wider ones take the long tiles'
+// way: 32 rows through q, k and v of rank 32 9.5 us where this way takes 11.7, 4 rows of rank 64 11.3 and 18.0.
 // meanwhile() runs once, while the first loads are on their way.
 template <int PASS, typename F>
 __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float *part, const int *row_s, int rows, int adapter, int r, int C, int rank_c,
@@ -213,67 +214,64 @@ __device__ __forceinline__ void shrink_short(const LoraArgs &a, float *h, float 
     const int s0 = (int)((long long)steps * p / parts), s1 = (int)((long long)steps * (p + 1) / parts);
     const bf16 *x0 = a.x + row_s[g] * a.x_stride, *x1 = a.x + row_s[g + 8] * a.x_stride;
     const int tiles_each = (r + 7) / 8, n_tiles = tiles_each * a.n_slices;
-#pragma unroll 1
-    for (int n0 = 0; n0 < n_tiles; n0 += PASS) {
-        float acc[PASS][4] = {};
-        const bf16 *w[PASS];
+    float acc[PASS][4] = {};
+    const bf16 *w[PASS];
 #pragma unroll
-        for (int j = 0; j < PASS; j++) {
-            const int nt = n0 + j, sl = slice_of(nt, tiles_each), row = (nt - sl * tiles_each) * 8 + g;
-            w[j] = nt < n_tiles && row < r ? a.slice[sl].a + ((long long)adapter * a.rank + row) * a.k : nullptr;
-        }
-        uint4 u, v, b[PASS];
-        auto load = [&](int s) {
-            const int k = 32 * s + 8 * t;
-            const uint4 zero = make_uint4(0, 0, 0, 0);
-            const bool in = s < s1 && k < a.k;
-            u = in ? __ldg(reinterpret_cast<const uint4 *>(x0 + k)) : zero;
-            v = in ? __ldg(reinterpret_cast<const uint4 *>(x1 + k)) : zero;
-#pragma unroll
-            for (int j = 0; j < PASS; j++) b[j] = in && w[j] ? __ldg(reinterpret_cast<const uint4 *>(w[j] + k)) : zero;
-        };
-        load(s0);
-        if (n0 == 0) meanwhile();
-#pragma unroll 1
-        for (int s = s0; s < s1; s++) {
-            const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
-#pragma unroll
-            for (int j = 0; j < PASS; j++)
-                if (n0 + j < n_tiles) {
-                    mma(acc[j], a0, b[j].x, b[j].y);
-                    mma(acc[j], a1, b[j].z, b[j].w);
-                }
-            load(s + 1);
-        }
-        float *own = part + warp * 16 * COLS;
-#pragma unroll
-        for (int j = 0; j < PASS; j++) {
-            *reinterpret_cast<float2 *>(own + g * COLS + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
-            *reinterpret_cast<float2 *>(own + (g + 8) * COLS + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
-        }
-        __syncthreads();
-        for (int i = tid; i < rows * COLS; i += LA_THREADS) {
-            const int row = i / COLS, col = i % COLS, nt = n0 + col / 8;
-            if (nt >= n_tiles) continue;
-            float f[LA_WARPS];
-#pragma unroll
-            for (int q = 0; q < LA_WARPS; q++) f[q] = part[(q * 16 + row) * COLS + col];
-#pragma unroll
-            for (int q = 1; q < LA_WARPS; q++) f[0] += f[q];
-            const int sl = slice_of(nt, tiles_each);
-            h[row * a.wide + sl * each + (nt - sl * tiles_each) * 8 + col % 8] = f[0];
-        }
-        __syncthreads();
+    for (int j = 0; j < PASS; j++) {
+        const int nt = j, sl = slice_of(nt, tiles_each), row = (nt - sl * tiles_each) * 8 + g;
+        w[j] = nt < n_tiles && row < r ? a.slice[sl].a + ((long long)adapter * a.rank + row) * a.k : nullptr;
     }
+    uint4 u, v, b[PASS];
+    auto load = [&](int s) {
+        const int k = 32 * s + 8 * t;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        const bool in = s < s1 && k < a.k;
+        u = in ? __ldg(reinterpret_cast<const uint4 *>(x0 + k)) : zero;
+        v = in ? __ldg(reinterpret_cast<const uint4 *>(x1 + k)) : zero;
+#pragma unroll
+        for (int j = 0; j < PASS; j++) b[j] = in && w[j] ? __ldg(reinterpret_cast<const uint4 *>(w[j] + k)) : zero;
+    };
+    load(s0);
+    meanwhile();
+#pragma unroll 1
+    for (int s = s0; s < s1; s++) {
+        const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
+#pragma unroll
+        for (int j = 0; j < PASS; j++)
+            if (j < n_tiles) {
+                mma(acc[j], a0, b[j].x, b[j].y);
+                mma(acc[j], a1, b[j].z, b[j].w);
+            }
+        load(s + 1);
+    }
+    float *own = part + warp * 16 * COLS;
+#pragma unroll
+    for (int j = 0; j < PASS; j++) {
+        *reinterpret_cast<float2 *>(own + g * COLS + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+        *reinterpret_cast<float2 *>(own + (g + 8) * COLS + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+    }
+    __syncthreads();
+    for (int i = tid; i < rows * COLS; i += LA_THREADS) {
+        const int row = i / COLS, col = i % COLS, nt = col / 8;
+        if (nt >= n_tiles) continue;
+        float f[LA_WARPS];
+#pragma unroll
+        for (int q = 0; q < LA_WARPS; q++) f[q] = part[(q * 16 + row) * COLS + col];
+#pragma unroll
+        for (int q = 1; q < LA_WARPS; q++) f[0] += f[q];
+        const int sl = slice_of(nt, tiles_each);
+        h[row * a.wide + sl * each + (nt - sl * tiles_each) * 8 + col % 8] = f[0];
+    }
+    __syncthreads();
 }
 
-// A x of a long tile, this CTA's part of k: x and A come through shared memory in stages of 64 elements of k (a row is 128 bytes,
+// A x of a long tile, or a wide one, this CTA's part of k: x and A come through shared memory in stages of 64 elements of k (a row is 128 bytes,
 // its 16-byte lines exchanged by the row's lowest bits, so that the eight rows of a matrix lie in different banks), so
 // that each is read once. Twelve warps have a pair of eight-column tiles each, for all rows. One asks for A, up to 64 rows a copy; two
 // copy the rows of x, which may lie anywhere. From registers alone, with each warp reading all of A for its rows, this part took
 // 2079 rows of rank 64 three times as long; with 16-byte copies for A, too, their number was the limit (44.6 us in all, then 36.7).
 constexpr int LA_STAGES = 4, LA_KC = 64, LA_COLS = 192;  // columns at a time
-constexpr int LA_STAGE_BYTES = (32 + LA_COLS) * LA_KC * 2;
+__host__ __device__ constexpr int lora_stage_bytes(int rows) { return (rows + LA_COLS) * LA_KC * 2; }
 constexpr int LA_READERS = LA_COLS / 16;  // warps; then one for A
 constexpr int LA_X_THREADS = 64;
 
@@ -283,10 +281,10 @@ struct LoraMaps {
 };
 
 // ring: 1024-byte aligned; bars: full, then empty, of each stage; down: zero, set when a wait has given up
-template <typename F>
+template <int ROWS, typename F>
 __device__ __forceinline__ void shrink_long(const LoraArgs &a, const LoraMaps &maps, float *h, unsigned char *ring, uint64_t *bars, int *down,
                                             const int *row_s, int rows, int adapter, int r, int C, int rank_c, F meanwhile) {
-    constexpr int ROWS = 32;
+    constexpr int MT = ROWS / 16, LA_STAGE_BYTES = lora_stage_bytes(ROWS);
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, each = a.wide / a.n_slices;
     const int k64 = (a.k + LA_KC - 1) / LA_KC, c0 = (int)((long long)k64 * rank_c / C), chunks = (int)((long long)k64 * (rank_c + 1) / C) - c0;
     const int tiles_each = (r + maps.box - 1) / maps.box * (maps.box / 8), n_tiles = tiles_each * a.n_slices;  // whole boxes
@@ -339,7 +337,7 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, const LoraMaps &m
 #pragma unroll 1
         for (int n0 = 0; n0 < n_tiles; n0 += LA_COLS / 8) {
             const int cols = min(LA_COLS, (n_tiles - n0) * 8);
-            float acc[2][2][4] = {};
+            float acc[MT][2][4] = {};
 #pragma unroll 1
             for (int c = 0; c < chunks; c++, it++) {
                 const int st = it % LA_STAGES;
@@ -348,16 +346,16 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, const LoraMaps &m
                     const uint32_t x_at = ring_at + st * LA_STAGE_BYTES, w_at = x_at + ROWS * LA_KC * 2;
 #pragma unroll
                     for (int s = 0; s < LA_KC / 16; s++) {
-                        uint32_t am[2][4], bm[4];
+                        uint32_t am[MT][4], bm[4];
 #pragma unroll
-                        for (int m = 0; m < 2; m++) {
+                        for (int m = 0; m < MT; m++) {
                             const int row = m * 16 + lane % 16, q = 2 * s + lane / 16;
                             load_matrices(am[m], x_at + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4));
                         }
                         const int row = warp * 16 + lane / 16 * 8 + lane % 8, q = 2 * s + lane / 8 % 2;
                         load_matrices(bm, w_at + row * (LA_KC * 2) + ((q ^ (row & 7)) << 4));
 #pragma unroll
-                        for (int m = 0; m < 2; m++) {
+                        for (int m = 0; m < MT; m++) {
                             mma(acc[m][0], am[m], bm[0], bm[1]);
                             mma(acc[m][1], am[m], bm[2], bm[3]);
                         }
@@ -374,7 +372,7 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, const LoraMaps &m
                 const int nt = n0 + 2 * warp + j, sl = slice_of(nt, tiles_each);
                 if (8 * (nt - n0) < cols) {
 #pragma unroll
-                    for (int m = 0; m < 2; m++) {
+                    for (int m = 0; m < MT; m++) {
                         float *to = h + (m * 16 + g) * a.wide + sl * each + (nt - sl * tiles_each) * 8 + 2 * t;
                         *reinterpret_cast<float2 *>(to) = make_float2(acc[m][j][0], acc[m][j][1]);
                         *reinterpret_cast<float2 *>(to + 8 * a.wide) = make_float2(acc[m][j][2], acc[m][j][3]);
@@ -388,7 +386,7 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, const LoraMaps &m
     __syncthreads();
 }
 
-// GATE_UP: slices 0 and 1 are gate and up, and what is written is silu(gate) * up. PASS: of a short tile.
+// GATE_UP: slices 0 and 1 are gate and up, and what is written is silu(gate) * up. PASS: 0 for a first product through shared memory.
 template <int ROWS, bool GATE_UP, int PASS>
 __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ LoraMaps maps) {
     constexpr int THREADS = LA_THREADS, WARPS = LA_WARPS, MT = ROWS == 16 || GATE_UP ? 1 : 2;  // MT: 16-row tiles of a warp in the second product
@@ -405,7 +403,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
     unsigned char *rest = reinterpret_cast<unsigned char *>(h + ROWS * wide);
     bf16 *hi = reinterpret_cast<bf16 *>(rest), *lo = hi + ROWS * pitch;
 
-    if (ROWS > 16 && tid == 0) {
+    if (PASS == 0 && tid == 0) {
         for (int st = 0; st < LA_STAGES; st++) {
             mbar_init(bars + st, 1 + LA_X_THREADS);
             mbar_init(bars + LA_STAGES + st, LA_READERS);
@@ -442,7 +440,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
     for (int sl = 0; sl < (GATE_UP ? 1 : a.n_slices); sl++) units += (a.slice[sl].n + 31) / 32;
     bool waiting = false;
     if (r > 0) {
-        if constexpr (ROWS == 16) {
+        if constexpr (PASS > 0) {
             auto ask = [&] {  // for what the second product will read
                 for (int u = rank_c * WARPS + warp; u < units; u += C * WARPS) {
                     int sl = 0, n0 = u;
@@ -469,7 +467,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1) lora_kernel(const __grid_consta
                     }
                 }
             };
-            shrink_long(a, maps, h, align_shared<1024>(wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest), bars, head_s + LA_HEAD - 1, row_s, rows, adapter, r, C, rank_c, ask);
+            shrink_long<ROWS>(a, maps, h, align_shared<1024>(wide <= LA_COLS ? reinterpret_cast<unsigned char *>(h) : rest), bars, head_s + LA_HEAD - 1, row_s, rows, adapter, r, C, rank_c, ask);
         }
         // the CTAs' parts, in their order. Few: each CTA adds up all of them; more: each some of the columns for all.
         if (C > 1) cluster.sync();
@@ -642,8 +640,8 @@ int pitch_of(int wide) { return wide / 32 % 2 ? wide : wide + 32; }
 template <int ROWS, int PASS>
 size_t lora_smem(int wide) {
     const size_t h = (size_t)ROWS * wide * 4, both = h + 2 * (size_t)ROWS * pitch_of(wide) * 2;
-    const size_t first = ROWS == 16 ? h + (size_t)LA_WARPS * 16 * 8 * PASS * 4
-                                    : (wide <= LA_COLS ? 0 : h) + 1024 + (size_t)LA_STAGES * LA_STAGE_BYTES;
+    const size_t first = PASS > 0 ? h + (size_t)LA_WARPS * 16 * 8 * PASS * 4
+                                    : (wide <= LA_COLS ? 0 : h) + 1024 + (size_t)LA_STAGES * lora_stage_bytes(ROWS);
     return 2 * LA_STAGES * 8 + (size_t)(ROWS + LA_HEAD) * 4 + std::max(first, both);
 }
 
@@ -660,20 +658,53 @@ bool overlap(const void *a, long long a_stride, int a_width, const void *b, long
     return d < 2LL * a_width || d + 2LL * b_width > s;
 }
 
+// Clusters of c CTAs that the device holds at once, a CTA an SM: fewer than its SMs would make, since a cluster stays within one of its parts
+// (148 SMs: 148, 74, 45, 33, 26, 22, 15, 15).
+int clusters_at_once(int c) {
+    static std::atomic<int> known[64][LA_MAX_CLUSTER + 1];
+    int d = 0;
+    cudaGetDevice(&d);
+    std::atomic<int> &n = known[d < 0 || d >= 64 ? 0 : d][c];
+    if (n.load(std::memory_order_relaxed) == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(c * num_sms()));
+        cfg.blockDim = dim3(LA_THREADS);
+        cfg.dynamicSmemBytes = 48 * 1024;
+        cudaLaunchAttribute shape;
+        shape.id = cudaLaunchAttributeClusterDimension;
+        shape.val.clusterDim.x = c;
+        shape.val.clusterDim.y = shape.val.clusterDim.z = 1;
+        cfg.attrs = &shape;
+        cfg.numAttrs = 1;
+        int held = 0;
+        if (cudaOccupancyMaxActiveClusters(&held, lora_kernel<32, false, 0>, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            held = 0;
+        }
+        n.store(held > 0 ? held : num_sms() / c, std::memory_order_relaxed);
+    }
+    return n.load(std::memory_order_relaxed);
+}
+
 template <int ROWS, bool GATE_UP, int PASS>
 int launch_lora(const LoraArgs &args, int tiles, cudaStream_t s) {
     auto kernel = lora_kernel<ROWS, GATE_UP, PASS>;
     const size_t smem = lora_smem<ROWS, PASS>(args.wide);
     cudaError_t e = allow_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return record_cuda_error(e);
-    // CTAs of a tile: as many as the SMs hold at once for as many tiles as there would be if each row took an adapter at random
-    // (64 rows, 64 adapters, about 41 tiles: clusters of 2 take 16.1 us, of 3 12.9, of 4 21.1)
-    const int kinds = args.n_adapters + 1;
-    const double expected = kinds * (1.0 - exp(-(double)args.n_rows / kinds)) + args.n_rows / ROWS;
-    const int cluster = std::max(1, std::min(LA_MAX_CLUSTER, (int)(num_sms() / expected)));
+    // CTAs of a tile: as many as the SMs hold at once for the tiles there may be. Of a short step as many as if each row took an adapter at
+    // random (64 rows, 64 adapters, 41 tiles: clusters of 2 take 16.1 us, of 3 12.9, of 4 21.1; 100 rows, 30 adapters of rank 64, 30
+    // tiles: of 3 18.2, of 4 15.2, of 5 25.3). A long step is mostly a chunk of one prompt: its tiles, and those of 32 rows of other
+    // adapters (831 rows, 53 adapters of rank 32: clusters of 1 take 41 us, of 2 25, of 4 16 if all rows are of one adapter, 30 if each is of
+    // any; 300 rows, 64 adapters: of 2 24, of 3 19 with such a chunk and 33 without).
+    const double kinds = args.n_adapters + 1, rows = args.n_rows, each = rows / kinds;
+    const double tiles_of = ROWS == 16 ? kinds * (1.0 - exp(-each)) * std::max(1.0, each / ROWS + 0.5)
+                                       : args.n_adapters * (1.0 - exp(-32.0 / kinds)) + (rows - 32.0) / ROWS;
+    int cluster = LA_MAX_CLUSTER;
+    while (cluster > 1 && clusters_at_once(cluster) < tiles_of) cluster--;
     LoraMaps maps = {};
     maps.box = std::min(64, args.rank & -args.rank);
-    if (ROWS > 16)
+    if (PASS == 0)
         for (int i = 0; i < args.n_slices; i++)
             if (!make_map_strided(&maps.a[i], args.slice[i].a, (long long)args.n_adapters * args.rank, args.k, args.k, maps.box)) return Q3_ERR_ARG;
     Q3_TRY_LAUNCH(launch(kernel, dim3((unsigned)tiles * cluster), dim3(LA_THREADS), smem, s, cluster, args, maps));
@@ -686,7 +717,7 @@ int launch_lora(const LoraArgs &args, int tiles, cudaStream_t s) {
     if (columns <= 16) return launch_lora<16, GATE_UP, 2>(args, tiles, s);
     if (columns <= 32) return launch_lora<16, GATE_UP, 4>(args, tiles, s);
     if (columns <= 48) return launch_lora<16, GATE_UP, 6>(args, tiles, s);
-    return launch_lora<16, GATE_UP, 12>(args, tiles, s);
+    return launch_lora<16, GATE_UP, 0>(args, tiles, s);
 }
 
 int plan_check(int n_rows, int n_adapters) {
