@@ -378,3 +378,12 @@ def test_plans_of_any_size(rows, n):
         assert ((out.double() - y).abs() <= bound + 2.0 ** -8 * y.abs() + 1e-37).all()
         assert torch.equal(out[chosen < 0], base[chosen < 0])
     assert q3.device_error() == 0
+
+
+@pytest.mark.parametrize("rows,k,rank,n", [(1, 8, 128, 1), (5, 264, 128, 3), (16, 1000, 72, 2), (31, 2560, 128, 40), (128, 2064, 128, 4), (128, 72, 40, 900)])
+def test_wide_short_steps(rows, k, rank, n):
+    # up to 384 columns of A x: as many as a pass holds, and two of them; clusters of each size
+    Case(rows, k, [136, 40, 8], rank, n, some(rows, n, rank), seed=k).add()
+    ranks = [(7 * i + rows) % (rank + 2) for i in range(n)]
+    Case(rows, k, [72, 72], rank, n, some(rows, n, rank + 1), seed=k, ranks=ranks).gate_up()
+    assert q3.device_error() == 0
