@@ -404,6 +404,7 @@ struct Bins {
             const unsigned span = (1u << shift) - 1;
             hi -= (unsigned)bin << shift;
             lo = hi - lo > span ? hi - span : lo;
+            if (hi == key_of(0.0f) - 1) hi--;  // the key of -0, which no logit has: compared as a float it would take the zeros in
         }
     }
 

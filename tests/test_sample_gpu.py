@@ -366,3 +366,18 @@ def test_greedy_rows_take_the_first_of_the_largest(vocab, dtype):
     x = x.cuda().to(dtype)
     out, prob = run(x, f32(*[0.999] * 8), t=f32(*[0.0] * 8), k=i32(*[3] * 8), draft=i32(*[vocab - 1] * 8))
     assert out.tolist() == want.tolist() and prob.tolist() == [1.0] * 8
+
+
+@pytest.mark.parametrize("unit", [1, 3, 4096])
+def test_zeros_above_subnormal_logits(unit):
+    # more tokens than are ranked directly share a bin with exact zeros and lie below them: cut by the bits of their keys, the bins'
+    # ends meet at the key of -0, which no logit has. Shuffled, and with top-k and top-p ends among them.
+    tiny = 2.0 ** -149
+    row = np.concatenate([[1.0, -1.0, 0x1fffff * tiny], np.zeros(50), -np.arange(1, 301) * tiny * unit, [-0x1fffff * tiny]]).astype(np.float32)
+    row[3::7][:5] = -0.0
+    g, n = np.random.default_rng(unit), 400
+    x = torch.from_numpy(np.stack([row, *(g.permutation(row) for _ in range(n - 1))])).cuda()
+    u = (torch.arange(n, device="cuda") + 0.5) / n
+    run(x, u)
+    run(x, u, k=i32(*g.integers(2, 360, n)), p=f32(*g.uniform(0.2, 1.0, n)))
+    run(x, u, t=f32(*g.uniform(0.5, 2.0, n)), draft=i32(*g.integers(0, 354, n)))
