@@ -90,24 +90,25 @@ struct Weigher {
     float peak;
     double c;  // log2 e / T
     // round(2^SL_BITS * 2^((x - peak) c)): the power's whole part goes to the exponent, the rest f in [-1/2, 1/2] through the
-    // Taylor polynomial of e^(f ln 2) (the first term left out is below 3e-13). No branches, so that a thread's
-    // weights overlap: one chain of these operations is 200 cycles.
+    // Chebyshev series of 2^f there, cut after the tenth term: off by 3.2e-16, a thousandth of a unit (the Taylor polynomial of as many
+    // terms by 3e-13, and weights by nearly a whole unit). No branches, so that a thread's weights overlap: one chain of these
+    // operations is 200 cycles.
     __device__ __forceinline__ u64 operator()(float x) const {
         const double t = ((double)x - (double)peak) * c;
         const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number, kept in the low bits
         const double shifted = t + magic;
         const int n = __double2loint(shifted);
         const double f = t - (shifted - magic);
-        double y = 7.054911620801121e-09;  // (ln 2)^k / k!, k = 10 down
-        y = fma(y, f, 1.0178086009239696e-07);
-        y = fma(y, f, 1.3215486790144305e-06);
-        y = fma(y, f, 1.5252733804059838e-05);
-        y = fma(y, f, 0.00015403530393381606);
-        y = fma(y, f, 0.0013333558146428441);
-        y = fma(y, f, 0.009618129107628477);
-        y = fma(y, f, 0.055504108664821576);
-        y = fma(y, f, 0.2402265069591007);
-        y = fma(y, f, 0.6931471805599453);
+        double y = 7.074194562613105e-09;  // the series as a polynomial in f, the tenth power first
+        y = fma(y, f, 1.020869083593037e-07);
+        y = fma(y, f, 1.3215432534254118e-06);
+        y = fma(y, f, 1.5252657257186041e-05);
+        y = fma(y, f, 0.00015403530463727982);
+        y = fma(y, f, 0.0013333558230170627);
+        y = fma(y, f, 0.009618129107587253);
+        y = fma(y, f, 0.05550410866444768);
+        y = fma(y, f, 0.24022650695910158);
+        y = fma(y, f, 0.69314718055995);
         y = fma(y, f, 1.0);
         y = __hiloint2double(__double2hiint(y) + ((n + SL_BITS) << 20), __double2loint(y));
         const u64 w = (u64)__double_as_longlong(y + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52: the sum's fraction bits

@@ -5,6 +5,7 @@ A token has to be the one whose interval of the running mass holds u M. Weights 
 on either side of it. Probabilities: one fp32 rounding, 2^-24, and the weights' errors.
 """
 import sys
+from decimal import Decimal, getcontext
 from pathlib import Path
 
 import numpy as np
@@ -381,3 +382,26 @@ def test_zeros_above_subnormal_logits(unit):
     run(x, u)
     run(x, u, k=i32(*g.integers(2, 360, n)), p=f32(*g.uniform(0.2, 1.0, n)))
     run(x, u, t=f32(*g.uniform(0.5, 2.0, n)), draft=i32(*g.integers(0, 354, n)))
+
+
+def test_weights_hold_their_bound():
+    # rows of the logits 0 and x: top-p keeps the second one if its weight passes 1 / p - 1, from which it is more than 2^-42 away in
+    # each of these; u takes the last one kept
+    getcontext().prec = 50
+    rows = [[float.fromhex(v) for v in row] for row in (
+        ("-0x1.4c8994p-1", "0x1.fb79dep+0", "0x1.29910ap-1"), ("-0x1.4f4aap-1", "0x1.f332c8p+0", "0x1.2a9634p-1"),
+        ("-0x1.d8946ap-2", "0x1.57d3ecp+0", "0x1.2b8e22p-1"), ("-0x1.ba55fcp-2", "0x1.448a1cp+0", "0x1.2b329ep-1"),
+        ("-0x1.f8b25ep-2", "0x1.70bf7ep+0", "0x1.2b6012p-1"), ("-0x1.8639f6p-2", "0x1.1f39c4p+0", "0x1.2b0fecp-1"),
+        ("-0x1.da3664p-3", "0x1.66f1acp-1", "0x1.29e564p-1"), ("-0x1.e66682p-3", "0x1.6164ccp-1", "0x1.2b9d46p-1"),
+        ("-0x1.473e14p-1", "0x1.ee64e4p+0", "0x1.29fac2p-1"), ("-0x1.2c5ea4p-1", "0x1.cd0d14p+0", "0x1.29549ap-1"))]
+    rows += [[x, t, p + 2.0 ** -24] for x, t, p in rows]  # and on the border's other side
+    want = []
+    for x, t, p in rows:
+        past = (Decimal(x) / Decimal(t)).exp() - (1 / Decimal(p) - 1)
+        assert abs(past) * 2 ** 42 > Decimal("1.05")
+        want.append(int(past > 0))
+    x = torch.tensor([[0.0, r[0]] for r in rows], dtype=torch.float32, device="cuda")
+    assert want == [0] * 10 + [1] * 10
+    out = torch.empty(len(rows), dtype=torch.int32, device="cuda")
+    q3.sample_logits(out, x, f32(*[1 - 2.0 ** -24] * len(rows)), f32(*(r[1] for r in rows)), top_p=f32(*(r[2] for r in rows)))
+    assert out.tolist() == want
