@@ -500,7 +500,8 @@ int q3_sample_logits(int *out, float *prob, const void *logits, int dtype, int r
  * For row r of a step and i = index[r]:
  *   out[r] = base[r] + scale[i] * B_i (A_i x[r])
  * with A_i [rank, k] and B_i [n, rank] of adapter i, for up to three projections of the same x (q, k and v). Products and sums are
- * fp32 (A x enters the second product with 16 bits of mantissa), rounded to bf16 once.
+ * fp32 (A x enters the second product with 16 bits of mantissa), rounded to bf16 once. Infinities and NaN go where fp32 takes them, and
+ * stay in their rows.
  *
  * q3_lora_plan sorts the step's rows by adapter, once per step, and all layers and projections use that plan. A plan is
  * plain device memory that the other calls only read; index, too, so plan and layers can be captured in one CUDA graph

@@ -387,3 +387,97 @@ def test_wide_short_steps(rows, k, rank, n):
     ranks = [(7 * i + rows) % (rank + 2) for i in range(n)]
     Case(rows, k, [72, 72], rank, n, some(rows, n, rank + 1), seed=k, ranks=ranks).gate_up()
     assert q3.device_error() == 0
+
+
+@pytest.mark.parametrize("rows,rank", [(5, 8), (20, 40), (150, 16)])
+def test_infinite_and_overflowing_weights(rows, rank):
+    # A x = -3.01171875, whose two bf16 parts have opposite signs, for rank 0, and 2, 4, ... for the others; B inf, huge, or huge of both signs.
+    # The second product's terms are of one sign or too far apart to depend on their order, so fp32 says the same in any.
+    inf, n, k = float("inf"), 64, 32
+    index = [i % 3 for i in range(rows)]
+    c = Case(rows, k, [n, n], rank, 3, index, scale=False)
+    c.x.zero_()
+    c.x[:, 0] = 1.0
+    c.x[:, 1] = 0.01171875
+    for a in c.a:
+        a.zero_()
+        a[:, :, 0] = 2.0 * torch.arange(rank, device="cuda")
+        a[:, 0, 0], a[:, 0, 1] = -3.0, -1.0
+    h = torch.cat([torch.tensor([-3.01171875]), 2.0 * torch.arange(1, rank)]).cuda()
+    for j, b in enumerate(c.b):
+        b.zero_()
+        b[:, :, 1] = 1.0
+        b[:, 1, 0] = inf       # -inf
+        b[:, 2, 0] = -inf      # inf
+        b[:, 3, 0] = 3e38      # overflows to -inf
+        b[:, 4, 0] = -3e38
+        b[:, 5, 2] = inf       # inf, of a value without a second part
+        b[:, 6, 0] = NAN
+        b[:, 7, 0], b[:, 7, 2] = inf, inf  # of both signs: NaN
+        b[1, 8 + 5 * j, 0] = inf           # one adapter's only
+    y = [torch.einsum("bnr,r->bn", b.float(), h)[torch.tensor(index, device="cuda")] + base.float() for b, base in zip(c.b, c.base)]
+    assert [torch.isfinite(v[0]).sum().item() for v in y] == [n - 7, n - 7]
+
+    def same(got, want):
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        some, fine = torch.isinf(want), torch.isfinite(want)
+        assert torch.equal(got[some].float(), want[some])
+        assert ((got - want)[fine].abs() <= 2.0 ** -8 * want[fine].abs() + 2.0 ** -20).all()  # the terms are exact, their sums below 16
+
+    outs = [torch.full_like(t, 5.0) for t in c.base]
+    q3.lora_add(outs, c.base, c.x, c.stack, c.plan)
+    for out, want in zip(outs, y):
+        same(out, want)
+    own = [t.clone() for t in c.base]
+    q3.lora_add(own, own, c.x, c.stack, c.plan)
+    assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(own, outs))
+    act = torch.full_like(c.base[0], 5.0)
+    q3.lora_gate_up(act, c.base[0], c.base[1], c.x, c.stack, c.plan)
+    g, u = y
+    want = g / (1 + torch.exp(-g)) * u
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isnan(act), torch.isnan(want)) and torch.equal(act[torch.isinf(want)].float(), want[torch.isinf(want)])
+    assert ((act - want)[fine].abs() <= 2.0 ** -8 * want[fine].abs() + 2.0 ** -10).all()
+
+
+@pytest.mark.parametrize("rows", [3, 140])
+def test_values_next_to_the_largest(rows):
+    # A x above the largest bf16 number but not above fp32's: its first part must not round to infinity
+    c = Case(rows, 8, [32], 8, 1, [0] * rows)
+    top = 3.3895313892515355e38  # bf16's largest
+    c.scale.fill_(1.0)
+    c.x.fill_(1.0)
+    c.a[0].zero_()
+    c.a[0][0, 0, 0] = top
+    c.a[0][0, 0, 1] = 1.2e36  # 0.9 of a step
+    c.b[0].zero_()
+    c.b[0][0, :, 0] = 0.5
+    h = torch.tensor(top, dtype=torch.float32) + c.a[0][0, 0, 1].float().cpu()
+    assert torch.isfinite(h) and torch.isinf(h.to(BF16))
+    c.base[0].zero_()
+    out = torch.empty_like(c.base[0])
+    q3.lora_add(out, c.base[0], c.x, c.stack, c.plan)
+    assert ((out.double() - 0.5 * h.double()).abs() <= 2.0 ** -8 * h.double()).all()
+
+
+@pytest.mark.parametrize("rows", [40, 300])
+def test_rows_beside_one_that_is_not_finite(rows):
+    # their tiles' other rows are the same to the bit; the row's own columns stay within the bound
+    c = Case(rows, 256, [2048, 40], 24, 3, [i % 3 for i in range(rows)])
+    want = c.add()
+    c.base[0][9, 5], c.base[0][9, 1030], c.base[1][17, 3], c.base[0][20, 2047] = float("inf"), NAN, float("-inf"), NAN
+    c.x[33] = NAN
+    outs = [torch.full_like(t, NAN) for t in c.base]
+    q3.lora_add(outs, c.base, c.x, c.stack, c.plan)
+    for j, (out, before) in enumerate(zip(outs, want)):
+        others = torch.ones(rows, dtype=torch.bool, device="cuda")
+        others[[9, 20, 33] if j == 0 else [17, 33]] = False
+        assert torch.equal(out[others], before[others]) and torch.isnan(out[33]).all()
+        y, bound = c.exact(j)
+        odd = ~torch.isfinite(c.base[j])
+        odd[33] = True
+        assert ((out.double() - y).abs() <= bound + 2.0 ** -8 * y.abs())[~odd].all()
+        assert torch.equal(torch.isnan(out[:33][odd[:33]]), torch.isnan(c.base[j][:33][odd[:33]]))
+    own = [t.clone() for t in c.base]
+    q3.lora_add(own, own, c.x, c.stack, c.plan)
+    assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(own, outs))
