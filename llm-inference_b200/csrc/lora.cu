@@ -395,8 +395,12 @@ __device__ __forceinline__ void shrink_long(const LoraArgs &a, const LoraMaps &m
     __syncthreads();
 }
 
-// (the compiler's own divide, with a branch for rare operands, costs the kernel registers and twice its time)
-__device__ __forceinline__ float silu_times(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+// silu(g) u. The divisor is from 1 to 2 for either sign, since __fdividef gives 0 for one past 2^126. (the compiler's own divide, with
+// a branch for rare operands, costs the kernel registers and twice its time)
+__device__ __forceinline__ float silu_times(float g, float u) {
+    const float e = __expf(-fabsf(g));
+    return __fdividef(g < 0.0f ? g * e : g, 1.0f + e) * u;
+}
 
 // A column of a row in fp32, A x whole again: h, and its lower parts `lower` further on; b: the column's row of B.
 __device__ __forceinline__ float column_again(const bf16 *h, int lower, const bf16 *b, int r, float base) {

@@ -481,3 +481,19 @@ def test_rows_beside_one_that_is_not_finite(rows):
     own = [t.clone() for t in c.base]
     q3.lora_add(own, own, c.x, c.stack, c.plan)
     assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(own, outs))
+
+
+@pytest.mark.parametrize("rows", [5, 140])
+def test_gates_far_below_zero(rows):
+    # 1 + e^-g passes 2^126 there, silu(g) is a number like others: the output's rounding, 2^-8 (twice the half step), and the
+    # exponential, which is off by 2 + 1.2 |g| steps of 2^-23 and, below the smallest normal number, by 2^-17 more: 2^-15
+    c = Case(rows, 16, [64, 64], 8, 2, [i % 2 for i in range(rows)])
+    c.x.zero_()
+    c.base[0].copy_(torch.linspace(-90, -80, rows * 64, device="cuda").view(rows, 64))
+    c.base[1].fill_(2.0)
+    act = torch.zeros_like(c.base[0])
+    q3.lora_gate_up(act, c.base[0], c.base[1], c.x, c.stack, c.plan)
+    g = c.base[0].double()
+    want = 2 * g * torch.exp(g) / (1 + torch.exp(g))
+    assert want.abs().min() > 2.0 ** -126
+    assert ((act.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -15) * want.abs()).all()
