@@ -539,8 +539,8 @@ typedef struct q3_lora {
 int q3_lora_add(const q3_lora_slice *slices, int n_slices, const q3_lora *l, void *stream);
 
 /* act = silu(gate) * up with gate and up as above (slices 0 and 1, whose out is not used), for the rows that have an
- * adapter; the others are left as they are: q3_gate_up_batched, whose taps are the two bases, has written them. act may be
- * either base (same stride). */
+ * adapter; the others are left as they are: q3_gate_up_batched, whose taps are the two bases, has written them. It rounds silu to
+ * bf16 on the way, this call does not, so rows whose adapter has neither are best given none. act may be either base (same stride). */
 int q3_lora_gate_up(q3_bf16 *act, long long act_stride, const q3_lora_slice *gate_up, const q3_lora *l, void *stream);
 
 #ifdef __cplusplus

@@ -102,6 +102,8 @@ class AdapterSet:
         self.scale = torch.zeros(n_adapters, dtype=torch.float32, device="cuda")
         self.loaded: set[int] = set()
         self._a, self._b, self._ranks = {}, {}, {}
+        # per layer, the adapters that have one of gate and up
+        self.with_gate_up: list[set[int]] = [set() for _ in range(shape.num_hidden_layers)]
         self.stacks: dict[str, list[LoraStack]] = {g: [] for g in GROUPS}
         for layer in range(shape.num_hidden_layers):
             for g, projs in GROUPS.items():
@@ -140,6 +142,9 @@ class AdapterSet:
                         a[:ta.shape[0]].copy_(ta)
                         b[:, :ta.shape[0]].copy_(tb)
                 self._ranks[layer, g][i] = most
+            self.with_gate_up[layer].discard(i)
+            if any((layer, p) in tensors for p in GROUPS["gate_up"]):
+                self.with_gate_up[layer].add(i)
         self.scale[i] = scale
         self.loaded.add(i)
 

@@ -188,7 +188,8 @@ class PagedServer:
         rows = max_seqs + chunk
         self.adapters = adapters
         if adapters is not None:
-            self.lora_plans = {n: LoraPlan(n, adapters.n_adapters) for n in self.plans}
+            # of all rows with an adapter, and of those whose adapter has gate or up: the others' keep their activation to the bit
+            self.lora_plans = {n: [LoraPlan(n, adapters.n_adapters) for _ in range(2)] for n in self.plans}
 
         def rows_of(n, count=rows):
             return torch.zeros(count, n, dtype=torch.bfloat16, device="cuda")
@@ -266,9 +267,9 @@ class PagedServer:
         px, pxb, pq, pk, pv, pa, pact = (b.data_ptr() for b in (x, xb, q, k, v, att, act))
         tokens = self._device(step.tokens + [0] * (rows - len(step.tokens)))
         chosen = [seqs.live[i].adapter for i in step.ids]
-        lora = None
-        if any(a >= 0 for a in chosen):
-            lora, stacks = self.lora_plans[rows], self.adapters.stacks
+        has, lora, planned = set(chosen) - {-1}, None, None
+        if has:
+            (lora, some), stacks = self.lora_plans[rows], self.adapters.stacks
             index = np.full(rows, -1, np.int32)
             index[:starts[-1]] = np.repeat(chosen, step.counts)
             lora.update(self._device(index))
@@ -291,10 +292,14 @@ class PagedServer:
             if lora:
                 lora_add(x, x, att, stacks["o"][l], lora)
             call("q3_rmsnorm_forward", pxb, px, p["post_attention_layernorm"], rows, H, eps, stream)
-            taps = (gate.data_ptr(), up.data_ptr()) if lora else (None, None)
+            changed = has & self.adapters.with_gate_up[l] if lora else None
+            if changed and changed not in (has, planned):
+                some.update(self._device(np.where(np.isin(index, list(changed)), index, -1)))
+                planned = changed
+            taps = (gate.data_ptr(), up.data_ptr()) if changed else (None, None)
             call("q3_gate_up_batched", pact, p["mlp.gate_proj"], p["mlp.up_proj"], pxb, rows, I, H, *taps, stream)
-            if lora:
-                lora_gate_up(act, gate, up, xb, stacks["gate_up"][l], lora)
+            if changed:
+                lora_gate_up(act, gate, up, xb, stacks["gate_up"][l], lora if changed == has else some)
             call("q3_gemv_residual_batched", px, p["mlp.down_proj"], pact, rows, H, I, None, stream)
             if lora:
                 lora_add(x, x, act, stacks["down"][l], lora)

@@ -188,3 +188,37 @@ def test_adapters_can_be_replaced():
         adapters.set(0, {(9, "self_attn.q_proj"): t2[0, "self_attn.o_proj"]}, 1.0)
     with pytest.raises(ValueError):
         PagedServer(DeviceWeights.random(SHAPES["hd128"], seed=1), n_pages=4, adapters=adapters)
+
+
+def test_an_adapter_leaves_the_projections_that_it_does_not_have():
+    # of zeros for q alone, beside one of everything, one with gate and up in the last layer only, and a sequence without: its logits
+    # are those of a server without adapters, to the bit
+    shape = SHAPES["tiny"]
+    w, last = DeviceWeights.random(shape, seed=4), shape.num_hidden_layers - 1
+    k, n = projection_sizes(shape)["self_attn.q_proj"]
+    adapters = AdapterSet(shape, 3, rank=8)
+    adapters.set(0, random_adapter(shape, 3, 8), 1.0)  # replaced
+    adapters.set(0, {(layer, "self_attn.q_proj"): (torch.ones(2, k), torch.zeros(n, 2)) for layer in range(last + 1)}, 1.0)
+    full, late = random_adapter(shape, 1, 8), random_adapter(shape, 2, 8)
+    late = {key: t for key, t in late.items() if key[0] == last or key[1] not in ("mlp.gate_proj", "mlp.up_proj")}
+    adapters.set(1, full, 1.5)
+    adapters.set(2, late, -0.7)
+    prompts = [list(range(5, 5 + n)) for n in (3, 40, 11, 7)]
+
+    def say(adapters, chosen, steps):
+        server = PagedServer(w, n_pages=64, page_size=8, max_seqs=6, max_positions=120, chunk=16, adapters=adapters)
+        ids = [server.add(p, adapter=a) for p, a in zip(prompts, chosen)]
+        return ids, run(server, steps)
+
+    ids, bare = say(None, [-1] * 4, 12)
+    for chosen in ([0, 0, -1, 0], [0, 0, 1, -1], [0, 0, 2, 1], [0, 0, 2, -1]):
+        same, seen = say(adapters, chosen, 12)
+        assert same == ids
+        for i, a in zip(ids, chosen):
+            got, want = ([s for s in x if s[0] == i] for x in (seen, bare))
+            if a <= 0:
+                assert len(got) == len(want) and all(x[1] == y[1] and torch.equal(x[2], y[2]) for x, y in zip(got, want)), (chosen, i)
+            else:
+                for _, before, logits in got:
+                    ref = plain_logits(Merged(w, *((full, 1.5) if a == 1 else (late, -0.7))), before)[-1]
+                    assert ((logits.float() - ref).square().mean() / ref.square().mean()).sqrt().item() < 2e-2
