@@ -20,6 +20,7 @@ token, the youngest give theirs back, and are taken in again later, prompt and t
 """
 from __future__ import annotations
 
+import operator
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -218,6 +219,12 @@ class PagedServer:
         seq = Sequence(prompt, **sampling)
         if not 0.0 <= seq.temperature < float("inf"):
             raise ValueError("the temperature must be a finite number from 0 on")
+        try:  # here, since an error in a step would stop all sequences
+            seq.top_k = operator.index(seq.top_k)
+            if seq.random is None:
+                seq.random = np.random.default_rng(seq.seed)
+        except (TypeError, ValueError) as e:
+            raise ValueError(f"top_k must be an int and the seed one from 0 on, or None: {e}") from None
         if not 0 <= seq.top_k < 2 ** 31 or not 0.0 <= seq.top_p <= 1.0 or not 0.0 <= seq.min_p <= 1.0:
             raise ValueError("top_k must be an int from 0 on, top_p and min_p within [0, 1]")
         if seq.adapter != -1 and (self.adapters is None or seq.adapter not in self.adapters.loaded):

@@ -183,3 +183,17 @@ def test_adapter_directories_are_checked(tmp_path):
         (d / "adapter_model.safetensors").write_bytes(broken)
         with pytest.raises(checkpoint.CheckpointError):
             adapters.read_adapter(d, shape)
+
+
+def test_the_server_checks_seeds_and_top_k():
+    # an error in a step would stop every sequence
+    s = server()
+    a = s.add([1], temperature=1.0, seed=5, top_k=np.int64(20))
+    for bad in (dict(seed=-1), dict(seed="a"), dict(seed=1.5), dict(top_k=0.5), dict(top_k=1.9), dict(top_k="20"), dict(top_k=None)):
+        with pytest.raises(ValueError):
+            s.add([1], temperature=1.0, **bad)
+    assert list(s.seqs.live) == [a] and s.seqs.live[a].top_k == 20
+    b = s.add([1], temperature=1.0, seed=5)
+    want = Sequence([1], seed=5)
+    want = [want.draw() for _ in range(3)]
+    assert [s.seqs.live[a].draw() for _ in want] == want and s.seqs.live[b].draw() == want[0]
