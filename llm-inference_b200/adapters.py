@@ -44,9 +44,13 @@ def read_adapter(path, s: Qwen3Shape):
     cfg = json.loads((d / "adapter_config.json").read_text())
     if cfg.get("peft_type", "LORA") != "LORA":
         raise CheckpointError(f"adapter type {cfg.get('peft_type')!r}, expected 'LORA'")
-    for key in ("use_dora", "rank_pattern", "alpha_pattern", "modules_to_save", "layer_replication", "lora_bias"):
+    for key in ("use_dora", "use_qalora", "rank_pattern", "alpha_pattern", "modules_to_save", "layer_replication", "lora_bias",
+                "alora_invocation_tokens", "arrow_config"):
         if cfg.get(key):
             raise CheckpointError(f"adapter_config.json: {key} is not supported")
+    # of these A and B start beside the base's weights as they are; others take a part out of the base first
+    if cfg.get("init_lora_weights") not in (None, True, False, "gaussian", "eva", "orthogonal"):
+        raise CheckpointError(f"adapter_config.json: init_lora_weights {cfg['init_lora_weights']!r} belongs to a changed base; save it converted")
     if cfg.get("bias", "none") != "none":
         raise CheckpointError("adapter_config.json: biases are not supported")
     r, alpha = cfg.get("r"), cfg.get("lora_alpha")

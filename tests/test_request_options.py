@@ -197,3 +197,16 @@ def test_the_server_checks_seeds_and_top_k():
     want = Sequence([1], seed=5)
     want = [want.draw() for _ in range(3)]
     assert [s.seqs.live[a].draw() for _ in want] == want and s.seqs.live[b].draw() == want[0]
+
+
+def test_adapters_of_another_base_or_kind_are_refused(tmp_path):
+    shape, d = checkpoint.PRESETS["tiny"], tmp_path / "a"
+    for cfg in ([dict(init_lora_weights=v) for v in ("pissa", "pissa_niter_16", "olora", "corda", "loftq", "lora_ga", {}, 2)] +
+                [dict(alora_invocation_tokens=[5, 6]), dict(use_qalora=True), dict(arrow_config={"top_k": 3})]):
+        write_adapter(d, shape, **cfg)
+        with pytest.raises(checkpoint.CheckpointError):
+            adapters.read_adapter(d, shape)
+    for cfg in ([dict(init_lora_weights=v) for v in (None, True, False, "gaussian", "eva", "orthogonal")] +
+                [dict(alora_invocation_tokens=None, use_qalora=False, arrow_config=None)]):
+        write_adapter(d, shape, **cfg)
+        assert adapters.read_adapter(d, shape)[1] == 2.0
