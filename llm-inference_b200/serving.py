@@ -217,9 +217,17 @@ class PagedServer:
                 raise ValueError(f"the mask must be {words} words of 32 bits")
             sampling["mask"] = mask[:words].astype(np.uint32).view(np.int32)
         seq = Sequence(prompt, **sampling)
+        try:  # here, since an error in a step would stop all sequences
+            for name in ("repetition", "frequency", "presence", "temperature", "top_p", "min_p"):
+                setattr(seq, name, float(getattr(seq, name)))
+            seq.bias = {int(t): float(v) for t, v in seq.bias.items()}
+        except (AttributeError, OverflowError, TypeError, ValueError) as e:
+            raise ValueError(f"penalties, the temperature, top_p and min_p must be numbers, biases numbers of token ids: {e}") from None
+        if any(not -2 ** 31 <= t < 2 ** 31 for t in seq.bias):
+            raise ValueError("a bias for no token id")
         if not 0.0 <= seq.temperature < float("inf"):
             raise ValueError("the temperature must be a finite number from 0 on")
-        try:  # here, since an error in a step would stop all sequences
+        try:
             seq.top_k = operator.index(seq.top_k)
             if seq.random is None:
                 seq.random = np.random.default_rng(seq.seed)

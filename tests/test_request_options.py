@@ -210,3 +210,16 @@ def test_adapters_of_another_base_or_kind_are_refused(tmp_path):
                 [dict(alora_invocation_tokens=None, use_qalora=False, arrow_config=None)]):
         write_adapter(d, shape, **cfg)
         assert adapters.read_adapter(d, shape)[1] == 2.0
+
+
+def test_the_server_checks_penalties_and_biases():
+    s = server()
+    a = s.add([1], repetition=np.float32(1.5), frequency=1, presence=0.5, bias={np.int64(3): 1, -1: -2.0, 10 ** 6: 0.5})
+    q = s.seqs.live[a]
+    assert (q.repetition, q.frequency, q.presence, q.bias) == (1.5, 1.0, 0.5, {3: 1.0, -1: -2.0, 10 ** 6: 0.5})
+    for bad in (dict(repetition="much"), dict(repetition=None), dict(frequency=[1.0, 2.0]), dict(presence={}), dict(bias={2 ** 31: 1.0}),
+                dict(bias={"the": 1.0}), dict(bias={3: "a"}), dict(bias={3: None}), dict(bias=[3]), dict(bias=None), dict(temperature="hot"),
+                dict(top_p=None), dict(min_p=1j)):
+        with pytest.raises(ValueError):
+            s.add([1], **bad)
+    assert list(s.seqs.live) == [a]
