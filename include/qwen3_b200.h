@@ -488,9 +488,9 @@ int q3_logits_process_bounded(void *out, const void *logits, int dtype, int rows
  * row that says otherwise. A draft outside [0, vocab) is none. Null arrays leave their part out; null temperature is 1.
  * temperature[r] not above 0 takes the first token. NaN logits and those of -inf are never taken; with an infinite
  * logit only its equals weigh. A row without any token gets -1 and prob 0. u below 0 or NaN counts as 0, from 1 on as
- * the largest below 1. Weights are whole multiples of 2^-41 of the largest, off by half a one (and a hundredth of that), 0 below it,
- * and their sums independent of order, so a row's result does not depend on its neighbours. rows at most 2^24; vocab at most 2^20. stride: elements
- * between rows. */
+ * the largest below 1. Weights are whole multiples of 2^-41 of the largest, off by half a one (and a hundredth of that), and their
+ * sums independent of order, so a row's result does not depend on its neighbours. rows at most 2^24; vocab at most 2^20.
+ * stride: elements between rows. */
 int q3_sample_logits(int *out, float *prob, const void *logits, int dtype, int rows, int vocab, long long stride,
                      const float *u, const float *temperature, const int *top_k, const float *top_p, const float *min_p,
                      const int *draft, void *stream);

@@ -9,9 +9,9 @@
 // (B h) neighbouring elements of its row, and its four columns of eight-column tiles are dealt out so that a lane writes eight
 // neighbouring outputs. What cannot be done without is the bytes of x, base, out and the present adapters' weights (a rank of 64 is 64
 // products for each element of x, a tenth of what the tensor cores could do meanwhile). Few rows are bound by the chain of loads
-// and two cluster barriers (one row through q, k and v 8.3 us, 32 rows 9.4), long steps by that chain in each warp beside the
-// bytes (2079 rows 35 us, of which the first product alone 14, the second alone 26.6; without the bases' loads that is 20.8, without
-// the stores 22.2, without matrix instructions 23.5, without B's loads 24.9).
+// and two cluster barriers (one row through q, k and v 8.4 us, 32 rows 9.6), long steps by that chain in each warp beside the
+// bytes (2079 rows 36 us; of 36.8 before the bases' early fetch the first product alone took 14, the second alone 26.6, that without the
+// bases' loads 20.8, without the stores 22.2, without matrix instructions 23.5, without B's loads 24.9).
 //
 // A x is held in 32 bits and enters the second product as two bf16 numbers, which together have 16 bits of it: its
 // rounding to one would be as large as the output's own.

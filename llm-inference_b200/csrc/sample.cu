@@ -23,9 +23,9 @@
 // cost more than all the arithmetic. The counts of values are added up by all CTAs, each for a share of the groups of values
 // that any has tokens of, and the sums go to the first CTA, which then needs no more barriers.
 //
-// Bound by the chain of these steps for few rows (one of 151936 bf16 12.5 us, 32 with all settings 17.7), by shared-memory
-// atomics for many (256 rows 45 us, 1.7 TB/s), and by instructions for fp32 rows (100 of 32003 35 us, the pass for the
-// histogram half of it).
+// Bound by the chain of these steps for few rows (one of 151936 bf16 12.5 us, 32 with all settings 17.6), for many half by
+// shared-memory atomics and half by phases in which most warps wait (256 rows 45 us, 1.7 TB/s), and by instructions for fp32 rows
+// (100 of 32003 35 us, the pass for the histogram half of it).
 #include <math.h>
 
 #include <algorithm>
